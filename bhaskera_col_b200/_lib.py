@@ -19,7 +19,7 @@ TQ_ERR_CUDA = -2
 TQ_ERR_WORKSPACE = -3
 TQ_ERR_DEVICE = -4
 TQ_F32, TQ_F16, TQ_BF16 = 0, 1, 2
-DEV_WAIT_TIMEOUT, DEV_BAD_BLOCK = 1, 2
+DEV_WAIT_TIMEOUT, DEV_BAD_BLOCK, DEV_BAD_POSITION, DEV_BAD_BATCH = 1, 2, 4, 8
 PAGE_TOKENS = 64
 PHASE_QPREP, PHASE_DECODE, PHASE_MERGE = 1, 2, 4
 
@@ -32,6 +32,8 @@ EXPORTED = (
     "tq_prefill_tensor_core",
     "tq_shared_alloc", "tq_shared_open", "tq_shared_close", "tq_shared_free",
     "tq_tables_bytes", "tq_init_tables",
+    "tq_qk_rope", "tq_append_ragged", "tq_dequantize_ragged",
+    "tq_attend_ragged_workspace_bytes", "tq_attend_ragged",
 )
 MAX_PEERS = 8
 SHARED_HANDLE_BYTES = 64
@@ -94,6 +96,32 @@ class PrefillArgs(ctypes.Structure):
                 ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
 
 
+class Rope(ctypes.Structure):
+    _fields_ = [("cos_sin", ctypes.c_void_p), ("positions", ctypes.c_int64),
+                ("rot_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32)]
+
+
+class HeadNorm(ctypes.Structure):
+    _fields_ = [("weight", ctypes.c_void_p), ("dtype", ctypes.c_int32),
+                ("eps", ctypes.c_float), ("offset", ctypes.c_float)]
+
+
+class Positions(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("bits", ctypes.c_int32),
+                ("stride", ctypes.c_int64 * 2)]
+
+
+class Ragged(ctypes.Structure):
+    _fields_ = [("requests", ctypes.c_int64), ("q_start", ctypes.c_void_p),
+                ("seq_lens", ctypes.c_void_p), ("max_q_len", ctypes.c_int64)]
+
+
+class AttendArgs(ctypes.Structure):
+    _fields_ = [("q", ctypes.POINTER(Tensor4)), ("out", ctypes.POINTER(Tensor4)),
+                ("batch", Ragged), ("scale", ctypes.c_float), ("causal", ctypes.c_int32),
+                ("engine", ctypes.c_int32)]
+
+
 _lock = threading.Lock()
 _lib: Optional[ctypes.CDLL] = None
 
@@ -137,6 +165,14 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
             "tq_shared_free": (I32, [VP]),
             "tq_tables_bytes": (SZ, [P(Geom)]),
             "tq_init_tables": (I32, [P(Geom), VP, VP, VP, VP, VP, VP, VP, SZ, P(Tables), VP]),
+            "tq_qk_rope": (I32, [P(Rope), P(Positions), P(Tensor4), P(Tensor4), P(HeadNorm),
+                                 P(Tensor4), P(Tensor4), P(HeadNorm), VP]),
+            "tq_append_ragged": (I32, [P(Geom), P(Tables), P(Cache), P(Tensor4), P(Tensor4),
+                                       P(Ragged), P(Rope), P(HeadNorm), P(Positions), VP]),
+            "tq_dequantize_ragged": (I32, [P(Geom), P(Tables), P(Cache), P(Ragged), P(Tensor4),
+                                           P(Tensor4), VP]),
+            "tq_attend_ragged_workspace_bytes": (SZ, [P(Geom), P(Cache), P(AttendArgs)]),
+            "tq_attend_ragged": (I32, [P(Geom), P(Tables), P(Cache), P(AttendArgs), VP, SZ, VP]),
         }
         for name, (res, args) in sig.items():
             fn = getattr(lib, name)

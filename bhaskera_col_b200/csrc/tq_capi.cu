@@ -465,6 +465,310 @@ size_t tq_prefill_workspace_bytes(const tq_geom* g, const tq_cache* c, const tq_
   return 2 * ((one + 255) & ~(size_t)255);
 }
 
+// ---------------------------------------------------------------------------
+// serving operators on ragged batches
+// ---------------------------------------------------------------------------
+// check_t4 for tensors that may have no rows (and then no memory).
+static int check_maybe_empty(const tq_tensor4* x, const char* what, const char* fn) {
+  if (!x || x->data) return check_t4(x, what, fn);
+  tq_tensor4 some = *x;
+  bool empty = false;
+  for (int i = 0; i < 4; ++i) empty = empty || x->shape[i] == 0;
+  if (empty) some.data = &some;
+  return check_t4(&some, what, fn);
+}
+
+static int check_rope(const tq_rope* r, int64_t D, const char* fn) {
+  if (!r) return TQ_OK;
+  if (!r->cos_sin || reinterpret_cast<uintptr_t>(r->cos_sin) % 16 || r->positions < 1) {
+    set_error("%s: rope needs a 16-byte aligned table of at least one position", fn);
+    return TQ_ERR_INVALID;
+  }
+  if (r->rot_dim < 2 || r->rot_dim % 2 || r->rot_dim > D) {
+    set_error("%s: rope.rot_dim must be even and in [2, %lld], got %d", fn, (long long)D,
+              r->rot_dim);
+    return TQ_ERR_INVALID;
+  }
+  return TQ_OK;
+}
+
+static int check_norm(const tq_head_norm* n, const char* fn) {
+  if (!n) return TQ_OK;
+  if (!n->weight || !valid_dtype(n->dtype) || !(n->eps >= 0.f)) {
+    set_error("%s: a head norm needs a weight of a supported type and eps >= 0", fn);
+    return TQ_ERR_INVALID;
+  }
+  return TQ_OK;
+}
+
+static int check_positions(const tq_positions* p, const char* fn) {
+  if (!p) return TQ_OK;
+  if (!p->data || (p->bits != 32 && p->bits != 64) ||
+      reinterpret_cast<uintptr_t>(p->data) % (p->bits / 8)) {
+    set_error("%s: positions must be aligned int32 or int64", fn);
+    return TQ_ERR_INVALID;
+  }
+  return TQ_OK;
+}
+
+// An output view must give every element its own place: with the dims in
+// order of their strides, each stride has to pass all that the dims before it
+// span.
+static int check_written(const tq_tensor4* x, const char* what, const char* fn) {
+  int idx[4] = {0, 1, 2, 3};
+  for (int i = 0; i < 4; ++i) {
+    if (x->shape[i] == 0) return TQ_OK;
+    for (int j = i + 1; j < 4; ++j)
+      if (x->stride[idx[j]] < x->stride[idx[i]]) std::swap(idx[i], idx[j]);
+  }
+  int64_t span = 1;
+  for (int i : idx) {
+    if (x->shape[i] == 1) continue;
+    if (x->stride[i] < span) {
+      set_error("%s: elements of %s share memory", fn, what);
+      return TQ_ERR_INVALID;
+    }
+    span += (x->shape[i] - 1) * x->stride[i];
+  }
+  return TQ_OK;
+}
+
+static void extent(const tq_tensor4* x, const char*& lo, const char*& hi) {
+  const int64_t es = x->dtype == TQ_F32 ? 4 : 2;
+  lo = hi = static_cast<const char*>(x->data);
+  for (int i = 0; i < 4; ++i) {
+    const int64_t d = (x->shape[i] - 1) * x->stride[i] * es;
+    if (d < 0) lo += d; else hi += d;
+  }
+  hi += es;
+}
+
+// y may be x itself, else they must not overlap.
+static int check_alias(const tq_tensor4* x, const tq_tensor4* y, const char* what, const char* fn) {
+  bool same = x->data == y->data;
+  for (int i = 0; i < 4; ++i) {
+    if (x->shape[i] == 0) return TQ_OK;
+    same = same && (x->shape[i] == 1 || x->stride[i] == y->stride[i]);
+  }
+  if (same) return TQ_OK;
+  const char *a, *b, *c, *d;
+  extent(x, a, b);
+  extent(y, c, d);
+  if (a < d && c < b) {
+    set_error("%s: %s overlaps its input without being the same view", fn, what);
+    return TQ_ERR_INVALID;
+  }
+  return TQ_OK;
+}
+
+int32_t tq_qk_rope(const tq_rope* rope, const tq_positions* pos, const tq_tensor4* q,
+                   const tq_tensor4* q_out, const tq_head_norm* q_norm, const tq_tensor4* k,
+                   const tq_tensor4* k_out, const tq_head_norm* k_norm, void* stream) {
+  NvtxRange range("tq_qk_rope");
+  const char* fn = "tq_qk_rope";
+  const tq_tensor4* x[2] = {q, k};
+  const tq_tensor4* y[2] = {q_out, k_out};
+  const tq_head_norm* norm[2] = {q_norm, k_norm};
+  const char* names[2] = {"q", "k"};
+  const char* outs[2] = {"q_out", "k_out"};
+  int rc;
+  if (!q && !k) { set_error("%s: neither q nor k is given", fn); return TQ_ERR_INVALID; }
+  const tq_tensor4* one = q ? q : k;
+  for (int w = 0; w < 2; ++w) {
+    if ((x[w] == nullptr) != (y[w] == nullptr)) {
+      set_error("%s: %s and %s come together", fn, names[w], outs[w]);
+      return TQ_ERR_INVALID;
+    }
+    if (!x[w]) continue;
+    if ((rc = check_maybe_empty(x[w], names[w], fn)) ||
+        (rc = check_maybe_empty(y[w], outs[w], fn)) ||
+        (rc = check_norm(norm[w], fn)) || (rc = check_written(y[w], outs[w], fn)))
+      return rc;
+    if (x[w]->dtype != y[w]->dtype) {
+      set_error("%s: %s and %s differ in type", fn, names[w], outs[w]);
+      return TQ_ERR_INVALID;
+    }
+    for (int i = 0; i < 4; ++i)
+      if (x[w]->shape[i] != y[w]->shape[i] || (i != 1 && x[w]->shape[i] != one->shape[i])) {
+        set_error("%s: shapes of q, k and their outputs disagree", fn);
+        return TQ_ERR_INVALID;
+      }
+    if ((rc = check_alias(x[w], y[w], outs[w], fn))) return rc;
+    if (!rope && !norm[w]) {
+      set_error("%s: %s has neither a rotation nor a norm", fn, names[w]);
+      return TQ_ERR_INVALID;
+    }
+  }
+  const int64_t D = one->shape[3];
+  if (D < 1 || D > 256) {
+    set_error("%s: head_dim %lld is outside [1, 256]", fn, (long long)D);
+    return TQ_ERR_INVALID;
+  }
+  if ((rc = check_rope(rope, D, fn))) return rc;
+  if (rope && !pos) { set_error("%s: a rotation needs positions", fn); return TQ_ERR_INVALID; }
+  if (one->shape[0] * one->shape[2] == 0) return TQ_OK;
+  if ((rc = check_positions(pos, fn))) return rc;
+  uint32_t* status = device_status_word();
+  if (!status) { set_error("%s: device status word unavailable", fn); return TQ_ERR_CUDA; }
+  return launch_qk_rope(rope, pos, x, y, norm, status, (cudaStream_t)stream);
+}
+
+static int check_ragged(const tq_ragged* b, const tq_cache* c, const char* fn) {
+  if (!b || b->requests < 1 || !b->q_start || !b->seq_lens ||
+      (reinterpret_cast<uintptr_t>(b->q_start) | reinterpret_cast<uintptr_t>(b->seq_lens)) % 4 ||
+      b->max_q_len < 0) {
+    set_error("%s: a batch needs at least one request, int32 q_start and seq_lens, and "
+              "max_q_len >= 0", fn);
+    return TQ_ERR_INVALID;
+  }
+  if (c->streams % b->requests) {
+    set_error("%s: %lld streams are no multiple of %lld requests", fn, (long long)c->streams,
+              (long long)b->requests);
+    return TQ_ERR_INVALID;
+  }
+  return TQ_OK;
+}
+
+static int check_flat(const tq_tensor4* x, const char* what, int64_t heads, const tq_geom* g,
+                      const char* fn) {
+  if (int rc = check_maybe_empty(x, what, fn)) return rc;
+  if (x->shape[0] != 1 || x->shape[1] != heads || x->shape[3] != g->head_dim) {
+    set_error("%s: %s must be (1, %lld, N, %d)", fn, what, (long long)heads, g->head_dim);
+    return TQ_ERR_INVALID;
+  }
+  return TQ_OK;
+}
+
+int32_t tq_append_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
+                         const tq_tensor4* k, const tq_tensor4* v, const tq_ragged* batch,
+                         const tq_rope* rope, const tq_head_norm* k_norm,
+                         const tq_positions* pos, void* stream) {
+  NvtxRange range("tq_append_ragged");
+  const char* fn = "tq_append_ragged";
+  int rc;
+  if ((rc = check_geom(g, fn)) || (rc = check_tables(g, t, fn)) || (rc = check_cache(c, fn)) ||
+      (rc = check_ragged(batch, c, fn)))
+    return rc;
+  const int64_t heads = c->streams / batch->requests;
+  if ((rc = check_flat(k, "k", heads, g, fn)) || (rc = check_flat(v, "v", heads, g, fn)) ||
+      (rc = check_rope(rope, g->head_dim, fn)) || (rc = check_norm(k_norm, fn)) ||
+      (k->shape[2] > 0 && (rc = check_positions(pos, fn))))
+    return rc;
+  if (g->head_dim > 128 || g->qjl) {
+    set_error("%s: head_dim at most 128 and no QJL sketch (got %d, qjl %d)", fn, g->head_dim,
+              g->qjl);
+    return TQ_ERR_INVALID;
+  }
+  if (k->shape[2] != v->shape[2]) {
+    set_error("%s: k and v differ in rows", fn);
+    return TQ_ERR_INVALID;
+  }
+  uint32_t* status = device_status_word();
+  if (!status) { set_error("%s: device status word unavailable", fn); return TQ_ERR_CUDA; }
+  return launch_append_ragged(g, t, c, k, v, batch, rope, k_norm, pos, status,
+                              (cudaStream_t)stream);
+}
+
+int32_t tq_dequantize_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
+                             const tq_ragged* batch, const tq_tensor4* k_out,
+                             const tq_tensor4* v_out, void* stream) {
+  NvtxRange range("tq_dequantize_ragged");
+  const char* fn = "tq_dequantize_ragged";
+  int rc;
+  if ((rc = check_geom(g, fn)) || (rc = check_tables(g, t, fn)) || (rc = check_cache(c, fn)) ||
+      (rc = check_ragged(batch, c, fn)))
+    return rc;
+  const int64_t heads = c->streams / batch->requests;
+  const tq_tensor4* o[2] = {k_out, v_out};
+  for (int w = 0; w < 2; ++w) {
+    const char* what = w ? "v_out" : "k_out";
+    if (o[w] && ((rc = check_flat(o[w], what, heads, g, fn)) || (rc = check_written(o[w], what, fn))))
+      return rc;
+  }
+  if (!k_out && !v_out) { set_error("%s: neither k_out nor v_out is given", fn); return TQ_ERR_INVALID; }
+  if (k_out && v_out && k_out->shape[2] != v_out->shape[2]) {
+    set_error("%s: k_out and v_out differ in rows", fn);
+    return TQ_ERR_INVALID;
+  }
+  if (g->head_dim > 128) {
+    set_error("%s: head_dim %d > 128 is not supported", fn, g->head_dim);
+    return TQ_ERR_INVALID;
+  }
+  uint32_t* status = device_status_word();
+  if (!status) { set_error("%s: device status word unavailable", fn); return TQ_ERR_CUDA; }
+  return launch_dequant_ragged(g, t, c, batch, k_out, v_out, status, (cudaStream_t)stream);
+}
+
+static int check_attend(const tq_geom* g, const tq_cache* c, const tq_attend_args* a,
+                        const char* fn) {
+  int rc;
+  if ((rc = check_geom(g, fn)) || (rc = check_cache(c, fn))) return rc;
+  if (!a) { set_error("%s: args are NULL", fn); return TQ_ERR_INVALID; }
+  if ((rc = check_ragged(&a->batch, c, fn)) || (rc = check_maybe_empty(a->q, "q", fn)))
+    return rc;
+  const int64_t Hkv = c->streams / a->batch.requests, Hq = a->q->shape[1];
+  if (Hq < 1 || Hq % Hkv) {
+    set_error("%s: %lld query heads are no multiple of %lld KV heads", fn, (long long)Hq,
+              (long long)Hkv);
+    return TQ_ERR_INVALID;
+  }
+  if ((rc = check_flat(a->q, "q", Hq, g, fn))) return rc;
+  if (a->engine < 0 || a->engine > 3) {
+    set_error("%s: engine must be 0 (fastest), 1 (mma.sync), 2 or 3 (tcgen05), got %d", fn,
+              a->engine);
+    return TQ_ERR_INVALID;
+  }
+  const bool tc = prefill_tc_applies(g);
+  if (a->engine >= 2 ? !tc
+                     : !prefill_supported(g->head_dim, g->key_bits, g->value_bits) &&
+                           !(a->engine == 0 && tc)) {
+    set_error("%s: no kernel for head_dim %d, key_bits %d, value_bits %d (engine %d)", fn,
+              g->head_dim, g->key_bits, g->value_bits, a->engine);
+    return TQ_ERR_INVALID;
+  }
+  if (a->q->shape[2] > (int64_t)1 << 30 || a->batch.requests > (int64_t)1 << 24 || Hq > 1024) {
+    set_error("%s: at most 2^30 rows, 2^24 requests and 1024 query heads", fn);
+    return TQ_ERR_INVALID;
+  }
+  return TQ_OK;
+}
+
+size_t tq_attend_ragged_workspace_bytes(const tq_geom* g, const tq_cache* c,
+                                        const tq_attend_args* a) {
+  if (check_attend(g, c, a, "tq_attend_ragged_workspace_bytes")) return 0;
+  return attend_ragged_workspace(g, c, a);
+}
+
+int32_t tq_attend_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
+                         const tq_attend_args* a, void* workspace, size_t workspace_bytes,
+                         void* stream) {
+  NvtxRange range("tq_attend_ragged");
+  const char* fn = "tq_attend_ragged";
+  int rc;
+  if ((rc = check_attend(g, c, a, fn)) || (rc = check_tables(g, t, fn))) return rc;
+  if ((rc = check_flat(a->out, "out", a->q->shape[1], g, fn)) ||
+      (rc = check_written(a->out, "out", fn)))
+    return rc;
+  if (a->out->shape[2] != a->q->shape[2]) {
+    set_error("%s: q and out differ in rows", fn);
+    return TQ_ERR_INVALID;
+  }
+  if (!t->rot_f16 || reinterpret_cast<uintptr_t>(t->rot_f16) % 16) {
+    set_error("%s: tables.rot_f16 (R as fp16, 16-byte aligned) is required", fn);
+    return TQ_ERR_INVALID;
+  }
+  if (!(a->scale > 0.f)) { set_error("%s: scale must be positive", fn); return TQ_ERR_INVALID; }
+  const size_t need = attend_ragged_workspace(g, c, a);
+  if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256) {
+    set_error("%s: a 256-byte aligned workspace of %zu bytes is needed, %zu given", fn, need,
+              workspace_bytes);
+    return TQ_ERR_WORKSPACE;
+  }
+  uint32_t* status = device_status_word();
+  if (!status) { set_error("%s: device status word unavailable", fn); return TQ_ERR_CUDA; }
+  return launch_attend_ragged(g, t, c, a, workspace, status, (cudaStream_t)stream);
+}
+
 int32_t tq_workspace_status(void* workspace, uint32_t* status, void* stream) {
   if (!workspace || !status) { set_error("tq_workspace_status: NULL argument"); return TQ_ERR_INVALID; }
   cudaStream_t st = (cudaStream_t)stream;

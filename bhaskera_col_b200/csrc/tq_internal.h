@@ -57,6 +57,29 @@ int launch_decode(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                   const tq_decode_args* a, void* ws, size_t ws_bytes, cudaStream_t st,
                   const StepInput* step = nullptr);
 
+// Serving operators on ragged batches (tq_rope.cu, tq_ragged.cu, tq_attend.cu).
+struct HeadXform;
+struct RaggedView;
+struct RaggedAttend;
+HeadXform head_xform(const tq_rope* rope, const tq_head_norm* norm);
+RaggedView ragged_view(const tq_ragged* b, int64_t N, const tq_cache* c);
+int launch_qk_rope(const tq_rope* rope, const tq_positions* pos, const tq_tensor4* const x[2],
+                   const tq_tensor4* const y[2], const tq_head_norm* const norm[2],
+                   uint32_t* status, cudaStream_t st);
+int launch_append_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
+                         const tq_tensor4* k, const tq_tensor4* v, const tq_ragged* batch,
+                         const tq_rope* rope, const tq_head_norm* norm, const tq_positions* pos,
+                         uint32_t* status, cudaStream_t st);
+int launch_dequant_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
+                          const tq_ragged* batch, const tq_tensor4* ko, const tq_tensor4* vo,
+                          uint32_t* status, cudaStream_t st);
+size_t attend_ragged_workspace(const tq_geom* g, const tq_cache* c, const tq_attend_args* a);
+int launch_attend_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
+                         const tq_attend_args* a, void* ws, uint32_t* status, cudaStream_t st);
+int launch_attend_mma(const tq_geom* g, const tq_tables* t, const tq_cache* c,
+                      const tq_attend_args* a, const RaggedAttend& rg, int64_t Hkv, int hc,
+                      int64_t grid, uint32_t* status, cudaStream_t st);
+
 // cudaLaunchKernelEx with programmatic stream serialisation (see pdl_wait).
 template <typename... KArgs, typename... Args>
 cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,

@@ -22,7 +22,9 @@
 // and an online softmax; P' = P * ||v|| folds the value norms in.
 #include "tq_common.cuh"
 #include "tq_internal.h"
+#include "tq_ragged.cuh"
 
+#include <limits.h>
 #include <math.h>
 
 namespace tq {
@@ -48,6 +50,7 @@ struct PrefillParams {
   int nqb;                      // query blocks per head
   const int32_t* kv_start;      // [B] first attended key of each batch row, or NULL
   uint32_t* status;
+  RaggedAttend rg;              // ragged batch (RG kernels): Tq, n_tokens come per request
 };
 
 template <int D, int KB, int VB>
@@ -89,7 +92,11 @@ __device__ __forceinline__ void frag_b_kn(uint32_t (&r)[4], const __half* base, 
   ldsm_x4_t(r, base + row * ld + col);
 }
 
-template <int D, int KB, int VB>
+// RG: a ragged batch (tq_attend_ragged).  A CTA takes one segment of the work
+// list: its request's rows and lengths, key tiles [kt0, kt1) of one block of
+// query positions; a tile cut into several segments leaves partial rows that
+// the tile's last CTA joins.
+template <int D, int KB, int VB, bool RG>
 __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p) {
   using G = Pf<D, KB, VB>;
   constexpr int NC = D / 16;                  // 16-wide chunks of D
@@ -109,17 +116,32 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
   const int gq = lane >> 2, tq = lane & 3;
   const int wph = kPfWarps / p.hc;                     // warps per head
   const int P = 16 * wph;                              // query positions per CTA
-  const int qb = p.nqb - 1 - (int)blockIdx.x;          // long rows first
   const int nchunk = (int)(p.g / p.hc);
-  const int64_t stream = (int64_t)blockIdx.y / nchunk;  // b * Hkv + kv head
-  const int chunk = (int)((int64_t)blockIdx.y % nchunk);
+  SegWork sw = {};
+  int qb = p.nqb - 1 - (int)blockIdx.x;                // long rows first
+  int64_t group = blockIdx.y;                          // (b, kv head, chunk of its query heads)
+  __shared__ int bad_key, last_flag;
+  if constexpr (RG) {
+    if (!take_segment(p.rg, sw)) return;
+    qb = sw.seg.tile;
+    group = sw.seg.req * (p.Hkv * nchunk) + sw.group;
+    p.Tq = sw.rq.q_len;
+    p.n_tokens = sw.rq.seq;
+    if (threadIdx.x == 0) bad_key = INT_MAX;
+  }
+  const int64_t stream = group / nchunk;               // b * Hkv + kv head
+  const int chunk = (int)(group % nchunk);
   const int64_t b = stream / p.Hkv, kvh = stream % p.Hkv;
+  // the batch row's first query row: batch stride, or the request's first row
+  const int64_t qrow = RG ? sw.rq.q0 * p.qs[2] : b * p.qs[0];
+  const int64_t orow = RG ? sw.rq.q0 * p.os[2] : b * p.os[0];
   const int64_t h = kvh * p.g + (int64_t)chunk * p.hc + warp / wph;   // this warp's head
   const int64_t t_base = p.n_tokens - p.Tq;            // position of query 0
   const int t0 = qb * P + (warp % wph) * 16;           // this warp's first query
   const int64_t qpos_max = t_base + tmin<int64_t>((int64_t)(qb + 1) * P, p.Tq) - 1;
   const int64_t kend = p.causal ? qpos_max + 1 : p.n_tokens;   // keys this CTA needs
-  const int ntiles = (int)((kend + 63) / 64);
+  const int tile0 = RG ? sw.seg.kt0 : 0;
+  const int ntiles = RG ? sw.seg.kt1 - tile0 : (int)((kend + 63) / 64);
   int64_t kst = 0;                                     // first attended key (left padding)
   if (p.kv_start) {
     const int v = __ldg(p.kv_start + b);
@@ -145,7 +167,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
   // pool address of this stream's page pg (block table or contiguous)
   auto page_src = [&](int64_t pg) -> const uint8_t* {
     bool ok;
-    const int64_t ps = page_slot(p.pm, stream, pg, ok);
+    const int64_t ps = page_slot(p.pm, stream, pg + tile0, ok);
     if (!ok) atomicOr(p.status, TQ_DEV_BAD_BLOCK);
     return p.pages + ps * (int64_t)PAGE;
   };
@@ -164,7 +186,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
     float acc[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-    const int64_t qbase = b * p.qs[0] + h * p.qs[1];
+    const int64_t qbase = qrow + h * p.qs[1];
     const int r0 = t0 + gq, r1 = r0 + 8;
     auto ld2 = [&](int r, int c) -> uint32_t {
       if (r >= p.Tq) return 0u;
@@ -256,10 +278,16 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
         }
       }
       if (tid < 64) {
-        const int64_t key = (int64_t)kt * 64 + tid;
+        const int64_t key = (int64_t)(kt + tile0) * 64 + tid;
         const bool kok = key < kend;
         kn[tid] = kok ? __half2float(reinterpret_cast<const __half*>(pg + p.off_kn)[tid]) : 0.f;
         vn[tid] = kok ? __half2float(reinterpret_cast<const __half*>(pg + p.off_vn)[tid]) : 0.f;
+        // 0 x inf would reach rows that do not see the key: a token whose norm
+        // is not finite counts as 0 and the rows that see it become NaN at the end
+        if (RG && !(isfinite(kn[tid]) && isfinite(vn[tid]))) {
+          kn[tid] = vn[tid] = 0.f;
+          atomicMin(&bad_key, (int)key);
+        }
       }
     }
     __syncthreads();
@@ -270,7 +298,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
                &full[st]);
     }
 
-    const int64_t k0 = (int64_t)kt * 64;
+    const int64_t k0 = (int64_t)(kt + tile0) * 64;
     if (active && k0 < warp_kend) {
       // ---- S = Q' K^T (16 x 64) -------------------------------------------
       float s[8][4];
@@ -365,7 +393,12 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
     l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    const float i0 = l0 > 0.f ? 1.f / l0 : 0.f, i1 = l1 > 0.f ? 1.f / l1 : 0.f;
+    float i0 = l0 > 0.f ? 1.f / l0 : 0.f, i1 = l1 > 0.f ? 1.f / l1 : 0.f;
+    if constexpr (RG) {
+      const int64_t last = p.n_tokens - 1;
+      if (l0 != l0 || bad_key <= (p.causal ? tmin(qp0, last) : last)) l0 = i0 = NAN;
+      if (l1 != l1 || bad_key <= (p.causal ? tmin(qp1, last) : last)) l1 = i1 = NAN;
+    }
     float acc[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
@@ -385,9 +418,25 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
       }
     }
     const int r0 = t0 + gq, r1 = r0 + 8;
-    const int64_t obase = b * p.os[0] + h * p.os[1];
+    const int64_t obase = orow + h * p.os[1];
+    const bool split = RG && sw.seg.slot >= 0;
+    if (split) {
+      const int64_t pr = part_row(p.rg.plan, sw.seg.slot, sw.group, 16 * warp + gq);
+      float* part = p.rg.plan.part + pr * D + 2 * tq;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if (r0 < p.Tq) *reinterpret_cast<float2*>(part + 8 * n) = make_float2(acc[n][0], acc[n][1]);
+        if (r1 < p.Tq)
+          *reinterpret_cast<float2*>(part + 8 * D + 8 * n) = make_float2(acc[n][2], acc[n][3]);
+      }
+      if (tq == 0) {
+        if (r0 < p.Tq) p.rg.plan.ml[pr] = make_float2(m0, l0);
+        if (r1 < p.Tq) p.rg.plan.ml[pr + 8] = make_float2(m1, l1);
+      }
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+      if (split) break;
       const int c = 8 * n + 2 * tq;
       if (r0 < p.Tq) {
         const int64_t o = obase + (int64_t)r0 * p.os[2] + (int64_t)c * p.os[3];
@@ -401,13 +450,23 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
       }
     }
   }
+  if constexpr (RG) {
+    if (sw.seg.slot >= 0)
+      join_partials<D>(p.rg.plan, sw, kPfWarps, p.out, p.o_dtype, p.os[3], &last_flag,
+                       [&](int row) -> int64_t {
+                         const int wr = row >> 4, t = qb * P + (wr % wph) * 16 + (row & 15);
+                         if (t >= p.Tq) return -1;
+                         const int64_t hh = kvh * p.g + (int64_t)chunk * p.hc + wr / wph;
+                         return orow + hh * p.os[1] + t * p.os[2];
+                       });
+  }
 }
 
 using PfFn = void (*)(PrefillParams);
 
-template <int D>
+template <int D, bool RG>
 PfFn pf_fn(int kb, int vb) {
-#define TQ_PF(K, V) if (kb == K && vb == V) return prefill_kernel<D, K, V>;
+#define TQ_PF(K, V) if (kb == K && vb == V) return prefill_kernel<D, K, V, RG>;
   TQ_PF(4, 2) TQ_PF(3, 3) TQ_PF(2, 2) TQ_PF(4, 4) TQ_PF(6, 4) TQ_PF(5, 5) TQ_PF(6, 6)
   TQ_PF(8, 8) TQ_PF(3, 2) TQ_PF(4, 3)
 #undef TQ_PF
@@ -417,9 +476,45 @@ PfFn pf_fn(int kb, int vb) {
 }  // namespace
 
 bool prefill_supported(int D, int kb, int vb) {
-  if (D == 128) return pf_fn<128>(kb, vb) != nullptr;
-  if (D == 64) return pf_fn<64>(kb, vb) != nullptr;
+  if (D == 128) return pf_fn<128, false>(kb, vb) != nullptr;
+  if (D == 64) return pf_fn<64, false>(kb, vb) != nullptr;
   return false;
+}
+
+// Ragged batch on the mma.sync kernel; `grid` bounds the work list.
+int launch_attend_mma(const tq_geom* G, const tq_tables* t, const tq_cache* c,
+                      const tq_attend_args* a, const RaggedAttend& rg, int64_t Hkv, int hc,
+                      int64_t grid, uint32_t* status, cudaStream_t st) {
+  PrefillParams p = {};
+  const PageGeom g = make_geom(G->head_dim, G->key_bits, G->value_bits, G->qjl);
+  p.pages = c->pages;
+  p.pm = page_map(c);
+  p.page_bytes = g.page_bytes;
+  p.page_pitch = (g.page_bytes + 127) & ~127;
+  p.off_v = g.off_v;
+  p.off_kn = g.off_kn;
+  p.off_vn = g.off_vn;
+  p.rot_h = reinterpret_cast<const __half*>(t->rot_f16);
+  p.kc = t->k_centroids;
+  p.vc = t->v_centroids;
+  p.q = a->q->data; p.q_dtype = a->q->dtype;
+  p.out = a->out->data; p.o_dtype = a->out->dtype;
+  for (int i = 0; i < 4; ++i) { p.qs[i] = a->q->stride[i]; p.os[i] = a->out->stride[i]; }
+  p.Hq = a->q->shape[1];
+  p.Hkv = Hkv;
+  p.g = p.Hq / Hkv;
+  p.hc = hc;
+  p.scale = a->scale;
+  p.causal = a->causal;
+  p.status = status;
+  p.rg = rg;
+  PfFn fn = G->head_dim == 128 ? pf_fn<128, true>(G->key_bits, G->value_bits)
+                               : pf_fn<64, true>(G->key_bits, G->value_bits);
+  const int smem = G->head_dim == 128 ? Pf<128, 4, 4>::smem(p.page_pitch)
+                                      : Pf<64, 4, 4>::smem(p.page_pitch);
+  if (set_smem_attr((const void*)fn, smem) != TQ_OK) return TQ_ERR_CUDA;
+  fn<<<(unsigned)grid, kPfThreads, smem, st>>>(p);
+  return check_launch("tq_attend_ragged");
 }
 
 int launch_prefill(const tq_geom* G, const tq_tables* t, const tq_cache* c,
@@ -428,7 +523,7 @@ int launch_prefill(const tq_geom* G, const tq_tables* t, const tq_cache* c,
     const int rc = launch_prefill_tc(G, t, c, a, status, st);
     if (rc != 1) return rc;
   }
-  PrefillParams p;
+  PrefillParams p = {};
   const PageGeom g = make_geom(G->head_dim, G->key_bits, G->value_bits, G->qjl);
   p.pages = c->pages;
   p.pm = page_map(c);
@@ -455,8 +550,8 @@ int launch_prefill(const tq_geom* G, const tq_tables* t, const tq_cache* c,
   p.nqb = (int)((p.Tq + 16 * (kPfWarps / p.hc) - 1) / (16 * (kPfWarps / p.hc)));
   p.status = status;
   if (p.Tq == 0) return TQ_OK;
-  PfFn fn = G->head_dim == 128 ? pf_fn<128>(G->key_bits, G->value_bits)
-                               : pf_fn<64>(G->key_bits, G->value_bits);
+  PfFn fn = G->head_dim == 128 ? pf_fn<128, false>(G->key_bits, G->value_bits)
+                               : pf_fn<64, false>(G->key_bits, G->value_bits);
   const int smem = G->head_dim == 128 ? Pf<128, 4, 4>::smem(p.page_pitch)
                                       : Pf<64, 4, 4>::smem(p.page_pitch);
   if (!fn) {

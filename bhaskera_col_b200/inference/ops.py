@@ -6,6 +6,7 @@ or PyTorch implementation) when the library or the device is unavailable.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from dataclasses import dataclass
@@ -421,4 +422,260 @@ def decode_attention(tables: LayerTables, pages: torch.Tensor, q: torch.Tensor,
     _lib.check("tq_decode_attn", lib.tq_decode_attn(
         ctypes.byref(g), ctypes.byref(t), ctypes.byref(c), ctypes.byref(a),
         ws.data_ptr(), ws.numel(), _stream(q.device)))
+    return out
+
+
+# ---------------------------------------------------------------------------
+# Serving operators on a flattened batch of requests
+# ---------------------------------------------------------------------------
+@dataclass
+class RopeTable:
+    """Rotary position embedding: row p of ``cos_sin`` (fp32 (positions,
+    rot_dim)) holds the cosines, then the sines, of position p's rot_dim / 2
+    angles.  Pair i is dims (i, rot_dim / 2 + i) of a head, or (2i, 2i + 1)
+    when ``interleaved``; dims from rot_dim on are not rotated."""
+    cos_sin: torch.Tensor
+    interleaved: bool = False
+
+    def __post_init__(self):
+        c = self.cos_sin
+        if c.dtype != torch.float32 or c.dim() != 2 or not c.is_contiguous():
+            raise ValueError("cos_sin must be a contiguous fp32 (positions, rot_dim) tensor")
+        if c.shape[0] < 1 or c.shape[1] < 2 or c.shape[1] % 2:
+            raise ValueError(f"cos_sin must hold a position and an even rot_dim, got {tuple(c.shape)}")
+        self._c = _lib.Rope(c.data_ptr(), c.shape[0], c.shape[1], 1 if self.interleaved else 0)
+
+    @classmethod
+    def build(cls, rot_dim: int, positions: int, base: float = 10000.0, interleaved: bool = False,
+              inv_freq: Optional[torch.Tensor] = None, scale: float = 1.0,
+              device: torch.device = torch.device("cuda")) -> "RopeTable":
+        """Angles position * base^(-2i / rot_dim), or position * inv_freq[i],
+        formed in 64 bits (an fp32 product is off by 0.03 rad at position
+        10^6); ``scale`` multiplies the cosines and sines (YaRN's attention
+        factor)."""
+        if inv_freq is None:
+            i = torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device)
+            inv_freq = float(base) ** (-i / rot_dim)
+        f = inv_freq.to(device=device, dtype=torch.float64)
+        if f.shape != (rot_dim // 2,):
+            raise ValueError(f"inv_freq must be ({rot_dim // 2},), got {tuple(f.shape)}")
+        a = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * f
+        return cls((torch.cat([a.cos(), a.sin()], -1) * scale).float().contiguous(), interleaved)
+
+
+@dataclass
+class HeadNorm:
+    """RMS norm of each head vector: x / sqrt(mean(x^2) + eps) * (weight +
+    offset); offset 1 for models that store weight - 1."""
+    weight: torch.Tensor
+    eps: float = 1e-6
+    offset: float = 0.0
+
+    def __post_init__(self):
+        w = self.weight
+        if w.dim() != 1 or w.dtype not in _DT or not w.is_contiguous():
+            raise ValueError("weight must be a contiguous (head_dim,) floating tensor")
+        if not self.eps >= 0:
+            raise ValueError(f"eps must be >= 0, got {self.eps}")
+        self._c = _lib.HeadNorm(w.data_ptr(), _DT[w.dtype], float(self.eps), float(self.offset))
+
+
+@dataclass
+class RaggedBatch:
+    """Requests of different lengths flattened into rows (vLLM's batch): row
+    q_start[r] + i is new token i of request r, at position seq_lens[r] -
+    (q_start[r + 1] - q_start[r]) + i; seq_lens counts the new tokens.  Both
+    stay on the device; ``max_q_len`` (>= the most new tokens of a request)
+    shapes launches and never a result.  Rows outside [q_start[0],
+    q_start[-1]) belong to no request and are left alone."""
+    q_start: torch.Tensor       # int32 (R + 1,), ascending
+    seq_lens: torch.Tensor      # int32 (R,)
+    max_q_len: int
+
+    def __post_init__(self):
+        a, b = self.q_start, self.seq_lens
+        if a.dtype != torch.int32 or b.dtype != torch.int32 or a.dim() != 1 or b.dim() != 1 or \
+                not a.is_contiguous() or not b.is_contiguous():
+            raise ValueError("q_start and seq_lens must be contiguous 1-d int32 tensors")
+        if b.shape[0] < 1 or a.shape[0] != b.shape[0] + 1:
+            raise ValueError(f"q_start must hold one entry more than seq_lens, got "
+                             f"{a.shape[0]} and {b.shape[0]}")
+        if a.device != b.device:
+            raise ValueError("q_start and seq_lens must be on the same device")
+        if self.max_q_len < 0:
+            raise ValueError(f"max_q_len must be >= 0, got {self.max_q_len}")
+        self._c = _lib.Ragged(b.shape[0], a.data_ptr(), b.data_ptr(), int(self.max_q_len))
+
+    @property
+    def requests(self) -> int:
+        return self.seq_lens.shape[0]
+
+
+def _inference_only(name: str, device: torch.device, *ts) -> None:
+    """All tensors on ``device`` (CUDA) and none that a backward pass would need."""
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("TurboQuant kernels need CUDA tensors (there is no CPU path)")
+        if t.device != device:
+            raise ValueError(f"{name}: tensors on {device} and {t.device}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or "
+                               "with detached tensors")
+
+
+def _on(device: torch.device):
+    """The launch's device made current (a no-op when it is)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _rows(x: torch.Tensor, name: str) -> _lib.Tensor4:
+    """A flattened (N, H, D) tensor as the (1, H, N, D) view of the C ABI."""
+    if x.dim() != 3:
+        raise ValueError(f"{name} must be (rows, heads, head_dim), got shape {tuple(x.shape)}")
+    if x.dtype not in _DT:
+        raise ValueError(f"unsupported dtype {x.dtype} of {name}")
+    n, h, d = x.shape
+    s = x.stride()
+    return _lib.Tensor4(x.data_ptr(), _DT[x.dtype], (1, h, n, d), (0, s[1], s[0], s[2]))
+
+
+def _heads(x: torch.Tensor, name: str) -> _lib.Tensor4:
+    return tensor4(x) if x.dim() == 4 else _rows(x, name)
+
+
+def _positions(pos: Optional[torch.Tensor], b: int, t: int) -> Optional[_lib.Positions]:
+    if pos is None:
+        return None
+    if pos.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"positions must be int32 or int64, got {pos.dtype}")
+    if tuple(pos.shape) == (b, t):
+        stride = pos.stride()
+    elif tuple(pos.shape) == (t,):
+        stride = (0, pos.stride(0))
+    else:
+        raise ValueError(f"positions must be ({t},) or ({b}, {t}), got {tuple(pos.shape)}")
+    return _lib.Positions(pos.data_ptr(), 64 if pos.dtype == torch.int64 else 32, stride)
+
+
+def _check_norm(norm: Optional[HeadNorm], d: int) -> None:
+    if norm is not None and norm.weight.shape[0] != d:
+        raise ValueError(f"a head norm of {norm.weight.shape[0]} weights for heads of {d}")
+
+
+def _ref(x):
+    return None if x is None else ctypes.byref(x)
+
+
+def qk_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], rope: Optional[RopeTable],
+            positions: Optional[torch.Tensor] = None, q_norm: Optional[HeadNorm] = None,
+            k_norm: Optional[HeadNorm] = None, q_out: Optional[torch.Tensor] = None,
+            k_out: Optional[torch.Tensor] = None):
+    """Norm (optional) and rotation (optional) of query and key heads in one
+    pass, in fp32 with one rounding: q (N, Hq, D), k (N, Hkv, D) with
+    positions (N,), or q (B, Hq, T, D), k (B, Hkv, T, D) with positions (T,)
+    or (B, T); any strides.  Either of q and k may be None.  ``q_out`` /
+    ``k_out``: where the results go (may be q / k itself).  A position outside
+    the table takes its row 0 and sets _lib.DEV_BAD_POSITION in the device
+    status word.  Returns (q_out, k_out)."""
+    one = q if q is not None else k
+    if one is None:
+        raise ValueError("neither q nor k is given")
+    if rope is not None and positions is None:
+        raise ValueError("a rotation needs positions")
+    b, t = (one.shape[0], one.shape[2]) if one.dim() == 4 else (1, one.shape[0])
+    _inference_only("qk_rope", one.device, q, k, q_out, k_out, positions,
+                    rope.cos_sin if rope is not None else None,
+                    q_norm.weight if q_norm is not None else None,
+                    k_norm.weight if k_norm is not None else None)
+    if q is not None:
+        _check_norm(q_norm, q.shape[-1])
+        q_out = torch.empty_like(q) if q_out is None else q_out
+    if k is not None:
+        _check_norm(k_norm, k.shape[-1])
+        k_out = torch.empty_like(k) if k_out is None else k_out
+    ts = [None if x is None else _heads(x, n) for x, n in
+          ((q, "q"), (q_out, "q_out"), (k, "k"), (k_out, "k_out"))]
+    pos = _positions(positions, b, t)
+    with _on(one.device):
+        _lib.check("tq_qk_rope", _lib.load().tq_qk_rope(
+            _ref(rope and rope._c), _ref(pos), _ref(ts[0]), _ref(ts[1]), _ref(q_norm and q_norm._c),
+            _ref(ts[2]), _ref(ts[3]), _ref(k_norm and k_norm._c), _stream(one.device)))
+    return q_out, k_out
+
+
+def append_ragged(tables: LayerTables, pages, k: torch.Tensor, v: torch.Tensor,
+                  batch: RaggedBatch, rope: Optional[RopeTable] = None,
+                  k_norm: Optional[HeadNorm] = None,
+                  positions: Optional[torch.Tensor] = None) -> None:
+    """Quantise and store a flattened batch's tokens, k and v (N, Hkv, D), at
+    their requests' positions; ``pages`` holds stream r * Hkv + h of request
+    r, head h.  k is normed and rotated on the way (both optional), by its
+    position in its request or by ``positions`` (N,).  A token whose position
+    lies outside the pages is dropped and sets _lib.DEV_BAD_POSITION."""
+    _inference_only("append_ragged", k.device, k, v, batch.q_start, positions,
+                    rope.cos_sin if rope is not None else None,
+                    k_norm.weight if k_norm is not None else None)
+    _check_norm(k_norm, k.shape[-1])
+    kt, vt, c = _rows(k, "k"), _rows(v, "v"), _cache_desc(pages)
+    pos = _positions(positions, 1, k.shape[0])
+    with _on(k.device):
+        _lib.check("tq_append_ragged", _lib.load().tq_append_ragged(
+            ctypes.byref(tables.geom()), ctypes.byref(tables.ctables()), ctypes.byref(c),
+            ctypes.byref(kt), ctypes.byref(vt), ctypes.byref(batch._c), _ref(rope and rope._c),
+            _ref(k_norm and k_norm._c), _ref(pos), _stream(k.device)))
+
+
+def dequantize_ragged(tables: LayerTables, pages, batch: RaggedBatch,
+                      k_out: Optional[torch.Tensor], v_out: Optional[torch.Tensor]) -> None:
+    """Write the stored keys and values of a flattened batch's tokens into the
+    rows of (N, Hkv, D) tensors; either may be None.  A row whose position
+    lies outside the pages is zeroed and sets _lib.DEV_BAD_POSITION."""
+    one = k_out if k_out is not None else v_out
+    if one is None:
+        raise ValueError("neither k_out nor v_out is given")
+    _inference_only("dequantize_ragged", one.device, k_out, v_out, batch.q_start)
+    kt = _rows(k_out, "k_out") if k_out is not None else None
+    vt = _rows(v_out, "v_out") if v_out is not None else None
+    c = _cache_desc(pages)
+    with _on(one.device):
+        _lib.check("tq_dequantize_ragged", _lib.load().tq_dequantize_ragged(
+            ctypes.byref(tables.geom()), ctypes.byref(tables.ctables()), ctypes.byref(c),
+            ctypes.byref(batch._c), _ref(kt), _ref(vt), _stream(one.device)))
+
+
+def attend_ragged(tables: LayerTables, pages, q: torch.Tensor, batch: RaggedBatch,
+                  scale: Optional[float] = None, causal: bool = True,
+                  out: Optional[torch.Tensor] = None,
+                  workspace: Optional[DecodeWorkspace] = None, engine: int = 0) -> torch.Tensor:
+    """Attention of a flattened batch q (N, Hq, D) straight off the packed
+    pages, each request's rows over its own tokens [0, seq_lens[r]): causal
+    (prompt chunks, draft tokens, single tokens, mixed), or with ``causal``
+    False every row over all of them (cross attention: the pages hold an
+    encoder's states, seq_lens their lengths).  A row that sees no key is
+    zero.  Work is split along long contexts; ``engine`` as in
+    prefill_attention.  Pass a ``workspace`` to reuse one buffer across
+    calls on one stream."""
+    _inference_only("attend_ragged", q.device, q, out, batch.q_start)
+    if out is None:
+        out = torch.empty_like(q)
+    lib = _lib.load()
+    qt, ot = _rows(q, "q"), _rows(out, "out")
+    g, c = tables.geom(), _cache_desc(pages)
+    a = _lib.AttendArgs(ctypes.pointer(qt), ctypes.pointer(ot), batch._c,
+                        float(scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])),
+                        1 if causal else 0, int(engine))
+    with _on(q.device):
+        nbytes = lib.tq_attend_ragged_workspace_bytes(ctypes.byref(g), ctypes.byref(c),
+                                                      ctypes.byref(a))
+        if nbytes == 0:
+            raise _lib.TqError("tq_attend_ragged_workspace_bytes", _lib.TQ_ERR_INVALID,
+                               _lib.last_error())
+        ws = (workspace or DecodeWorkspace()).get(nbytes, q.device)
+        _lib.check("tq_attend_ragged", lib.tq_attend_ragged(
+            ctypes.byref(g), ctypes.byref(tables.ctables()), ctypes.byref(c), ctypes.byref(a),
+            ws.data_ptr(), ws.numel(), _stream(q.device)))
     return out

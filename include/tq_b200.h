@@ -63,6 +63,10 @@ extern "C" {
 /* device status word bits (written by kernels into the workspace) */
 #define TQ_DEV_WAIT_TIMEOUT 1u  /* a bounded mbarrier wait ran out          */
 #define TQ_DEV_BAD_BLOCK 2u     /* a block-table entry was outside the pool */
+#define TQ_DEV_BAD_POSITION 4u  /* a position outside the rotation table or,
+                                   in a ragged append, outside the pages      */
+#define TQ_DEV_BAD_BATCH 8u     /* a ragged batch's row offsets do not ascend
+                                   within the tensor's rows                   */
 
 typedef struct tq_geom {
   int32_t head_dim;    /* D: multiple of 32, 32..256                        */
@@ -336,6 +340,113 @@ int32_t tq_append_tensor_core(const tq_geom* g, const tq_tables* t, const tq_ten
  * its bounded waits ran out).  Blocking copy on `stream`.  No reference
  * counterpart: the reference's append runs on the host. */
 int32_t tq_device_status(uint32_t* status, void* stream);
+
+/* --------------------------------------------------------------------------
+ * Serving operators on a flattened batch of requests: what runs between a
+ * layer's q/k/v projections and its output projection.  No counterpart in the
+ * reference (its models rotate and norm in transformers, and its cache takes
+ * one length for the whole batch).  Device-side errors of these entries go
+ * to the library status word (tq_device_status).
+ * ------------------------------------------------------------------------*/
+
+/* Rotary position embedding of a head vector's first rot_dim dims by the
+ * angles of its position: (a, b) -> (a cos - b sin, b cos + a sin) for pair i
+ * at dims (i, rot_dim/2 + i), or (2i, 2i + 1) when interleaved; the other dims
+ * pass through.  A position outside the table takes its row 0 and sets
+ * TQ_DEV_BAD_POSITION. */
+typedef struct tq_rope {
+  const float* cos_sin;       /* [positions][rot_dim]: cos of pair i at i, its
+                                 sin at rot_dim/2 + i; 16-byte aligned        */
+  int64_t positions;
+  int32_t rot_dim;            /* even, 2..head_dim                            */
+  int32_t interleaved;
+} tq_rope;
+
+/* RMS norm of a head vector, before the rotation:
+ * x / sqrt(mean(x^2) + eps) * (weight + offset), in fp32. */
+typedef struct tq_head_norm {
+  const void* weight;         /* [head_dim]                                   */
+  int32_t dtype;              /* TQ_F32 / TQ_F16 / TQ_BF16                    */
+  float eps;
+  float offset;               /* 0, or 1 for weights stored as w - 1          */
+} tq_head_norm;
+
+/* Positions of the tokens, (B, T) with strides in elements (0: broadcast). */
+typedef struct tq_positions {
+  const void* data;           /* device                                       */
+  int32_t bits;               /* 32 or 64 (signed)                            */
+  int64_t stride[2];
+} tq_positions;
+
+/* Norm and rotation of query and key heads in one pass: q (B, Hq, T, D) and k
+ * (B, Hkv, T, D) to q_out and k_out of the same shapes and types, computed in
+ * fp32 and rounded once.  Either pair may be NULL; so may a norm, and rope
+ * (then positions are not read).  An output may be its input (same view), else
+ * it must not overlap the inputs.  D: 1..256. */
+int32_t tq_qk_rope(const tq_rope* rope, const tq_positions* pos, const tq_tensor4* q,
+                   const tq_tensor4* q_out, const tq_head_norm* q_norm, const tq_tensor4* k,
+                   const tq_tensor4* k_out, const tq_head_norm* k_norm, void* stream);
+
+/* A flattened batch: row q_start[r] + i of a tensor (1, H, N, D) is token i of
+ * request r's new tokens, at position seq_lens[r] - (q_start[r+1] -
+ * q_start[r]) + i of the request.  Rows outside [q_start[0],
+ * q_start[requests]) belong to no request: they are neither read nor
+ * written.  Request r's pages are those of streams r * Hkv + h. */
+typedef struct tq_ragged {
+  int64_t requests;           /* R                                            */
+  const int32_t* q_start;     /* device [R + 1], ascending                    */
+  const int32_t* seq_lens;    /* device [R]: tokens of the request, the new
+                                 ones included                                */
+  int64_t max_q_len;          /* >= the most new tokens of a request (shapes
+                                 the launch; results do not depend on it)     */
+} tq_ragged;
+
+/* tq_append of a ragged batch: k and v (1, Hkv, N, D) go to the positions of
+ * their tokens, k normed (k_norm) and rotated (rope) on the way, both
+ * optional.  pos: rotation positions of the rows (stride[1]; NULL: each
+ * token's position in its request).  A token whose position lies outside the
+ * pages is dropped and sets TQ_DEV_BAD_POSITION.  Codes as tq_append's of the
+ * rotated vector in fp32 (no rounding to k's type in between).  head_dim <=
+ * 128, no QJL sketch. */
+int32_t tq_append_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
+                         const tq_tensor4* k, const tq_tensor4* v, const tq_ragged* batch,
+                         const tq_rope* rope, const tq_head_norm* k_norm,
+                         const tq_positions* pos, void* stream);
+
+/* tq_dequantize of a ragged batch: the stored keys and values of the batch's
+ * tokens to their rows of k_out / v_out (1, Hkv, N, D); either may be NULL.  A
+ * row whose position lies outside the pages is zeroed and sets
+ * TQ_DEV_BAD_POSITION. */
+int32_t tq_dequantize_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
+                             const tq_ragged* batch, const tq_tensor4* k_out,
+                             const tq_tensor4* v_out, void* stream);
+
+/* Attention of a ragged batch straight off the packed pages: row i of request
+ * r attends the request's tokens [0, seq_lens[r]), with causal only those at
+ * or before its own position.  causal = 0 with seq_lens the lengths of stored
+ * encoder states is cross attention (the queries are then no tokens of the
+ * cache).  A row that sees no key is zero.  Scores, values and geometries as
+ * in tq_prefill_attn (no QJL sketch, no window).  A stored norm that is not
+ * finite makes NaN of the rows that attend its token and of no other. */
+typedef struct tq_attend_args {
+  const tq_tensor4* q;        /* (1, Hq, N, D)                                */
+  const tq_tensor4* out;
+  tq_ragged batch;
+  float scale;                /* softmax scale                                */
+  int32_t causal;
+  int32_t engine;             /* 0: the fastest kernel for the shape; 1: the
+                                 mma.sync kernel; 2 / 3: the tcgen05 kernel
+                                 with 128 / 256 rows per CTA                  */
+} tq_attend_args;
+
+/* 0 on bad arguments.  The workspace must be 256-byte aligned and belongs to
+ * one call at a time (calls on one stream may share it, with decode calls
+ * too: its first 64 bytes, the decode's status word, are left alone). */
+size_t tq_attend_ragged_workspace_bytes(const tq_geom* g, const tq_cache* c,
+                                        const tq_attend_args* a);
+int32_t tq_attend_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
+                         const tq_attend_args* a, void* workspace, size_t workspace_bytes,
+                         void* stream);
 
 /* Device memory shareable with the other processes of one node (CUDA IPC on
  * a plain allocation; no multicast object).  tq_shared_alloc returns a zeroed

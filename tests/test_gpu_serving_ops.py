@@ -1,0 +1,610 @@
+"""The serving operators on ragged batches (qk_rope, append_ragged, dequantize_ragged,
+attend_ragged) against their plain forms in 64 bits.
+
+Tolerances (u = 2^-24; half_ulp(t) = eps(t) / 2):
+  * qk_rope: one rounding to the output type, half_ulp |y|, plus the fp32 arithmetic
+    (serving_oracle.rope_slack); fp16 results below 2^-14 are off by at most 2^-25;
+  * append_ragged codes: an fp32 dot product of unit vectors is off by at most D u <= 7.6e-6 and the
+    normed, rotated input by 16 u of its largest entry, so a code may differ from the 64-bit one
+    only where the rotated value lies within 1e-5 of a boundary; norms: fp16 half ulp plus 32 u;
+  * dequantize_ragged: half_ulp |x| plus 2^-16 n sum_j |c_j R_ji| (D = 128 fp32 terms: 2^-17);
+  * attend_ragged: the bar of the prefill tests for fp16 tensor-core operands, cosine >= 0.9999
+    and max-abs within 4e-3 max|o| plus half an ulp of the output type.
+"""
+import numpy as np
+import pytest
+import torch
+
+import serving_oracle as S
+from bhaskera_col_b200 import _lib
+from bhaskera_col_b200.inference import ops
+from test_gpu_parity import DEV, cosine, make_tables
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def randn(shape, seed, dtype=BF16, outlier=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(shape, generator=g)
+    if outlier:
+        x[..., outlier % shape[-1]] *= 8
+    return x.to(dtype).to(DEV)
+
+
+def int32(x):
+    return torch.tensor(list(x), dtype=torch.int32, device=DEV)
+
+
+def make_batch(lens, lead=0):
+    """lens: (new tokens, tokens in the cache) per request; the first row is `lead`."""
+    start = np.concatenate([[0], np.cumsum([a for a, _ in lens])]) + lead
+    seq = [b for _, b in lens]
+    return (ops.RaggedBatch(int32(start), int32(seq), max([a for a, _ in lens] + [0])),
+            start.tolist(), seq)
+
+
+def make_paged(tables, streams, tokens, seed=0):
+    """An empty pool in shuffled order behind a block table, and the table."""
+    P = max(-(-tokens // 64), 1)
+    pb = ops.page_bytes(tables.head_dim, tables.key_bits, tables.value_bits, False)
+    g = torch.Generator().manual_seed(seed)
+    perm = torch.randperm(streams * P + 3, generator=g)[: streams * P].to(torch.int32).view(streams, P)
+    pool = torch.zeros((streams * P + 3, pb), dtype=torch.uint8, device=DEV)
+    return ops.PagedPages(pool, perm.to(DEV))
+
+
+def contiguous(pages):
+    return pages.pool[pages.block_table.long()] if isinstance(pages, ops.PagedPages) else pages
+
+
+def fill(tables, pages, R, H, tokens, seed):
+    """Every request's tokens [0, tokens) stored through tq_append."""
+    k, v = (randn((R, H, tokens, tables.head_dim), seed + i, outlier=5 + i) for i in range(2))
+    ops.append(tables, pages, k, v, 0)
+
+
+def ok_status():
+    torch.cuda.synchronize()
+    return ops.device_status(DEV)
+
+
+# ------------------------------------------------------------------------------------- qk_rope
+def check_rope(got, x, table, pos, norm):
+    w = norm.weight if norm else None
+    eps, off = (norm.eps, norm.offset) if norm else (0.0, 0.0)
+    cs = table.cos_sin if table else None
+    want = S.rope(x, cs, pos, table.interleaved if table else False, w, eps, off)
+    tol = S.half_ulp(x.dtype) * np.abs(want) + S.rope_slack(x, w, eps, off)
+    if x.dtype == F16:
+        tol = tol + 2.0 ** -25
+    err = np.abs(got.detach().cpu().double().numpy() - want)
+    assert (err <= tol).all(), (err - tol).max()
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n,hq,hkv,D,rot,norm", [
+    (1, 1, 1, 128, 128, False), (5, 8, 2, 128, 128, True), (131, 5, 1, 64, 64, True),
+    (33, 4, 4, 128, 64, False), (17, 3, 3, 96, 32, True), (9, 2, 1, 256, 256, True),
+    (7, 2, 2, 80, 48, True), (3, 1, 1, 2, 2, False), (64, 40, 8, 128, 128, True)])
+def test_qk_rope_matches_plain_form(n, hq, hkv, D, rot, norm, dtype, interleaved):
+    table = ops.RopeTable.build(rot, 5000, interleaved=interleaved, device=DEV)
+    pos = torch.randint(0, 5000, (n,), generator=torch.Generator().manual_seed(n))
+    pos[0], pos[-1] = 0, 4999
+    norms = [ops.HeadNorm(randn((D,), 7 + i, dtype if i else F32), 1e-6, float(i))
+             if norm else None for i in range(2)]
+    q, k = randn((n, hq, D), 1, dtype, 3), randn((n, hkv, D), 2, dtype)
+    for bits in (torch.int32, torch.int64):
+        qo, ko = ops.qk_rope(q, k, table, pos.to(DEV, bits), *norms)
+        assert qo.dtype == dtype and qo.shape == q.shape
+        check_rope(qo, q, table, pos.numpy(), norms[0])
+        check_rope(ko, k, table, pos.numpy(), norms[1])
+    assert ok_status() == 0
+
+
+def test_qk_rope_views_in_place_and_one_side():
+    """Slices of one fused projection, rotated in place; HF's (B, H, T, D) transposed layout;
+    broadcast positions and broadcast inputs; rows a multiple of nothing."""
+    table = ops.RopeTable.build(128, 300, device=DEV)
+    n, hq, hkv, D = 19, 6, 2, 128
+    fused = randn((n, (hq + 2 * hkv) * D), 3)
+    keep = fused.clone()
+    q = fused[:, : hq * D].view(n, hq, D)
+    k = fused[:, hq * D: (hq + hkv) * D].view(n, hkv, D)
+    pos = torch.arange(n, device=DEV) * 7
+    qk = q.clone(), k.clone()
+    ops.qk_rope(q, k, table, pos, q_out=q, k_out=k)
+    check_rope(q, qk[0], table, pos.cpu().numpy(), None)
+    check_rope(k, qk[1], table, pos.cpu().numpy(), None)
+    assert torch.equal(fused[:, (hq + hkv) * D:], keep[:, (hq + hkv) * D:])      # v untouched
+    # (B, H, T, D) views of (B, T, H, D) memory, odd element offset, positions (T,) and (B, T)
+    B, T = 2, 13
+    raw = randn((B * T * hq * D + 1,), 4)
+    x = raw[1:].view(B, T, hq, D).transpose(1, 2)
+    for p in (torch.arange(T, device=DEV), torch.arange(B * T, device=DEV).view(B, T).flip(0)):
+        y, none = ops.qk_rope(x, None, table, p)
+        assert none is None
+        pp = p.expand(B, T).cpu().numpy()
+        for b in range(B):
+            check_rope(y[b].transpose(0, 1), x[b].transpose(0, 1), table, pp[b], None)
+    # one head read by all (stride 0), and a reversed head dim order through strides
+    one = randn((n, 1, D), 5).expand(n, 4, D)
+    y, _ = ops.qk_rope(one, None, table, pos)
+    check_rope(y, one.contiguous(), table, pos.cpu().numpy(), None)
+    z = randn((n, D, 3), 6).transpose(1, 2)
+    _, y = ops.qk_rope(None, z, table, pos)
+    check_rope(y, z.contiguous(), table, pos.cpu().numpy(), None)
+    # only a norm
+    norm = ops.HeadNorm(randn((D,), 8), 1e-5)
+    y, _ = ops.qk_rope(z, None, None, None, q_norm=norm)
+    check_rope(y, z.contiguous(), None, None, norm)
+    # no rows
+    e, _ = ops.qk_rope(z[:0], None, table, pos[:0])
+    assert e.shape == (0, 3, D) and ok_status() == 0
+
+
+def test_qk_rope_extremes():
+    """Zero rows stay zero under the norm, huge and tiny rows keep their direction, NaN and inf
+    stay in their own head; a position outside the table is flagged and turns by row 0."""
+    table = ops.RopeTable.build(64, 100, device=DEV)
+    x = randn((6, 2, 64), 1, F32)
+    x[0] = 0
+    x[1] *= 1e18
+    x[2] *= 1e-18
+    x[3, 0, 5] = float("nan")
+    x[4, 1, 6] = float("inf")
+    norm = ops.HeadNorm(torch.ones(64, device=DEV), 1e-6)
+    pos = torch.tensor([1, 2, 3, 4, 5, 6], device=DEV)
+    y, _ = ops.qk_rope(x, None, table, pos, q_norm=norm)
+    assert (y[0] == 0).all()
+    want = S.rope(x, table.cos_sin, pos.cpu().numpy(), False, norm.weight, 1e-6)
+    ok = [(1, 0), (1, 1), (2, 0), (2, 1), (3, 1), (4, 0), (5, 0), (5, 1)]
+    for r, h in ok:
+        w = want[r, h]
+        assert np.abs(y[r, h].cpu().double().numpy() - w).max() <= 40 * 2.0 ** -24 * np.abs(w).max()
+    assert y[3, 0].isnan().any() and y[4, 1].isnan().any()
+    assert ok_status() == 0
+    bad = torch.tensor([100, -1, 0, 99, 1 << 40, 5], device=DEV)
+    y, _ = ops.qk_rope(x[5:].expand(6, 2, 64).contiguous(), None, table, bad)
+    assert ok_status() == _lib.DEV_BAD_POSITION
+    assert torch.equal(y[0], y[2]) and torch.equal(y[1], y[2]) and torch.equal(y[4], y[2])
+
+
+def test_rope_table_far_positions():
+    """Angles come from 64 bits: at position 10^6 the table is the rounding of the exact values."""
+    t = ops.RopeTable.build(32, 1_000_001, base=500000.0, scale=1.25, device=DEV)
+    f = 500000.0 ** (-np.arange(0, 32, 2) / 32)
+    a = 1_000_000 * f
+    want = 1.25 * np.concatenate([np.cos(a), np.sin(a)])
+    # 64-bit angle off by 2^-53 * 1e6 at most (2e-10), then one rounding to fp32
+    assert np.abs(t.cos_sin[1_000_000].cpu().double().numpy() - want).max() <= 1.25 * 2.0 ** -24 + 1e-9
+
+
+# --------------------------------------------------------------- append_ragged, dequantize_ragged
+LENS = {
+    "decode": [(1, 1), (1, 64), (1, 65), (1, 200)],
+    "prompts": [(70, 70), (128, 128), (1, 1), (63, 63)],
+    "mixed": [(5, 130), (1, 77), (0, 50), (64, 64), (129, 300), (3, 3)],
+    "one": [(1, 1)],
+}
+
+
+def check_stored(tables, pages, k, v, start, seq, R, H, kx):
+    """Codes and norms of every new token against 64 bits; kx: the transformed keys in 64 bits."""
+    D = tables.head_dim
+    tokens = contiguous(pages).shape[1] * 64
+    f = S.parse(tables, contiguous(pages), tokens)
+    Rm = tables.rot.cpu().double().numpy()
+    r, pos = S.positions(start, seq, k.shape[0])
+    rows = np.nonzero(r >= 0)[0]
+    for name, x, bnd in (("k", kx, tables.k_boundaries), ("v", v.cpu().double().numpy(), tables.v_boundaries)):
+        b = bnd.cpu().double().numpy()
+        idx = f[f"{name}_idx"].reshape(R, H, tokens, D)[r[rows], :, pos[rows]]
+        nrm = f[f"{name}_norm"].reshape(R, H, tokens)[r[rows], :, pos[rows]].astype(np.float64)
+        xs = x[rows]
+        n = np.linalg.norm(xs, axis=-1)
+        y = (xs / np.maximum(n, 1e-8)[..., None]) @ Rm.T
+        want = (y[..., None] > b).sum(-1)
+        off = idx != want
+        assert off.mean() <= 1e-4
+        near = np.abs(y[..., None] - b).min(-1)
+        assert (near[off] <= 1e-5).all()
+        assert (np.abs(idx - want) <= 1).all()
+        assert (np.abs(nrm - n) <= n * (2.0 ** -11 + 32 * 2.0 ** -24) + 2.0 ** -25).all()
+
+
+def check_read(tables, pages, batch, start, seq, n, H, dtype):
+    D = tables.head_dim
+    tokens = contiguous(pages).shape[1] * 64
+    kd, vd = S.dense(tables, contiguous(pages), tokens)
+    f = S.parse(tables, contiguous(pages), tokens)
+    aR = np.abs(tables.rot.cpu().double().numpy())
+    r, pos = S.positions(start, seq, n)
+    outs = [torch.full((n, H, D), 7.0, dtype=dtype, device=DEV) for _ in range(2)]
+    ops.dequantize_ragged(tables, pages, batch, *outs)
+    for name, out, x, c in (("k", outs[0], kd, tables.k_centroids), ("v", outs[1], vd, tables.v_centroids)):
+        got = out.cpu().double().numpy()
+        ac = np.abs(c.cpu().double().numpy())[f[f"{name}_idx"]] @ aR
+        slack = (ac * f[f"{name}_norm"].astype(np.float64)[..., None]).reshape(-1, H, tokens, D)
+        x = x.reshape(-1, H, tokens, D)
+        for i in range(n):
+            if r[i] < 0:
+                assert (got[i] == 7.0).all()
+                continue
+            want = x[r[i], :, pos[i]]
+            tol = S.half_ulp(dtype) * np.abs(want) + 2.0 ** -16 * slack[r[i], :, pos[i]] + 2.0 ** -25
+            assert (np.abs(got[i] - want) <= tol).all()
+    only = torch.full((n, H, D), 7.0, dtype=dtype, device=DEV)
+    ops.dequantize_ragged(tables, pages, batch, None, only)
+    assert torch.equal(only, outs[1])
+
+
+@pytest.mark.parametrize("D,kb,vb,H,dtype,xform", [
+    (128, 4, 2, 2, BF16, "rope"), (128, 4, 4, 8, BF16, "norm+rope"), (128, 3, 3, 1, F16, "norm"),
+    (128, 8, 1, 3, F32, "interleaved"), (64, 3, 3, 4, F16, "rope"), (64, 4, 2, 5, BF16, "none"),
+    (64, 6, 5, 2, F32, "interleaved"), (96, 5, 7, 1, BF16, "norm+rope"),
+    (32, 2, 2, 2, BF16, "rope"), (128, 2, 3, 5, BF16, "interleaved"), (128, 6, 6, 2, BF16, "none")])
+@pytest.mark.parametrize("lens", sorted(LENS))
+def test_append_ragged_and_read_back(D, kb, vb, H, dtype, xform, lens):
+    tables = make_tables(D, kb, vb, False)
+    lens = LENS[lens]
+    R = len(lens)
+    batch, start, seq = make_batch(lens, lead=2)
+    n = start[-1] + 3                                     # rows before and behind the batch
+    pages = make_paged(tables, R * H, max(seq))
+    before = pages.pool.clone()
+    k, v = randn((n, H, D), 1, dtype, 9), randn((n, H, D), 2, dtype, 11)
+    rope = None if xform in ("none", "norm") else \
+        ops.RopeTable.build(D if xform != "interleaved" else D // 2, 400,
+                            interleaved=xform == "interleaved", device=DEV)
+    norm = ops.HeadNorm(1 + 0.2 * randn((D,), 3, F32), 1e-6) if "norm" in xform else None
+    ops.append_ragged(tables, pages, k, v, batch, rope=rope, k_norm=norm)
+    assert ok_status() == 0
+    r, pos = S.positions(start, seq, n)
+    kx = S.rope(k, rope.cos_sin if rope else None, np.maximum(pos, 0), xform == "interleaved",
+                norm.weight if norm else None, 1e-6)
+    check_stored(tables, pages, k, v, start, seq, R, H, kx)
+    # nothing but the new tokens changed: blank them and compare with the pool before
+    geom_rows = {(int(pages.block_table[r[i] * H + h, pos[i] // 64]), int(pos[i] % 64))
+                 for i in range(n) if r[i] >= 0 for h in range(H)}
+    after = pages.pool.clone()
+    kr, vr = D * kb // 8, D * vb // 8
+    for pg, sl in geom_rows:
+        for off, row in ((0, kr), (64 * kr, vr), (64 * (kr + vr), 2), (64 * (kr + vr) + 128, 2)):
+            after[pg, off + sl * row: off + (sl + 1) * row] = 0
+    assert torch.equal(after, before)
+    for t in (dtype, BF16):
+        check_read(tables, pages, batch, start, seq, n, H, t)
+    assert ok_status() == 0
+
+
+def test_append_ragged_equals_append_and_takes_strides():
+    """Without a transform the codes are tq_append's; k and v may be slices of one projection;
+    rotation positions may be given; contiguous pages work like paged ones."""
+    D, H, R = 128, 2, 3
+    tables = make_tables(D, 4, 2, False)
+    lens = [(40, 40), (33, 33), (1, 1)]
+    batch, start, seq = make_batch(lens)
+    n = start[-1]
+    fused = randn((n, 3 * H * D), 5)
+    k, v = fused[:, H * D: 2 * H * D].view(n, H, D), fused[:, 2 * H * D:].view(n, H, D)
+    pb = ops.page_bytes(D, 4, 2, False)
+    pages = torch.zeros((R * H, 1, pb), dtype=torch.uint8, device=DEV)
+    ops.append_ragged(tables, pages, k, v, batch)
+    ref = torch.zeros_like(pages)
+    for r, (m, _) in enumerate(lens):
+        rows = slice(start[r], start[r + 1])
+        ops.append(tables, ref[r * H: (r + 1) * H], k[rows].transpose(0, 1).unsqueeze(0),
+                   v[rows].transpose(0, 1).unsqueeze(0), 0)
+    a, b = S.parse(tables, pages, 64), S.parse(tables, ref, 64)
+    for name in ("k_idx", "v_idx"):
+        assert (a[name] != b[name]).mean() <= 1e-4
+    for name in ("k_norm", "v_norm"):
+        assert (a[name] != b[name]).mean() <= 1e-3
+    # rotation positions other than the places in the request
+    rope = ops.RopeTable.build(D, 5000, device=DEV)
+    pos = torch.randint(0, 5000, (n,), generator=torch.Generator().manual_seed(1)).to(DEV)
+    for p in (pos, pos.to(torch.int32), pos.repeat_interleave(2)[::2]):
+        pages.zero_()
+        ops.append_ragged(tables, pages, k, v, batch, rope=rope, positions=p)
+        check_stored(tables, pages, k, v, start, seq, R, H,
+                     S.rope(k, rope.cos_sin, pos.cpu().numpy()))
+    assert ok_status() == 0
+
+
+def test_append_ragged_bad_places():
+    """Tokens beyond the pages or before the start are dropped and flagged, pages outside the pool
+    neither written nor read; the others are stored; read-back zeroes what has no place."""
+    D, H = 128, 2
+    tables = make_tables(D, 4, 4, False)
+    batch, start, seq = make_batch([(3, 66), (4, 2), (2, 2), (2, 2)])
+    n = start[-1]
+    pages = make_paged(tables, 4 * H, 64)                 # room for 64 tokens a request
+    pages.block_table[2 * H] = -1
+    pages.block_table[2 * H + 1] = pages.pool.shape[0]
+    k, v = randn((n, H, D), 1), randn((n, H, D), 2)
+    ops.append_ragged(tables, pages, k, v, batch)
+    assert ok_status() == _lib.DEV_BAD_POSITION | _lib.DEV_BAD_BLOCK
+    out = torch.full((n, H, D), 7.0, dtype=BF16, device=DEV)
+    ops.dequantize_ragged(tables, pages, batch, out, None)
+    assert ok_status() == _lib.DEV_BAD_POSITION | _lib.DEV_BAD_BLOCK
+    stored = (out.float() * k.float()).sum((1, 2)) > 0.9 * k.float().square().sum((1, 2))
+    # request 0: positions 63 (stored), 64, 65 (outside); request 1: -2, -1 (outside), 0, 1
+    assert stored[:7].tolist() == [True, False, False, False, False, True, True]
+    assert (out[[1, 2, 3, 4]] == 0).all() and (out[7:9] == 0).all()
+    assert stored[9:].all()
+
+
+def test_append_ragged_zero_and_extreme_rows():
+    """A zero vector stores norm 0 and reads back as 0; norms of 1e-7 and 6e4 stay exact to fp16;
+    NaN keeps to its own vector."""
+    D, H = 128, 1
+    tables = make_tables(D, 4, 4, False)
+    batch, start, seq = make_batch([(5, 5)])
+    k = randn((5, H, D), 1, F32)
+    k /= k.norm(dim=-1, keepdim=True)
+    k[0] = 0
+    k[1] *= 1e-7
+    k[2] *= 6e4
+    k[3, 0, 7] = float("nan")
+    pages = make_paged(tables, H, 64)
+    ops.append_ragged(tables, pages, k, k, batch)
+    out = torch.empty((5, H, D), dtype=F32, device=DEV)
+    ops.dequantize_ragged(tables, pages, batch, out, None)
+    assert (out[0] == 0).all()
+    for i in (1, 2, 4):
+        n = k[i].norm().item()
+        assert abs(out[i].norm().item() / n - 1) < 0.1 if i != 1 else out[i].norm().item() < 2e-7
+        assert cosine(out[i].cpu(), k[i].cpu()) > 0.98 or i == 1
+    assert out[[0, 2, 4]].isfinite().all()
+    assert ok_status() == 0
+
+
+# ------------------------------------------------------------------------------- attend_ragged
+def check_attend(out, want, dtype, rows=None):
+    got = out.detach().cpu().double().numpy()
+    inside = ~np.isnan(want).any((1, 2))
+    g, w = got[inside], want[inside]
+    assert np.isfinite(g).all()
+    top = np.abs(w).max()
+    assert (g[np.abs(w).max((1, 2)) == 0] == 0).all()
+    assert cosine(g, w) >= 0.9999
+    assert np.abs(g - w).max() <= 4e-3 * top + S.half_ulp(dtype) * top
+
+
+ATTEND = {
+    "tokens": ([(1, 1), (1, 64), (1, 65), (1, 513)], True),
+    "drafts": ([(3, 5), (8, 700), (1, 129), (5, 64)], True),
+    "chunks": ([(130, 130), (65, 400), (1, 90), (0, 33), (257, 257)], True),
+    "empty rows": ([(6, 2), (3, 0), (2, 2), (0, 0)], True),
+    "cross": ([(1, 300), (7, 1), (40, 129), (3, 0), (5, 64)], False),
+    "split": ([(3, 5000)], True),
+    "split cross": ([(2, 3000), (1, 10)], False),
+}
+GEOM = [(128, 4, 2, 8, 2), (128, 4, 4, 5, 1), (128, 3, 3, 6, 2), (128, 2, 2, 2, 2),
+        (128, 6, 4, 8, 1), (128, 8, 8, 4, 2), (64, 4, 4, 4, 4), (64, 3, 3, 12, 4)]
+
+
+@pytest.mark.parametrize("case", sorted(ATTEND))
+@pytest.mark.parametrize("D,kb,vb,Hq,H", GEOM)
+def test_attend_ragged_matches_plain_form(D, kb, vb, Hq, H, case):
+    lens, causal = ATTEND[case]
+    tables = make_tables(D, kb, vb, False)
+    R = len(lens)
+    batch, start, seq = make_batch(lens, lead=1)
+    n = start[-1] + 2
+    pages = make_paged(tables, R * H, max(max(seq), 1))
+    fill(tables, pages, R, H, pages.shape[1] * 64, 3)
+    kd, vd = (x.reshape(R, H, -1, D) for x in S.dense(tables, contiguous(pages), pages.shape[1] * 64))
+    ws = ops.DecodeWorkspace()
+    engines = [0, 1] if D == 64 or kb == 8 else [0, 1, 2, 3]
+    if (D, kb, vb) == (128, 6, 4):
+        engines = [0, 1, 2, 3]
+    for dtype in (BF16, F32):
+        q = randn((n, Hq, D), 4, dtype)
+        want = S.attend(q, kd, vd, start, seq, S.default_scale(D), causal)
+        for engine in engines if dtype == BF16 else [0]:
+            out = torch.full_like(q, 7.0)
+            got = ops.attend_ragged(tables, pages, q, batch, causal=causal, out=out, workspace=ws,
+                                    engine=engine)
+            assert got is out and ok_status() == 0
+            outside = np.isnan(want).any((1, 2))
+            assert (out[torch.from_numpy(outside).to(DEV)] == 7.0).all()
+            check_attend(out, want, dtype)
+            again = ops.attend_ragged(tables, pages, q, batch, causal=causal, engine=engine)
+            inside = torch.from_numpy(~outside).to(DEV)
+            assert torch.equal(again[inside], out[inside])       # joined in a fixed order
+    assert ws.status() == 0
+
+
+def test_attend_ragged_views_scale_and_max_q_len():
+    """q a slice of one projection, out transposed memory, a scale; a larger max_q_len than needed
+    changes nothing beyond rounding; contiguous pages."""
+    D, Hq, H, R = 128, 4, 2, 3
+    tables = make_tables(D, 4, 4, False)
+    batch, start, seq = make_batch([(4, 200), (9, 9), (1, 64)])
+    n = start[-1]
+    pb = ops.page_bytes(D, 4, 4, False)
+    pages = torch.zeros((R * H, 4, pb), dtype=torch.uint8, device=DEV)
+    fill(tables, pages, R, H, 256, 8)
+    kd, vd = (x.reshape(R, H, -1, D) for x in S.dense(tables, pages, 256))
+    q = randn((n, (Hq + 2) * D + 1), 1, F16)[:, 1: 1 + Hq * D].view(n, Hq, D)
+    want = S.attend(q, kd, vd, start, seq, 0.05, True)
+    out = torch.empty((Hq, n, D), dtype=F16, device=DEV).transpose(0, 1)
+    ops.attend_ragged(tables, pages, q, batch, scale=0.05, out=out)
+    check_attend(out, want, F16)
+    wide = ops.RaggedBatch(batch.q_start, batch.seq_lens, 5000)
+    check_attend(ops.attend_ragged(tables, pages, q, wide, scale=0.05), want, F16)
+    one = ops.RaggedBatch(batch.q_start, batch.seq_lens, 0)          # a wrong bound is only slower
+    check_attend(ops.attend_ragged(tables, pages, q, one, scale=0.05), want, F16)
+    assert ok_status() == 0
+
+
+@pytest.mark.parametrize("engine", [1, 2, 3])
+def test_attend_ragged_infinite_and_nan_norms(engine):
+    """A key or value whose stored norm is inf or NaN makes NaN of the rows that see it and of no
+    other: earlier rows of the chunk and other requests stay as they were."""
+    D, Hq, H = 128, 2, 1
+    tables = make_tables(D, 4, 4, False)
+    batch, start, seq = make_batch([(70, 70), (5, 900)])
+    n = start[-1]
+    pages = make_paged(tables, 2 * H, 900)
+    fill(tables, pages, 2, H, pages.shape[1] * 64, 1)
+    q = randn((n, Hq, D), 2)
+    clean = ops.attend_ragged(tables, pages, q, batch, engine=engine)
+    kr = D * 4 // 8
+    norms = 64 * 2 * kr
+    for what in (0, 128):                                  # K norms, V norms
+        for bad in (float("inf"), float("nan")):
+            pool = pages.pool.clone()
+            pg = int(pages.block_table[0, 0])
+            at = norms + what + 2 * 40                     # token 40 of request 0
+            pool[pg, at: at + 2] = torch.tensor([bad], dtype=F16).view(torch.uint8).to(DEV)
+            # beyond the end of request 1 (page of tokens 896..959), nothing looks there
+            pg1 = int(pages.block_table[1, 14])
+            at1 = norms + what + 2 * 10
+            pool[pg1, at1: at1 + 2] = torch.tensor([bad], dtype=F16).view(torch.uint8).to(DEV)
+            out = ops.attend_ragged(tables, ops.PagedPages(pool, pages.block_table), q, batch,
+                                    engine=engine)
+            assert torch.equal(out[:40], clean[:40]) and torch.equal(out[70:], clean[70:])
+            assert out[40:70].isnan().all()
+    assert ok_status() == 0
+
+
+def test_attend_ragged_bad_pages_and_batches():
+    """Block-table entries outside the pool are flagged and never read; offsets that do not ascend
+    run nothing and are flagged."""
+    D, H = 128, 1
+    tables = make_tables(D, 4, 2, False)
+    batch, start, seq = make_batch([(2, 100), (2, 100)])
+    pages = make_paged(tables, 2, 128)
+    fill(tables, pages, 2, H, 128, 1)
+    q = randn((4, 2, D), 2)
+    clean = ops.attend_ragged(tables, pages, q, batch)
+    pages.block_table[1, 0] = -1
+    pages.block_table[1, 1] = pages.pool.shape[0]
+    for engine in (1, 2, 3):
+        out = ops.attend_ragged(tables, pages, q, batch, engine=engine)
+        assert ok_status() == _lib.DEV_BAD_BLOCK
+        assert (out[:2].float() - clean[:2].float()).abs().max() < 0.02 and out.isfinite().all()
+    huge = ops.RaggedBatch(int32([0, 4] * 40 + [4]), int32([100] * 80), 4)
+    many = make_paged(tables, 80, 128)
+    ops.attend_ragged(tables, many, q, huge)
+    assert ok_status() in (0, _lib.DEV_BAD_BATCH)
+    wild = ops.RaggedBatch(int32([-5, 90, 1 << 30]), int32([1 << 30, -7]), 4)
+    ops.attend_ragged(tables, pages, q, wild)
+    ops.append_ragged(tables, pages, q[:, :1].contiguous(), q[:, :1].contiguous(), wild)
+    torch.cuda.synchronize()
+    ops.device_status(DEV)
+
+
+# ---------------------------------------------------------------------------------- together
+def test_serving_step_together_captured_and_on_another_stream():
+    """rope -> append -> attend as a serving step runs them, eager, on a side stream and replayed
+    from a graph after the inputs and lengths changed in place: the same bits each time."""
+    D, Hq, H, R = 128, 8, 2, 4
+    tables = make_tables(D, 4, 2, False)
+    rope = ops.RopeTable.build(D, 1000, device=DEV)
+    norms = [ops.HeadNorm(1 + 0.1 * randn((D,), i, F32)) for i in range(2)]
+    lens = [[(1, 100), (4, 260), (1, 65), (2, 2)], [(2, 102), (1, 261), (3, 68), (2, 4)]]
+    pages = make_paged(tables, R * H, 320)
+    fill(tables, pages, R, H, 320, 1)
+    pool0 = pages.pool.clone()
+    ws = ops.DecodeWorkspace()
+    n = 8
+    data = [tuple(randn((n, h, D), 10 * i + j) for j, h in enumerate((Hq, H, H))) for i in range(2)]
+
+    def step(q, k, v, batch, pos, w):
+        qr, _ = ops.qk_rope(q, None, rope, pos, q_norm=norms[0])
+        ops.append_ragged(tables, pages, k, v, batch, rope=rope, k_norm=norms[1])
+        return ops.attend_ragged(tables, pages, qr, batch, workspace=w)
+
+    def args(i):
+        batch, start, seq = make_batch(lens[i])
+        _, pos = S.positions(start, seq, n)
+        return (*data[i], batch, int32(pos))
+
+    eager = []
+    for i in range(2):
+        pages.pool.copy_(pool0)
+        eager.append((step(*args(i), ws), pages.pool.clone()))
+        start, seq = args(i)[3].q_start.tolist(), args(i)[3].seq_lens.tolist()
+        kd, vd = (x.reshape(R, H, -1, D) for x in S.dense(tables, contiguous(pages), 320))
+        qx = torch.from_numpy(S.rope(data[i][0], rope.cos_sin, args(i)[4].cpu().numpy(), False,
+                                     norms[0].weight, 1e-6))
+        want = S.attend(qx, kd, vd, start, seq, S.default_scale(D), True)
+        want[start[-1]:] = np.nan
+        check_attend(eager[i][0], want, BF16)
+    side = torch.cuda.Stream()
+    pages.pool.copy_(pool0)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        out = step(*args(1), ops.DecodeWorkspace())
+    side.synchronize()
+    m = int(args(1)[3].q_start[-1])
+    assert torch.equal(out[:m], eager[1][0][:m]) and torch.equal(pages.pool, eager[1][1])
+    # one graph, replayed on both sets of inputs
+    live = [x if isinstance(x, ops.RaggedBatch) else x.clone() for x in args(0)]
+    graph_ws = ops.DecodeWorkspace()
+    pages.pool.copy_(pool0)
+    step(*live, graph_ws)                                  # workspace in place before the capture
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*live, graph_ws)
+    for i in (0, 1, 0):
+        pages.pool.copy_(pool0)
+        for dst, src in zip(live, args(i)):
+            if isinstance(dst, ops.RaggedBatch):
+                dst.q_start.copy_(src.q_start)
+                dst.seq_lens.copy_(src.seq_lens)
+            else:
+                dst.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        m = int(args(i)[3].q_start[-1])
+        assert torch.equal(out[:m], eager[i][0][:m]) and torch.equal(pages.pool, eager[i][1])
+    assert ok_status() == 0
+
+
+def test_decode_and_ragged_forms_agree():
+    """One new token a request: append_ragged + attend_ragged give what the fused decode step
+    gives (same pages up to boundary codes, outputs within the fp16 operands' bar)."""
+    D, Hq, H, R = 128, 8, 2, 3
+    tables = make_tables(D, 4, 2, False)
+    seq = [65, 200, 1]
+    pages = make_paged(tables, R * H, 256)
+    fill(tables, pages, R, H, 256, 1)
+    pool0 = pages.pool.clone()
+    q, k, v = randn((R, Hq, D), 1), randn((R, H, D), 2), randn((R, H, D), 3)
+    want = ops.decode_step(tables, pages, k.unsqueeze(2), v.unsqueeze(2), 255, q.unsqueeze(2),
+                           seq_lens=int32(seq))[:, :, 0]
+    pool1 = pages.pool.clone()
+    pages.pool.copy_(pool0)
+    batch, _, _ = make_batch([(1, s) for s in seq])
+    ops.append_ragged(tables, pages, k, v, batch)
+    assert (pages.pool != pool1).float().mean() < 1e-4
+    pages.pool.copy_(pool1)
+    got = ops.attend_ragged(tables, pages, q, batch)
+    assert cosine(got.float().cpu(), want.float().cpu()) >= 0.9999
+    assert (got.float() - want.float()).abs().max() <= 8e-3 * want.float().abs().max() + 2.0 ** -8
+    assert ok_status() == 0
+
+
+def test_no_rows():
+    """A batch without rows (and requests without new tokens) runs every operator and writes nothing."""
+    D, H = 128, 2
+    tables = make_tables(D, 4, 2, False)
+    pages = make_paged(tables, 2 * H, 64)
+    batch, _, _ = make_batch([(0, 0), (0, 30)])
+    x = torch.empty((0, H, D), dtype=BF16, device=DEV)
+    rope = ops.RopeTable.build(D, 10, device=DEV)
+    ops.append_ragged(tables, pages, x, x, batch, rope=rope)
+    ops.dequantize_ragged(tables, pages, batch, x, x)
+    assert ops.attend_ragged(tables, pages, x, batch).shape == (0, H, D)
+    y = torch.full((3, H, D), 7.0, dtype=BF16, device=DEV)          # rows of no request
+    ops.append_ragged(tables, pages, y, y, batch)
+    ops.dequantize_ragged(tables, pages, batch, y, None)
+    ops.attend_ragged(tables, pages, y.clone(), batch, out=y)
+    assert (y == 7).all() and (pages.pool == 0).all() and ok_status() == 0
