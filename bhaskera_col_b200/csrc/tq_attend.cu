@@ -8,8 +8,13 @@
 //     L = max(kMinTiles, ceil(all key tiles / wanted CTAs)),
 // one CTA each.  The list is built on the device (the lengths live there), so
 // the host neither waits nor reads them; it launches an upper bound of CTAs.
+// Two kernels share a batch: requests of few query rows take tiles of 8 or 16
+// rows (tq_attend_few.cu), the others tiles of 128 or more, each from a list of
+// its own.
 #include "tq_internal.h"
 #include "tq_ragged.cuh"
+
+#include <initializer_list>
 
 namespace tq {
 namespace {
@@ -17,9 +22,11 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kWaves = 3;                  // segments wanted per SM
 constexpr int kMinKeys = 512;              // shortest segment worth a CTA's set-up
+constexpr int kFewWaves = 4, kFewMinKeys = 768;   // the same for the few-row kernel
 
 struct PlanParams {
   RaggedView rv;
+  int64_t q_lo, q_hi;                      // the list's requests: q_lo < q_len <= q_hi
   int pcta, keys;                          // query positions per tile, keys per key tile
   int causal, G;
   int64_t wanted;                          // segments wanted, all head groups together
@@ -35,6 +42,14 @@ __device__ __forceinline__ int key_tiles(const PlanParams& p, const Request& q, 
   int64_t kend = q.seq;
   if (p.causal) kend = q.seq - q.q_len + tmin<int64_t>((i + 1) * p.pcta, q.q_len);
   return kend > 0 ? (int)((kend + p.keys - 1) / p.keys) : 0;
+}
+
+// Request r, empty where it belongs to the other list.
+__device__ __forceinline__ Request listed_request(const PlanParams& p, int64_t r) {
+  Request q = {};
+  if (r < p.rv.R) q = request_at(p.rv, r);
+  if (q.q_len <= p.q_lo || q.q_len > p.q_hi) q.q_len = 0;
+  return q;
 }
 
 // Inclusive scan over the block of a pair of counts packed as hi:lo 32 bits.
@@ -60,7 +75,8 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t x, uint64_t* warp_tot, u
 // One CTA, one thread per request; a request of more than 32 tiles is walked
 // by its whole warp.  Pass 0 sums the key tiles, pass 1 counts and writes the
 // segments (in request and tile order: the list does not depend on timing).
-__global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p) {
+__global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p0, PlanParams p1) {
+  const PlanParams& p = blockIdx.x == 0 ? p0 : p1;         // one CTA per list
   __shared__ uint64_t warp_tot[kPlanThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31;
   for (int i = tid; i < p.max_slot * p.G; i += kPlanThreads) p.arrived[i] = 0;
@@ -68,8 +84,7 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p)
   uint64_t total = 0, sum = 0;
   for (int64_t r0 = 0; r0 < p.rv.R; r0 += kPlanThreads) {
     const int64_t r = r0 + tid;
-    Request q = {};
-    if (r < p.rv.R) q = request_at(p.rv, r);
+    const Request q = listed_request(p, r);
     const int64_t tiles = (q.q_len + p.pcta - 1) / p.pcta;
     uint64_t mine = 0;
     if (tiles <= 32)
@@ -118,8 +133,7 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p)
   uint64_t base = 0;
   for (int64_t r0 = 0; r0 < p.rv.R; r0 += kPlanThreads) {
     const int64_t r = r0 + tid;
-    Request q = {};
-    if (r < p.rv.R) q = request_at(p.rv, r);
+    const Request q = listed_request(p, r);
     const int64_t tiles = (q.q_len + p.pcta - 1) / p.pcta;
     uint64_t mine = 0;
     if (tiles <= 32)
@@ -178,42 +192,77 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p)
   }
 }
 
-// Shape of the launch: head group, query positions and rows of a CTA, and the
-// bounds of the work list; the workspace follows from it.
-struct AttendShape {
-  int engine, hc, pcta, rows, keys, G;
-  int64_t Hkv, wanted;
-  int64_t max_seg, max_slot;
-  size_t off_segs, off_arrived, off_ml, off_part, bytes;
+// Shape of one list's launch: head group, query positions and rows of a CTA,
+// the bounds of the work list and its place in the workspace.
+struct ListShape {
+  bool used;
+  int64_t q_lo, q_hi;
+  int hc, pcta, rows, keys, G;
+  int64_t wanted, max_seg, max_slot;
+  size_t off_nseg, off_segs, off_arrived, off_ml, off_part;
 };
+
+struct AttendShape {
+  int engine;                              // of the wide list
+  int64_t Hkv;
+  ListShape few, wide;
+  size_t bytes;
+};
+
+// Query rows of a request and KV head up to which the few-row kernel is taken.
+constexpr int kFewRows = 64;
 
 AttendShape attend_shape(const tq_geom* G, const tq_cache* c, const tq_attend_args* a) {
   AttendShape s = {};
-  const int64_t R = a->batch.requests, N = a->q->shape[2];
+  const int64_t R = a->batch.requests, N = a->q->shape[2], most = INT64_MAX;
   s.Hkv = c->streams / R;
   const int64_t g = a->q->shape[1] / s.Hkv;
   s.engine = 1;
-  s.hc = g % 8 == 0 ? 8 : g % 4 == 0 ? 4 : g % 2 == 0 ? 2 : 1;
-  s.rows = 128;
-  s.keys = 64;
-  s.pcta = s.rows / s.hc;
-  s.G = (int)(s.Hkv * (g / s.hc));
-  s.wanted = (int64_t)kWaves * device_sm_count();
-  // tiles: one per started block of positions; L cuts off at most wanted / G
-  // segments beyond them, and a cut tile has at most twice its extra ones
-  const int64_t extra = s.wanted / s.G + 1;
-  s.max_seg = N / s.pcta + R + extra;
-  s.max_slot = 2 * extra;
-  size_t off = 256;
+  const bool can = attend_few_applies(G) && (a->engine == 0 || a->engine == 4);
+  const int64_t few_q = a->engine == 4 ? most : tmax<int64_t>(kFewRows / g, 1);
+  size_t off = 256;                        // the first 64 bytes: the decode's status word
   auto take = [&](size_t bytes) {
     const size_t at = off;
     off = (off + bytes + 255) & ~(size_t)255;
     return at;
   };
-  s.off_segs = take(s.max_seg * sizeof(RaggedSeg));
-  s.off_arrived = take(s.max_slot * s.G * 4);
-  s.off_ml = take((size_t)s.max_slot * s.G * s.rows * 8);
-  s.off_part = take((size_t)s.max_slot * s.G * s.rows * G->head_dim * 4);
+  auto finish = [&](ListShape& l) {
+    l.used = true;
+    l.G = (int)(s.Hkv * ((g + l.hc - 1) / l.hc));
+    // tiles: one per started block of positions; L cuts off at most wanted / G
+    // segments beyond them, and a cut tile has at most twice its extra ones
+    const int64_t extra = l.wanted / l.G + 1;
+    l.max_seg = N / l.pcta + R + extra;
+    l.max_slot = 2 * extra;
+    l.off_segs = take(l.max_seg * sizeof(RaggedSeg));
+    l.off_arrived = take(l.max_slot * l.G * 4);
+    l.off_ml = take((size_t)l.max_slot * l.G * l.rows * 8);
+    l.off_part = take((size_t)l.max_slot * l.G * l.rows * G->head_dim * 4);
+  };
+  const bool wide = !can || a->batch.max_q_len > few_q;
+  if (can) {
+    ListShape& l = s.few;
+    l.q_hi = wide ? few_q : most;
+    l.rows = g * a->batch.max_q_len <= 8 ? 8 : 16;
+    l.hc = (int)tmin<int64_t>(g, l.rows);
+    l.pcta = l.rows / l.hc;
+    l.keys = kPageTokens;
+    l.wanted = (int64_t)kFewWaves * device_sm_count();
+    l.off_nseg = 64;
+    finish(l);
+  }
+  if (wide) {
+    ListShape& l = s.wide;
+    l.q_lo = can ? few_q : 0;
+    l.q_hi = most;
+    l.hc = g % 8 == 0 ? 8 : g % 4 == 0 ? 4 : g % 2 == 0 ? 2 : 1;
+    l.rows = 128;
+    l.pcta = l.rows / l.hc;
+    l.keys = kPageTokens;
+    l.wanted = (int64_t)kWaves * device_sm_count();
+    l.off_nseg = 68;
+    finish(l);
+  }
   s.bytes = off;
   return s;
 }
@@ -229,32 +278,48 @@ int launch_attend_ragged(const tq_geom* G, const tq_tables* t, const tq_cache* c
   const AttendShape s = attend_shape(G, c, a);
   if (a->q->shape[2] == 0) return TQ_OK;
   uint8_t* base = static_cast<uint8_t*>(ws);
-  PlanParams p;
-  p.rv = ragged_view(&a->batch, a->q->shape[2], c);
-  p.pcta = s.pcta;
-  p.keys = s.keys;
-  p.causal = a->causal;
-  p.G = s.G;
-  p.wanted = s.wanted;
-  p.min_tiles = kMinKeys / s.keys;
-  p.max_seg = (int)s.max_seg;
-  p.max_slot = (int)s.max_slot;
-  p.nseg = reinterpret_cast<int32_t*>(base + 64);   // below: the decode's status word
-  p.segs = reinterpret_cast<RaggedSeg*>(base + s.off_segs);
-  p.arrived = reinterpret_cast<int32_t*>(base + s.off_arrived);
-  p.status = status;
-  ragged_plan_kernel<<<1, kPlanThreads, 0, st>>>(p);
+  RaggedAttend rg[2];
+  PlanParams plan[2];
+  int lists = 0;
+  for (const ListShape* l : {&s.few, &s.wide}) {
+    if (!l->used) continue;
+    PlanParams& p = plan[lists];
+    p.rv = ragged_view(&a->batch, a->q->shape[2], c);
+    p.q_lo = l->q_lo;
+    p.q_hi = l->q_hi;
+    p.pcta = l->pcta;
+    p.keys = l->keys;
+    p.causal = a->causal;
+    p.G = l->G;
+    p.wanted = l->wanted;
+    p.min_tiles = (l == &s.few ? kFewMinKeys : kMinKeys) / l->keys;
+    p.max_seg = (int)l->max_seg;
+    p.max_slot = (int)l->max_slot;
+    p.nseg = reinterpret_cast<int32_t*>(base + l->off_nseg);
+    p.segs = reinterpret_cast<RaggedSeg*>(base + l->off_segs);
+    p.arrived = reinterpret_cast<int32_t*>(base + l->off_arrived);
+    p.status = status;
+    RaggedAttend& r = rg[lists++];
+    r.rv = p.rv;
+    r.plan.segs = p.segs;
+    r.plan.nseg = p.nseg;
+    r.plan.arrived = p.arrived;
+    r.plan.ml = reinterpret_cast<float2*>(base + l->off_ml);
+    r.plan.part = reinterpret_cast<float*>(base + l->off_part);
+    r.plan.G = l->G;
+    r.plan.rows = l->rows;
+  }
+  ragged_plan_kernel<<<lists, kPlanThreads, 0, st>>>(plan[0], plan[lists - 1]);
   if (check_launch("tq_attend_ragged/plan") != TQ_OK) return TQ_ERR_CUDA;
-  RaggedAttend rg;
-  rg.rv = p.rv;
-  rg.plan.segs = p.segs;
-  rg.plan.nseg = p.nseg;
-  rg.plan.arrived = p.arrived;
-  rg.plan.ml = reinterpret_cast<float2*>(base + s.off_ml);
-  rg.plan.part = reinterpret_cast<float*>(base + s.off_part);
-  rg.plan.G = s.G;
-  rg.plan.rows = s.rows;
-  return launch_attend_mma(G, t, c, a, rg, s.Hkv, s.hc, s.max_seg * s.G, status, st);
+  if (s.few.used) {
+    const int rc = launch_attend_few(G, t, c, a, rg[0], s.Hkv, s.few.hc, s.few.pcta, s.few.rows,
+                                     s.few.max_seg * s.few.G, status, st);
+    if (rc != TQ_OK) return rc;
+  }
+  if (s.wide.used)
+    return launch_attend_mma(G, t, c, a, rg[lists - 1], s.Hkv, s.wide.hc,
+                             s.wide.max_seg * s.wide.G, status, st);
+  return TQ_OK;
 }
 
 }  // namespace tq

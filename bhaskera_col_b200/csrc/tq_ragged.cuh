@@ -149,8 +149,21 @@ __device__ __forceinline__ int64_t part_row(const RaggedPlan& pl, int slot, int 
   return ((int64_t)slot * pl.G + group) * pl.rows + row;
 }
 
-// Called by every thread of a CTA that has stored its partial rows (out / l
-// and {m, l}) of a split tile: the last CTA of the tile joins the partials,
+// Called by every thread of a CTA that has stored its part of a split tile:
+// true for the tile's last CTA, which then sees the parts of all others.
+__device__ __forceinline__ bool last_of_tile(const RaggedPlan& pl, const SegWork& w, int* flag) {
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    const int done = atomicAdd(pl.arrived + (int64_t)w.seg.first * pl.G + w.group, 1);
+    *flag = done == w.seg.parts - 1;
+    __threadfence();
+  }
+  __syncthreads();
+  return *flag != 0;
+}
+
+// The last CTA of a split tile joins its partials (out / l and {m, l}),
 //   M = max_s m_s, w_s = l_s 2^(m_s - M), out = sum_s w_s out_s / sum_s w_s,
 // in slot order whatever the order of arrival, one warp per row.  `row_out(row)`
 // gives the element offset of a row's output, or -1 for a row without a query.
@@ -159,16 +172,8 @@ template <int D, class RowOut>
 __device__ __forceinline__ void join_partials(const RaggedPlan& pl, const SegWork& w, int nwarps,
                                               void* out, int o_dtype, int64_t o_stride,
                                               int* last_flag, RowOut row_out) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  __syncthreads();
-  if (tid == 0) {
-    __threadfence();
-    const int done = atomicAdd(pl.arrived + (int64_t)w.seg.first * pl.G + w.group, 1);
-    *last_flag = done == w.seg.parts - 1;
-    __threadfence();
-  }
-  __syncthreads();
-  if (!*last_flag) return;
+  if (!last_of_tile(pl, w, last_flag)) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int row = warp; row < pl.rows; row += nwarps) {
     const int64_t at = row_out(row);
     if (at < 0) continue;

@@ -657,7 +657,7 @@ def attend_ragged(tables: LayerTables, pages, q: torch.Tensor, batch: RaggedBatc
     False every row over all of them (cross attention: the pages hold an
     encoder's states, seq_lens their lengths).  A row that sees no key is
     zero.  Work is split along long contexts; ``engine`` as in
-    prefill_attention.  Pass a ``workspace`` to reuse one buffer across
+    prefill_attention, and 4 for the kernel of few query rows.  Pass a ``workspace`` to reuse one buffer across
     calls on one stream."""
     _inference_only("attend_ragged", q.device, q, out, batch.q_start)
     if out is None:
