@@ -22,7 +22,7 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kWaves = 3;                  // segments wanted per SM
 constexpr int kMinKeys = 512;              // shortest segment worth a CTA's set-up
-constexpr int kFewWaves = 4, kFewMinKeys = 768;   // the same for the few-row kernel
+constexpr int kFewWaves = 6, kFewMinKeys = 512;   // the same for the few-row kernel
 
 struct PlanParams {
   RaggedView rv;

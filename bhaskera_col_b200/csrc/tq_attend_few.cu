@@ -2,19 +2,22 @@
 // per request and KV head: single tokens, draft verification, short chunks.
 //
 // A CTA holds NQ = 8 NT query rows (positions x heads of one GQA group) and a
-// range of keys.  Its W warps take 16-token tiles in turn, each with its own
-// running max, sum and output, and never meet before the end, so no barrier
-// or copy pipeline stands between a warp and its loads.  Per tile:
+// range of pages.  Its four warps take a quarter (16 tokens) of every page,
+// each with its own running max, sum and output, and never meet before the
+// end, so no barrier or copy pipeline stands between a warp and its loads;
+// three CTAs share an SM, so one's set-up and end hide behind the others'
+// pages.  Per tile of 16 tokens:
 //   S^T = K^ Q'^T  tokens on M, query rows on N: mma.sync m16n8k16 (a handful
 //                  of rows would leave a 128-row tcgen05 tile empty);
 //   O^T += V^^T P'^T  with P' = exp2(S n_k - m) n_v as fp16.
 // A thread's codes are contiguous in a page row (quad order for K, octet order
 // for V), so both operands go from one coalesced global load per row straight
-// into fragment registers, through a table of code pairs: entry e is the
-// half2 of pair e, copied for all 32 lanes (no bank conflicts), K pairs in the
-// first and V pairs in the second 128 bytes of a 256-byte row.  The table sits
-// at a multiple of 64 KB, so one byte permute (or shift + mask) of the codes
-// is the whole shared-memory address.  V pairs join the codes of two tokens,
+// into fragment registers, through a table indexed by a byte of codes: the
+// half2 of a pair of 4-bit codes, or of pairs of 2-bit codes of two rows (6 bits of
+// two 3-bit codes take a shift and a mask instead).  Copies for 32 (16: 8-byte
+// entries are served in halves of a warp) lanes leave no bank conflicts, K in
+// the first and V in the second 128 bytes of a 256-byte row, so one byte
+// permute of the codes is the offset.  V pairs join the codes of two tokens,
 // interleaved by two masks per word.
 // The running max moves only when a score passes it by kRoom (a vote; the
 // shuffles and the rescale of 32 NT outputs run then: nearly every tile has a
@@ -38,6 +41,7 @@ constexpr float kLog2eF = 1.4426950408889634f;
 // 2^7, and with a value norm of at most 2^8 P' <= 2^15 stays in fp16 (for
 // larger norms the max moves at once, p <= 1 and P' <= the norm itself).
 constexpr float kRoom = 7.f;
+constexpr float kNoMax = -1e30f;   // below every score
 
 struct FewParams {
   const uint8_t* pages;
@@ -56,74 +60,116 @@ struct FewParams {
   RaggedAttend rg;
 };
 
-template <int D, int NT>
+constexpr int kW = 4;                                       // warps: quarters of a page
+
+template <int D, int KB, int VB, int NT>
 struct Few {
-  static constexpr int W = NT == 1 ? 16 : 12;              // warps
   static constexpr int NQ = 8 * NT;
-  static constexpr int LDO = D + 4;                        // floats per row of a partial (banks)
-  static constexpr int kBufs = W >= 8 ? 8 : W;             // partials summed at a time
-  // offsets from a 64 KB boundary: the pair table, then (the table is dead
-  // after the loop) the partial outputs over it
-  static constexpr int OFF_Q = 65536;                      // q' fp16 [NQ][D]
-  static constexpr int OFF_M = OFF_Q + 16 * D * 2;         // [W][NQ] running max
-  static constexpr int OFF_L = OFF_M + W * NQ * 4;         // [W][NQ] sums
-  static constexpr int OFF_U = OFF_L + W * NQ * 4;         // [16][LDO] joined output
-  static constexpr int LDA = D / 2 + 4;                    // words per row of a rotation operand
-  static constexpr int OFF_A = OFF_U + 16 * LDO * 4;       // [2: hi, lo][16][LDA] fp16 pairs
-  static constexpr int OFF_R = OFF_A + 2 * 16 * LDA * 4;   // [16] sums of the rows, flags
+  static constexpr bool KQ = KB == 2, VQ = VB == 2;         // two pairs per table entry
+  static constexpr int KF = KQ ? 8 : 2 * KB, VF = VQ ? 8 : 2 * VB;   // bits of an index
+  static constexpr int ROWS = 1 << (KF > VF ? KF : VF);     // table rows of 256 bytes
+  static constexpr int LDO = D + 4;                         // floats per row of an output (banks)
+  static constexpr int LDA = D / 2 + 4;                     // words per row of a rotation operand
+  // after the loop the table is dead: partial outputs, then the joined one and
+  // the operand of the last rotation take its place
+  static constexpr int OFF_P = 0;                           // [kW][NQ][LDO]
+  static constexpr int OFF_A = kW * NQ * LDO * 4;           // [2: hi, lo][16][LDA] fp16 pairs
+  static constexpr int LOOP = ROWS * 256, END = OFF_A + 2 * 16 * LDA * 4;
+  static constexpr int OFF_Q = LOOP > END ? LOOP : END;     // q' fp16 [NQ][D]
+  static constexpr int OFF_M = OFF_Q + 16 * D * 2;          // [kW][NQ] running max
+  static constexpr int OFF_L = OFF_M + kW * NQ * 4;         // [kW][NQ] sums
+  static constexpr int OFF_R = OFF_L + kW * NQ * 4;         // [16] sums, [16] maxima, flags
   static constexpr int BYTES = OFF_R + 256;
-  static_assert(kBufs * NQ * LDO * 4 <= 65536 + 4096, "partials");
 };
 
 // N consecutive bytes of codes as little-endian words.  Multiples of 4 are
-// aligned vector loads; other counts load the words that hold them and shift.
+// aligned loads; other counts load the words that hold them and shift by `sh`.
 template <int N>
 struct Codes { uint32_t w[(N + 3) / 4]; };
 
 template <int N>
-__device__ __forceinline__ Codes<N> load_codes(const uint8_t* row, int off) {
+__device__ __forceinline__ Codes<N> load_codes(const uint8_t* p, uint32_t sh) {
   Codes<N> c;
   if constexpr (N == 16) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + off));
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
     c.w[0] = v.x; c.w[1] = v.y; c.w[2] = v.z; c.w[3] = v.w;
   } else if constexpr (N == 8) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(row + off));
+    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
     c.w[0] = v.x; c.w[1] = v.y;
   } else if constexpr (N % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i < N / 4; ++i) c.w[i] = __ldg(reinterpret_cast<const uint32_t*>(row + off) + i);
+    for (int i = 0; i < N / 4; ++i) c.w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
   } else if constexpr (N == 2) {
-    c.w[0] = __ldg(reinterpret_cast<const uint16_t*>(row + off));
+    c.w[0] = __ldg(reinterpret_cast<const uint16_t*>(p));
   } else {
-    // 3 or 6 bytes at a multiple of 3: two words (the second may lie past the
-    // row, but within the page: norms follow the codes)
-    const uint32_t* p = reinterpret_cast<const uint32_t*>(row + (off & ~3));
-    const uint32_t a = __ldg(p), b = __ldg(p + 1), sh = (uint32_t)(off & 3) * 8;
+    // 3 or 6 bytes: two words (the second may lie past the row, but within
+    // the page: norms follow the codes)
+    const uint32_t a = __ldg(reinterpret_cast<const uint32_t*>(p));
+    const uint32_t b = __ldg(reinterpret_cast<const uint32_t*>(p) + 1);
     c.w[0] = __funnelshift_r(a, b, sh);
     if constexpr (N > 4) c.w[1] = b >> sh;
   }
   return c;
 }
 
-// Shared address of the table row of field `k` (FB bits each, low first) of
-// the words: (field << 8) | lane address.
+// Aligned start and shift of N bytes at offset `off`.
+template <int N>
+__device__ __forceinline__ int code_start(int off, uint32_t& sh) {
+  constexpr bool odd = N % 4 != 0 && N != 2;
+  sh = odd ? (uint32_t)(off & 3) * 8 : 0;
+  return odd ? off & ~3 : off;
+}
+
+// Table offset of field `k` (FB bits each, low first) of the words, for this
+// lane: (field << 8) | lane offset.
 template <int FB, int NW>
-__device__ __forceinline__ uint32_t field_addr(const uint32_t (&w)[NW], int k, uint32_t lane_addr) {
+__device__ __forceinline__ uint32_t field_at(const uint32_t (&w)[NW], int k, uint32_t lane_off) {
   const int bo = FB * k, wi = bo >> 5, sh = bo & 31;
   if constexpr (FB == 8) {
-    return __byte_perm(w[wi], lane_addr, 0x7604u | (uint32_t)((sh >> 3) << 4));
+    return __byte_perm(w[wi], lane_off, 0x5504u | (uint32_t)((sh >> 3) << 4));
   } else {
     constexpr uint32_t mask = ((1u << FB) - 1u) << 8;
     uint32_t x;
     if (sh + FB > 32) x = __funnelshift_r(w[wi], w[wi + 1 < NW ? wi + 1 : wi], sh) << 8;
     else if (sh >= 8) x = w[wi] >> (sh - 8);
     else x = w[wi] << (8 - sh);
-    return (x & mask) | lane_addr;
+    return (x & mask) | lane_off;
   }
 }
 
-__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
-  return *reinterpret_cast<const uint32_t*>(__cvta_shared_to_generic(addr));
+// One pair of each of two rows (registers a0 and a1, or a2 and a3, of an A
+// fragment): field k of x and of y, or, with quad entries, byte k of x.
+template <int FB, bool Q, int NW>
+__device__ __forceinline__ void look_up2(const unsigned char* table, const uint32_t (&x)[NW],
+                                         const uint32_t (&y)[NW], int k, uint32_t lane_off,
+                                         uint32_t& r0, uint32_t& r1) {
+  if constexpr (Q) {
+    // bytes of even fields lie in x, of odd fields in y (join_nibbles)
+    const uint32_t at = (k & 1) ? field_at<8>(y, k >> 1, lane_off) : field_at<8>(x, k >> 1, lane_off);
+    const uint2 v = *reinterpret_cast<const uint2*>(table + at);
+    r0 = v.x;
+    r1 = v.y;
+  } else {
+    r0 = *reinterpret_cast<const uint32_t*>(table + field_at<FB>(x, k, lane_off));
+    r1 = *reinterpret_cast<const uint32_t*>(table + field_at<FB>(y, k, lane_off));
+  }
+}
+
+// Nibbles of x (low) and y (high) joined into bytes: even ones into x, odd into y.
+template <int NW>
+__device__ __forceinline__ void join_nibbles(uint32_t (&x)[NW], uint32_t (&y)[NW]) {
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    const uint32_t e = (x[i] & 0x0F0F0F0Fu) | ((y[i] << 4) & 0xF0F0F0F0u);
+    y[i] = ((x[i] >> 4) & 0x0F0F0F0Fu) | (y[i] & 0xF0F0F0F0u);
+    x[i] = e;
+  }
+}
+
+__device__ __forceinline__ const uint8_t* page_at(const uint8_t* base, int e, int page_bytes) {
+  const uint8_t* r;
+  asm("mad.wide.s32 %0, %1, %2, %3;" : "=l"(r) : "r"(e), "r"(page_bytes), "l"(base));
+  return r;
 }
 
 // Fields of two tokens' VB-bit codes joined into pairs: even entries in e, odd
@@ -194,21 +240,34 @@ __device__ __forceinline__ void rotate_tile(float (&c)[4], const float* m, const
   }
 }
 
+// One 128-byte half of the table's rows from a codebook.
+template <int BITS, bool Q>
+__device__ __forceinline__ void fill_table(unsigned char* half, const float* cent, int tid,
+                                           int nthreads) {
+  constexpr int N = 1 << (Q ? 4 * BITS : 2 * BITS);
+  constexpr uint32_t M = (1u << BITS) - 1u;
+  for (int i = tid; i < 8 * N; i += nthreads) {
+    const uint32_t e = (uint32_t)i >> 3;
+    const uint32_t x = pack_half2(__ldg(cent + (e & M)), __ldg(cent + ((e >> BITS) & M)));
+    const uint32_t y = Q ? pack_half2(__ldg(cent + ((e >> (2 * BITS)) & M)),
+                                      __ldg(cent + ((e >> (3 * BITS)) & M))) : x;
+    reinterpret_cast<uint4*>(half + e * 256)[i & 7] = make_uint4(x, y, x, y);
+  }
+}
+
 template <int D, int KB, int VB, int NT>
-__global__ void __launch_bounds__(32 * Few<D, NT>::W, 1) attend_few_kernel(FewParams p) {
-  using F = Few<D, NT>;
+__global__ void __launch_bounds__(32 * kW, 3) attend_few_kernel(FewParams p) {
+  using F = Few<D, KB, VB, NT>;
   using Tile = FewTile<D, KB, VB>;
-  constexpr int W = F::W, NQ = F::NQ, NC = D / 16, kThreads = 32 * W;
-  extern __shared__ __align__(128) unsigned char smem_raw[];
+  constexpr int NQ = F::NQ, NC = D / 16, kThreads = 32 * kW, LDA = F::LDA, LDO = F::LDO;
+  constexpr int KROW = D * KB / 8, VROW = D * VB / 8;
+  extern __shared__ __align__(128) unsigned char sm[];
   SegWork sw;
   if (!take_segment(p.rg, sw)) return;
-  // the table at a multiple of 64 KB of shared address space
-  const uint32_t raw = smem_u32(smem_raw);
-  unsigned char* sm = smem_raw + (((raw + 65535u) & ~65535u) - raw);
-  const uint32_t sbase = smem_u32(sm);
   float* mw = reinterpret_cast<float*>(sm + F::OFF_M);
   float* lw = reinterpret_cast<float*>(sm + F::OFF_L);
-  float* U = reinterpret_cast<float*>(sm + F::OFF_U);
+  float* U = reinterpret_cast<float*>(sm + F::OFF_P);
+  uint32_t* A = reinterpret_cast<uint32_t*>(sm + F::OFF_A);
   float* rowl = reinterpret_cast<float*>(sm + F::OFF_R);
   int* flags = reinterpret_cast<int*>(sm + F::OFF_R + 128);   // last CTA, first bad key
 
@@ -232,25 +291,50 @@ __global__ void __launch_bounds__(32 * Few<D, NT>::W, 1) attend_few_kernel(FewPa
   };
   const int kend = p.causal ? (int)max(t_base + min(pos0 + p.pcta, q_len), (int64_t)0) : (int)seq;
 
-  // ---- table, query rows -------------------------------------------------------
-  if (tid == 0) flags[1] = INT_MAX;
-  for (int i = tid; i < (1 << (2 * KB)) * 8; i += kThreads) {
-    const int e = i >> 3;
-    const uint32_t v = pack_half2(__ldg(p.kc + (e & ((1 << KB) - 1))), __ldg(p.kc + (e >> KB)));
-    reinterpret_cast<uint4*>(sm + e * 256)[i & 7] = make_uint4(v, v, v, v);
-  }
-  for (int i = tid; i < (1 << (2 * VB)) * 8; i += kThreads) {
-    const int e = i >> 3;
-    const uint32_t v = pack_half2(__ldg(p.vc + (e & ((1 << VB) - 1))), __ldg(p.vc + (e >> VB)));
-    reinterpret_cast<uint4*>(sm + e * 256 + 128)[i & 7] = make_uint4(v, v, v, v);
-  }
-  // 16-byte piece k of row n, quad t of q' (quad order): its place in the row
-  auto q_piece = [](int n, int t, int k) {
-    const int f = D == 128 ? ((t >> 1) | ((n & 1) << 1)) : (n & 1);
-    return n * (D / 8) + t * (D / 32) + (k ^ f);
+  // ---- the thread's place in every page and the first pages' loads -------------
+  uint32_t ksh, vsh;
+  const int s0 = 16 * warp;                                // first token of the quarter
+  const uint8_t* pk = p.pages + (s0 + gq) * KROW + code_start<Tile::KN>(tq * Tile::KN, ksh);
+  const uint8_t* pv = p.pages + p.off_v + (s0 + 2 * tq) * VROW +
+                      code_start<Tile::VN>(gq * Tile::VN, vsh);
+  const uint8_t* pn = p.pages + p.off_kn + 2 * (s0 + gq);
+  const int pend = min(sw.seg.kt1, (kend + 63) >> 6);      // pages [kt0, pend)
+  const int32_t* bt = p.pm.bt ? p.pm.bt + stream * p.pm.bt_stride : nullptr;
+  const int slot0 = (int)(stream * p.pm.pps);              // contiguous layout
+  const int nblocks = p.pm.bt ? (int)p.pm.nblocks : INT_MAX;
+  bool bad_block = false;
+  auto entry = [&](int pg) -> int {
+    pg = min(pg, pend - 1);
+    return bt ? __ldg(bt + pg) : slot0 + pg;
   };
-  uint32_t* A = reinterpret_cast<uint32_t*>(sm + F::OFF_A);
-  constexpr int LDA = F::LDA;
+  auto load_tile = [&](Tile& x, int e) {
+    const bool ok = (unsigned)e < (unsigned)nblocks;       // e < 0 fails too
+    bad_block = bad_block || !ok;
+    e = ok ? e : 0;
+    const uint8_t* k = page_at(pk, e, p.page_bytes);
+    const uint8_t* v = page_at(pv, e, p.page_bytes);
+    const uint8_t* n = page_at(pn, e, p.page_bytes);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      x.k[i] = load_codes<Tile::KN>(k + 8 * i * KROW, ksh);
+      x.n[i] = (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(n + 16 * i)) |
+               ((uint32_t)__ldg(reinterpret_cast<const uint16_t*>(n + 128 + 16 * i)) << 16);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      x.v[i] = load_codes<Tile::VN>(v + ((i & 1) + 8 * (i >> 1)) * VROW, vsh);
+  };
+  int pg = sw.seg.kt0;
+  const bool any = pg < pend;
+  Tile cur, nxt;
+  int e_next = 0;
+  if (any) {
+    load_tile(cur, entry(pg));
+    e_next = entry(pg + 1);
+  }
+
+  // ---- query rows, table ---------------------------------------------------------
+  if (tid == 0) flags[1] = INT_MAX;
   for (int i = tid; i < 16 * D / 2; i += kThreads) {
     const int n = i / (D / 2), w = i % (D / 2);
     float x = 0.f, y = 0.f;
@@ -262,7 +346,13 @@ __global__ void __launch_bounds__(32 * Few<D, NT>::W, 1) attend_few_kernel(FewPa
     split2(x, y, A[n * LDA + w], A[(16 + n) * LDA + w]);
   }
   __syncthreads();
-  for (int jt = warp; jt < D / 8; jt += W) {
+  // 16-byte piece k of row n, quad t of q' (quad order): its place in the row
+  auto q_piece = [](int n, int t, int k) {
+    const int f = D == 128 ? ((t >> 1) | ((n & 1) << 1)) : (n & 1);
+    return n * (D / 8) + t * (D / 32) + (k ^ f);
+  };
+#pragma unroll 1
+  for (int jt = warp; jt < D / 8; jt += kW) {
     float c[4];
     rotate_tile<D, LDA>(c, p.rot + 8 * jt * D, A, lane);
     // pair (8 jt + 2 tq, + 1): word jt of quad tq
@@ -270,76 +360,60 @@ __global__ void __launch_bounds__(32 * Few<D, NT>::W, 1) attend_few_kernel(FewPa
     qw[4 * q_piece(gq, tq, jt >> 2) + (jt & 3)] = pack_half2(c[0], c[1]);
     if (NQ > 8) qw[4 * q_piece(gq + 8, tq, jt >> 2) + (jt & 3)] = pack_half2(c[2], c[3]);
   }
+  __syncthreads();                                         // the table takes A's place
+  fill_table<KB, F::KQ>(sm, p.kc, tid, kThreads);
+  fill_table<VB, F::VQ>(sm + 128, p.vc, tid, kThreads);
   __syncthreads();
 
-  // ---- key tiles -------------------------------------------------------------------
+  // ---- pages -----------------------------------------------------------------------
   float O[NC][NT][4];
 #pragma unroll
   for (int i = 0; i < NC; ++i)
 #pragma unroll
     for (int n = 0; n < NT; ++n) O[i][n][0] = O[i][n][1] = O[i][n][2] = O[i][n][3] = 0.f;
-  float m[NT][2], bias[NT][2], l[NT][2];
+  // m: what scores are taken relative to; finite from the start, so a row
+  // without keys needs no case of its own
+  float m[NT][2], l[NT][2];
   int lim[NT][2], lim_min = INT_MAX;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      m[n][c] = -INFINITY;
-      bias[n][c] = l[n][c] = 0.f;
+      m[n][c] = kNoMax;
+      l[n][c] = 0.f;
       lim[n][c] = row_lim(8 * n + 2 * tq + c);
       lim_min = min(lim_min, lim[n][c]);
     }
   lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, 1));
   lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, 2));
+  const uint32_t k_lane = F::KQ ? 8 * (lane & 15) : 4 * lane;
+  const uint32_t v_lane = 128 + (F::VQ ? 8 * (lane & 15) : 4 * lane);
+  int bad_key = INT_MAX;
 
-  const uint32_t lane_addr = sbase + 4 * lane;
-  const int tend = min(4 * sw.seg.kt1, (kend + 15) >> 4);
-  auto entry = [&](int t) -> int64_t { return t < tend ? page_entry(p.pm, stream, t >> 2) : 0; };
-  auto load_tile = [&](Tile& x, int64_t e, int t) {
-    if (!entry_ok(p.pm, e)) {
-      atomicOr(p.status, TQ_DEV_BAD_BLOCK);
-      e = 0;
-    }
-    const uint8_t* pg = p.pages + e * (int64_t)p.page_bytes;
-    const int s0 = 16 * (t & 3);                           // first token of the tile in its page
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int tok = s0 + gq + 8 * i;
-      x.k[i] = load_codes<Tile::KN>(pg + tok * (D * KB / 8), tq * Tile::KN);
-      x.n[i] = (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(pg + p.off_kn) + tok) |
-               ((uint32_t)__ldg(reinterpret_cast<const uint16_t*>(pg + p.off_vn) + tok) << 16);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int tok = s0 + 2 * tq + (i & 1) + 8 * (i >> 1);
-      x.v[i] = load_codes<Tile::VN>(pg + p.off_v + tok * (D * VB / 8), gq * Tile::VN);
-    }
-  };
-
-  int t = 4 * sw.seg.kt0 + warp;
-  Tile cur, nxt;
-  if (t < tend) load_tile(cur, entry(t), t);
-  int64_t e_next = entry(t + W);
-  for (; t < tend; t += W) {
-    if (t + W < tend) load_tile(nxt, e_next, t + W);
-    e_next = entry(t + 2 * W);
-    const int key0 = 16 * t + gq;
+  // one page: `cur` is used, `nxt` takes the next page's codes
+  auto step = [&](Tile& cur, Tile& nxt) {
+    load_tile(nxt, e_next);
+    e_next = entry(pg + 2);
+    const int key0 = 64 * pg + s0 + gq;
     float kn[2], vn[2], s[NT][4];
+    // norms: 0 past the end; a token whose norm is not finite counts as 0 (0 x
+    // inf would reach rows that do not see it) and the rows that see it become
+    // NaN at the end
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const __half2 h = *reinterpret_cast<const __half2*>(&cur.n[i]);
+      uint32_t h = cur.n[i];
       const bool in = key0 + 8 * i < kend;
-      kn[i] = in ? __low2float(h) : 0.f;
-      vn[i] = in ? __high2float(h) : 0.f;
-      // 0 x inf would reach rows that do not see the key: a token whose norm is
-      // not finite counts as 0 and the rows that see it become NaN at the end
-      if (!(fabsf(kn[i]) + fabsf(vn[i]) < INFINITY)) {
-        kn[i] = vn[i] = 0.f;
-        atomicMin(&flags[1], key0 + 8 * i);
-      }
+      // exponent 31 in either half carries into its sign bit
+      const bool fin = (((h & 0x7FFF7FFFu) + 0x04000400u) & 0x80008000u) == 0;
+      if (in && !fin) bad_key = min(bad_key, key0 + 8 * i);
+      h = in && fin ? h : 0u;
+      const __half2 h2 = *reinterpret_cast<const __half2*>(&h);
+      kn[i] = __low2float(h2);
+      vn[i] = __high2float(h2);
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    if (F::KQ) join_nibbles(cur.k[0].w, cur.k[1].w);
     // S^T: two chunks of 16 dims share one 16-byte piece of q'
 #pragma unroll
     for (int c2 = 0; c2 < NC / 2; ++c2) {
@@ -351,47 +425,48 @@ __global__ void __launch_bounds__(32 * Few<D, NT>::W, 1) attend_few_kernel(FewPa
       for (int c = 0; c < 2; ++c) {
         uint32_t a[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          a[i] = lds32(field_addr<2 * KB>(cur.k[i & 1].w, 2 * (2 * c2 + c) + (i >> 1), lane_addr));
+        for (int i = 0; i < 2; ++i)
+          look_up2<2 * KB, F::KQ>(sm, cur.k[0].w, cur.k[1].w, 2 * (2 * c2 + c) + i, k_lane,
+                                  a[2 * i], a[2 * i + 1]);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
           mma_f16_16816(s[n], a, c ? qb[n].z : qb[n].x, c ? qb[n].w : qb[n].y);
       }
     }
-    bool up = false;
+    // relative to m
+    float d[NT][4], top = -INFINITY;
+    const bool edge = 64 * pg + s0 + 15 > lim_min;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[n][i] *= kn[i >> 1];
-    if (16 * t + 15 > lim_min) {
+      for (int i = 0; i < 4; ++i) d[n][i] = fmaf(s[n][i], kn[i >> 1], -m[n][i & 1]);
+    if (edge) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (key0 + 8 * (i >> 1) > lim[n][i & 1]) s[n][i] = -INFINITY;
+          if (key0 + 8 * (i >> 1) > lim[n][i & 1]) d[n][i] = -INFINITY;
     }
-    const float room[2] = {vn[0] > 256.f ? 0.f : kRoom, vn[1] > 256.f ? 0.f : kRoom};
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) up = up || s[n][i] > m[n][i & 1] + room[i >> 1];
-    if (__any_sync(0xffffffffu, up)) {
+    for (int n = 0; n < NT; ++n) top = fmaxf(fmaxf(fmaxf(top, d[n][0]), fmaxf(d[n][1], d[n][2])), d[n][3]);
+    if (__any_sync(0xffffffffu, top > (fmaxf(vn[0], vn[1]) > 256.f ? 0.f : kRoom))) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          float x = fmaxf(s[n][c], s[n][2 + c]);
+          // the largest score of the column in this tile
+          float x = fmaxf(edge && key0 > lim[n][c] ? -INFINITY : s[n][c] * kn[0],
+                          edge && key0 + 8 > lim[n][c] ? -INFINITY : s[n][2 + c] * kn[1]);
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          const float mn = fmaxf(m[n][c], x);
-          const float b = mn == -INFINITY ? 0.f : mn;
-          const float f = fast_exp2(m[n][c] - b);          // 0 before the first key
+          const float mn = fmaxf(m[n][c], x), f = fast_exp2(m[n][c] - mn);
           l[n][c] *= f;
 #pragma unroll
           for (int i = 0; i < NC; ++i) { O[i][n][c] *= f; O[i][n][2 + c] *= f; }
           m[n][c] = mn;
-          bias[n][c] = b;
+          d[n][c] = edge && key0 > lim[n][c] ? -INFINITY : fmaf(s[n][c], kn[0], -mn);
+          d[n][2 + c] = edge && key0 + 8 > lim[n][c] ? -INFINITY : fmaf(s[n][2 + c], kn[1], -mn);
         }
     }
     uint32_t pb[NT][2];
@@ -399,8 +474,7 @@ __global__ void __launch_bounds__(32 * Few<D, NT>::W, 1) attend_few_kernel(FewPa
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float p0 = fast_exp2(s[n][2 * i] - bias[n][0]);
-        const float p1 = fast_exp2(s[n][2 * i + 1] - bias[n][1]);
+        const float p0 = fast_exp2(d[n][2 * i]), p1 = fast_exp2(d[n][2 * i + 1]);
         l[n][0] += p0;
         l[n][1] += p1;
         pb[n][i] = movmatrix_trans(pack_half2(p0 * vn[i], p1 * vn[i]));
@@ -408,19 +482,29 @@ __global__ void __launch_bounds__(32 * Few<D, NT>::W, 1) attend_few_kernel(FewPa
     }
     uint32_t ve[2][(Tile::VN + 3) / 4], vo[2][(Tile::VN + 3) / 4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) join_tokens<VB>(cur.v[2 * i], cur.v[2 * i + 1], ve[i], vo[i]);
+    for (int i = 0; i < 2; ++i) {
+      join_tokens<VB>(cur.v[2 * i], cur.v[2 * i + 1], ve[i], vo[i]);
+      if (F::VQ) join_nibbles(ve[i], vo[i]);
+    }
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       uint32_t a[4];
-      a[0] = lds32(field_addr<2 * VB>(ve[0], c, lane_addr) + 128);
-      a[1] = lds32(field_addr<2 * VB>(vo[0], c, lane_addr) + 128);
-      a[2] = lds32(field_addr<2 * VB>(ve[1], c, lane_addr) + 128);
-      a[3] = lds32(field_addr<2 * VB>(vo[1], c, lane_addr) + 128);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        look_up2<2 * VB, F::VQ>(sm, ve[i], vo[i], c, v_lane, a[2 * i], a[2 * i + 1]);
 #pragma unroll
       for (int n = 0; n < NT; ++n) mma_f16_16816(O[c][n], a, pb[n][0], pb[n][1]);
     }
-    cur = nxt;
+  };
+#pragma unroll 1
+  while (pg < pend) {                                      // by twos: no copies between tiles
+    step(cur, nxt);
+    if (++pg >= pend) break;
+    step(nxt, cur);
+    ++pg;
   }
+  if (bad_block) atomicOr(p.status, TQ_DEV_BAD_BLOCK);
+  if (bad_key != INT_MAX) atomicMin(&flags[1], bad_key);
 
   // ---- the warps' partials: common max, sum in warp order ---------------------------
 #pragma unroll
@@ -436,56 +520,43 @@ __global__ void __launch_bounds__(32 * Few<D, NT>::W, 1) attend_few_kernel(FewPa
         lw[warp * NQ + 8 * n + 2 * tq + c] = x;
       }
     }
-  __syncthreads();
+  __syncthreads();                                         // and the table is dead
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      float M = -INFINITY;
-      for (int w = 0; w < W; ++w) M = fmaxf(M, mw[w * NQ + 8 * n + 2 * tq + c]);
-      const float f = M == -INFINITY ? 0.f : fast_exp2(m[n][c] - M);
+      const int col = 8 * n + 2 * tq + c;
+      float M = mw[col];
 #pragma unroll
-      for (int i = 0; i < NC; ++i) { O[i][n][c] *= f; O[i][n][2 + c] *= f; }
+      for (int w = 1; w < kW; ++w) M = fmaxf(M, mw[w * NQ + col]);
+      const float f = fast_exp2(m[n][c] - M);
+      float* mine = U + (warp * NQ + col) * LDO + gq;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        mine[16 * i] = O[i][n][c] * f;
+        mine[16 * i + 8] = O[i][n][2 + c] * f;
+      }
     }
-  float* buf = reinterpret_cast<float*>(sm);
-  constexpr int B = F::kBufs, LDO = F::LDO;
-  auto at = [&](int n, int i, int c) {                     // O[i][n][c] of this thread
-    return (8 * n + 2 * tq + (c & 1)) * LDO + 16 * i + gq + 8 * (c >> 1);
-  };
-#pragma unroll
-  for (int round = (W - 1) / B; round >= 0; --round) {
-    if (warp / B == round) {
-      float* mine = buf + (warp % B) * NQ * LDO;
-      const bool add = round * B + B + warp % B < W;       // a later round left its sum here
-#pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int i = 0; i < NC; ++i)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float x = O[i][n][c];
-            if (add) x += mine[at(n, i, c)];
-            mine[at(n, i, c)] = x;
-          }
-    }
-    __syncthreads();
-  }
-  for (int i = tid; i < NQ * D; i += kThreads) {
-    const int n = i / D, d = i % D;
-    float x = 0.f;
-#pragma unroll
-    for (int w = 0; w < B; ++w) x += buf[(w * NQ + n) * LDO + d];
-    U[n * LDO + d] = x;
-  }
   if (tid < NQ) {
-    float M = -INFINITY, x = 0.f;
-    for (int w = 0; w < W; ++w) M = fmaxf(M, mw[w * NQ + tid]);
-    for (int w = 0; w < W; ++w)
-      x += M == -INFINITY ? 0.f : lw[w * NQ + tid] * fast_exp2(mw[w * NQ + tid] - M);
-    const int lm = row_lim(tid);
-    if (flags[1] <= lm) x = NAN;
+    float M = mw[tid], x = 0.f;
+#pragma unroll
+    for (int w = 1; w < kW; ++w) M = fmaxf(M, mw[w * NQ + tid]);
+#pragma unroll
+    for (int w = 0; w < kW; ++w) x += lw[w * NQ + tid] * fast_exp2(mw[w * NQ + tid] - M);
+    if (flags[1] <= row_lim(tid)) x = NAN;
     rowl[tid] = x;
     rowl[16 + tid] = M;
+  }
+  __syncthreads();
+  for (int i = tid; i < NQ * D / 4; i += kThreads) {
+    const int n = i / (D / 4), at = n * LDO + 4 * (i % (D / 4));
+    float4 x = *reinterpret_cast<const float4*>(U + at);
+#pragma unroll
+    for (int w = 1; w < kW; ++w) {
+      const float4 y = *reinterpret_cast<const float4*>(U + w * NQ * LDO + at);
+      x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+    }
+    *reinterpret_cast<float4*>(U + at) = x;
   }
   __syncthreads();
 
@@ -493,21 +564,18 @@ __global__ void __launch_bounds__(32 * Few<D, NT>::W, 1) attend_few_kernel(FewPa
   if (sw.seg.slot >= 0) {
     const RaggedPlan& pl = p.rg.plan;
     for (int i = tid; i < NQ * D / 4; i += kThreads) {
-      const int n = i / (D / 4), d = 4 * (i % (D / 4));
+      const int n = i / (D / 4), at = 4 * (i % (D / 4));
       if (row_valid(n))
-        *reinterpret_cast<float4*>(pl.part + part_row(pl, sw.seg.slot, sw.group, n) * D + d) =
-            *reinterpret_cast<const float4*>(U + n * LDO + d);
+        *reinterpret_cast<float4*>(pl.part + part_row(pl, sw.seg.slot, sw.group, n) * D + at) =
+            *reinterpret_cast<const float4*>(U + n * LDO + at);
     }
     if (tid < NQ) pl.ml[part_row(pl, sw.seg.slot, sw.group, tid)] = make_float2(rowl[16 + tid], rowl[tid]);
     if (!last_of_tile(pl, sw, &flags[0])) return;
-    // row n's parts over the lanes of a warp for {m, l}, then its dims over them
-    for (int n = warp; n < NQ; n += W) {
+    for (int n = warp; n < NQ; n += kW) {
       if (!row_valid(n)) continue;
-      float M = -INFINITY;
-      for (int s = lane; s < sw.seg.parts; s += 32) {
-        const float2 ml = __ldcg(pl.ml + part_row(pl, sw.seg.first + s, sw.group, n));
-        M = fmaxf(M, ml.x);
-      }
+      float M = kNoMax;
+      for (int s = lane; s < sw.seg.parts; s += 32)
+        M = fmaxf(M, __ldcg(pl.ml + part_row(pl, sw.seg.first + s, sw.group, n)).x);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
       float sum = 0.f, acc[D / 32];
@@ -517,7 +585,7 @@ __global__ void __launch_bounds__(32 * Few<D, NT>::W, 1) attend_few_kernel(FewPa
       for (int s = 0; s < sw.seg.parts; ++s) {
         const int64_t pr = part_row(pl, sw.seg.first + s, sw.group, n);
         const float2 ml = __ldcg(pl.ml + pr);
-        const float w = M == -INFINITY ? 0.f : fast_exp2(ml.x - M);
+        const float w = fast_exp2(ml.x - M);
         sum = fmaf(w, ml.y, sum);
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(w, __ldcg(pl.part + pr * D + 32 * i + lane), acc[i]);
@@ -550,7 +618,8 @@ __global__ void __launch_bounds__(32 * Few<D, NT>::W, 1) attend_few_kernel(FewPa
     o_ok[r] = n < NQ && row_valid(n);
     o_at[r] = o_ok[r] ? row_at(n, p.os) : 0;
   }
-  for (int jt = warp; jt < D / 8; jt += W) {
+#pragma unroll 1
+  for (int jt = warp; jt < D / 8; jt += kW) {
     float c[4];
     rotate_tile<D, LDA>(c, p.rot_t + 8 * jt * D, A, lane);
 #pragma unroll
@@ -566,8 +635,9 @@ __global__ void __launch_bounds__(32 * Few<D, NT>::W, 1) attend_few_kernel(FewPa
 using FewFn = void (*)(FewParams);
 
 template <int D, int NT>
-FewFn few_fn(int kb, int vb) {
-#define TQ_FEW(K, V) if (kb == K && vb == V) return attend_few_kernel<D, K, V, NT>;
+FewFn few_fn(int kb, int vb, int& bytes) {
+#define TQ_FEW(K, V) \
+  if (kb == K && vb == V) { bytes = Few<D, K, V, NT>::BYTES; return attend_few_kernel<D, K, V, NT>; }
   TQ_FEW(4, 2) TQ_FEW(4, 3) TQ_FEW(4, 4) TQ_FEW(3, 2) TQ_FEW(3, 3) TQ_FEW(3, 4)
   TQ_FEW(2, 2) TQ_FEW(2, 3) TQ_FEW(2, 4)
 #undef TQ_FEW
@@ -577,8 +647,9 @@ FewFn few_fn(int kb, int vb) {
 }  // namespace
 
 bool attend_few_applies(const tq_geom* G) {
-  if (G->head_dim == 128) return few_fn<128, 1>(G->key_bits, G->value_bits) != nullptr;
-  if (G->head_dim == 64) return few_fn<64, 1>(G->key_bits, G->value_bits) != nullptr;
+  int bytes;
+  if (G->head_dim == 128) return few_fn<128, 1>(G->key_bits, G->value_bits, bytes) != nullptr;
+  if (G->head_dim == 64) return few_fn<64, 1>(G->key_bits, G->value_bits, bytes) != nullptr;
   return false;
 }
 
@@ -610,12 +681,10 @@ int launch_attend_few(const tq_geom* G, const tq_tables* t, const tq_cache* c,
   p.status = status;
   p.rg = rg;
   FewFn fn;
-  int bytes, threads;
+  int bytes = 0;
   auto pick = [&](auto d, auto nt) {
     constexpr int D = decltype(d)::value, NT = decltype(nt)::value;
-    fn = few_fn<D, NT>(G->key_bits, G->value_bits);
-    bytes = Few<D, NT>::BYTES;
-    threads = 32 * Few<D, NT>::W;
+    fn = few_fn<D, NT>(G->key_bits, G->value_bits, bytes);
   };
   using I1 = std::integral_constant<int, 1>;
   using I2 = std::integral_constant<int, 2>;
@@ -624,9 +693,8 @@ int launch_attend_few(const tq_geom* G, const tq_tables* t, const tq_cache* c,
   } else {
     if (rows == 8) pick(std::integral_constant<int, 64>(), I1()); else pick(std::integral_constant<int, 64>(), I2());
   }
-  bytes += 65536;                         // slack to reach a 64 KB boundary
   if (set_smem_attr((const void*)fn, bytes) != TQ_OK) return TQ_ERR_CUDA;
-  fn<<<(unsigned)grid, threads, bytes, st>>>(p);
+  fn<<<(unsigned)grid, 32 * kW, bytes, st>>>(p);
   return check_launch("tq_attend_ragged/few");
 }
 

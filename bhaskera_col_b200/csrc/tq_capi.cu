@@ -731,6 +731,11 @@ static int check_attend(const tq_geom* g, const tq_cache* c, const tq_attend_arg
     set_error("%s: at most 2^30 rows, 2^24 requests and 1024 query heads", fn);
     return TQ_ERR_INVALID;
   }
+  if ((c->block_table ? c->num_blocks : c->streams * c->pages_per_stream) > INT32_MAX ||
+      c->pages_per_stream > INT32_MAX / TQ_PAGE_TOKENS) {
+    set_error("%s: more pages than 32 bits count", fn);
+    return TQ_ERR_INVALID;
+  }
   return TQ_OK;
 }
 
