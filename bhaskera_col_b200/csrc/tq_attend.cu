@@ -203,7 +203,7 @@ struct ListShape {
 };
 
 struct AttendShape {
-  int engine;                              // of the wide list
+  bool tc;                                 // the wide list runs on tcgen05
   int64_t Hkv;
   ListShape few, wide;
   size_t bytes;
@@ -217,9 +217,9 @@ AttendShape attend_shape(const tq_geom* G, const tq_cache* c, const tq_attend_ar
   const int64_t R = a->batch.requests, N = a->q->shape[2], most = INT64_MAX;
   s.Hkv = c->streams / R;
   const int64_t g = a->q->shape[1] / s.Hkv;
-  s.engine = 1;
-  const bool can = attend_few_applies(G) && (a->engine == 0 || a->engine == 4);
-  const int64_t few_q = a->engine == 4 ? most : tmax<int64_t>(kFewRows / g, 1);
+  s.tc = prefill_tc_applies(G) && a->engine != 1;
+  const bool can = attend_few_applies(G) && (a->engine == 0 || a->engine == 3);
+  const int64_t few_q = a->engine == 3 ? most : tmax<int64_t>(kFewRows / g, 1);
   size_t off = 256;                        // the first 64 bytes: the decode's status word
   auto take = [&](size_t bytes) {
     const size_t at = off;
@@ -255,10 +255,12 @@ AttendShape attend_shape(const tq_geom* G, const tq_cache* c, const tq_attend_ar
     ListShape& l = s.wide;
     l.q_lo = can ? few_q : 0;
     l.q_hi = most;
+    // both kernels take 8, 4, 2 or 1 heads; the tcgen05 one two tiles of 128
+    // rows that share their keys
     l.hc = g % 8 == 0 ? 8 : g % 4 == 0 ? 4 : g % 2 == 0 ? 2 : 1;
-    l.rows = 128;
+    l.rows = s.tc ? 256 : 128;
     l.pcta = l.rows / l.hc;
-    l.keys = kPageTokens;
+    l.keys = s.tc ? 2 * kPageTokens : kPageTokens;
     l.wanted = (int64_t)kWaves * device_sm_count();
     l.off_nseg = 68;
     finish(l);
@@ -316,6 +318,9 @@ int launch_attend_ragged(const tq_geom* G, const tq_tables* t, const tq_cache* c
                                      s.few.max_seg * s.few.G, status, st);
     if (rc != TQ_OK) return rc;
   }
+  if (s.wide.used && s.tc)
+    return launch_attend_tc(G, t, c, a, rg[lists - 1], s.Hkv, s.wide.max_seg * s.wide.G, status,
+                            st);
   if (s.wide.used)
     return launch_attend_mma(G, t, c, a, rg[lists - 1], s.Hkv, s.wide.hc,
                              s.wide.max_seg * s.wide.G, status, st);

@@ -713,16 +713,16 @@ static int check_attend(const tq_geom* g, const tq_cache* c, const tq_attend_arg
     return TQ_ERR_INVALID;
   }
   if ((rc = check_flat(a->q, "q", Hq, g, fn))) return rc;
-  if (a->engine < 0 || a->engine > 4) {
-    set_error("%s: engine must be 0 (fastest), 1 (mma.sync), 2 or 3 (tcgen05) or 4 (few rows), "
-              "got %d", fn, a->engine);
+  if (a->engine < 0 || a->engine > 3) {
+    set_error("%s: engine must be 0 (fastest), 1 (mma.sync), 2 (tcgen05) or 3 (few rows), got %d",
+              fn, a->engine);
     return TQ_ERR_INVALID;
   }
   const bool tc = prefill_tc_applies(g);
-  if (a->engine == 4 ? !attend_few_applies(g)
-      : a->engine >= 2 ? !tc
-                     : !prefill_supported(g->head_dim, g->key_bits, g->value_bits) &&
-                           !(a->engine == 0 && tc)) {
+  const bool mma = prefill_supported(g->head_dim, g->key_bits, g->value_bits);
+  if (a->engine == 0 ? !mma && !tc
+      : a->engine == 1 ? !mma
+      : a->engine == 2 ? !tc : !attend_few_applies(g)) {
     set_error("%s: no kernel for head_dim %d, key_bits %d, value_bits %d (engine %d)", fn,
               g->head_dim, g->key_bits, g->value_bits, a->engine);
     return TQ_ERR_INVALID;

@@ -80,6 +80,9 @@ bool attend_few_applies(const tq_geom* g);
 int launch_attend_few(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                       const tq_attend_args* a, const RaggedAttend& rg, int64_t Hkv, int hc,
                       int pcta, int rows, int64_t grid, uint32_t* status, cudaStream_t st);
+int launch_attend_tc(const tq_geom* g, const tq_tables* t, const tq_cache* c,
+                     const tq_attend_args* a, const RaggedAttend& rg, int64_t Hkv, int64_t grid,
+                     uint32_t* status, cudaStream_t st);
 int launch_attend_mma(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                       const tq_attend_args* a, const RaggedAttend& rg, int64_t Hkv, int hc,
                       int64_t grid, uint32_t* status, cudaStream_t st);

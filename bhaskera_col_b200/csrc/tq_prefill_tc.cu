@@ -704,12 +704,15 @@ __global__ void __launch_bounds__(128) window_rotate_kernel(WinParams p) {
     p.out[which][(s * p.W + w0 + r) * kD + tid] = __float2half_rn(acc[r]);
 }
 
-int launch_prefill_tc(const tq_geom* G, const tq_tables* t, const tq_cache* c,
-                      const tq_prefill_args* a, uint32_t* status, cudaStream_t st) {
-  if (!prefill_tc_applies(G)) return 1;
-  TcFn fn = tc_fn(G->key_bits, G->value_bits);
+namespace {
+
+// What a launch of either kernel takes from the geometry, tables and views:
+// hc heads x 128 / hc positions per 128-row tile, no window, no batch rows.
+TcPrefillParams tc_params(const tq_geom* G, const tq_tables* t, const tq_cache* c,
+                          const tq_tensor4* q, const tq_tensor4* out, int64_t Hkv, float scale,
+                          int causal, uint32_t* status) {
+  TcPrefillParams p = {};
   const PageGeom g = make_geom(G->head_dim, G->key_bits, G->value_bits, G->qjl);
-  TcPrefillParams p;
   p.pages = c->pages;
   p.pm = page_map(c);
   p.page_bytes = g.page_bytes;
@@ -720,21 +723,41 @@ int launch_prefill_tc(const tq_geom* G, const tq_tables* t, const tq_cache* c,
   p.rot = t->rot;
   p.kc = t->k_centroids;
   p.vc = t->v_centroids;
-  p.q = a->q->data; p.q_dtype = a->q->dtype; p.q_vec = vec_ok(a->q);
-  p.out = a->out->data; p.o_dtype = a->out->dtype; p.o_vec = vec_ok(a->out);
-  for (int i = 0; i < 4; ++i) { p.qs[i] = a->q->stride[i]; p.os[i] = a->out->stride[i]; }
-  const int64_t B = a->q->shape[0], Hq = a->q->shape[1];
-  p.Hkv = c->streams / B;
-  p.g = Hq / p.Hkv;
+  p.q = q->data; p.q_dtype = q->dtype; p.q_vec = vec_ok(q);
+  p.out = out->data; p.o_dtype = out->dtype; p.o_vec = vec_ok(out);
+  for (int i = 0; i < 4; ++i) { p.qs[i] = q->stride[i]; p.os[i] = out->stride[i]; }
+  p.Hkv = Hkv;
+  p.g = q->shape[1] / Hkv;
   p.hc = p.g % 8 == 0 ? 8 : p.g % 4 == 0 ? 4 : p.g % 2 == 0 ? 2 : 1;
-  const int P = kRows / p.hc;
-  p.pshift = 0;
-  while ((1 << p.pshift) < P) ++p.pshift;
+  p.pcta = kRows / p.hc;
+  while ((1 << p.pshift) < p.pcta) ++p.pshift;
+  p.qscale = scale * kLog2e;
+  p.causal = causal;
+  p.status = status;
+  return p;
+}
+
+}  // namespace
+
+// Ragged batch on the 256-row kernel; `grid` bounds the work list.
+int launch_attend_tc(const tq_geom* G, const tq_tables* t, const tq_cache* c,
+                     const tq_attend_args* a, const RaggedAttend& rg, int64_t Hkv, int64_t grid,
+                     uint32_t* status, cudaStream_t st) {
+  TcPrefillParams p = tc_params(G, t, c, a->q, a->out, Hkv, a->scale, a->causal, status);
+  p.rg = rg;
+  return launch_attend_tc2(p, G->key_bits, G->value_bits, grid, st);
+}
+
+int launch_prefill_tc(const tq_geom* G, const tq_tables* t, const tq_cache* c,
+                      const tq_prefill_args* a, uint32_t* status, cudaStream_t st) {
+  if (!prefill_tc_applies(G)) return 1;
+  TcFn fn = tc_fn(G->key_bits, G->value_bits);
+  const int64_t B = a->q->shape[0], Hq = a->q->shape[1];
+  TcPrefillParams p = tc_params(G, t, c, a->q, a->out, c->streams / B, a->scale, a->causal, status);
+  const int P = p.pcta;
   p.Tq = a->q->shape[2];
   p.n_tokens = a->n_tokens;
   p.nqb = (int)((p.Tq + P - 1) / P);
-  p.qscale = a->scale * kLog2e;
-  p.causal = a->causal;
   p.kv_start = a->kv_start;
   p.W = a->window_k ? a->window_k->shape[2] : 0;
   p.wk = p.wv = nullptr;
@@ -768,9 +791,6 @@ int launch_prefill_tc(const tq_geom* G, const tq_tables* t, const tq_cache* c,
   }
   p.rk = rk;
   p.rv = rv;
-  p.status = status;
-  p.pcta = P;
-  p.tile_head_step = p.tile_pos_step = 0;
   if (p.Tq == 0) return TQ_OK;
   // chunks longer than one 128-row block: the 256-row kernel (engine 0 or 3)
   if (a->engine == 3 || (a->engine == 0 && p.Tq > P)) {

@@ -13,7 +13,11 @@
 
 #include "tq_common.cuh"
 #include "tq_internal.h"
+#include "tq_ragged.cuh"
 #include "tq_tc.cuh"
+
+#include <limits.h>
+#include <math.h>
 
 namespace tq {
 namespace pftc {
@@ -50,7 +54,58 @@ struct TcPrefillParams {
   const __half* wv;
   int64_t W;
   uint32_t* status;
+  RaggedAttend rg;              // ragged batch (RG kernels): Tq, n_tokens come per request
 };
+
+// What one CTA works on: a block of query positions of one head group, over
+// key tiles [tile0, tile0 + ntiles).
+struct Job {
+  int qb, chunk, tile0, ntiles;
+  int64_t stream, kvh, b;
+  int64_t qrow, orow;           // element offsets of the batch row's first query row
+  int64_t t_base, qpos_max, kend;
+  SegWork sw;                   // RG: the segment
+};
+
+// The whole batch row of blockIdx.y, or (RG) one segment of the ragged work
+// list, whose lengths replace p's.  false: nothing for this CTA.
+template <bool RG>
+__device__ __forceinline__ bool take_job(TcPrefillParams& p, int pcta, Job& j) {
+  const int nchunk = (int)(p.g / p.hc);
+  int64_t group = blockIdx.y;
+  j.qb = p.nqb - 1 - (int)blockIdx.x;                  // long rows first
+  if constexpr (RG) {
+    if (!take_segment(p.rg, j.sw)) return false;
+    j.qb = j.sw.seg.tile;
+    group = j.sw.seg.req * (p.Hkv * nchunk) + j.sw.group;
+    p.Tq = j.sw.rq.q_len;
+    p.n_tokens = j.sw.rq.seq;
+  }
+  j.stream = group / nchunk;
+  j.chunk = (int)(group % nchunk);
+  j.b = j.stream / p.Hkv;
+  j.kvh = j.stream % p.Hkv;
+  j.qrow = RG ? j.sw.rq.q0 * p.qs[2] : j.b * p.qs[0];
+  j.orow = RG ? j.sw.rq.q0 * p.os[2] : j.b * p.os[0];
+  j.t_base = p.n_tokens - p.Tq;
+  j.qpos_max = j.t_base + tmin<int64_t>((int64_t)(j.qb + 1) * pcta, p.Tq) - 1;
+  j.kend = p.causal ? j.qpos_max + 1 : p.n_tokens;
+  j.tile0 = RG ? j.sw.seg.kt0 : 0;
+  j.ntiles = RG ? j.sw.seg.kt1 - j.tile0 : (int)((j.kend + kKeys - 1) / kKeys);
+  return true;
+}
+
+// Rows of a tile without any key (RG): zeros, one warp per row.
+template <class RowOut>
+__device__ __forceinline__ void zero_rows(const TcPrefillParams& p, int rows, int nwarps,
+                                          RowOut row_out) {
+  const int lane = threadIdx.x & 31;
+  for (int row = threadIdx.x >> 5; row < rows; row += nwarps) {
+    const int64_t at = row_out(row);
+    if (at < 0) continue;
+    for (int d = lane; d < kD; d += 32) store_elem(p.out, p.o_dtype, at + d * p.os[3], 0.f);
+  }
+}
 
 // D (+)= A B with A and B in shared memory (kind::f16: fp16 or bf16 by idesc).
 __device__ __forceinline__ void umma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
@@ -289,6 +344,8 @@ struct TcParamsView {
   int64_t kend;                 // keys this CTA needs
   int64_t kpacked;              // keys [0, kpacked) are in pages, the rest in the window
   int64_t W;                    // window tokens (rows of the rotated window buffers)
+  int tile0;                    // key tile of the CTA's tile 0
+  int* bad_key;                 // RG: first key whose norm is not finite (shared memory)
 };
 
 // One operand's codes and norms that a decoder thread needs for one tile:
@@ -300,10 +357,13 @@ struct HalfRegs {
   uint32_t n[NR];               // fp16 norm bits
 };
 
-template <int NB, int NR>
-__device__ __forceinline__ void load_half(HalfRegs<NB, NR>& t, const TcParamsView& pv, int j,
+// RG: a norm that is not finite counts as 0 (0 x inf would reach the rows of
+// the tile that do not see the key) and its key is noted.
+template <int NB, int NR, bool RG = false>
+__device__ __forceinline__ void load_half(HalfRegs<NB, NR>& t, const TcParamsView& pv, int jj,
                                           int off_codes, int off_norm) {
   constexpr int RPP = NR / 2, STEP = 64 / RPP;
+  const int j = RG ? jj + pv.tile0 : jj;
   const uint8_t* pgs[2];
   const int64_t kpend = tmin<int64_t>(pv.kend, pv.kpacked);   // needed keys held in pages
 #pragma unroll
@@ -324,6 +384,10 @@ __device__ __forceinline__ void load_half(HalfRegs<NB, NR>& t, const TcParamsVie
       const uint8_t* pg = pgs[pgi];
       load_stream<NB>(t.c[r], pg + off_codes + key_in_page * (16 * NB) + pv.part * (4 * NB));
       t.n[r] = __ldg(reinterpret_cast<const unsigned short*>(pg + off_norm) + key_in_page);
+      if (RG && (t.n[r] & 0x7C00u) == 0x7C00u) {
+        t.n[r] = 0u;
+        atomicMin(pv.bad_key, (int)key);
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < NB; ++i) t.c[r].w[i] = 0u;
@@ -380,5 +444,8 @@ __device__ __forceinline__ bool tile_has_window(const TcParamsView& pv, int j) {
 // variant exists for (kb, vb), or an error.
 int launch_prefill_tc2(const pftc::TcPrefillParams& base, int kb, int vb, int64_t B, int64_t Hq,
                        cudaStream_t st);
+// The same kernel on a ragged work list of `grid` CTAs at most.
+int launch_attend_tc2(const pftc::TcPrefillParams& base, int kb, int vb, int64_t grid,
+                      cudaStream_t st);
 
 }  // namespace tq

@@ -29,6 +29,9 @@
 // the first V^ tile; after the last MMA of the loop R_V hi / lo replace q'_A
 // / q'_B, O^_A hi / lo the K stages and O^_B hi / lo the V stages.
 //
+// RG: a ragged batch (tq_attend_ragged); a CTA takes one segment of the work
+// list and leaves partial rows where the tile has several.
+//
 // Every wait is bounded; on expiry the kernel sets TQ_DEV_WAIT_TIMEOUT in the
 // status word, the other roles see the abort flag, no MMA is left in flight
 // and tensor memory is released.
@@ -55,6 +58,7 @@ constexpr uint32_t OFF_LUT = 6 * kStage;
 constexpr uint32_t kLutMax = 32768;
 constexpr uint32_t OFF_BAR = OFF_LUT + kLutMax;
 constexpr uint32_t SMEM_BYTES = OFF_BAR + 256 + 1024;   // + alignment slack
+static_assert(SMEM_BYTES <= 227 * 1024, "shared memory");
 
 enum Bar {
   B_ROT = 0, B_QP = 1, B_KFULL = 3, B_KEMPTY = 5, B_VFULL = 7, B_VEMPTY = 9, B_SFULL = 11,
@@ -77,7 +81,7 @@ __device__ __forceinline__ RowId row_id(const TcPrefillParams& p, int qb, int X,
   return r;
 }
 
-template <int KB, int VB>
+template <int KB, int VB, bool RG>
 __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParams p) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -86,17 +90,24 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + OFF_BAR);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + B_COUNT);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + B_COUNT + 1);
+  int* flags = reinterpret_cast<int*>(bars + B_COUNT + 2);   // RG: last CTA, first bad key
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int qb = p.nqb - 1 - (int)blockIdx.x;          // long rows first
-  const int nchunk = (int)(p.g / p.hc);
-  const int64_t stream = (int64_t)blockIdx.y / nchunk;
-  const int chunk = (int)((int64_t)blockIdx.y % nchunk);
-  const int64_t b = stream / p.Hkv, kvh = stream % p.Hkv;
-  const int64_t t_base = p.n_tokens - p.Tq;
-  const int64_t qpos_max = t_base + tmin<int64_t>((int64_t)(qb + 1) * p.pcta, p.Tq) - 1;
-  const int64_t kend = p.causal ? qpos_max + 1 : p.n_tokens;
-  const int ntiles = (int)((kend + kKeys - 1) / kKeys);
+  Job jb;
+  if (!take_job<RG>(p, p.pcta, jb)) return;
+  const int qb = jb.qb, chunk = jb.chunk, ntiles = jb.ntiles;
+  const int64_t stream = jb.stream, b = jb.b, kvh = jb.kvh, t_base = jb.t_base;
+  const int64_t qpos_max = jb.qpos_max, kend = jb.kend;
+  // output offset of the CTA's row (tile A's 128 rows, then tile B's), or -1
+  auto row_out = [&](int row) -> int64_t {
+    const RowId id = row_id(p, qb, row >> 7, row & 127);
+    if (id.pos >= p.Tq) return -1;
+    return jb.orow + (kvh * p.g + (int64_t)chunk * p.hc + id.head) * p.os[1] + id.pos * p.os[2];
+  };
+  if (RG && ntiles == 0) {
+    zero_rows(p, 256, kWarps, row_out);
+    return;
+  }
 
   if (tid == 0) {
     mbar_init(&bars[B_ROT], 1);
@@ -115,6 +126,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
     mbar_init(&bars[B_OUT], 1);
     mbar_init(&bars[B_MMA], 1);
     *abort_flag = 0;
+    if (RG) flags[1] = INT_MAX;
     fence_mbar_init();
   }
   if (warp == 0) {
@@ -137,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
       const int64_t h = kvh * p.g + (int64_t)chunk * p.hc + id.head;
       raw4[m] = make_uint4(0, 0, 0, 0);
       if (id.pos < p.Tq) {
-        const int64_t base = b * p.qs[0] + h * p.qs[1] + (int64_t)id.pos * p.qs[2];
+        const int64_t base = jb.qrow + h * p.qs[1] + (int64_t)id.pos * p.qs[2];
         if (p.q_vec) {
           raw4[m] = __ldg(reinterpret_cast<const uint4*>(
                               reinterpret_cast<const uint16_t*>(p.q) + base) + c);
@@ -324,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
                                                  abort_flag, p.status));
       if (!ok) break;
       tc::tc_fence_after();
-      const int64_t k0 = (int64_t)j * kKeys;
+      const int64_t k0 = (int64_t)(j + jb.tile0) * kKeys;
       const bool need_mask = k0 + kKeys - 1 > lim || k0 < kst;
       // pass 1: row max (four independent 3-input chains)
       float mx;
@@ -409,7 +421,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
       ok = __all_sync(0xffffffffu, wait_or_abort(&bars[B_ODONE], 0u, abort_flag, p.status));
     if (ok) {
       tc::tc_fence_after();
-      const float il = l > 0.f ? 1.f / l : 0.f;
+      // RG: a row that sees a key of a norm that is not finite
+      if (RG && (l != l || flags[1] <= lim)) l = NAN;
+      const float il = (RG ? l != 0.f : l > 0.f) ? 1.f / l : 0.f;
       const uint32_t ohi = sbase + (X == 0 ? OFF_K : OFF_V), olo = ohi + kStage;
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
@@ -440,13 +454,23 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
     if (ok) {
       tc::tc_fence_after();
       const int64_t h = kvh * p.g + (int64_t)chunk * p.hc + id.head;
-      const int64_t base = b * p.os[0] + h * p.os[1] + (int64_t)id.pos * p.os[2];
+      const int64_t base = jb.orow + h * p.os[1] + (int64_t)id.pos * p.os[2];
+      const bool split = RG && jb.sw.seg.slot >= 0;
+      const int64_t pr = split ? part_row(p.rg.plan, jb.sw.seg.slot, jb.sw.group, 128 * X + rr) : 0;
+      if (split && valid) p.rg.plan.ml[pr] = make_float2(m, l);
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t x[32];
         tc::tmem_ld_x32(scol + 32 * c, x);
         tmem_ld_wait(x);
         if (!valid) continue;
+        if (split) {
+          uint4* dst = reinterpret_cast<uint4*>(p.rg.plan.part + pr * kD) + 8 * c;
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            dst[q] = make_uint4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
+          continue;
+        }
         if (p.o_vec) {
           uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.out) + base) + 4 * c;
 #pragma unroll
@@ -495,8 +519,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
       pv.part = part;
     }
     pv.kend = kend;
-    pv.W = p.W;
-    pv.kpacked = p.n_tokens - p.W;
+    pv.W = RG ? 0 : p.W;
+    pv.kpacked = p.n_tokens - pv.W;
+    pv.tile0 = jb.tile0;
+    pv.bad_key = flags + 1;
     const unsigned char* lk = sm + OFF_LUT + 4 * (lane & (p.rk - 1));
     const unsigned char* lv = sm + OFF_LUT + 4 * nk * p.rk + 4 * (lane & (p.rv - 1));
     const int rk4 = 4 * p.rk, rv4 = 4 * p.rv;
@@ -504,17 +530,17 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
     HalfRegs<KB, 2> kc, kn;
     HalfRegs<VB, 2> vc, vn;
     bool ok = true;
-    load_half<KB>(kc, pv, 0, 0, p.off_kn);
+    load_half<KB, 2, RG>(kc, pv, 0, 0, p.off_kn);
     decode_half<KB>(kc, lk, rk4, sm + OFF_K, co);
-    if (tile_has_window(pv, 0)) window_half<2>(pv, 0, p.wk, sm + OFF_K, co);
+    if (!RG && tile_has_window(pv, 0)) window_half<2>(pv, 0, p.wk, sm + OFF_K, co);
     tc::fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) tc::mbar_arrive_cta(&bars[B_KFULL]);
-    if (ntiles > 1) load_half<KB>(kc, pv, 1, 0, p.off_kn);
-    load_half<VB>(vc, pv, 0, p.off_v, p.off_vn);
+    if (ntiles > 1) load_half<KB, 2, RG>(kc, pv, 1, 0, p.off_kn);
+    load_half<VB, 2, RG>(vc, pv, 0, p.off_v, p.off_vn);
     for (int j = 0; j < ntiles; ++j) {
-      if (j + 2 < ntiles) load_half<KB>(kn, pv, j + 2, 0, p.off_kn);
-      if (j + 1 < ntiles) load_half<VB>(vn, pv, j + 1, p.off_v, p.off_vn);
+      if (j + 2 < ntiles) load_half<KB, 2, RG>(kn, pv, j + 2, 0, p.off_kn);
+      if (j + 1 < ntiles) load_half<VB, 2, RG>(vn, pv, j + 1, p.off_v, p.off_vn);
       if (j + 1 < ntiles) {
         // K^ of tile j + 1: both S MMAs of tile j - 1 have read this stage
         const int jk = j + 1, sk = jk & 1;
@@ -523,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
                              p.status);
         if (!__all_sync(0xffffffffu, ok)) break;
         decode_half<KB>(kc, lk, rk4, sm + OFF_K + sk * kStage, co);
-        if (tile_has_window(pv, jk)) window_half<2>(pv, jk, p.wk, sm + OFF_K + sk * kStage, co);
+        if (!RG && tile_has_window(pv, jk)) window_half<2>(pv, jk, p.wk, sm + OFF_K + sk * kStage, co);
         tc::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive_cta(&bars[B_KFULL + sk]);
@@ -538,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
         ok = wait_or_abort(&bars[B_ROT], 0u, abort_flag, p.status);
       if (!__all_sync(0xffffffffu, ok)) break;
       decode_half<VB>(vc, lv, rv4, sm + OFF_V + s * kStage, co);
-      if (tile_has_window(pv, j)) window_half<2>(pv, j, p.wv, sm + OFF_V + s * kStage, co);
+      if (!RG && tile_has_window(pv, j)) window_half<2>(pv, j, p.wv, sm + OFF_V + s * kStage, co);
       tc::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive_cta(&bars[B_VFULL + s]);
@@ -581,12 +607,17 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, kTmemCols);
   }
+  if constexpr (RG) {
+    if (jb.sw.seg.slot >= 0)
+      join_partials<kD>(p.rg.plan, jb.sw, kWarps, p.out, p.o_dtype, p.os[3], &flags[0], row_out);
+  }
 }
 
 using TcFn = void (*)(TcPrefillParams);
 
+template <bool RG>
 TcFn tc2_fn(int kb, int vb) {
-#define TQ_PTC(K, V) if (kb == K && vb == V) return prefill_tc2_kernel<K, V>;
+#define TQ_PTC(K, V) if (kb == K && vb == V) return prefill_tc2_kernel<K, V, RG>;
   TQ_PTC(4, 2) TQ_PTC(4, 4) TQ_PTC(3, 3) TQ_PTC(2, 2) TQ_PTC(3, 2) TQ_PTC(4, 3)
   TQ_PTC(2, 4) TQ_PTC(3, 4) TQ_PTC(2, 3) TQ_PTC(6, 4) TQ_PTC(5, 5) TQ_PTC(6, 6) TQ_PTC(5, 4)
 #undef TQ_PTC
@@ -595,12 +626,13 @@ TcFn tc2_fn(int kb, int vb) {
 
 }  // namespace
 
-int launch_prefill_tc2(const TcPrefillParams& base, int kb, int vb, int64_t B, int64_t Hq,
-                       cudaStream_t st) {
-  TcFn fn = tc2_fn(kb, vb);
-  if (!fn) return 1;
+namespace {
+
+// Two tiles of 128 rows: with hc >= 2 they split the heads, else the
+// positions; pair tables within 32 KB: 32 lane copies where they fit, else
+// 16 / 8.
+TcPrefillParams tc2_params(const TcPrefillParams& base, int kb, int vb) {
   TcPrefillParams p = base;
-  // two tiles of 128 rows: with hc >= 2 they split the heads, else the positions
   const int hct = p.hc >= 2 ? p.hc / 2 : 1;
   const int Pt = 128 / hct;
   p.pshift = 0;
@@ -608,8 +640,6 @@ int launch_prefill_tc2(const TcPrefillParams& base, int kb, int vb, int64_t B, i
   p.pcta = p.hc >= 2 ? Pt : 256;
   p.tile_head_step = p.hc >= 2 ? hct : 0;
   p.tile_pos_step = p.hc >= 2 ? 0 : 128;
-  p.nqb = (int)((p.Tq + p.pcta - 1) / p.pcta);
-  // pair tables within 32 KB: 32 lane copies where they fit, else 16 / 8
   const int nk = 1 << (2 * kb), nv = 1 << (2 * vb);
   int rk = 32, rv = 32;
   while ((nk * rk + nv * rv) * 4 > (int)kLutMax) {
@@ -617,10 +647,30 @@ int launch_prefill_tc2(const TcPrefillParams& base, int kb, int vb, int64_t B, i
   }
   p.rk = rk;
   p.rv = rv;
+  return p;
+}
+
+}  // namespace
+
+int launch_prefill_tc2(const TcPrefillParams& base, int kb, int vb, int64_t B, int64_t Hq,
+                       cudaStream_t st) {
+  TcFn fn = tc2_fn<false>(kb, vb);
+  if (!fn) return 1;
+  TcPrefillParams p = tc2_params(base, kb, vb);
+  p.nqb = (int)((p.Tq + p.pcta - 1) / p.pcta);
   if (set_smem_attr((const void*)fn, SMEM_BYTES) != TQ_OK) return TQ_ERR_CUDA;
   dim3 grid((unsigned)p.nqb, (unsigned)(B * Hq / p.hc));
   fn<<<grid, kThreads, SMEM_BYTES, st>>>(p);
   return check_launch("tq_prefill_attn");
+}
+
+int launch_attend_tc2(const TcPrefillParams& base, int kb, int vb, int64_t grid,
+                      cudaStream_t st) {
+  TcFn fn = tc2_fn<true>(kb, vb);
+  const TcPrefillParams p = tc2_params(base, kb, vb);
+  if (set_smem_attr((const void*)fn, SMEM_BYTES) != TQ_OK) return TQ_ERR_CUDA;
+  fn<<<(unsigned)grid, kThreads, SMEM_BYTES, st>>>(p);
+  return check_launch("tq_attend_ragged");
 }
 
 }  // namespace tq

@@ -656,9 +656,10 @@ def attend_ragged(tables: LayerTables, pages, q: torch.Tensor, batch: RaggedBatc
     (prompt chunks, draft tokens, single tokens, mixed), or with ``causal``
     False every row over all of them (cross attention: the pages hold an
     encoder's states, seq_lens their lengths).  A row that sees no key is
-    zero.  Work is split along long contexts; ``engine`` as in
-    prefill_attention, and 4 for the kernel of few query rows.  Pass a ``workspace`` to reuse one buffer across
-    calls on one stream."""
+    zero.  Work is split along long contexts.  ``engine`` 0 picks the kernels
+    by each request's rows; 1 is the mma.sync kernel, 2 the tcgen05 kernel, 3
+    the kernel of few query rows.  Pass a ``workspace`` to reuse one buffer
+    across calls on one stream."""
     _inference_only("attend_ragged", q.device, q, out, batch.q_start)
     if out is None:
         out = torch.empty_like(q)

@@ -435,10 +435,9 @@ typedef struct tq_attend_args {
   float scale;                /* softmax scale                                */
   int32_t causal;
   int32_t engine;             /* 0: the fastest kernels for the lengths; 1: the
-                                 mma.sync kernel; 2 / 3: the tcgen05 kernel
-                                 with 128 / 256 rows per CTA; 4: the kernel
-                                 of 8 or 16 rows per CTA (head_dim 64 or 128,
-                                 codes of 2 to 4 bits)                        */
+                                 mma.sync kernel; 2: the tcgen05 kernel (256
+                                 rows per CTA); 3: the kernel of 8 or 16 rows
+                                 per CTA (codes of 2 to 4 bits)               */
 } tq_attend_args;
 
 /* 0 on bad arguments.  The workspace must be 256-byte aligned and belongs to
