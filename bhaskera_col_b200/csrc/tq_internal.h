@@ -73,6 +73,15 @@ int launch_append_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c
 int launch_dequant_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                           const tq_ragged* batch, const tq_tensor4* ko, const tq_tensor4* vo,
                           uint32_t* status, cudaStream_t st);
+// The tensor-core forms (tq_ragged_tc.cu): TQ_OK when they ran, 1 when they do
+// not apply (the caller runs the CUDA-core kernels), or an error.
+int launch_append_ragged_tc(const tq_geom* g, const tq_tables* t, const tq_cache* c,
+                            const tq_tensor4* k, const tq_tensor4* v, const tq_ragged* batch,
+                            const tq_rope* rope, const tq_head_norm* norm, const tq_positions* pos,
+                            uint32_t* status, cudaStream_t st);
+int launch_dequant_ragged_tc(const tq_geom* g, const tq_tables* t, const tq_cache* c,
+                             const tq_ragged* batch, const tq_tensor4* ko, const tq_tensor4* vo,
+                             uint32_t* status, cudaStream_t st);
 size_t attend_ragged_workspace(const tq_geom* g, const tq_cache* c, const tq_attend_args* a);
 int launch_attend_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                          const tq_attend_args* a, void* ws, uint32_t* status, cudaStream_t st);

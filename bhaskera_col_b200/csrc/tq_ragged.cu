@@ -243,6 +243,8 @@ int launch_append_ragged(const tq_geom* G, const tq_tables* t, const tq_cache* c
   p.pos_stride = pos ? pos->stride[1] : 0;
   const int64_t nvec = p.rv.N * p.H;
   if (nvec == 0) return TQ_OK;
+  if (const int rc = launch_append_ragged_tc(G, t, c, k, v, batch, rope, norm, pos, status, st); rc != 1)
+    return rc;
   const int D = G->head_dim;
   const size_t smem = D == 32 ? append_ragged_smem<32>() : D == 64 ? append_ragged_smem<64>()
                     : D == 96 ? append_ragged_smem<96>() : append_ragged_smem<128>();
@@ -263,6 +265,7 @@ int launch_dequant_ragged(const tq_geom* G, const tq_tables* t, const tq_cache* 
   p.status = status;
   const int64_t nvec = p.rv.N * p.H;
   if (nvec == 0) return TQ_OK;
+  if (const int rc = launch_dequant_ragged_tc(G, t, c, batch, ko, vo, status, st); rc != 1) return rc;
   const int D = G->head_dim;
   void (*fn)(RaggedKV) = D == 32 ? read_ragged_kernel<32> : D == 64 ? read_ragged_kernel<64>
                        : D == 96 ? read_ragged_kernel<96> : read_ragged_kernel<128>;

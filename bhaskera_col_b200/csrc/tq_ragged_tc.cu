@@ -1,0 +1,1000 @@
+// tq_ragged_tc.cu — ragged append and ragged read-back on the 5th-generation
+// tensor cores (head_dim 64 and 128); other shapes run the CUDA-core kernels of
+// tq_ragged.cu, which give the math.
+//
+// A tile is 128 consecutive head vectors of the flattened batch (token-major,
+// so the heads of a token share its row of the rotation table and a tile is
+// contiguous in memory), M of one tcgen05.mma with N = K = head_dim.  One
+// persistent CTA per SM, a launch each for K and V, three roles:
+//   warps 0-7   operand makers: 16 vectors each.  Append: load, norm, rotate,
+//               norm again, split into fp16; read-back: codes -> centroids
+//               through lane-replicated tables.  They also find each vector's
+//               request, position and page.
+//   warp 8      one thread issues the MMAs into one of two accumulators
+//   warps 9-    epilogue, one thread per vector and 32 columns.  Append:
+//               bucketize and pack; read-back: times the norm, out through
+//               shared memory so that rows leave in whole lines
+//
+// Append: y n s 2^6 = (x s) (2^6 R)^T with s the power of two that puts ||x||
+// into [2^10, 2^11), x s = hi + lo and 2^6 R = hi + lo in fp16 (22 bits, the
+// scales keep lo out of the subnormals), fp32 accumulation:
+//   hi hi + hi lo, and + lo hi where x has more than fp16's bits (fp32 inputs,
+//   a normed or rotated k; a bf16 or fp16 x is its own hi).
+// R's rows lie in the packed order of the row (K quad order, V octet order), so
+// accumulator column p is the coordinate stored at position p.
+// Bucketize without branches, exactly: a cell of the grid 0.4 x the smallest
+// gap wide holds at most one boundary in its window, so the cell's entry {-b
+// 2^100, codes below} and the sign of y - b give the code (the same scheme as
+// tq_append_tc.cu).  Tables that do not fit take a binary search.
+//
+// Read-back: x = (c R) n with R's rows in packed order as the K dimension,
+// c and R as fp16 hi + lo (three products); for bf16 results c = hi alone: its
+// rounding, 2^-11 of each term, is an eighth of the result's own.
+//
+// Bounds: HBM (256 B in, 66 out per 4-bit vector of 128 bf16, or the reverse);
+// next the append's epilogue (8 instructions a coordinate) and the makers.
+//
+// Every wait is bounded; on expiry the kernel sets TQ_DEV_WAIT_TIMEOUT in the
+// status word, no MMA is left in flight and tensor memory is released.
+#include "tq_internal.h"
+#include "tq_ragged.cuh"
+#include "tq_tc.cuh"
+
+#include <limits.h>
+
+namespace tq {
+namespace {
+
+constexpr int kM = 128;                    // vectors per tile
+constexpr int kMakers = 8;                 // maker warps, 16 vectors each
+constexpr int kRing = 4;                   // tiles of per-vector data in flight
+constexpr int kSmem = 227 * 1024;
+constexpr float kCmp = 1.2676506e30f;      // 2^100
+constexpr float kRScale = 64.f;
+
+struct RaggedTc {
+  PageGeom g;
+  const float* cent[2];
+  const float* bnd[2];
+  const float* rot;                        // R [D][D]
+  uint8_t* pages;
+  PageMap pm;
+  uint32_t* status;
+  RaggedView rv;
+  int H, ntiles, nvec;                     // heads, tiles, vectors (rows x heads)
+  const void* x[2];                        // append: inputs; read-back: outputs (NULL: absent)
+  int dtype[2];
+  int64_t stride[2][3];                    // head, row, dim
+  int vec[2];                              // read-back: rows take 16-byte stores
+  int use_lo[2];                           // append: x has more bits than fp16
+  HeadXform f;                             // of K (append)
+  const void* pos; int pos64; int64_t pos_stride;
+};
+
+template <int D>
+struct Shape {
+  static constexpr int kSplit = D / 32;                    // epilogue warps per lane quarter
+  static constexpr int kEpi = 4 * kSplit;
+  static constexpr int kThreads = 32 * (kMakers + 1 + kEpi);
+  static constexpr int kTerm = kM * D * 2;                 // one fp16 operand tile
+  static constexpr int kB = D * D * 2;                     // one term of R
+  static constexpr int kLanes = D / 8;                     // lanes per vector (8 values each)
+};
+
+// Byte offset of 16-byte chunk c of row r: [64-column half][rows][128 B], swizzled.
+template <int ROWS>
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+  return (uint32_t)((c >> 3) * (ROWS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+__device__ __forceinline__ void expired(uint32_t* status, volatile int* abort_flag) {
+  *abort_flag = 1;
+  atomicOr(status, TQ_DEV_WAIT_TIMEOUT);
+}
+
+// Bounded wait (2 s) that also ends once another role has given up.
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                         uint32_t* status) {
+  uint64_t t0 = 0;
+  for (uint32_t i = 0;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 63u) == 63u) {
+      if (*abort_flag) return false;
+      const uint64_t t = global_ns();
+      if (t0 == 0) t0 = t;
+      else if (t - t0 > 2000000000ull) break;
+    }
+  }
+  expired(status, abort_flag);
+  return false;
+}
+
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pack_half2(a, b);
+  const __half2 h = *reinterpret_cast<const __half2*>(&hi);
+  lo = pack_half2(a - __low2float(h), b - __high2float(h));
+}
+
+// R's rows in packed order, times kRScale, as fp16 hi at `b` and lo behind it.
+template <int D>
+__device__ __forceinline__ void stage_rotation(unsigned char* b, const float* rot, int which,
+                                               int tid, int nthreads) {
+  for (int i = tid; i < D * D / 8; i += nthreads) {
+    const int r = i / (D / 8), c = i % (D / 8);
+    const int row = which == 0 ? k_coord_at(r, D) : v_coord_at(r, D);
+    const float4* src = reinterpret_cast<const float4*>(rot + row * D + 8 * c);
+    const float4 u = __ldg(src), v = __ldg(src + 1);
+    uint32_t h[4], l[4];
+    split_pair(u.x * kRScale, u.y * kRScale, h[0], l[0]);
+    split_pair(u.z * kRScale, u.w * kRScale, h[1], l[1]);
+    split_pair(v.x * kRScale, v.y * kRScale, h[2], l[2]);
+    split_pair(v.z * kRScale, v.w * kRScale, h[3], l[3]);
+    const uint32_t at = chunk_at<D>(r, c);
+    *reinterpret_cast<uint4*>(b + at) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(b + Shape<D>::kB + at) = make_uint4(l[0], l[1], l[2], l[3]);
+  }
+}
+
+// What the epilogue needs of each vector of a tile.
+struct Vec {
+  uint8_t* page;                           // NULL: no place
+  float n, inv;                            // norm; append: factor of the accumulator
+  int slot;                                // token in its page
+  int state;                               // 0: row of no request, 1: no place, 2: stored
+};
+
+// Lane i < 16 of a maker warp finds vector v0 + i; `row`: its row of the
+// rotation table.
+__device__ __forceinline__ Vec find_vector(const RaggedTc& p, int i, int nvec, int lane, int& row) {
+  Vec v;
+  v.page = nullptr;
+  v.n = v.inv = 0.f;
+  v.slot = v.state = 0;
+  row = 0;
+  if (lane >= 16 || i >= nvec) return v;
+  const int n = i / p.H, h = i % p.H;
+  const int64_t r = request_of(p.rv, n);
+  if (r < 0) return v;
+  v.state = 1;
+  const int64_t pos = (int64_t)__ldg(p.rv.seq_lens + r) - __ldg(p.rv.q_start + r + 1) + n;
+  if (pos < 0 || pos >= p.rv.cap) {
+    atomicOr(p.status, TQ_DEV_BAD_POSITION);
+    return v;
+  }
+  bool ok;
+  const int64_t ps = page_slot(p.pm, r * p.H + h, pos / kPageTokens, ok);
+  if (!ok) {
+    atomicOr(p.status, TQ_DEV_BAD_BLOCK);
+    return v;
+  }
+  v.page = p.pages + ps * (int64_t)p.g.page_bytes;
+  v.slot = (int)(pos % kPageTokens);
+  v.state = 2;
+  if (p.f.cos_sin) {
+    int64_t at = pos;
+    if (p.pos)
+      at = p.pos64 ? (int64_t)__ldg(reinterpret_cast<const long long*>(p.pos) + n * p.pos_stride)
+                   : (int64_t)__ldg(reinterpret_cast<const int*>(p.pos) + n * p.pos_stride);
+    row = (int)table_row(p.f, at, p.status);
+  }
+  return v;
+}
+
+// Shared pieces of both kernels: barriers, the issuing thread, the accumulators.
+struct Pipe {
+  uint64_t* a_full;                        // [2] maker warps
+  uint64_t* a_empty;                       // [2] MMA commit
+  uint64_t* acc_full;                      // [2] MMA commit
+  uint64_t* acc_empty;                     // [2] epilogue warps
+  volatile int* abort_flag;
+  uint32_t* tmem_slot;
+};
+
+__device__ __forceinline__ Pipe make_pipe(unsigned char* at) {
+  uint64_t* b = reinterpret_cast<uint64_t*>(at);
+  Pipe p;
+  p.a_full = b;
+  p.a_empty = b + 2;
+  p.acc_full = b + 4;
+  p.acc_empty = b + 6;
+  p.tmem_slot = reinterpret_cast<uint32_t*>(b + 8);
+  p.abort_flag = reinterpret_cast<volatile int*>(b + 9);
+  return p;
+}
+constexpr int kPipeBytes = 128;
+
+__device__ __forceinline__ void init_pipe(const Pipe& p, int epi_warps) {
+  for (int i = 0; i < 2; ++i) {
+    mbar_init(&p.a_full[i], kMakers);
+    mbar_init(&p.a_empty[i], 1);
+    mbar_init(&p.acc_full[i], 1);
+    mbar_init(&p.acc_empty[i], epi_warps);
+  }
+  *p.abort_flag = 0;
+  fence_mbar_init();
+}
+
+// One thread: the MMAs of every tile.  terms(stage, term, a, b) gives the
+// operand addresses of each product or false past the last.
+template <int D, int STAGES, bool B_MN, class Terms>
+__device__ __forceinline__ void issue_tiles(const Pipe& pp, uint32_t tmem, int first, int step,
+                                            int ntiles, uint32_t* status, Terms terms) {
+  constexpr uint32_t idesc = tc::idesc_f16_f32(kM, D) | (B_MN ? 1u << 16 : 0u);
+  int it = 0, issued = 0;
+  for (int tile = first; tile < ntiles; tile += step, ++it) {
+    const int st = it % STAGES, ac = it & 1;
+    if (!wait_for(&pp.a_full[st], (uint32_t)((it / STAGES) & 1), pp.abort_flag, status) ||
+        (it >= 2 &&
+         !wait_for(&pp.acc_empty[ac], (uint32_t)(((it / 2) - 1) & 1), pp.abort_flag, status)))
+      break;
+    tc::tc_fence_after();
+    uint32_t a, b;
+    for (int term = 0; terms(st, term, a, b); ++term)
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const uint64_t ad =
+            tc::sdesc_kmajor_sw128(a + (uint32_t)((ks >> 2) * (kM * 128) + (ks & 3) * 32));
+        uint64_t bd;
+        if (B_MN) {
+          // 16 rows of K on; N blocks of 64 columns D x 128 B apart
+          bd = tc::sdesc_kmajor_sw128(b + ks * 2048);
+          bd = (bd & ~((uint64_t)0x3FFF << 16)) | ((uint64_t)((D * 128) >> 4) << 16);
+        } else {
+          bd = tc::sdesc_kmajor_sw128(b + (uint32_t)((ks >> 2) * (D * 128) + (ks & 3) * 32));
+        }
+        tc::umma_bf16(tmem + (uint32_t)(ac * D), ad, bd, idesc, (term | ks) ? 1u : 0u);
+      }
+    tc::umma_commit(&pp.a_empty[st]);
+    tc::umma_commit(&pp.acc_full[ac]);
+    issued = it + 1;
+  }
+  // the last commit tracks every MMA issued before it
+  if (issued > 0)
+    mbar_wait_bounded(&pp.acc_full[(issued - 1) & 1], (uint32_t)(((issued - 1) / 2) & 1), 16u);
+}
+
+// ---------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------
+template <int D>
+struct AppendSmem {
+  static constexpr int OFF_B = 0;
+  static constexpr int OFF_A = OFF_B + 2 * Shape<D>::kB;           // 2 stages of hi, lo
+  static constexpr int OFF_BND = OFF_A + 4 * Shape<D>::kTerm;      // [256]
+  static constexpr int OFF_VEC = OFF_BND + 1024;                   // [kRing][kM]
+  static constexpr int OFF_PIPE = OFF_VEC + kRing * kM * (int)sizeof(Vec);
+  static constexpr int OFF_LUT = OFF_PIPE + kPipeBytes;
+  static constexpr int LUT_BYTES = kSmem - 1024 - OFF_LUT;         // 1 KB: slack to align the base
+  static_assert(LUT_BYTES >= 8 * 1024, "shared memory");
+  static_assert(OFF_A % 1024 == 0 && Shape<D>::kTerm % 1024 == 0, "swizzled tiles");
+};
+
+// Four 16-bit values of a vector in fp32.
+__device__ __forceinline__ void widen4(uint2 u, int dtype, float* v) {
+  if (dtype == TQ_BF16) {
+    v[0] = __uint_as_float(u.x << 16);
+    v[1] = __uint_as_float(u.x & 0xFFFF0000u);
+    v[2] = __uint_as_float(u.y << 16);
+    v[3] = __uint_as_float(u.y & 0xFFFF0000u);
+  } else {
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+    v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+  }
+}
+
+template <int N>
+__device__ __forceinline__ float sum_lanes(float x) {
+#pragma unroll
+  for (int o = N / 2; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+template <int D, int BITS>
+__global__ void __launch_bounds__(Shape<D>::kThreads, 1) append_ragged_tc_kernel(RaggedTc p, int which) {
+  using S = Shape<D>;
+  using SM = AppendSmem<D>;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  unsigned char* sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+  const Pipe pp = make_pipe(sm + SM::OFF_PIPE);
+  float* lutpar = reinterpret_cast<float*>(sm + SM::OFF_PIPE + 96);
+  float* bnd = reinterpret_cast<float*>(sm + SM::OFF_BND);
+  Vec* ring = reinterpret_cast<Vec*>(sm + SM::OFF_VEC);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int nb = (1 << BITS) - 1;
+  const int nvec = p.nvec;
+
+  // the V kernel may start beside the K kernel (they share no byte); it ends
+  // after it, so that whatever follows sees both
+  pdl_launch_dependents();
+  if (tid == 0) init_pipe(pp, S::kEpi);
+  if (warp == kMakers) {
+    tc::tmem_alloc(pp.tmem_slot, 2 * D);
+    tc::tmem_relinquish();
+  }
+  for (int i = tid; i < nb; i += S::kThreads) bnd[i] = p.bnd[which][i];
+  stage_rotation<D>(sm + SM::OFF_B, p.rot, which, tid, S::kThreads);
+  __syncthreads();
+  if (tid == 0) {
+    float gap = 1.f;
+    for (int i = 0; i + 1 < nb; ++i) gap = fminf(gap, bnd[i + 1] - bnd[i]);
+    const float w = 0.4f * gap;
+    const float span = fmaxf(fabsf(bnd[0]), fabsf(bnd[nb - 1]));
+    const float L = ceilf(span / w) + 3.f, nc = 2.f * L + 1.f;
+    const bool ok = w > 0.f && nc * 128.f <= (float)SM::LUT_BYTES && span < 1.f;
+    lutpar[0] = 1.f / (2.f * L * w);       // u = sat(v * lutpar[0] + 0.5)
+    lutpar[1] = 2.f * L;                   // cell = round(u * 2L)
+    lutpar[2] = ok ? nc : 0.f;
+    lutpar[3] = w;
+  }
+  __syncthreads();
+  const int ncells = (int)lutpar[2];
+  {
+    const float w = lutpar[3], L = 0.5f * lutpar[1];
+    for (int i = tid; i < ncells * 16; i += S::kThreads) {
+      const int c = i >> 4;
+      const float wl = ((float)c - L - 1.f) * w, wh = ((float)c - L + 1.f) * w;
+      const int base = bucketize_lt(bnd, nb, wl);
+      const float nbk = (base < nb && bnd[base] <= wh) ? -bnd[base] * kCmp : -INFINITY;
+      reinterpret_cast<float2*>(sm + SM::OFF_LUT)[i] = make_float2(nbk, (float)base);
+    }
+  }
+  tc::fence_proxy_async_smem();
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = *pp.tmem_slot;
+  const int first = blockIdx.x, step = gridDim.x;
+  const bool use_lo = p.use_lo[which] != 0;
+
+  if (warp < kMakers) {
+    // ------------------------------------------------------------ operand makers
+    constexpr int RPI = 32 / S::kLanes, NIT = 16 / RPI;    // vectors per pass, passes
+    const int l = lane % S::kLanes, sub = lane / S::kLanes;
+    const HeadXform f = which == 0 ? p.f : HeadXform{};
+    // the lane's two groups of four dims: partners of the rotation (halves), or
+    // plain halves of the vector
+    const int half = f.rot / 2;
+    const bool pairs = f.cos_sin && !f.interleaved;        // (i, half + i)
+    int ga = 4 * l, gb = D / 2 + 4 * l;
+    bool turn = f.cos_sin != nullptr;                      // this lane rotates
+    if (pairs) {
+      if (4 * l < half) { gb = half + 4 * l; }
+      else { ga = f.rot + 2 * (4 * l - half); gb = ga + 4; turn = false; }
+    }
+    const bool turn_a = turn && (pairs || ga < f.rot), turn_b = turn && !pairs && gb < f.rot;
+    float w[8];
+    if (f.weight) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        w[e] = load_elem(f.weight, f.w_dtype, e < 4 ? ga + e : gb + e - 4) + f.w_offset;
+    }
+    const int64_t* xs = p.stride[which];
+    int it = 0;
+    for (int tile = first; tile < p.ntiles; tile += step, ++it) {
+      const int st = it & 1;
+      Vec* vec = ring + (it % kRing) * kM + 16 * warp;
+      const int v0 = tile * kM + 16 * warp;
+      // every vector's 16-bit values in flight while its place is found (32-bit
+      // ones would take twice the registers: loaded when they are used)
+      const bool wide = p.dtype[which] == TQ_F32;
+      auto base_of = [&](int i) {
+        return (int64_t)(i / p.H) * xs[1] + (int64_t)(i % p.H) * xs[0];
+      };
+      uint2 xa[NIT], xb[NIT];
+#pragma unroll
+      for (int k = 0; k < NIT; ++k) {
+        const int i = v0 + k * RPI + sub;
+        xa[k] = xb[k] = make_uint2(0u, 0u);
+        if (!wide && i < nvec) {
+          const uint16_t* x = static_cast<const uint16_t*>(p.x[which]) + base_of(i);
+          xa[k] = __ldg(reinterpret_cast<const uint2*>(x + ga));
+          xb[k] = __ldg(reinterpret_cast<const uint2*>(x + gb));
+        }
+      }
+      int trow;
+      const Vec place = find_vector(p, v0 + lane, nvec, lane, trow);
+      // the stage is free, and with it the ring's entry: its tile's epilogue
+      // ran before this stage's last MMAs could start
+      bool ok = it < 2 || wait_for(&pp.a_empty[st], (uint32_t)(((it / 2) - 1) & 1), pp.abort_flag,
+                                   p.status);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      if (lane < 16) vec[lane] = place;
+      __syncwarp();
+      unsigned char* hi = sm + SM::OFF_A + st * 2 * S::kTerm;
+      int last_row = -1;
+      float4 ca = make_float4(0.f, 0.f, 0.f, 0.f), sa = ca, cb = ca;
+#pragma unroll
+      for (int k = 0; k < NIT; ++k) {
+        const int vi = k * RPI + sub;                      // vector of the warp's 16
+        float v[8];
+        if (wide) {
+          float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+          if (v0 + vi < nvec) {
+            const float* x = static_cast<const float*>(p.x[which]) + base_of(v0 + vi);
+            a = __ldg(reinterpret_cast<const float4*>(x + ga));
+            b = __ldg(reinterpret_cast<const float4*>(x + gb));
+          }
+          v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+          v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+          widen4(xa[k], p.dtype[which], v);
+          widen4(xb[k], p.dtype[which], v + 4);
+        }
+        if (f.weight) {
+          float ss = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) ss = fmaf(v[e], v[e], ss);
+          const float r = 1.f / sqrtf(sum_lanes<S::kLanes>(ss) / (float)D + f.eps);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = v[e] * r * w[e];
+        }
+        if (f.cos_sin) {
+          const int row = __shfl_sync(0xffffffffu, trow, vi);
+          if (row != last_row) {                           // heads of one token share it
+            last_row = row;
+            const float* cs = f.cos_sin + (int64_t)row * f.rot;
+            if (pairs) {
+              if (turn_a) {
+                ca = __ldg(reinterpret_cast<const float4*>(cs + ga));
+                sa = __ldg(reinterpret_cast<const float4*>(cs + half + ga));
+              }
+            } else {
+              if (turn_a) {
+                const float2 c = __ldg(reinterpret_cast<const float2*>(cs + ga / 2));
+                const float2 s = __ldg(reinterpret_cast<const float2*>(cs + half + ga / 2));
+                ca = make_float4(c.x, c.y, s.x, s.y);
+              }
+              if (turn_b) {
+                const float2 c = __ldg(reinterpret_cast<const float2*>(cs + gb / 2));
+                const float2 s = __ldg(reinterpret_cast<const float2*>(cs + half + gb / 2));
+                cb = make_float4(c.x, c.y, s.x, s.y);
+              }
+            }
+          }
+          auto rotate = [](float& a, float& b, float c, float s) {
+            const float t = a * c - b * s;
+            b = b * c + a * s;
+            a = t;
+          };
+          if (pairs) {
+            if (turn_a) {
+              rotate(v[0], v[4], ca.x, sa.x);
+              rotate(v[1], v[5], ca.y, sa.y);
+              rotate(v[2], v[6], ca.z, sa.z);
+              rotate(v[3], v[7], ca.w, sa.w);
+            }
+          } else {
+            if (turn_a) { rotate(v[0], v[1], ca.x, ca.z); rotate(v[2], v[3], ca.y, ca.w); }
+            if (turn_b) { rotate(v[4], v[5], cb.x, cb.z); rotate(v[6], v[7], cb.y, cb.w); }
+          }
+        }
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fmaf(v[e], v[e], ss);
+        const float n = sqrtf(sum_lanes<S::kLanes>(ss));
+        // 2^(10 - exponent of n), from 2^-117 to 2^100
+        const int ex = (int)((__float_as_uint(n) >> 23) & 255u) - 127;
+        const float s = __uint_as_float((uint32_t)(127 + 10 - max(ex, -90)) << 23);
+        if (l == 0) {
+          vec[vi].n = n;
+          vec[vi].inv = 1.f / (s * fmaxf(n, 1e-8f) * kRScale);
+        }
+        const int r = 16 * warp + vi;
+        uint32_t h[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) split_pair(v[2 * e] * s, v[2 * e + 1] * s, h[e], lo[e]);
+        const uint32_t aa = chunk_at<kM>(r, ga >> 3) + ((ga & 4) << 1);
+        const uint32_t ab = chunk_at<kM>(r, gb >> 3) + ((gb & 4) << 1);
+        *reinterpret_cast<uint2*>(hi + aa) = make_uint2(h[0], h[1]);
+        *reinterpret_cast<uint2*>(hi + ab) = make_uint2(h[2], h[3]);
+        if (use_lo) {
+          *reinterpret_cast<uint2*>(hi + S::kTerm + aa) = make_uint2(lo[0], lo[1]);
+          *reinterpret_cast<uint2*>(hi + S::kTerm + ab) = make_uint2(lo[2], lo[3]);
+        }
+      }
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive_cta(&pp.a_full[st]);
+    }
+  } else if (warp == kMakers) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      const uint32_t a0 = smem_u32(sm + SM::OFF_A), b0 = smem_u32(sm + SM::OFF_B);
+      issue_tiles<D, 2, false>(pp, tmem, first, step, p.ntiles, p.status,
+                               [&](int st, int term, uint32_t& a, uint32_t& b) {
+                                 a = a0 + st * 2 * S::kTerm + (term == 2 ? S::kTerm : 0);
+                                 b = b0 + (term == 1 ? S::kB : 0);
+                                 return term < (use_lo ? 3 : 2);
+                               });
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int q = warp & 3, part = (warp - kMakers - 1) >> 2;
+    const int r = 32 * q + lane;
+    const int row_bytes = D * BITS / 8;
+    const int sec = which == 0 ? p.g.off_k : p.g.off_v, noff = which == 0 ? p.g.off_kn : p.g.off_vn;
+    const uint32_t lane_off = smem_u32(sm + SM::OFF_LUT) + (uint32_t)((lane & 15) * 8) -
+                              (0x4B000000u << 7);
+    const float par0 = lutpar[0], c2l = lutpar[1];
+    int it = 0;
+    for (int tile = first; tile < p.ntiles; tile += step, ++it) {
+      const int ac = it & 1;
+      bool ok = wait_for(&pp.acc_full[ac], (uint32_t)((it / 2) & 1), pp.abort_flag, p.status);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc::tc_fence_after();
+      uint32_t yb[32];
+      tc::tmem_ld_x32(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(ac * D + 32 * part), yb);
+      const Vec v = ring[(it % kRing) * kM + r];
+      tc::tmem_wait_ld();
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive_cta(&pp.acc_empty[ac]);
+      uint32_t words[BITS];
+#pragma unroll
+      for (int x = 0; x < BITS; ++x) words[x] = 0u;
+      if (ncells > 0) {
+        // codes gather in runs of <= 23 bits as acc = 2^23 + field, exactly
+        const float ca = v.inv * par0, cK = v.inv * kCmp;
+        auto flush = [&](float acc, int o, int len) {
+          const uint32_t bits = __float_as_uint(acc) & ((1u << len) - 1u);
+          const int wi = o >> 5, sh = o & 31;
+          words[wi] += bits << sh;
+          if (sh + len > 32) words[wi + 1] += bits >> (32 - sh);
+        };
+        float acc = 8388608.f;
+        int gs = 0, gl = 0;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const int bo = j * BITS;
+          if (gl > 0 && (gl + BITS > 23 || (bo & 31) == 0)) {
+            flush(acc, gs, gl);
+            acc = 8388608.f;
+            gs = bo;
+            gl = 0;
+          }
+          const float y = __uint_as_float(yb[j]);
+          const float u = __saturatef(fmaf(y, ca, 0.5f));
+          const float cell = fmaf(u, c2l, 8388608.f);
+          const float2 e = tc::lds_f2((__float_as_uint(cell) << 7) + lane_off);
+          const float above = __saturatef(fmaf(y, cK, e.x) * kCmp);
+          acc = fmaf(e.y + above, (float)(1u << gl), acc);
+          gl += BITS;
+        }
+        flush(acc, gs, gl);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const uint32_t code = (uint32_t)bucketize_lt(bnd, nb, __uint_as_float(yb[j]) * v.inv);
+          const int bo = j * BITS, wi = bo >> 5, sh = bo & 31;
+          words[wi] += code << sh;
+          if (sh + BITS > 32) words[wi + 1] += code >> (32 - sh);
+        }
+      }
+      if (v.page) {
+        uint8_t* row = v.page + sec + v.slot * row_bytes + part * (4 * BITS);
+        if constexpr (BITS % 4 == 0) {
+#pragma unroll
+          for (int x = 0; x < BITS / 4; ++x)
+            reinterpret_cast<uint4*>(row)[x] = make_uint4(words[4 * x], words[4 * x + 1],
+                                                          words[4 * x + 2], words[4 * x + 3]);
+        } else if constexpr (BITS % 2 == 0) {
+#pragma unroll
+          for (int x = 0; x < BITS / 2; ++x)
+            reinterpret_cast<uint2*>(row)[x] = make_uint2(words[2 * x], words[2 * x + 1]);
+        } else {
+#pragma unroll
+          for (int x = 0; x < BITS; ++x) reinterpret_cast<uint32_t*>(row)[x] = words[x];
+        }
+        if (part == 0) reinterpret_cast<__half*>(v.page + noff)[v.slot] = __float2half_rn(v.n);
+      }
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == kMakers) {
+    __syncwarp();
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, 2 * D);
+  }
+  pdl_wait();
+}
+
+// ---------------------------------------------------------------------------
+// read-back
+// ---------------------------------------------------------------------------
+// LO: c as hi + lo (fp16 and fp32 results), one operand stage; else c = hi, two.
+template <int D, int BITS, bool LO>
+struct ReadSmem {
+  static constexpr int STAGES = LO ? 1 : 2, RING = STAGES + 2;      // see the makers
+  static constexpr bool kPair = BITS <= 4;                         // table of code pairs
+  // entry: fp16 pair hi (and lo) of two codes, or one code's {hi, lo}; copies
+  // for 32 lanes of 4-byte entries, 16 of 8-byte ones: 128 bytes
+  static constexpr int OFF_B = 0;
+  static constexpr int OFF_A = OFF_B + 2 * Shape<D>::kB;
+  static constexpr int OFF_OUT = OFF_A + (LO ? 2 : STAGES) * Shape<D>::kTerm;   // [kM][D] results
+  static constexpr int OFF_LUT = OFF_OUT + kM * D * (LO ? 4 : 2);
+  static constexpr int LUT_BYTES = (1 << (kPair ? 2 * BITS : BITS)) * 128;
+  static constexpr int OFF_N = OFF_LUT + LUT_BYTES;                // [RING][kM] norms
+  static constexpr int OFF_ST = OFF_N + RING * kM * 4;             // [RING][kM] states (bytes)
+  static constexpr int OFF_PIPE = OFF_ST + RING * kM;
+  static constexpr int BYTES = OFF_PIPE + kPipeBytes + 1024;
+  static_assert(BYTES <= kSmem, "shared memory");
+};
+
+// The 8 codes of chunk c of a packed row: 8 * BITS bits from byte c * BITS on.
+template <int BITS>
+__device__ __forceinline__ uint64_t load_chunk(const uint8_t* row, int c) {
+  const int off = c * BITS;
+  if constexpr (BITS == 8) return __ldg(reinterpret_cast<const unsigned long long*>(row + off));
+  if constexpr (BITS == 4) return __ldg(reinterpret_cast<const uint32_t*>(row + off));
+  if constexpr (BITS == 2) return __ldg(reinterpret_cast<const uint16_t*>(row + off));
+  if constexpr (BITS == 1) return __ldg(row + off);
+  // the words that hold them (reads stay inside the page: norms follow the codes)
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(row + (off & ~3));
+  const int sh = (off & 3) * 8;
+  uint64_t v = (uint64_t)__ldg(w) | ((uint64_t)__ldg(w + 1) << 32);
+  v >>= sh;
+  if (BITS > 5 && sh > 0) v |= (uint64_t)__ldg(w + 2) << (64 - sh);
+  return v;
+}
+
+template <int D, int BITS, bool LO>
+__global__ void __launch_bounds__(Shape<D>::kThreads, 1) read_ragged_tc_kernel(RaggedTc p, int which) {
+  using S = Shape<D>;
+  using SM = ReadSmem<D, BITS, LO>;
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  unsigned char* sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+  const Pipe pp = make_pipe(sm + SM::OFF_PIPE);
+  float* norms = reinterpret_cast<float*>(sm + SM::OFF_N);
+  uint8_t* states = sm + SM::OFF_ST;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int nvec = p.nvec;
+
+  // the V kernel may start beside the K kernel (they share no byte); it ends
+  // after it, so that whatever follows sees both
+  pdl_launch_dependents();
+  if (tid == 0) init_pipe(pp, S::kEpi);
+  if (warp == kMakers) {
+    tc::tmem_alloc(pp.tmem_slot, 2 * D);
+    tc::tmem_relinquish();
+  }
+  stage_rotation<D>(sm + SM::OFF_B, p.rot, which, tid, S::kThreads);
+  {
+    const float* cent = p.cent[which];
+    constexpr uint32_t mask = (1u << BITS) - 1u;
+    for (int i = tid; i < SM::LUT_BYTES / 16; i += S::kThreads) {
+      const uint32_t e = (uint32_t)i >> 3;
+      uint32_t h, l;
+      if (SM::kPair) {
+        split_pair(__ldg(cent + (e & mask)), __ldg(cent + (e >> BITS)), h, l);
+      } else {
+        split_pair(__ldg(cent + e), 0.f, h, l);            // low halves: hi, lo of one code
+        h = (h & 0xFFFFu) | (l << 16);
+      }
+      const uint4 x = SM::kPair && LO ? make_uint4(h, l, h, l) : make_uint4(h, h, h, h);
+      reinterpret_cast<uint4*>(sm + SM::OFF_LUT)[i] = x;
+    }
+  }
+  tc::fence_proxy_async_smem();
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = *pp.tmem_slot;
+  const int first = blockIdx.x, step = gridDim.x;
+  const int row_bytes = D * BITS / 8;
+  const int sec = which == 0 ? p.g.off_k : p.g.off_v, noff = which == 0 ? p.g.off_kn : p.g.off_vn;
+
+  if (warp < kMakers) {
+    // ------------------------------------------------------------ operand makers
+    constexpr int RPI = 32 / S::kLanes, NIT = 16 / RPI;
+    const int l = lane % S::kLanes, sub = lane / S::kLanes;
+    const unsigned char* lut = sm + SM::OFF_LUT + (SM::kPair && LO ? 8 * (lane & 15) : 4 * lane);
+    int it = 0;
+    for (int tile = first; tile < p.ntiles; tile += step, ++it) {
+      const int st = it % SM::STAGES;
+      int trow;
+      const Vec place = find_vector(p, tile * kM + 16 * warp + lane, nvec, lane, trow);
+      const unsigned long long mine = reinterpret_cast<unsigned long long>(
+          place.page ? place.page + sec + place.slot * row_bytes : nullptr);
+      const float n = place.page ? __half2float(__ldg(reinterpret_cast<const __half*>(
+                                       place.page + noff) + place.slot)) : 0.f;
+      uint64_t codes[NIT];
+#pragma unroll
+      for (int k = 0; k < NIT; ++k) {
+        const uint8_t* row = reinterpret_cast<const uint8_t*>(
+            __shfl_sync(0xffffffffu, mine, k * RPI + sub));
+        codes[k] = row ? load_chunk<BITS>(row, l) : 0;
+      }
+      bool ok = it < SM::STAGES ||
+                wait_for(&pp.a_empty[st], (uint32_t)(((it / SM::STAGES) - 1) & 1), pp.abort_flag,
+                         p.status);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      if (lane < 16) {
+        const int at = (it % SM::RING) * kM + 16 * warp + lane;
+        norms[at] = n;
+        states[at] = (uint8_t)place.state;
+      }
+      unsigned char* hi = sm + SM::OFF_A + st * S::kTerm;
+#pragma unroll
+      for (int k = 0; k < NIT; ++k) {
+        const int r = 16 * warp + k * RPI + sub;
+        uint32_t h[4], lo[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (SM::kPair) {
+            const uint32_t idx = (uint32_t)(codes[k] >> (2 * BITS * e)) & ((1u << (2 * BITS)) - 1u);
+            if constexpr (LO) {
+              const uint2 x = *reinterpret_cast<const uint2*>(lut + idx * 128);
+              h[e] = x.x;
+              lo[e] = x.y;
+            } else {
+              h[e] = *reinterpret_cast<const uint32_t*>(lut + idx * 128);
+            }
+          } else {
+            const uint32_t i0 = (uint32_t)(codes[k] >> (2 * BITS * e)) & ((1u << BITS) - 1u);
+            const uint32_t i1 = (uint32_t)(codes[k] >> (2 * BITS * e + BITS)) & ((1u << BITS) - 1u);
+            const uint32_t a = *reinterpret_cast<const uint32_t*>(lut + i0 * 128);
+            const uint32_t b = *reinterpret_cast<const uint32_t*>(lut + i1 * 128);
+            h[e] = __byte_perm(a, b, 0x5410);
+            lo[e] = __byte_perm(a, b, 0x7632);
+          }
+        }
+        const uint32_t at = chunk_at<kM>(r, l);
+        *reinterpret_cast<uint4*>(hi + at) = make_uint4(h[0], h[1], h[2], h[3]);
+        if (LO)
+          *reinterpret_cast<uint4*>(hi + S::kTerm + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive_cta(&pp.a_full[st]);
+    }
+  } else if (warp == kMakers) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      const uint32_t a0 = smem_u32(sm + SM::OFF_A), b0 = smem_u32(sm + SM::OFF_B);
+      issue_tiles<D, SM::STAGES, true>(pp, tmem, first, step, p.ntiles, p.status,
+                                       [&](int st, int term, uint32_t& a, uint32_t& b) {
+                                         a = a0 + st * S::kTerm + (term == 2 ? S::kTerm : 0);
+                                         b = b0 + (term == 1 ? S::kB : 0);
+                                         return term < (LO ? 3 : 2);
+                                       });
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ epilogue
+    const int q = warp & 3, part = (warp - kMakers - 1) >> 2;
+    const int dtype = p.dtype[which];
+    const int es = dtype == TQ_F32 ? 4 : 2;
+    const int64_t* xs = p.stride[which];
+    unsigned char* out = sm + SM::OFF_OUT;
+    // 16-byte piece c of row r, rotated so that rows and pieces spread over the banks
+    const int pieces = D * es / 16;
+    auto piece = [&](int r, int c) { return out + r * (D * es) + ((c ^ (r & 7)) << 4); };
+    int it = 0;
+    for (int tile = first; tile < p.ntiles; tile += step, ++it) {
+      const int ac = it & 1;
+      bool ok = wait_for(&pp.acc_full[ac], (uint32_t)((it / 2) & 1), pp.abort_flag, p.status);
+      if (!__all_sync(0xffffffffu, ok)) ok = false;
+      // the lane quarter's warps go on or leave together
+      {
+        uint32_t all;
+        asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n"
+                     " bar.red.and.pred q, %2, %3, p;\n selp.u32 %0, 1, 0, q;\n}"
+                     : "=r"(all) : "r"((uint32_t)ok), "r"(1 + q), "r"(32 * S::kSplit) : "memory");
+        if (!all) {
+          *pp.abort_flag = 1;
+          break;
+        }
+      }
+      tc::tc_fence_after();
+      uint32_t x[32];
+      tc::tmem_ld_x32(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(ac * D + 32 * part), x);
+      const int r = 32 * q + lane, at = (it % SM::RING) * kM + r;
+      const float n = norms[at] * (1.f / kRScale);
+      // this warp's 32 / kSplit rows on the way out
+      constexpr int ROWS = 32 / S::kSplit;
+      const int r0 = 32 * q + ROWS * part;
+      uint32_t state = 0;                                  // of row r0 + lane
+      if (lane < ROWS) state = states[(it % SM::RING) * kM + r0 + lane];
+      tc::tmem_wait_ld();
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive_cta(&pp.acc_empty[ac]);
+      if (dtype == TQ_F32) {
+        if constexpr (LO) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            *reinterpret_cast<float4*>(piece(r, 8 * part + c)) =
+                make_float4(__uint_as_float(x[4 * c]) * n, __uint_as_float(x[4 * c + 1]) * n,
+                            __uint_as_float(x[4 * c + 2]) * n, __uint_as_float(x[4 * c + 3]) * n);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t h[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float a = __uint_as_float(x[8 * c + 2 * e]) * n;
+            const float b = __uint_as_float(x[8 * c + 2 * e + 1]) * n;
+            if (dtype == TQ_F16) {
+              h[e] = pack_half2(a, b);
+            } else {
+              const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+              h[e] = *reinterpret_cast<const uint32_t*>(&v);
+            }
+          }
+          *reinterpret_cast<uint4*>(piece(r, 4 * part + c)) = make_uint4(h[0], h[1], h[2], h[3]);
+        }
+      }
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + q), "r"(32 * S::kSplit) : "memory");
+      const int v0 = tile * kM + r0;
+      if (p.vec[which]) {
+        for (int i = lane; i < ROWS * pieces; i += 32) {
+          const int rr = i / pieces, c = i % pieces;
+          const uint32_t stt = __shfl_sync(0xffffffffu, state, rr);
+          const int v = v0 + rr;
+          if (stt == 0 || v >= nvec) continue;
+          const int64_t o = (int64_t)(v / p.H) * xs[1] + (int64_t)(v % p.H) * xs[0];
+          uint4 y = *reinterpret_cast<const uint4*>(piece(r0 + rr, c));
+          if (stt == 1) y = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(static_cast<char*>(const_cast<void*>(p.x[which])) + o * es + 16 * c) = y;
+        }
+      } else {
+        for (int i = lane; i < ROWS * D; i += 32) {
+          const int rr = i / D, d = i % D;
+          const uint32_t stt = __shfl_sync(0xffffffffu, state, rr);
+          const int v = v0 + rr;
+          if (stt == 0 || v >= nvec) continue;
+          const unsigned char* src = piece(r0 + rr, d * es / 16) + (d * es) % 16;
+          const int64_t o = (int64_t)(v / p.H) * xs[1] + (int64_t)(v % p.H) * xs[0] + d * xs[2];
+          char* dst = static_cast<char*>(const_cast<void*>(p.x[which])) + o * es;
+          if (es == 4) *reinterpret_cast<uint32_t*>(dst) = stt == 1 ? 0u : *reinterpret_cast<const uint32_t*>(src);
+          else *reinterpret_cast<uint16_t*>(dst) = stt == 1 ? (uint16_t)0 : *reinterpret_cast<const uint16_t*>(src);
+        }
+      }
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + q), "r"(32 * S::kSplit) : "memory");
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == kMakers) {
+    __syncwarp();
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, 2 * D);
+  }
+  pdl_wait();
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+using RaggedFn = void (*)(RaggedTc, int);
+
+template <int D>
+RaggedFn append_fn(int bits) {
+  switch (bits) {
+    case 1: return append_ragged_tc_kernel<D, 1>;
+    case 2: return append_ragged_tc_kernel<D, 2>;
+    case 3: return append_ragged_tc_kernel<D, 3>;
+    case 4: return append_ragged_tc_kernel<D, 4>;
+    case 5: return append_ragged_tc_kernel<D, 5>;
+    case 6: return append_ragged_tc_kernel<D, 6>;
+    case 7: return append_ragged_tc_kernel<D, 7>;
+    default: return append_ragged_tc_kernel<D, 8>;
+  }
+}
+
+template <int D, bool LO>
+RaggedFn read_fn(int bits, int& bytes) {
+#define TQ_RD(B) case B: bytes = ReadSmem<D, B, LO>::BYTES; return read_ragged_tc_kernel<D, B, LO>;
+  switch (bits) { TQ_RD(1) TQ_RD(2) TQ_RD(3) TQ_RD(4) TQ_RD(5) TQ_RD(6) TQ_RD(7) TQ_RD(8) }
+#undef TQ_RD
+  return nullptr;
+}
+
+RaggedTc tc_params(const tq_geom* G, const tq_tables* t, const tq_cache* c,
+                   const tq_tensor4* const x[2], const tq_ragged* batch, uint32_t* status) {
+  RaggedTc p = {};
+  p.g = make_geom(G->head_dim, G->key_bits, G->value_bits, G->qjl);
+  p.cent[0] = t->k_centroids; p.cent[1] = t->v_centroids;
+  p.bnd[0] = t->k_boundaries; p.bnd[1] = t->v_boundaries;
+  p.rot = t->rot;
+  p.pages = c->pages;
+  p.pm = page_map(c);
+  p.status = status;
+  for (int w = 0; w < 2; ++w) {
+    if (!x[w]) continue;
+    p.x[w] = x[w]->data;
+    p.dtype[w] = x[w]->dtype;
+    for (int i = 0; i < 3; ++i) p.stride[w][i] = x[w]->stride[i + 1];
+    p.H = (int)x[w]->shape[1];
+    p.rv = ragged_view(batch, x[w]->shape[2], c);
+  }
+  p.nvec = (int)(p.rv.N * p.H);
+  p.ntiles = (p.nvec + kM - 1) / kM;
+  return p;
+}
+
+// `beside`: may start before the previous launch (the K kernel) has ended.
+int launch_one(RaggedFn fn, unsigned grid, int threads, int bytes, cudaStream_t st,
+               const RaggedTc& p, int which, bool beside, const char* what) {
+  if (beside) return launch_result(launch_pdl(fn, dim3(grid), dim3(threads), bytes, st, p, which), what);
+  fn<<<grid, threads, bytes, st>>>(p, which);
+  return check_launch(what);
+}
+
+// Rows that take loads (stores) of four values (16 bytes).
+bool rows_aligned(const tq_tensor4* x, int bytes) {
+  const int es = x->dtype == TQ_F32 ? 4 : 2;
+  if (x->stride[3] != 1 || reinterpret_cast<uintptr_t>(x->data) % bytes) return false;
+  for (int i = 1; i < 3; ++i)
+    if (x->shape[i] > 1 && (x->stride[i] * es) % bytes) return false;
+  return true;
+}
+
+}  // namespace
+
+// Both return TQ_OK when they ran, 1 when they do not apply, or an error.
+int launch_append_ragged_tc(const tq_geom* G, const tq_tables* t, const tq_cache* c,
+                            const tq_tensor4* k, const tq_tensor4* v, const tq_ragged* batch,
+                            const tq_rope* rope, const tq_head_norm* norm, const tq_positions* pos,
+                            uint32_t* status, cudaStream_t st) {
+  const int D = G->head_dim;
+  if (D != 64 && D != 128) return 1;
+  if (k->shape[1] * k->shape[2] > INT32_MAX - kM || (rope && rope->rot_dim % 8)) return 1;
+  if (reinterpret_cast<uintptr_t>(t->rot) % 16) return 1;
+  const tq_tensor4* x[2] = {k, v};
+  for (int w = 0; w < 2; ++w)
+    if (!rows_aligned(x[w], x[w]->dtype == TQ_F32 ? 16 : 8)) return 1;
+  RaggedTc p = tc_params(G, t, c, x, batch, status);
+  p.f = head_xform(rope, norm);
+  p.pos = pos ? pos->data : nullptr;
+  p.pos64 = pos && pos->bits == 64;
+  p.pos_stride = pos ? pos->stride[1] : 0;
+  p.use_lo[0] = rope || norm || k->dtype == TQ_F32;
+  p.use_lo[1] = v->dtype == TQ_F32;
+  const unsigned grid = (unsigned)tmin(p.ntiles, device_sm_count());
+  for (int w = 0; w < 2; ++w) {
+    const int bits = w == 0 ? G->key_bits : G->value_bits;
+    RaggedFn fn = D == 128 ? append_fn<128>(bits) : append_fn<64>(bits);
+    if (set_smem_attr((const void*)fn, kSmem) != TQ_OK) return TQ_ERR_CUDA;
+    const int threads = D == 128 ? Shape<128>::kThreads : Shape<64>::kThreads;
+    if (const int rc = launch_one(fn, grid, threads, kSmem, st, p, w, w == 1, "tq_append_ragged"))
+      return rc;
+  }
+  return TQ_OK;
+}
+
+int launch_dequant_ragged_tc(const tq_geom* G, const tq_tables* t, const tq_cache* c,
+                             const tq_ragged* batch, const tq_tensor4* ko, const tq_tensor4* vo,
+                             uint32_t* status, cudaStream_t st) {
+  const int D = G->head_dim;
+  const tq_tensor4* x[2] = {ko, vo};
+  const tq_tensor4* one = ko ? ko : vo;
+  if (D != 64 && D != 128) return 1;
+  if (one->shape[1] * one->shape[2] > INT32_MAX - kM) return 1;
+  if (reinterpret_cast<uintptr_t>(t->rot) % 16) return 1;
+  RaggedTc p = tc_params(G, t, c, x, batch, status);
+  const unsigned grid = (unsigned)tmin(p.ntiles, device_sm_count());
+  for (int w = 0; w < 2; ++w) {
+    if (!x[w]) continue;
+    p.vec[w] = rows_aligned(x[w], 16);
+    const int bits = w == 0 ? G->key_bits : G->value_bits;
+    int bytes = 0;
+    const bool lo = x[w]->dtype != TQ_BF16;
+    RaggedFn fn = D == 128 ? (lo ? read_fn<128, true>(bits, bytes) : read_fn<128, false>(bits, bytes))
+                           : (lo ? read_fn<64, true>(bits, bytes) : read_fn<64, false>(bits, bytes));
+    if (set_smem_attr((const void*)fn, bytes) != TQ_OK) return TQ_ERR_CUDA;
+    const int threads = D == 128 ? Shape<128>::kThreads : Shape<64>::kThreads;
+    if (const int rc = launch_one(fn, grid, threads, bytes, st, p, w, w == 1 && ko,
+                                  "tq_dequantize_ragged"))
+      return rc;
+  }
+  return TQ_OK;
+}
+
+}  // namespace tq
