@@ -6,14 +6,16 @@
 // so the heads of a token share its row of the rotation table and a tile is
 // contiguous in memory), M of one tcgen05.mma with N = K = head_dim.  One
 // persistent CTA per SM, a launch each for K and V, three roles:
-//   warps 0-7   operand makers: 16 vectors each.  Append: load, norm, rotate,
-//               norm again, split into fp16; read-back: codes -> centroids
-//               through lane-replicated tables.  They also find each vector's
-//               request, position and page.
-//   warp 8      one thread issues the MMAs into one of two accumulators
-//   warps 9-    epilogue, one thread per vector and 32 columns.  Append:
-//               bucketize and pack; read-back: times the norm, out through
-//               shared memory so that rows leave in whole lines
+//   makers      operand of the next tile.  Append (16 warps): load, norm,
+//               rotate, norm again, split into fp16; read-back (8 warps): codes
+//               -> centroids through lane-replicated tables.  They also find
+//               each vector's request, position and page, and fetch one tile
+//               ahead of what they make.
+//   issuer      one thread issues the MMAs into one of two accumulators
+//   epilogue    one thread per vector and 32 columns at a time.  Append (8
+//               warps): bucketize and pack; read-back (4 per 32 columns): times
+//               the norm, out through shared memory so that rows leave in
+//               whole lines
 //
 // Append: y n s 2^6 = (x s) (2^6 R)^T with s the power of two that puts ||x||
 // into [2^10, 2^11), x s = hi + lo and 2^6 R = hi + lo in fp16 (22 bits, the
@@ -41,12 +43,12 @@
 #include "tq_tc.cuh"
 
 #include <limits.h>
+#include <type_traits>
 
 namespace tq {
 namespace {
 
 constexpr int kM = 128;                    // vectors per tile
-constexpr int kMakers = 8;                 // maker warps, 16 vectors each
 constexpr int kRing = 4;                   // tiles of per-vector data in flight
 constexpr int kSmem = 227 * 1024;
 constexpr float kCmp = 1.2676506e30f;      // 2^100
@@ -71,14 +73,22 @@ struct RaggedTc {
   const void* pos; int pos64; int64_t pos_stride;
 };
 
+// MAKERS maker warps (kM / MAKERS vectors each), the issuing warp, SPLIT
+// epilogue warps per lane quarter of tensor memory.
+template <int D, int MAKERS, int SPLIT>
+struct Roles {
+  static constexpr int kMakers = MAKERS, kVecs = kM / MAKERS, kSplit = SPLIT, kEpi = 4 * SPLIT;
+  static constexpr int kThreads = 32 * (MAKERS + 1 + kEpi);
+};
+// Making an append operand (norms, rotation, split) takes twice its epilogue's
+// instructions, a read-back operand half of it.
+template <int D> using AppendRoles = Roles<D, 16, 2>;
+template <int D> using ReadRoles = Roles<D, 8, D / 32>;
+
 template <int D>
 struct Shape {
-  static constexpr int kSplit = D / 32;                    // epilogue warps per lane quarter
-  static constexpr int kEpi = 4 * kSplit;
-  static constexpr int kThreads = 32 * (kMakers + 1 + kEpi);
   static constexpr int kTerm = kM * D * 2;                 // one fp16 operand tile
   static constexpr int kB = D * D * 2;                     // one term of R
-  static constexpr int kLanes = D / 8;                     // lanes per vector (8 values each)
 };
 
 // Byte offset of 16-byte chunk c of row r: [64-column half][rows][128 B], swizzled.
@@ -92,18 +102,17 @@ __device__ __forceinline__ void expired(uint32_t* status, volatile int* abort_fl
   atomicOr(status, TQ_DEV_WAIT_TIMEOUT);
 }
 
-// Bounded wait (2 s) that also ends once another role has given up.
+// Bounded wait (2 s) that also ends once another role has given up.  Suspended
+// for up to 20 us at a time: polling warps took half of the issue slots.
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
                                          uint32_t* status) {
   uint64_t t0 = 0;
-  for (uint32_t i = 0;; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 63u) == 63u) {
-      if (*abort_flag) return false;
-      const uint64_t t = global_ns();
-      if (t0 == 0) t0 = t;
-      else if (t - t0 > 2000000000ull) break;
-    }
+  while (true) {
+    if (mbar_try_wait_hint(bar, parity, 20000u)) return true;
+    if (*abort_flag) return false;
+    const uint64_t t = global_ns();
+    if (t0 == 0) t0 = t;
+    else if (t - t0 > 2000000000ull) break;
   }
   expired(status, abort_flag);
   return false;
@@ -143,15 +152,14 @@ struct Vec {
   int state;                               // 0: row of no request, 1: no place, 2: stored
 };
 
-// Lane i < 16 of a maker warp finds vector v0 + i; `row`: its row of the
-// rotation table.
-__device__ __forceinline__ Vec find_vector(const RaggedTc& p, int i, int nvec, int lane, int& row) {
+// A maker warp's lane finds vector i; `row`: its row of the rotation table.
+__device__ __forceinline__ Vec find_vector(const RaggedTc& p, int i, int nvec, bool mine, int& row) {
   Vec v;
   v.page = nullptr;
   v.n = v.inv = 0.f;
   v.slot = v.state = 0;
   row = 0;
-  if (lane >= 16 || i >= nvec) return v;
+  if (!mine || i >= nvec) return v;
   const int n = i / p.H, h = i % p.H;
   const int64_t r = request_of(p.rv, n);
   if (r < 0) return v;
@@ -203,9 +211,9 @@ __device__ __forceinline__ Pipe make_pipe(unsigned char* at) {
 }
 constexpr int kPipeBytes = 128;
 
-__device__ __forceinline__ void init_pipe(const Pipe& p, int epi_warps) {
+__device__ __forceinline__ void init_pipe(const Pipe& p, int makers, int epi_warps) {
   for (int i = 0; i < 2; ++i) {
-    mbar_init(&p.a_full[i], kMakers);
+    mbar_init(&p.a_full[i], makers);
     mbar_init(&p.a_empty[i], 1);
     mbar_init(&p.acc_full[i], 1);
     mbar_init(&p.acc_empty[i], epi_warps);
@@ -291,8 +299,11 @@ __device__ __forceinline__ float sum_lanes(float x) {
 }
 
 template <int D, int BITS>
-__global__ void __launch_bounds__(Shape<D>::kThreads, 1) append_ragged_tc_kernel(RaggedTc p, int which) {
+__global__ void __launch_bounds__(AppendRoles<D>::kThreads, 1)
+append_ragged_tc_kernel(RaggedTc p, int which) {
   using S = Shape<D>;
+  using W = AppendRoles<D>;
+  constexpr int kMakers = W::kMakers, kThreads = W::kThreads;
   using SM = AppendSmem<D>;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -308,31 +319,35 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) append_ragged_tc_kernel
   // the V kernel may start beside the K kernel (they share no byte); it ends
   // after it, so that whatever follows sees both
   pdl_launch_dependents();
-  if (tid == 0) init_pipe(pp, S::kEpi);
+  if (tid == 0) init_pipe(pp, kMakers, W::kEpi);
   if (warp == kMakers) {
     tc::tmem_alloc(pp.tmem_slot, 2 * D);
     tc::tmem_relinquish();
   }
-  for (int i = tid; i < nb; i += S::kThreads) bnd[i] = p.bnd[which][i];
-  stage_rotation<D>(sm + SM::OFF_B, p.rot, which, tid, S::kThreads);
+  for (int i = tid; i < nb; i += kThreads) bnd[i] = p.bnd[which][i];
+  stage_rotation<D>(sm + SM::OFF_B, p.rot, which, tid, kThreads);
   __syncthreads();
-  if (tid == 0) {
+  if (warp == 0) {
     float gap = 1.f;
-    for (int i = 0; i + 1 < nb; ++i) gap = fminf(gap, bnd[i + 1] - bnd[i]);
+    for (int i = lane; i + 1 < nb; i += 32) gap = fminf(gap, bnd[i + 1] - bnd[i]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) gap = fminf(gap, __shfl_xor_sync(0xffffffffu, gap, o));
     const float w = 0.4f * gap;
     const float span = fmaxf(fabsf(bnd[0]), fabsf(bnd[nb - 1]));
     const float L = ceilf(span / w) + 3.f, nc = 2.f * L + 1.f;
     const bool ok = w > 0.f && nc * 128.f <= (float)SM::LUT_BYTES && span < 1.f;
-    lutpar[0] = 1.f / (2.f * L * w);       // u = sat(v * lutpar[0] + 0.5)
-    lutpar[1] = 2.f * L;                   // cell = round(u * 2L)
-    lutpar[2] = ok ? nc : 0.f;
-    lutpar[3] = w;
+    if (lane == 0) {
+      lutpar[0] = 1.f / (2.f * L * w);     // u = sat(v * lutpar[0] + 0.5)
+      lutpar[1] = 2.f * L;                 // cell = round(u * 2L)
+      lutpar[2] = ok ? nc : 0.f;
+      lutpar[3] = w;
+    }
   }
   __syncthreads();
   const int ncells = (int)lutpar[2];
   {
     const float w = lutpar[3], L = 0.5f * lutpar[1];
-    for (int i = tid; i < ncells * 16; i += S::kThreads) {
+    for (int i = tid; i < ncells * 16; i += kThreads) {
       const int c = i >> 4;
       const float wl = ((float)c - L - 1.f) * w, wh = ((float)c - L + 1.f) * w;
       const int base = bucketize_lt(bnd, nb, wl);
@@ -350,109 +365,112 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) append_ragged_tc_kernel
 
   if (warp < kMakers) {
     // ------------------------------------------------------------ operand makers
-    constexpr int RPI = 32 / S::kLanes, NIT = 16 / RPI;    // vectors per pass, passes
-    const int l = lane % S::kLanes, sub = lane / S::kLanes;
+    // D / 16 lanes per vector, two groups of eight dims each
+    constexpr int LV = D / 16, RPI = 32 / LV, NIT = W::kVecs / RPI;   // vectors per pass, passes
+    static_assert(NIT >= 1, "a warp's vectors fill its lanes");
+    const int l = lane % LV, sub = lane / LV;
     const HeadXform f = which == 0 ? p.f : HeadXform{};
-    // the lane's two groups of four dims: partners of the rotation (halves), or
-    // plain halves of the vector
+    // the groups: partners of the rotation (halves), or plain halves of the vector
     const int half = f.rot / 2;
     const bool pairs = f.cos_sin && !f.interleaved;        // (i, half + i)
-    int ga = 4 * l, gb = D / 2 + 4 * l;
+    int ga = 8 * l, gb = D / 2 + 8 * l;
     bool turn = f.cos_sin != nullptr;                      // this lane rotates
     if (pairs) {
-      if (4 * l < half) { gb = half + 4 * l; }
-      else { ga = f.rot + 2 * (4 * l - half); gb = ga + 4; turn = false; }
+      if (ga < half) { gb = half + ga; }
+      else { ga = f.rot + 2 * (8 * l - half); gb = ga + 8; turn = false; }
     }
     const bool turn_a = turn && (pairs || ga < f.rot), turn_b = turn && !pairs && gb < f.rot;
-    float w[8];
-    if (f.weight) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        w[e] = load_elem(f.weight, f.w_dtype, e < 4 ? ga + e : gb + e - 4) + f.w_offset;
-    }
     const int64_t* xs = p.stride[which];
-    int it = 0;
-    for (int tile = first; tile < p.ntiles; tile += step, ++it) {
-      const int st = it & 1;
-      Vec* vec = ring + (it % kRing) * kM + 16 * warp;
-      const int v0 = tile * kM + 16 * warp;
-      // every vector's 16-bit values in flight while its place is found (32-bit
-      // ones would take twice the registers: loaded when they are used)
-      const bool wide = p.dtype[which] == TQ_F32;
-      auto base_of = [&](int i) {
-        return (int64_t)(i / p.H) * xs[1] + (int64_t)(i % p.H) * xs[0];
-      };
-      uint2 xa[NIT], xb[NIT];
+    const int dtype = p.dtype[which];
+    const bool wide = dtype == TQ_F32;
+    // 16-bit values of a tile's vectors (32-bit ones would take twice the
+    // registers: loaded when they are used)
+    struct Raw { uint4 a[NIT], b[NIT]; };
+    auto base_of = [&](int i) {
+      return (int64_t)(i / p.H) * xs[1] + (int64_t)(i % p.H) * xs[0];
+    };
+    auto load_raw = [&](Raw& x, int v0) {
 #pragma unroll
       for (int k = 0; k < NIT; ++k) {
         const int i = v0 + k * RPI + sub;
-        xa[k] = xb[k] = make_uint2(0u, 0u);
+        x.a[k] = x.b[k] = make_uint4(0u, 0u, 0u, 0u);
         if (!wide && i < nvec) {
-          const uint16_t* x = static_cast<const uint16_t*>(p.x[which]) + base_of(i);
-          xa[k] = __ldg(reinterpret_cast<const uint2*>(x + ga));
-          xb[k] = __ldg(reinterpret_cast<const uint2*>(x + gb));
+          const uint16_t* at = static_cast<const uint16_t*>(p.x[which]) + base_of(i);
+          x.a[k] = __ldg(reinterpret_cast<const uint4*>(at + ga));
+          x.b[k] = __ldg(reinterpret_cast<const uint4*>(at + gb));
         }
       }
-      int trow;
-      const Vec place = find_vector(p, v0 + lane, nvec, lane, trow);
+    };
+    auto vec0 = [&](int tile) { return tile * kM + W::kVecs * warp; };
+    auto find = [&](int tile, int& row) {
+      return find_vector(p, vec0(tile) + lane, nvec, lane < W::kVecs, row);
+    };
+    Raw cur, nxt;
+    int trow = 0, trow_next = 0;
+    Vec place = {}, place_next = {};
+    if (first < p.ntiles) {
+      load_raw(cur, vec0(first));
+      place = find(first, trow);
+    }
+    int it = 0;
+    for (int tile = first; tile < p.ntiles; tile += step, ++it) {
+      const int st = it & 1;
+      Vec* vec = ring + (it % kRing) * kM + W::kVecs * warp;
+      const int v0 = vec0(tile);
+      // the next tile's values and places while this one is made
+      if (tile + step < p.ntiles) {
+        load_raw(nxt, vec0(tile + step));
+        place_next = find(tile + step, trow_next);
+        if (f.cos_sin) {
+          // its first and last rows of the rotation table (often all of them)
+          const int r = __shfl_sync(0xffffffffu, trow_next, lane < 16 ? 0 : W::kVecs - 1);
+          const float* at = f.cos_sin + (int64_t)r * f.rot + 32 * (lane & 15);
+          if (32 * (lane & 15) < f.rot) asm volatile("prefetch.global.L1 [%0];" ::"l"(at));
+        }
+      }
       // the stage is free, and with it the ring's entry: its tile's epilogue
       // ran before this stage's last MMAs could start
       bool ok = it < 2 || wait_for(&pp.a_empty[st], (uint32_t)(((it / 2) - 1) & 1), pp.abort_flag,
                                    p.status);
       if (!__all_sync(0xffffffffu, ok)) break;
-      if (lane < 16) vec[lane] = place;
+      if (lane < W::kVecs) vec[lane] = place;
       __syncwarp();
       unsigned char* hi = sm + SM::OFF_A + st * 2 * S::kTerm;
-      int last_row = -1;
-      float4 ca = make_float4(0.f, 0.f, 0.f, 0.f), sa = ca, cb = ca;
 #pragma unroll
       for (int k = 0; k < NIT; ++k) {
-        const int vi = k * RPI + sub;                      // vector of the warp's 16
-        float v[8];
+        const int vi = k * RPI + sub;                      // vector of the warp's
+        float v[16];
         if (wide) {
-          float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-          if (v0 + vi < nvec) {
-            const float* x = static_cast<const float*>(p.x[which]) + base_of(v0 + vi);
-            a = __ldg(reinterpret_cast<const float4*>(x + ga));
-            b = __ldg(reinterpret_cast<const float4*>(x + gb));
+          const bool in = v0 + vi < nvec;
+          const float* x = static_cast<const float*>(p.x[which]) + base_of(in ? v0 + vi : 0);
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            const float4 y = __ldg(reinterpret_cast<const float4*>(x + (e < 8 ? ga + e : gb + e - 8)));
+            v[e] = in ? y.x : 0.f;
+            v[e + 1] = in ? y.y : 0.f;
+            v[e + 2] = in ? y.z : 0.f;
+            v[e + 3] = in ? y.w : 0.f;
           }
-          v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-          v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
         } else {
-          widen4(xa[k], p.dtype[which], v);
-          widen4(xb[k], p.dtype[which], v + 4);
+          widen4(make_uint2(cur.a[k].x, cur.a[k].y), dtype, v);
+          widen4(make_uint2(cur.a[k].z, cur.a[k].w), dtype, v + 4);
+          widen4(make_uint2(cur.b[k].x, cur.b[k].y), dtype, v + 8);
+          widen4(make_uint2(cur.b[k].z, cur.b[k].w), dtype, v + 12);
         }
         if (f.weight) {
           float ss = 0.f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) ss = fmaf(v[e], v[e], ss);
-          const float r = 1.f / sqrtf(sum_lanes<S::kLanes>(ss) / (float)D + f.eps);
+          for (int e = 0; e < 16; ++e) ss = fmaf(v[e], v[e], ss);
+          const float r = 1.f / sqrtf(sum_lanes<LV>(ss) / (float)D + f.eps);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = v[e] * r * w[e];
+          for (int e = 0; e < 16; ++e) {
+            const float w = load_elem(f.weight, f.w_dtype, e < 8 ? ga + e : gb + e - 8) + f.w_offset;
+            v[e] = v[e] * r * w;
+          }
         }
         if (f.cos_sin) {
           const int row = __shfl_sync(0xffffffffu, trow, vi);
-          if (row != last_row) {                           // heads of one token share it
-            last_row = row;
-            const float* cs = f.cos_sin + (int64_t)row * f.rot;
-            if (pairs) {
-              if (turn_a) {
-                ca = __ldg(reinterpret_cast<const float4*>(cs + ga));
-                sa = __ldg(reinterpret_cast<const float4*>(cs + half + ga));
-              }
-            } else {
-              if (turn_a) {
-                const float2 c = __ldg(reinterpret_cast<const float2*>(cs + ga / 2));
-                const float2 s = __ldg(reinterpret_cast<const float2*>(cs + half + ga / 2));
-                ca = make_float4(c.x, c.y, s.x, s.y);
-              }
-              if (turn_b) {
-                const float2 c = __ldg(reinterpret_cast<const float2*>(cs + gb / 2));
-                const float2 s = __ldg(reinterpret_cast<const float2*>(cs + half + gb / 2));
-                cb = make_float4(c.x, c.y, s.x, s.y);
-              }
-            }
-          }
+          const float* cs = f.cos_sin + (int64_t)row * f.rot;
           auto rotate = [](float& a, float& b, float c, float s) {
             const float t = a * c - b * s;
             b = b * c + a * s;
@@ -460,43 +478,60 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) append_ragged_tc_kernel
           };
           if (pairs) {
             if (turn_a) {
-              rotate(v[0], v[4], ca.x, sa.x);
-              rotate(v[1], v[5], ca.y, sa.y);
-              rotate(v[2], v[6], ca.z, sa.z);
-              rotate(v[3], v[7], ca.w, sa.w);
+#pragma unroll
+              for (int e = 0; e < 8; e += 4) {
+                const float4 c = __ldg(reinterpret_cast<const float4*>(cs + ga + e));
+                const float4 s = __ldg(reinterpret_cast<const float4*>(cs + half + ga + e));
+                rotate(v[e], v[8 + e], c.x, s.x);
+                rotate(v[e + 1], v[9 + e], c.y, s.y);
+                rotate(v[e + 2], v[10 + e], c.z, s.z);
+                rotate(v[e + 3], v[11 + e], c.w, s.w);
+              }
             }
           } else {
-            if (turn_a) { rotate(v[0], v[1], ca.x, ca.z); rotate(v[2], v[3], ca.y, ca.w); }
-            if (turn_b) { rotate(v[4], v[5], cb.x, cb.z); rotate(v[6], v[7], cb.y, cb.w); }
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              if (g ? turn_b : turn_a) {
+                const int at = (g ? gb : ga) / 2;
+                const float4 c = __ldg(reinterpret_cast<const float4*>(cs + at));
+                const float4 s = __ldg(reinterpret_cast<const float4*>(cs + half + at));
+                rotate(v[8 * g], v[8 * g + 1], c.x, s.x);
+                rotate(v[8 * g + 2], v[8 * g + 3], c.y, s.y);
+                rotate(v[8 * g + 4], v[8 * g + 5], c.z, s.z);
+                rotate(v[8 * g + 6], v[8 * g + 7], c.w, s.w);
+              }
+            }
           }
         }
         float ss = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(v[e], v[e], ss);
-        const float n = sqrtf(sum_lanes<S::kLanes>(ss));
-        // 2^(10 - exponent of n), from 2^-117 to 2^100
+        for (int e = 0; e < 16; ++e) ss = fmaf(v[e], v[e], ss);
+        const float n = sqrtf(sum_lanes<LV>(ss));
+        // 2^(10 - exponent of n), from 2^-118 to 2^100
         const int ex = (int)((__float_as_uint(n) >> 23) & 255u) - 127;
         const float s = __uint_as_float((uint32_t)(127 + 10 - max(ex, -90)) << 23);
         if (l == 0) {
           vec[vi].n = n;
           vec[vi].inv = 1.f / (s * fmaxf(n, 1e-8f) * kRScale);
         }
-        const int r = 16 * warp + vi;
-        uint32_t h[4], lo[4];
+        const int r = W::kVecs * warp + vi;
+        const uint32_t aa = chunk_at<kM>(r, ga >> 3), ab = chunk_at<kM>(r, gb >> 3);
+        uint32_t h[8], lo[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) split_pair(v[2 * e] * s, v[2 * e + 1] * s, h[e], lo[e]);
-        const uint32_t aa = chunk_at<kM>(r, ga >> 3) + ((ga & 4) << 1);
-        const uint32_t ab = chunk_at<kM>(r, gb >> 3) + ((gb & 4) << 1);
-        *reinterpret_cast<uint2*>(hi + aa) = make_uint2(h[0], h[1]);
-        *reinterpret_cast<uint2*>(hi + ab) = make_uint2(h[2], h[3]);
+        for (int e = 0; e < 8; ++e) split_pair(v[2 * e] * s, v[2 * e + 1] * s, h[e], lo[e]);
+        *reinterpret_cast<uint4*>(hi + aa) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(hi + ab) = make_uint4(h[4], h[5], h[6], h[7]);
         if (use_lo) {
-          *reinterpret_cast<uint2*>(hi + S::kTerm + aa) = make_uint2(lo[0], lo[1]);
-          *reinterpret_cast<uint2*>(hi + S::kTerm + ab) = make_uint2(lo[2], lo[3]);
+          *reinterpret_cast<uint4*>(hi + S::kTerm + aa) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          *reinterpret_cast<uint4*>(hi + S::kTerm + ab) = make_uint4(lo[4], lo[5], lo[6], lo[7]);
         }
       }
       tc::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive_cta(&pp.a_full[st]);
+      cur = nxt;
+      place = place_next;
+      trow = trow_next;
     }
   } else if (warp == kMakers) {
     // ------------------------------------------------------------ MMA issuer
@@ -512,6 +547,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) append_ragged_tc_kernel
     __syncwarp();
   } else {
     // ------------------------------------------------------------ epilogue
+    constexpr int NCH = D / W::kSplit / 32;                // runs of 32 columns per thread
     const int q = warp & 3, part = (warp - kMakers - 1) >> 2;
     const int r = 32 * q + lane;
     const int row_bytes = D * BITS / 8;
@@ -525,71 +561,78 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) append_ragged_tc_kernel
       bool ok = wait_for(&pp.acc_full[ac], (uint32_t)((it / 2) & 1), pp.abort_flag, p.status);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc::tc_fence_after();
-      uint32_t yb[32];
-      tc::tmem_ld_x32(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(ac * D + 32 * part), yb);
       const Vec v = ring[(it % kRing) * kM + r];
-      tc::tmem_wait_ld();
-      tc::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive_cta(&pp.acc_empty[ac]);
-      uint32_t words[BITS];
+      const float ca = v.inv * par0, cK = v.inv * kCmp;
 #pragma unroll
-      for (int x = 0; x < BITS; ++x) words[x] = 0u;
-      if (ncells > 0) {
-        // codes gather in runs of <= 23 bits as acc = 2^23 + field, exactly
-        const float ca = v.inv * par0, cK = v.inv * kCmp;
-        auto flush = [&](float acc, int o, int len) {
-          const uint32_t bits = __float_as_uint(acc) & ((1u << len) - 1u);
-          const int wi = o >> 5, sh = o & 31;
-          words[wi] += bits << sh;
-          if (sh + len > 32) words[wi + 1] += bits >> (32 - sh);
-        };
-        float acc = 8388608.f;
-        int gs = 0, gl = 0;
+      for (int ch = 0; ch < NCH; ++ch) {
+        const int run = part * NCH + ch;                   // 32 positions of the row
+        uint32_t yb[32];
+        tc::tmem_ld_x32(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(ac * D + 32 * run), yb);
+        tc::tmem_wait_ld();
+        if (ch == NCH - 1) {
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive_cta(&pp.acc_empty[ac]);
+        }
+        uint32_t words[BITS];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const int bo = j * BITS;
-          if (gl > 0 && (gl + BITS > 23 || (bo & 31) == 0)) {
-            flush(acc, gs, gl);
-            acc = 8388608.f;
-            gs = bo;
-            gl = 0;
+        for (int x = 0; x < BITS; ++x) words[x] = 0u;
+        if (ncells > 0) {
+          // codes gather in runs of <= 23 bits as acc = 2^23 + field, exactly
+          auto flush = [&](float acc, int o, int len) {
+            const uint32_t bits = __float_as_uint(acc) & ((1u << len) - 1u);
+            const int wi = o >> 5, sh = o & 31;
+            words[wi] += bits << sh;
+            if (sh + len > 32) words[wi + 1] += bits >> (32 - sh);
+          };
+          float acc = 8388608.f;
+          int gs = 0, gl = 0;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const int bo = j * BITS;
+            if (gl > 0 && (gl + BITS > 23 || (bo & 31) == 0)) {
+              flush(acc, gs, gl);
+              acc = 8388608.f;
+              gs = bo;
+              gl = 0;
+            }
+            const float y = __uint_as_float(yb[j]);
+            const float u = __saturatef(fmaf(y, ca, 0.5f));
+            const float cell = fmaf(u, c2l, 8388608.f);
+            const float2 e = tc::lds_f2((__float_as_uint(cell) << 7) + lane_off);
+            const float above = __saturatef(fmaf(y, cK, e.x) * kCmp);
+            acc = fmaf(e.y + above, (float)(1u << gl), acc);
+            gl += BITS;
           }
-          const float y = __uint_as_float(yb[j]);
-          const float u = __saturatef(fmaf(y, ca, 0.5f));
-          const float cell = fmaf(u, c2l, 8388608.f);
-          const float2 e = tc::lds_f2((__float_as_uint(cell) << 7) + lane_off);
-          const float above = __saturatef(fmaf(y, cK, e.x) * kCmp);
-          acc = fmaf(e.y + above, (float)(1u << gl), acc);
-          gl += BITS;
-        }
-        flush(acc, gs, gl);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const uint32_t code = (uint32_t)bucketize_lt(bnd, nb, __uint_as_float(yb[j]) * v.inv);
-          const int bo = j * BITS, wi = bo >> 5, sh = bo & 31;
-          words[wi] += code << sh;
-          if (sh + BITS > 32) words[wi + 1] += code >> (32 - sh);
-        }
-      }
-      if (v.page) {
-        uint8_t* row = v.page + sec + v.slot * row_bytes + part * (4 * BITS);
-        if constexpr (BITS % 4 == 0) {
-#pragma unroll
-          for (int x = 0; x < BITS / 4; ++x)
-            reinterpret_cast<uint4*>(row)[x] = make_uint4(words[4 * x], words[4 * x + 1],
-                                                          words[4 * x + 2], words[4 * x + 3]);
-        } else if constexpr (BITS % 2 == 0) {
-#pragma unroll
-          for (int x = 0; x < BITS / 2; ++x)
-            reinterpret_cast<uint2*>(row)[x] = make_uint2(words[2 * x], words[2 * x + 1]);
+          flush(acc, gs, gl);
         } else {
 #pragma unroll
-          for (int x = 0; x < BITS; ++x) reinterpret_cast<uint32_t*>(row)[x] = words[x];
+          for (int j = 0; j < 32; ++j) {
+            const uint32_t code = (uint32_t)bucketize_lt(bnd, nb, __uint_as_float(yb[j]) * v.inv);
+            const int bo = j * BITS, wi = bo >> 5, sh = bo & 31;
+            words[wi] += code << sh;
+            if (sh + BITS > 32) words[wi + 1] += code >> (32 - sh);
+          }
         }
-        if (part == 0) reinterpret_cast<__half*>(v.page + noff)[v.slot] = __float2half_rn(v.n);
+        if (v.page) {
+          uint8_t* row = v.page + sec + v.slot * row_bytes + run * (4 * BITS);
+          if constexpr (BITS % 4 == 0) {
+#pragma unroll
+            for (int x = 0; x < BITS / 4; ++x)
+              reinterpret_cast<uint4*>(row)[x] = make_uint4(words[4 * x], words[4 * x + 1],
+                                                            words[4 * x + 2], words[4 * x + 3]);
+          } else if constexpr (BITS % 2 == 0) {
+#pragma unroll
+            for (int x = 0; x < BITS / 2; ++x)
+              reinterpret_cast<uint2*>(row)[x] = make_uint2(words[2 * x], words[2 * x + 1]);
+          } else {
+#pragma unroll
+            for (int x = 0; x < BITS; ++x) reinterpret_cast<uint32_t*>(row)[x] = words[x];
+          }
+        }
       }
+      if (v.page && part == 0)
+        reinterpret_cast<__half*>(v.page + noff)[v.slot] = __float2half_rn(v.n);
     }
   }
   tc::tc_fence_before();
@@ -610,6 +653,7 @@ template <int D, int BITS, bool LO>
 struct ReadSmem {
   static constexpr int STAGES = LO ? 1 : 2, RING = STAGES + 2;      // see the makers
   static constexpr bool kPair = BITS <= 4;                         // table of code pairs
+  using Chunk = typename std::conditional<(BITS <= 4), uint32_t, uint64_t>::type;   // 8 codes
   // entry: fp16 pair hi (and lo) of two codes, or one code's {hi, lo}; copies
   // for 32 lanes of 4-byte entries, 16 of 8-byte ones: 128 bytes
   static constexpr int OFF_B = 0;
@@ -642,8 +686,11 @@ __device__ __forceinline__ uint64_t load_chunk(const uint8_t* row, int c) {
 }
 
 template <int D, int BITS, bool LO>
-__global__ void __launch_bounds__(Shape<D>::kThreads, 1) read_ragged_tc_kernel(RaggedTc p, int which) {
+__global__ void __launch_bounds__(ReadRoles<D>::kThreads, 1)
+read_ragged_tc_kernel(RaggedTc p, int which) {
   using S = Shape<D>;
+  using W = ReadRoles<D>;
+  constexpr int kMakers = W::kMakers, kThreads = W::kThreads;
   using SM = ReadSmem<D, BITS, LO>;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -657,16 +704,16 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) read_ragged_tc_kernel(R
   // the V kernel may start beside the K kernel (they share no byte); it ends
   // after it, so that whatever follows sees both
   pdl_launch_dependents();
-  if (tid == 0) init_pipe(pp, S::kEpi);
+  if (tid == 0) init_pipe(pp, kMakers, W::kEpi);
   if (warp == kMakers) {
     tc::tmem_alloc(pp.tmem_slot, 2 * D);
     tc::tmem_relinquish();
   }
-  stage_rotation<D>(sm + SM::OFF_B, p.rot, which, tid, S::kThreads);
+  stage_rotation<D>(sm + SM::OFF_B, p.rot, which, tid, kThreads);
   {
     const float* cent = p.cent[which];
     constexpr uint32_t mask = (1u << BITS) - 1u;
-    for (int i = tid; i < SM::LUT_BYTES / 16; i += S::kThreads) {
+    for (int i = tid; i < SM::LUT_BYTES / 16; i += kThreads) {
       const uint32_t e = (uint32_t)i >> 3;
       uint32_t h, l;
       if (SM::kPair) {
@@ -690,43 +737,52 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) read_ragged_tc_kernel(R
 
   if (warp < kMakers) {
     // ------------------------------------------------------------ operand makers
-    constexpr int RPI = 32 / S::kLanes, NIT = 16 / RPI;
-    const int l = lane % S::kLanes, sub = lane / S::kLanes;
+    // D / 8 lanes per vector, eight codes each
+    constexpr int LV = D / 8, RPI = 32 / LV, NIT = W::kVecs / RPI;
+    const int l = lane % LV, sub = lane / LV;
     const unsigned char* lut = sm + SM::OFF_LUT + (SM::kPair && LO ? 8 * (lane & 15) : 4 * lane);
-    int it = 0;
-    for (int tile = first; tile < p.ntiles; tile += step, ++it) {
-      const int st = it % SM::STAGES;
+    using Chunk = typename SM::Chunk;
+    struct Raw { Chunk codes[NIT]; float n; int state; };
+    auto load_raw = [&](Raw& x, int tile) {
       int trow;
-      const Vec place = find_vector(p, tile * kM + 16 * warp + lane, nvec, lane, trow);
+      const Vec place = find_vector(p, tile * kM + W::kVecs * warp + lane, nvec, lane < W::kVecs, trow);
       const unsigned long long mine = reinterpret_cast<unsigned long long>(
           place.page ? place.page + sec + place.slot * row_bytes : nullptr);
-      const float n = place.page ? __half2float(__ldg(reinterpret_cast<const __half*>(
-                                       place.page + noff) + place.slot)) : 0.f;
-      uint64_t codes[NIT];
+      x.n = place.page ? __half2float(__ldg(reinterpret_cast<const __half*>(place.page + noff) +
+                                            place.slot)) : 0.f;
+      x.state = place.state;
 #pragma unroll
       for (int k = 0; k < NIT; ++k) {
         const uint8_t* row = reinterpret_cast<const uint8_t*>(
             __shfl_sync(0xffffffffu, mine, k * RPI + sub));
-        codes[k] = row ? load_chunk<BITS>(row, l) : 0;
+        x.codes[k] = row ? (Chunk)load_chunk<BITS>(row, l) : (Chunk)0;
       }
+    };
+    Raw cur, nxt;
+    if (first < p.ntiles) load_raw(cur, first);
+    int it = 0;
+    for (int tile = first; tile < p.ntiles; tile += step, ++it) {
+      const int st = it % SM::STAGES;
+      if (tile + step < p.ntiles) load_raw(nxt, tile + step);
       bool ok = it < SM::STAGES ||
                 wait_for(&pp.a_empty[st], (uint32_t)(((it / SM::STAGES) - 1) & 1), pp.abort_flag,
                          p.status);
       if (!__all_sync(0xffffffffu, ok)) break;
-      if (lane < 16) {
-        const int at = (it % SM::RING) * kM + 16 * warp + lane;
-        norms[at] = n;
-        states[at] = (uint8_t)place.state;
+      if (lane < W::kVecs) {
+        const int at = (it % SM::RING) * kM + W::kVecs * warp + lane;
+        norms[at] = cur.n;
+        states[at] = (uint8_t)cur.state;
       }
       unsigned char* hi = sm + SM::OFF_A + st * S::kTerm;
 #pragma unroll
       for (int k = 0; k < NIT; ++k) {
-        const int r = 16 * warp + k * RPI + sub;
+        const Chunk codes = cur.codes[k];
+        const int r = W::kVecs * warp + k * RPI + sub;
         uint32_t h[4], lo[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if constexpr (SM::kPair) {
-            const uint32_t idx = (uint32_t)(codes[k] >> (2 * BITS * e)) & ((1u << (2 * BITS)) - 1u);
+            const uint32_t idx = (uint32_t)(codes >> (2 * BITS * e)) & ((1u << (2 * BITS)) - 1u);
             if constexpr (LO) {
               const uint2 x = *reinterpret_cast<const uint2*>(lut + idx * 128);
               h[e] = x.x;
@@ -735,8 +791,8 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) read_ragged_tc_kernel(R
               h[e] = *reinterpret_cast<const uint32_t*>(lut + idx * 128);
             }
           } else {
-            const uint32_t i0 = (uint32_t)(codes[k] >> (2 * BITS * e)) & ((1u << BITS) - 1u);
-            const uint32_t i1 = (uint32_t)(codes[k] >> (2 * BITS * e + BITS)) & ((1u << BITS) - 1u);
+            const uint32_t i0 = (uint32_t)(codes >> (2 * BITS * e)) & ((1u << BITS) - 1u);
+            const uint32_t i1 = (uint32_t)(codes >> (2 * BITS * e + BITS)) & ((1u << BITS) - 1u);
             const uint32_t a = *reinterpret_cast<const uint32_t*>(lut + i0 * 128);
             const uint32_t b = *reinterpret_cast<const uint32_t*>(lut + i1 * 128);
             h[e] = __byte_perm(a, b, 0x5410);
@@ -751,6 +807,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) read_ragged_tc_kernel(R
       tc::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive_cta(&pp.a_full[st]);
+      cur = nxt;
     }
   } else if (warp == kMakers) {
     // ------------------------------------------------------------ MMA issuer
@@ -784,7 +841,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) read_ragged_tc_kernel(R
         uint32_t all;
         asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n"
                      " bar.red.and.pred q, %2, %3, p;\n selp.u32 %0, 1, 0, q;\n}"
-                     : "=r"(all) : "r"((uint32_t)ok), "r"(1 + q), "r"(32 * S::kSplit) : "memory");
+                     : "=r"(all) : "r"((uint32_t)ok), "r"(1 + q), "r"(32 * W::kSplit) : "memory");
         if (!all) {
           *pp.abort_flag = 1;
           break;
@@ -796,7 +853,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) read_ragged_tc_kernel(R
       const int r = 32 * q + lane, at = (it % SM::RING) * kM + r;
       const float n = norms[at] * (1.f / kRScale);
       // this warp's 32 / kSplit rows on the way out
-      constexpr int ROWS = 32 / S::kSplit;
+      constexpr int ROWS = 32 / W::kSplit;
       const int r0 = 32 * q + ROWS * part;
       uint32_t state = 0;                                  // of row r0 + lane
       if (lane < ROWS) state = states[(it % SM::RING) * kM + r0 + lane];
@@ -830,7 +887,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) read_ragged_tc_kernel(R
           *reinterpret_cast<uint4*>(piece(r, 4 * part + c)) = make_uint4(h[0], h[1], h[2], h[3]);
         }
       }
-      asm volatile("bar.sync %0, %1;" ::"r"(1 + q), "r"(32 * S::kSplit) : "memory");
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + q), "r"(32 * W::kSplit) : "memory");
       const int v0 = tile * kM + r0;
       if (p.vec[which]) {
         for (int i = lane; i < ROWS * pieces; i += 32) {
@@ -856,7 +913,7 @@ __global__ void __launch_bounds__(Shape<D>::kThreads, 1) read_ragged_tc_kernel(R
           else *reinterpret_cast<uint16_t*>(dst) = stt == 1 ? (uint16_t)0 : *reinterpret_cast<const uint16_t*>(src);
         }
       }
-      asm volatile("bar.sync %0, %1;" ::"r"(1 + q), "r"(32 * S::kSplit) : "memory");
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + q), "r"(32 * W::kSplit) : "memory");
     }
   }
   tc::tc_fence_before();
@@ -927,12 +984,12 @@ int launch_one(RaggedFn fn, unsigned grid, int threads, int bytes, cudaStream_t 
   return check_launch(what);
 }
 
-// Rows that take loads (stores) of four values (16 bytes).
-bool rows_aligned(const tq_tensor4* x, int bytes) {
+// Rows that take 16-byte loads and stores.
+bool rows_aligned(const tq_tensor4* x) {
   const int es = x->dtype == TQ_F32 ? 4 : 2;
-  if (x->stride[3] != 1 || reinterpret_cast<uintptr_t>(x->data) % bytes) return false;
+  if (x->stride[3] != 1 || reinterpret_cast<uintptr_t>(x->data) % 16) return false;
   for (int i = 1; i < 3; ++i)
-    if (x->shape[i] > 1 && (x->stride[i] * es) % bytes) return false;
+    if (x->shape[i] > 1 && (x->stride[i] * es) % 16) return false;
   return true;
 }
 
@@ -945,11 +1002,11 @@ int launch_append_ragged_tc(const tq_geom* G, const tq_tables* t, const tq_cache
                             uint32_t* status, cudaStream_t st) {
   const int D = G->head_dim;
   if (D != 64 && D != 128) return 1;
-  if (k->shape[1] * k->shape[2] > INT32_MAX - kM || (rope && rope->rot_dim % 8)) return 1;
+  if (k->shape[1] * k->shape[2] > INT32_MAX - kM || (rope && rope->rot_dim % 16)) return 1;
   if (reinterpret_cast<uintptr_t>(t->rot) % 16) return 1;
   const tq_tensor4* x[2] = {k, v};
   for (int w = 0; w < 2; ++w)
-    if (!rows_aligned(x[w], x[w]->dtype == TQ_F32 ? 16 : 8)) return 1;
+    if (!rows_aligned(x[w])) return 1;
   RaggedTc p = tc_params(G, t, c, x, batch, status);
   p.f = head_xform(rope, norm);
   p.pos = pos ? pos->data : nullptr;
@@ -962,7 +1019,7 @@ int launch_append_ragged_tc(const tq_geom* G, const tq_tables* t, const tq_cache
     const int bits = w == 0 ? G->key_bits : G->value_bits;
     RaggedFn fn = D == 128 ? append_fn<128>(bits) : append_fn<64>(bits);
     if (set_smem_attr((const void*)fn, kSmem) != TQ_OK) return TQ_ERR_CUDA;
-    const int threads = D == 128 ? Shape<128>::kThreads : Shape<64>::kThreads;
+    const int threads = D == 128 ? AppendRoles<128>::kThreads : AppendRoles<64>::kThreads;
     if (const int rc = launch_one(fn, grid, threads, kSmem, st, p, w, w == 1, "tq_append_ragged"))
       return rc;
   }
@@ -982,14 +1039,14 @@ int launch_dequant_ragged_tc(const tq_geom* G, const tq_tables* t, const tq_cach
   const unsigned grid = (unsigned)tmin(p.ntiles, device_sm_count());
   for (int w = 0; w < 2; ++w) {
     if (!x[w]) continue;
-    p.vec[w] = rows_aligned(x[w], 16);
+    p.vec[w] = rows_aligned(x[w]);
     const int bits = w == 0 ? G->key_bits : G->value_bits;
     int bytes = 0;
     const bool lo = x[w]->dtype != TQ_BF16;
     RaggedFn fn = D == 128 ? (lo ? read_fn<128, true>(bits, bytes) : read_fn<128, false>(bits, bytes))
                            : (lo ? read_fn<64, true>(bits, bytes) : read_fn<64, false>(bits, bytes));
     if (set_smem_attr((const void*)fn, bytes) != TQ_OK) return TQ_ERR_CUDA;
-    const int threads = D == 128 ? Shape<128>::kThreads : Shape<64>::kThreads;
+    const int threads = D == 128 ? ReadRoles<128>::kThreads : ReadRoles<64>::kThreads;
     if (const int rc = launch_one(fn, grid, threads, bytes, st, p, w, w == 1 && ko,
                                   "tq_dequantize_ragged"))
       return rc;
