@@ -5,12 +5,12 @@
 // A tile is 128 consecutive head vectors of the flattened batch (token-major,
 // so the heads of a token share its row of the rotation table and a tile is
 // contiguous in memory), M of one tcgen05.mma with N = K = head_dim.  One
-// persistent CTA per SM, a launch each for K and V, three roles:
+// persistent CTA per SM, a launch each for K and V, four roles:
 //   makers      operand of the next tile.  Append (16 warps): load, norm,
 //               rotate, norm again, split into fp16; read-back (8 warps): codes
-//               -> centroids through lane-replicated tables.  They also find
-//               each vector's request, position and page, and fetch one tile
-//               ahead of what they make.
+//               -> centroids through lane-replicated tables.  They fetch one
+//               tile ahead of what they make.
+//   locators    two warps find each vector's request, position and page
 //   issuer      one thread issues the MMAs into one of two accumulators
 //   epilogue    one thread per vector and 32 columns at a time.  Append (8
 //               warps): bucketize and pack; read-back (4 per 32 columns): times
@@ -54,6 +54,23 @@ constexpr int kSmem = 227 * 1024;
 constexpr float kCmp = 1.2676506e30f;      // 2^100
 constexpr float kRScale = 64.f;
 
+// i / d for 0 <= i < 2^31 as a product: m = ceil(2^(31 + s) / d), 2^s >= d.
+struct FastDiv {
+  uint32_t m, s;
+  int d;
+  __device__ __forceinline__ int div(int i) const {
+    return (int)(((uint64_t)(uint32_t)i * m) >> (31 + s));
+  }
+};
+FastDiv fast_div(int d) {
+  FastDiv f;
+  f.d = d;
+  f.s = 0;
+  while ((1 << f.s) < d) ++f.s;
+  f.m = (uint32_t)((((uint64_t)1 << (31 + f.s)) + d - 1) / d);
+  return f;
+}
+
 struct RaggedTc {
   PageGeom g;
   const float* cent[2];
@@ -64,6 +81,7 @@ struct RaggedTc {
   uint32_t* status;
   RaggedView rv;
   int H, ntiles, nvec;                     // heads, tiles, vectors (rows x heads)
+  FastDiv by_h;
   const void* x[2];                        // append: inputs; read-back: outputs (NULL: absent)
   int dtype[2];
   int64_t stride[2][3];                    // head, row, dim
@@ -73,12 +91,13 @@ struct RaggedTc {
   const void* pos; int pos64; int64_t pos_stride;
 };
 
-// MAKERS maker warps (kM / MAKERS vectors each), the issuing warp, SPLIT
-// epilogue warps per lane quarter of tensor memory.
+// MAKERS maker warps (kM / MAKERS vectors each), the issuing warp, two
+// locators, SPLIT epilogue warps per lane quarter of tensor memory.
 template <int D, int MAKERS, int SPLIT>
 struct Roles {
   static constexpr int kMakers = MAKERS, kVecs = kM / MAKERS, kSplit = SPLIT, kEpi = 4 * SPLIT;
-  static constexpr int kThreads = 32 * (MAKERS + 1 + kEpi);
+  static constexpr int kIssuer = MAKERS, kLocators = MAKERS + 1, kEpi0 = MAKERS + 3;
+  static constexpr int kThreads = 32 * (kEpi0 + kEpi);
 };
 // Making an append operand (norms, rotation, split) takes twice its epilogue's
 // instructions, a read-back operand half of it.
@@ -102,17 +121,19 @@ __device__ __forceinline__ void expired(uint32_t* status, volatile int* abort_fl
   atomicOr(status, TQ_DEV_WAIT_TIMEOUT);
 }
 
-// Bounded wait (2 s) that also ends once another role has given up.  Suspended
-// for up to 20 us at a time: polling warps took half of the issue slots.
+// Bounded wait (2 s) that also ends once another role has given up.  The
+// thread is suspended between polls, and only every 16th looks at the clock.
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
                                          uint32_t* status) {
   uint64_t t0 = 0;
-  while (true) {
+  for (uint32_t i = 1;; ++i) {
     if (mbar_try_wait_hint(bar, parity, 20000u)) return true;
-    if (*abort_flag) return false;
-    const uint64_t t = global_ns();
-    if (t0 == 0) t0 = t;
-    else if (t - t0 > 2000000000ull) break;
+    if ((i & 15u) == 0) {
+      if (*abort_flag) return false;
+      const uint64_t t = global_ns();
+      if (t0 == 0) t0 = t;
+      else if (t - t0 > 2000000000ull) break;
+    }
   }
   expired(status, abort_flag);
   return false;
@@ -124,68 +145,86 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint3
   lo = pack_half2(a - __low2float(h), b - __high2float(h));
 }
 
-// R's rows in packed order, times kRScale, as fp16 hi at `b` and lo behind it.
-template <int D>
+// R's rows in packed order, times kRScale, as fp16 hi at `b` and lo behind it,
+// by N threads with all their loads in flight.
+template <int D, int N>
 __device__ __forceinline__ void stage_rotation(unsigned char* b, const float* rot, int which,
-                                               int tid, int nthreads) {
-  for (int i = tid; i < D * D / 8; i += nthreads) {
+                                               int tid) {
+  constexpr int IT = (D * D / 8 + N - 1) / N;
+  float4 u[IT], v[IT];
+#pragma unroll
+  for (int k = 0; k < IT; ++k) {
+    const int i = tid + k * N;
+    if (i >= D * D / 8) break;
     const int r = i / (D / 8), c = i % (D / 8);
     const int row = which == 0 ? k_coord_at(r, D) : v_coord_at(r, D);
     const float4* src = reinterpret_cast<const float4*>(rot + row * D + 8 * c);
-    const float4 u = __ldg(src), v = __ldg(src + 1);
+    u[k] = __ldg(src);
+    v[k] = __ldg(src + 1);
+  }
+#pragma unroll
+  for (int k = 0; k < IT; ++k) {
+    const int i = tid + k * N;
+    if (i >= D * D / 8) break;
     uint32_t h[4], l[4];
-    split_pair(u.x * kRScale, u.y * kRScale, h[0], l[0]);
-    split_pair(u.z * kRScale, u.w * kRScale, h[1], l[1]);
-    split_pair(v.x * kRScale, v.y * kRScale, h[2], l[2]);
-    split_pair(v.z * kRScale, v.w * kRScale, h[3], l[3]);
-    const uint32_t at = chunk_at<D>(r, c);
+    split_pair(u[k].x * kRScale, u[k].y * kRScale, h[0], l[0]);
+    split_pair(u[k].z * kRScale, u[k].w * kRScale, h[1], l[1]);
+    split_pair(v[k].x * kRScale, v[k].y * kRScale, h[2], l[2]);
+    split_pair(v[k].z * kRScale, v[k].w * kRScale, h[3], l[3]);
+    const uint32_t at = chunk_at<D>(i / (D / 8), i % (D / 8));
     *reinterpret_cast<uint4*>(b + at) = make_uint4(h[0], h[1], h[2], h[3]);
     *reinterpret_cast<uint4*>(b + Shape<D>::kB + at) = make_uint4(l[0], l[1], l[2], l[3]);
   }
 }
 
-// What the epilogue needs of each vector of a tile.
-struct Vec {
-  uint8_t* page;                           // NULL: no place
-  float n, inv;                            // norm; append: factor of the accumulator
-  int slot;                                // token in its page
-  int state;                               // 0: row of no request, 1: no place, 2: stored
+// A tile's vectors, one ring entry: where they lie (locators) and what the
+// makers leave for the epilogue.
+struct Vecs {
+  uint8_t* page[kM];                       // NULL: no place
+  int slot[kM];                            // token in its page
+  int row[kM];                             // row of the rotation table
+  float n[kM];                             // norm
+  float inv[kM];                           // append: factor of the accumulator
+  uint8_t state[kM];                       // 0: row of no request, 1: no place, 2: stored
 };
 
-// A maker warp's lane finds vector i; `row`: its row of the rotation table.
-__device__ __forceinline__ Vec find_vector(const RaggedTc& p, int i, int nvec, bool mine, int& row) {
-  Vec v;
-  v.page = nullptr;
-  v.n = v.inv = 0.f;
-  v.slot = v.state = 0;
-  row = 0;
-  if (!mine || i >= nvec) return v;
-  const int n = i / p.H, h = i % p.H;
-  const int64_t r = request_of(p.rv, n);
-  if (r < 0) return v;
-  v.state = 1;
-  const int64_t pos = (int64_t)__ldg(p.rv.seq_lens + r) - __ldg(p.rv.q_start + r + 1) + n;
-  if (pos < 0 || pos >= p.rv.cap) {
-    atomicOr(p.status, TQ_DEV_BAD_POSITION);
-    return v;
+// Find vector i for entry `at` of its tile.
+__device__ __forceinline__ void find_vector(const RaggedTc& p, int i, Vecs& v, int at) {
+  uint8_t* page = nullptr;
+  int slot = 0, row = 0, state = 0;
+  if (i < p.nvec) {
+    const int n = p.by_h.div(i), h = i - n * p.H;
+    const int64_t r = request_of(p.rv, n);
+    if (r >= 0) {
+      state = 1;
+      const int64_t pos = (int64_t)__ldg(p.rv.seq_lens + r) - __ldg(p.rv.q_start + r + 1) + n;
+      if (pos < 0 || pos >= p.rv.cap) {
+        atomicOr(p.status, TQ_DEV_BAD_POSITION);
+      } else {
+        bool ok;
+        const int64_t ps = page_slot(p.pm, r * p.H + h, pos / kPageTokens, ok);
+        if (!ok) {
+          atomicOr(p.status, TQ_DEV_BAD_BLOCK);
+        } else {
+          page = p.pages + ps * (int64_t)p.g.page_bytes;
+          slot = (int)(pos % kPageTokens);
+          state = 2;
+          if (p.f.cos_sin) {
+            int64_t to = pos;
+            if (p.pos)
+              to = p.pos64
+                       ? (int64_t)__ldg(reinterpret_cast<const long long*>(p.pos) + n * p.pos_stride)
+                       : (int64_t)__ldg(reinterpret_cast<const int*>(p.pos) + n * p.pos_stride);
+            row = (int)table_row(p.f, to, p.status);
+          }
+        }
+      }
+    }
   }
-  bool ok;
-  const int64_t ps = page_slot(p.pm, r * p.H + h, pos / kPageTokens, ok);
-  if (!ok) {
-    atomicOr(p.status, TQ_DEV_BAD_BLOCK);
-    return v;
-  }
-  v.page = p.pages + ps * (int64_t)p.g.page_bytes;
-  v.slot = (int)(pos % kPageTokens);
-  v.state = 2;
-  if (p.f.cos_sin) {
-    int64_t at = pos;
-    if (p.pos)
-      at = p.pos64 ? (int64_t)__ldg(reinterpret_cast<const long long*>(p.pos) + n * p.pos_stride)
-                   : (int64_t)__ldg(reinterpret_cast<const int*>(p.pos) + n * p.pos_stride);
-    row = (int)table_row(p.f, at, p.status);
-  }
-  return v;
+  v.page[at] = page;
+  v.slot[at] = slot;
+  v.row[at] = row;
+  v.state[at] = (uint8_t)state;
 }
 
 // Shared pieces of both kernels: barriers, the issuing thread, the accumulators.
@@ -194,6 +233,8 @@ struct Pipe {
   uint64_t* a_empty;                       // [2] MMA commit
   uint64_t* acc_full;                      // [2] MMA commit
   uint64_t* acc_empty;                     // [2] epilogue warps
+  uint64_t* loc_full;                      // [kRing] a locator: the tile's places are known
+  uint64_t* loc_free;                      // [kRing] epilogue warps
   volatile int* abort_flag;
   uint32_t* tmem_slot;
 };
@@ -205,11 +246,13 @@ __device__ __forceinline__ Pipe make_pipe(unsigned char* at) {
   p.a_empty = b + 2;
   p.acc_full = b + 4;
   p.acc_empty = b + 6;
-  p.tmem_slot = reinterpret_cast<uint32_t*>(b + 8);
-  p.abort_flag = reinterpret_cast<volatile int*>(b + 9);
+  p.loc_full = b + 8;
+  p.loc_free = b + 8 + kRing;
+  p.tmem_slot = reinterpret_cast<uint32_t*>(b + 8 + 2 * kRing);
+  p.abort_flag = reinterpret_cast<volatile int*>(b + 9 + 2 * kRing);
   return p;
 }
-constexpr int kPipeBytes = 128;
+constexpr int kPipeBytes = 192;            // with 16 bytes of the lookup grid at its end
 
 __device__ __forceinline__ void init_pipe(const Pipe& p, int makers, int epi_warps) {
   for (int i = 0; i < 2; ++i) {
@@ -218,8 +261,32 @@ __device__ __forceinline__ void init_pipe(const Pipe& p, int makers, int epi_war
     mbar_init(&p.acc_full[i], 1);
     mbar_init(&p.acc_empty[i], epi_warps);
   }
+  for (int i = 0; i < kRing; ++i) {
+    mbar_init(&p.loc_full[i], 1);
+    mbar_init(&p.loc_free[i], epi_warps);
+  }
   *p.abort_flag = 0;
   fence_mbar_init();
+}
+
+// Two warps, every other tile each: four vectors per lane.  A vector's place is
+// a chain of dependent loads (offsets, length, block table); found by warps of
+// their own and up to kRing tiles ahead, the chain delays nobody.
+__device__ __forceinline__ void locate_tiles(const RaggedTc& p, const Pipe& pp, Vecs* ring,
+                                             int which_warp, int first, int step) {
+  const int lane = threadIdx.x & 31;
+  int it = 0;
+  for (int tile = first; tile < p.ntiles; tile += step, ++it) {
+    if ((it & 1) != which_warp) continue;
+    const int e = it % kRing;
+    const bool ok = it < kRing || wait_for(&pp.loc_free[e], (uint32_t)(((it / kRing) - 1) & 1),
+                                           pp.abort_flag, p.status);
+    if (!__all_sync(0xffffffffu, ok)) break;
+#pragma unroll
+    for (int k = 0; k < kM / 32; ++k) find_vector(p, tile * kM + 32 * k + lane, ring[e], 32 * k + lane);
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive_cta(&pp.loc_full[e]);
+  }
 }
 
 // One thread: the MMAs of every tile.  terms(stage, term, a, b) gives the
@@ -269,8 +336,9 @@ struct AppendSmem {
   static constexpr int OFF_B = 0;
   static constexpr int OFF_A = OFF_B + 2 * Shape<D>::kB;           // 2 stages of hi, lo
   static constexpr int OFF_BND = OFF_A + 4 * Shape<D>::kTerm;      // [256]
-  static constexpr int OFF_VEC = OFF_BND + 1024;                   // [kRing][kM]
-  static constexpr int OFF_PIPE = OFF_VEC + kRing * kM * (int)sizeof(Vec);
+  static constexpr int OFF_W = OFF_BND + 1024;                     // [D] norm weights
+  static constexpr int OFF_VEC = OFF_W + 4 * D;                    // [kRing]
+  static constexpr int OFF_PIPE = OFF_VEC + kRing * (int)sizeof(Vecs);
   static constexpr int OFF_LUT = OFF_PIPE + kPipeBytes;
   static constexpr int LUT_BYTES = kSmem - 1024 - OFF_LUT;         // 1 KB: slack to align the base
   static_assert(LUT_BYTES >= 8 * 1024, "shared memory");
@@ -309,9 +377,9 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
   const uint32_t raw = smem_u32(smem_raw);
   unsigned char* sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);
   const Pipe pp = make_pipe(sm + SM::OFF_PIPE);
-  float* lutpar = reinterpret_cast<float*>(sm + SM::OFF_PIPE + 96);
+  float* lutpar = reinterpret_cast<float*>(sm + SM::OFF_PIPE + kPipeBytes - 16);
   float* bnd = reinterpret_cast<float*>(sm + SM::OFF_BND);
-  Vec* ring = reinterpret_cast<Vec*>(sm + SM::OFF_VEC);
+  Vecs* ring = reinterpret_cast<Vecs*>(sm + SM::OFF_VEC);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int nb = (1 << BITS) - 1;
   const int nvec = p.nvec;
@@ -320,12 +388,16 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
   // after it, so that whatever follows sees both
   pdl_launch_dependents();
   if (tid == 0) init_pipe(pp, kMakers, W::kEpi);
-  if (warp == kMakers) {
+  if (warp == W::kIssuer) {
     tc::tmem_alloc(pp.tmem_slot, 2 * D);
     tc::tmem_relinquish();
   }
   for (int i = tid; i < nb; i += kThreads) bnd[i] = p.bnd[which][i];
-  stage_rotation<D>(sm + SM::OFF_B, p.rot, which, tid, kThreads);
+  float* weight = reinterpret_cast<float*>(sm + SM::OFF_W);
+  if (which == 0 && p.f.weight)
+    for (int i = tid; i < D; i += kThreads)
+      weight[i] = load_elem(p.f.weight, p.f.w_dtype, i) + p.f.w_offset;
+  stage_rotation<D, kThreads>(sm + SM::OFF_B, p.rot, which, tid);
   __syncthreads();
   if (warp == 0) {
     float gap = 1.f;
@@ -387,7 +459,8 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
     // registers: loaded when they are used)
     struct Raw { uint4 a[NIT], b[NIT]; };
     auto base_of = [&](int i) {
-      return (int64_t)(i / p.H) * xs[1] + (int64_t)(i % p.H) * xs[0];
+      const int n = p.by_h.div(i);
+      return (int64_t)n * xs[1] + (int64_t)(i - n * p.H) * xs[0];
     };
     auto load_raw = [&](Raw& x, int v0) {
 #pragma unroll
@@ -402,39 +475,19 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
       }
     };
     auto vec0 = [&](int tile) { return tile * kM + W::kVecs * warp; };
-    auto find = [&](int tile, int& row) {
-      return find_vector(p, vec0(tile) + lane, nvec, lane < W::kVecs, row);
-    };
     Raw cur, nxt;
-    int trow = 0, trow_next = 0;
-    Vec place = {}, place_next = {};
-    if (first < p.ntiles) {
-      load_raw(cur, vec0(first));
-      place = find(first, trow);
-    }
+    if (first < p.ntiles) load_raw(cur, vec0(first));
     int it = 0;
     for (int tile = first; tile < p.ntiles; tile += step, ++it) {
       const int st = it & 1;
-      Vec* vec = ring + (it % kRing) * kM + W::kVecs * warp;
       const int v0 = vec0(tile);
-      // the next tile's values and places while this one is made
-      if (tile + step < p.ntiles) {
-        load_raw(nxt, vec0(tile + step));
-        place_next = find(tile + step, trow_next);
-        if (f.cos_sin) {
-          // its first and last rows of the rotation table (often all of them)
-          const int r = __shfl_sync(0xffffffffu, trow_next, lane < 16 ? 0 : W::kVecs - 1);
-          const float* at = f.cos_sin + (int64_t)r * f.rot + 32 * (lane & 15);
-          if (32 * (lane & 15) < f.rot) asm volatile("prefetch.global.L1 [%0];" ::"l"(at));
-        }
-      }
-      // the stage is free, and with it the ring's entry: its tile's epilogue
-      // ran before this stage's last MMAs could start
-      bool ok = it < 2 || wait_for(&pp.a_empty[st], (uint32_t)(((it / 2) - 1) & 1), pp.abort_flag,
-                                   p.status);
+      if (tile + step < p.ntiles) load_raw(nxt, vec0(tile + step));
+      bool ok = wait_for(&pp.loc_full[it % kRing], (uint32_t)((it / kRing) & 1), pp.abort_flag,
+                         p.status) &&
+                (it < 2 || wait_for(&pp.a_empty[st], (uint32_t)(((it / 2) - 1) & 1), pp.abort_flag,
+                                    p.status));
       if (!__all_sync(0xffffffffu, ok)) break;
-      if (lane < W::kVecs) vec[lane] = place;
-      __syncwarp();
+      Vecs& vec = ring[it % kRing];
       unsigned char* hi = sm + SM::OFF_A + st * 2 * S::kTerm;
 #pragma unroll
       for (int k = 0; k < NIT; ++k) {
@@ -463,14 +516,16 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
           for (int e = 0; e < 16; ++e) ss = fmaf(v[e], v[e], ss);
           const float r = 1.f / sqrtf(sum_lanes<LV>(ss) / (float)D + f.eps);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const float w = load_elem(f.weight, f.w_dtype, e < 8 ? ga + e : gb + e - 8) + f.w_offset;
-            v[e] = v[e] * r * w;
+          for (int e = 0; e < 16; e += 4) {
+            const float4 w = *reinterpret_cast<const float4*>(weight + (e < 8 ? ga + e : gb + e - 8));
+            v[e] *= r * w.x;
+            v[e + 1] *= r * w.y;
+            v[e + 2] *= r * w.z;
+            v[e + 3] *= r * w.w;
           }
         }
         if (f.cos_sin) {
-          const int row = __shfl_sync(0xffffffffu, trow, vi);
-          const float* cs = f.cos_sin + (int64_t)row * f.rot;
+          const float* cs = f.cos_sin + (int64_t)vec.row[W::kVecs * warp + vi] * f.rot;
           auto rotate = [](float& a, float& b, float c, float s) {
             const float t = a * c - b * s;
             b = b * c + a * s;
@@ -510,11 +565,11 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
         // 2^(10 - exponent of n), from 2^-118 to 2^100
         const int ex = (int)((__float_as_uint(n) >> 23) & 255u) - 127;
         const float s = __uint_as_float((uint32_t)(127 + 10 - max(ex, -90)) << 23);
-        if (l == 0) {
-          vec[vi].n = n;
-          vec[vi].inv = 1.f / (s * fmaxf(n, 1e-8f) * kRScale);
-        }
         const int r = W::kVecs * warp + vi;
+        if (l == 0) {
+          vec.n[r] = n;
+          vec.inv[r] = 1.f / (s * fmaxf(n, 1e-8f) * kRScale);
+        }
         const uint32_t aa = chunk_at<kM>(r, ga >> 3), ab = chunk_at<kM>(r, gb >> 3);
         uint32_t h[8], lo[8];
 #pragma unroll
@@ -530,10 +585,8 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
       __syncwarp();
       if (lane == 0) tc::mbar_arrive_cta(&pp.a_full[st]);
       cur = nxt;
-      place = place_next;
-      trow = trow_next;
     }
-  } else if (warp == kMakers) {
+  } else if (warp == W::kIssuer) {
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0) {
       const uint32_t a0 = smem_u32(sm + SM::OFF_A), b0 = smem_u32(sm + SM::OFF_B);
@@ -545,10 +598,12 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
                                });
     }
     __syncwarp();
+  } else if (warp < W::kEpi0) {
+    locate_tiles(p, pp, ring, warp - W::kLocators, first, step);
   } else {
     // ------------------------------------------------------------ epilogue
     constexpr int NCH = D / W::kSplit / 32;                // runs of 32 columns per thread
-    const int q = warp & 3, part = (warp - kMakers - 1) >> 2;
+    const int q = warp & 3, part = (warp - W::kEpi0) >> 2;
     const int r = 32 * q + lane;
     const int row_bytes = D * BITS / 8;
     const int sec = which == 0 ? p.g.off_k : p.g.off_v, noff = which == 0 ? p.g.off_kn : p.g.off_vn;
@@ -561,8 +616,10 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
       bool ok = wait_for(&pp.acc_full[ac], (uint32_t)((it / 2) & 1), pp.abort_flag, p.status);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc::tc_fence_after();
-      const Vec v = ring[(it % kRing) * kM + r];
-      const float ca = v.inv * par0, cK = v.inv * kCmp;
+      const Vecs& vec = ring[it % kRing];
+      uint8_t* const page = vec.page[r];
+      const int slot = vec.slot[r];
+      const float n = vec.n[r], inv = vec.inv[r], ca = inv * par0, cK = inv * kCmp;
 #pragma unroll
       for (int ch = 0; ch < NCH; ++ch) {
         const int run = part * NCH + ch;                   // 32 positions of the row
@@ -572,7 +629,10 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
         if (ch == NCH - 1) {
           tc::tc_fence_before();
           __syncwarp();
-          if (lane == 0) tc::mbar_arrive_cta(&pp.acc_empty[ac]);
+          if (lane == 0) {
+            tc::mbar_arrive_cta(&pp.acc_empty[ac]);
+            tc::mbar_arrive_cta(&pp.loc_free[it % kRing]);
+          }
         }
         uint32_t words[BITS];
 #pragma unroll
@@ -608,14 +668,14 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            const uint32_t code = (uint32_t)bucketize_lt(bnd, nb, __uint_as_float(yb[j]) * v.inv);
+            const uint32_t code = (uint32_t)bucketize_lt(bnd, nb, __uint_as_float(yb[j]) * inv);
             const int bo = j * BITS, wi = bo >> 5, sh = bo & 31;
             words[wi] += code << sh;
             if (sh + BITS > 32) words[wi + 1] += code >> (32 - sh);
           }
         }
-        if (v.page) {
-          uint8_t* row = v.page + sec + v.slot * row_bytes + run * (4 * BITS);
+        if (page) {
+          uint8_t* row = page + sec + slot * row_bytes + run * (4 * BITS);
           if constexpr (BITS % 4 == 0) {
 #pragma unroll
             for (int x = 0; x < BITS / 4; ++x)
@@ -631,13 +691,13 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
           }
         }
       }
-      if (v.page && part == 0)
-        reinterpret_cast<__half*>(v.page + noff)[v.slot] = __float2half_rn(v.n);
+      if (page && part == 0)
+        reinterpret_cast<__half*>(page + noff)[slot] = __float2half_rn(n);
     }
   }
   tc::tc_fence_before();
   __syncthreads();
-  if (warp == kMakers) {
+  if (warp == W::kIssuer) {
     __syncwarp();
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, 2 * D);
@@ -651,19 +711,20 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
 // LO: c as hi + lo (fp16 and fp32 results), one operand stage; else c = hi, two.
 template <int D, int BITS, bool LO>
 struct ReadSmem {
-  static constexpr int STAGES = LO ? 1 : 2, RING = STAGES + 2;      // see the makers
+  static constexpr int STAGES = LO ? 1 : 2;
   static constexpr bool kPair = BITS <= 4;                         // table of code pairs
   using Chunk = typename std::conditional<(BITS <= 4), uint32_t, uint64_t>::type;   // 8 codes
   // entry: fp16 pair hi (and lo) of two codes, or one code's {hi, lo}; copies
   // for 32 lanes of 4-byte entries, 16 of 8-byte ones: 128 bytes
   static constexpr int OFF_B = 0;
   static constexpr int OFF_A = OFF_B + 2 * Shape<D>::kB;
-  static constexpr int OFF_OUT = OFF_A + (LO ? 2 : STAGES) * Shape<D>::kTerm;   // [kM][D] results
-  static constexpr int OFF_LUT = OFF_OUT + kM * D * (LO ? 4 : 2);
+  // results on their way out, [rows][D]: all 128 rows of 16-bit values; of 32-bit
+  // ones half a tile at a time
+  static constexpr int OFF_OUT = OFF_A + (LO ? 2 : STAGES) * Shape<D>::kTerm;
+  static constexpr int OFF_LUT = OFF_OUT + kM * D * 2;
   static constexpr int LUT_BYTES = (1 << (kPair ? 2 * BITS : BITS)) * 128;
-  static constexpr int OFF_N = OFF_LUT + LUT_BYTES;                // [RING][kM] norms
-  static constexpr int OFF_ST = OFF_N + RING * kM * 4;             // [RING][kM] states (bytes)
-  static constexpr int OFF_PIPE = OFF_ST + RING * kM;
+  static constexpr int OFF_VEC = OFF_LUT + LUT_BYTES;              // [kRing]
+  static constexpr int OFF_PIPE = OFF_VEC + kRing * (int)sizeof(Vecs);
   static constexpr int BYTES = OFF_PIPE + kPipeBytes + 1024;
   static_assert(BYTES <= kSmem, "shared memory");
 };
@@ -696,8 +757,7 @@ read_ragged_tc_kernel(RaggedTc p, int which) {
   const uint32_t raw = smem_u32(smem_raw);
   unsigned char* sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);
   const Pipe pp = make_pipe(sm + SM::OFF_PIPE);
-  float* norms = reinterpret_cast<float*>(sm + SM::OFF_N);
-  uint8_t* states = sm + SM::OFF_ST;
+  Vecs* ring = reinterpret_cast<Vecs*>(sm + SM::OFF_VEC);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int nvec = p.nvec;
 
@@ -705,11 +765,11 @@ read_ragged_tc_kernel(RaggedTc p, int which) {
   // after it, so that whatever follows sees both
   pdl_launch_dependents();
   if (tid == 0) init_pipe(pp, kMakers, W::kEpi);
-  if (warp == kMakers) {
+  if (warp == W::kIssuer) {
     tc::tmem_alloc(pp.tmem_slot, 2 * D);
     tc::tmem_relinquish();
   }
-  stage_rotation<D>(sm + SM::OFF_B, p.rot, which, tid, kThreads);
+  stage_rotation<D, kThreads>(sm + SM::OFF_B, p.rot, which, tid);
   {
     const float* cent = p.cent[which];
     constexpr uint32_t mask = (1u << BITS) - 1u;
@@ -742,37 +802,37 @@ read_ragged_tc_kernel(RaggedTc p, int which) {
     const int l = lane % LV, sub = lane / LV;
     const unsigned char* lut = sm + SM::OFF_LUT + (SM::kPair && LO ? 8 * (lane & 15) : 4 * lane);
     using Chunk = typename SM::Chunk;
-    struct Raw { Chunk codes[NIT]; float n; int state; };
-    auto load_raw = [&](Raw& x, int tile) {
-      int trow;
-      const Vec place = find_vector(p, tile * kM + W::kVecs * warp + lane, nvec, lane < W::kVecs, trow);
-      const unsigned long long mine = reinterpret_cast<unsigned long long>(
-          place.page ? place.page + sec + place.slot * row_bytes : nullptr);
-      x.n = place.page ? __half2float(__ldg(reinterpret_cast<const __half*>(place.page + noff) +
-                                            place.slot)) : 0.f;
-      x.state = place.state;
+    struct Raw { Chunk codes[NIT]; float n; };
+    // a tile's codes and (lanes < kVecs) norms, once its places are known
+    auto load_raw = [&](Raw& x, int it) -> bool {
+      if (!__all_sync(0xffffffffu, wait_for(&pp.loc_full[it % kRing], (uint32_t)((it / kRing) & 1),
+                                            pp.abort_flag, p.status)))
+        return false;
+      const Vecs& vec = ring[it % kRing];
+      const int r0 = W::kVecs * warp;
 #pragma unroll
       for (int k = 0; k < NIT; ++k) {
-        const uint8_t* row = reinterpret_cast<const uint8_t*>(
-            __shfl_sync(0xffffffffu, mine, k * RPI + sub));
-        x.codes[k] = row ? (Chunk)load_chunk<BITS>(row, l) : (Chunk)0;
+        const int r = r0 + k * RPI + sub;
+        const uint8_t* page = vec.page[r];
+        x.codes[k] = page ? (Chunk)load_chunk<BITS>(page + sec + vec.slot[r] * row_bytes, l) : (Chunk)0;
       }
+      x.n = 0.f;
+      if (lane < W::kVecs && vec.page[r0 + lane])
+        x.n = __half2float(__ldg(reinterpret_cast<const __half*>(vec.page[r0 + lane] + noff) +
+                                 vec.slot[r0 + lane]));
+      return true;
     };
     Raw cur, nxt;
-    if (first < p.ntiles) load_raw(cur, first);
+    bool more = first < p.ntiles && load_raw(cur, 0);
     int it = 0;
-    for (int tile = first; tile < p.ntiles; tile += step, ++it) {
+    for (int tile = first; more && tile < p.ntiles; tile += step, ++it) {
       const int st = it % SM::STAGES;
-      if (tile + step < p.ntiles) load_raw(nxt, tile + step);
+      if (tile + step < p.ntiles) more = load_raw(nxt, it + 1);
       bool ok = it < SM::STAGES ||
                 wait_for(&pp.a_empty[st], (uint32_t)(((it / SM::STAGES) - 1) & 1), pp.abort_flag,
                          p.status);
       if (!__all_sync(0xffffffffu, ok)) break;
-      if (lane < W::kVecs) {
-        const int at = (it % SM::RING) * kM + W::kVecs * warp + lane;
-        norms[at] = cur.n;
-        states[at] = (uint8_t)cur.state;
-      }
+      if (lane < W::kVecs) ring[it % kRing].n[W::kVecs * warp + lane] = cur.n;
       unsigned char* hi = sm + SM::OFF_A + st * S::kTerm;
 #pragma unroll
       for (int k = 0; k < NIT; ++k) {
@@ -809,7 +869,7 @@ read_ragged_tc_kernel(RaggedTc p, int which) {
       if (lane == 0) tc::mbar_arrive_cta(&pp.a_full[st]);
       cur = nxt;
     }
-  } else if (warp == kMakers) {
+  } else if (warp == W::kIssuer) {
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0) {
       const uint32_t a0 = smem_u32(sm + SM::OFF_A), b0 = smem_u32(sm + SM::OFF_B);
@@ -821,104 +881,123 @@ read_ragged_tc_kernel(RaggedTc p, int which) {
                                        });
     }
     __syncwarp();
+  } else if (warp < W::kEpi0) {
+    locate_tiles(p, pp, ring, warp - W::kLocators, first, step);
   } else {
     // ------------------------------------------------------------ epilogue
-    const int q = warp & 3, part = (warp - kMakers - 1) >> 2;
-    const int dtype = p.dtype[which];
-    const int es = dtype == TQ_F32 ? 4 : 2;
+    // The kSplit warps of a lane quarter hold 32 rows x 32 columns each; they
+    // put them into shared memory and take ROWS whole rows each out of it.
+    constexpr int ROWS = 32 / W::kSplit;
+    const int q = warp & 3, part = (warp - W::kEpi0) >> 2;
+    const int es = p.dtype[which] == TQ_F32 ? 4 : 2;
+    const bool bf16 = p.dtype[which] == TQ_BF16;
     const int64_t* xs = p.stride[which];
-    unsigned char* out = sm + SM::OFF_OUT;
-    // 16-byte piece c of row r, rotated so that rows and pieces spread over the banks
-    const int pieces = D * es / 16;
-    auto piece = [&](int r, int c) { return out + r * (D * es) + ((c ^ (r & 7)) << 4); };
+    char* const dst = static_cast<char*>(const_cast<void*>(p.x[which]));
+    unsigned char* out = sm + SM::OFF_OUT + q * (32 * D * 2);
+    // 16-byte piece c of the quarter's row r (16-bit values), moved so that a
+    // warp's pieces spread over the banks
+    constexpr int PIECES = D / 8;
+    auto piece = [&](int r, int c) { return out + (r * PIECES + (c ^ (r & 7))) * 16; };
+    auto quarter_sync = [&] {
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + q), "r"(32 * W::kSplit) : "memory");
+    };
     int it = 0;
     for (int tile = first; tile < p.ntiles; tile += step, ++it) {
       const int ac = it & 1;
-      bool ok = wait_for(&pp.acc_full[ac], (uint32_t)((it / 2) & 1), pp.abort_flag, p.status);
-      if (!__all_sync(0xffffffffu, ok)) ok = false;
-      // the lane quarter's warps go on or leave together
-      {
-        uint32_t all;
-        asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n"
-                     " bar.red.and.pred q, %2, %3, p;\n selp.u32 %0, 1, 0, q;\n}"
-                     : "=r"(all) : "r"((uint32_t)ok), "r"(1 + q), "r"(32 * W::kSplit) : "memory");
-        if (!all) {
-          *pp.abort_flag = 1;
-          break;
-        }
+      uint32_t all = wait_for(&pp.acc_full[ac], (uint32_t)((it / 2) & 1), pp.abort_flag, p.status);
+      // the lane quarter's warps go on or leave together (and: the rows of the
+      // last tile have left shared memory)
+      asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %0, 0;\n"
+                   " bar.red.and.pred q, %1, %2, p;\n selp.u32 %0, 1, 0, q;\n}"
+                   : "+r"(all) : "r"(1 + q), "r"(32 * W::kSplit) : "memory");
+      if (!all) {
+        *pp.abort_flag = 1;
+        break;
       }
       tc::tc_fence_after();
       uint32_t x[32];
       tc::tmem_ld_x32(tmem + ((uint32_t)(32 * q) << 16) + (uint32_t)(ac * D + 32 * part), x);
-      const int r = 32 * q + lane, at = (it % SM::RING) * kM + r;
-      const float n = norms[at] * (1.f / kRScale);
-      // this warp's 32 / kSplit rows on the way out
-      constexpr int ROWS = 32 / W::kSplit;
-      const int r0 = 32 * q + ROWS * part;
-      uint32_t state = 0;                                  // of row r0 + lane
-      if (lane < ROWS) state = states[(it % SM::RING) * kM + r0 + lane];
+      const Vecs& vec = ring[it % kRing];
+      const float n = vec.n[32 * q + lane] * (1.f / kRScale);
+      // lane < ROWS: the offset of the row it sends out, and what becomes of it
+      const int mine = 32 * q + ROWS * part + lane, v = tile * kM + mine;
+      int state = 0;
+      int64_t at = 0;
+      if (lane < ROWS && v < nvec) {
+        state = vec.state[mine];
+        const int row = p.by_h.div(v);
+        at = ((int64_t)row * xs[1] + (int64_t)(v - row * p.H) * xs[0]) * es;
+      }
       tc::tmem_wait_ld();
       tc::tc_fence_before();
       __syncwarp();
-      if (lane == 0) tc::mbar_arrive_cta(&pp.acc_empty[ac]);
-      if (dtype == TQ_F32) {
-        if constexpr (LO) {
+      if (lane == 0) {
+        tc::mbar_arrive_cta(&pp.acc_empty[ac]);
+        tc::mbar_arrive_cta(&pp.loc_free[it % kRing]);
+      }
 #pragma unroll
-          for (int c = 0; c < 8; ++c)
-            *reinterpret_cast<float4*>(piece(r, 8 * part + c)) =
-                make_float4(__uint_as_float(x[4 * c]) * n, __uint_as_float(x[4 * c + 1]) * n,
-                            __uint_as_float(x[4 * c + 2]) * n, __uint_as_float(x[4 * c + 3]) * n);
-        }
-      } else {
+      for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * n);
+      if (es == 2) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t h[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float a = __uint_as_float(x[8 * c + 2 * e]) * n;
-            const float b = __uint_as_float(x[8 * c + 2 * e + 1]) * n;
-            if (dtype == TQ_F16) {
-              h[e] = pack_half2(a, b);
-            } else {
-              const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-              h[e] = *reinterpret_cast<const uint32_t*>(&v);
-            }
+            const float a = __uint_as_float(x[8 * c + 2 * e]), b = __uint_as_float(x[8 * c + 2 * e + 1]);
+            const __nv_bfloat162 y = __floats2bfloat162_rn(a, b);
+            h[e] = bf16 ? *reinterpret_cast<const uint32_t*>(&y) : pack_half2(a, b);
           }
-          *reinterpret_cast<uint4*>(piece(r, 4 * part + c)) = make_uint4(h[0], h[1], h[2], h[3]);
+          *reinterpret_cast<uint4*>(piece(lane, 4 * part + c)) = make_uint4(h[0], h[1], h[2], h[3]);
         }
-      }
-      asm volatile("bar.sync %0, %1;" ::"r"(1 + q), "r"(32 * W::kSplit) : "memory");
-      const int v0 = tile * kM + r0;
-      if (p.vec[which]) {
-        for (int i = lane; i < ROWS * pieces; i += 32) {
-          const int rr = i / pieces, c = i % pieces;
-          const uint32_t stt = __shfl_sync(0xffffffffu, state, rr);
-          const int v = v0 + rr;
-          if (stt == 0 || v >= nvec) continue;
-          const int64_t o = (int64_t)(v / p.H) * xs[1] + (int64_t)(v % p.H) * xs[0];
-          uint4 y = *reinterpret_cast<const uint4*>(piece(r0 + rr, c));
-          if (stt == 1) y = make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(static_cast<char*>(const_cast<void*>(p.x[which])) + o * es + 16 * c) = y;
+        quarter_sync();
+        if (p.vec[which]) {
+#pragma unroll
+          for (int i = 0; i < ROWS * PIECES / 32; ++i) {
+            const int rr = (32 * i + lane) / PIECES, c = lane % PIECES;
+            const int64_t o = __shfl_sync(0xffffffffu, at, rr);
+            const int stt = __shfl_sync(0xffffffffu, state, rr);
+            uint4 y = *reinterpret_cast<const uint4*>(piece(ROWS * part + rr, c));
+            if (stt == 1) y = make_uint4(0, 0, 0, 0);
+            if (stt) *reinterpret_cast<uint4*>(dst + o + 16 * c) = y;
+          }
+        } else {
+          for (int i = lane; i < ROWS * D; i += 32) {
+            const int rr = i / D, d = i % D;
+            const int64_t o = __shfl_sync(0xffffffffu, at, rr);
+            const int stt = __shfl_sync(0xffffffffu, state, rr);
+            const uint16_t y = reinterpret_cast<const uint16_t*>(piece(ROWS * part + rr, d / 8))[d % 8];
+            if (stt) *reinterpret_cast<uint16_t*>(dst + o + 2 * d * xs[2]) = stt == 1 ? (uint16_t)0 : y;
+          }
         }
       } else {
-        for (int i = lane; i < ROWS * D; i += 32) {
-          const int rr = i / D, d = i % D;
-          const uint32_t stt = __shfl_sync(0xffffffffu, state, rr);
-          const int v = v0 + rr;
-          if (stt == 0 || v >= nvec) continue;
-          const unsigned char* src = piece(r0 + rr, d * es / 16) + (d * es) % 16;
-          const int64_t o = (int64_t)(v / p.H) * xs[1] + (int64_t)(v % p.H) * xs[0] + d * xs[2];
-          char* dst = static_cast<char*>(const_cast<void*>(p.x[which])) + o * es;
-          if (es == 4) *reinterpret_cast<uint32_t*>(dst) = stt == 1 ? 0u : *reinterpret_cast<const uint32_t*>(src);
-          else *reinterpret_cast<uint16_t*>(dst) = stt == 1 ? (uint16_t)0 : *reinterpret_cast<const uint16_t*>(src);
+        // 32-bit values: the even, then the odd rows of the quarter
+#pragma unroll
+        for (int odd = 0; odd < 2; ++odd) {
+          if (odd) quarter_sync();
+          if ((lane & 1) == odd) {
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              *reinterpret_cast<uint4*>(out + (lane & ~1) * PIECES * 16 +
+                                        (((8 * part + c) ^ ((lane >> 1) & 7)) << 4)) =
+                  make_uint4(x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
+          }
+          quarter_sync();
+          for (int i = lane; i < ROWS / 2 * D; i += 32) {
+            const int pr = i / D, d = i % D, rr = 2 * pr + odd;   // row of this warp's ROWS
+            const int row = ROWS * part + 2 * pr;                 // even row of the quarter
+            const int64_t o = __shfl_sync(0xffffffffu, at, rr);
+            const int stt = __shfl_sync(0xffffffffu, state, rr);
+            const uint32_t y = reinterpret_cast<const uint32_t*>(
+                out + row * PIECES * 16 + (((d / 4) ^ ((row >> 1) & 7)) << 4))[d % 4];
+            if (stt) *reinterpret_cast<uint32_t*>(dst + o + 4 * d * xs[2]) = stt == 1 ? 0u : y;
+          }
         }
       }
-      asm volatile("bar.sync %0, %1;" ::"r"(1 + q), "r"(32 * W::kSplit) : "memory");
     }
   }
   tc::tc_fence_before();
   __syncthreads();
-  if (warp == kMakers) {
+  if (warp == W::kIssuer) {
     __syncwarp();
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, 2 * D);
@@ -972,6 +1051,7 @@ RaggedTc tc_params(const tq_geom* G, const tq_tables* t, const tq_cache* c,
     p.rv = ragged_view(batch, x[w]->shape[2], c);
   }
   p.nvec = (int)(p.rv.N * p.H);
+  p.by_h = fast_div(p.H);
   p.ntiles = (p.nvec + kM - 1) / kM;
   return p;
 }
