@@ -121,14 +121,15 @@ __device__ __forceinline__ void expired(uint32_t* status, volatile int* abort_fl
   atomicOr(status, TQ_DEV_WAIT_TIMEOUT);
 }
 
-// Bounded wait (2 s) that also ends once another role has given up.  The
-// thread is suspended between polls, and only every 16th looks at the clock.
+// Bounded wait (2 s) that also ends once another role has given up.  No
+// suspend-time hint: a hinted wait of the issuing thread resumed up to 2 us
+// late, twice a tile's MMAs.
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
                                          uint32_t* status) {
   uint64_t t0 = 0;
   for (uint32_t i = 1;; ++i) {
-    if (mbar_try_wait_hint(bar, parity, 20000u)) return true;
-    if ((i & 15u) == 0) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 255u) == 0) {
       if (*abort_flag) return false;
       const uint64_t t = global_ns();
       if (t0 == 0) t0 = t;
@@ -188,43 +189,26 @@ struct Vecs {
   uint8_t state[kM];                       // 0: row of no request, 1: no place, 2: stored
 };
 
-// Find vector i for entry `at` of its tile.
-__device__ __forceinline__ void find_vector(const RaggedTc& p, int i, Vecs& v, int at) {
-  uint8_t* page = nullptr;
-  int slot = 0, row = 0, state = 0;
-  if (i < p.nvec) {
-    const int n = p.by_h.div(i), h = i - n * p.H;
-    const int64_t r = request_of(p.rv, n);
-    if (r >= 0) {
-      state = 1;
-      const int64_t pos = (int64_t)__ldg(p.rv.seq_lens + r) - __ldg(p.rv.q_start + r + 1) + n;
-      if (pos < 0 || pos >= p.rv.cap) {
-        atomicOr(p.status, TQ_DEV_BAD_POSITION);
-      } else {
-        bool ok;
-        const int64_t ps = page_slot(p.pm, r * p.H + h, pos / kPageTokens, ok);
-        if (!ok) {
-          atomicOr(p.status, TQ_DEV_BAD_BLOCK);
-        } else {
-          page = p.pages + ps * (int64_t)p.g.page_bytes;
-          slot = (int)(pos % kPageTokens);
-          state = 2;
-          if (p.f.cos_sin) {
-            int64_t to = pos;
-            if (p.pos)
-              to = p.pos64
-                       ? (int64_t)__ldg(reinterpret_cast<const long long*>(p.pos) + n * p.pos_stride)
-                       : (int64_t)__ldg(reinterpret_cast<const int*>(p.pos) + n * p.pos_stride);
-            row = (int)table_row(p.f, to, p.status);
-          }
-        }
-      }
-    }
+// The batch's offsets and lengths in shared memory where they fit (a search
+// over global memory costs a trip to L2 per step: 6 us for 64 requests).
+constexpr int kStaged = 512;
+struct Requests {
+  const int32_t* q_start;
+  const int32_t* seq_lens;
+};
+constexpr int kStagedBytes = (2 * kStaged + 4) * 4;
+
+__device__ __forceinline__ Requests stage_requests(const RaggedView& v, unsigned char* at, int tid,
+                                                   int nthreads) {
+  Requests q = {v.q_start, v.seq_lens};
+  if (v.R <= kStaged) {
+    int32_t* s = reinterpret_cast<int32_t*>(at);
+    for (int i = tid; i <= v.R; i += nthreads) s[i] = __ldg(v.q_start + i);
+    for (int i = tid; i < v.R; i += nthreads) s[kStaged + 4 + i] = __ldg(v.seq_lens + i);
+    q.q_start = s;
+    q.seq_lens = s + kStaged + 4;
   }
-  v.page[at] = page;
-  v.slot[at] = slot;
-  v.row[at] = row;
-  v.state[at] = (uint8_t)state;
+  return q;
 }
 
 // Shared pieces of both kernels: barriers, the issuing thread, the accumulators.
@@ -233,7 +217,7 @@ struct Pipe {
   uint64_t* a_empty;                       // [2] MMA commit
   uint64_t* acc_full;                      // [2] MMA commit
   uint64_t* acc_empty;                     // [2] epilogue warps
-  uint64_t* loc_full;                      // [kRing] a locator: the tile's places are known
+  uint64_t* loc_full;                      // [kRing] locators: the tile's places are known
   uint64_t* loc_free;                      // [kRing] epilogue warps
   volatile int* abort_flag;
   uint32_t* tmem_slot;
@@ -262,28 +246,64 @@ __device__ __forceinline__ void init_pipe(const Pipe& p, int makers, int epi_war
     mbar_init(&p.acc_empty[i], epi_warps);
   }
   for (int i = 0; i < kRing; ++i) {
-    mbar_init(&p.loc_full[i], 1);
+    mbar_init(&p.loc_full[i], 2);
     mbar_init(&p.loc_free[i], epi_warps);
   }
   *p.abort_flag = 0;
   fence_mbar_init();
 }
 
-// Two warps, every other tile each: four vectors per lane.  A vector's place is
-// a chain of dependent loads (offsets, length, block table); found by warps of
+// Two warps, half a tile each: two vectors per lane.  A vector's place is a
+// chain of dependent loads (offsets, length, block table); found by warps of
 // their own and up to kRing tiles ahead, the chain delays nobody.
 __device__ __forceinline__ void locate_tiles(const RaggedTc& p, const Pipe& pp, Vecs* ring,
-                                             int which_warp, int first, int step) {
-  const int lane = threadIdx.x & 31;
+                                             const Requests& rq, int half, int first, int step) {
+  constexpr int NV = kM / 64;
+  const int lane = threadIdx.x & 31, R = (int)p.rv.R;
   int it = 0;
   for (int tile = first; tile < p.ntiles; tile += step, ++it) {
-    if ((it & 1) != which_warp) continue;
     const int e = it % kRing;
     const bool ok = it < kRing || wait_for(&pp.loc_free[e], (uint32_t)(((it / kRing) - 1) & 1),
                                            pp.abort_flag, p.status);
     if (!__all_sync(0xffffffffu, ok)) break;
+    int64_t pos[NV], entry[NV], to[NV];
+    int n[NV], state[NV];
+    const int begin = rq.q_start[0], end = rq.q_start[R];
 #pragma unroll
-    for (int k = 0; k < kM / 32; ++k) find_vector(p, tile * kM + 32 * k + lane, ring[e], 32 * k + lane);
+    for (int k = 0; k < NV; ++k) {
+      const int i = tile * kM + 64 * half + 32 * k + lane;
+      n[k] = p.by_h.div(i);
+      const int h = i - n[k] * p.H;
+      state[k] = i < p.nvec && n[k] >= begin && n[k] < end;
+      int lo = 0, hi = R;                  // q_start[lo] <= n < q_start[hi] at the end
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (rq.q_start[mid] <= n[k]) lo = mid; else hi = mid;
+      }
+      pos[k] = (int64_t)rq.seq_lens[lo] - rq.q_start[lo + 1] + n[k];
+      const bool in = state[k] && pos[k] >= 0 && pos[k] < p.rv.cap;
+      if (state[k] && !in) atomicOr(p.status, TQ_DEV_BAD_POSITION);
+      entry[k] = in ? page_entry(p.pm, (int64_t)lo * p.H + h, pos[k] / kPageTokens) : -1;
+      to[k] = pos[k];
+      if (p.pos && in)
+        to[k] = p.pos64
+                    ? (int64_t)__ldg(reinterpret_cast<const long long*>(p.pos) + n[k] * p.pos_stride)
+                    : (int64_t)__ldg(reinterpret_cast<const int*>(p.pos) + n[k] * p.pos_stride);
+      if (in) state[k] = 2;
+    }
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int at = 64 * half + 32 * k + lane;
+      if (state[k] == 2 && !entry_ok(p.pm, entry[k])) {
+        atomicOr(p.status, TQ_DEV_BAD_BLOCK);
+        state[k] = 1;
+      }
+      const bool in = state[k] == 2;
+      ring[e].page[at] = in ? p.pages + entry[k] * (int64_t)p.g.page_bytes : nullptr;
+      ring[e].slot[at] = (int)(pos[k] & (kPageTokens - 1));
+      ring[e].row[at] = in && p.f.cos_sin ? (int)table_row(p.f, to[k], p.status) : 0;
+      ring[e].state[at] = (uint8_t)state[k];
+    }
     __syncwarp();
     if (lane == 0) tc::mbar_arrive_cta(&pp.loc_full[e]);
   }
@@ -337,12 +357,14 @@ struct AppendSmem {
   static constexpr int OFF_A = OFF_B + 2 * Shape<D>::kB;           // 2 stages of hi, lo
   static constexpr int OFF_BND = OFF_A + 4 * Shape<D>::kTerm;      // [256]
   static constexpr int OFF_W = OFF_BND + 1024;                     // [D] norm weights
-  static constexpr int OFF_VEC = OFF_W + 4 * D;                    // [kRing]
+  static constexpr int OFF_REQ = OFF_W + 4 * D;                    // offsets and lengths
+  static constexpr int OFF_VEC = OFF_REQ + kStagedBytes;           // [kRing]
   static constexpr int OFF_PIPE = OFF_VEC + kRing * (int)sizeof(Vecs);
   static constexpr int OFF_LUT = OFF_PIPE + kPipeBytes;
   static constexpr int LUT_BYTES = kSmem - 1024 - OFF_LUT;         // 1 KB: slack to align the base
   static_assert(LUT_BYTES >= 8 * 1024, "shared memory");
   static_assert(OFF_A % 1024 == 0 && Shape<D>::kTerm % 1024 == 0, "swizzled tiles");
+  static_assert(OFF_VEC % 8 == 0 && OFF_PIPE % 8 == 0 && OFF_LUT % 16 == 0, "alignment");
 };
 
 // Four 16-bit values of a vector in fp32.
@@ -397,8 +419,16 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
   if (which == 0 && p.f.weight)
     for (int i = tid; i < D; i += kThreads)
       weight[i] = load_elem(p.f.weight, p.f.w_dtype, i) + p.f.w_offset;
+  const Requests requests = stage_requests(p.rv, sm + SM::OFF_REQ, tid, kThreads);
   stage_rotation<D, kThreads>(sm + SM::OFF_B, p.rot, which, tid);
+  tc::fence_proxy_async_smem();
+  tc::tc_fence_before();
   __syncthreads();
+  // the locators need no more; the others agree on the lookup table
+  const bool locator = warp >= W::kLocators && warp < W::kEpi0;
+  auto others_sync = [&] {
+    asm volatile("bar.sync 7, %0;" ::"n"(kThreads - 64) : "memory");
+  };
   if (warp == 0) {
     float gap = 1.f;
     for (int i = lane; i + 1 < nb; i += 32) gap = fminf(gap, bnd[i + 1] - bnd[i]);
@@ -415,22 +445,22 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
       lutpar[3] = w;
     }
   }
-  __syncthreads();
-  const int ncells = (int)lutpar[2];
-  {
+  if (!locator) others_sync();
+  const int ncells = locator ? 0 : (int)lutpar[2];
+  if (!locator) {
     const float w = lutpar[3], L = 0.5f * lutpar[1];
-    for (int i = tid; i < ncells * 16; i += kThreads) {
+    for (int i = tid < 32 * W::kLocators ? tid : tid - 64; i < ncells * 16; i += kThreads - 64) {
       const int c = i >> 4;
       const float wl = ((float)c - L - 1.f) * w, wh = ((float)c - L + 1.f) * w;
       const int base = bucketize_lt(bnd, nb, wl);
       const float nbk = (base < nb && bnd[base] <= wh) ? -bnd[base] * kCmp : -INFINITY;
       reinterpret_cast<float2*>(sm + SM::OFF_LUT)[i] = make_float2(nbk, (float)base);
     }
+    tc::fence_proxy_async_smem();
+    tc::tc_fence_before();
+    others_sync();
+    tc::tc_fence_after();
   }
-  tc::fence_proxy_async_smem();
-  tc::tc_fence_before();
-  __syncthreads();
-  tc::tc_fence_after();
   const uint32_t tmem = *pp.tmem_slot;
   const int first = blockIdx.x, step = gridDim.x;
   const bool use_lo = p.use_lo[which] != 0;
@@ -599,7 +629,7 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
     }
     __syncwarp();
   } else if (warp < W::kEpi0) {
-    locate_tiles(p, pp, ring, warp - W::kLocators, first, step);
+    locate_tiles(p, pp, ring, requests, warp - W::kLocators, first, step);
   } else {
     // ------------------------------------------------------------ epilogue
     constexpr int NCH = D / W::kSplit / 32;                // runs of 32 columns per thread
@@ -723,7 +753,8 @@ struct ReadSmem {
   static constexpr int OFF_OUT = OFF_A + (LO ? 2 : STAGES) * Shape<D>::kTerm;
   static constexpr int OFF_LUT = OFF_OUT + kM * D * 2;
   static constexpr int LUT_BYTES = (1 << (kPair ? 2 * BITS : BITS)) * 128;
-  static constexpr int OFF_VEC = OFF_LUT + LUT_BYTES;              // [kRing]
+  static constexpr int OFF_REQ = OFF_LUT + LUT_BYTES;              // offsets and lengths
+  static constexpr int OFF_VEC = OFF_REQ + kStagedBytes;           // [kRing]
   static constexpr int OFF_PIPE = OFF_VEC + kRing * (int)sizeof(Vecs);
   static constexpr int BYTES = OFF_PIPE + kPipeBytes + 1024;
   static_assert(BYTES <= kSmem, "shared memory");
@@ -769,6 +800,7 @@ read_ragged_tc_kernel(RaggedTc p, int which) {
     tc::tmem_alloc(pp.tmem_slot, 2 * D);
     tc::tmem_relinquish();
   }
+  const Requests requests = stage_requests(p.rv, sm + SM::OFF_REQ, tid, kThreads);
   stage_rotation<D, kThreads>(sm + SM::OFF_B, p.rot, which, tid);
   {
     const float* cent = p.cent[which];
@@ -882,7 +914,7 @@ read_ragged_tc_kernel(RaggedTc p, int which) {
     }
     __syncwarp();
   } else if (warp < W::kEpi0) {
-    locate_tiles(p, pp, ring, warp - W::kLocators, first, step);
+    locate_tiles(p, pp, ring, requests, warp - W::kLocators, first, step);
   } else {
     // ------------------------------------------------------------ epilogue
     // The kSplit warps of a lane quarter hold 32 rows x 32 columns each; they
