@@ -512,10 +512,20 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
       const int st = it & 1;
       const int v0 = vec0(tile);
       if (tile + step < p.ntiles) load_raw(nxt, vec0(tile + step));
-      bool ok = wait_for(&pp.loc_full[it % kRing], (uint32_t)((it / kRing) & 1), pp.abort_flag,
-                         p.status) &&
-                (it < 2 || wait_for(&pp.a_empty[st], (uint32_t)(((it / 2) - 1) & 1), pp.abort_flag,
-                                    p.status));
+      bool ok = true;
+      if (it == 0 || f.cos_sin == nullptr)
+        ok = wait_for(&pp.loc_full[it % kRing], (uint32_t)((it / kRing) & 1), pp.abort_flag, p.status);
+      if (f.cos_sin && ok && tile + step < p.ntiles) {
+        // the next tile's rows of the rotation table on their way into L1
+        const int e = (it + 1) % kRing;
+        ok = wait_for(&pp.loc_full[e], (uint32_t)(((it + 1) / kRing) & 1), pp.abort_flag, p.status);
+        constexpr int LINES = 32 / W::kVecs;               // 128-byte lines per lane's vector
+        const float* at = f.cos_sin + (int64_t)ring[e].row[W::kVecs * warp + lane / LINES] * f.rot;
+        for (int c = 32 * (lane % LINES); c < f.rot; c += 32 * LINES)
+          asm volatile("prefetch.global.L1 [%0];" ::"l"(at + c));
+      }
+      ok = ok && (it < 2 || wait_for(&pp.a_empty[st], (uint32_t)(((it / 2) - 1) & 1),
+                                     pp.abort_flag, p.status));
       if (!__all_sync(0xffffffffu, ok)) break;
       Vecs& vec = ring[it % kRing];
       unsigned char* hi = sm + SM::OFF_A + st * 2 * S::kTerm;
@@ -544,7 +554,7 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
           float ss = 0.f;
 #pragma unroll
           for (int e = 0; e < 16; ++e) ss = fmaf(v[e], v[e], ss);
-          const float r = 1.f / sqrtf(sum_lanes<LV>(ss) / (float)D + f.eps);
+          const float r = rsqrtf(fmaf(sum_lanes<LV>(ss), 1.f / (float)D, f.eps));
 #pragma unroll
           for (int e = 0; e < 16; e += 4) {
             const float4 w = *reinterpret_cast<const float4*>(weight + (e < 8 ? ga + e : gb + e - 8));
@@ -591,14 +601,19 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
         float ss = 0.f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) ss = fmaf(v[e], v[e], ss);
-        const float n = sqrtf(sum_lanes<LV>(ss));
-        // 2^(10 - exponent of n), from 2^-118 to 2^100
-        const int ex = (int)((__float_as_uint(n) >> 23) & 255u) - 127;
-        const float s = __uint_as_float((uint32_t)(127 + 10 - max(ex, -90)) << 23);
+        ss = sum_lanes<LV>(ss);
+        // the norm and its reciprocal from one rsqrt (2^-22), s = 2^(10 -
+        // exponent of the norm) from 2^-118 to 2^100 and its reciprocal from
+        // the exponent bits: no division or root on the way
+        const float rn = rsqrtf(ss);
+        const float n = ss == 0.f || ss == INFINITY ? ss : ss * rn;
+        const int ex = max((int)((__float_as_uint(n) >> 23) & 255u) - 127, -90);
+        const float s = __uint_as_float((uint32_t)(127 + 10 - ex) << 23);
+        const float rs = __uint_as_float((uint32_t)(127 - 10 + tmin(ex, 127)) << 23);
         const int r = W::kVecs * warp + vi;
         if (l == 0) {
           vec.n[r] = n;
-          vec.inv[r] = 1.f / (s * fmaxf(n, 1e-8f) * kRScale);
+          vec.inv[r] = (n < 1e-8f ? 1e8f : rn) * rs * (1.f / kRScale);
         }
         const uint32_t aa = chunk_at<kM>(r, ga >> 3), ab = chunk_at<kM>(r, gb >> 3);
         uint32_t h[8], lo[8];
