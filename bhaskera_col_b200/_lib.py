@@ -165,14 +165,12 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
             "tq_shared_free": (I32, [VP]),
             "tq_tables_bytes": (SZ, [P(Geom)]),
             "tq_init_tables": (I32, [P(Geom), VP, VP, VP, VP, VP, VP, VP, SZ, P(Tables), VP]),
-            "tq_qk_rope": (I32, [P(Rope), P(Positions), P(Tensor4), P(Tensor4), P(HeadNorm),
-                                 P(Tensor4), P(Tensor4), P(HeadNorm), VP]),
-            "tq_append_ragged": (I32, [P(Geom), P(Tables), P(Cache), P(Tensor4), P(Tensor4),
-                                       P(Ragged), P(Rope), P(HeadNorm), P(Positions), VP]),
-            "tq_dequantize_ragged": (I32, [P(Geom), P(Tables), P(Cache), P(Ragged), P(Tensor4),
-                                           P(Tensor4), VP]),
-            "tq_attend_ragged_workspace_bytes": (SZ, [P(Geom), P(Cache), P(AttendArgs)]),
-            "tq_attend_ragged": (I32, [P(Geom), P(Tables), P(Cache), P(AttendArgs), VP, SZ, VP]),
+            # descriptors of the serving operators are packed by ops.py: addresses
+            "tq_qk_rope": (I32, [VP] * 9),
+            "tq_append_ragged": (I32, [VP] * 10),
+            "tq_dequantize_ragged": (I32, [VP] * 7),
+            "tq_attend_ragged_workspace_bytes": (SZ, [VP] * 3),
+            "tq_attend_ragged": (I32, [VP] * 5 + [SZ, VP]),
         }
         for name, (res, args) in sig.items():
             fn = getattr(lib, name)

@@ -55,6 +55,7 @@
 #include "tq_internal.h"
 #include "tq_tc.cuh"
 
+#include <atomic>
 #include <mutex>
 
 namespace tq {
@@ -709,11 +710,19 @@ int launch_append_tc(const tq_geom* G, const tq_tables* t, const tq_cache* c,
 }
 
 uint32_t* device_status_word() {
+  // looked up once per device: the address does not move
+  static std::atomic<uint32_t*> known[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) dev = -1;
+  if (dev >= 0 && dev < 64)
+    if (uint32_t* w = known[dev].load(std::memory_order_relaxed)) return w;
   void* addr = nullptr;
   if (cudaGetSymbolAddress(&addr, g_tc_status) != cudaSuccess) {
     cudaGetLastError();
     return nullptr;
   }
+  if (dev >= 0 && dev < 64)
+    known[dev].store(static_cast<uint32_t*>(addr), std::memory_order_relaxed);
   return static_cast<uint32_t*>(addr);
 }
 

@@ -9,6 +9,8 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
+import struct
+import threading
 from dataclasses import dataclass
 from typing import Optional
 
@@ -513,14 +515,15 @@ class RaggedBatch:
 
 def _inference_only(name: str, device: torch.device, *ts) -> None:
     """All tensors on ``device`` (CUDA) and none that a backward pass would need."""
+    if device.type != "cuda":
+        raise RuntimeError("TurboQuant kernels need CUDA tensors (there is no CPU path)")
+    grad = torch.is_grad_enabled()
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise RuntimeError("TurboQuant kernels need CUDA tensors (there is no CPU path)")
         if t.device != device:
             raise ValueError(f"{name}: tensors on {device} and {t.device}")
-        if t.requires_grad and torch.is_grad_enabled():
+        if grad and t.requires_grad:
             raise RuntimeError(f"{name} has no backward pass: call it under torch.no_grad() or "
                                "with detached tensors")
 
@@ -532,33 +535,76 @@ def _on(device: torch.device):
     return torch.cuda.device(device)
 
 
-def _rows(x: torch.Tensor, name: str) -> _lib.Tensor4:
+class _Descriptors(threading.local):
+    """The C descriptors of one call of this thread, packed into one buffer: a
+    ctypes structure costs 2 us to fill, more than the kernels of a small step."""
+
+    def __init__(self):
+        self.buf = ctypes.create_string_buffer(1024)
+        self.base = ctypes.addressof(self.buf)
+
+
+_desc = _Descriptors()
+_T4, _POS, _CACHE = (struct.Struct(f) for f in ("@Pi8q", "@Pi2q", "@PqqPqq"))
+_ATTEND = struct.Struct("@PPqPPqfii")
+# where each descriptor of a call lies in the buffer
+_AT_Q, _AT_QO, _AT_K, _AT_KO, _AT_POS, _AT_CACHE, _AT_ARGS = 0, 128, 256, 384, 512, 576, 640
+for _s, _c in ((_T4, _lib.Tensor4), (_POS, _lib.Positions), (_CACHE, _lib.Cache),
+               (_ATTEND, _lib.AttendArgs)):
+    assert _s.size <= ctypes.sizeof(_c) <= 128
+
+
+def _rows(at: int, x: Optional[torch.Tensor], name: str) -> Optional[int]:
     """A flattened (N, H, D) tensor as the (1, H, N, D) view of the C ABI."""
+    if x is None:
+        return None
+    dt = _DT.get(x.dtype)
     if x.dim() != 3:
         raise ValueError(f"{name} must be (rows, heads, head_dim), got shape {tuple(x.shape)}")
-    if x.dtype not in _DT:
+    if dt is None:
         raise ValueError(f"unsupported dtype {x.dtype} of {name}")
     n, h, d = x.shape
-    s = x.stride()
-    return _lib.Tensor4(x.data_ptr(), _DT[x.dtype], (1, h, n, d), (0, s[1], s[0], s[2]))
+    sn, sh, sd = x.stride()
+    _T4.pack_into(_desc.buf, at, x.data_ptr(), dt, 1, h, n, d, 0, sh, sn, sd)
+    return _desc.base + at
 
 
-def _heads(x: torch.Tensor, name: str) -> _lib.Tensor4:
-    return tensor4(x) if x.dim() == 4 else _rows(x, name)
+def _heads(at: int, x: Optional[torch.Tensor], name: str) -> Optional[int]:
+    if x is None or x.dim() != 4:
+        return _rows(at, x, name)
+    dt = _DT.get(x.dtype)
+    if dt is None:
+        raise ValueError(f"unsupported dtype {x.dtype} of {name}")
+    _T4.pack_into(_desc.buf, at, x.data_ptr(), dt, *x.shape, *x.stride())
+    return _desc.base + at
 
 
-def _positions(pos: Optional[torch.Tensor], b: int, t: int) -> Optional[_lib.Positions]:
+def _positions(pos: Optional[torch.Tensor], b: int, t: int) -> Optional[int]:
     if pos is None:
         return None
     if pos.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"positions must be int32 or int64, got {pos.dtype}")
-    if tuple(pos.shape) == (b, t):
-        stride = pos.stride()
-    elif tuple(pos.shape) == (t,):
+    shape = tuple(pos.shape)
+    if shape == (t,):
         stride = (0, pos.stride(0))
+    elif shape == (b, t):
+        stride = pos.stride()
     else:
-        raise ValueError(f"positions must be ({t},) or ({b}, {t}), got {tuple(pos.shape)}")
-    return _lib.Positions(pos.data_ptr(), 64 if pos.dtype == torch.int64 else 32, stride)
+        raise ValueError(f"positions must be ({t},) or ({b}, {t}), got {shape}")
+    _POS.pack_into(_desc.buf, _AT_POS, pos.data_ptr(), 64 if pos.dtype == torch.int64 else 32,
+                   *stride)
+    return _desc.base + _AT_POS
+
+
+def _pages(pages) -> int:
+    if isinstance(pages, PagedPages):
+        bt, pool = pages.block_table, pages.pool
+        _CACHE.pack_into(_desc.buf, _AT_CACHE, pool.data_ptr(), bt.shape[0], bt.shape[1],
+                         bt.data_ptr(), bt.stride(0), pool.shape[0])
+    else:
+        _CACHE.pack_into(_desc.buf, _AT_CACHE, pages.data_ptr(), pages.shape[0], pages.shape[1],
+                         0, 0, 0)
+    return _desc.base + _AT_CACHE
 
 
 def _check_norm(norm: Optional[HeadNorm], d: int) -> None:
@@ -597,13 +643,11 @@ def qk_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], rope: Optional
     if k is not None:
         _check_norm(k_norm, k.shape[-1])
         k_out = torch.empty_like(k) if k_out is None else k_out
-    ts = [None if x is None else _heads(x, n) for x, n in
-          ((q, "q"), (q_out, "q_out"), (k, "k"), (k_out, "k_out"))]
-    pos = _positions(positions, b, t)
     with _on(one.device):
         _lib.check("tq_qk_rope", _lib.load().tq_qk_rope(
-            _ref(rope and rope._c), _ref(pos), _ref(ts[0]), _ref(ts[1]), _ref(q_norm and q_norm._c),
-            _ref(ts[2]), _ref(ts[3]), _ref(k_norm and k_norm._c), _stream(one.device)))
+            _ref(rope and rope._c), _positions(positions, b, t), _heads(_AT_Q, q, "q"),
+            _heads(_AT_QO, q_out, "q_out"), _ref(q_norm and q_norm._c), _heads(_AT_K, k, "k"),
+            _heads(_AT_KO, k_out, "k_out"), _ref(k_norm and k_norm._c), _stream(one.device)))
     return q_out, k_out
 
 
@@ -620,13 +664,12 @@ def append_ragged(tables: LayerTables, pages, k: torch.Tensor, v: torch.Tensor,
                     rope.cos_sin if rope is not None else None,
                     k_norm.weight if k_norm is not None else None)
     _check_norm(k_norm, k.shape[-1])
-    kt, vt, c = _rows(k, "k"), _rows(v, "v"), _cache_desc(pages)
-    pos = _positions(positions, 1, k.shape[0])
     with _on(k.device):
         _lib.check("tq_append_ragged", _lib.load().tq_append_ragged(
-            ctypes.byref(tables.geom()), ctypes.byref(tables.ctables()), ctypes.byref(c),
-            ctypes.byref(kt), ctypes.byref(vt), ctypes.byref(batch._c), _ref(rope and rope._c),
-            _ref(k_norm and k_norm._c), _ref(pos), _stream(k.device)))
+            ctypes.byref(tables.geom()), ctypes.byref(tables.ctables()), _pages(pages),
+            _rows(_AT_K, k, "k"), _rows(_AT_KO, v, "v"), ctypes.byref(batch._c),
+            _ref(rope and rope._c), _ref(k_norm and k_norm._c),
+            _positions(positions, 1, k.shape[0]), _stream(k.device)))
 
 
 def dequantize_ragged(tables: LayerTables, pages, batch: RaggedBatch,
@@ -638,13 +681,11 @@ def dequantize_ragged(tables: LayerTables, pages, batch: RaggedBatch,
     if one is None:
         raise ValueError("neither k_out nor v_out is given")
     _inference_only("dequantize_ragged", one.device, k_out, v_out, batch.q_start)
-    kt = _rows(k_out, "k_out") if k_out is not None else None
-    vt = _rows(v_out, "v_out") if v_out is not None else None
-    c = _cache_desc(pages)
     with _on(one.device):
         _lib.check("tq_dequantize_ragged", _lib.load().tq_dequantize_ragged(
-            ctypes.byref(tables.geom()), ctypes.byref(tables.ctables()), ctypes.byref(c),
-            ctypes.byref(batch._c), _ref(kt), _ref(vt), _stream(one.device)))
+            ctypes.byref(tables.geom()), ctypes.byref(tables.ctables()), _pages(pages),
+            ctypes.byref(batch._c), _rows(_AT_K, k_out, "k_out"), _rows(_AT_KO, v_out, "v_out"),
+            _stream(one.device)))
 
 
 def attend_ragged(tables: LayerTables, pages, q: torch.Tensor, batch: RaggedBatch,
@@ -664,19 +705,19 @@ def attend_ragged(tables: LayerTables, pages, q: torch.Tensor, batch: RaggedBatc
     if out is None:
         out = torch.empty_like(q)
     lib = _lib.load()
-    qt, ot = _rows(q, "q"), _rows(out, "out")
-    g, c = tables.geom(), _cache_desc(pages)
-    a = _lib.AttendArgs(ctypes.pointer(qt), ctypes.pointer(ot), batch._c,
-                        float(scale if scale is not None else 1.0 / math.sqrt(q.shape[-1])),
-                        1 if causal else 0, int(engine))
+    g, c, bc = ctypes.byref(tables.geom()), _pages(pages), batch._c
+    _ATTEND.pack_into(_desc.buf, _AT_ARGS, _rows(_AT_Q, q, "q"), _rows(_AT_QO, out, "out"),
+                      bc.requests, bc.q_start, bc.seq_lens, bc.max_q_len,
+                      scale if scale is not None else 1.0 / math.sqrt(q.shape[-1]),
+                      1 if causal else 0, int(engine))
+    args = _desc.base + _AT_ARGS
     with _on(q.device):
-        nbytes = lib.tq_attend_ragged_workspace_bytes(ctypes.byref(g), ctypes.byref(c),
-                                                      ctypes.byref(a))
+        nbytes = lib.tq_attend_ragged_workspace_bytes(g, c, args)
         if nbytes == 0:
             raise _lib.TqError("tq_attend_ragged_workspace_bytes", _lib.TQ_ERR_INVALID,
                                _lib.last_error())
         ws = (workspace or DecodeWorkspace()).get(nbytes, q.device)
         _lib.check("tq_attend_ragged", lib.tq_attend_ragged(
-            ctypes.byref(g), ctypes.byref(tables.ctables()), ctypes.byref(c), ctypes.byref(a),
-            ws.data_ptr(), ws.numel(), _stream(q.device)))
+            g, ctypes.byref(tables.ctables()), c, args, ws.data_ptr(), ws.numel(),
+            _stream(q.device)))
     return out
