@@ -20,176 +20,144 @@ namespace tq {
 namespace {
 
 constexpr int kPlanThreads = 1024;
+constexpr int kClasses = 32;               // length classes of segments
 constexpr int kWaves = 3;                  // segments wanted per SM
 constexpr int kMinKeys = 512;              // shortest segment worth a CTA's set-up
-constexpr int kFewWaves = 6, kFewMinKeys = 512;   // the same for the few-row kernel
+constexpr int kFewWaves = 5, kFewMinKeys = 512;   // the same for the few-row kernel
 
 struct PlanParams {
   RaggedView rv;
   int64_t q_lo, q_hi;                      // the list's requests: q_lo < q_len <= q_hi
-  int pcta, keys;                          // query positions per tile, keys per key tile
+  int pcta, keys, key_shift;               // query positions per tile, keys per key tile (2^shift)
   int causal, G;
   int64_t wanted;                          // segments wanted, all head groups together
   int min_tiles, max_seg, max_slot;
   RaggedSeg* segs;
   int32_t* nseg;
+  int32_t* next;
   int32_t* arrived;
   uint32_t* status;
 };
 
-// Key tiles of query block i of a request.
-__device__ __forceinline__ int key_tiles(const PlanParams& p, const Request& q, int64_t i) {
-  int64_t kend = q.seq;
-  if (p.causal) kend = q.seq - q.q_len + tmin<int64_t>((i + 1) * p.pcta, q.q_len);
-  return kend > 0 ? (int)((kend + p.keys - 1) / p.keys) : 0;
+// A listed request in the plan's terms.
+struct Tiles {
+  int tiles, q_len, seq;
+};
+
+__device__ __forceinline__ Tiles listed_request(const PlanParams& p, int64_t r) {
+  Tiles t = {0, 0, 0};
+  if (r >= p.rv.R) return t;
+  const Request q = request_at(p.rv, r);
+  if (q.q_len <= p.q_lo || q.q_len > p.q_hi) return t;
+  t.q_len = (int)q.q_len;
+  t.seq = (int)q.seq;
+  t.tiles = (t.q_len + p.pcta - 1) / p.pcta;
+  return t;
 }
 
-// Request r, empty where it belongs to the other list.
-__device__ __forceinline__ Request listed_request(const PlanParams& p, int64_t r) {
-  Request q = {};
-  if (r < p.rv.R) q = request_at(p.rv, r);
-  if (q.q_len <= p.q_lo || q.q_len > p.q_hi) q.q_len = 0;
-  return q;
+// Key tiles of query block i.
+__device__ __forceinline__ int key_tiles(const PlanParams& p, const Tiles& t, int i) {
+  int kend = t.seq;
+  if (p.causal) kend = t.seq - t.q_len + (int)tmin<int64_t>((int64_t)(i + 1) * p.pcta, t.q_len);
+  return kend > 0 ? (kend + p.keys - 1) >> p.key_shift : 0;
 }
 
-// Inclusive scan over the block of a pair of counts packed as hi:lo 32 bits.
-__device__ __forceinline__ uint64_t block_scan(uint64_t x, uint64_t* warp_tot, uint64_t& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint64_t y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
+// f(request, tile, key tiles) for every tile: a thread per request, a warp
+// for a request of more than 32 tiles.
+template <class F>
+__device__ __forceinline__ void for_tiles(const PlanParams& p, F f) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  for (int64_t r0 = 0; r0 < p.rv.R; r0 += kPlanThreads) {
+    const Tiles t = listed_request(p, r0 + tid);
+    if (t.tiles <= 32)
+      for (int i = 0; i < t.tiles; ++i) f((int)(r0 + tid), i, key_tiles(p, t, i));
+    for (unsigned big = __ballot_sync(0xffffffffu, t.tiles > 32); big; big &= big - 1) {
+      const int src = __ffs(big) - 1;
+      Tiles b;
+      b.tiles = __shfl_sync(0xffffffffu, t.tiles, src);
+      b.q_len = __shfl_sync(0xffffffffu, t.q_len, src);
+      b.seq = __shfl_sync(0xffffffffu, t.seq, src);
+      for (int i = lane; i < b.tiles; i += 32) f((int)(r0 + (tid & ~31) + src), i, key_tiles(p, b, i));
+    }
   }
-  if (lane == 31) warp_tot[warp] = x;
-  __syncthreads();
-  uint64_t before = 0;
-  total = 0;
-  for (int w = 0; w < kPlanThreads / 32; ++w) {
-    if (w < warp) before += warp_tot[w];
-    total += warp_tot[w];
-  }
-  __syncthreads();
-  return x + before;
 }
 
-// One CTA, one thread per request; a request of more than 32 tiles is walked
-// by its whole warp.  Pass 0 sums the key tiles, pass 1 counts and writes the
-// segments (in request and tile order: the list does not depend on timing).
+// One CTA per list.  Pass 0 sums the key tiles, pass 1 counts the segments of
+// each length class, pass 2 writes them, long classes first (whatever is taken
+// last should be short).  Places within a class come from atomics, so the
+// order varies from run to run; results do not depend on it: a tile's segments
+// have consecutive slots and are joined in slot order.
 __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p0, PlanParams p1) {
-  const PlanParams& p = blockIdx.x == 0 ? p0 : p1;         // one CTA per list
-  __shared__ uint64_t warp_tot[kPlanThreads / 32];
+  const PlanParams& p = blockIdx.x == 0 ? p0 : p1;
+  __shared__ unsigned long long all;
+  __shared__ unsigned place[kClasses + 1];                 // segments per class, then their next place
+  __shared__ unsigned slots;
   const int tid = threadIdx.x, lane = tid & 31;
   for (int i = tid; i < p.max_slot * p.G; i += kPlanThreads) p.arrived[i] = 0;
-  // f(request, tile, lane's turn) for every tile of this thread's request
-  uint64_t total = 0, sum = 0;
-  for (int64_t r0 = 0; r0 < p.rv.R; r0 += kPlanThreads) {
-    const int64_t r = r0 + tid;
-    const Request q = listed_request(p, r);
-    const int64_t tiles = (q.q_len + p.pcta - 1) / p.pcta;
-    uint64_t mine = 0;
-    if (tiles <= 32)
-      for (int64_t i = 0; i < tiles; ++i) mine += key_tiles(p, q, i);
-    for (unsigned big = __ballot_sync(0xffffffffu, tiles > 32); big; big &= big - 1) {
-      const int src = __ffs(big) - 1;
-      Request bq;
-      bq.q0 = 0;
-      bq.q_len = __shfl_sync(0xffffffffu, q.q_len, src);
-      bq.seq = __shfl_sync(0xffffffffu, q.seq, src);
-      const int64_t bt = __shfl_sync(0xffffffffu, tiles, src);
-      uint64_t part = 0;
-      for (int64_t i = lane; i < bt; i += 32) part += key_tiles(p, bq, i);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-      if (lane == src) mine = part;
-    }
-    block_scan(mine, warp_tot, sum);
-    total += sum;
+  if (tid == 0) {
+    all = 0;
+    slots = 0;
+    *p.next = 0;
   }
-  const int64_t all = (int64_t)total * p.G;
-  const int L = (int)tmax<int64_t>(p.min_tiles, (all + p.wanted - 1) / p.wanted);
-
-  // segments (low word) and partial slots (high word) of one tile
-  auto cuts = [&](int nkt) -> uint64_t {
-    const uint64_t ns = nkt > L ? (uint64_t)((nkt + L - 1) / L) : 1;
-    return ns | (ns > 1 ? ns << 32 : 0);
-  };
-  auto put = [&](int64_t r, int64_t i, int nkt, uint64_t at) {
-    const int ns = (int)(uint32_t)cuts(nkt);
-    const int64_t seg = (uint32_t)at, slot = (uint32_t)(at >> 32);
-    if (seg + ns > p.max_seg || (ns > 1 && slot + ns > p.max_slot)) return;   // see below
+  if (tid <= kClasses) place[tid] = 0;
+  __syncthreads();
+  unsigned long long mine = 0;
+  for_tiles(p, [&](int, int, int nkt) { mine += nkt; });
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) atomicAdd(&all, mine);
+  __syncthreads();
+  const unsigned long long total = all * (unsigned)p.G;
+  const int L = (int)tmax<unsigned long long>(p.min_tiles, (total + p.wanted - 1) / p.wanted);
+  // class of a segment of n key tiles: 0 the longest (L), 31 the shortest
+  auto class_of = [&](int n) { return kClasses - 1 - (int)((unsigned)(n * kClasses - 1) / (unsigned)L); };
+  for_tiles(p, [&](int, int, int nkt) {
+    const int ns = nkt > L ? (nkt + L - 1) / L : 1;
+    atomicAdd(&place[class_of(tmax(1, (nkt + ns - 1) / ns))], (unsigned)ns);
+    if (ns > 1) atomicAdd(&slots, (unsigned)ns);
+  });
+  __syncthreads();
+  if (tid < 32) {
+    // exclusive sums of the classes; the bounds of the list hold for ascending
+    // offsets, and a batch that breaks them is not run
+    const unsigned own = place[lane];
+    unsigned x = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    place[lane] = x - own;
+    if (lane == 31) {
+      const bool ok = x <= (unsigned)p.max_seg && slots <= (unsigned)p.max_slot;
+      if (!ok) atomicOr(p.status, TQ_DEV_BAD_BATCH);
+      place[kClasses] = ok;
+      *p.nseg = ok ? (int)x : 0;
+      slots = 0;
+    }
+  }
+  __syncthreads();
+  if (!place[kClasses]) return;
+  for_tiles(p, [&](int r, int i, int nkt) {
+    const int ns = nkt > L ? (nkt + L - 1) / L : 1;
+    const int base = nkt / ns, more = nkt - base * ns;     // `more` segments take one tile extra
+    const unsigned at = atomicAdd(&place[class_of(tmax(1, (nkt + ns - 1) / ns))], (unsigned)ns);
+    const unsigned slot = ns > 1 ? atomicAdd(&slots, (unsigned)ns) : 0;
+    int kt = 0;
     for (int s = 0; s < ns; ++s) {
       RaggedSeg g;
-      g.req = (int32_t)r;
-      g.tile = (int32_t)i;
-      g.kt0 = (int32_t)((int64_t)nkt * s / ns);
-      g.kt1 = (int32_t)((int64_t)nkt * (s + 1) / ns);
-      g.slot = ns > 1 ? (int32_t)slot + s : -1;
-      g.first = (int32_t)slot;
+      g.req = r;
+      g.tile = i;
+      g.kt0 = kt;
+      kt += base + (s < more);
+      g.kt1 = kt;
+      g.slot = ns > 1 ? (int)slot + s : -1;
+      g.first = (int)slot;
       g.parts = ns;
       g.pad = 0;
-      p.segs[seg + s] = g;
+      p.segs[at + s] = g;
     }
-  };
-  uint64_t base = 0;
-  for (int64_t r0 = 0; r0 < p.rv.R; r0 += kPlanThreads) {
-    const int64_t r = r0 + tid;
-    const Request q = listed_request(p, r);
-    const int64_t tiles = (q.q_len + p.pcta - 1) / p.pcta;
-    uint64_t mine = 0;
-    if (tiles <= 32)
-      for (int64_t i = 0; i < tiles; ++i) mine += cuts(key_tiles(p, q, i));
-    const unsigned bigs = __ballot_sync(0xffffffffu, tiles > 32);
-    for (unsigned big = bigs; big; big &= big - 1) {
-      const int src = __ffs(big) - 1;
-      Request bq;
-      bq.q0 = 0;
-      bq.q_len = __shfl_sync(0xffffffffu, q.q_len, src);
-      bq.seq = __shfl_sync(0xffffffffu, q.seq, src);
-      const int64_t bt = __shfl_sync(0xffffffffu, tiles, src);
-      uint64_t part = 0;
-      for (int64_t i = lane; i < bt; i += 32) part += cuts(key_tiles(p, bq, i));
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-      if (lane == src) mine = part;
-    }
-    uint64_t at = base + block_scan(mine, warp_tot, sum) - mine;
-    base += sum;
-    if (tiles <= 32)
-      for (int64_t i = 0; i < tiles; ++i) {
-        const int nkt = key_tiles(p, q, i);
-        put(r, i, nkt, at);
-        at += cuts(nkt);
-      }
-    for (unsigned big = bigs; big; big &= big - 1) {
-      const int src = __ffs(big) - 1;
-      Request bq;
-      bq.q0 = 0;
-      bq.q_len = __shfl_sync(0xffffffffu, q.q_len, src);
-      bq.seq = __shfl_sync(0xffffffffu, q.seq, src);
-      const int64_t bt = __shfl_sync(0xffffffffu, tiles, src);
-      const int64_t br = __shfl_sync(0xffffffffu, r, src);
-      uint64_t run = __shfl_sync(0xffffffffu, at, src);
-      for (int64_t i0 = 0; i0 < bt; i0 += 32) {
-        const int64_t i = i0 + lane;
-        const int nkt = i < bt ? key_tiles(p, bq, i) : 0;
-        const uint64_t own = i < bt ? cuts(nkt) : 0;
-        uint64_t x = own;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint64_t y = __shfl_up_sync(0xffffffffu, x, o);
-          if (lane >= o) x += y;
-        }
-        if (i < bt) put(br, i, nkt, run + x - own);
-        run += __shfl_sync(0xffffffffu, x, 31);
-      }
-    }
-  }
-  // the bounds hold for ascending offsets; a batch that breaks them is not run
-  if (tid == 0) {
-    const bool ok = (uint32_t)base <= (uint32_t)p.max_seg && (base >> 32) <= (uint64_t)p.max_slot;
-    if (!ok) atomicOr(p.status, TQ_DEV_BAD_BATCH);
-    *p.nseg = ok ? (int32_t)(uint32_t)base : 0;
-  }
+  });
 }
 
 // Shape of one list's launch: head group, query positions and rows of a CTA,
@@ -262,7 +230,7 @@ AttendShape attend_shape(const tq_geom* G, const tq_cache* c, const tq_attend_ar
     l.pcta = l.rows / l.hc;
     l.keys = s.tc ? 2 * kPageTokens : kPageTokens;
     l.wanted = (int64_t)kWaves * device_sm_count();
-    l.off_nseg = 68;
+    l.off_nseg = 72;
     finish(l);
   }
   s.bytes = off;
@@ -298,6 +266,8 @@ int launch_attend_ragged(const tq_geom* G, const tq_tables* t, const tq_cache* c
     p.max_seg = (int)l->max_seg;
     p.max_slot = (int)l->max_slot;
     p.nseg = reinterpret_cast<int32_t*>(base + l->off_nseg);
+    p.next = p.nseg + 1;
+    p.key_shift = l->keys == 64 ? 6 : 7;
     p.segs = reinterpret_cast<RaggedSeg*>(base + l->off_segs);
     p.arrived = reinterpret_cast<int32_t*>(base + l->off_arrived);
     p.status = status;
@@ -305,6 +275,7 @@ int launch_attend_ragged(const tq_geom* G, const tq_tables* t, const tq_cache* c
     r.rv = p.rv;
     r.plan.segs = p.segs;
     r.plan.nseg = p.nseg;
+    r.plan.next = p.next;
     r.plan.arrived = p.arrived;
     r.plan.ml = reinterpret_cast<float2*>(base + l->off_ml);
     r.plan.part = reinterpret_cast<float*>(base + l->off_part);

@@ -14,11 +14,11 @@
 // for V), so both operands go from one coalesced global load per row straight
 // into fragment registers, through a table indexed by a byte of codes: the
 // half2 of a pair of 4-bit codes, or of pairs of 2-bit codes of two rows (6 bits of
-// two 3-bit codes take a shift and a mask instead).  Copies for 32 (16: 8-byte
-// entries are served in halves of a warp) lanes leave no bank conflicts, K in
-// the first and V in the second 128 bytes of a 256-byte row, so one byte
-// permute of the codes is the offset.  V pairs join the codes of two tokens,
-// interleaved by two masks per word.
+// two 3-bit codes take a shift and a mask instead).  Copies for 32 lanes (16 of
+// 8-byte entries, which are served in halves of a warp) leave no bank conflicts
+// and make a row 128 bytes, so one dot product of the codes' word is the
+// address.  V pairs join the codes of two tokens, interleaved by two masks per
+// word.
 // The running max moves only when a score passes it by kRoom (a vote; the
 // shuffles and the rescale of 32 NT outputs run then: nearly every tile has a
 // new max among its 16 rows, so moving it at once cost a fifth of the time).
@@ -66,15 +66,14 @@ template <int D, int KB, int VB, int NT>
 struct Few {
   static constexpr int NQ = 8 * NT;
   static constexpr bool KQ = KB == 2, VQ = VB == 2;         // two pairs per table entry
-  static constexpr int KF = KQ ? 8 : 2 * KB, VF = VQ ? 8 : 2 * VB;   // bits of an index
-  static constexpr int ROWS = 1 << (KF > VF ? KF : VF);     // table rows of 256 bytes
+  static constexpr int KT = 128 << (KQ ? 8 : 2 * KB), VT = 128 << (VQ ? 8 : 2 * VB);   // tables
   static constexpr int LDO = D + 4;                         // floats per row of an output (banks)
   static constexpr int LDA = D / 2 + 4;                     // words per row of a rotation operand
   // after the loop the table is dead: partial outputs, then the joined one and
   // the operand of the last rotation take its place
   static constexpr int OFF_P = 0;                           // [kW][NQ][LDO]
   static constexpr int OFF_A = kW * NQ * LDO * 4;           // [2: hi, lo][16][LDA] fp16 pairs
-  static constexpr int LOOP = ROWS * 256, END = OFF_A + 2 * 16 * LDA * 4;
+  static constexpr int LOOP = KT + VT, END = OFF_A + 2 * 16 * LDA * 4;
   static constexpr int OFF_Q = LOOP > END ? LOOP : END;     // q' fp16 [NQ][D]
   static constexpr int OFF_M = OFF_Q + 16 * D * 2;          // [kW][NQ] running max
   static constexpr int OFF_L = OFF_M + kW * NQ * 4;         // [kW][NQ] sums
@@ -120,38 +119,45 @@ __device__ __forceinline__ int code_start(int off, uint32_t& sh) {
   return odd ? off & ~3 : off;
 }
 
-// Table offset of field `k` (FB bits each, low first) of the words, for this
-// lane: (field << 8) | lane offset.
+// Shared address of the table row of field `k` (FB bits each, low first) of the
+// words: base + 128 field.  A byte takes one dot product with 128 in its place.
 template <int FB, int NW>
-__device__ __forceinline__ uint32_t field_at(const uint32_t (&w)[NW], int k, uint32_t lane_off) {
+__device__ __forceinline__ uint32_t field_at(const uint32_t (&w)[NW], int k, uint32_t base) {
   const int bo = FB * k, wi = bo >> 5, sh = bo & 31;
   if constexpr (FB == 8) {
-    return __byte_perm(w[wi], lane_off, 0x5504u | (uint32_t)((sh >> 3) << 4));
+    return __dp4a(w[wi], 128u << sh, base);
   } else {
-    constexpr uint32_t mask = ((1u << FB) - 1u) << 8;
+    constexpr uint32_t mask = ((1u << FB) - 1u) << 7;
     uint32_t x;
-    if (sh + FB > 32) x = __funnelshift_r(w[wi], w[wi + 1 < NW ? wi + 1 : wi], sh) << 8;
-    else if (sh >= 8) x = w[wi] >> (sh - 8);
-    else x = w[wi] << (8 - sh);
-    return (x & mask) | lane_off;
+    if (sh + FB > 32) x = __funnelshift_r(w[wi], w[wi + 1 < NW ? wi + 1 : wi], sh) << 7;
+    else if (sh >= 7) x = w[wi] >> (sh - 7);
+    else x = w[wi] << (7 - sh);
+    return (x & mask) + base;
   }
+}
+
+// volatile: not to be moved over the barriers around the table's lifetime
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ void lds64(uint32_t addr, uint32_t& x, uint32_t& y) {
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(x), "=r"(y) : "r"(addr));
 }
 
 // One pair of each of two rows (registers a0 and a1, or a2 and a3, of an A
 // fragment): field k of x and of y, or, with quad entries, byte k of x.
 template <int FB, bool Q, int NW>
-__device__ __forceinline__ void look_up2(const unsigned char* table, const uint32_t (&x)[NW],
-                                         const uint32_t (&y)[NW], int k, uint32_t lane_off,
-                                         uint32_t& r0, uint32_t& r1) {
+__device__ __forceinline__ void look_up2(uint32_t base, const uint32_t (&x)[NW],
+                                         const uint32_t (&y)[NW], int k, uint32_t& r0,
+                                         uint32_t& r1) {
   if constexpr (Q) {
     // bytes of even fields lie in x, of odd fields in y (join_nibbles)
-    const uint32_t at = (k & 1) ? field_at<8>(y, k >> 1, lane_off) : field_at<8>(x, k >> 1, lane_off);
-    const uint2 v = *reinterpret_cast<const uint2*>(table + at);
-    r0 = v.x;
-    r1 = v.y;
+    lds64((k & 1) ? field_at<8>(y, k >> 1, base) : field_at<8>(x, k >> 1, base), r0, r1);
   } else {
-    r0 = *reinterpret_cast<const uint32_t*>(table + field_at<FB>(x, k, lane_off));
-    r1 = *reinterpret_cast<const uint32_t*>(table + field_at<FB>(y, k, lane_off));
+    r0 = lds32(field_at<FB>(x, k, base));
+    r1 = lds32(field_at<FB>(y, k, base));
   }
 }
 
@@ -240,9 +246,9 @@ __device__ __forceinline__ void rotate_tile(float (&c)[4], const float* m, const
   }
 }
 
-// One 128-byte half of the table's rows from a codebook.
+// A table of 128-byte rows from a codebook.
 template <int BITS, bool Q>
-__device__ __forceinline__ void fill_table(unsigned char* half, const float* cent, int tid,
+__device__ __forceinline__ void fill_table(unsigned char* table, const float* cent, int tid,
                                            int nthreads) {
   constexpr int N = 1 << (Q ? 4 * BITS : 2 * BITS);
   constexpr uint32_t M = (1u << BITS) - 1u;
@@ -251,19 +257,18 @@ __device__ __forceinline__ void fill_table(unsigned char* half, const float* cen
     const uint32_t x = pack_half2(__ldg(cent + (e & M)), __ldg(cent + ((e >> BITS) & M)));
     const uint32_t y = Q ? pack_half2(__ldg(cent + ((e >> (2 * BITS)) & M)),
                                       __ldg(cent + ((e >> (3 * BITS)) & M))) : x;
-    reinterpret_cast<uint4*>(half + e * 256)[i & 7] = make_uint4(x, y, x, y);
+    reinterpret_cast<uint4*>(table + e * 128)[i & 7] = make_uint4(x, y, x, y);
   }
 }
 
+// One segment of the work list.
 template <int D, int KB, int VB, int NT>
-__global__ void __launch_bounds__(32 * kW, 3) attend_few_kernel(FewParams p) {
+__device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork& sw,
+                                               unsigned char* sm) {
   using F = Few<D, KB, VB, NT>;
   using Tile = FewTile<D, KB, VB>;
   constexpr int NQ = F::NQ, NC = D / 16, kThreads = 32 * kW, LDA = F::LDA, LDO = F::LDO;
   constexpr int KROW = D * KB / 8, VROW = D * VB / 8;
-  extern __shared__ __align__(128) unsigned char sm[];
-  SegWork sw;
-  if (!take_segment(p.rg, sw)) return;
   float* mw = reinterpret_cast<float*>(sm + F::OFF_M);
   float* lw = reinterpret_cast<float*>(sm + F::OFF_L);
   float* U = reinterpret_cast<float*>(sm + F::OFF_P);
@@ -362,7 +367,7 @@ __global__ void __launch_bounds__(32 * kW, 3) attend_few_kernel(FewParams p) {
   }
   __syncthreads();                                         // the table takes A's place
   fill_table<KB, F::KQ>(sm, p.kc, tid, kThreads);
-  fill_table<VB, F::VQ>(sm + 128, p.vc, tid, kThreads);
+  fill_table<VB, F::VQ>(sm + F::KT, p.vc, tid, kThreads);
   __syncthreads();
 
   // ---- pages -----------------------------------------------------------------------
@@ -386,8 +391,8 @@ __global__ void __launch_bounds__(32 * kW, 3) attend_few_kernel(FewParams p) {
     }
   lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, 1));
   lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, 2));
-  const uint32_t k_lane = F::KQ ? 8 * (lane & 15) : 4 * lane;
-  const uint32_t v_lane = 128 + (F::VQ ? 8 * (lane & 15) : 4 * lane);
+  const uint32_t k_base = smem_u32(sm) + (F::KQ ? 8 * (lane & 15) : 4 * lane);
+  const uint32_t v_base = smem_u32(sm + F::KT) + (F::VQ ? 8 * (lane & 15) : 4 * lane);
   int bad_key = INT_MAX;
 
   // one page: `cur` is used, `nxt` takes the next page's codes
@@ -426,8 +431,8 @@ __global__ void __launch_bounds__(32 * kW, 3) attend_few_kernel(FewParams p) {
         uint32_t a[4];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          look_up2<2 * KB, F::KQ>(sm, cur.k[0].w, cur.k[1].w, 2 * (2 * c2 + c) + i, k_lane,
-                                  a[2 * i], a[2 * i + 1]);
+          look_up2<2 * KB, F::KQ>(k_base, cur.k[0].w, cur.k[1].w, 2 * (2 * c2 + c) + i, a[2 * i],
+                                  a[2 * i + 1]);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
           mma_f16_16816(s[n], a, c ? qb[n].z : qb[n].x, c ? qb[n].w : qb[n].y);
@@ -491,7 +496,7 @@ __global__ void __launch_bounds__(32 * kW, 3) attend_few_kernel(FewParams p) {
       uint32_t a[4];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        look_up2<2 * VB, F::VQ>(sm, ve[i], vo[i], c, v_lane, a[2 * i], a[2 * i + 1]);
+        look_up2<2 * VB, F::VQ>(v_base, ve[i], vo[i], c, a[2 * i], a[2 * i + 1]);
 #pragma unroll
       for (int n = 0; n < NT; ++n) mma_f16_16816(O[c][n], a, pb[n][0], pb[n][1]);
     }
@@ -632,6 +637,20 @@ __global__ void __launch_bounds__(32 * kW, 3) attend_few_kernel(FewParams p) {
   }
 }
 
+template <int D, int KB, int VB, int NT>
+__global__ void __launch_bounds__(32 * kW, 3) attend_few_kernel(FewParams p) {
+  extern __shared__ __align__(128) unsigned char sm[];
+  // segments in the list's order (long ones first), whoever is free next
+  __shared__ int next;
+  while (true) {
+    __syncthreads();                                       // the last segment is done with
+    if (threadIdx.x == 0) next = atomicAdd(p.rg.plan.next, 1);
+    __syncthreads();
+    SegWork sw;
+    if (!take_segment(p.rg, next, sw)) return;
+    attend_segment<D, KB, VB, NT>(p, sw, sm);
+  }
+}
 using FewFn = void (*)(FewParams);
 
 template <int D, int NT>
@@ -694,7 +713,9 @@ int launch_attend_few(const tq_geom* G, const tq_tables* t, const tq_cache* c,
     if (rows == 8) pick(std::integral_constant<int, 64>(), I1()); else pick(std::integral_constant<int, 64>(), I2());
   }
   if (set_smem_attr((const void*)fn, bytes) != TQ_OK) return TQ_ERR_CUDA;
-  fn<<<(unsigned)grid, 32 * kW, bytes, st>>>(p);
+  // CTAs that fit at once
+  const int64_t fit = (int64_t)device_sm_count() * occupancy((const void*)fn, 32 * kW, bytes);
+  fn<<<(unsigned)tmin(grid, fit), 32 * kW, bytes, st>>>(p);
   return check_launch("tq_attend_ragged/few");
 }
 

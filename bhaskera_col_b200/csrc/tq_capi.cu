@@ -732,7 +732,7 @@ static int check_attend(const tq_geom* g, const tq_cache* c, const tq_attend_arg
     return TQ_ERR_INVALID;
   }
   if ((c->block_table ? c->num_blocks : c->streams * c->pages_per_stream) > INT32_MAX ||
-      c->pages_per_stream > INT32_MAX / TQ_PAGE_TOKENS) {
+      c->pages_per_stream > INT32_MAX / TQ_PAGE_TOKENS / 2) {
     set_error("%s: more pages than 32 bits count", fn);
     return TQ_ERR_INVALID;
   }

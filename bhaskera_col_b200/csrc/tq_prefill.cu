@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
   int64_t group = blockIdx.y;                          // (b, kv head, chunk of its query heads)
   __shared__ int bad_key, last_flag;
   if constexpr (RG) {
-    if (!take_segment(p.rg, sw)) return;
+    if (!take_segment(p.rg, blockIdx.x, sw)) return;
     qb = sw.seg.tile;
     group = sw.seg.req * (p.Hkv * nchunk) + sw.group;
     p.Tq = sw.rq.q_len;

@@ -75,7 +75,7 @@ __device__ __forceinline__ bool take_job(TcPrefillParams& p, int pcta, Job& j) {
   int64_t group = blockIdx.y;
   j.qb = p.nqb - 1 - (int)blockIdx.x;                  // long rows first
   if constexpr (RG) {
-    if (!take_segment(p.rg, j.sw)) return false;
+    if (!take_segment(p.rg, blockIdx.x, j.sw)) return false;
     j.qb = j.sw.seg.tile;
     group = j.sw.seg.req * (p.Hkv * nchunk) + j.sw.group;
     p.Tq = j.sw.rq.q_len;

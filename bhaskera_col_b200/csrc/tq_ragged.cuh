@@ -115,6 +115,7 @@ struct RaggedSeg {
 struct RaggedPlan {
   const RaggedSeg* segs;
   const int32_t* nseg;
+  int32_t* next;              // next (segment, head group) to be taken
   int32_t* arrived;           // [slots][G] finished segments of the tile, at its first slot
   float* part;                // [slots][G][rows][D] partial outputs
   float2* ml;                 // [slots][G][rows] running max (log2) and sum
@@ -134,10 +135,10 @@ struct SegWork {
   int group;
 };
 
-// false: no segment for this CTA (the grid is an upper bound).
-__device__ __forceinline__ bool take_segment(const RaggedAttend& a, SegWork& w) {
-  const int si = (int)(blockIdx.x / (unsigned)a.plan.G);
-  w.group = (int)(blockIdx.x % (unsigned)a.plan.G);
+// Item `i` of the list (segment x head group); false past its end.
+__device__ __forceinline__ bool take_segment(const RaggedAttend& a, unsigned i, SegWork& w) {
+  const int si = (int)(i / (unsigned)a.plan.G);
+  w.group = (int)(i % (unsigned)a.plan.G);
   if (si >= *a.plan.nseg) return false;
   w.seg = a.plan.segs[si];
   w.rq = request_at(a.rv, w.seg.req);
