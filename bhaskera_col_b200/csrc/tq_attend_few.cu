@@ -81,35 +81,40 @@ struct Few {
   static constexpr int BYTES = OFF_R + 256;
 };
 
-// N consecutive bytes of codes as little-endian words.  Multiples of 4 are
-// aligned loads; other counts load the words that hold them and shift by `sh`.
+// N consecutive bytes of codes as little-endian words.  Multiples of 4 (and 2)
+// are aligned loads; for other counts the words that hold them, shifted by `sh`
+// when they are used: a prefetched value must not be touched before that.
 template <int N>
-struct Codes { uint32_t w[(N + 3) / 4]; };
-
-template <int N>
-__device__ __forceinline__ Codes<N> load_codes(const uint8_t* p, uint32_t sh) {
-  Codes<N> c;
-  if constexpr (N == 16) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-    c.w[0] = v.x; c.w[1] = v.y; c.w[2] = v.z; c.w[3] = v.w;
-  } else if constexpr (N == 8) {
-    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-    c.w[0] = v.x; c.w[1] = v.y;
-  } else if constexpr (N % 4 == 0) {
+struct Codes {
+  static constexpr bool kOdd = N % 4 != 0 && N != 2;
+  static constexpr int NW = (N + 3) / 4, NR = kOdd ? 2 : NW;
+  uint32_t raw[NR];
+  __device__ __forceinline__ void load(const uint8_t* p) {
+    if constexpr (N == 16) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+      raw[0] = v.x; raw[1] = v.y; raw[2] = v.z; raw[3] = v.w;
+    } else if constexpr (N == 8) {
+      const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+      raw[0] = v.x; raw[1] = v.y;
+    } else if constexpr (N == 2) {
+      raw[0] = __ldg(reinterpret_cast<const uint16_t*>(p));
+    } else {
+      // 3 or 6 bytes: two words (the second may lie past the row, but within
+      // the page: norms follow the codes)
 #pragma unroll
-    for (int i = 0; i < N / 4; ++i) c.w[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
-  } else if constexpr (N == 2) {
-    c.w[0] = __ldg(reinterpret_cast<const uint16_t*>(p));
-  } else {
-    // 3 or 6 bytes: two words (the second may lie past the row, but within
-    // the page: norms follow the codes)
-    const uint32_t a = __ldg(reinterpret_cast<const uint32_t*>(p));
-    const uint32_t b = __ldg(reinterpret_cast<const uint32_t*>(p) + 1);
-    c.w[0] = __funnelshift_r(a, b, sh);
-    if constexpr (N > 4) c.w[1] = b >> sh;
+      for (int i = 0; i < NR; ++i) raw[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
+    }
   }
-  return c;
-}
+  __device__ __forceinline__ void words(uint32_t (&w)[NW], uint32_t sh) const {
+    if constexpr (kOdd) {
+      w[0] = __funnelshift_r(raw[0], raw[1], sh);
+      if constexpr (NW > 1) w[1] = raw[1] >> sh;
+    } else {
+#pragma unroll
+      for (int i = 0; i < NW; ++i) w[i] = raw[i];
+    }
+  }
+};
 
 // Aligned start and shift of N bytes at offset `off`.
 template <int N>
@@ -180,10 +185,9 @@ __device__ __forceinline__ const uint8_t* page_at(const uint8_t* base, int e, in
 
 // Fields of two tokens' VB-bit codes joined into pairs: even entries in e, odd
 // ones in o (2 VB bits each, entry 2 k (+ 1) at field k).
-template <int VB, int N>
-__device__ __forceinline__ void join_tokens(const Codes<N>& a, const Codes<N>& b,
-                                            uint32_t (&e)[(N + 3) / 4], uint32_t (&o)[(N + 3) / 4]) {
-  constexpr int NW = (N + 3) / 4;
+template <int VB, int NW>
+__device__ __forceinline__ void join_tokens(const uint32_t (&a)[NW], const uint32_t (&b)[NW],
+                                            uint32_t (&e)[NW], uint32_t (&o)[NW]) {
   // VB bits of every 2 VB, continued across the words
 #pragma unroll
   for (int i = 0; i < NW; ++i) {
@@ -191,13 +195,13 @@ __device__ __forceinline__ void join_tokens(const Codes<N>& a, const Codes<N>& b
 #pragma unroll
     for (int t = 0; t < 32; ++t)
       if ((((32 * i + t) / VB) & 1) == 0) m |= 1u << t;
-    const uint32_t am = a.w[i] & m;
-    uint32_t bl = b.w[i] << VB;                            // b's even codes up by VB
-    if (i > 0) bl = __funnelshift_l(b.w[i - 1], b.w[i], VB);
+    const uint32_t am = a[i] & m;
+    uint32_t bl = b[i] << VB;                              // b's even codes up by VB
+    if (i > 0) bl = __funnelshift_l(b[i - 1], b[i], VB);
     e[i] = am | (bl & ~m);
-    uint32_t ar = a.w[i] >> VB;                            // a's odd codes down by VB
-    if (i + 1 < NW) ar = __funnelshift_r(a.w[i], a.w[i + 1], VB);
-    o[i] = (ar & m) | (b.w[i] & ~m);
+    uint32_t ar = a[i] >> VB;                              // a's odd codes down by VB
+    if (i + 1 < NW) ar = __funnelshift_r(a[i], a[i + 1], VB);
+    o[i] = (ar & m) | (b[i] & ~m);
   }
 }
 
@@ -206,7 +210,7 @@ struct FewTile {
   static constexpr int KN = D / 4 * KB / 8, VN = D / 8 * VB / 8;
   Codes<KN> k[2];               // tokens gq, gq + 8: quad tq
   Codes<VN> v[4];               // tokens 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9: octet gq
-  uint32_t n[2];                // fp16 norms of tokens gq, gq + 8: k low, v high
+  uint16_t kn[2], vn[2];        // fp16 norms of tokens gq, gq + 8
 };
 
 // fp16 hi + lo of a pair (2^-22 of each value)
@@ -321,13 +325,12 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
     const uint8_t* n = page_at(pn, e, p.page_bytes);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      x.k[i] = load_codes<Tile::KN>(k + 8 * i * KROW, ksh);
-      x.n[i] = (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(n + 16 * i)) |
-               ((uint32_t)__ldg(reinterpret_cast<const uint16_t*>(n + 128 + 16 * i)) << 16);
+      x.k[i].load(k + 8 * i * KROW);
+      x.kn[i] = __ldg(reinterpret_cast<const uint16_t*>(n + 16 * i));
+      x.vn[i] = __ldg(reinterpret_cast<const uint16_t*>(n + 128 + 16 * i));
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      x.v[i] = load_codes<Tile::VN>(v + ((i & 1) + 8 * (i >> 1)) * VROW, vsh);
+    for (int i = 0; i < 4; ++i) x.v[i].load(v + ((i & 1) + 8 * (i >> 1)) * VROW);
   };
   int pg = sw.seg.kt0;
   const bool any = pg < pend;
@@ -406,7 +409,7 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
     // NaN at the end
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      uint32_t h = cur.n[i];
+      uint32_t h = (uint32_t)cur.kn[i] | ((uint32_t)cur.vn[i] << 16);
       const bool in = key0 + 8 * i < kend;
       // exponent 31 in either half carries into its sign bit
       const bool fin = (((h & 0x7FFF7FFFu) + 0x04000400u) & 0x80008000u) == 0;
@@ -418,7 +421,10 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-    if (F::KQ) join_nibbles(cur.k[0].w, cur.k[1].w);
+    uint32_t kw[2][Codes<Tile::KN>::NW];
+    cur.k[0].words(kw[0], ksh);
+    cur.k[1].words(kw[1], ksh);
+    if (F::KQ) join_nibbles(kw[0], kw[1]);
     // S^T: two chunks of 16 dims share one 16-byte piece of q'
 #pragma unroll
     for (int c2 = 0; c2 < NC / 2; ++c2) {
@@ -431,8 +437,7 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
         uint32_t a[4];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          look_up2<2 * KB, F::KQ>(k_base, cur.k[0].w, cur.k[1].w, 2 * (2 * c2 + c) + i, a[2 * i],
-                                  a[2 * i + 1]);
+          look_up2<2 * KB, F::KQ>(k_base, kw[0], kw[1], 2 * (2 * c2 + c) + i, a[2 * i], a[2 * i + 1]);
 #pragma unroll
         for (int n = 0; n < NT; ++n)
           mma_f16_16816(s[n], a, c ? qb[n].z : qb[n].x, c ? qb[n].w : qb[n].y);
@@ -485,10 +490,14 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
         pb[n][i] = movmatrix_trans(pack_half2(p0 * vn[i], p1 * vn[i]));
       }
     }
-    uint32_t ve[2][(Tile::VN + 3) / 4], vo[2][(Tile::VN + 3) / 4];
+    constexpr int VW = Codes<Tile::VN>::NW;
+    uint32_t ve[2][VW], vo[2][VW];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      join_tokens<VB>(cur.v[2 * i], cur.v[2 * i + 1], ve[i], vo[i]);
+      uint32_t x[VW], y[VW];
+      cur.v[2 * i].words(x, vsh);
+      cur.v[2 * i + 1].words(y, vsh);
+      join_tokens<VB>(x, y, ve[i], vo[i]);
       if (F::VQ) join_nibbles(ve[i], vo[i]);
     }
 #pragma unroll
