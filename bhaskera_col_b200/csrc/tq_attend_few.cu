@@ -335,10 +335,11 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
   int pg = sw.seg.kt0;
   const bool any = pg < pend;
   Tile cur, nxt;
-  int e_next = 0;
+  int e_next = 0, e_after = 0;
   if (any) {
-    load_tile(cur, entry(pg));
     e_next = entry(pg + 1);
+    e_after = entry(pg + 2);
+    load_tile(cur, entry(pg));
   }
 
   // ---- query rows, table ---------------------------------------------------------
@@ -401,7 +402,11 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
   // one page: `cur` is used, `nxt` takes the next page's codes
   auto step = [&](Tile& cur, Tile& nxt) {
     load_tile(nxt, e_next);
-    e_next = entry(pg + 2);
+    e_next = e_after;
+    if (warp == 0 && lane == 0 && (unsigned)e_after < (unsigned)nblocks)
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;"
+                   ::"l"(page_at(p.pages, e_after, p.page_bytes)), "r"(p.page_bytes) : "memory");
+    e_after = entry(pg + 3);
     const int key0 = 64 * pg + s0 + gq;
     float kn[2], vn[2], s[NT][4];
     // norms: 0 past the end; a token whose norm is not finite counts as 0 (0 x
