@@ -79,6 +79,7 @@ struct Few {
   static constexpr int OFF_L = OFF_M + kW * NQ * 4;         // [kW][NQ] sums
   static constexpr int OFF_R = OFF_L + kW * NQ * 4;         // [16] sums, [16] maxima, flags
   static constexpr int BYTES = OFF_R + 256;
+  static_assert(OFF_Q - OFF_A >= 8 * NQ * 16, "room for a batch of parts");
 };
 
 // N consecutive bytes of codes as little-endian words.  Multiples of 4 (and 2)
@@ -590,29 +591,72 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
     }
     if (tid < NQ) pl.ml[part_row(pl, sw.seg.slot, sw.group, tid)] = make_float2(rowl[16 + tid], rowl[tid]);
     if (!last_of_tile(pl, sw, &flags[0])) return;
-    for (int n = warp; n < NQ; n += kW) {
-      if (!row_valid(n)) continue;
-      float M = kNoMax;
-      for (int s = lane; s < sw.seg.parts; s += 32)
-        M = fmaxf(M, __ldcg(pl.ml + part_row(pl, sw.seg.first + s, sw.group, n)).x);
+    // every part's {m, l} in one trip, then the weights 2^(m - M); parts come in
+    // slot order whatever the order of arrival
+    const int parts = sw.seg.parts;
+    float2* wl = reinterpret_cast<float2*>(sm + F::OFF_A);   // [parts][NQ] of a batch of parts
+    constexpr int kBatch = (F::OFF_Q - F::OFF_A) / (8 * NQ);
+    constexpr int NE = NQ * D / 4 / kThreads;              // float4 columns per thread
+    float4 acc[NE];
+    const float* src[NE];                                  // the first part's values, or NULL
+    const int64_t next_part = (int64_t)pl.G * pl.rows * D;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-      float sum = 0.f, acc[D / 32];
+    for (int k = 0; k < NE; ++k) {
+      const int i = tid + k * kThreads, n = i / (D / 4);
+      acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      src[k] = row_valid(n) ? pl.part + part_row(pl, sw.seg.first, sw.group, n) * D + 4 * (i % (D / 4))
+                            : nullptr;
+    }
+    float run_m = kNoMax, run_l = 0.f;                     // of row tid (tid < NQ)
+    for (int s0 = 0; s0 < parts; s0 += kBatch) {
+      const int ns = min(kBatch, parts - s0);
+      for (int i = tid; i < ns * NQ; i += kThreads)
+        wl[i] = __ldcg(pl.ml + part_row(pl, sw.seg.first + s0 + i / NQ, sw.group, i % NQ));
+      __syncthreads();
+      if (tid < NQ) {
+        float M = run_m;
+        for (int s = 0; s < ns; ++s) M = fmaxf(M, wl[s * NQ + tid].x);
+        const float f = fast_exp2(run_m - M);              // of what earlier batches left
+        run_l *= f;
+        for (int s = 0; s < ns; ++s) {
+          const float w = fast_exp2(wl[s * NQ + tid].x - M);
+          run_l = fmaf(w, wl[s * NQ + tid].y, run_l);
+          wl[s * NQ + tid].x = w;
+        }
+        run_m = M;
+        rowl[tid] = f;
+      }
+      __syncthreads();
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+      for (int k = 0; k < NE; ++k) {
+        const int n = (tid + k * kThreads) / (D / 4);
+        const float f = rowl[n];
+        acc[k].x *= f; acc[k].y *= f; acc[k].z *= f; acc[k].w *= f;
+      }
 #pragma unroll 4
-      for (int s = 0; s < sw.seg.parts; ++s) {
-        const int64_t pr = part_row(pl, sw.seg.first + s, sw.group, n);
-        const float2 ml = __ldcg(pl.ml + pr);
-        const float w = fast_exp2(ml.x - M);
-        sum = fmaf(w, ml.y, sum);
+      for (int s = 0; s < ns; ++s) {
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) acc[i] = fmaf(w, __ldcg(pl.part + pr * D + 32 * i + lane), acc[i]);
+        for (int k = 0; k < NE; ++k) {
+          if (!src[k]) continue;
+          const float4 x = __ldcg(reinterpret_cast<const float4*>(src[k] + s * next_part));
+          const float w = wl[s * NQ + (tid + k * kThreads) / (D / 4)].x;
+          acc[k].x = fmaf(w, x.x, acc[k].x);
+          acc[k].y = fmaf(w, x.y, acc[k].y);
+          acc[k].z = fmaf(w, x.z, acc[k].z);
+          acc[k].w = fmaf(w, x.w, acc[k].w);
+        }
       }
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) U[n * LDO + 32 * i + lane] = acc[i];
-      if (lane == 0) rowl[n] = sum;
+      for (int k = 0; k < NE; ++k)
+        if (src[k]) src[k] += ns * next_part;
+      __syncthreads();
     }
+#pragma unroll
+    for (int k = 0; k < NE; ++k) {
+      const int i = tid + k * kThreads;
+      *reinterpret_cast<float4*>(U + i / (D / 4) * LDO + 4 * (i % (D / 4))) = acc[k];
+    }
+    if (tid < NQ) rowl[tid] = run_l;
     __syncthreads();
   }
 
