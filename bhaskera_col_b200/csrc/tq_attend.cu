@@ -82,12 +82,112 @@ __device__ __forceinline__ void for_tiles(const PlanParams& p, F f) {
   }
 }
 
-// One CTA per list.  Pass 0 sums the key tiles, pass 1 counts the segments of
+// ---------------------------------------------------------------------------
+// q' = scale log2(e) q R^T of the few-row list's queries, fp16 in quad order:
+// CTAs of the plan's launch beside the lists' own.
+// ---------------------------------------------------------------------------
+struct QueryParams {
+  const void* q; int q_dtype; int q_vec; int64_t qs[3];    // head, row, dim; 16-byte pieces
+  const __half* rot_h;
+  __half* qp;
+  int64_t qp_stride;                                       // FewParams::qp_stride
+  float qscale;
+  int Hq, D, blocks;                                       // blocks of 64 rows looked at per request
+};
+
+constexpr int kQRows = 64;
+
+// 32 warps: four tiles of 16 rows, eight warps each, every eighth 8-wide slice
+// of the result.
+template <int D>
+__device__ __forceinline__ void rotate_queries(const PlanParams& p, const QueryParams& qp, int first,
+                                               int step, unsigned char* sm) {
+  constexpr int LD = D + 8;                                // halves per staged row (banks)
+  __half* A = reinterpret_cast<__half*>(sm);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, tq = lane & 3;
+  for (int64_t item = first; item < p.rv.R * qp.blocks; item += step) {
+    const int64_t r = item / qp.blocks;
+    const Request rq = request_at(p.rv, r);
+    if (rq.q_len <= p.q_lo || rq.q_len > p.q_hi) continue;
+    const int64_t tok0 = qp.qp_stride ? r * qp.qp_stride : rq.q0;
+    const int64_t rows = rq.q_len * qp.Hq;
+    for (int64_t row0 = (item % qp.blocks) * kQRows; row0 < rows; row0 += (int64_t)qp.blocks * kQRows) {
+      __syncthreads();
+      for (int i = tid; i < kQRows * D / 8; i += kPlanThreads) {
+        const int n = i / (D / 8), c = i % (D / 8);
+        const int row = (int)row0 + n;
+        uint32_t w[4] = {0u, 0u, 0u, 0u};
+        if (row < rows) {
+          const int tok = row / qp.Hq, h = row - tok * qp.Hq;
+          const int64_t at = (rq.q0 + tok) * qp.qs[1] + h * qp.qs[0] + (int64_t)(8 * c) * qp.qs[2];
+          if (qp.q_vec) {
+            const uint4 x = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(qp.q) + at));
+            const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = qp.q_dtype == TQ_F16
+                                   ? __half22float2(*reinterpret_cast<const __half2*>(&u[e]))
+                                   : make_float2(__uint_as_float(u[e] << 16),
+                                                 __uint_as_float(u[e] & 0xFFFF0000u));
+              w[e] = pack_half2(f.x * qp.qscale, f.y * qp.qscale);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = pack_half2(load_elem(qp.q, qp.q_dtype, at + (2 * e) * qp.qs[2]) * qp.qscale,
+                                load_elem(qp.q, qp.q_dtype, at + (2 * e + 1) * qp.qs[2]) * qp.qscale);
+          }
+        }
+        *reinterpret_cast<uint4*>(A + n * LD + 8 * c) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      __syncthreads();
+      const int m0 = 16 * (warp >> 3);
+      for (int jt = warp & 7; jt < D / 8; jt += 8) {
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t b[D / 16][2];
+        const uint32_t* R = reinterpret_cast<const uint32_t*>(qp.rot_h + (8 * jt + gq) * D) + tq;
+#pragma unroll
+        for (int ch = 0; ch < D / 16; ++ch) {
+          b[ch][0] = __ldg(R + 8 * ch);
+          b[ch][1] = __ldg(R + 8 * ch + 4);
+        }
+#pragma unroll
+        for (int ch = 0; ch < D / 16; ++ch) {
+          uint32_t a[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            a[i] = *reinterpret_cast<const uint32_t*>(A + (m0 + gq + 8 * (i & 1)) * LD + 16 * ch +
+                                                      2 * tq + 8 * (i >> 1));
+          mma_f16_16816(c, a, b[ch][0], b[ch][1]);
+        }
+        // dims 8 jt + 2 tq, + 1: word jt of quad tq
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int64_t row = row0 + m0 + gq + 8 * i;
+          if (row < rows)
+            reinterpret_cast<uint32_t*>(qp.qp + (tok0 * qp.Hq + row) * D)[tq * (D / 8) + jt] =
+                pack_half2(c[2 * i], c[2 * i + 1]);
+        }
+      }
+    }
+  }
+}
+
+// One CTA per list (and the queries' CTAs).  Pass 0 sums the key tiles, pass 1 counts the segments of
 // each length class, pass 2 writes them, long classes first (whatever is taken
 // last should be short).  Places within a class come from atomics, so the
 // order varies from run to run; results do not depend on it: a tile's segments
 // have consecutive slots and are joined in slot order.
-__global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p0, PlanParams p1) {
+__global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p0, PlanParams p1,
+                                                                   int lists, QueryParams qp) {
+  pdl_launch_dependents();
+  if ((int)blockIdx.x >= lists) {
+    __shared__ __align__(16) unsigned char sm[kQRows * (128 + 8) * 2];
+    const int first = blockIdx.x - lists, step = gridDim.x - lists;
+    if (qp.D == 128) rotate_queries<128>(p0, qp, first, step, sm);
+    else rotate_queries<64>(p0, qp, first, step, sm);
+    return;
+  }
   const PlanParams& p = blockIdx.x == 0 ? p0 : p1;
   __shared__ unsigned long long all;
   __shared__ unsigned place[kClasses + 1];                 // segments per class, then their next place
@@ -167,12 +267,12 @@ struct ListShape {
   int64_t q_lo, q_hi;
   int hc, pcta, rows, keys, G;
   int64_t wanted, max_seg, max_slot;
-  size_t off_nseg, off_segs, off_arrived, off_ml, off_part;
+  size_t off_nseg, off_segs, off_arrived, off_ml, off_part, off_qp;
 };
 
 struct AttendShape {
   bool tc;                                 // the wide list runs on tcgen05
-  int64_t Hkv;
+  int64_t Hkv, qp_stride;
   ListShape few, wide;
   size_t bytes;
 };
@@ -218,6 +318,9 @@ AttendShape attend_shape(const tq_geom* G, const tq_cache* c, const tq_attend_ar
     l.wanted = (int64_t)kFewWaves * device_sm_count();
     l.off_nseg = 64;
     finish(l);
+    // q' rows of its tokens: beside a wide list at most few_q of each request
+    s.qp_stride = wide ? few_q : 0;
+    l.off_qp = take((size_t)(wide ? R * few_q : N) * a->q->shape[1] * G->head_dim * 2);
   }
   if (wide) {
     ListShape& l = s.wide;
@@ -282,11 +385,29 @@ int launch_attend_ragged(const tq_geom* G, const tq_tables* t, const tq_cache* c
     r.plan.G = l->G;
     r.plan.rows = l->rows;
   }
-  ragged_plan_kernel<<<lists, kPlanThreads, 0, st>>>(plan[0], plan[lists - 1]);
+  QueryParams qp = {};
+  int query_ctas = 0;
+  if (s.few.used) {
+    qp.q = a->q->data;
+    qp.q_dtype = a->q->dtype;
+    for (int i = 0; i < 3; ++i) qp.qs[i] = a->q->stride[i + 1];
+    qp.q_vec = qp.q_dtype != TQ_F32 && qp.qs[2] == 1 && reinterpret_cast<uintptr_t>(qp.q) % 16 == 0 &&
+               qp.qs[0] % 8 == 0 && qp.qs[1] % 8 == 0;
+    qp.rot_h = reinterpret_cast<const __half*>(t->rot_f16);
+    qp.qp = reinterpret_cast<__half*>(base + s.few.off_qp);
+    qp.qp_stride = s.qp_stride;
+    qp.qscale = a->scale * 1.4426950408889634f;
+    qp.Hq = (int)a->q->shape[1];
+    qp.D = G->head_dim;
+    const int64_t most = s.qp_stride ? s.qp_stride : tmax<int64_t>(a->batch.max_q_len, 1);
+    qp.blocks = (int)tmin<int64_t>((most * qp.Hq + kQRows - 1) / kQRows, 1 << 16);
+    query_ctas = (int)tmin<int64_t>(a->batch.requests * qp.blocks, device_sm_count());
+  }
+  ragged_plan_kernel<<<lists + query_ctas, kPlanThreads, 0, st>>>(plan[0], plan[lists - 1], lists, qp);
   if (check_launch("tq_attend_ragged/plan") != TQ_OK) return TQ_ERR_CUDA;
   if (s.few.used) {
     const int rc = launch_attend_few(G, t, c, a, rg[0], s.Hkv, s.few.hc, s.few.pcta, s.few.rows,
-                                     s.few.max_seg * s.few.G, status, st);
+                                     qp.qp, s.qp_stride, s.few.max_seg * s.few.G, status, st);
     if (rc != TQ_OK) return rc;
   }
   if (s.wide.used && s.tc)

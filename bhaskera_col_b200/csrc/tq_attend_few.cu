@@ -23,9 +23,9 @@
 // shuffles and the rescale of 32 NT outputs run then: nearly every tile has a
 // new max among its 16 rows, so moving it at once cost a fifth of the time).
 //
-// q' = scale log2(e) q R^T and out = O R run on the same MMAs with both sides
-// split into fp16 hi + lo (three products, 2^-22), once per CTA and once per
-// output row.
+// q' = scale log2(e) q R^T comes ready from the launch that builds the work list
+// (rotated in every segment it was most of a segment's set-up); out = O R runs on
+// the same MMAs with O split into fp16 hi + lo, once per output row.
 #include "tq_internal.h"
 #include "tq_ragged.cuh"
 
@@ -36,7 +36,6 @@
 namespace tq {
 namespace {
 
-constexpr float kLog2eF = 1.4426950408889634f;
 // A score may pass the running max by this much before the max moves: p <=
 // 2^7, and with a value norm of at most 2^8 P' <= 2^15 stays in fp16 (for
 // larger norms the max moves at once, p <= 1 and P' <= the norm itself).
@@ -47,14 +46,14 @@ struct FewParams {
   const uint8_t* pages;
   PageMap pm;
   int page_bytes, off_v, off_kn, off_vn;
-  const float* rot;             // R [D][D]
-  const float* rot_t;           // R^T [D][D]
+  const __half* rot_h;          // R [D][D] fp16
+  const __half* qp;             // q' rows (ragged_plan_kernel), [token][Hq][D] in quad order
+  int64_t qp_stride;            // tokens of q' per request; 0: q' follows the batch's rows
   const float* kc;
   const float* vc;
-  const void* q; int q_dtype; int64_t qs[3];     // head, row, dim
-  void* out; int o_dtype; int64_t os[3];
+  void* out; int o_dtype; int o_pair; int64_t os[3];   // head, row, dim; pairs in one store
   int Hkv, g, hc, nchunk, pcta;
-  float qscale;                 // softmax scale x log2(e)
+  int Hq;
   int causal;
   uint32_t* status;
   RaggedAttend rg;
@@ -71,8 +70,9 @@ struct Few {
   static constexpr int LDA = D / 2 + 4;                     // words per row of a rotation operand
   // after the loop the table is dead: partial outputs, then the joined one and
   // the operand of the last rotation take its place
-  static constexpr int OFF_P = 0;                           // [kW][NQ][LDO]
-  static constexpr int OFF_A = kW * NQ * LDO * 4;           // [2: hi, lo][16][LDA] fp16 pairs
+  static constexpr int OFF_P = 0;                           // [kW][NQ][LDO], the sum in the first
+  static constexpr int OFF_ROT = (NQ * LDO * 4 + 127) & ~127;      // R fp16, over the other three
+  static constexpr int OFF_A = tmax(OFF_ROT + 2 * D * D, kW * NQ * LDO * 4);   // [hi, lo][16][LDA]
   static constexpr int LOOP = KT + VT, END = OFF_A + 2 * 16 * LDA * 4;
   static constexpr int OFF_Q = LOOP > END ? LOOP : END;     // q' fp16 [NQ][D]
   static constexpr int OFF_M = OFF_Q + 16 * D * 2;          // [kW][NQ] running max
@@ -221,34 +221,15 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
   lo = pack_half2(a - __low2float(h), b - __high2float(h));
 }
 
-// c[16 rows][8 cols] = a[16][D] M[cols][D]^T: the rows of a as fp16 pairs hi and
-// lo in shared memory, M fp32 row-major with this n-tile's rows at `m`.
-template <int D, int LDA>
-__device__ __forceinline__ void rotate_tile(float (&c)[4], const float* m, const uint32_t* a,
-                                            int lane) {
-  const int gq = lane >> 2, tq = lane & 3;
-  c[0] = c[1] = c[2] = c[3] = 0.f;
-  float2 mv[D / 16][2];
-#pragma unroll
-  for (int ch = 0; ch < D / 16; ++ch) {
-    mv[ch][0] = __ldg(reinterpret_cast<const float2*>(m + gq * D + 16 * ch + 2 * tq));
-    mv[ch][1] = __ldg(reinterpret_cast<const float2*>(m + gq * D + 16 * ch + 2 * tq + 8));
-  }
-#pragma unroll
-  for (int ch = 0; ch < D / 16; ++ch) {
-    uint32_t bh[2], bl[2], ah[4], al[4];
-    split2(mv[ch][0].x, mv[ch][0].y, bh[0], bl[0]);
-    split2(mv[ch][1].x, mv[ch][1].y, bh[1], bl[1]);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int at = (gq + 8 * (i & 1)) * LDA + 8 * ch + tq + 4 * (i >> 1);
-      ah[i] = a[at];
-      al[i] = a[16 * LDA + at];
-    }
-    mma_f16_16816(c, ah, bh[0], bh[1]);
-    mma_f16_16816(c, al, bh[0], bh[1]);
-    mma_f16_16816(c, ah, bl[0], bl[1]);
-  }
+// B fragment (16 deep, 8 wide) of R[j][i], j = 16 ch + .. deep, i = 8 jt + .. wide,
+// from R's fp16 rows in shared memory, their 16-byte pieces moved by row (r7).
+template <int D>
+__device__ __forceinline__ void frag_of_rotation(uint32_t (&b)[2], const unsigned char* r, int ch,
+                                                 int jt, int lane) {
+  const int row = 16 * ch + (lane & 15);
+  const unsigned char* at = r + row * (2 * D) + ((jt ^ (row & 7)) << 4);
+  asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];"
+               : "=r"(b[0]), "=r"(b[1]) : "r"(smem_u32(at)));
 }
 
 // A table of 128-byte rows from a codebook.
@@ -345,34 +326,23 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
 
   // ---- query rows, table ---------------------------------------------------------
   if (tid == 0) flags[1] = INT_MAX;
-  for (int i = tid; i < 16 * D / 2; i += kThreads) {
-    const int n = i / (D / 2), w = i % (D / 2);
-    float x = 0.f, y = 0.f;
-    if (n < NQ && row_valid(n)) {
-      const int64_t o = row_at(n, p.qs) + (int64_t)(2 * w) * p.qs[2];
-      x = p.qscale * load_elem(p.q, p.q_dtype, o);
-      y = p.qscale * load_elem(p.q, p.q_dtype, o + p.qs[2]);
-    }
-    split2(x, y, A[n * LDA + w], A[(16 + n) * LDA + w]);
-  }
-  __syncthreads();
   // 16-byte piece k of row n, quad t of q' (quad order): its place in the row
   auto q_piece = [](int n, int t, int k) {
     const int f = D == 128 ? ((t >> 1) | ((n & 1) << 1)) : (n & 1);
     return n * (D / 8) + t * (D / 32) + (k ^ f);
   };
-#pragma unroll 1
-  for (int jt = warp; jt < D / 8; jt += kW) {
-    float c[4];
-    rotate_tile<D, LDA>(c, p.rot + 8 * jt * D, A, lane);
-    // pair (8 jt + 2 tq, + 1): word jt of quad tq
-    uint32_t* qw = reinterpret_cast<uint32_t*>(sm + F::OFF_Q);
-    qw[4 * q_piece(gq, tq, jt >> 2) + (jt & 3)] = pack_half2(c[0], c[1]);
-    if (NQ > 8) qw[4 * q_piece(gq + 8, tq, jt >> 2) + (jt & 3)] = pack_half2(c[2], c[3]);
+  const int64_t tok0 = p.qp_stride ? sw.seg.req * p.qp_stride : sw.rq.q0;
+  for (int i = tid; i < NQ * D / 8; i += kThreads) {
+    const int n = i / (D / 8), c = i % (D / 8);
+    unsigned char* dst = sm + F::OFF_Q + 16 * q_piece(n, c / (D / 32), c % (D / 32));
+    if (row_valid(n))
+      cp_async16(dst, p.qp + ((tok0 + row_pos(n)) * p.Hq + h0 + n % p.hc) * D + 8 * c);
+    else
+      *reinterpret_cast<uint4*>(dst) = make_uint4(0u, 0u, 0u, 0u);
   }
-  __syncthreads();                                         // the table takes A's place
   fill_table<KB, F::KQ>(sm, p.kc, tid, kThreads);
   fill_table<VB, F::VQ>(sm + F::KT, p.vc, tid, kThreads);
+  cp_async_wait_all();
   __syncthreads();
 
   // ---- pages -----------------------------------------------------------------------
@@ -579,6 +549,11 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
     *reinterpret_cast<float4*>(U + at) = x;
   }
   __syncthreads();
+  // R for the last rotation, on its way while a split tile's parts come together
+  for (int i = tid; i < D * D / 8; i += kThreads) {
+    const int r = i / (D / 8), c = i % (D / 8);
+    cp_async16(sm + F::OFF_ROT + r * (2 * D) + ((c ^ (r & 7)) << 4), p.rot_h + 8 * i);
+  }
 
   // ---- a split tile: partials out, the last CTA joins them -----------------------
   if (sw.seg.slot >= 0) {
@@ -590,7 +565,10 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
             *reinterpret_cast<const float4*>(U + n * LDO + at);
     }
     if (tid < NQ) pl.ml[part_row(pl, sw.seg.slot, sw.group, tid)] = make_float2(rowl[16 + tid], rowl[tid]);
-    if (!last_of_tile(pl, sw, &flags[0])) return;
+    if (!last_of_tile(pl, sw, &flags[0])) {
+      cp_async_wait_all();                                 // nothing in flight into what comes next
+      return;
+    }
     // every part's {m, l} in one trip, then the weights 2^(m - M); parts come in
     // slot order whatever the order of arrival
     const int parts = sw.seg.parts;
@@ -672,6 +650,7 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
     }
     split2(u.x, u.y, A[n * LDA + w], A[(16 + n) * LDA + w]);
   }
+  cp_async_wait_all();
   __syncthreads();
   int64_t o_at[2];
   bool o_ok[2];
@@ -683,14 +662,32 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
   }
 #pragma unroll 1
   for (int jt = warp; jt < D / 8; jt += kW) {
-    float c[4];
-    rotate_tile<D, LDA>(c, p.rot_t + 8 * jt * D, A, lane);
+    float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ch = 0; ch < NC; ++ch) {
+      uint32_t r[2], ah[4], al[4];
+      frag_of_rotation<D>(r, sm + F::OFF_ROT, ch, jt, lane);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = (gq + 8 * (i & 1)) * LDA + 8 * ch + tq + 4 * (i >> 1);
+        ah[i] = A[at];
+        al[i] = A[16 * LDA + at];
+      }
+      mma_f16_16816(c, ah, r[0], r[1]);
+      mma_f16_16816(c, al, r[0], r[1]);
+    }
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       if (!o_ok[r]) continue;
       const int64_t o = o_at[r] + (int64_t)(8 * jt + 2 * tq) * p.os[2];
-      store_elem(p.out, p.o_dtype, o, c[2 * r]);
-      store_elem(p.out, p.o_dtype, o + p.os[2], c[2 * r + 1]);
+      if (p.o_pair) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(c[2 * r], c[2 * r + 1]);
+        reinterpret_cast<uint32_t*>(p.out)[o >> 1] =
+            p.o_dtype == TQ_BF16 ? *reinterpret_cast<const uint32_t*>(&h) : pack_half2(c[2 * r], c[2 * r + 1]);
+      } else {
+        store_elem(p.out, p.o_dtype, o, c[2 * r]);
+        store_elem(p.out, p.o_dtype, o + p.os[2], c[2 * r + 1]);
+      }
     }
   }
 }
@@ -700,6 +697,7 @@ __global__ void __launch_bounds__(32 * kW, 3) attend_few_kernel(FewParams p) {
   extern __shared__ __align__(128) unsigned char sm[];
   // segments in the list's order (long ones first), whoever is free next
   __shared__ int next;
+  pdl_wait();                                              // the list and q'
   while (true) {
     __syncthreads();                                       // the last segment is done with
     if (threadIdx.x == 0) next = atomicAdd(p.rg.plan.next, 1);
@@ -732,7 +730,8 @@ bool attend_few_applies(const tq_geom* G) {
 
 int launch_attend_few(const tq_geom* G, const tq_tables* t, const tq_cache* c,
                       const tq_attend_args* a, const RaggedAttend& rg, int64_t Hkv, int hc,
-                      int pcta, int rows, int64_t grid, uint32_t* status, cudaStream_t st) {
+                      int pcta, int rows, const __half* qp, int64_t qp_stride, int64_t grid,
+                      uint32_t* status, cudaStream_t st) {
   FewParams p;
   const PageGeom g = make_geom(G->head_dim, G->key_bits, G->value_bits, G->qjl);
   p.pages = c->pages;
@@ -741,19 +740,21 @@ int launch_attend_few(const tq_geom* G, const tq_tables* t, const tq_cache* c,
   p.off_v = g.off_v;
   p.off_kn = g.off_kn;
   p.off_vn = g.off_vn;
-  p.rot = t->rot;
-  p.rot_t = t->rot_t;
+  p.rot_h = reinterpret_cast<const __half*>(t->rot_f16);
+  p.qp = qp;
+  p.qp_stride = qp_stride;
   p.kc = t->k_centroids;
   p.vc = t->v_centroids;
-  p.q = a->q->data; p.q_dtype = a->q->dtype;
+  p.Hq = (int)a->q->shape[1];
   p.out = a->out->data; p.o_dtype = a->out->dtype;
-  for (int i = 0; i < 3; ++i) { p.qs[i] = a->q->stride[i + 1]; p.os[i] = a->out->stride[i + 1]; }
+  for (int i = 0; i < 3; ++i) p.os[i] = a->out->stride[i + 1];
+  p.o_pair = p.o_dtype != TQ_F32 && p.os[2] == 1 && reinterpret_cast<uintptr_t>(p.out) % 4 == 0 &&
+             (a->out->shape[1] == 1 || p.os[0] % 2 == 0) && (a->out->shape[2] == 1 || p.os[1] % 2 == 0);
   p.Hkv = (int)Hkv;
   p.g = (int)(a->q->shape[1] / Hkv);
   p.hc = hc;
   p.nchunk = (p.g + hc - 1) / hc;
   p.pcta = pcta;
-  p.qscale = a->scale * kLog2eF;
   p.causal = a->causal;
   p.status = status;
   p.rg = rg;
@@ -773,8 +774,8 @@ int launch_attend_few(const tq_geom* G, const tq_tables* t, const tq_cache* c,
   if (set_smem_attr((const void*)fn, bytes) != TQ_OK) return TQ_ERR_CUDA;
   // CTAs that fit at once
   const int64_t fit = (int64_t)device_sm_count() * occupancy((const void*)fn, 32 * kW, bytes);
-  fn<<<(unsigned)tmin(grid, fit), 32 * kW, bytes, st>>>(p);
-  return check_launch("tq_attend_ragged/few");
+  return launch_result(launch_pdl(fn, dim3((unsigned)tmin(grid, fit)), dim3(32 * kW), bytes, st, p),
+                       "tq_attend_ragged/few");
 }
 
 }  // namespace tq

@@ -1,6 +1,7 @@
 // tq_internal.h — host-side glue shared by the .cu translation units.
 #pragma once
 
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -88,7 +89,8 @@ int launch_attend_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c
 bool attend_few_applies(const tq_geom* g);
 int launch_attend_few(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                       const tq_attend_args* a, const RaggedAttend& rg, int64_t Hkv, int hc,
-                      int pcta, int rows, int64_t grid, uint32_t* status, cudaStream_t st);
+                      int pcta, int rows, const __half* qp, int64_t qp_stride, int64_t grid,
+                      uint32_t* status, cudaStream_t st);
 int launch_attend_tc(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                      const tq_attend_args* a, const RaggedAttend& rg, int64_t Hkv, int64_t grid,
                      uint32_t* status, cudaStream_t st);
