@@ -499,15 +499,42 @@ class TurboQuantKVCache(BaseKVCache):
         ``layer_idx``'s packed history and window (GQA: Hq % Hkv == 0)."""
         return self._stores[layer_idx].attend(query_states, scale=scale, out=out)
 
+    def _rotated(self, q: torch.Tensor, k: torch.Tensor, layer_idx: int,
+                 rope: Optional[ops.RopeTable], positions: Optional[torch.Tensor],
+                 q_norm: Optional[ops.HeadNorm], k_norm: Optional[ops.HeadNorm]):
+        """Query and key heads normed and rotated in one pass, at the positions
+        that the new tokens take in the cache unless ``positions`` says others."""
+        if rope is None and q_norm is None and k_norm is None:
+            if positions is not None:
+                raise ValueError("positions come with rope")
+            return q, k
+        if rope is not None and positions is None:
+            n = self._stores[layer_idx].tokens
+            positions = torch.arange(n, n + q.shape[2], device=q.device)
+        both = rope is not None or (q_norm is not None and k_norm is not None)
+        q_out, k_out = ops.qk_rope(q if both or q_norm is not None else None,
+                                   k if both or k_norm is not None else None, rope, positions,
+                                   q_norm=q_norm, k_norm=k_norm)
+        return (q if q_out is None else q_out), (k if k_out is None else k_out)
+
     def decode(self, query_states: torch.Tensor, key_states: torch.Tensor,
                value_states: torch.Tensor, layer_idx: int, scale: Optional[float] = None,
                out: Optional[torch.Tensor] = None, gather=None,
-               kv_start: Optional[torch.Tensor] = None) -> torch.Tensor:
+               kv_start: Optional[torch.Tensor] = None, rope: Optional[ops.RopeTable] = None,
+               positions: Optional[torch.Tensor] = None,
+               q_norm: Optional[ops.HeadNorm] = None,
+               k_norm: Optional[ops.HeadNorm] = None) -> torch.Tensor:
         """One decode step of one layer: store the new token(s) (reference
         update() semantics, including the residual window) and return the
         attention of query_states (B, Hq, 1, D) over the whole cache, without
         materialising dense K/V.  ``kv_start`` (int32 (B,) on the device):
-        each batch row's first attended position (left padding)."""
+        each batch row's first attended position (left padding).  With
+        ``rope`` (and / or the head norms) query and key come as they leave
+        their projections and are normed and rotated here (ops.qk_rope):
+        ``positions`` (T,) or (B, T), by default the new tokens' places in the
+        cache (a padded batch passes its own)."""
+        query_states, key_states = self._rotated(query_states, key_states, layer_idx, rope,
+                                                 positions, q_norm, k_norm)
         return self._stores[layer_idx].decode(query_states, key_states, value_states,
                                               self.residual_window, scale=scale, out=out,
                                               gather=gather, kv_start=kv_start)
@@ -515,11 +542,17 @@ class TurboQuantKVCache(BaseKVCache):
     def prefill(self, query_states: torch.Tensor, key_states: torch.Tensor,
                 value_states: torch.Tensor, layer_idx: int, scale: Optional[float] = None,
                 causal: bool = True, out: Optional[torch.Tensor] = None,
-                kv_start: Optional[torch.Tensor] = None) -> torch.Tensor:
+                kv_start: Optional[torch.Tensor] = None, rope: Optional[ops.RopeTable] = None,
+                positions: Optional[torch.Tensor] = None,
+                q_norm: Optional[ops.HeadNorm] = None,
+                k_norm: Optional[ops.HeadNorm] = None) -> torch.Tensor:
         """A prefill forward of one layer: store the T new tokens (residual
         window included) and return the causal attention of query_states
         (B, Hq, T, D) over the whole cache (the SDPA that follows update() in
-        the reference), without dense K/V.  ``kv_start``: left padding."""
+        the reference), without dense K/V.  ``kv_start``: left padding.
+        ``rope``, ``positions`` and the head norms as in decode()."""
+        query_states, key_states = self._rotated(query_states, key_states, layer_idx, rope,
+                                                 positions, q_norm, k_norm)
         return self._stores[layer_idx].prefill(query_states, key_states, value_states,
                                                self.residual_window, scale=scale,
                                                causal=causal, out=out, kv_start=kv_start)

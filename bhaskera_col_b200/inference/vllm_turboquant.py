@@ -14,7 +14,12 @@ computes the attention from those pages with the fused kernels:
   lengths read on the device (tq_decode_args.seq_lens), so the call needs no
   host synchronisation;
 * prefill and chunked-prefill requests append their new tokens at position
-  seq_len - query_len and run the prefill attention over the packed context.
+  seq_len - query_len and run the prefill attention over the packed context;
+* a model that hands over its heads before their norms and rotation
+  (``forward(..., rope=...)``) runs every batch, whatever its mix, as three
+  calls without host synchronisation: ops.qk_rope on the queries,
+  ops.append_ragged (keys normed and rotated on the way into their pages) and
+  ops.attend_ragged.
 
 The compressor is the reference's vLLM one (vllm_turboquant.py:170-230): the
 MSE codebooks without the QJL sketch, rotation seed 42 + 13 * layer
@@ -62,6 +67,26 @@ class VLLMBatch:
     max_query_len: int
     query_start_loc_cpu: Optional[List[int]] = None
     seq_lens_cpu: Optional[List[int]] = None
+    _ragged: Optional[ops.RaggedBatch] = None
+    _positions: Optional[torch.Tensor] = None
+
+    def ragged(self) -> ops.RaggedBatch:
+        """The batch as the ragged operators take it (one per step, shared by
+        the layers)."""
+        if self._ragged is None:
+            self._ragged = ops.RaggedBatch(self.query_start_loc, self.seq_lens,
+                                           self.max_query_len)
+        return self._ragged
+
+    def positions(self) -> torch.Tensor:
+        """int64 (num_actual_tokens,): each token's position in its request,
+        computed on the device once per step."""
+        if self._positions is None:
+            start = self.query_start_loc.long()
+            base = torch.repeat_interleave(self.seq_lens.long() - start[1:], start.diff(),
+                                           output_size=self.num_actual_tokens)
+            self._positions = base + torch.arange(self.num_actual_tokens, device=start.device)
+        return self._positions
 
     @classmethod
     def from_metadata(cls, md) -> "VLLMBatch":
@@ -125,6 +150,7 @@ class TurboQuantPagedAttention:
         self.pool = torch.zeros((num_blocks * self.pages_per_block * num_kv_heads,
                                  self.page_bytes), dtype=torch.uint8, device=self.device)
         self.workspace = ops.DecodeWorkspace()
+        self.ragged_workspace = ops.DecodeWorkspace()
         self.tokens_stored = 0
         self.decode_tokens = 0
 
@@ -145,12 +171,25 @@ class TurboQuantPagedAttention:
     # -- attention ------------------------------------------------------------
     def forward(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                 batch: VLLMBatch, out: Optional[torch.Tensor] = None,
-                stream_table: Optional[torch.Tensor] = None) -> torch.Tensor:
+                stream_table: Optional[torch.Tensor] = None,
+                rope: Optional[ops.RopeTable] = None, q_norm: Optional[ops.HeadNorm] = None,
+                k_norm: Optional[ops.HeadNorm] = None,
+                positions: Optional[torch.Tensor] = None) -> torch.Tensor:
         """query (N, Hq, D), key / value (N, Hkv, D) in vLLM's flattened token
-        order; stores the tokens, returns the (N, Hq, D) attention output."""
+        order; stores the tokens, returns the (N, Hq, D) attention output.
+
+        With ``rope`` (and / or the head norms) query and key come as they
+        leave their projections: they are normed and rotated here, by each
+        token's position in its request or by ``positions`` (N,), and the
+        whole batch runs as three calls."""
         if out is None:
             out = torch.empty_like(query)
         st = stream_table if stream_table is not None else self.stream_table(batch.block_table)
+        if rope is not None or q_norm is not None or k_norm is not None:
+            return self._forward_ragged(query, key, value, batch, out, st, rope, q_norm, k_norm,
+                                        positions)
+        if positions is not None:
+            raise ValueError("positions come with rope")
         H = self.num_kv_heads
         R = batch.seq_lens.shape[0]
         cap = st.shape[1] * PAGE_TOKENS
@@ -187,6 +226,35 @@ class TurboQuantPagedAttention:
                                   sl[r], scale=self.scale, causal=True,
                                   out=out[qs:qe].permute(1, 0, 2).unsqueeze(0))
         return out
+
+    def _forward_ragged(self, query, key, value, batch, out, st, rope, q_norm, k_norm, positions):
+        n = batch.num_actual_tokens
+        rb, pages = batch.ragged(), self.paged(st)
+        self.tokens_stored += n
+        if batch.max_query_len <= 1:
+            self.decode_tokens += n
+        q = query[:n]
+        if rope is not None or q_norm is not None:
+            at = positions[:n] if positions is not None else \
+                (batch.positions() if rope is not None else None)
+            q, _ = ops.qk_rope(q, None, rope, at, q_norm=q_norm)
+        ops.append_ragged(self.tables, pages, key[:n], value[:n], rb, rope=rope, k_norm=k_norm,
+                          positions=positions[:n] if positions is not None else None)
+        ops.attend_ragged(self.tables, pages, q, rb, scale=self.scale, out=out[:n],
+                          workspace=self.ragged_workspace)
+        return out
+
+    def read(self, batch: VLLMBatch, dtype: torch.dtype = torch.bfloat16,
+             stream_table: Optional[torch.Tensor] = None):
+        """The stored keys and values of a batch's tokens as dense (N, Hkv, D)
+        tensors (a batch whose query lengths are whole contexts reads those:
+        for handing a prefix to another attention or cache).  Tokens without a
+        place in the pages read as 0."""
+        st = stream_table if stream_table is not None else self.stream_table(batch.block_table)
+        shape = (batch.num_actual_tokens, self.num_kv_heads, self.head_dim)
+        k, v = (torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
+        ops.dequantize_ragged(self.tables, self.paged(st), batch.ragged(), k, v)
+        return k, v
 
     def _decode(self, q, k, v, out, seq_lens, st, cap):
         ops.decode_step(self.tables, self.paged(st), k.unsqueeze(2), v.unsqueeze(2), cap - 1,

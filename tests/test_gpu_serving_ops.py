@@ -610,3 +610,85 @@ def test_no_rows():
     ops.dequantize_ragged(tables, pages, batch, y, None)
     ops.attend_ragged(tables, pages, y.clone(), batch, out=y)
     assert (y == 7).all() and (pages.pool == 0).all() and ok_status() == 0
+
+
+# ------------------------------------------------------------------- through the public classes
+def test_paged_attention_layer_with_rope_matches_rotated_heads():
+    """TurboQuantPagedAttention.forward(rope=...) over a served schedule (prompts, mixed and
+    decode-only steps, padding rows behind the batch) against the 64-bit form on what it stored; the
+    pages against append of the rotated keys; read() gives the pages' tokens."""
+    from bhaskera_col_b200.inference.vllm_turboquant import TurboQuantPagedAttention, VLLMBatch
+    D, Hq, H = 128, 8, 2
+    layer = TurboQuantPagedAttention(5, 32, Hq, H, D, num_blocks=40, block_size=64, key_bits=4,
+                                     value_bits=2, device=DEV)
+    rope = ops.RopeTable.build(D, 1000, interleaved=True, device=DEV)
+    qn, kn = (ops.HeadNorm(1 + 0.1 * randn((D,), i, F32)) for i in range(2))
+    free = torch.randperm(40, generator=torch.Generator().manual_seed(3)).tolist()
+    blocks, length, stored = {}, {}, {}
+    steps = [[("A", 130), ("B", 64), ("C", 1)], [("A", 1), ("B", 3), ("C", 70)],
+             [("C", 1), ("A", 1), ("B", 1)], [("B", 129), ("A", 1)]]
+    for i, work in enumerate(steps):
+        start, seq = [0], []
+        for r, n in work:
+            blocks.setdefault(r, [])
+            length[r] = length.get(r, 0) + n
+            while len(blocks[r]) * 64 < length[r]:
+                blocks[r].append(free.pop())
+            start.append(start[-1] + n)
+            seq.append(length[r])
+        N = start[-1]
+        bt = torch.zeros((len(work), max(len(blocks[r]) for r, _ in work) + 1), dtype=torch.int32)
+        for j, (r, _) in enumerate(work):
+            bt[j, : len(blocks[r])] = torch.tensor(blocks[r], dtype=torch.int32)
+        batch = VLLMBatch(int32(start), int32(seq), bt.to(DEV), N, max(n for _, n in work))
+        q, k, v = (randn((N + 2, h, D), 10 * i + j, BF16, 7) for j, h in enumerate((Hq, H, H)))
+        out = torch.full_like(q, 7.0)
+        got = layer.forward(q, k, v, batch, out=out, rope=rope, q_norm=qn, k_norm=kn)
+        assert got is out and (out[N:] == 7.0).all() and ok_status() == 0
+        assert batch.query_start_loc_cpu is None and batch.seq_lens_cpu is None     # no host copies
+        req, pos = S.positions(start, seq, N)
+        assert batch.positions().tolist() == pos.tolist()
+        pages = layer.paged(layer.stream_table(batch.block_table))
+        kx = S.rope(k[:N], rope.cos_sin, pos, True, kn.weight, 1e-6)
+        check_stored(layer.tables, pages, k[:N], v[:N], start, seq, len(work), H, kx)
+        tokens = pages.shape[1] * 64
+        kd, vd = (x.reshape(len(work), H, -1, D) for x in S.dense(layer.tables, contiguous(pages), tokens))
+        qx = torch.from_numpy(S.rope(q[:N], rope.cos_sin, pos, True, qn.weight, 1e-6))
+        check_attend(out[:N], S.attend(qx, kd, vd, start, seq, layer.scale, True), BF16)
+        rk, rv = layer.read(batch)
+        for t, x in ((rk, kd), (rv, vd)):
+            want = x[req, :, pos]
+            assert np.abs(t.double().cpu().numpy() - want).max() <= 2.0 ** -7 * np.abs(want).max()
+    assert layer.tokens_stored == sum(n for w in steps for _, n in w)
+    with pytest.raises(ValueError, match="rope"):
+        layer.forward(q, k, v, batch, positions=batch.positions())
+
+
+def test_cache_with_rope_matches_rotated_heads():
+    """TurboQuantKVCache.prefill / decode(rope=...) store and attend exactly what they do for heads
+    rotated by qk_rope beforehand, at the cache's own positions or given ones."""
+    from bhaskera_col_b200.inference import TurboQuantKVCache
+    B, Hq, H, D, T = 2, 4, 2, 128, 37
+    rope = ops.RopeTable.build(D, 500, device=DEV)
+    qn, kn = (ops.HeadNorm(1 + 0.1 * randn((D,), i, F32)) for i in range(2))
+
+    def cache():
+        return TurboQuantKVCache(1, B, H, D, residual_window=0, protected_layers=0, device=DEV,
+                                 max_seq_len=128)
+
+    a, b = cache(), cache()
+    pads = torch.tensor([[5], [0]], device=DEV)
+    for i, n in enumerate((T, 1, 1)):
+        q, k, v = (randn((B, h, n, D), 5 * i + j) for j, h in enumerate((Hq, H, H)))
+        at = torch.arange(n, device=DEV) + (0 if i == 0 else T + i - 1)
+        given = (at[None] - pads).clamp_min(0) if i == 2 else None
+        call = (a.prefill, b.prefill) if n > 1 else (a.decode, b.decode)
+        qr, kr = ops.qk_rope(q, k, rope, at if given is None else given, qn, kn)
+        want = call[1](qr, kr, v, 0)
+        got = call[0](q, k, v, 0, rope=rope, positions=given, q_norm=qn, k_norm=kn)
+        assert torch.equal(got, want)
+    assert torch.equal(a._stores[0]._pages, b._stores[0]._pages) and ok_status() == 0
+    # only one norm: the other heads pass through
+    q, k, v = (randn((B, h, 1, D), 50 + j) for j, h in enumerate((Hq, H, H)))
+    kr = ops.qk_rope(None, k, None, k_norm=kn)[1]
+    assert torch.equal(a.decode(q, k, v, 0, k_norm=kn), b.decode(q, kr, v, 0))
