@@ -692,3 +692,30 @@ def test_cache_with_rope_matches_rotated_heads():
     q, k, v = (randn((B, h, 1, D), 50 + j) for j, h in enumerate((Hq, H, H)))
     kr = ops.qk_rope(None, k, None, k_norm=kn)[1]
     assert torch.equal(a.decode(q, k, v, 0, k_norm=kn), b.decode(q, kr, v, 0))
+
+
+def test_inputs_of_a_backward_pass_and_mixed_devices_are_refused():
+    x = randn((3, 2, 128), 1, F32).requires_grad_()
+    table = ops.RopeTable.build(128, 10, device=DEV)
+    pos = torch.arange(3, device=DEV)
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        ops.qk_rope(x, None, table, pos)
+    with torch.no_grad():
+        ops.qk_rope(x, None, table, pos)
+    ops.qk_rope(x.detach(), None, table, pos)
+    with pytest.raises(ValueError, match="tensors on"):
+        ops.qk_rope(x.detach(), None, table, pos.cpu())
+    with pytest.raises(ValueError, match="positions"):
+        ops.qk_rope(x.detach(), None, table, pos[:2])
+    with pytest.raises(ValueError, match="weights"):
+        ops.qk_rope(x.detach(), None, None, q_norm=ops.HeadNorm(torch.ones(64, device=DEV)))
+    batch, _, _ = make_batch([(3, 3)])
+    tables = make_tables(128, 4, 2, False)
+    pages = make_paged(tables, 2, 64)
+    for call in (lambda: ops.append_ragged(tables, pages, x, x, batch),
+                 lambda: ops.attend_ragged(tables, pages, x, batch)):
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            call()
+    with pytest.raises(_lib.TqError, match="overlaps"):
+        buf = randn((4, 2, 128), 2)
+        ops.qk_rope(buf[:3], None, table, pos, q_out=buf[1:])

@@ -1,0 +1,253 @@
+"""Host side of the serving operators (CPU only): refusals of the C entries before anything touches
+the device, checks of the Python wrappers, and the arithmetic the kernels rely on."""
+import ctypes
+import random
+
+import pytest
+import torch
+
+from bhaskera_col_b200 import _lib
+from bhaskera_col_b200.inference import ops
+
+I64x4 = ctypes.c_int64 * 4
+
+
+def t4(shape, stride=None, dtype=_lib.TQ_BF16, data=1 << 20):
+    if stride is None:
+        stride = [shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3], 1]
+    return _lib.Tensor4(data, dtype, I64x4(*shape), I64x4(*stride))
+
+
+def far(shape, **kw):
+    return t4(shape, data=1 << 30, **kw)
+
+
+def rope_call(rope=None, pos=None, q=None, qo=None, qn=None, k=None, ko=None, kn=None):
+    r = lambda x: None if x is None else ctypes.byref(x)  # noqa: E731
+    rc = _lib.load().tq_qk_rope(r(rope), r(pos), r(q), r(qo), r(qn), r(k), r(ko), r(kn), None)
+    return rc, _lib.last_error()
+
+
+ROPE = _lib.Rope(4096, 100, 128, 0)
+POS = _lib.Positions(4096, 64, (ctypes.c_int64 * 2)(0, 1))
+NORM = _lib.HeadNorm(4096, _lib.TQ_F32, 1e-6, 0.0)
+X = (1, 4, 7, 128)
+
+
+@pytest.mark.parametrize("kw,what", [
+    (dict(), "neither"),
+    (dict(rope=ROPE, pos=POS, q=t4(X)), "come together"),
+    (dict(q=t4(X), qo=far(X)), "neither a rotation nor a norm"),
+    (dict(rope=ROPE, q=t4(X), qo=far(X)), "needs positions"),
+    (dict(rope=_lib.Rope(4096, 100, 63, 0), pos=POS, q=t4(X), qo=far(X)), "rot_dim"),
+    (dict(rope=_lib.Rope(4096, 100, 130, 0), pos=POS, q=t4(X), qo=far(X)), "rot_dim"),
+    (dict(rope=_lib.Rope(4096, 100, 0, 0), pos=POS, q=t4(X), qo=far(X)), "rot_dim"),
+    (dict(rope=_lib.Rope(4100, 100, 128, 0), pos=POS, q=t4(X), qo=far(X)), "table"),
+    (dict(rope=_lib.Rope(4096, 0, 128, 0), pos=POS, q=t4(X), qo=far(X)), "table"),
+    (dict(rope=ROPE, pos=_lib.Positions(4096, 16, POS.stride), q=t4(X), qo=far(X)), "positions"),
+    (dict(rope=ROPE, pos=_lib.Positions(4100, 64, POS.stride), q=t4(X), qo=far(X)), "positions"),
+    (dict(qn=_lib.HeadNorm(4096, 7, 1e-6, 0), q=t4(X), qo=far(X)), "head norm"),
+    (dict(qn=_lib.HeadNorm(4096, 0, -1e-6, 0), q=t4(X), qo=far(X)), "head norm"),
+    (dict(qn=_lib.HeadNorm(4096, 0, float("nan"), 0), q=t4(X), qo=far(X)), "head norm"),
+    (dict(qn=NORM, q=t4(X), qo=far((1, 4, 6, 128))), "disagree"),
+    (dict(qn=NORM, q=t4(X), qo=far(X, dtype=_lib.TQ_F16)), "differ in type"),
+    (dict(qn=NORM, kn=NORM, q=t4(X), qo=far(X), k=t4((1, 2, 6, 128)), ko=far((1, 2, 6, 128))),
+     "disagree"),
+    (dict(qn=NORM, q=t4((1, 1, 1, 257)), qo=far((1, 1, 1, 257))), "head_dim"),
+    (dict(qn=NORM, q=t4(X), qo=t4(X, stride=[0, 0, 128, 1], data=1 << 30)), "share memory"),
+    (dict(qn=NORM, q=t4(X), qo=t4(X, stride=[0, 64, 512, 1], data=1 << 30)), "share memory"),
+    (dict(qn=NORM, q=t4(X), qo=t4(X, data=(1 << 20) + 256)), "overlaps"),
+    (dict(qn=NORM, q=t4(X), qo=t4(X, stride=[0, 128, 512, 1])), "overlaps"),
+    (dict(qn=NORM, q=t4(X, data=None), qo=far(X)), "NULL"),
+])
+def test_qk_rope_refusals(kw, what):
+    rc, err = rope_call(**kw)
+    assert rc == _lib.TQ_ERR_INVALID and what in err, err
+
+
+def geom(D=128, kb=4, vb=2, qjl=0):
+    return _lib.Geom(D, kb, vb, qjl)
+
+
+TABLES = _lib.Tables(*([4096] * 11))
+CACHE = _lib.Cache(1 << 20, 6, 4, 0, 0, 0)                 # 3 requests x 2 heads
+BATCH = _lib.Ragged(3, 4096, 4096, 9)
+KV = (1, 2, 10, 128)
+
+
+def entry(fn, g=None, t=TABLES, c=CACHE, batch=BATCH, k=t4(KV), v=t4(KV), rope=None, norm=None,
+          pos=None):
+    r = lambda x: None if x is None else ctypes.byref(x)  # noqa: E731
+    lib = _lib.load()
+    g = g or geom()
+    if fn == "append":
+        rc = lib.tq_append_ragged(r(g), r(t), r(c), r(k), r(v), r(batch), r(rope), r(norm), r(pos), None)
+    else:
+        rc = lib.tq_dequantize_ragged(r(g), r(t), r(c), r(batch), r(k), r(v), None)
+    return rc, _lib.last_error()
+
+
+@pytest.mark.parametrize("fn", ["append", "read"])
+@pytest.mark.parametrize("kw,what", [
+    (dict(g=geom(D=48)), "head_dim"),
+    (dict(g=geom(kb=9)), "bit widths"),
+    (dict(t=_lib.Tables()), "NULL"),
+    (dict(c=_lib.Cache(0, 6, 4)), "cache"),
+    (dict(c=_lib.Cache(1 << 20, 6, 4, 4096, 3, 5)), "block table"),
+    (dict(batch=_lib.Ragged(0, 4096, 4096, 9)), "batch"),
+    (dict(batch=_lib.Ragged(3, 0, 4096, 9)), "batch"),
+    (dict(batch=_lib.Ragged(3, 4096, 4098, 9)), "batch"),
+    (dict(batch=_lib.Ragged(3, 4096, 4096, -1)), "batch"),
+    (dict(batch=_lib.Ragged(4, 4096, 4096, 9)), "multiple"),
+    (dict(k=t4((1, 3, 10, 128))), "must be"),
+    (dict(v=t4((2, 2, 10, 128))), "must be"),
+    (dict(k=t4((1, 2, 10, 64))), "must be"),
+    (dict(k=t4((1, 2, 9, 128))), "differ in rows"),
+    (dict(g=geom(D=256), k=t4((1, 2, 10, 256)), v=t4((1, 2, 10, 256))), "128"),
+])
+def test_ragged_store_and_read_refusals(fn, kw, what):
+    rc, err = entry(fn, **kw)
+    assert rc == _lib.TQ_ERR_INVALID and what in err, err
+
+
+def test_more_append_and_read_refusals():
+    for kw, what in ((dict(g=geom(qjl=1)), "QJL"), (dict(rope=_lib.Rope(4096, 10, 200, 0)), "rot_dim"),
+                     (dict(norm=_lib.HeadNorm(None, 0, 1e-6, 0)), "head norm"),
+                     (dict(pos=_lib.Positions(None, 64, POS.stride)), "positions")):
+        rc, err = entry("append", **kw)
+        assert rc == _lib.TQ_ERR_INVALID and what in err, err
+    rc, err = entry("read", k=None, v=None)
+    assert rc == _lib.TQ_ERR_INVALID and "neither" in err
+    rc, err = entry("read", k=t4(KV, stride=[0, 0, 128, 1]))
+    assert rc == _lib.TQ_ERR_INVALID and "share memory" in err
+
+
+def attend(g=None, c=CACHE, q=t4((1, 4, 10, 128)), out=None, batch=BATCH, scale=0.1, engine=0,
+           t=TABLES, ws=1 << 20, nbytes=None):
+    lib = _lib.load()
+    g = g or geom()
+    out = out or far(tuple(q.shape))
+    a = _lib.AttendArgs(ctypes.pointer(q), ctypes.pointer(out), batch, scale, 1, engine)
+    need = lib.tq_attend_ragged_workspace_bytes(ctypes.byref(g), ctypes.byref(c), ctypes.byref(a))
+    if nbytes is None:
+        nbytes = need
+    rc = lib.tq_attend_ragged(ctypes.byref(g), ctypes.byref(t), ctypes.byref(c), ctypes.byref(a), ws,
+                              nbytes, None)
+    return rc, _lib.last_error(), need
+
+
+@pytest.mark.parametrize("kw,what", [
+    (dict(engine=4), "engine"), (dict(engine=-1), "engine"),
+    (dict(g=geom(D=96), q=t4((1, 4, 10, 96))), "no kernel"),
+    (dict(g=geom(kb=7)), "no kernel"),
+    (dict(g=geom(D=64), q=t4((1, 4, 10, 64)), engine=2), "no kernel"),
+    (dict(g=geom(kb=8, vb=8), engine=3), "no kernel"),
+    (dict(q=t4((1, 3, 10, 128))), "multiple"),
+    (dict(q=t4((1, 4, 10, 64))), "must be"),
+    (dict(batch=_lib.Ragged(5, 4096, 4096, 1)), "multiple"),
+    (dict(q=t4((1, 2048, 1, 128))), "1024 query heads"),
+    (dict(c=_lib.Cache(1 << 20, 6, 1 << 27)), "32 bits"),
+])
+def test_attend_refusals(kw, what):
+    rc, err, need = attend(**kw)
+    assert rc == _lib.TQ_ERR_INVALID and need == 0 and what in err, err
+
+
+def test_attend_refusals_of_the_call_alone():
+    for kw, what in ((dict(out=far((1, 4, 9, 128))), "differ in rows"),
+                     (dict(out=t4((1, 4, 10, 128), stride=[0, 0, 128, 1])), "share memory"),
+                     (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"),
+                     (dict(t=_lib.Tables(*([4096] * 9))), "rot_f16")):
+        rc, err, need = attend(**kw)
+        assert rc == _lib.TQ_ERR_INVALID and need > 0 and what in err, err
+    for kw in (dict(nbytes=100), dict(ws=(1 << 20) + 64), dict(ws=None)):
+        rc, err, need = attend(**kw)
+        assert rc == _lib.TQ_ERR_WORKSPACE and str(need) in err
+
+
+def test_wrapper_checks():
+    x = torch.zeros((3, 2, 128))
+    table = ops.RopeTable(torch.zeros((5, 128)))
+    batch = ops.RaggedBatch(torch.tensor([0, 3], dtype=torch.int32),
+                            torch.tensor([3], dtype=torch.int32), 3)
+    for call in (lambda: ops.qk_rope(x, None, table, torch.arange(3)),
+                 lambda: ops.append_ragged(None, None, x, x, batch),
+                 lambda: ops.dequantize_ragged(None, None, batch, x, x),
+                 lambda: ops.attend_ragged(None, None, x, batch)):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            call()
+    with pytest.raises(ValueError, match="neither"):
+        ops.qk_rope(None, None, table)
+    with pytest.raises(ValueError, match="positions"):
+        ops.qk_rope(x, None, table)
+    with pytest.raises(ValueError, match="neither"):
+        ops.dequantize_ragged(None, None, batch, None, None)
+    for bad in (torch.zeros((5, 128)).double(), torch.zeros((5, 127)), torch.zeros(5),
+                torch.zeros((0, 128)), torch.zeros((128, 5)).t()):
+        with pytest.raises(ValueError):
+            ops.RopeTable(bad)
+    with pytest.raises(ValueError):
+        ops.RopeTable.build(64, 10, inv_freq=torch.ones(31), device="cpu")
+    for kw in (dict(weight=torch.ones((2, 2))), dict(weight=torch.ones(4, dtype=torch.int32)),
+               dict(weight=torch.ones(8)[::2]), dict(weight=torch.ones(4), eps=-1.0)):
+        with pytest.raises(ValueError):
+            ops.HeadNorm(**kw)
+    i = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    for a in ((i(0, 3), i(3, 4), 3), (i(0, 3).long(), i(3), 3), (i(0, 3), i(3).float(), 3),
+              (i(0), i(), 0), (i(0, 3), i(3), -1), (i(0, 9, 3, 9)[::2], i(3), 3)):
+        with pytest.raises(ValueError):
+            ops.RaggedBatch(*a)
+
+
+def test_rope_table_values():
+    t = ops.RopeTable.build(8, 20, base=100.0, scale=2.0, device="cpu")
+    p = torch.arange(20, dtype=torch.float64)[:, None]
+    a = p * 100.0 ** (-torch.arange(0, 8, 2, dtype=torch.float64) / 8)
+    assert torch.equal(t.cos_sin, (2 * torch.cat([a.cos(), a.sin()], -1)).float())
+    f = torch.tensor([1.0, 0.5, 0.25, 0.125])
+    t = ops.RopeTable.build(8, 20, inv_freq=f, interleaved=True, device="cpu")
+    assert t.interleaved and torch.equal(t.cos_sin[:, :4], (p * f.double()).cos().float())
+
+
+def test_division_by_multiplication_is_exact():
+    """The kernels' i / d: m = ceil(2^(31 + s) / d), 2^s >= d, for every i below 2^31.  The quotient
+    can go wrong only beside a multiple of d, and the error grows with i."""
+    for d in list(range(1, 300)) + [511, 512, 513, 1000, 1024, 65535, 65536]:
+        s = (d - 1).bit_length()
+        m = -(-(1 << (31 + s)) // d)
+        assert m < 1 << 32
+        top = (1 << 31) - 1
+        ks = {1, 2, 3, top // d, top // d - 1, top // d // 2} | {random.Random(d).randrange(1, top // d + 1)
+                                                                 for _ in range(50)}
+        for k in ks:
+            for i in (k * d - 1, k * d, k * d + 1):
+                if 0 <= i <= top:
+                    assert (i * m) >> (31 + s) == i // d
+
+
+def test_attention_work_list_fits_its_bounds():
+    """The launch's bounds on segments and partial slots hold for any lengths: tiles are at most
+    N / pcta + R, and segments of at most L = max(min, ceil(all / wanted)) key tiles add at most
+    wanted / G each way."""
+    rng = random.Random(0)
+    for _ in range(300):
+        R = rng.randrange(1, 40)
+        q = [rng.choice([0, 1, rng.randrange(1, 9), rng.randrange(1, 3000)]) for _ in range(R)]
+        t = [rng.choice([0, 1, rng.randrange(1, 100000)]) for _ in range(R)]
+        causal = rng.random() < 0.5
+        seq = [a + b for a, b in zip(q, t)] if causal else t
+        pcta, keys = rng.choice([1, 2, 4, 16, 64]), rng.choice([64, 128])
+        G, wanted, least = rng.choice([1, 5, 8, 64, 300]), 148 * rng.choice([3, 5]), rng.choice([4, 8])
+        tiles = []
+        for a, s in zip(q, seq):
+            for i in range(-(-a // pcta)):
+                kend = s - a + min((i + 1) * pcta, a) if causal else s
+                tiles.append(max(0, -(-kend // keys)))
+        L = max(least, -(-sum(tiles) * G // wanted))
+        ns = [max(1, -(-n // L)) for n in tiles]
+        extra = wanted // G + 1
+        assert sum(ns) <= sum(q) // pcta + R + extra
+        assert sum(n for n in ns if n > 1) <= 2 * extra
+        for n, k in zip(tiles, ns):                        # parts cover the tile, none above L
+            base, more = divmod(n, k)
+            assert base + (more > 0) <= L
