@@ -285,8 +285,9 @@ AttendShape attend_shape(const tq_geom* G, const tq_cache* c, const tq_attend_ar
   const int64_t R = a->batch.requests, N = a->q->shape[2], most = INT64_MAX;
   s.Hkv = c->streams / R;
   const int64_t g = a->q->shape[1] / s.Hkv;
-  s.tc = prefill_tc_applies(G) && a->engine != 1;
-  const bool can = attend_few_applies(G) && (a->engine == 0 || a->engine == 3);
+  const bool pick = a->engine == 0 && !attend_precise(a);
+  s.tc = prefill_tc_applies(G) && (pick || a->engine == 2);
+  const bool can = attend_few_applies(G) && (pick || a->engine == 3);
   const int64_t few_q = a->engine == 3 ? most : tmax<int64_t>(kFewRows / g, 1);
   size_t off = 256;                        // the first 64 bytes: the decode's status word
   auto take = [&](size_t bytes) {

@@ -94,6 +94,8 @@ int launch_attend_few(const tq_geom* g, const tq_tables* t, const tq_cache* c,
 int launch_attend_tc(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                      const tq_attend_args* a, const RaggedAttend& rg, int64_t Hkv, int64_t grid,
                      uint32_t* status, cudaStream_t st);
+// fp16 and fp32 results ask for more than the fp16 operands that a bf16 one hides.
+inline bool attend_precise(const tq_attend_args* a) { return a->out->dtype != TQ_BF16; }
 int launch_attend_mma(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                       const tq_attend_args* a, const RaggedAttend& rg, int64_t Hkv, int hc,
                       int64_t grid, uint32_t* status, cudaStream_t st);

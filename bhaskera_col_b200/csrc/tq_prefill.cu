@@ -39,6 +39,7 @@ struct PrefillParams {
   PageMap pm;
   int page_bytes, page_pitch, off_v, off_kn, off_vn;   // page geometry (make_geom)
   const __half* rot_h;          // R [D][D] fp16, row-major
+  const float* rot;             // R [D][D] (HP kernels)
   const float* kc;
   const float* vc;
   const void* q; int q_dtype; int64_t qs[4];     // (B, Hq, Tq, D)
@@ -53,7 +54,9 @@ struct PrefillParams {
   RaggedAttend rg;              // ragged batch (RG kernels): Tq, n_tokens come per request
 };
 
-template <int D, int KB, int VB>
+// HP: the products take both operands as fp16 hi + lo (hi hi + lo hi + hi lo, 22
+// bits): R, the centroids, the queries and the probabilities.
+template <int D, int KB, int VB, bool HP>
 struct Pf {
   static constexpr int KROW = D * KB / 8, VROW = D * VB / 8;
   static constexpr int LD = D + 8;                          // padded fp16 row (ldmatrix)
@@ -63,9 +66,19 @@ struct Pf {
   static constexpr int OFF_NRM = OFF_VS + 64 * LD * 2;     // kn[64], vn[64] floats
   static constexpr int OFF_LUT = OFF_NRM + 512;            // K, V fp16 tables (256 each)
   static constexpr int OFF_BAR = OFF_LUT + 1024;
-  static constexpr int OFF_STG = OFF_BAR + 128;            // 2 page stages (runtime size)
+  static constexpr int OFF_LO = OFF_BAR + 128;             // HP: R, K, V and the tables, lo
+  static constexpr int LO_K = D * LD, LO_V = LO_K + 64 * LD, LO_LUT = LO_V + 64 * LD;   // halves
+  static constexpr int OFF_STG = OFF_LO + (HP ? LO_LUT * 2 + 1024 : 0);   // 2 page stages (runtime size)
   static int smem(int page_pitch) { return OFF_STG + 2 * page_pitch; }
 };
+
+// fp16 hi of a pair, and lo (2^-22 of each value in both)
+__device__ __forceinline__ uint32_t split_half2(float a, float b, uint32_t& lo) {
+  const uint32_t hi = pack_half2(a, b);
+  const __half2 h = *reinterpret_cast<const __half2*>(&hi);
+  lo = pack_half2(a - __low2float(h), b - __high2float(h));
+  return hi;
+}
 
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], const void* p) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -96,9 +109,9 @@ __device__ __forceinline__ void frag_b_kn(uint32_t (&r)[4], const __half* base, 
 // list: its request's rows and lengths, key tiles [kt0, kt1) of one block of
 // query positions; a tile cut into several segments leaves partial rows that
 // the tile's last CTA joins.
-template <int D, int KB, int VB, bool RG>
+template <int D, int KB, int VB, bool RG, bool HP>
 __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p) {
-  using G = Pf<D, KB, VB>;
+  using G = Pf<D, KB, VB, HP>;
   constexpr int NC = D / 16;                  // 16-wide chunks of D
   constexpr int NT = D / 8;                   // 8-wide n-tiles of D
   extern __shared__ __align__(128) unsigned char smem[];
@@ -109,6 +122,12 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
   float* vn = kn + 64;
   __half* lutk = reinterpret_cast<__half*>(smem + G::OFF_LUT);
   __half* lutv = lutk + 256;
+  // HP: the low parts
+  __half* Rl = reinterpret_cast<__half*>(smem + G::OFF_LO);
+  __half* Kl = Rl + G::LO_K;
+  __half* Vl = Rl + G::LO_V;
+  __half* lutkl = Rl + G::LO_LUT;
+  __half* lutvl = lutkl + 256;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + G::OFF_BAR);
   const uint32_t PAGE = (uint32_t)p.page_bytes;
 
@@ -154,14 +173,29 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
     fence_mbar_init();
   }
   // R (fp16) and the centroid tables
-  for (int i = tid; i < D * D / 8; i += kPfThreads) {
-    const int r = i / (D / 8), c8 = i % (D / 8);
-    *reinterpret_cast<uint4*>(Rs + r * G::LD + c8 * 8) =
-        __ldg(reinterpret_cast<const uint4*>(p.rot_h + r * D) + c8);
+  if constexpr (HP) {
+    for (int i = tid; i < D * D / 2; i += kPfThreads) {
+      const int r = i / (D / 2), c = 2 * (i % (D / 2));
+      const float* src = p.rot + r * D + c;
+      uint32_t lo;
+      *reinterpret_cast<uint32_t*>(Rs + r * G::LD + c) = split_half2(__ldg(src), __ldg(src + 1), lo);
+      *reinterpret_cast<uint32_t*>(Rl + r * G::LD + c) = lo;
+    }
+  } else {
+    for (int i = tid; i < D * D / 8; i += kPfThreads) {
+      const int r = i / (D / 8), c8 = i % (D / 8);
+      *reinterpret_cast<uint4*>(Rs + r * G::LD + c8 * 8) =
+          __ldg(reinterpret_cast<const uint4*>(p.rot_h + r * D) + c8);
+    }
   }
   for (int i = tid; i < 256; i += kPfThreads) {
-    lutk[i] = __float2half_rn(i < (1 << KB) ? __ldg(p.kc + i) : 0.f);
-    lutv[i] = __float2half_rn(i < (1 << VB) ? __ldg(p.vc + i) : 0.f);
+    const float k = i < (1 << KB) ? __ldg(p.kc + i) : 0.f, v = i < (1 << VB) ? __ldg(p.vc + i) : 0.f;
+    lutk[i] = __float2half_rn(k);
+    lutv[i] = __float2half_rn(v);
+    if constexpr (HP) {
+      lutkl[i] = __float2half_rn(k - __half2float(lutk[i]));
+      lutvl[i] = __float2half_rn(v - __half2float(lutv[i]));
+    }
   }
   __syncthreads();
   // pool address of this stream's page pg (block table or contiguous)
@@ -180,7 +214,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
 
   // ---- queries: q' = (scale q) R^T as fp16 A fragments (log2e folded in) ----
   const bool active = t0 < p.Tq;
-  uint32_t qf[NC][4];
+  uint32_t qf[NC][4], ql[HP ? NC : 1][4];
   {
     const float sc = p.scale;
     float acc[NT][4];
@@ -188,32 +222,47 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
     for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
     const int64_t qbase = qrow + h * p.qs[1];
     const int r0 = t0 + gq, r1 = r0 + 8;
-    auto ld2 = [&](int r, int c) -> uint32_t {
+    auto ld2 = [&](int r, int c, uint32_t& lo) -> uint32_t {
+      lo = 0u;
       if (r >= p.Tq) return 0u;
       const int64_t o = qbase + (int64_t)r * p.qs[2] + (int64_t)c * p.qs[3];
-      return pack_half2(sc * load_elem(p.q, p.q_dtype, o), sc * load_elem(p.q, p.q_dtype, o + p.qs[3]));
+      const float x = sc * load_elem(p.q, p.q_dtype, o), y = sc * load_elem(p.q, p.q_dtype, o + p.qs[3]);
+      if constexpr (HP) return split_half2(x, y, lo);
+      return pack_half2(x, y);
     };
 #pragma unroll
     for (int kc = 0; kc < NC; ++kc) {
-      uint32_t a[4];
-      a[0] = active ? ld2(r0, 16 * kc + 2 * tq) : 0u;
-      a[1] = active ? ld2(r1, 16 * kc + 2 * tq) : 0u;
-      a[2] = active ? ld2(r0, 16 * kc + 2 * tq + 8) : 0u;
-      a[3] = active ? ld2(r1, 16 * kc + 2 * tq + 8) : 0u;
+      uint32_t a[4] = {0u, 0u, 0u, 0u}, al[4] = {0u, 0u, 0u, 0u};
+      if (active) {
+        a[0] = ld2(r0, 16 * kc + 2 * tq, al[0]);
+        a[1] = ld2(r1, 16 * kc + 2 * tq, al[1]);
+        a[2] = ld2(r0, 16 * kc + 2 * tq + 8, al[2]);
+        a[3] = ld2(r1, 16 * kc + 2 * tq + 8, al[3]);
+      }
 #pragma unroll
       for (int n = 0; n < NT; n += 2) {
         uint32_t bf[4];
         frag_b_nk(bf, Rs, G::LD, 8 * n, 16 * kc, lane);   // B[k][n] = R[n][k]
         mma_f16_16816(acc[n], a, bf[0], bf[1]);
         mma_f16_16816(acc[n + 1], a, bf[2], bf[3]);
+        if constexpr (HP) {
+          mma_f16_16816(acc[n], al, bf[0], bf[1]);
+          mma_f16_16816(acc[n + 1], al, bf[2], bf[3]);
+          frag_b_nk(bf, Rl, G::LD, 8 * n, 16 * kc, lane);
+          mma_f16_16816(acc[n], a, bf[0], bf[1]);
+          mma_f16_16816(acc[n + 1], a, bf[2], bf[3]);
+        }
       }
     }
 #pragma unroll
     for (int kc = 0; kc < NC; ++kc) {
-      qf[kc][0] = pack_half2(acc[2 * kc][0] * kLog2eP, acc[2 * kc][1] * kLog2eP);
-      qf[kc][1] = pack_half2(acc[2 * kc][2] * kLog2eP, acc[2 * kc][3] * kLog2eP);
-      qf[kc][2] = pack_half2(acc[2 * kc + 1][0] * kLog2eP, acc[2 * kc + 1][1] * kLog2eP);
-      qf[kc][3] = pack_half2(acc[2 * kc + 1][2] * kLog2eP, acc[2 * kc + 1][3] * kLog2eP);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = acc[2 * kc + (i >> 1)][2 * (i & 1)] * kLog2eP;
+        const float y = acc[2 * kc + (i >> 1)][2 * (i & 1) + 1] * kLog2eP;
+        if constexpr (HP) qf[kc][i] = split_half2(x, y, ql[kc][i]);
+        else qf[kc][i] = pack_half2(x, y);
+      }
     }
   }
 
@@ -256,6 +305,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
         const int j = e >> 2, r = e & 3;
         const int coord = 16 * j + 2 * qd + (r & 1) + ((r >> 1) << 3);
         Ks[tok * G::LD + coord] = lutk[code];
+        if constexpr (HP) Kl[tok * G::LD + coord] = lutkl[code];
       }
       // V: thread -> (token, two octets); octet o lists coordinates o, o+8, ...
       constexpr int OB = (D / 8) * VB;                 // bits per octet
@@ -275,6 +325,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
             code = __funnelshift_r(w, w2, bo & 31) & ((1u << VB) - 1u);
           }
           Vs[tok * G::LD + oct + 8 * c] = lutv[code];
+          if constexpr (HP) Vl[tok * G::LD + oct + 8 * c] = lutvl[code];
         }
       }
       if (tid < 64) {
@@ -312,6 +363,13 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
           frag_b_nk(bf, Ks, G::LD, 8 * n, 16 * kc, lane);
           mma_f16_16816(s[n], qf[kc], bf[0], bf[1]);
           mma_f16_16816(s[n + 1], qf[kc], bf[2], bf[3]);
+          if constexpr (HP) {
+            mma_f16_16816(s[n], ql[kc], bf[0], bf[1]);
+            mma_f16_16816(s[n + 1], ql[kc], bf[2], bf[3]);
+            frag_b_nk(bf, Kl, G::LD, 8 * n, 16 * kc, lane);
+            mma_f16_16816(s[n], qf[kc], bf[0], bf[1]);
+            mma_f16_16816(s[n + 1], qf[kc], bf[2], bf[3]);
+          }
         }
       }
       // norms, causal mask, running max
@@ -354,7 +412,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
       }
       const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
       // ---- P' = P * ||v|| as A fragments; O += P' V ----------------------
-      uint32_t pa[4][4];
+      uint32_t pa[4][4], pl[HP ? 4 : 1][4];
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
         const int kl = 8 * n + 2 * tq;
@@ -363,8 +421,14 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
         l0 += p00 + p01;
         l1 += p10 + p11;
         const float w0 = vn[kl], w1 = vn[kl + 1];
-        pa[n >> 1][(n & 1) * 2 + 0] = pack_half2(p00 * w0, p01 * w1);
-        pa[n >> 1][(n & 1) * 2 + 1] = pack_half2(p10 * w0, p11 * w1);
+        const int i = (n & 1) * 2;
+        if constexpr (HP) {
+          pa[n >> 1][i] = split_half2(p00 * w0, p01 * w1, pl[n >> 1][i]);
+          pa[n >> 1][i + 1] = split_half2(p10 * w0, p11 * w1, pl[n >> 1][i + 1]);
+        } else {
+          pa[n >> 1][i] = pack_half2(p00 * w0, p01 * w1);
+          pa[n >> 1][i + 1] = pack_half2(p10 * w0, p11 * w1);
+        }
       }
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk) {
@@ -375,6 +439,13 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
           frag_b_kn(bf, Vs, G::LD, 8 * n, 16 * kk, lane);
           mma_f16_16816(O[n], a, bf[0], bf[1]);
           mma_f16_16816(O[n + 1], a, bf[2], bf[3]);
+          if constexpr (HP) {
+            mma_f16_16816(O[n], pl[kk], bf[0], bf[1]);
+            mma_f16_16816(O[n + 1], pl[kk], bf[2], bf[3]);
+            frag_b_kn(bf, Vl, G::LD, 8 * n, 16 * kk, lane);
+            mma_f16_16816(O[n], a, bf[0], bf[1]);
+            mma_f16_16816(O[n + 1], a, bf[2], bf[3]);
+          }
         }
       }
     }
@@ -404,17 +475,27 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
     for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
 #pragma unroll
     for (int kc = 0; kc < NC; ++kc) {
-      uint32_t a[4];
-      a[0] = pack_half2(O[2 * kc][0] * i0, O[2 * kc][1] * i0);
-      a[1] = pack_half2(O[2 * kc][2] * i1, O[2 * kc][3] * i1);
-      a[2] = pack_half2(O[2 * kc + 1][0] * i0, O[2 * kc + 1][1] * i0);
-      a[3] = pack_half2(O[2 * kc + 1][2] * i1, O[2 * kc + 1][3] * i1);
+      uint32_t a[4], al[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = O[2 * kc + (i >> 1)][2 * (i & 1)] * (i & 1 ? i1 : i0);
+        const float y = O[2 * kc + (i >> 1)][2 * (i & 1) + 1] * (i & 1 ? i1 : i0);
+        if constexpr (HP) a[i] = split_half2(x, y, al[i]);
+        else a[i] = pack_half2(x, y);
+      }
 #pragma unroll
       for (int n = 0; n < NT; n += 2) {
         uint32_t bf[4];
         frag_b_kn(bf, Rs, G::LD, 8 * n, 16 * kc, lane);   // B[k][n] = R[k][n]
         mma_f16_16816(acc[n], a, bf[0], bf[1]);
         mma_f16_16816(acc[n + 1], a, bf[2], bf[3]);
+        if constexpr (HP) {
+          mma_f16_16816(acc[n], al, bf[0], bf[1]);
+          mma_f16_16816(acc[n + 1], al, bf[2], bf[3]);
+          frag_b_kn(bf, Rl, G::LD, 8 * n, 16 * kc, lane);
+          mma_f16_16816(acc[n], a, bf[0], bf[1]);
+          mma_f16_16816(acc[n + 1], a, bf[2], bf[3]);
+        }
       }
     }
     const int r0 = t0 + gq, r1 = r0 + 8;
@@ -464,9 +545,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
 
 using PfFn = void (*)(PrefillParams);
 
-template <int D, bool RG>
+template <int D, bool RG, bool HP = false>
 PfFn pf_fn(int kb, int vb) {
-#define TQ_PF(K, V) if (kb == K && vb == V) return prefill_kernel<D, K, V, RG>;
+#define TQ_PF(K, V) if (kb == K && vb == V) return prefill_kernel<D, K, V, RG, HP>;
   TQ_PF(4, 2) TQ_PF(3, 3) TQ_PF(2, 2) TQ_PF(4, 4) TQ_PF(6, 4) TQ_PF(5, 5) TQ_PF(6, 6)
   TQ_PF(8, 8) TQ_PF(3, 2) TQ_PF(4, 3)
 #undef TQ_PF
@@ -481,7 +562,9 @@ bool prefill_supported(int D, int kb, int vb) {
   return false;
 }
 
-// Ragged batch on the mma.sync kernel; `grid` bounds the work list.
+// Ragged batch on the mma.sync kernel; `grid` bounds the work list.  bf16 results
+// take single fp16 operands (their rounding, 2^-12 of each, is a sixteenth of the
+// result's own); fp16 and fp32 ones hi + lo.
 int launch_attend_mma(const tq_geom* G, const tq_tables* t, const tq_cache* c,
                       const tq_attend_args* a, const RaggedAttend& rg, int64_t Hkv, int hc,
                       int64_t grid, uint32_t* status, cudaStream_t st) {
@@ -508,10 +591,18 @@ int launch_attend_mma(const tq_geom* G, const tq_tables* t, const tq_cache* c,
   p.causal = a->causal;
   p.status = status;
   p.rg = rg;
-  PfFn fn = G->head_dim == 128 ? pf_fn<128, true>(G->key_bits, G->value_bits)
-                               : pf_fn<64, true>(G->key_bits, G->value_bits);
-  const int smem = G->head_dim == 128 ? Pf<128, 4, 4>::smem(p.page_pitch)
-                                      : Pf<64, 4, 4>::smem(p.page_pitch);
+  p.rot = t->rot;
+  const int kb = G->key_bits, vb = G->value_bits;
+  const bool wide = G->head_dim == 128;
+  PfFn fn;
+  int smem;
+  if (attend_precise(a)) {
+    fn = wide ? pf_fn<128, true, true>(kb, vb) : pf_fn<64, true, true>(kb, vb);
+    smem = wide ? Pf<128, 4, 4, true>::smem(p.page_pitch) : Pf<64, 4, 4, true>::smem(p.page_pitch);
+  } else {
+    fn = wide ? pf_fn<128, true>(kb, vb) : pf_fn<64, true>(kb, vb);
+    smem = wide ? Pf<128, 4, 4, false>::smem(p.page_pitch) : Pf<64, 4, 4, false>::smem(p.page_pitch);
+  }
   if (set_smem_attr((const void*)fn, smem) != TQ_OK) return TQ_ERR_CUDA;
   fn<<<(unsigned)grid, kPfThreads, smem, st>>>(p);
   return check_launch("tq_attend_ragged");
@@ -552,8 +643,8 @@ int launch_prefill(const tq_geom* G, const tq_tables* t, const tq_cache* c,
   if (p.Tq == 0) return TQ_OK;
   PfFn fn = G->head_dim == 128 ? pf_fn<128, false>(G->key_bits, G->value_bits)
                                : pf_fn<64, false>(G->key_bits, G->value_bits);
-  const int smem = G->head_dim == 128 ? Pf<128, 4, 4>::smem(p.page_pitch)
-                                      : Pf<64, 4, 4>::smem(p.page_pitch);
+  const int smem = G->head_dim == 128 ? Pf<128, 4, 4, false>::smem(p.page_pitch)
+                                      : Pf<64, 4, 4, false>::smem(p.page_pitch);
   if (!fn) {
     set_error("tq_prefill_attn: no kernel for head_dim %d, key_bits %d, value_bits %d",
               G->head_dim, G->key_bits, G->value_bits);

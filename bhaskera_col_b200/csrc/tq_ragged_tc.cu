@@ -53,6 +53,12 @@ constexpr int kRing = 4;                   // tiles of per-vector data in flight
 constexpr int kSmem = 227 * 1024;
 constexpr float kCmp = 1.2676506e30f;      // 2^100
 constexpr float kRScale = 64.f;
+// Append: a coordinate of the unit vector R x / ||x|| this near to a boundary is
+// computed again in 64 bits, so that the codes are those of exact arithmetic.
+// The operands' 22 bits and the sums' rounding leave the first value a few 1e-8
+// off (one code in 600,000 came out wrong); 5e-7 is over ten times that, and one
+// coordinate in 60,000 (128 dims, 4 bits).
+constexpr float kNear = 3e-7f;
 
 // i / d for 0 <= i < 2^31 as a product: m = ceil(2^(31 + s) / d), 2^s >= d.
 struct FastDiv {
@@ -351,13 +357,24 @@ __device__ __forceinline__ void issue_tiles(const Pipe& pp, uint32_t tmem, int f
 // ---------------------------------------------------------------------------
 // append
 // ---------------------------------------------------------------------------
+// A run of 32 coordinates with one beside a boundary, noted by the epilogue.
+struct Again {
+  uint8_t* out;                            // the run's codes in its page row
+  int i;                                   // vector
+  uint32_t row;                            // of the rotation table; run of the vector in bits 30, 31
+};
+// Noted per epilogue warp, in the warp's order, and left as they are past that:
+// at one run in 2,000 the 8 warps' lists last for 60,000 vectors of 128 per SM.
+constexpr int kAgain = 32;
+
 template <int D>
 struct AppendSmem {
   static constexpr int OFF_B = 0;
   static constexpr int OFF_A = OFF_B + 2 * Shape<D>::kB;           // 2 stages of hi, lo
   static constexpr int OFF_BND = OFF_A + 4 * Shape<D>::kTerm;      // [256]
   static constexpr int OFF_W = OFF_BND + 1024;                     // [D] norm weights
-  static constexpr int OFF_REQ = OFF_W + 4 * D;                    // offsets and lengths
+  static constexpr int OFF_AGAIN = OFF_W + 4 * D;                  // noted runs, their counts
+  static constexpr int OFF_REQ = OFF_AGAIN + AppendRoles<D>::kEpi * (kAgain * (int)sizeof(Again) + 4);
   static constexpr int OFF_VEC = OFF_REQ + kStagedBytes;           // [kRing]
   static constexpr int OFF_PIPE = OFF_VEC + kRing * (int)sizeof(Vecs);
   static constexpr int OFF_LUT = OFF_PIPE + kPipeBytes;
@@ -388,9 +405,74 @@ __device__ __forceinline__ float sum_lanes(float x) {
   return x;
 }
 
+// The run's codes in 64 bits, a coordinate per lane; xs: D doubles of the warp's.
+template <int D, int BITS>
+__device__ __forceinline__ void exact_run(const RaggedTc& p, int which, const float* weight,
+                                          const float* bnd, const Again& e, double* xs) {
+  constexpr int nb = (1 << BITS) - 1;
+  const int lane = threadIdx.x & 31;
+  const HeadXform& f = p.f;
+  const bool norm = which == 0 && f.weight;
+  const int rot = which == 0 && f.cos_sin ? f.rot : 0, half = rot / 2;
+  const int64_t* st = p.stride[which];
+  const int n = p.by_h.div(e.i);
+  const int64_t base = (int64_t)n * st[1] + (int64_t)(e.i - n * p.H) * st[0];
+  const float* cs = f.cos_sin + (int64_t)(e.row & 0x3FFFFFFFu) * rot;
+  // the sums before the rotation (the head norm's) and of what it gives
+  double raw = 0.0, ss = 0.0;
+#pragma unroll
+  for (int k = 0; k < D / 32; ++k) {
+    const int d = lane + 32 * k;
+    double x = load_elem(p.x[which], p.dtype[which], base + d);
+    raw += x * x;
+    if (norm) x *= weight[d];
+    if (d < rot) {
+      const int a = f.interleaved ? d >> 1 : d < half ? d : d - half;    // angle
+      const bool second = f.interleaved ? d & 1 : d >= half;
+      const int with = f.interleaved ? d ^ 1 : second ? d - half : d + half;
+      double z = load_elem(p.x[which], p.dtype[which], base + with);
+      if (norm) z *= weight[with];
+      x = x * cs[a] + z * (second ? cs[half + a] : -cs[half + a]);
+    }
+    ss += x * x;
+    xs[d] = x;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    raw += __shfl_xor_sync(0xffffffffu, raw, o);
+    ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  }
+  __syncwarp();
+  const int col = 32 * (e.row >> 30) + lane;
+  const float4* R = reinterpret_cast<const float4*>(
+      p.rot + (which == 0 ? k_coord_at(col, D) : v_coord_at(col, D)) * D);
+  double y[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll 8
+  for (int d = 0; d < D; d += 4) {
+    const float4 w = __ldg(R + d / 4);
+    y[0] += xs[d] * w.x;
+    y[1] += xs[d + 1] * w.y;
+    y[2] += xs[d + 2] * w.z;
+    y[3] += xs[d + 3] * w.w;
+  }
+  __syncwarp();                            // before the next run's xs
+  // the head norm's factor matters where the unit vector's floor of 1e-8 does
+  const double r = norm ? rsqrt(raw / D + (double)f.eps) : 1.0;
+  const double len = fmax(sqrt(ss) * r, 1e-8), v = ((y[0] + y[1]) + (y[2] + y[3])) * r;
+  uint32_t code = 0;
+  for (int k = 0; k < nb; ++k) code += bnd[k] * len < v;
+#pragma unroll
+  for (int x = 0; x < BITS; ++x) {
+    const int sh = lane * BITS - 32 * x;   // the code's place in word x
+    const uint32_t own = sh <= -BITS || sh >= 32 ? 0u : sh >= 0 ? code << sh : code >> -sh;
+    const uint32_t word = __reduce_or_sync(0xffffffffu, own);
+    if (lane == x) reinterpret_cast<uint32_t*>(e.out)[x] = word;
+  }
+}
+
 template <int D, int BITS>
 __global__ void __launch_bounds__(AppendRoles<D>::kThreads, 1)
-append_ragged_tc_kernel(RaggedTc p, int which) {
+append_ragged_tc_kernel(const __grid_constant__ RaggedTc p, int which) {
   using S = Shape<D>;
   using W = AppendRoles<D>;
   constexpr int kMakers = W::kMakers, kThreads = W::kThreads;
@@ -416,6 +498,8 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
   }
   for (int i = tid; i < nb; i += kThreads) bnd[i] = p.bnd[which][i];
   float* weight = reinterpret_cast<float*>(sm + SM::OFF_W);
+  Again* again = reinterpret_cast<Again*>(sm + SM::OFF_AGAIN);    // [epilogue warps][kAgain]
+  int* nagain = reinterpret_cast<int*>(again + W::kEpi * kAgain);
   if (which == 0 && p.f.weight)
     for (int i = tid; i < D; i += kThreads)
       weight[i] = load_elem(p.f.weight, p.f.w_dtype, i) + p.f.w_offset;
@@ -655,7 +739,8 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
     const uint32_t lane_off = smem_u32(sm + SM::OFF_LUT) + (uint32_t)((lane & 15) * 8) -
                               (0x4B000000u << 7);
     const float par0 = lutpar[0], c2l = lutpar[1];
-    int it = 0;
+    Again* mine = again + kAgain * (warp - W::kEpi0);
+    int it = 0, noted = 0;
     for (int tile = first; tile < p.ntiles; tile += step, ++it) {
       const int ac = it & 1;
       bool ok = wait_for(&pp.acc_full[ac], (uint32_t)((it / 2) & 1), pp.abort_flag, p.status);
@@ -674,14 +759,12 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
         if (ch == NCH - 1) {
           tc::tc_fence_before();
           __syncwarp();
-          if (lane == 0) {
-            tc::mbar_arrive_cta(&pp.acc_empty[ac]);
-            tc::mbar_arrive_cta(&pp.loc_free[it % kRing]);
-          }
+          if (lane == 0) tc::mbar_arrive_cta(&pp.acc_empty[ac]);
         }
         uint32_t words[BITS];
 #pragma unroll
         for (int x = 0; x < BITS; ++x) words[x] = 0u;
+        float near = INFINITY;             // least distance to a boundary, times 2^100
         if (ncells > 0) {
           // codes gather in runs of <= 23 bits as acc = 2^23 + field, exactly
           auto flush = [&](float acc, int o, int len) {
@@ -705,7 +788,9 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
             const float u = __saturatef(fmaf(y, ca, 0.5f));
             const float cell = fmaf(u, c2l, 8388608.f);
             const float2 e = tc::lds_f2((__float_as_uint(cell) << 7) + lane_off);
-            const float above = __saturatef(fmaf(y, cK, e.x) * kCmp);
+            const float over = fmaf(y, cK, e.x);
+            const float above = __saturatef(over * kCmp);
+            near = fminf(near, fabsf(over));
             acc = fmaf(e.y + above, (float)(1u << gl), acc);
             gl += BITS;
           }
@@ -713,7 +798,10 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            const uint32_t code = (uint32_t)bucketize_lt(bnd, nb, __uint_as_float(yb[j]) * inv);
+            const float y = __uint_as_float(yb[j]) * inv;
+            const uint32_t code = (uint32_t)bucketize_lt(bnd, nb, y);
+            near = fminf(near, kCmp * fminf(code > 0 ? fabsf(y - bnd[code - 1]) : 1.f,
+                                            code < nb ? fabsf(y - bnd[code]) : 1.f));
             const int bo = j * BITS, wi = bo >> 5, sh = bo & 31;
             words[wi] += code << sh;
             if (sh + BITS > 32) words[wi + 1] += code >> (32 - sh);
@@ -735,10 +823,22 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
             for (int x = 0; x < BITS; ++x) reinterpret_cast<uint32_t*>(row)[x] = words[x];
           }
         }
+        const bool note = near < kNear * kCmp && n > 0.f && page;
+        const uint32_t notes = __ballot_sync(0xffffffffu, note);
+        if (notes) {
+          const int at = noted + __popc(notes & ((1u << lane) - 1u));
+          if (note && at < kAgain)
+            mine[at] = {page + sec + slot * row_bytes + run * (4 * BITS), tile * kM + r,
+                        (uint32_t)vec.row[r] | (uint32_t)run << 30};
+          noted += __popc(notes);
+        }
       }
       if (page && part == 0)
         reinterpret_cast<__half*>(page + noff)[slot] = __float2half_rn(n);
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive_cta(&pp.loc_free[it % kRing]);
     }
+    if (lane == 0) nagain[warp - W::kEpi0] = tmin(noted, kAgain);
   }
   tc::tc_fence_before();
   __syncthreads();
@@ -746,6 +846,13 @@ append_ragged_tc_kernel(RaggedTc p, int which) {
     __syncwarp();
     tc::tc_fence_after();
     tc::tmem_dealloc(tmem, 2 * D);
+  }
+  // runs beside a boundary again, over the operands' place
+  double* xs = reinterpret_cast<double*>(sm + SM::OFF_A) + D * warp;
+  for (int w = 0, k = warp; w < W::kEpi; ++w) {
+    for (; k < nagain[w]; k += kThreads / 32)
+      exact_run<D, BITS>(p, which, weight, bnd, again[kAgain * w + k], xs);
+    k -= nagain[w];
   }
   pdl_wait();
 }
@@ -1129,7 +1236,7 @@ int launch_append_ragged_tc(const tq_geom* G, const tq_tables* t, const tq_cache
                             uint32_t* status, cudaStream_t st) {
   const int D = G->head_dim;
   if (D != 64 && D != 128) return 1;
-  if (k->shape[1] * k->shape[2] > INT32_MAX - kM || (rope && rope->rot_dim % 16)) return 1;
+  if (k->shape[1] * k->shape[2] > INT32_MAX - kM || (rope && (rope->rot_dim % 16 || rope->positions >> 30))) return 1;
   if (reinterpret_cast<uintptr_t>(t->rot) % 16) return 1;
   const tq_tensor4* x[2] = {k, v};
   for (int w = 0; w < 2; ++w)

@@ -719,3 +719,35 @@ def test_inputs_of_a_backward_pass_and_mixed_devices_are_refused():
     with pytest.raises(_lib.TqError, match="overlaps"):
         buf = randn((4, 2, 128), 2)
         ops.qk_rope(buf[:3], None, table, pos, q_out=buf[1:])
+
+
+@pytest.mark.parametrize("D,kb,vb,dtype,pairs,norm", [
+    (64, 3, 3, F16, "interleaved", False), (64, 4, 2, F32, "half", True),
+    (128, 4, 4, BF16, "half", True), (128, 5, 1, F16, "part", True), (128, 6, 4, BF16, "none", False)])
+def test_append_ragged_codes_are_those_of_exact_arithmetic(D, kb, vb, dtype, pairs, norm):
+    """A million coordinates: about one of 32-bit arithmetic's codes in a million is off by one;
+    none is here.  Coordinates within 64-bit rounding (1e-12) of a boundary may go either way."""
+    tables = make_tables(D, kb, vb, False)
+    H, n = 4, (1 << 20) // (4 * D) - 5
+    batch, start, seq = make_batch([(n - 700, n - 700), (700, 900)])
+    pages = make_paged(tables, 2 * H, max(seq))
+    k, v = randn((n, H, D), 21, dtype), randn((n, H, D), 22, dtype, 7)
+    rope = None if pairs == "none" else \
+        ops.RopeTable.build(D // 2 if pairs == "part" else D, n,
+                            interleaved=pairs == "interleaved", device=DEV)
+    w = ops.HeadNorm(1 + 0.2 * randn((D,), 23, F32), 1e-6) if norm else None
+    ops.append_ragged(tables, pages, k, v, batch, rope=rope, k_norm=w)
+    got = S.parse(tables, contiguous(pages), max(seq))
+    r, pos = S.positions(start, seq, n)
+    kx = S.rope(k, rope.cos_sin if rope else None, pos, pairs == "interleaved",
+                w.weight if w else None, 1e-6)
+    R = tables.rot.double().cpu().numpy()
+    for name, x, bnd in (("k_idx", kx, tables.k_boundaries), ("v_idx", v, tables.v_boundaries)):
+        x = np.asarray(x.double().cpu().numpy() if torch.is_tensor(x) else x, dtype=np.float64)
+        y = (x / np.linalg.norm(x, axis=-1, keepdims=True)) @ R.T
+        b = bnd.double().cpu().numpy()[: (1 << (kb if name[0] == "k" else vb)) - 1]
+        at = np.searchsorted(b, y, side="left")
+        gap = np.abs(y[..., None] - b[np.clip(np.stack([at - 1, at], -1), 0, len(b) - 1)]).min(-1)
+        have = got[name].reshape(2, H, -1, D)[r, :, pos]
+        assert not ((have != at) & (gap > 1e-12)).any()
+    assert ok_status() == 0
