@@ -89,7 +89,8 @@ __device__ __forceinline__ void for_tiles(const PlanParams& p, F f) {
 struct QueryParams {
   const void* q; int q_dtype; int q_vec; int64_t qs[3];    // head, row, dim; 16-byte pieces
   const __half* rot_h;
-  __half* qp;
+  const float* rot;                                        // for hi + lo, or NULL
+  __half* qp;                                              // [token][Hq][D], or [2][D] of hi and lo
   int64_t qp_stride;                                       // FewParams::qp_stride
   float qscale;
   int Hq, D, blocks;                                       // blocks of 64 rows looked at per request
@@ -97,13 +98,21 @@ struct QueryParams {
 
 constexpr int kQRows = 64;
 
+__device__ __forceinline__ uint32_t split_half2(float a, float b, uint32_t& lo) {
+  const uint32_t hi = pack_half2(a, b);
+  const __half2 h = *reinterpret_cast<const __half2*>(&hi);
+  lo = pack_half2(a - __low2float(h), b - __high2float(h));
+  return hi;
+}
+
 // 32 warps: four tiles of 16 rows, eight warps each, every eighth 8-wide slice
-// of the result.
-template <int D>
+// of the result.  HP: q and R as fp16 hi + lo (three products), so is q'.
+template <int D, bool HP>
 __device__ __forceinline__ void rotate_queries(const PlanParams& p, const QueryParams& qp, int first,
                                                int step, unsigned char* sm) {
   constexpr int LD = D + 8;                                // halves per staged row (banks)
   __half* A = reinterpret_cast<__half*>(sm);
+  __half* Al = A + kQRows * LD;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, tq = lane & 3;
   for (int64_t item = first; item < p.rv.R * qp.blocks; item += step) {
     const int64_t r = item / qp.blocks;
@@ -116,7 +125,7 @@ __device__ __forceinline__ void rotate_queries(const PlanParams& p, const QueryP
       for (int i = tid; i < kQRows * D / 8; i += kPlanThreads) {
         const int n = i / (D / 8), c = i % (D / 8);
         const int row = (int)row0 + n;
-        uint32_t w[4] = {0u, 0u, 0u, 0u};
+        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (row < rows) {
           const int tok = row / qp.Hq, h = row - tok * qp.Hq;
           const int64_t at = (rq.q0 + tok) * qp.qs[1] + h * qp.qs[0] + (int64_t)(8 * c) * qp.qs[2];
@@ -125,48 +134,78 @@ __device__ __forceinline__ void rotate_queries(const PlanParams& p, const QueryP
             const uint32_t u[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float2 f = qp.q_dtype == TQ_F16
+              const float2 y = qp.q_dtype == TQ_F16
                                    ? __half22float2(*reinterpret_cast<const __half2*>(&u[e]))
                                    : make_float2(__uint_as_float(u[e] << 16),
                                                  __uint_as_float(u[e] & 0xFFFF0000u));
-              w[e] = pack_half2(f.x * qp.qscale, f.y * qp.qscale);
+              f[2 * e] = y.x;
+              f[2 * e + 1] = y.y;
             }
           } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              w[e] = pack_half2(load_elem(qp.q, qp.q_dtype, at + (2 * e) * qp.qs[2]) * qp.qscale,
-                                load_elem(qp.q, qp.q_dtype, at + (2 * e + 1) * qp.qs[2]) * qp.qscale);
+            for (int e = 0; e < 8; ++e) f[e] = load_elem(qp.q, qp.q_dtype, at + e * qp.qs[2]);
           }
         }
+        uint32_t w[4], l[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = split_half2(f[2 * e] * qp.qscale, f[2 * e + 1] * qp.qscale, l[e]);
         *reinterpret_cast<uint4*>(A + n * LD + 8 * c) = make_uint4(w[0], w[1], w[2], w[3]);
+        if constexpr (HP) *reinterpret_cast<uint4*>(Al + n * LD + 8 * c) = make_uint4(l[0], l[1], l[2], l[3]);
       }
       __syncthreads();
       const int m0 = 16 * (warp >> 3);
       for (int jt = warp & 7; jt < D / 8; jt += 8) {
         float c[4] = {0.f, 0.f, 0.f, 0.f};
         uint32_t b[D / 16][2];
-        const uint32_t* R = reinterpret_cast<const uint32_t*>(qp.rot_h + (8 * jt + gq) * D) + tq;
-#pragma unroll
-        for (int ch = 0; ch < D / 16; ++ch) {
-          b[ch][0] = __ldg(R + 8 * ch);
-          b[ch][1] = __ldg(R + 8 * ch + 4);
-        }
-#pragma unroll
-        for (int ch = 0; ch < D / 16; ++ch) {
-          uint32_t a[4];
+        auto frag = [&](uint32_t (&a)[4], const __half* at, int ch) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            a[i] = *reinterpret_cast<const uint32_t*>(A + (m0 + gq + 8 * (i & 1)) * LD + 16 * ch +
+            a[i] = *reinterpret_cast<const uint32_t*>(at + (m0 + gq + 8 * (i & 1)) * LD + 16 * ch +
                                                       2 * tq + 8 * (i >> 1));
-          mma_f16_16816(c, a, b[ch][0], b[ch][1]);
+        };
+        uint32_t a[4];
+        if constexpr (HP) {
+          const float2* R = reinterpret_cast<const float2*>(qp.rot + (8 * jt + gq) * D) + tq;
+          uint32_t bl[D / 16][2];
+#pragma unroll
+          for (int ch = 0; ch < D / 16; ++ch)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float2 x = __ldg(R + 8 * ch + 4 * i);
+              b[ch][i] = split_half2(x.x, x.y, bl[ch][i]);
+            }
+#pragma unroll
+          for (int ch = 0; ch < D / 16; ++ch) {
+            frag(a, A, ch);
+            mma_f16_16816(c, a, b[ch][0], b[ch][1]);
+            mma_f16_16816(c, a, bl[ch][0], bl[ch][1]);
+            frag(a, Al, ch);
+            mma_f16_16816(c, a, b[ch][0], b[ch][1]);
+          }
+        } else {
+          const uint32_t* R = reinterpret_cast<const uint32_t*>(qp.rot_h + (8 * jt + gq) * D) + tq;
+#pragma unroll
+          for (int ch = 0; ch < D / 16; ++ch) {
+            b[ch][0] = __ldg(R + 8 * ch);
+            b[ch][1] = __ldg(R + 8 * ch + 4);
+          }
+#pragma unroll
+          for (int ch = 0; ch < D / 16; ++ch) {
+            frag(a, A, ch);
+            mma_f16_16816(c, a, b[ch][0], b[ch][1]);
+          }
         }
         // dims 8 jt + 2 tq, + 1: word jt of quad tq
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int64_t row = row0 + m0 + gq + 8 * i;
-          if (row < rows)
-            reinterpret_cast<uint32_t*>(qp.qp + (tok0 * qp.Hq + row) * D)[tq * (D / 8) + jt] =
-                pack_half2(c[2 * i], c[2 * i + 1]);
+          if (row < rows) {
+            uint32_t* dst = reinterpret_cast<uint32_t*>(qp.qp + (tok0 * qp.Hq + row) * (HP ? 2 * D : D)) +
+                            tq * (D / 8) + jt;
+            uint32_t lo;
+            dst[0] = split_half2(c[2 * i], c[2 * i + 1], lo);
+            if constexpr (HP) dst[D / 2] = lo;
+          }
         }
       }
     }
@@ -182,10 +221,12 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p0
                                                                    int lists, QueryParams qp) {
   pdl_launch_dependents();
   if ((int)blockIdx.x >= lists) {
-    __shared__ __align__(16) unsigned char sm[kQRows * (128 + 8) * 2];
+    __shared__ __align__(16) unsigned char sm[2 * kQRows * (128 + 8) * 2];
     const int first = blockIdx.x - lists, step = gridDim.x - lists;
-    if (qp.D == 128) rotate_queries<128>(p0, qp, first, step, sm);
-    else rotate_queries<64>(p0, qp, first, step, sm);
+    if (qp.D == 128 && qp.rot) rotate_queries<128, true>(p0, qp, first, step, sm);
+    else if (qp.D == 128) rotate_queries<128, false>(p0, qp, first, step, sm);
+    else if (qp.rot) rotate_queries<64, true>(p0, qp, first, step, sm);
+    else rotate_queries<64, false>(p0, qp, first, step, sm);
     return;
   }
   const PlanParams& p = blockIdx.x == 0 ? p0 : p1;
@@ -285,9 +326,10 @@ AttendShape attend_shape(const tq_geom* G, const tq_cache* c, const tq_attend_ar
   const int64_t R = a->batch.requests, N = a->q->shape[2], most = INT64_MAX;
   s.Hkv = c->streams / R;
   const int64_t g = a->q->shape[1] / s.Hkv;
-  const bool pick = a->engine == 0 && !attend_precise(a);
-  s.tc = prefill_tc_applies(G) && (pick || a->engine == 2);
-  const bool can = attend_few_applies(G) && (pick || a->engine == 3);
+  // fp16 and fp32 results of many rows: the tcgen05 kernel's operands are single
+  // fp16 values (error 7e-4, against 2.1e-4 of fp16's own rounding), so mma.sync
+  s.tc = prefill_tc_applies(G) && (a->engine == 2 || (a->engine == 0 && !attend_precise(a)));
+  const bool can = attend_few_applies(G) && (a->engine == 0 || a->engine == 3);
   const int64_t few_q = a->engine == 3 ? most : tmax<int64_t>(kFewRows / g, 1);
   size_t off = 256;                        // the first 64 bytes: the decode's status word
   auto take = [&](size_t bytes) {
@@ -321,7 +363,8 @@ AttendShape attend_shape(const tq_geom* G, const tq_cache* c, const tq_attend_ar
     finish(l);
     // q' rows of its tokens: beside a wide list at most few_q of each request
     s.qp_stride = wide ? few_q : 0;
-    l.off_qp = take((size_t)(wide ? R * few_q : N) * a->q->shape[1] * G->head_dim * 2);
+    l.off_qp = take((size_t)(wide ? R * few_q : N) * a->q->shape[1] * G->head_dim *
+                    (attend_precise(a) ? 4 : 2));
   }
   if (wide) {
     ListShape& l = s.wide;
@@ -395,6 +438,7 @@ int launch_attend_ragged(const tq_geom* G, const tq_tables* t, const tq_cache* c
     qp.q_vec = qp.q_dtype != TQ_F32 && qp.qs[2] == 1 && reinterpret_cast<uintptr_t>(qp.q) % 16 == 0 &&
                qp.qs[0] % 8 == 0 && qp.qs[1] % 8 == 0;
     qp.rot_h = reinterpret_cast<const __half*>(t->rot_f16);
+    qp.rot = attend_precise(a) ? t->rot : nullptr;
     qp.qp = reinterpret_cast<__half*>(base + s.few.off_qp);
     qp.qp_stride = s.qp_stride;
     qp.qscale = a->scale * 1.4426950408889634f;

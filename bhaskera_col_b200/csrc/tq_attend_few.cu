@@ -47,7 +47,8 @@ struct FewParams {
   PageMap pm;
   int page_bytes, off_v, off_kn, off_vn;
   const __half* rot_h;          // R [D][D] fp16
-  const __half* qp;             // q' rows (ragged_plan_kernel), [token][Hq][D] in quad order
+  const float* rot;             // R [D][D] (HP)
+  const __half* qp;             // q' rows (ragged_plan_kernel), [token][Hq][D] in quad order; HP: [2][D], hi and lo
   int64_t qp_stride;            // tokens of q' per request; 0: q' follows the batch's rows
   const float* kc;
   const float* vc;
@@ -61,10 +62,12 @@ struct FewParams {
 
 constexpr int kW = 4;                                       // warps: quarters of a page
 
-template <int D, int KB, int VB, int NT>
+// HP (fp16 and fp32 results): both operands of every product as fp16 hi + lo (hi hi
+// + hi lo + lo hi, 22 bits).  A table entry then holds a pair's hi and lo.
+template <int D, int KB, int VB, int NT, bool HP>
 struct Few {
   static constexpr int NQ = 8 * NT;
-  static constexpr bool KQ = KB == 2, VQ = VB == 2;         // two pairs per table entry
+  static constexpr bool KQ = KB == 2 && !HP, VQ = VB == 2 && !HP;   // two pairs per table entry
   static constexpr int KT = 128 << (KQ ? 8 : 2 * KB), VT = 128 << (VQ ? 8 : 2 * VB);   // tables
   static constexpr int LDO = D + 4;                         // floats per row of an output (banks)
   static constexpr int LDA = D / 2 + 4;                     // words per row of a rotation operand
@@ -75,7 +78,7 @@ struct Few {
   static constexpr int OFF_A = tmax(OFF_ROT + 2 * D * D, kW * NQ * LDO * 4);   // [hi, lo][16][LDA]
   static constexpr int LOOP = KT + VT, END = OFF_A + 2 * 16 * LDA * 4;
   static constexpr int OFF_Q = LOOP > END ? LOOP : END;     // q' fp16 [NQ][D]
-  static constexpr int OFF_M = OFF_Q + 16 * D * 2;          // [kW][NQ] running max
+  static constexpr int OFF_M = OFF_Q + (HP ? 2 : 1) * 16 * D * 2;   // (HP: and lo); [kW][NQ] running max
   static constexpr int OFF_L = OFF_M + kW * NQ * 4;         // [kW][NQ] sums
   static constexpr int OFF_R = OFF_L + kW * NQ * 4;         // [16] sums, [16] maxima, flags
   static constexpr int BYTES = OFF_R + 256;
@@ -152,6 +155,15 @@ __device__ __forceinline__ void lds64(uint32_t addr, uint32_t& x, uint32_t& y) {
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(x), "=r"(y) : "r"(addr));
 }
 
+// HP: field k of x and of y, hi and lo.
+template <int FB, int NW>
+__device__ __forceinline__ void look_up_split(uint32_t base, const uint32_t (&x)[NW],
+                                              const uint32_t (&y)[NW], int k, uint32_t& h0,
+                                              uint32_t& h1, uint32_t& l0, uint32_t& l1) {
+  lds64(field_at<FB>(x, k, base), h0, l0);
+  lds64(field_at<FB>(y, k, base), h1, l1);
+}
+
 // One pair of each of two rows (registers a0 and a1, or a2 and a3, of an A
 // fragment): field k of x and of y, or, with quad entries, byte k of x.
 template <int FB, bool Q, int NW>
@@ -215,10 +227,11 @@ struct FewTile {
 };
 
 // fp16 hi + lo of a pair (2^-22 of each value)
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = pack_half2(a, b);
+__device__ __forceinline__ uint32_t split2(float a, float b, uint32_t& lo) {
+  const uint32_t hi = pack_half2(a, b);
   const __half2 h = *reinterpret_cast<const __half2*>(&hi);
   lo = pack_half2(a - __low2float(h), b - __high2float(h));
+  return hi;
 }
 
 // B fragment (16 deep, 8 wide) of R[j][i], j = 16 ch + .. deep, i = 8 jt + .. wide,
@@ -232,26 +245,48 @@ __device__ __forceinline__ void frag_of_rotation(uint32_t (&b)[2], const unsigne
                : "=r"(b[0]), "=r"(b[1]) : "r"(smem_u32(at)));
 }
 
+// c += O R of 8 columns (8 jt ..): O's hi words, and its lo where LO.
+template <int D, bool LO>
+__device__ __forceinline__ void rotate_slice(float (&c)[4], const unsigned char* rot,
+                                             const uint32_t* A, int jt, int lane) {
+  constexpr int LDA = D / 2 + 4;
+  const int gq = lane >> 2, tq = lane & 3;
+#pragma unroll
+  for (int ch = 0; ch < D / 16; ++ch) {
+    uint32_t r[2], ah[4], al[4];
+    frag_of_rotation<D>(r, rot, ch, jt, lane);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = (gq + 8 * (i & 1)) * LDA + 8 * ch + tq + 4 * (i >> 1);
+      ah[i] = A[at];
+      if (LO) al[i] = A[16 * LDA + at];
+    }
+    mma_f16_16816(c, ah, r[0], r[1]);
+    if (LO) mma_f16_16816(c, al, r[0], r[1]);
+  }
+}
+
 // A table of 128-byte rows from a codebook.
-template <int BITS, bool Q>
+template <int BITS, bool Q, bool HP>
 __device__ __forceinline__ void fill_table(unsigned char* table, const float* cent, int tid,
                                            int nthreads) {
   constexpr int N = 1 << (Q ? 4 * BITS : 2 * BITS);
   constexpr uint32_t M = (1u << BITS) - 1u;
   for (int i = tid; i < 8 * N; i += nthreads) {
     const uint32_t e = (uint32_t)i >> 3;
-    const uint32_t x = pack_half2(__ldg(cent + (e & M)), __ldg(cent + ((e >> BITS) & M)));
-    const uint32_t y = Q ? pack_half2(__ldg(cent + ((e >> (2 * BITS)) & M)),
+    uint32_t lo;
+    const uint32_t x = split2(__ldg(cent + (e & M)), __ldg(cent + ((e >> BITS) & M)), lo);
+    const uint32_t y = HP ? lo : Q ? pack_half2(__ldg(cent + ((e >> (2 * BITS)) & M)),
                                       __ldg(cent + ((e >> (3 * BITS)) & M))) : x;
     reinterpret_cast<uint4*>(table + e * 128)[i & 7] = make_uint4(x, y, x, y);
   }
 }
 
 // One segment of the work list.
-template <int D, int KB, int VB, int NT>
+template <int D, int KB, int VB, int NT, bool HP>
 __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork& sw,
                                                unsigned char* sm) {
-  using F = Few<D, KB, VB, NT>;
+  using F = Few<D, KB, VB, NT, HP>;
   using Tile = FewTile<D, KB, VB>;
   constexpr int NQ = F::NQ, NC = D / 16, kThreads = 32 * kW, LDA = F::LDA, LDO = F::LDO;
   constexpr int KROW = D * KB / 8, VROW = D * VB / 8;
@@ -332,16 +367,20 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
     return n * (D / 8) + t * (D / 32) + (k ^ f);
   };
   const int64_t tok0 = p.qp_stride ? sw.seg.req * p.qp_stride : sw.rq.q0;
-  for (int i = tid; i < NQ * D / 8; i += kThreads) {
-    const int n = i / (D / 8), c = i % (D / 8);
-    unsigned char* dst = sm + F::OFF_Q + 16 * q_piece(n, c / (D / 32), c % (D / 32));
-    if (row_valid(n))
-      cp_async16(dst, p.qp + ((tok0 + row_pos(n)) * p.Hq + h0 + n % p.hc) * D + 8 * c);
-    else
-      *reinterpret_cast<uint4*>(dst) = make_uint4(0u, 0u, 0u, 0u);
-  }
-  fill_table<KB, F::KQ>(sm, p.kc, tid, kThreads);
-  fill_table<VB, F::VQ>(sm + F::KT, p.vc, tid, kThreads);
+  constexpr int kQLo = 16 * D * 2;                         // HP: lo behind hi
+#pragma unroll
+  for (int part = 0; part < (HP ? 2 : 1); ++part)
+    for (int i = tid; i < NQ * D / 8; i += kThreads) {
+      const int n = i / (D / 8), c = i % (D / 8);
+      unsigned char* dst = sm + F::OFF_Q + part * kQLo + 16 * q_piece(n, c / (D / 32), c % (D / 32));
+      if (row_valid(n))
+        cp_async16(dst, p.qp + ((tok0 + row_pos(n)) * p.Hq + h0 + n % p.hc) * (HP ? 2 * D : D) +
+                            part * D + 8 * c);
+      else
+        *reinterpret_cast<uint4*>(dst) = make_uint4(0u, 0u, 0u, 0u);
+    }
+  fill_table<KB, F::KQ, HP>(sm, p.kc, tid, kThreads);
+  fill_table<VB, F::VQ, HP>(sm + F::KT, p.vc, tid, kThreads);
   cp_async_wait_all();
   __syncthreads();
 
@@ -366,8 +405,8 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
     }
   lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, 1));
   lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, 2));
-  const uint32_t k_base = smem_u32(sm) + (F::KQ ? 8 * (lane & 15) : 4 * lane);
-  const uint32_t v_base = smem_u32(sm + F::KT) + (F::VQ ? 8 * (lane & 15) : 4 * lane);
+  const uint32_t k_base = smem_u32(sm) + (F::KQ || HP ? 8 * (lane & 15) : 4 * lane);
+  const uint32_t v_base = smem_u32(sm + F::KT) + (F::VQ || HP ? 8 * (lane & 15) : 4 * lane);
   int bad_key = INT_MAX;
 
   // one page: `cur` is used, `nxt` takes the next page's codes
@@ -404,19 +443,32 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
     // S^T: two chunks of 16 dims share one 16-byte piece of q'
 #pragma unroll
     for (int c2 = 0; c2 < NC / 2; ++c2) {
-      uint4 qb[NT];
+      uint4 qb[NT], ql[HP ? NT : 1];
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-        qb[n] = *reinterpret_cast<const uint4*>(sm + F::OFF_Q + 16 * q_piece(8 * n + gq, tq, c2));
+      for (int n = 0; n < NT; ++n) {
+        const unsigned char* at = sm + F::OFF_Q + 16 * q_piece(8 * n + gq, tq, c2);
+        qb[n] = *reinterpret_cast<const uint4*>(at);
+        if constexpr (HP) ql[n] = *reinterpret_cast<const uint4*>(at + kQLo);
+      }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        uint32_t a[4];
+        uint32_t a[4], al[4];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          look_up2<2 * KB, F::KQ>(k_base, kw[0], kw[1], 2 * (2 * c2 + c) + i, a[2 * i], a[2 * i + 1]);
+        for (int i = 0; i < 2; ++i) {
+          const int k = 2 * (2 * c2 + c) + i;
+          if constexpr (HP)
+            look_up_split<2 * KB>(k_base, kw[0], kw[1], k, a[2 * i], a[2 * i + 1], al[2 * i], al[2 * i + 1]);
+          else
+            look_up2<2 * KB, F::KQ>(k_base, kw[0], kw[1], k, a[2 * i], a[2 * i + 1]);
+        }
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
           mma_f16_16816(s[n], a, c ? qb[n].z : qb[n].x, c ? qb[n].w : qb[n].y);
+          if constexpr (HP) {
+            mma_f16_16816(s[n], a, c ? ql[n].z : ql[n].x, c ? ql[n].w : ql[n].y);
+            mma_f16_16816(s[n], al, c ? qb[n].z : qb[n].x, c ? qb[n].w : qb[n].y);
+          }
+        }
       }
     }
     // relative to m
@@ -455,7 +507,7 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
           d[n][2 + c] = edge && key0 + 8 > lim[n][c] ? -INFINITY : fmaf(s[n][2 + c], kn[1], -mn);
         }
     }
-    uint32_t pb[NT][2];
+    uint32_t pb[NT][2], pl[HP ? NT : 1][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -463,7 +515,13 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
         const float p0 = fast_exp2(d[n][2 * i]), p1 = fast_exp2(d[n][2 * i + 1]);
         l[n][0] += p0;
         l[n][1] += p1;
-        pb[n][i] = movmatrix_trans(pack_half2(p0 * vn[i], p1 * vn[i]));
+        if constexpr (HP) {
+          uint32_t lo;
+          pb[n][i] = movmatrix_trans(split2(p0 * vn[i], p1 * vn[i], lo));
+          pl[n][i] = movmatrix_trans(lo);
+        } else {
+          pb[n][i] = movmatrix_trans(pack_half2(p0 * vn[i], p1 * vn[i]));
+        }
       }
     }
     constexpr int VW = Codes<Tile::VN>::NW;
@@ -478,12 +536,22 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
     }
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      uint32_t a[4];
+      uint32_t a[4], al[4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        look_up2<2 * VB, F::VQ>(v_base, ve[i], vo[i], c, a[2 * i], a[2 * i + 1]);
+      for (int i = 0; i < 2; ++i) {
+        if constexpr (HP)
+          look_up_split<2 * VB>(v_base, ve[i], vo[i], c, a[2 * i], a[2 * i + 1], al[2 * i], al[2 * i + 1]);
+        else
+          look_up2<2 * VB, F::VQ>(v_base, ve[i], vo[i], c, a[2 * i], a[2 * i + 1]);
+      }
 #pragma unroll
-      for (int n = 0; n < NT; ++n) mma_f16_16816(O[c][n], a, pb[n][0], pb[n][1]);
+      for (int n = 0; n < NT; ++n) {
+        mma_f16_16816(O[c][n], a, pb[n][0], pb[n][1]);
+        if constexpr (HP) {
+          mma_f16_16816(O[c][n], a, pl[n][0], pl[n][1]);
+          mma_f16_16816(O[c][n], al, pb[n][0], pb[n][1]);
+        }
+      }
     }
   };
 #pragma unroll 1
@@ -552,7 +620,18 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
   // R for the last rotation, on its way while a split tile's parts come together
   for (int i = tid; i < D * D / 8; i += kThreads) {
     const int r = i / (D / 8), c = i % (D / 8);
-    cp_async16(sm + F::OFF_ROT + r * (2 * D) + ((c ^ (r & 7)) << 4), p.rot_h + 8 * i);
+    unsigned char* dst = sm + F::OFF_ROT + r * (2 * D) + ((c ^ (r & 7)) << 4);
+    if constexpr (HP) {                                    // lo first
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 x = __ldg(reinterpret_cast<const float2*>(p.rot + 8 * i) + e);
+        split2(x.x, x.y, w[e]);
+      }
+      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+      cp_async16(dst, p.rot_h + 8 * i);
+    }
   }
 
   // ---- a split tile: partials out, the last CTA joins them -----------------------
@@ -648,7 +727,7 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
       u.x *= il;
       u.y *= il;
     }
-    split2(u.x, u.y, A[n * LDA + w], A[(16 + n) * LDA + w]);
+    A[n * LDA + w] = split2(u.x, u.y, A[(16 + n) * LDA + w]);
   }
   cp_async_wait_all();
   __syncthreads();
@@ -660,22 +739,31 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
     o_ok[r] = n < NQ && row_valid(n);
     o_at[r] = o_ok[r] ? row_at(n, p.os) : 0;
   }
-#pragma unroll 1
-  for (int jt = warp; jt < D / 8; jt += kW) {
-    float c[4] = {0.f, 0.f, 0.f, 0.f};
+  constexpr int NJ = D / 8 / kW;
+  // HP: O^hi R^lo first, then the place's other half
+  float lo[HP ? NJ : 1][4];
+  if constexpr (HP) {
 #pragma unroll
-    for (int ch = 0; ch < NC; ++ch) {
-      uint32_t r[2], ah[4], al[4];
-      frag_of_rotation<D>(r, sm + F::OFF_ROT, ch, jt, lane);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int at = (gq + 8 * (i & 1)) * LDA + 8 * ch + tq + 4 * (i >> 1);
-        ah[i] = A[at];
-        al[i] = A[16 * LDA + at];
-      }
-      mma_f16_16816(c, ah, r[0], r[1]);
-      mma_f16_16816(c, al, r[0], r[1]);
+    for (int j = 0; j < NJ; ++j) {
+      lo[j][0] = lo[j][1] = lo[j][2] = lo[j][3] = 0.f;
+      rotate_slice<D, false>(lo[j], sm + F::OFF_ROT, A, warp + kW * j, lane);
     }
+    __syncthreads();
+    for (int i = tid; i < D * D / 8; i += kThreads) {
+      const int r = i / (D / 8), c = i % (D / 8);
+      cp_async16(sm + F::OFF_ROT + r * (2 * D) + ((c ^ (r & 7)) << 4), p.rot_h + 8 * i);
+    }
+    cp_async_wait_all();
+    __syncthreads();
+  }
+#pragma unroll(HP ? NJ : 1)
+  for (int j = 0; j < NJ; ++j) {
+    const int jt = warp + kW * j;
+    float c[4] = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (HP)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[i] = lo[j][i];
+    rotate_slice<D, true>(c, sm + F::OFF_ROT, A, jt, lane);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       if (!o_ok[r]) continue;
@@ -692,8 +780,8 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
   }
 }
 
-template <int D, int KB, int VB, int NT>
-__global__ void __launch_bounds__(32 * kW, 3) attend_few_kernel(FewParams p) {
+template <int D, int KB, int VB, int NT, bool HP>
+__global__ void __launch_bounds__(32 * kW, HP && D * NT == 256 ? 2 : 3) attend_few_kernel(FewParams p) {
   extern __shared__ __align__(128) unsigned char sm[];
   // segments in the list's order (long ones first), whoever is free next
   __shared__ int next;
@@ -704,15 +792,15 @@ __global__ void __launch_bounds__(32 * kW, 3) attend_few_kernel(FewParams p) {
     __syncthreads();
     SegWork sw;
     if (!take_segment(p.rg, next, sw)) return;
-    attend_segment<D, KB, VB, NT>(p, sw, sm);
+    attend_segment<D, KB, VB, NT, HP>(p, sw, sm);
   }
 }
 using FewFn = void (*)(FewParams);
 
-template <int D, int NT>
+template <int D, int NT, bool HP>
 FewFn few_fn(int kb, int vb, int& bytes) {
 #define TQ_FEW(K, V) \
-  if (kb == K && vb == V) { bytes = Few<D, K, V, NT>::BYTES; return attend_few_kernel<D, K, V, NT>; }
+  if (kb == K && vb == V) { bytes = Few<D, K, V, NT, HP>::BYTES; return attend_few_kernel<D, K, V, NT, HP>; }
   TQ_FEW(4, 2) TQ_FEW(4, 3) TQ_FEW(4, 4) TQ_FEW(3, 2) TQ_FEW(3, 3) TQ_FEW(3, 4)
   TQ_FEW(2, 2) TQ_FEW(2, 3) TQ_FEW(2, 4)
 #undef TQ_FEW
@@ -723,8 +811,8 @@ FewFn few_fn(int kb, int vb, int& bytes) {
 
 bool attend_few_applies(const tq_geom* G) {
   int bytes;
-  if (G->head_dim == 128) return few_fn<128, 1>(G->key_bits, G->value_bits, bytes) != nullptr;
-  if (G->head_dim == 64) return few_fn<64, 1>(G->key_bits, G->value_bits, bytes) != nullptr;
+  if (G->head_dim == 128) return few_fn<128, 1, false>(G->key_bits, G->value_bits, bytes) != nullptr;
+  if (G->head_dim == 64) return few_fn<64, 1, false>(G->key_bits, G->value_bits, bytes) != nullptr;
   return false;
 }
 
@@ -741,6 +829,7 @@ int launch_attend_few(const tq_geom* G, const tq_tables* t, const tq_cache* c,
   p.off_kn = g.off_kn;
   p.off_vn = g.off_vn;
   p.rot_h = reinterpret_cast<const __half*>(t->rot_f16);
+  p.rot = t->rot;
   p.qp = qp;
   p.qp_stride = qp_stride;
   p.kc = t->k_centroids;
@@ -762,7 +851,8 @@ int launch_attend_few(const tq_geom* G, const tq_tables* t, const tq_cache* c,
   int bytes = 0;
   auto pick = [&](auto d, auto nt) {
     constexpr int D = decltype(d)::value, NT = decltype(nt)::value;
-    fn = few_fn<D, NT>(G->key_bits, G->value_bits, bytes);
+    fn = attend_precise(a) ? few_fn<D, NT, true>(G->key_bits, G->value_bits, bytes)
+                           : few_fn<D, NT, false>(G->key_bits, G->value_bits, bytes);
   };
   using I1 = std::integral_constant<int, 1>;
   using I2 = std::integral_constant<int, 2>;
