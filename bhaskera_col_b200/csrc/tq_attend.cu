@@ -8,8 +8,8 @@
 //     L = max(kMinTiles, ceil(all key tiles / wanted CTAs)),
 // one CTA each.  The list is built on the device (the lengths live there), so
 // the host neither waits nor reads them; it launches an upper bound of CTAs.
-// Two kernels share a batch: requests of few query rows take tiles of 8 or 16
-// rows (tq_attend_few.cu), the others tiles of 128 or more, each from a list of
+// Two kernels may share a batch: requests of few query rows take tiles of 8 or 16
+// rows (tq_attend_few.cu), the others tiles of 256 (tcgen05), each from a list of
 // its own.
 #include "tq_internal.h"
 #include "tq_ragged.cuh"
@@ -318,19 +318,26 @@ struct AttendShape {
   size_t bytes;
 };
 
-// Query rows of a request and KV head up to which the few-row kernel is taken.
-constexpr int kFewRows = 64;
+// Query rows of a request and KV head up to which the few-row kernel is taken
+// where the tcgen05 kernel could be: 16 requests of 3,000-5,000 keys, D128, four
+// heads a group: 64 rows 132 us against 207, 128 rows 216 against 229, 256 rows 387
+// against 274.  Elsewhere it takes every request: the mma.sync kernel, which it
+// replaces there, is behind at any number of rows (D64: 16 rows 41 us against 234,
+// 1,024 rows 908 against 1,390; D128, fp16 results, 1,024 rows 3,397 against 4,009)
+// and runs the codes that the few-row kernel has no table for (above 4 bits).
+constexpr int kFewRows = 128;
 
 AttendShape attend_shape(const tq_geom* G, const tq_cache* c, const tq_attend_args* a) {
   AttendShape s = {};
   const int64_t R = a->batch.requests, N = a->q->shape[2], most = INT64_MAX;
   s.Hkv = c->streams / R;
   const int64_t g = a->q->shape[1] / s.Hkv;
-  // fp16 and fp32 results of many rows: the tcgen05 kernel's operands are single
-  // fp16 values (error 7e-4, against 2.1e-4 of fp16's own rounding), so mma.sync
+  // the tcgen05 kernel's operands are single fp16 values: for fp16 and fp32 results
+  // (error 7e-4, against 2.1e-4 of fp16's own rounding) only when asked for, although
+  // it is six times as fast from 1,024 rows on (562 us against 3,397)
   s.tc = prefill_tc_applies(G) && (a->engine == 2 || (a->engine == 0 && !attend_precise(a)));
   const bool can = attend_few_applies(G) && (a->engine == 0 || a->engine == 3);
-  const int64_t few_q = a->engine == 3 ? most : tmax<int64_t>(kFewRows / g, 1);
+  const int64_t few_q = s.tc ? tmax<int64_t>(kFewRows / g, 1) : most;
   size_t off = 256;                        // the first 64 bytes: the decode's status word
   auto take = [&](size_t bytes) {
     const size_t at = off;
