@@ -21,9 +21,10 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kClasses = 32;               // length classes of segments
-constexpr int kWaves = 3;                  // segments wanted per SM
-constexpr int kMinKeys = 512;              // shortest segment worth a CTA's set-up
-constexpr int kFewWaves = 5, kFewMinKeys = 512;   // the same for the few-row kernel
+// Segments wanted per SM (more even the ends, fewer save set-ups and joins) and the
+// shortest segment worth a CTA's set-up; the few-row kernel runs three CTAs a SM.
+constexpr int kWaves = 3, kMinKeys = 512;
+constexpr int kFewWaves = 5, kFewMinKeys = 512;
 
 struct PlanParams {
   RaggedView rv;

@@ -26,6 +26,12 @@
 // q' = scale log2(e) q R^T comes ready from the launch that builds the work list
 // (rotated in every segment it was most of a segment's set-up); out = O R runs on
 // the same MMAs with O split into fp16 hi + lo, once per output row.
+//
+// Bound by the loop's shared-memory wavefronts (65 % of the SM's) and latency,
+// 1.25 us a page and CTA; HBM would allow a fifth.  K4/V2, 8 KV heads of 128, g 4:
+// 252 draft tokens over 256,960 159 us, 1.3 TB/s; K3/V3, g 5: 5 tokens over
+// 131,001 140 us.  HP reads eight bytes a lookup and multiplies three times:
+// 335 and 290 us.
 #include "tq_internal.h"
 #include "tq_ragged.cuh"
 

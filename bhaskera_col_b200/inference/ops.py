@@ -430,8 +430,26 @@ def decode_attention(tables: LayerTables, pages: torch.Tensor, q: torch.Tensor,
 # ---------------------------------------------------------------------------
 # Serving operators on a flattened batch of requests
 # ---------------------------------------------------------------------------
-@dataclass
-class RopeTable:
+class _Described:
+    """A frozen dataclass of tensors with its C descriptor, made once (2 us) and
+    again when a tensor's memory has moved (``module.to()`` swaps it)."""
+
+    def _ptrs(self):
+        return tuple(x.data_ptr() for x in self._tensors())
+
+    def __post_init__(self):
+        object.__setattr__(self, "_c", self._describe())
+        object.__setattr__(self, "_at", self._ptrs())
+
+    @property
+    def c(self):
+        if self._ptrs() != self._at:
+            self.__post_init__()
+        return self._c
+
+
+@dataclass(frozen=True, eq=False)
+class RopeTable(_Described):
     """Rotary position embedding: row p of ``cos_sin`` (fp32 (positions,
     rot_dim)) holds the cosines, then the sines, of position p's rot_dim / 2
     angles.  Pair i is dims (i, rot_dim / 2 + i) of a head, or (2i, 2i + 1)
@@ -439,13 +457,16 @@ class RopeTable:
     cos_sin: torch.Tensor
     interleaved: bool = False
 
-    def __post_init__(self):
+    def _tensors(self):
+        return (self.cos_sin,)
+
+    def _describe(self):
         c = self.cos_sin
         if c.dtype != torch.float32 or c.dim() != 2 or not c.is_contiguous():
             raise ValueError("cos_sin must be a contiguous fp32 (positions, rot_dim) tensor")
         if c.shape[0] < 1 or c.shape[1] < 2 or c.shape[1] % 2:
             raise ValueError(f"cos_sin must hold a position and an even rot_dim, got {tuple(c.shape)}")
-        self._c = _lib.Rope(c.data_ptr(), c.shape[0], c.shape[1], 1 if self.interleaved else 0)
+        return _lib.Rope(c.data_ptr(), c.shape[0], c.shape[1], 1 if self.interleaved else 0)
 
     @classmethod
     def build(cls, rot_dim: int, positions: int, base: float = 10000.0, interleaved: bool = False,
@@ -465,25 +486,28 @@ class RopeTable:
         return cls((torch.cat([a.cos(), a.sin()], -1) * scale).float().contiguous(), interleaved)
 
 
-@dataclass
-class HeadNorm:
+@dataclass(frozen=True, eq=False)
+class HeadNorm(_Described):
     """RMS norm of each head vector: x / sqrt(mean(x^2) + eps) * (weight +
     offset); offset 1 for models that store weight - 1."""
     weight: torch.Tensor
     eps: float = 1e-6
     offset: float = 0.0
 
-    def __post_init__(self):
+    def _tensors(self):
+        return (self.weight,)
+
+    def _describe(self):
         w = self.weight
         if w.dim() != 1 or w.dtype not in _DT or not w.is_contiguous():
             raise ValueError("weight must be a contiguous (head_dim,) floating tensor")
         if not self.eps >= 0:
             raise ValueError(f"eps must be >= 0, got {self.eps}")
-        self._c = _lib.HeadNorm(w.data_ptr(), _DT[w.dtype], float(self.eps), float(self.offset))
+        return _lib.HeadNorm(w.data_ptr(), _DT[w.dtype], float(self.eps), float(self.offset))
 
 
-@dataclass
-class RaggedBatch:
+@dataclass(frozen=True, eq=False)
+class RaggedBatch(_Described):
     """Requests of different lengths flattened into rows (vLLM's batch): row
     q_start[r] + i is new token i of request r, at position seq_lens[r] -
     (q_start[r + 1] - q_start[r]) + i; seq_lens counts the new tokens.  Both
@@ -494,7 +518,10 @@ class RaggedBatch:
     seq_lens: torch.Tensor      # int32 (R,)
     max_q_len: int
 
-    def __post_init__(self):
+    def _tensors(self):
+        return (self.q_start, self.seq_lens)
+
+    def _describe(self):
         a, b = self.q_start, self.seq_lens
         if a.dtype != torch.int32 or b.dtype != torch.int32 or a.dim() != 1 or b.dim() != 1 or \
                 not a.is_contiguous() or not b.is_contiguous():
@@ -506,7 +533,7 @@ class RaggedBatch:
             raise ValueError("q_start and seq_lens must be on the same device")
         if self.max_q_len < 0:
             raise ValueError(f"max_q_len must be >= 0, got {self.max_q_len}")
-        self._c = _lib.Ragged(b.shape[0], a.data_ptr(), b.data_ptr(), int(self.max_q_len))
+        return _lib.Ragged(b.shape[0], a.data_ptr(), b.data_ptr(), int(self.max_q_len))
 
     @property
     def requests(self) -> int:
@@ -596,9 +623,19 @@ def _positions(pos: Optional[torch.Tensor], b: int, t: int) -> Optional[int]:
     return _desc.base + _AT_POS
 
 
-def _pages(pages) -> int:
-    if isinstance(pages, PagedPages):
-        bt, pool = pages.block_table, pages.pool
+def _pages(tables: LayerTables, pages, device: torch.device) -> int:
+    paged = isinstance(pages, PagedPages)
+    x = pages.pool if paged else pages
+    if x.device != device or tables.rot.device != device:
+        raise ValueError(f"pages on {x.device}, tables on {tables.rot.device}, heads on {device}")
+    if x.dtype != torch.uint8 or x.dim() != (2 if paged else 3) or not x.is_contiguous():
+        raise ValueError("pages must be contiguous uint8 (streams, pages, page_bytes), a pool "
+                         "(num_blocks, page_bytes)")
+    want = page_bytes(tables.head_dim, tables.key_bits, tables.value_bits, tables.qjl)
+    if x.shape[-1] != want:
+        raise ValueError(f"pages of {x.shape[-1]} bytes where the tables' take {want}")
+    if paged:
+        bt, pool = pages.block_table, x
         _CACHE.pack_into(_desc.buf, _AT_CACHE, pool.data_ptr(), bt.shape[0], bt.shape[1],
                          bt.data_ptr(), bt.stride(0), pool.shape[0])
     else:
@@ -651,9 +688,9 @@ def qk_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], rope: Optional
         k_out = torch.empty_like(k) if k_out is None else k_out
     with _on(one.device):
         _lib.check("tq_qk_rope", _lib.load().tq_qk_rope(
-            _ref(rope and rope._c), _positions(positions, b, t), _heads(_AT_Q, q, "q"),
-            _heads(_AT_QO, q_out, "q_out"), _ref(q_norm and q_norm._c), _heads(_AT_K, k, "k"),
-            _heads(_AT_KO, k_out, "k_out"), _ref(k_norm and k_norm._c), _raw_stream(one.device)))
+            _ref(rope and rope.c), _positions(positions, b, t), _heads(_AT_Q, q, "q"),
+            _heads(_AT_QO, q_out, "q_out"), _ref(q_norm and q_norm.c), _heads(_AT_K, k, "k"),
+            _heads(_AT_KO, k_out, "k_out"), _ref(k_norm and k_norm.c), _raw_stream(one.device)))
     return q_out, k_out
 
 
@@ -672,9 +709,10 @@ def append_ragged(tables: LayerTables, pages, k: torch.Tensor, v: torch.Tensor,
     _check_norm(k_norm, k.shape[-1])
     with _on(k.device):
         _lib.check("tq_append_ragged", _lib.load().tq_append_ragged(
-            ctypes.byref(tables.geom()), ctypes.byref(tables.ctables()), _pages(pages),
-            _rows(_AT_K, k, "k"), _rows(_AT_KO, v, "v"), ctypes.byref(batch._c),
-            _ref(rope and rope._c), _ref(k_norm and k_norm._c),
+            ctypes.byref(tables.geom()), ctypes.byref(tables.ctables()),
+            _pages(tables, pages, k.device),
+            _rows(_AT_K, k, "k"), _rows(_AT_KO, v, "v"), ctypes.byref(batch.c),
+            _ref(rope and rope.c), _ref(k_norm and k_norm.c),
             _positions(positions, 1, k.shape[0]), _raw_stream(k.device)))
 
 
@@ -689,8 +727,9 @@ def dequantize_ragged(tables: LayerTables, pages, batch: RaggedBatch,
     _inference_only("dequantize_ragged", one.device, k_out, v_out, batch.q_start)
     with _on(one.device):
         _lib.check("tq_dequantize_ragged", _lib.load().tq_dequantize_ragged(
-            ctypes.byref(tables.geom()), ctypes.byref(tables.ctables()), _pages(pages),
-            ctypes.byref(batch._c), _rows(_AT_K, k_out, "k_out"), _rows(_AT_KO, v_out, "v_out"),
+            ctypes.byref(tables.geom()), ctypes.byref(tables.ctables()),
+            _pages(tables, pages, one.device),
+            ctypes.byref(batch.c), _rows(_AT_K, k_out, "k_out"), _rows(_AT_KO, v_out, "v_out"),
             _raw_stream(one.device)))
 
 
@@ -704,14 +743,15 @@ def attend_ragged(tables: LayerTables, pages, q: torch.Tensor, batch: RaggedBatc
     False every row over all of them (cross attention: the pages hold an
     encoder's states, seq_lens their lengths).  A row that sees no key is
     zero.  Work is split along long contexts.  ``engine`` 0 picks the kernels
-    by each request's rows; 1 is the mma.sync kernel, 2 the tcgen05 kernel, 3
-    the kernel of few query rows.  Pass a ``workspace`` to reuse one buffer
+    by each request's rows and the type of ``out`` (fp16 and fp32 results are
+    exact to their rounding and to 2^-18); 1 is the mma.sync kernel, 2 the
+    tcgen05 kernel (error 7e-4 in any type), 3 the kernel of few query rows.  Pass a ``workspace`` to reuse one buffer
     across calls on one stream."""
     _inference_only("attend_ragged", q.device, q, out, batch.q_start)
     if out is None:
         out = torch.empty_like(q)
     lib = _lib.load()
-    g, c, bc = ctypes.byref(tables.geom()), _pages(pages), batch._c
+    g, c, bc = ctypes.byref(tables.geom()), _pages(tables, pages, q.device), batch.c
     _ATTEND.pack_into(_desc.buf, _AT_ARGS, _rows(_AT_Q, q, "q"), _rows(_AT_QO, out, "out"),
                       bc.requests, bc.q_start, bc.seq_lens, bc.max_q_len,
                       scale if scale is not None else 1.0 / math.sqrt(q.shape[-1]),

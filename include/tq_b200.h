@@ -406,8 +406,11 @@ typedef struct tq_ragged {
  * optional.  pos: rotation positions of the rows (stride[1]; NULL: each
  * token's position in its request).  A token whose position lies outside the
  * pages is dropped and sets TQ_DEV_BAD_POSITION.  Codes as tq_append's of the
- * rotated vector in fp32 (no rounding to k's type in between).  head_dim <=
- * 128, no QJL sketch. */
+ * rotated vector, not rounded to k's type in between.  Head dims 64 and 128 on
+ * 16-byte rows (and rot_dim a multiple of 16) run on the tensor cores, their
+ * codes those of exact arithmetic; other shapes on the CUDA cores in fp32, a
+ * code in about a million then one off, beside its boundary.  head_dim <= 128,
+ * no QJL sketch. */
 int32_t tq_append_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                          const tq_tensor4* k, const tq_tensor4* v, const tq_ragged* batch,
                          const tq_rope* rope, const tq_head_norm* k_norm,
@@ -434,10 +437,13 @@ typedef struct tq_attend_args {
   tq_ragged batch;
   float scale;                /* softmax scale                                */
   int32_t causal;
-  int32_t engine;             /* 0: the fastest kernels for the lengths; 1: the
-                                 mma.sync kernel; 2: the tcgen05 kernel (256
-                                 rows per CTA); 3: the kernel of 8 or 16 rows
-                                 per CTA (codes of 2 to 4 bits)               */
+  int32_t engine;             /* 0: the fastest kernels for the lengths whose
+                                 error stays below the result type's rounding;
+                                 1: the mma.sync kernel; 2: the tcgen05 kernel
+                                 (256 rows per CTA; fp16 operands, relative
+                                 error 7e-4 whatever the result's type); 3: the
+                                 kernel of 8 or 16 rows per CTA (codes of 2 to
+                                 4 bits)                                      */
 } tq_attend_args;
 
 /* 0 on bad arguments.  The workspace must be 256-byte aligned and belongs to

@@ -199,6 +199,44 @@ def test_wrapper_checks():
             ops.RaggedBatch(*a)
 
 
+def test_descriptors_follow_their_tensors():
+    """A description is frozen; memory that moved under its tensor (module.to()) is seen."""
+    w = torch.nn.Parameter(torch.ones(8))
+    norm = ops.HeadNorm(w)
+    first = norm.c.weight
+    w.data = torch.ones(8, dtype=torch.bfloat16)
+    assert norm.c.weight == w.data_ptr() != first and norm.c.dtype == _lib.TQ_BF16
+    with pytest.raises(AttributeError):
+        norm.eps = 1.0
+    batch = ops.RaggedBatch(torch.tensor([0, 3], dtype=torch.int32),
+                            torch.tensor([3], dtype=torch.int32), 3)
+    with pytest.raises(AttributeError):
+        batch.max_q_len = 4
+
+
+def tables_on(device, D=128, kb=4, vb=2):
+    z = lambda *n: torch.zeros(n, device=device)  # noqa: E731
+    return ops.LayerTables(D, kb, vb, False, z(1 << kb), z((1 << kb) - 1), z(1 << vb),
+                           z((1 << vb) - 1), z(D, D))
+
+
+def test_pages_that_do_not_fit_are_refused():
+    t, dev = tables_on("cpu"), torch.device("cpu")
+    pb = ops.page_bytes(128, 4, 2, False)
+    pages = torch.zeros((4, 2, pb), dtype=torch.uint8)
+    assert ops._pages(t, pages, dev)
+    table = torch.zeros((4, 2), dtype=torch.int32)
+    assert ops._pages(t, ops.PagedPages(pages[0], table), dev)
+    for bad in (pages[:, ::2], pages[..., :-64], pages.float(), pages[0],
+                torch.zeros((4, 2, pb + 64), dtype=torch.uint8), pages.transpose(0, 1),
+                ops.PagedPages(torch.zeros((4, pb + 64), dtype=torch.uint8), table),
+                ops.PagedPages(torch.zeros((4, 2 * pb), dtype=torch.uint8)[:, :pb], table)):
+        with pytest.raises(ValueError, match="pages"):
+            ops._pages(t, bad, dev)
+    with pytest.raises(ValueError, match="tables on"):
+        ops._pages(t, pages, torch.device("cuda", 0))
+
+
 def test_rope_table_values():
     t = ops.RopeTable.build(8, 20, base=100.0, scale=2.0, device="cpu")
     p = torch.arange(20, dtype=torch.float64)[:, None]
