@@ -20,10 +20,15 @@ namespace tq {
 namespace {
 
 constexpr int kPlanThreads = 1024;
+constexpr unsigned long long kOneTile = 1ull << 40;   // tiles counted above their key tiles
 constexpr int kClasses = 32;               // length classes of segments
 // Segments wanted per SM (more even the ends, fewer save set-ups and joins) and the
-// shortest segment worth a CTA's set-up; the few-row kernel runs three CTAs a SM.
-constexpr int kWaves = 3, kMinKeys = 512;
+// shortest segment worth a CTA's set-up, in keys.  Wide list, 8,899 rows of prompt
+// chunks: 605 us with 2 a SM, 611 with 1, 660 with 3, 720 with 5.  Few-row list
+// (three CTAs a SM): 131,001 keys 142 us with 5 a SM, 172 with 3, 157 with 8; 64
+// requests' drafts 163, 166, 168.  Shortest: one request of 2,000 keys 35 us with 512,
+// 33 with 256, 43 with 1,024; 64 of 1,000 keys 46, 57, 47.
+constexpr int kWaves = 2, kMinKeys = 512;
 constexpr int kFewWaves = 5, kFewMinKeys = 512;
 
 struct PlanParams {
@@ -244,13 +249,16 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p0
   if (tid <= kClasses) place[tid] = 0;
   __syncthreads();
   unsigned long long mine = 0;
-  for_tiles(p, [&](int, int, int nkt) { mine += nkt; });
+  for_tiles(p, [&](int, int, int nkt) { mine += nkt + kOneTile; });
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
   if (lane == 0) atomicAdd(&all, mine);
   __syncthreads();
-  const unsigned long long total = all * (unsigned)p.G;
-  const int L = (int)tmax<unsigned long long>(p.min_tiles, (total + p.wanted - 1) / p.wanted);
+  const unsigned long long total = (all & (kOneTile - 1)) * (unsigned)p.G;
+  // tiles that fill half of the wanted CTAs by themselves need no short segments
+  // (16 batches of encoder states, 304 rows: 36.7 us, with them 41.2)
+  const int least = (all / kOneTile) * (unsigned)p.G * 2 >= p.wanted ? 2 * p.min_tiles : p.min_tiles;
+  const int L = (int)tmax<unsigned long long>(least, (total + p.wanted - 1) / p.wanted);
   // class of a segment of n key tiles: 0 the longest (L), 31 the shortest
   auto class_of = [&](int n) { return kClasses - 1 - (int)((unsigned)(n * kClasses - 1) / (unsigned)L); };
   for_tiles(p, [&](int, int, int nkt) {

@@ -412,8 +412,8 @@ __device__ __forceinline__ float sum_lanes(float x) {
 
 // The run's codes in 64 bits, a coordinate per lane; xs: D doubles of the warp's.
 template <int D, int BITS>
-__device__ __forceinline__ void exact_run(const RaggedTc& p, int which, const float* weight,
-                                          const float* bnd, const Again& e, double* xs) {
+__device__ __forceinline__ void exact_run(const RaggedTc& p, int which, const float* bnd,
+                                          const Again& e, double* xs) {
   constexpr int nb = (1 << BITS) - 1;
   const int lane = threadIdx.x & 31;
   const HeadXform& f = p.f;
@@ -423,21 +423,23 @@ __device__ __forceinline__ void exact_run(const RaggedTc& p, int which, const fl
   const int n = p.by_h.div(e.i);
   const int64_t base = (int64_t)n * st[1] + (int64_t)(e.i - n * p.H) * st[0];
   const float* cs = f.cos_sin + (int64_t)(e.row & 0x3FFFFFFFu) * rot;
+  auto value = [&](int d) {
+    const double x = load_elem(p.x[which], p.dtype[which], base + d);
+    return norm ? x * ((double)load_elem(f.weight, f.w_dtype, d) + f.w_offset) : x;
+  };
   // the sums before the rotation (the head norm's) and of what it gives
   double raw = 0.0, ss = 0.0;
 #pragma unroll
   for (int k = 0; k < D / 32; ++k) {
     const int d = lane + 32 * k;
-    double x = load_elem(p.x[which], p.dtype[which], base + d);
-    raw += x * x;
-    if (norm) x *= weight[d];
+    const double own = load_elem(p.x[which], p.dtype[which], base + d);
+    raw += own * own;
+    double x = value(d);
     if (d < rot) {
       const int a = f.interleaved ? d >> 1 : d < half ? d : d - half;    // angle
       const bool second = f.interleaved ? d & 1 : d >= half;
       const int with = f.interleaved ? d ^ 1 : second ? d - half : d + half;
-      double z = load_elem(p.x[which], p.dtype[which], base + with);
-      if (norm) z *= weight[with];
-      x = x * cs[a] + z * (second ? cs[half + a] : -cs[half + a]);
+      x = x * cs[a] + value(with) * (second ? cs[half + a] : -cs[half + a]);
     }
     ss += x * x;
     xs[d] = x;
@@ -856,7 +858,7 @@ append_ragged_tc_kernel(const __grid_constant__ RaggedTc p, int which) {
   double* xs = reinterpret_cast<double*>(sm + SM::OFF_A) + D * warp;
   for (int w = 0, k = warp; w < W::kEpi; ++w) {
     for (; k < nagain[w]; k += kThreads / 32)
-      exact_run<D, BITS>(p, which, weight, bnd, again[kAgain * w + k], xs);
+      exact_run<D, BITS>(p, which, bnd, again[kAgain * w + k], xs);
     k -= nagain[w];
   }
   pdl_wait();

@@ -405,7 +405,9 @@ typedef struct tq_ragged {
  * their tokens, k normed (k_norm) and rotated (rope) on the way, both
  * optional.  pos: rotation positions of the rows (stride[1]; NULL: each
  * token's position in its request).  A token whose position lies outside the
- * pages is dropped and sets TQ_DEV_BAD_POSITION.  Codes as tq_append's of the
+ * pages is dropped and sets TQ_DEV_BAD_POSITION.  No two tokens of a call may
+ * share a place (two requests may share pages that neither writes); what is
+ * stored there would be a mix of both.  Codes as tq_append's of the
  * rotated vector, not rounded to k's type in between.  Head dims 64 and 128 on
  * 16-byte rows (and rot_dim a multiple of 16) run on the tensor cores, their
  * codes those of exact arithmetic; other shapes on the CUDA cores in fp32, a

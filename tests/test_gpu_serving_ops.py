@@ -735,12 +735,12 @@ def test_append_ragged_codes_are_those_of_exact_arithmetic(D, kb, vb, dtype, pai
     rope = None if pairs == "none" else \
         ops.RopeTable.build(D // 2 if pairs == "part" else D, n,
                             interleaved=pairs == "interleaved", device=DEV)
-    w = ops.HeadNorm(1 + 0.2 * randn((D,), 23, F32), 1e-6) if norm else None
+    w = ops.HeadNorm(0.2 * randn((D,), 23, F32), 1e-6, 1.0) if norm else None
     ops.append_ragged(tables, pages, k, v, batch, rope=rope, k_norm=w)
     got = S.parse(tables, contiguous(pages), max(seq))
     r, pos = S.positions(start, seq, n)
     kx = S.rope(k, rope.cos_sin if rope else None, pos, pairs == "interleaved",
-                w.weight if w else None, 1e-6)
+                w.weight if w else None, 1e-6, 1.0)
     R = tables.rot.double().cpu().numpy()
     for name, x, bnd in (("k_idx", kx, tables.k_boundaries), ("v_idx", v, tables.v_boundaries)):
         x = np.asarray(x.double().cpu().numpy() if torch.is_tensor(x) else x, dtype=np.float64)
