@@ -69,12 +69,13 @@ __device__ __forceinline__ int key_tiles(const PlanParams& p, const Tiles& t, in
 }
 
 // f(request, tile, key tiles) for every tile: a thread per request, a warp
-// for a request of more than 32 tiles.
+// for a request of more than 32 tiles.  `own`: this thread's first request, read
+// once for all passes.
 template <class F>
-__device__ __forceinline__ void for_tiles(const PlanParams& p, F f) {
+__device__ __forceinline__ void for_tiles(const PlanParams& p, const Tiles& own, F f) {
   const int tid = threadIdx.x, lane = tid & 31;
   for (int64_t r0 = 0; r0 < p.rv.R; r0 += kPlanThreads) {
-    const Tiles t = listed_request(p, r0 + tid);
+    const Tiles t = r0 == 0 ? own : listed_request(p, r0 + tid);
     if (t.tiles <= 32)
       for (int i = 0; i < t.tiles; ++i) f((int)(r0 + tid), i, key_tiles(p, t, i));
     for (unsigned big = __ballot_sync(0xffffffffu, t.tiles > 32); big; big &= big - 1) {
@@ -240,6 +241,7 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p0
   __shared__ unsigned place[kClasses + 1];                 // segments per class, then their next place
   __shared__ unsigned slots;
   const int tid = threadIdx.x, lane = tid & 31;
+  const Tiles own = listed_request(p, tid);
   for (int i = tid; i < p.max_slot * p.G; i += kPlanThreads) p.arrived[i] = 0;
   if (tid == 0) {
     all = 0;
@@ -249,7 +251,7 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p0
   if (tid <= kClasses) place[tid] = 0;
   __syncthreads();
   unsigned long long mine = 0;
-  for_tiles(p, [&](int, int, int nkt) { mine += nkt + kOneTile; });
+  for_tiles(p, own, [&](int, int, int nkt) { mine += nkt + kOneTile; });
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
   if (lane == 0) atomicAdd(&all, mine);
@@ -261,7 +263,7 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p0
   const int L = (int)tmax<unsigned long long>(least, (total + p.wanted - 1) / p.wanted);
   // class of a segment of n key tiles: 0 the longest (L), 31 the shortest
   auto class_of = [&](int n) { return kClasses - 1 - (int)((unsigned)(n * kClasses - 1) / (unsigned)L); };
-  for_tiles(p, [&](int, int, int nkt) {
+  for_tiles(p, own, [&](int, int, int nkt) {
     const int ns = nkt > L ? (nkt + L - 1) / L : 1;
     atomicAdd(&place[class_of(tmax(1, (nkt + ns - 1) / ns))], (unsigned)ns);
     if (ns > 1) atomicAdd(&slots, (unsigned)ns);
@@ -288,7 +290,7 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p0
   }
   __syncthreads();
   if (!place[kClasses]) return;
-  for_tiles(p, [&](int r, int i, int nkt) {
+  for_tiles(p, own, [&](int r, int i, int nkt) {
     const int ns = nkt > L ? (nkt + L - 1) / L : 1;
     const int base = nkt / ns, more = nkt - base * ns;     // `more` segments take one tile extra
     const unsigned at = atomicAdd(&place[class_of(tmax(1, (nkt + ns - 1) / ns))], (unsigned)ns);

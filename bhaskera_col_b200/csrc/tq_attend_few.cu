@@ -288,10 +288,17 @@ __device__ __forceinline__ void fill_table(unsigned char* table, const float* ce
   }
 }
 
+template <int D, int KB, int VB, int NT, bool HP>
+__device__ __forceinline__ void fill_tables(const FewParams& p, unsigned char* sm) {
+  using F = Few<D, KB, VB, NT, HP>;
+  fill_table<KB, F::KQ, HP>(sm, p.kc, threadIdx.x, 32 * kW);
+  fill_table<VB, F::VQ, HP>(sm + F::KT, p.vc, threadIdx.x, 32 * kW);
+}
+
 // One segment of the work list.
 template <int D, int KB, int VB, int NT, bool HP>
 __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork& sw,
-                                               unsigned char* sm) {
+                                               unsigned char* sm, bool filled) {
   using F = Few<D, KB, VB, NT, HP>;
   using Tile = FewTile<D, KB, VB>;
   constexpr int NQ = F::NQ, NC = D / 16, kThreads = 32 * kW, LDA = F::LDA, LDO = F::LDO;
@@ -385,8 +392,7 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
       else
         *reinterpret_cast<uint4*>(dst) = make_uint4(0u, 0u, 0u, 0u);
     }
-  fill_table<KB, F::KQ, HP>(sm, p.kc, tid, kThreads);
-  fill_table<VB, F::VQ, HP>(sm + F::KT, p.vc, tid, kThreads);
+  if (!filled) fill_tables<D, KB, VB, NT, HP>(p, sm);
   cp_async_wait_all();
   __syncthreads();
 
@@ -791,14 +797,16 @@ __global__ void __launch_bounds__(32 * kW, HP && D * NT == 256 ? 2 : 3) attend_f
   extern __shared__ __align__(128) unsigned char sm[];
   // segments in the list's order (long ones first), whoever is free next
   __shared__ int next;
+  bool filled = true;
+  fill_tables<D, KB, VB, NT, HP>(p, sm);                   // beside the launch before
   pdl_wait();                                              // the list and q'
-  while (true) {
+  for (;; filled = false) {
     __syncthreads();                                       // the last segment is done with
     if (threadIdx.x == 0) next = atomicAdd(p.rg.plan.next, 1);
     __syncthreads();
     SegWork sw;
     if (!take_segment(p.rg, next, sw)) return;
-    attend_segment<D, KB, VB, NT, HP>(p, sw, sm);
+    attend_segment<D, KB, VB, NT, HP>(p, sw, sm, filled);
   }
 }
 using FewFn = void (*)(FewParams);
