@@ -470,7 +470,14 @@ size_t tq_prefill_workspace_bytes(const tq_geom* g, const tq_cache* c, const tq_
 // ---------------------------------------------------------------------------
 // check_t4 for tensors that may have no rows (and then no memory).
 static int check_maybe_empty(const tq_tensor4* x, const char* what, const char* fn) {
-  if (!x || x->data) return check_t4(x, what, fn);
+  if (!x || x->data) {
+    if (int rc = check_t4(x, what, fn)) return rc;
+    if (reinterpret_cast<uintptr_t>(x->data) % (x->dtype == TQ_F32 ? 4 : 2)) {
+      set_error("%s: %s is not aligned to its elements", fn, what);
+      return TQ_ERR_INVALID;
+    }
+    return TQ_OK;
+  }
   tq_tensor4 some = *x;
   bool empty = false;
   for (int i = 0; i < 4; ++i) empty = empty || x->shape[i] == 0;
@@ -545,7 +552,7 @@ static void extent(const tq_tensor4* x, const char*& lo, const char*& hi) {
 
 // y may be x itself, else they must not overlap.
 static int check_alias(const tq_tensor4* x, const tq_tensor4* y, const char* what, const char* fn) {
-  bool same = x->data == y->data;
+  bool same = x->data == y->data && x->dtype == y->dtype;
   for (int i = 0; i < 4; ++i) {
     if (x->shape[i] == 0) return TQ_OK;
     same = same && (x->shape[i] == 1 || x->stride[i] == y->stride[i]);
@@ -712,7 +719,12 @@ static int check_attend(const tq_geom* g, const tq_cache* c, const tq_attend_arg
               (long long)Hkv);
     return TQ_ERR_INVALID;
   }
-  if ((rc = check_flat(a->q, "q", Hq, g, fn))) return rc;
+  if ((rc = check_flat(a->q, "q", Hq, g, fn)) || (rc = check_flat(a->out, "out", Hq, g, fn)))
+    return rc;
+  if (a->out->shape[2] != a->q->shape[2]) {
+    set_error("%s: q and out differ in rows", fn);
+    return TQ_ERR_INVALID;
+  }
   if (a->engine < 0 || a->engine > 3) {
     set_error("%s: engine must be 0 (fastest), 1 (mma.sync), 2 (tcgen05) or 3 (few rows), got %d",
               fn, a->engine);
@@ -720,7 +732,7 @@ static int check_attend(const tq_geom* g, const tq_cache* c, const tq_attend_arg
   }
   const bool tc = prefill_tc_applies(g);
   const bool mma = prefill_supported(g->head_dim, g->key_bits, g->value_bits);
-  if (a->engine == 0 ? !mma && !tc
+  if (a->engine == 0 ? !mma && !tc && !attend_few_applies(g)
       : a->engine == 1 ? !mma
       : a->engine == 2 ? !tc : !attend_few_applies(g)) {
     set_error("%s: no kernel for head_dim %d, key_bits %d, value_bits %d (engine %d)", fn,
@@ -752,13 +764,8 @@ int32_t tq_attend_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c
   const char* fn = "tq_attend_ragged";
   int rc;
   if ((rc = check_attend(g, c, a, fn)) || (rc = check_tables(g, t, fn))) return rc;
-  if ((rc = check_flat(a->out, "out", a->q->shape[1], g, fn)) ||
-      (rc = check_written(a->out, "out", fn)))
+  if ((rc = check_written(a->out, "out", fn)) || (rc = check_alias(a->q, a->out, "out", fn)))
     return rc;
-  if (a->out->shape[2] != a->q->shape[2]) {
-    set_error("%s: q and out differ in rows", fn);
-    return TQ_ERR_INVALID;
-  }
   if (!t->rot_f16 || reinterpret_cast<uintptr_t>(t->rot_f16) % 16) {
     set_error("%s: tables.rot_f16 (R as fp16, 16-byte aligned) is required", fn);
     return TQ_ERR_INVALID;

@@ -68,7 +68,7 @@ class VLLMBatch:
     query_start_loc_cpu: Optional[List[int]] = None
     seq_lens_cpu: Optional[List[int]] = None
     _ragged: Optional[ops.RaggedBatch] = None
-    _positions: Optional[torch.Tensor] = None
+    _positions: Optional[tuple] = None
 
     def ragged(self) -> ops.RaggedBatch:
         """The batch as the ragged operators take it (one per step, shared by
@@ -80,13 +80,23 @@ class VLLMBatch:
 
     def positions(self) -> torch.Tensor:
         """int64 (num_actual_tokens,): each token's position in its request,
-        computed on the device once per step."""
-        if self._positions is None:
-            start = self.query_start_loc.long()
-            base = torch.repeat_interleave(self.seq_lens.long() - start[1:], start.diff(),
-                                           output_size=self.num_actual_tokens)
-            self._positions = base + torch.arange(self.num_actual_tokens, device=start.device)
-        return self._positions
+        computed on the device.  The layers of a step share it, as long as the
+        versions of the offsets and lengths show them unchanged: not while a
+        graph is captured, whose replays have lengths of their own, nor for
+        inference tensors, which keep no version."""
+        ts = (self.query_start_loc, self.seq_lens)
+        fresh = any(t.is_inference() for t in ts) or (
+            ts[0].is_cuda and torch.cuda.is_current_stream_capturing())
+        of = None if fresh else (*((t.data_ptr(), t._version) for t in ts), self.num_actual_tokens)
+        if not fresh and self._positions is not None and self._positions[0] == of:
+            return self._positions[1]
+        start = self.query_start_loc.long()
+        base = torch.repeat_interleave(self.seq_lens.long() - start[1:], start.diff(),
+                                       output_size=self.num_actual_tokens)
+        at = base + torch.arange(self.num_actual_tokens, device=start.device)
+        if not fresh:
+            self._positions = (of, at)
+        return at
 
     @classmethod
     def from_metadata(cls, md) -> "VLLMBatch":

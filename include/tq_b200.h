@@ -435,7 +435,8 @@ int32_t tq_dequantize_ragged(const tq_geom* g, const tq_tables* t, const tq_cach
  * finite makes NaN of the rows that attend its token and of no other. */
 typedef struct tq_attend_args {
   const tq_tensor4* q;        /* (1, Hq, N, D)                                */
-  const tq_tensor4* out;
+  const tq_tensor4* out;      /* may be q (same view), else it must not overlap
+                                 it; its type may differ from q's              */
   tq_ragged batch;
   float scale;                /* softmax scale                                */
   int32_t causal;

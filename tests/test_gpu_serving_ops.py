@@ -751,3 +751,82 @@ def test_append_ragged_codes_are_those_of_exact_arithmetic(D, kb, vb, dtype, pai
         have = got[name].reshape(2, H, -1, D)[r, :, pos]
         assert not ((have != at) & (gap > 1e-12)).any()
     assert ok_status() == 0
+
+
+@pytest.mark.parametrize("engine", [0, 1, 3])
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("D,kb,vb,Hq,H", [(128, 4, 2, 8, 2), (128, 3, 3, 20, 1), (64, 2, 2, 4, 4),
+                                          (64, 3, 4, 6, 2), (64, 6, 6, 4, 2), (128, 2, 4, 6, 2)])
+def test_attend_ragged_fp16_and_fp32_results_are_exact_to_their_type(D, kb, vb, Hq, H, dtype, engine):
+    """Operands of 22 bits: a score is off by at most 2^-20 |scale q k| (three products of two
+    values that are each off by 2^-22, and the sums), so is its exponential, relatively; P and V add
+    3 x 2^-22 and the sums of fp32 less than 2^-18."""
+    codes = (kb, vb)
+    if engine == 3 and max(codes) > 4 or engine == 1 and codes in ((3, 4), (2, 4)):
+        pytest.skip("no such kernel")
+    tables = make_tables(D, kb, vb, False)
+    lens = [(3, 700), (200, 300), (1, 1), (2, 0), (40, 1500)]
+    batch, start, seq = make_batch(lens)
+    pages = make_paged(tables, len(lens) * H, 1500)
+    fill(tables, pages, len(lens), H, pages.shape[1] * 64, 31)
+    kd, vd = (x.reshape(len(lens), H, -1, D) for x in S.dense(tables, contiguous(pages), pages.shape[1] * 64))
+    q = randn((start[-1], Hq, D), 32, dtype)
+    want = S.attend(q, kd, vd, start, seq, D ** -0.5, True)
+    got = ops.attend_ragged(tables, pages, q, batch, engine=engine).double().cpu().numpy()
+    most = D ** -0.5 * np.linalg.norm(q.double().cpu().numpy(), axis=-1).max() * \
+        np.linalg.norm(kd, axis=-1).max()
+    top = np.abs(vd).max()
+    tol = (2 * most * 2.0 ** -20 + 2.0 ** -18) * top
+    assert (np.abs(got - want) <= tol + S.half_ulp(dtype) * np.abs(want) + 2.0 ** -25).all()
+    out = q.clone()                                       # in place
+    ops.attend_ragged(tables, pages, out, batch, out=out, engine=engine)
+    assert np.array_equal(out.double().cpu().numpy(), got)
+    assert ok_status() == 0
+
+
+@pytest.mark.parametrize("engine", [1, 2, 3])
+def test_attend_ragged_in_place(engine):
+    """out may be q: every CTA of a cut tile has read its queries before the last one writes."""
+    tables = make_tables(128, 4, 2, False)
+    lens = [(5, 4000), (150, 3000), (1, 64)]
+    batch, start, seq = make_batch(lens)
+    pages = make_paged(tables, len(lens) * 2, 4000)
+    fill(tables, pages, len(lens), 2, pages.shape[1] * 64, 33)
+    q = randn((start[-1], 8, 128), 34, BF16)
+    want = ops.attend_ragged(tables, pages, q, batch, engine=engine)
+    for _ in range(5):
+        out = q.clone()
+        ops.attend_ragged(tables, pages, out, batch, out=out, engine=engine)
+        assert torch.equal(out, want)
+    assert ok_status() == 0
+
+
+def test_paged_attention_layer_with_rope_replays_with_new_lengths():
+    """A captured forward of a batch that an eager one has used takes its positions from the
+    lengths at replay."""
+    from bhaskera_col_b200.inference.vllm_turboquant import TurboQuantPagedAttention, VLLMBatch
+    D, Hq, H, R = 128, 4, 2, 3
+    rope = ops.RopeTable.build(D, 300, device=DEV)
+    q, k, v = (randn((R, h, D), 41 + j, BF16) for j, h in enumerate((Hq, H, H)))
+    table = torch.arange(2 * R, dtype=torch.int32, device=DEV).view(R, 2)
+    outs = []
+    for graph in (False, True):
+        layer = TurboQuantPagedAttention(5, 32, Hq, H, D, num_blocks=2 * R, block_size=64,
+                                         key_bits=4, value_bits=2, device=DEV)
+        batch = VLLMBatch(int32([0, 1, 2, 3]), int32([10, 64, 1]), table, R, 1)
+        out = torch.empty_like(q)
+        layer.forward(q, k, v, batch, out=out, rope=rope)
+        first = out.clone()
+        if graph:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                layer.forward(q, k, v, batch, out=out, rope=rope)
+        batch.seq_lens.add_(1)
+        if graph:
+            g.replay()
+        else:
+            layer.forward(q, k, v, batch, out=out, rope=rope)
+        outs.append((first, out.clone(), layer.pool.clone()))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    assert ok_status() == 0

@@ -59,6 +59,8 @@ X = (1, 4, 7, 128)
     (dict(qn=NORM, q=t4(X), qo=t4(X, data=(1 << 20) + 256)), "overlaps"),
     (dict(qn=NORM, q=t4(X), qo=t4(X, stride=[0, 128, 512, 1])), "overlaps"),
     (dict(qn=NORM, q=t4(X, data=None), qo=far(X)), "NULL"),
+    (dict(qn=NORM, q=t4(X, data=4097), qo=far(X)), "aligned"),
+    (dict(qn=NORM, q=t4(X, dtype=_lib.TQ_F32, data=4098), qo=far(X, dtype=_lib.TQ_F32)), "aligned"),
 ])
 def test_qk_rope_refusals(kw, what):
     rc, err = rope_call(**kw)
@@ -147,14 +149,27 @@ def attend(g=None, c=CACHE, q=t4((1, 4, 10, 128)), out=None, batch=BATCH, scale=
     (dict(batch=_lib.Ragged(5, 4096, 4096, 1)), "multiple"),
     (dict(q=t4((1, 2048, 1, 128))), "1024 query heads"),
     (dict(c=_lib.Cache(1 << 20, 6, 1 << 27)), "32 bits"),
+    (dict(out=far((1, 4, 9, 128))), "differ in rows"),
+    (dict(out=far((1, 2, 10, 128))), "must be"),
 ])
 def test_attend_refusals(kw, what):
     rc, err, need = attend(**kw)
     assert rc == _lib.TQ_ERR_INVALID and need == 0 and what in err, err
 
 
+def test_attend_workspace_query_without_tensors():
+    lib = _lib.load()
+    q, g = t4((1, 4, 10, 128)), geom()
+    for a in (_lib.AttendArgs(None, ctypes.pointer(q), BATCH, 0.1, 1, 0),
+              _lib.AttendArgs(ctypes.pointer(q), None, BATCH, 0.1, 1, 0)):
+        assert lib.tq_attend_ragged_workspace_bytes(ctypes.byref(g), ctypes.byref(CACHE),
+                                                    ctypes.byref(a)) == 0
+        assert "NULL" in _lib.last_error()
+
+
 def test_attend_refusals_of_the_call_alone():
-    for kw, what in ((dict(out=far((1, 4, 9, 128))), "differ in rows"),
+    for kw, what in ((dict(out=t4((1, 4, 10, 128), data=(1 << 20) + 256)), "overlaps"),
+                     (dict(out=t4((1, 4, 10, 128), dtype=_lib.TQ_F32)), "overlaps"),
                      (dict(out=t4((1, 4, 10, 128), stride=[0, 0, 128, 1])), "share memory"),
                      (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"),
                      (dict(t=_lib.Tables(*([4096] * 9))), "rot_f16")):
@@ -235,6 +250,22 @@ def test_pages_that_do_not_fit_are_refused():
             ops._pages(t, bad, dev)
     with pytest.raises(ValueError, match="tables on"):
         ops._pages(t, pages, torch.device("cuda", 0))
+
+
+def test_positions_follow_the_batch():
+    """A batch's positions are computed once, and again when its lengths change in place."""
+    from bhaskera_col_b200.inference.vllm_turboquant import VLLMBatch
+    i = lambda *v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    b = VLLMBatch(i(0, 2, 2, 5), i(7, 4, 3), torch.zeros((3, 1), dtype=torch.int32), 5, 3)
+    assert b.positions().tolist() == [5, 6, 0, 1, 2]
+    assert b.positions() is b.positions()
+    b.seq_lens.add_(10)
+    assert b.positions().tolist() == [15, 16, 10, 11, 12]
+    with torch.inference_mode():
+        c = VLLMBatch(i(0, 2, 2, 5), i(7, 4, 3), b.block_table, 5, 3)
+        assert c.positions().tolist() == [5, 6, 0, 1, 2]
+        c.seq_lens.add_(1)
+        assert c.positions().tolist() == [6, 7, 1, 2, 3]
 
 
 def test_rope_table_values():
