@@ -29,8 +29,8 @@
 //
 // Bound by the loop's shared-memory wavefronts (65 % of the SM's) and latency,
 // 1.25 us a page and CTA; HBM would allow a fifth.  K4/V2, 8 KV heads of 128, g 4:
-// 252 draft tokens over 256,960 159 us, 1.3 TB/s; K3/V3, g 5: 5 tokens over
-// 131,001 140 us.  HP reads eight bytes a lookup and multiplies three times:
+// 252 draft tokens over 256,960 156 us, 1.3 TB/s; K3/V3, g 5: 5 tokens over
+// 131,001 142 us.  HP reads eight bytes a lookup and multiplies three times:
 // 335 and 290 us.
 #include "tq_internal.h"
 #include "tq_ragged.cuh"

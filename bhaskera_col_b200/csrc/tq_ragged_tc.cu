@@ -61,8 +61,8 @@ constexpr float kRScale = 64.f;
 // Append: a coordinate of the unit vector R x / ||x|| this near to a boundary is
 // computed again in 64 bits, so that the codes are those of exact arithmetic.
 // The operands' 22 bits and the sums' rounding leave the first value a few 1e-8
-// off (one code in 600,000 came out wrong); 5e-7 is over ten times that, and one
-// coordinate in 60,000 (128 dims, 4 bits).
+// off (one code in 600,000 came out wrong); 3e-7 is several times that and takes
+// one coordinate in 50,000 (128 dims, 4 bits).
 constexpr float kNear = 3e-7f;
 
 // i / d for 0 <= i < 2^31 as a product: m = ceil(2^(31 + s) / d), 2^s >= d.
@@ -368,8 +368,11 @@ struct Again {
   int i;                                   // vector
   uint32_t row;                            // of the rotation table; run of the vector in bits 30, 31
 };
-// Noted per epilogue warp, in the warp's order, and left as they are past that:
-// at one run in 2,000 the 8 warps' lists last for 60,000 vectors of 128 per SM.
+// Noted per epilogue warp, in the warp's order; runs past that keep their first
+// values.  At one run in 1,600 the 8 warps' lists last for 100,000 vectors of 128
+// per SM and launch, 15 million in all.  (Redone at once in the epilogue, a run's
+// cold code held up its warp: whole prompts 125 us against 107; by the locators
+// between their tiles, it held up the tiles: 138 us.)
 constexpr int kAgain = 32;
 
 template <int D>

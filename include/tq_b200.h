@@ -410,8 +410,9 @@ typedef struct tq_ragged {
  * stored there would be a mix of both.  Codes as tq_append's of the
  * rotated vector, not rounded to k's type in between.  Head dims 64 and 128 on
  * 16-byte rows (and rot_dim a multiple of 16) run on the tensor cores, their
- * codes those of exact arithmetic; other shapes on the CUDA cores in fp32, a
- * code in about a million then one off, beside its boundary.  head_dim <= 128,
+ * codes those of exact arithmetic (for some 10^7 vectors a call; behind them,
+ * and in other shapes, which run on the CUDA cores, those of fp32: a code in
+ * about a million is one off, beside its boundary).  head_dim <= 128,
  * no QJL sketch. */
 int32_t tq_append_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                          const tq_tensor4* k, const tq_tensor4* v, const tq_ragged* batch,
