@@ -72,11 +72,13 @@ class VLLMBatch:
 
     def ragged(self) -> ops.RaggedBatch:
         """The batch as the ragged operators take it (one per step, shared by
-        the layers)."""
-        if self._ragged is None:
-            self._ragged = ops.RaggedBatch(self.query_start_loc, self.seq_lens,
-                                           self.max_query_len)
-        return self._ragged
+        the layers; a new one once a field has been replaced)."""
+        b = self._ragged
+        if b is None or b.q_start is not self.query_start_loc or \
+                b.seq_lens is not self.seq_lens or b.max_q_len != self.max_query_len:
+            b = self._ragged = ops.RaggedBatch(self.query_start_loc, self.seq_lens,
+                                               self.max_query_len)
+        return b
 
     def positions(self) -> torch.Tensor:
         """int64 (num_actual_tokens,): each token's position in its request,

@@ -320,3 +320,22 @@ def test_attention_work_list_fits_its_bounds():
         for n, k in zip(tiles, ns):                        # parts cover the tile, none above L
             base, more = divmod(n, k)
             assert base + (more > 0) <= L
+
+
+def vllm_batch(start, seq, n, most):
+    from bhaskera_col_b200.inference.vllm_turboquant import VLLMBatch
+    i = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    return VLLMBatch(i(start), i(seq), torch.zeros((len(seq), 1), dtype=torch.int32), n, most)
+
+
+def test_ragged_batch_follows_replaced_fields():
+    """A step that replaces the batch's offsets, lengths or bound is described by the new ones."""
+    b = vllm_batch([0, 2, 5], [7, 3], 5, 3)
+    first = b.ragged()
+    assert b.ragged() is first                             # one description for the layers of a step
+    b.seq_lens = b.seq_lens + 1
+    assert b.ragged().seq_lens is b.seq_lens and b.ragged().q_start is first.q_start
+    b.query_start_loc = b.query_start_loc.clone()
+    assert b.ragged().q_start is b.query_start_loc
+    b.max_query_len = 9
+    assert b.ragged().max_q_len == 9 and b.ragged().seq_lens is b.seq_lens
