@@ -82,20 +82,23 @@ class VLLMBatch:
 
     def positions(self) -> torch.Tensor:
         """int64 (num_actual_tokens,): each token's position in its request,
-        computed on the device.  The layers of a step share it, as long as the
-        versions of the offsets and lengths show them unchanged: not while a
-        graph is captured, whose replays have lengths of their own, nor for
-        inference tensors, which keep no version."""
+        computed on the device; 0 for rows of no request (padding) and for
+        tokens before their request's start.  The layers of a step share it, as
+        long as the versions of the offsets and lengths show them unchanged: not
+        while a graph is captured, whose replays have lengths of their own, nor
+        for inference tensors, which keep no version."""
         ts = (self.query_start_loc, self.seq_lens)
         fresh = any(t.is_inference() for t in ts) or (
             ts[0].is_cuda and torch.cuda.is_current_stream_capturing())
         of = None if fresh else (*((t.data_ptr(), t._version) for t in ts), self.num_actual_tokens)
         if not fresh and self._positions is not None and self._positions[0] == of:
             return self._positions[1]
-        start = self.query_start_loc.long()
-        base = torch.repeat_interleave(self.seq_lens.long() - start[1:], start.diff(),
-                                       output_size=self.num_actual_tokens)
-        at = base + torch.arange(self.num_actual_tokens, device=start.device)
+        start = self.query_start_loc
+        row = torch.arange(self.num_actual_tokens, dtype=start.dtype, device=start.device)
+        # request r's rows are in interval r + 1 of the offsets; intervals 0 and
+        # R + 1 lie outside the batch: far below 0
+        first = torch.nn.functional.pad((self.seq_lens - start[1:]).long(), (1, 1), value=-2 ** 40)
+        at = (first[torch.searchsorted(start, row, right=True)] + row).clamp_(min=0)
         if not fresh:
             self._positions = (of, at)
         return at

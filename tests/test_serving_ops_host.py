@@ -339,3 +339,13 @@ def test_ragged_batch_follows_replaced_fields():
     assert b.ragged().q_start is b.query_start_loc
     b.max_query_len = 9
     assert b.ragged().max_q_len == 9 and b.ragged().seq_lens is b.seq_lens
+
+
+def test_positions_of_a_padded_batch():
+    """Rows before the first request and behind the last (padding of a captured batch) are at 0, and
+    so are tokens that lie before their request's start; requests without rows take no part."""
+    assert vllm_batch([0, 2, 2, 3], [7, 4, 1], 6, 2).positions().tolist() == [5, 6, 0, 0, 0, 0]
+    assert vllm_batch([2, 4, 5], [9, 3], 7, 2).positions().tolist() == [0, 0, 7, 8, 2, 0, 0]
+    assert vllm_batch([0, 3], [1], 3, 3).positions().tolist() == [0, 0, 0]
+    assert vllm_batch([0, 0], [5], 2, 0).positions().tolist() == [0, 0]
+    assert vllm_batch([0, 2, 5], [7, 3], 5, 3).positions().dtype == torch.int64
