@@ -68,7 +68,7 @@ class VLLMBatch:
     query_start_loc_cpu: Optional[List[int]] = None
     seq_lens_cpu: Optional[List[int]] = None
     _ragged: Optional[ops.RaggedBatch] = None
-    _positions: Optional[tuple] = None
+    _positions: Optional[torch.Tensor] = None
 
     def ragged(self) -> ops.RaggedBatch:
         """The batch as the ragged operators take it (one per step, shared by
@@ -82,26 +82,25 @@ class VLLMBatch:
 
     def positions(self) -> torch.Tensor:
         """int64 (num_actual_tokens,): each token's position in its request,
-        computed on the device; 0 for rows of no request (padding) and for
-        tokens before their request's start.  The layers of a step share it, as
-        long as the versions of the offsets and lengths show them unchanged: not
-        while a graph is captured, whose replays have lengths of their own, nor
-        for inference tensors, which keep no version."""
-        ts = (self.query_start_loc, self.seq_lens)
-        fresh = any(t.is_inference() for t in ts) or (
-            ts[0].is_cuda and torch.cuda.is_current_stream_capturing())
-        of = None if fresh else (*((t.data_ptr(), t._version) for t in ts), self.num_actual_tokens)
-        if not fresh and self._positions is not None and self._positions[0] == of:
-            return self._positions[1]
+        computed on the device from the offsets and lengths as they are now; 0
+        for rows of no request (padding) and for tokens before their request's
+        start.  Some eight small launches: a model computes them once a step and
+        hands them to every layer's forward(positions=).  Later calls write the
+        same tensor anew (not while a graph is captured, which owns its own,
+        nor in inference mode)."""
         start = self.query_start_loc
         row = torch.arange(self.num_actual_tokens, dtype=start.dtype, device=start.device)
         # request r's rows are in interval r + 1 of the offsets; intervals 0 and
         # R + 1 lie outside the batch: far below 0
         first = torch.nn.functional.pad((self.seq_lens - start[1:]).long(), (1, 1), value=-2 ** 40)
-        at = (first[torch.searchsorted(start, row, right=True)] + row).clamp_(min=0)
-        if not fresh:
-            self._positions = (of, at)
-        return at
+        at = first[torch.searchsorted(start, row, right=True)] + row
+        if torch.is_inference_mode_enabled() or at.is_inference() or (
+                at.is_cuda and torch.cuda.is_current_stream_capturing()):
+            return at.clamp_(min=0)
+        if self._positions is None or self._positions.shape != at.shape or \
+                self._positions.device != at.device:
+            self._positions = torch.empty_like(at)
+        return torch.clamp(at, min=0, out=self._positions)
 
     @classmethod
     def from_metadata(cls, md) -> "VLLMBatch":

@@ -349,3 +349,16 @@ def test_positions_of_a_padded_batch():
     assert vllm_batch([0, 3], [1], 3, 3).positions().tolist() == [0, 0, 0]
     assert vllm_batch([0, 0], [5], 2, 0).positions().tolist() == [0, 0]
     assert vllm_batch([0, 2, 5], [7, 3], 5, 3).positions().dtype == torch.int64
+
+
+def test_positions_follow_writes_that_torch_does_not_count():
+    """A graph's replay and .data write lengths without a new version."""
+    b = vllm_batch([0, 2, 5], [7, 3], 5, 3)
+    assert b.positions().tolist() == [5, 6, 0, 1, 2]
+    b.seq_lens.data.add_(4)
+    assert b.positions().tolist() == [9, 10, 4, 5, 6]
+    b.num_actual_tokens = 6
+    assert b.positions().tolist() == [9, 10, 4, 5, 6, 0]
+    with torch.inference_mode():
+        assert b.positions().tolist() == [9, 10, 4, 5, 6, 0]
+    assert not b.positions().is_inference()
