@@ -432,18 +432,19 @@ def decode_attention(tables: LayerTables, pages: torch.Tensor, q: torch.Tensor,
 # ---------------------------------------------------------------------------
 class _Described:
     """A frozen dataclass of tensors with its C descriptor, made once (2 us) and
-    again when a tensor's memory has moved (``module.to()`` swaps it)."""
+    again when a tensor's memory, type or shape is another (``module.to()`` swaps
+    them, and may put the new ones at the old address)."""
 
-    def _ptrs(self):
-        return tuple(x.data_ptr() for x in self._tensors())
+    def _views(self):
+        return [(x.data_ptr(), x.dtype, x.shape, x.stride()) for x in self._tensors()]
 
     def __post_init__(self):
         object.__setattr__(self, "_c", self._describe())
-        object.__setattr__(self, "_at", self._ptrs())
+        object.__setattr__(self, "_of", self._views())
 
     @property
     def c(self):
-        if self._ptrs() != self._at:
+        if self._views() != self._of:
             self.__post_init__()
         return self._c
 

@@ -362,3 +362,26 @@ def test_positions_follow_writes_that_torch_does_not_count():
     with torch.inference_mode():
         assert b.positions().tolist() == [9, 10, 4, 5, 6, 0]
     assert not b.positions().is_inference()
+
+
+def test_descriptors_follow_type_and_shape_at_one_address():
+    """module.half() may put a weight of another type at the address of the old one."""
+    buf = torch.zeros(64, dtype=torch.uint8)
+    w = torch.nn.Parameter(buf[:32].view(torch.float32))
+    norm = ops.HeadNorm(w)
+    assert norm.c.dtype == _lib.TQ_F32
+    w.data = buf[:16].view(torch.float16)
+    assert norm.c.weight == buf.data_ptr() and norm.c.dtype == _lib.TQ_F16
+    w.data = buf[:32].view(torch.float16)[::2]
+    with pytest.raises(ValueError, match="contiguous"):
+        norm.c
+    buf = torch.zeros(48)
+    table = ops.RopeTable(buf.view(6, 8))
+    assert (table.c.positions, table.c.rot_dim) == (6, 8)
+    table.cos_sin.data = buf[:16].view(4, 4)
+    assert table.c.cos_sin == buf.data_ptr() and (table.c.positions, table.c.rot_dim) == (4, 4)
+    buf = torch.zeros(8, dtype=torch.int32)
+    batch = ops.RaggedBatch(buf[:4], buf[4:7], 1)
+    assert batch.c.requests == 3
+    batch.seq_lens.data, batch.q_start.data = buf[4:6], buf[:3]
+    assert batch.c.requests == 2 and batch.c.q_start == buf.data_ptr()
