@@ -245,15 +245,34 @@ def dequantize(tables: LayerTables, pages: torch.Tensor, t0: int, t1: int,
         ctypes.byref(vo) if vo is not None else None, _stream(pages.device)))
 
 
+def _capturing(device: torch.device) -> bool:
+    return device.type == "cuda" and torch.cuda.is_current_stream_capturing()
+
+
 class DecodeWorkspace:
-    """Grow-only device scratch for tq_decode_attn (first 4 bytes: status word)."""
+    """Grow-only device scratch of the attention calls (first 4 bytes: status
+    word), one call at a time: calls of one stream may share it, and so may
+    graphs that are replayed on one stream.  A buffer that a captured call
+    has been given is kept as long as the workspace, since every replay writes
+    to it; keep the workspace as long as the graph."""
 
     def __init__(self):
         self.buf: Optional[torch.Tensor] = None
+        self._captured = False      # a graph holds the address of buf
+        self._unset = False         # allocated while capturing: zeroed by the graph's replay only
+        self._kept = []             # earlier buffers whose address a graph holds
 
     def get(self, nbytes: int, device: torch.device) -> torch.Tensor:
+        capturing = _capturing(device)
         if self.buf is None or self.buf.numel() < nbytes or self.buf.device != device:
+            if self._captured:
+                self._kept.append(self.buf)
             self.buf = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=device)
+            self._captured, self._unset = False, capturing
+        elif self._unset and not capturing:
+            self.buf.zero_()
+            self._unset = False
+        self._captured = self._captured or capturing
         return self.buf
 
     def status(self) -> int:

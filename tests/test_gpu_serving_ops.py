@@ -830,3 +830,40 @@ def test_paged_attention_layer_with_rope_replays_with_new_lengths():
     for a, b in zip(*outs):
         assert torch.equal(a, b)
     assert ok_status() == 0
+
+
+def test_captured_layer_replays_after_its_workspace_grew():
+    """A decode step is captured, a larger eager prompt follows (the workspace grows), other tensors
+    take whatever memory was given back, and the graph is replayed: they stay as they were and the
+    replay gives what an eager step gives."""
+    from bhaskera_col_b200.inference.vllm_turboquant import TurboQuantPagedAttention, VLLMBatch
+    D, Hq, H, R, T = 128, 8, 2, 4, 700
+    rope = ops.RopeTable.build(D, 2000, device=DEV)
+    layer = TurboQuantPagedAttention(5, 32, Hq, H, D, num_blocks=24 * R, block_size=64, key_bits=4,
+                                     value_bits=2, device=DEV)
+    table = torch.arange(24 * R, dtype=torch.int32, device=DEV).view(R, 24)
+    heads = lambda n, s: [randn((n, h, D), s + j) for j, h in enumerate((Hq, H, H))]  # noqa: E731
+    decode = VLLMBatch(int32(range(R + 1)), int32([10, 64, 1, 33]), table, R, 1)
+    step = heads(R, 51)
+    out = torch.empty_like(step[0])
+    layer.forward(*step, decode, out=out, rope=rope)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        layer.forward(*step, decode, out=out, rope=rope)
+    held = layer.ragged_workspace.buf
+    prompts = VLLMBatch(int32([T * i for i in range(R + 1)]), int32([T] * R), table, T * R, T)
+    layer.forward(*heads(T * R, 61), prompts, rope=rope)
+    assert layer.ragged_workspace.buf.numel() > held.numel()
+    at, size = held.data_ptr(), held.numel()
+    del held
+    fill = [torch.full((size,), 7, dtype=torch.uint8, device=DEV) for _ in range(4)]
+    assert all(x.data_ptr() + size <= at or at + size <= x.data_ptr() for x in fill)
+    decode.seq_lens.copy_(int32([T + 1] * R))
+    pool = layer.pool.clone()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all((x == 7).all() for x in fill)
+    got, stored = out.clone(), layer.pool.clone()
+    layer.pool.copy_(pool)
+    layer.forward(*step, decode, out=out, rope=rope)
+    assert torch.equal(out, got) and torch.equal(layer.pool, stored) and ok_status() == 0

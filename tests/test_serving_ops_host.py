@@ -385,3 +385,33 @@ def test_descriptors_follow_type_and_shape_at_one_address():
     assert batch.c.requests == 3
     batch.seq_lens.data, batch.q_start.data = buf[4:6], buf[:3]
     assert batch.c.requests == 2 and batch.c.q_start == buf.data_ptr()
+
+
+def test_workspace_keeps_what_a_capture_has_seen(monkeypatch):
+    """A captured call goes on using its buffer at every replay: growing must not give it back."""
+    import gc
+    import weakref
+    dev, capturing = torch.device("cpu"), [False]
+    monkeypatch.setattr(ops, "_capturing", lambda device: capturing[0], raising=False)
+    ws = ops.DecodeWorkspace()
+    first = weakref.ref(ws.get(1000, dev))
+    second = weakref.ref(ws.get(2000, dev))
+    gc.collect()
+    assert first() is None and ws.get(1500, dev) is second()    # nothing captured: one buffer
+    capturing[0] = True
+    assert ws.get(1800, dev) is second()
+    capturing[0] = False
+    third = weakref.ref(ws.get(3000, dev))
+    fourth = weakref.ref(ws.get(4000, dev))
+    gc.collect()
+    assert second() is not None and third() is None and ws.get(10, dev) is fourth()
+    # a buffer first taken while capturing holds nothing before the graph has run: cleared for others
+    ws = ops.DecodeWorkspace()
+    capturing[0] = True
+    own = ws.get(100, dev)
+    own.fill_(7)
+    assert ws.get(50, dev) is own and (own == 7).all()
+    capturing[0] = False
+    assert ws.get(100, dev) is own and (own == 0).all()
+    own.fill_(7)
+    assert ws.get(100, dev) is own and (own == 7).all()
