@@ -245,14 +245,16 @@ __global__ void __launch_bounds__(kRowThreads, 3) rope_rows_kernel(RopeParams p,
     }
   }
   const int64_t yb = b * s.ys[0] + t * s.ys[2] + (int64_t)h0 * s.ys[1];
+  // The sums cross lanes, and a warp holds groups of q and of k, so every lane
+  // takes part where either side has a norm, and heads past a run's end are
+  // worked on too (zeros).
+  const bool normed = p.side[0].f.weight != nullptr || p.side[1].f.weight != nullptr;
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
-    // heads past the run's end are worked on too (zeros): the lanes of a warp
-    // stay together for the sums
     f2 u[P / 2], v[P / 2];
     a[i].widen(u);
     c[i].widen(v);
-    if (s.f.weight) {
+    if (normed) {
       f2 sq = tc::f2_mul(u[0], u[0]);
       sq = tc::f2_fma(v[0], v[0], sq);
 #pragma unroll
@@ -262,7 +264,7 @@ __global__ void __launch_bounds__(kRowThreads, 3) rope_rows_kernel(RopeParams p,
       float ss = lo + hi;
 #pragma unroll
       for (int o = LV / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      const float r = rsqrtf(fmaf(ss, 1.f / (float)D, s.f.eps));
+      const float r = s.f.weight ? rsqrtf(fmaf(ss, 1.f / (float)D, s.f.eps)) : 1.f;
       const f2 rr = tc::f2_make(r, r);
 #pragma unroll
       for (int e = 0; e < P / 2; ++e) {

@@ -867,3 +867,26 @@ def test_captured_layer_replays_after_its_workspace_grew():
     layer.pool.copy_(pool)
     layer.forward(*step, decode, out=out, rope=rope)
     assert torch.equal(out, got) and torch.equal(layer.pool, stored) and ok_status() == 0
+
+
+@pytest.mark.parametrize("rope", ["half", "interleaved", "none"])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n,hq,hkv,D", [(3, 8, 2, 128), (7, 5, 1, 64), (1, 4, 4, 128), (5, 2, 3, 256),
+                                        (9, 1, 1, 32), (2, 9, 5, 80)])
+def test_qk_rope_norm_of_one_side(n, hq, hkv, D, dtype, rope):
+    """Only the queries or only the keys are normed, in one call for both: heads of either side lie
+    beside each other in a warp."""
+    table = None if rope == "none" else ops.RopeTable.build(D, 50, interleaved=rope == "interleaved",
+                                                            device=DEV)
+    pos = torch.arange(n) * 5
+    q, k = randn((n, hq, D), 1, dtype, 3), randn((n, hkv, D), 2, dtype)
+    norm = ops.HeadNorm(1 + 0.2 * randn((D,), 7, F32), 1e-6)
+    for norms in ((norm, None), (None, norm)):
+        if table is None:
+            with pytest.raises(_lib.TqError, match="neither a rotation nor a norm"):
+                ops.qk_rope(q, k, None, None, *norms)
+            continue
+        qo, ko = ops.qk_rope(q, k, table, pos.to(DEV), *norms)
+        check_rope(qo, q, table, pos.numpy(), norms[0])
+        check_rope(ko, k, table, pos.numpy(), norms[1])
+    assert ok_status() == 0
