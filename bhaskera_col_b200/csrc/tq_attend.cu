@@ -338,16 +338,29 @@ struct AttendShape {
 // and runs the codes that the few-row kernel has no table for (above 4 bits).
 constexpr int kFewRows = 128;
 
+// The kernels that a call may use: few rows, and tcgen05 (else mma.sync) for the
+// others.  The tcgen05 kernel's operands are single fp16 values: for fp16 and fp32
+// results (error 7e-4, against 2.1e-4 of fp16's own rounding) only when asked for,
+// although it is six times as fast from 1,024 rows on (562 us against 3,397).
+struct Kernels {
+  bool few, tc;
+};
+
+Kernels attend_kernels(const tq_geom* G, const tq_attend_args* a) {
+  Kernels k;
+  k.few = attend_few_applies(G) && (a->engine == 0 || a->engine == 3);
+  k.tc = prefill_tc_applies(G) && (a->engine == 2 || (a->engine == 0 && !attend_precise(a)));
+  return k;
+}
+
 AttendShape attend_shape(const tq_geom* G, const tq_cache* c, const tq_attend_args* a) {
   AttendShape s = {};
   const int64_t R = a->batch.requests, N = a->q->shape[2], most = INT64_MAX;
   s.Hkv = c->streams / R;
   const int64_t g = a->q->shape[1] / s.Hkv;
-  // the tcgen05 kernel's operands are single fp16 values: for fp16 and fp32 results
-  // (error 7e-4, against 2.1e-4 of fp16's own rounding) only when asked for, although
-  // it is six times as fast from 1,024 rows on (562 us against 3,397)
-  s.tc = prefill_tc_applies(G) && (a->engine == 2 || (a->engine == 0 && !attend_precise(a)));
-  const bool can = attend_few_applies(G) && (a->engine == 0 || a->engine == 3);
+  const Kernels kernels = attend_kernels(G, a);
+  s.tc = kernels.tc;
+  const bool can = kernels.few;
   const int64_t few_q = s.tc ? tmax<int64_t>(kFewRows / g, 1) : most;
   size_t off = 256;                        // the first 64 bytes: the decode's status word
   auto take = [&](size_t bytes) {
@@ -403,6 +416,11 @@ AttendShape attend_shape(const tq_geom* G, const tq_cache* c, const tq_attend_ar
 }
 
 }  // namespace
+
+bool attend_applies(const tq_geom* G, const tq_attend_args* a) {
+  const Kernels k = attend_kernels(G, a);
+  return k.few || k.tc || (a->engine <= 1 && attend_mma_applies(G));
+}
 
 size_t attend_ragged_workspace(const tq_geom* G, const tq_cache* c, const tq_attend_args* a) {
   return attend_shape(G, c, a).bytes;

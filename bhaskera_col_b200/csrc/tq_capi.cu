@@ -81,6 +81,7 @@ int set_smem_attr(const void* kernel, size_t bytes) {
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                        (int)bytes);
   if (e != cudaSuccess) {
+    cudaGetLastError();   // not to be found by the next launch's check
     set_error("cudaFuncSetAttribute(%zu bytes of shared memory): %s", bytes, cudaGetErrorString(e));
     return TQ_ERR_CUDA;
   }
@@ -730,11 +731,7 @@ static int check_attend(const tq_geom* g, const tq_cache* c, const tq_attend_arg
               fn, a->engine);
     return TQ_ERR_INVALID;
   }
-  const bool tc = prefill_tc_applies(g);
-  const bool mma = prefill_supported(g->head_dim, g->key_bits, g->value_bits);
-  if (a->engine == 0 ? !mma && !tc && !attend_few_applies(g)
-      : a->engine == 1 ? !mma
-      : a->engine == 2 ? !tc : !attend_few_applies(g)) {
+  if (!attend_applies(g, a)) {
     set_error("%s: no kernel for head_dim %d, key_bits %d, value_bits %d (engine %d)", fn,
               g->head_dim, g->key_bits, g->value_bits, a->engine);
     return TQ_ERR_INVALID;

@@ -86,7 +86,10 @@ int launch_dequant_ragged_tc(const tq_geom* g, const tq_tables* t, const tq_cach
 size_t attend_ragged_workspace(const tq_geom* g, const tq_cache* c, const tq_attend_args* a);
 int launch_attend_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                          const tq_attend_args* a, void* ws, uint32_t* status, cudaStream_t st);
+// Whether some kernel attends a batch of this geometry, result type and engine.
+bool attend_applies(const tq_geom* g, const tq_attend_args* a);
 bool attend_few_applies(const tq_geom* g);
+bool attend_mma_applies(const tq_geom* g);
 int launch_attend_few(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                       const tq_attend_args* a, const RaggedAttend& rg, int64_t Hkv, int hc,
                       int pcta, int rows, const __half* qp, int64_t qp_stride, int64_t grid,

@@ -550,6 +550,8 @@ PfFn pf_fn(int kb, int vb) {
 #define TQ_PF(K, V) if (kb == K && vb == V) return prefill_kernel<D, K, V, RG, HP>;
   TQ_PF(4, 2) TQ_PF(3, 3) TQ_PF(2, 2) TQ_PF(4, 4) TQ_PF(6, 4) TQ_PF(5, 5) TQ_PF(6, 6)
   TQ_PF(8, 8) TQ_PF(3, 2) TQ_PF(4, 3)
+  // a ragged batch's fp16 and fp32 results have no tcgen05 kernel to take these
+  if constexpr (RG) { TQ_PF(5, 4) }
 #undef TQ_PF
   return nullptr;
 }
@@ -559,6 +561,12 @@ PfFn pf_fn(int kb, int vb) {
 bool prefill_supported(int D, int kb, int vb) {
   if (D == 128) return pf_fn<128, false>(kb, vb) != nullptr;
   if (D == 64) return pf_fn<64, false>(kb, vb) != nullptr;
+  return false;
+}
+
+bool attend_mma_applies(const tq_geom* G) {
+  if (G->head_dim == 128) return pf_fn<128, true>(G->key_bits, G->value_bits) != nullptr;
+  if (G->head_dim == 64) return pf_fn<64, true>(G->key_bits, G->value_bits) != nullptr;
   return false;
 }
 

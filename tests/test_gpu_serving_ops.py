@@ -890,3 +890,34 @@ def test_qk_rope_norm_of_one_side(n, hq, hkv, D, dtype, rope):
         check_rope(qo, q, table, pos.numpy(), norms[0])
         check_rope(ko, k, table, pos.numpy(), norms[1])
     assert ok_status() == 0
+
+
+@pytest.mark.parametrize("engine", [0, 1, 2, 3])
+@pytest.mark.parametrize("D", [64, 128])
+def test_attend_ragged_runs_what_it_accepts(D, engine):
+    """Every pair of code widths and every result type: the call is refused before anything runs, or
+    gives the right result; few and many rows.  A refusal leaves nothing behind for the next call."""
+    H, Hq = 1, 4
+    batch, start, seq = make_batch([(2, 40), (70, 100)])
+    ran = set()
+    for kb in range(1, 9):
+        for vb in range(1, 9):
+            tables = make_tables(D, kb, vb, False)
+            pages = make_paged(tables, 2 * H, 100)
+            fill(tables, pages, 2, H, 128, 3)
+            kd, vd = (x.reshape(2, H, -1, D) for x in S.dense(tables, contiguous(pages), 128))
+            for dtype in (BF16, F16, F32):
+                q = randn((start[-1], Hq, D), 4, dtype)
+                try:
+                    got = ops.attend_ragged(tables, pages, q, batch, engine=engine)
+                except _lib.TqError as e:
+                    assert "no kernel for" in str(e) and "workspace_bytes" in str(e)
+                    continue
+                ran.add((kb, vb, dtype))
+                check_attend(got, S.attend(q, kd, vd, start, seq, S.default_scale(D), True), dtype)
+    assert ok_status() == 0
+    pairs = {t: {(k, v) for k, v, u in ran if u == t} for t in (BF16, F16, F32)}
+    assert pairs[F16] == pairs[F32]
+    if engine == 0:      # what bf16 models run, fp16 ones do too: protected layers' widths among them
+        assert pairs[BF16] == pairs[F32] and {(6, 4), (6, 6), (5, 5), (4, 4)} <= pairs[F32]
+        assert D == 64 or (5, 4) in pairs[F32]

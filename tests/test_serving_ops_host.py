@@ -415,3 +415,22 @@ def test_workspace_keeps_what_a_capture_has_seen(monkeypatch):
     assert ws.get(100, dev) is own and (own == 0).all()
     own.fill_(7)
     assert ws.get(100, dev) is own and (own == 7).all()
+
+
+@pytest.mark.parametrize("engine", [0, 1, 2, 3])
+@pytest.mark.parametrize("dtype", [_lib.TQ_BF16, _lib.TQ_F16, _lib.TQ_F32])
+def test_attend_workspace_query_accepts_what_the_call_does(dtype, engine):
+    """Code widths that the query sizes a workspace for are those that the call goes on with (here up
+    to its workspace check)."""
+    for D in (64, 128):
+        for kb in range(1, 9):
+            for vb in range(1, 9):
+                q = t4((1, 4, 10, D), dtype=dtype)
+                rc, err, need = attend(g=geom(D, kb, vb), q=q, out=far((1, 4, 10, D), dtype=dtype),
+                                       engine=engine, nbytes=0)
+                assert (need > 0) == (rc == _lib.TQ_ERR_WORKSPACE), err
+                assert need > 0 or "no kernel" in err
+    # the protected layers of K3/V2: (5, 4)
+    rc, _, need = attend(g=geom(kb=5, vb=4), q=t4((1, 4, 10, 128), dtype=dtype),
+                         out=far((1, 4, 10, 128), dtype=dtype), engine=engine, nbytes=0)
+    assert (need > 0) == (engine < 3)
