@@ -47,16 +47,18 @@ struct PlanParams {
 
 // A listed request in the plan's terms.
 struct Tiles {
-  int tiles, q_len, seq;
+  int tiles, q_len, seq, base;
 };
 
 __device__ __forceinline__ Tiles listed_request(const PlanParams& p, int64_t r) {
-  Tiles t = {0, 0, 0};
+  Tiles t = {0, 0, 0, 0};
   if (r >= p.rv.R) return t;
   const Request q = request_at(p.rv, r);
   if (q.q_len <= p.q_lo || q.q_len > p.q_hi) return t;
   t.q_len = (int)q.q_len;
   t.seq = (int)q.seq;
+  t.base = (int)q.base;
+  if (t.base + t.q_len > t.seq) atomicOr(p.status, TQ_DEV_BAD_POSITION);   // longer than its pages
   t.tiles = (t.q_len + p.pcta - 1) / p.pcta;
   return t;
 }
@@ -64,7 +66,7 @@ __device__ __forceinline__ Tiles listed_request(const PlanParams& p, int64_t r) 
 // Key tiles of query block i.
 __device__ __forceinline__ int key_tiles(const PlanParams& p, const Tiles& t, int i) {
   int kend = t.seq;
-  if (p.causal) kend = t.seq - t.q_len + (int)tmin<int64_t>((int64_t)(i + 1) * p.pcta, t.q_len);
+  if (p.causal) kend = tmin(kend, t.base + (int)tmin<int64_t>((int64_t)(i + 1) * p.pcta, t.q_len));
   return kend > 0 ? (kend + p.keys - 1) >> p.key_shift : 0;
 }
 
@@ -84,6 +86,7 @@ __device__ __forceinline__ void for_tiles(const PlanParams& p, const Tiles& own,
       b.tiles = __shfl_sync(0xffffffffu, t.tiles, src);
       b.q_len = __shfl_sync(0xffffffffu, t.q_len, src);
       b.seq = __shfl_sync(0xffffffffu, t.seq, src);
+      b.base = __shfl_sync(0xffffffffu, t.base, src);
       for (int i = lane; i < b.tiles; i += 32) f((int)(r0 + (tid & ~31) + src), i, key_tiles(p, b, i));
     }
   }

@@ -155,10 +155,11 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
   const int64_t qrow = RG ? sw.rq.q0 * p.qs[2] : b * p.qs[0];
   const int64_t orow = RG ? sw.rq.q0 * p.os[2] : b * p.os[0];
   const int64_t h = kvh * p.g + (int64_t)chunk * p.hc + warp / wph;   // this warp's head
-  const int64_t t_base = p.n_tokens - p.Tq;            // position of query 0
+  const int64_t t_base = RG ? sw.rq.base : p.n_tokens - p.Tq;   // position of query 0
   const int t0 = qb * P + (warp % wph) * 16;           // this warp's first query
   const int64_t qpos_max = t_base + tmin<int64_t>((int64_t)(qb + 1) * P, p.Tq) - 1;
-  const int64_t kend = p.causal ? qpos_max + 1 : p.n_tokens;   // keys this CTA needs
+  // keys this CTA needs
+  const int64_t kend = p.causal ? tmin<int64_t>(qpos_max + 1, p.n_tokens) : p.n_tokens;
   const int tile0 = RG ? sw.seg.kt0 : 0;
   const int ntiles = RG ? sw.seg.kt1 - tile0 : (int)((kend + 63) / 64);
   int64_t kst = 0;                                     // first attended key (left padding)

@@ -19,6 +19,7 @@ struct RaggedView {
 
 struct Request {
   int64_t q0, q_len, seq;     // first row, rows, tokens in the cache (new ones included)
+  int64_t base;               // position of the first row
 };
 
 // Request r, with offsets outside the tensors cut to them: a wrong offset
@@ -29,6 +30,7 @@ __device__ __forceinline__ Request request_at(const RaggedView& v, int64_t r) {
   q.q0 = tmin(tmax<int64_t>(a, 0), v.N);
   q.q_len = tmax<int64_t>(tmin(b, v.N) - q.q0, 0);
   q.seq = tmin(tmax<int64_t>(s, 0), v.cap);
+  q.base = tmax<int64_t>(s, 0) - q.q_len;   // of the length as it is: rows keep their places
   return q;
 }
 

@@ -762,7 +762,8 @@ def attend_ragged(tables: LayerTables, pages, q: torch.Tensor, batch: RaggedBatc
     (prompt chunks, draft tokens, single tokens, mixed), or with ``causal``
     False every row over all of them (cross attention: the pages hold an
     encoder's states, seq_lens their lengths).  A row that sees no key is
-    zero.  Work is split along long contexts.  ``engine`` 0 picks the kernels
+    zero; a request longer than its pages attends what they hold and sets
+    _lib.DEV_BAD_POSITION.  Work is split along long contexts.  ``engine`` 0 picks the kernels
     by each request's rows and the type of ``out`` (fp16 and fp32 results are
     exact to their rounding and to 2^-18); 1 is the mma.sync kernel, 2 the
     tcgen05 kernel (error 7e-4 in any type), 3 the kernel of few query rows.  Pass a ``workspace`` to reuse one buffer

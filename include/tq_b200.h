@@ -63,8 +63,8 @@ extern "C" {
 /* device status word bits (written by kernels into the workspace) */
 #define TQ_DEV_WAIT_TIMEOUT 1u  /* a bounded mbarrier wait ran out          */
 #define TQ_DEV_BAD_BLOCK 2u     /* a block-table entry was outside the pool */
-#define TQ_DEV_BAD_POSITION 4u  /* a position outside the rotation table or,
-                                   in a ragged append, outside the pages      */
+#define TQ_DEV_BAD_POSITION 4u  /* a position outside the rotation table or, in
+                                   a ragged batch, outside the pages          */
 #define TQ_DEV_BAD_BATCH 8u     /* a ragged batch's row offsets do not ascend
                                    within the tensor's rows                   */
 
@@ -431,7 +431,9 @@ int32_t tq_dequantize_ragged(const tq_geom* g, const tq_tables* t, const tq_cach
  * r attends the request's tokens [0, seq_lens[r]), with causal only those at
  * or before its own position.  causal = 0 with seq_lens the lengths of stored
  * encoder states is cross attention (the queries are then no tokens of the
- * cache).  A row that sees no key is zero.  Scores, values and geometries as
+ * cache).  A row that sees no key is zero.  A request longer than its pages
+ * (seq_lens[r] tokens where they hold fewer) attends the tokens that they hold
+ * and sets TQ_DEV_BAD_POSITION.  Scores, values and geometries as
  * in tq_prefill_attn (no QJL sketch, no window).  A stored norm that is not
  * finite makes NaN of the rows that attend its token and of no other. */
 typedef struct tq_attend_args {

@@ -921,3 +921,24 @@ def test_attend_ragged_runs_what_it_accepts(D, engine):
     if engine == 0:      # what bf16 models run, fp16 ones do too: protected layers' widths among them
         assert pairs[BF16] == pairs[F32] and {(6, 4), (6, 6), (5, 5), (4, 4)} <= pairs[F32]
         assert D == 64 or (5, 4) in pairs[F32]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("engine,dtype", [(0, BF16), (1, BF16), (2, BF16), (3, BF16), (0, F32), (1, F32)])
+def test_attend_ragged_requests_longer_than_their_pages(engine, dtype, causal):
+    """Rows keep the positions that the lengths give them; they see the tokens that the pages hold."""
+    D, Hq, H = 128, 8, 2
+    tables = make_tables(D, 4, 2, False)
+    lens = [(40, 150), (3, 129), (2, 128), (5, 400), (150, 150), (1, (1 << 31) - 1)]
+    batch, start, seq = make_batch(lens)
+    pages = make_paged(tables, len(lens) * H, 128)
+    fill(tables, pages, len(lens), H, 128, 3)
+    kd, vd = (x.reshape(len(lens), H, -1, D) for x in S.dense(tables, contiguous(pages), 128))
+    q = randn((start[-1], Hq, D), 4, dtype)
+    got = ops.attend_ragged(tables, pages, q, batch, causal=causal, engine=engine)
+    assert ok_status() == _lib.DEV_BAD_POSITION
+    check_attend(got, S.attend(q, kd, vd, start, seq, S.default_scale(D), causal), dtype)
+    fits, _, _ = make_batch([(2, 128), (3, 60), (0, 1 << 20)])       # a request without rows is not run
+    ops.attend_ragged(tables, ops.PagedPages(pages.pool, pages.block_table[: 3 * H]), q[:5], fits,
+                      causal=causal, engine=engine)
+    assert ok_status() == 0
