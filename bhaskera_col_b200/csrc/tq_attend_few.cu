@@ -317,7 +317,8 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
   const int nh = min(p.hc, p.g - chunk * p.hc);            // heads of this CTA
   const int64_t stream = (int64_t)sw.seg.req * p.Hkv + kvh;
   const int q_len = (int)sw.rq.q_len, pos0 = sw.seg.tile * p.pcta;
-  const int64_t seq = sw.rq.seq, t_base = sw.rq.base;      // position of the request's row 0
+  // keys in the pages, position of the request's row 0: 32 bits (base + q_len is a length)
+  const int seq = (int)sw.rq.seq, t_base = (int)sw.rq.base;
   // row n of the CTA: position pos0 + n / hc, head h0 + n % hc
   auto row_pos = [&](int n) { return n < p.pcta * p.hc ? pos0 + n / p.hc : INT_MAX; };
   auto row_valid = [&](int n) { return row_pos(n) < q_len && n % p.hc < nh; };
@@ -326,10 +327,9 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
   };
   // the last key row n sees
   auto row_lim = [&](int n) -> int {
-    return p.causal && row_valid(n) ? (int)min(t_base + row_pos(n), seq - 1) : (int)seq - 1;
+    return p.causal && row_valid(n) ? min(t_base + row_pos(n), seq - 1) : seq - 1;
   };
-  const int kend =
-      p.causal ? (int)max(min(t_base + min(pos0 + p.pcta, q_len), seq), (int64_t)0) : (int)seq;
+  const int kend = p.causal ? max(min(t_base + min(pos0 + p.pcta, q_len), seq), 0) : seq;
 
   // ---- the thread's place in every page and the first pages' loads -------------
   uint32_t ksh, vsh;
