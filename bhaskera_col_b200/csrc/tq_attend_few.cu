@@ -22,6 +22,9 @@
 // The running max moves only when a score passes it by kRoom (a vote; the
 // shuffles and the rescale of 32 NT outputs run then: nearly every tile has a
 // new max among its 16 rows, so moving it at once cost a fifth of the time).
+// Value norms enter P' times a power of two that puts the largest one so far near
+// kNorm (the same vote moves it), and a row of O is scaled by one of its own before
+// its last rotation: fp16 ends at 2^-24, where the norms of a cache need not.
 //
 // q' = scale log2(e) q R^T comes ready from the launch that builds the work list
 // (rotated in every segment it was most of a segment's set-up); out = O R runs on
@@ -30,8 +33,10 @@
 // Bound by the loop's shared-memory wavefronts (65 % of the SM's) and latency,
 // 1.25 us a page and CTA; HBM would allow a fifth.  K4/V2, 8 KV heads of 128, g 4:
 // 252 draft tokens over 256,960 156 us, 1.3 TB/s; K3/V3, g 5: 5 tokens over
-// 131,001 142 us.  HP reads eight bytes a lookup and multiplies three times:
-// 335 and 290 us.
+// 131,001 140 us.  HP reads eight bytes a lookup and multiplies three times:
+// 317 and 272 us.  168 registers are the most for three CTAs an SM; what the loop
+// needs rarely (each row's last key, the bad pages' flag) is kept out of them, since
+// a spilled one cost up to 25 us of the second.
 #include "tq_internal.h"
 #include "tq_ragged.cuh"
 
@@ -43,14 +48,15 @@ namespace tq {
 namespace {
 
 // A score may pass the running max by this much before the max moves: p <=
-// 2^7, and with a value norm of at most 2^8 P' <= 2^15 stays in fp16 (for
-// larger norms the max moves at once, p <= 1 and P' <= the norm itself).
+// 2^7, and with scaled value norms below 2^8 P' < 2^15 stays in fp16.
 constexpr float kRoom = 7.f;
+constexpr float kNorm = 256.f;
 constexpr float kNoMax = -1e30f;   // below every score
 
 struct FewParams {
   const uint8_t* pages;
   PageMap pm;
+  int nblocks;                  // pages that a table entry may name
   int page_bytes, off_v, off_kn, off_vn;
   const __half* rot_h;          // R [D][D] fp16
   const float* rot;             // R [D][D] (HP)
@@ -309,6 +315,7 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
   uint32_t* A = reinterpret_cast<uint32_t*>(sm + F::OFF_A);
   float* rowl = reinterpret_cast<float*>(sm + F::OFF_R);
   int* flags = reinterpret_cast<int*>(sm + F::OFF_R + 128);   // last CTA, first bad key
+  int* lims = reinterpret_cast<int*>(sm + F::OFF_R + 192);    // [NQ] last key each row sees
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int gq = lane >> 2, tq = lane & 3;
@@ -334,26 +341,23 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
   // ---- the thread's place in every page and the first pages' loads -------------
   uint32_t ksh, vsh;
   const int s0 = 16 * warp;                                // first token of the quarter
-  const uint8_t* pk = p.pages + (s0 + gq) * KROW + code_start<Tile::KN>(tq * Tile::KN, ksh);
-  const uint8_t* pv = p.pages + p.off_v + (s0 + 2 * tq) * VROW +
-                      code_start<Tile::VN>(gq * Tile::VN, vsh);
-  const uint8_t* pn = p.pages + p.off_kn + 2 * (s0 + gq);
+  const int at_k = (s0 + gq) * KROW + code_start<Tile::KN>(tq * Tile::KN, ksh);
+  const int at_v = p.off_v + (s0 + 2 * tq) * VROW + code_start<Tile::VN>(gq * Tile::VN, vsh);
+  const int at_n = p.off_kn + 2 * (s0 + gq);
   const int pend = min(sw.seg.kt1, (kend + 63) >> 6);      // pages [kt0, pend)
   const int32_t* bt = p.pm.bt ? p.pm.bt + stream * p.pm.bt_stride : nullptr;
   const int slot0 = (int)(stream * p.pm.pps);              // contiguous layout
-  const int nblocks = p.pm.bt ? (int)p.pm.nblocks : INT_MAX;
-  bool bad_block = false;
   auto entry = [&](int pg) -> int {
     pg = min(pg, pend - 1);
     return bt ? __ldg(bt + pg) : slot0 + pg;
   };
   auto load_tile = [&](Tile& x, int e) {
-    const bool ok = (unsigned)e < (unsigned)nblocks;       // e < 0 fails too
-    bad_block = bad_block || !ok;
-    e = ok ? e : 0;
-    const uint8_t* k = page_at(pk, e, p.page_bytes);
-    const uint8_t* v = page_at(pv, e, p.page_bytes);
-    const uint8_t* n = page_at(pn, e, p.page_bytes);
+    if ((unsigned)e >= (unsigned)p.nblocks) {              // e < 0 too
+      atomicOr(p.status, TQ_DEV_BAD_BLOCK);
+      e = 0;
+    }
+    const uint8_t* page = page_at(p.pages, e, p.page_bytes);
+    const uint8_t *k = page + at_k, *v = page + at_v, *n = page + at_n;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       x.k[i].load(k + 8 * i * KROW);
@@ -375,6 +379,7 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
 
   // ---- query rows, table ---------------------------------------------------------
   if (tid == 0) flags[1] = INT_MAX;
+  if (tid < NQ) lims[tid] = row_lim(tid);
   // 16-byte piece k of row n, quad t of q' (quad order): its place in the row
   auto q_piece = [](int n, int t, int k) {
     const int f = D == 128 ? ((t >> 1) | ((n & 1) << 1)) : (n & 1);
@@ -406,27 +411,28 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
   // m: what scores are taken relative to; finite from the start, so a row
   // without keys needs no case of its own
   float m[NT][2], l[NT][2];
-  int lim[NT][2], lim_min = INT_MAX;
+  float vs = 4194304.f;                                    // scale of the value norms, 2^22 at most
+  int lim_min = INT_MAX;
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       m[n][c] = kNoMax;
       l[n][c] = 0.f;
-      lim[n][c] = row_lim(8 * n + 2 * tq + c);
-      lim_min = min(lim_min, lim[n][c]);
+      lim_min = min(lim_min, lims[8 * n + 2 * tq + c]);
     }
   lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, 1));
   lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, 2));
   const uint32_t k_base = smem_u32(sm) + (F::KQ || HP ? 8 * (lane & 15) : 4 * lane);
   const uint32_t v_base = smem_u32(sm + F::KT) + (F::VQ || HP ? 8 * (lane & 15) : 4 * lane);
+
   int bad_key = INT_MAX;
 
   // one page: `cur` is used, `nxt` takes the next page's codes
   auto step = [&](Tile& cur, Tile& nxt) {
     load_tile(nxt, e_next);
     e_next = e_after;
-    if (warp == 0 && lane == 0 && (unsigned)e_after < (unsigned)nblocks)
+    if (warp == 0 && lane == 0 && (unsigned)e_after < (unsigned)p.nblocks)
       asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;"
                    ::"l"(page_at(p.pages, e_after, p.page_bytes)), "r"(p.page_bytes) : "memory");
     e_after = entry(pg + 3);
@@ -445,7 +451,7 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
       h = in && fin ? h : 0u;
       const __half2 h2 = *reinterpret_cast<const __half2*>(&h);
       kn[i] = __low2float(h2);
-      vn[i] = __high2float(h2);
+      vn[i] = __high2float(h2) * vs;
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
@@ -487,6 +493,8 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
     // relative to m
     float d[NT][4], top = -INFINITY;
     const bool edge = 64 * pg + s0 + 15 > lim_min;
+    // key i of the tile hidden from column c of slice n
+    auto hidden = [&](int n, int i, int c) { return key0 + 8 * i > lims[8 * n + 2 * tq + c]; };
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -496,28 +504,34 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (key0 + 8 * (i >> 1) > lim[n][i & 1]) d[n][i] = -INFINITY;
+          if (hidden(n, i >> 1, i & 1)) d[n][i] = -INFINITY;
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) top = fmaxf(fmaxf(fmaxf(top, d[n][0]), fmaxf(d[n][1], d[n][2])), d[n][3]);
-    if (__any_sync(0xffffffffu, top > (fmaxf(vn[0], vn[1]) > 256.f ? 0.f : kRoom))) {
+    if (__any_sync(0xffffffffu, top > kRoom || fmaxf(vn[0], vn[1]) >= kNorm)) {
+      // the largest norm of the tile, below 2^(e + 1): down to below kNorm
+      const int e = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vn[0], vn[1]))) >> 23) - 127;
+      const float r = __uint_as_float((uint32_t)(127 - max(e - 7, 0)) << 23);
+      vs *= r;
+      vn[0] *= r;
+      vn[1] *= r;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           // the largest score of the column in this tile
-          float x = fmaxf(edge && key0 > lim[n][c] ? -INFINITY : s[n][c] * kn[0],
-                          edge && key0 + 8 > lim[n][c] ? -INFINITY : s[n][2 + c] * kn[1]);
+          const bool out0 = edge && hidden(n, 0, c), out1 = edge && hidden(n, 1, c);
+          float x = fmaxf(out0 ? -INFINITY : s[n][c] * kn[0], out1 ? -INFINITY : s[n][2 + c] * kn[1]);
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
           const float mn = fmaxf(m[n][c], x), f = fast_exp2(m[n][c] - mn);
           l[n][c] *= f;
 #pragma unroll
-          for (int i = 0; i < NC; ++i) { O[i][n][c] *= f; O[i][n][2 + c] *= f; }
+          for (int i = 0; i < NC; ++i) { O[i][n][c] *= f * r; O[i][n][2 + c] *= f * r; }
           m[n][c] = mn;
-          d[n][c] = edge && key0 > lim[n][c] ? -INFINITY : fmaf(s[n][c], kn[0], -mn);
-          d[n][2 + c] = edge && key0 + 8 > lim[n][c] ? -INFINITY : fmaf(s[n][2 + c], kn[1], -mn);
+          d[n][c] = out0 ? -INFINITY : fmaf(s[n][c], kn[0], -mn);
+          d[n][2 + c] = out1 ? -INFINITY : fmaf(s[n][2 + c], kn[1], -mn);
         }
     }
     uint32_t pb[NT][2], pl[HP ? NT : 1][2];
@@ -574,7 +588,7 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
     step(nxt, cur);
     ++pg;
   }
-  if (bad_block) atomicOr(p.status, TQ_DEV_BAD_BLOCK);
+
   if (bad_key != INT_MAX) atomicMin(&flags[1], bad_key);
 
   // ---- the warps' partials: common max, sum in warp order ---------------------------
@@ -600,7 +614,8 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
       float M = mw[col];
 #pragma unroll
       for (int w = 1; w < kW; ++w) M = fmaxf(M, mw[w * NQ + col]);
-      const float f = fast_exp2(m[n][c] - M);
+      // times 1 / vs (exponents: vs is a power of two)
+      const float f = fast_exp2(m[n][c] - M) * __uint_as_float(0x7F000000u - __float_as_uint(vs));
       float* mine = U + (warp * NQ + col) * LDO + gq;
 #pragma unroll
       for (int i = 0; i < NC; ++i) {
@@ -731,26 +746,45 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
   }
 
   // ---- out = (O / l) R ---------------------------------------------------------------
-  for (int i = tid; i < 16 * D / 2; i += kThreads) {
-    const int n = i / (D / 2), w = i % (D / 2);
-    float2 u = make_float2(0.f, 0.f);
-    if (n < NQ && row_valid(n)) {
-      const float x = rowl[n], il = x == 0.f ? 0.f : 1.f / x;
-      u = *reinterpret_cast<const float2*>(U + n * LDO + 2 * w);
-      u.x *= il;
-      u.y *= il;
+  // a warp per row: O / l times the power of two that puts its largest value into
+  // [2^10, 2^11), which the result is divided by
+#pragma unroll
+  for (int n0 = 0; n0 < 16; n0 += kW) {
+    const int n = n0 + warp;
+    float2 u[D / 64];
+    float top = 0.f;
+    const bool valid = n < NQ && row_valid(n);
+    const float x = valid ? rowl[n] : 0.f, il = x == 0.f ? 0.f : 1.f / x;
+#pragma unroll
+    for (int k = 0; k < D / 64; ++k) {
+      u[k] = make_float2(0.f, 0.f);
+      if (valid) u[k] = *reinterpret_cast<const float2*>(U + n * LDO + 2 * (lane + 32 * k));
+      u[k].x *= il;
+      u[k].y *= il;
+      top = fmaxf(top, fmaxf(fabsf(u[k].x), fabsf(u[k].y)));
     }
-    A[n * LDA + w] = split2(u.x, u.y, A[(16 + n) * LDA + w]);
+    // (a row of NaN has none: the maximum leaves NaN out; of zeros neither)
+    const int e = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(top)) >> 23) - 127;
+    const int up = e == 128 ? 0 : min(10 - e, 100);
+    const float s = __uint_as_float((uint32_t)(127 + up) << 23);
+    if (lane == 0) rowl[16 + n] = __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll
+    for (int k = 0; k < D / 64; ++k) {
+      const int w = lane + 32 * k;
+      A[n * LDA + w] = split2(u[k].x * s, u[k].y * s, A[(16 + n) * LDA + w]);
+    }
   }
   cp_async_wait_all();
   __syncthreads();
   int64_t o_at[2];
   bool o_ok[2];
+  float o_inv[2];
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const int n = gq + 8 * r;
     o_ok[r] = n < NQ && row_valid(n);
     o_at[r] = o_ok[r] ? row_at(n, p.os) : 0;
+    o_inv[r] = rowl[16 + n];
   }
   constexpr int NJ = D / 8 / kW;
   // HP: O^hi R^lo first, then the place's other half
@@ -781,13 +815,14 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
     for (int r = 0; r < 2; ++r) {
       if (!o_ok[r]) continue;
       const int64_t o = o_at[r] + (int64_t)(8 * jt + 2 * tq) * p.os[2];
+      const float x = c[2 * r] * o_inv[r], y = c[2 * r + 1] * o_inv[r];
       if (p.o_pair) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(c[2 * r], c[2 * r + 1]);
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
         reinterpret_cast<uint32_t*>(p.out)[o >> 1] =
-            p.o_dtype == TQ_BF16 ? *reinterpret_cast<const uint32_t*>(&h) : pack_half2(c[2 * r], c[2 * r + 1]);
+            p.o_dtype == TQ_BF16 ? *reinterpret_cast<const uint32_t*>(&h) : pack_half2(x, y);
       } else {
-        store_elem(p.out, p.o_dtype, o, c[2 * r]);
-        store_elem(p.out, p.o_dtype, o + p.os[2], c[2 * r + 1]);
+        store_elem(p.out, p.o_dtype, o, x);
+        store_elem(p.out, p.o_dtype, o + p.os[2], y);
       }
     }
   }
@@ -839,6 +874,7 @@ int launch_attend_few(const tq_geom* G, const tq_tables* t, const tq_cache* c,
   const PageGeom g = make_geom(G->head_dim, G->key_bits, G->value_bits, G->qjl);
   p.pages = c->pages;
   p.pm = page_map(c);
+  p.nblocks = p.pm.bt ? (int)p.pm.nblocks : INT_MAX;
   p.page_bytes = g.page_bytes;
   p.off_v = g.off_v;
   p.off_kn = g.off_kn;

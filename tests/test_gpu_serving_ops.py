@@ -942,3 +942,68 @@ def test_attend_ragged_requests_longer_than_their_pages(engine, dtype, causal):
     ops.attend_ragged(tables, ops.PagedPages(pages.pool, pages.block_table[: 3 * H]), q[:5], fits,
                       causal=causal, engine=engine)
     assert ok_status() == 0
+
+
+def value_norms(tables, pool):
+    """The fp16 value norms in a pool's pages (a view)."""
+    at = pool.shape[1] - 128
+    return pool[:, at:].view(F16)
+
+
+SMALL = [(3, 700), (130, 300), (1, 1), (40, 1500), (2, 5000)]
+
+
+@pytest.mark.parametrize("engine,dtype", [(3, BF16), (3, F32), (0, F32)])
+@pytest.mark.parametrize("D,kb,vb,Hq,H", [(128, 4, 2, 8, 2), (128, 3, 3, 20, 1), (64, 2, 4, 3, 3)])
+def test_attend_ragged_scales_with_the_value_norms(D, kb, vb, Hq, H, engine, dtype):
+    """Value norms times a power of two (all of them normal halves before and after) give the result
+    times that power, to the bit: no product ends at fp16's smallest values."""
+    tables = make_tables(D, kb, vb, False)
+    batch, start, _ = make_batch(SMALL)
+    pages = make_paged(tables, len(SMALL) * H, 5000)
+    fill(tables, pages, len(SMALL), H, pages.shape[1] * 64, 71)
+    q = randn((start[-1], Hq, D), 72, dtype)
+    want = ops.attend_ragged(tables, pages, q, batch, engine=engine)
+    norms = value_norms(tables, pages.pool)
+    kept = norms.clone()
+    assert kept[kept > 0].min() >= 4 and kept.max() < 2 ** 7
+    for e in (-16, -9, 5, 9):
+        norms.copy_(kept * 2.0 ** e)
+        got = ops.attend_ragged(tables, pages, q, batch, engine=engine)
+        assert torch.equal(got, want * 2.0 ** e), e
+    assert ok_status() == 0
+
+
+@pytest.mark.parametrize("engine", [0, 3])
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("D,kb,vb,Hq,H", [(128, 4, 2, 8, 2), (128, 3, 3, 20, 1), (64, 2, 4, 3, 3)])
+def test_attend_ragged_results_of_small_and_mixed_value_norms(D, kb, vb, Hq, H, dtype, engine):
+    """fp16 and fp32 results with the bounds of 22-bit operands (2 most 2^-20 + 2^-18, see above)
+    taken of the very terms of each sum, W_i = sum_j |R_ji| sum_t p_t n_t |c_tj|, where the norms of
+    all or some tokens are far below 1 or above it."""
+    tables = make_tables(D, kb, vb, False)
+    batch, start, seq = make_batch(SMALL[:4])
+    R = len(seq)
+    pages = make_paged(tables, R * H, 1500)
+    fill(tables, pages, R, H, pages.shape[1] * 64, 73)
+    tokens = pages.shape[1] * 64
+    q = randn((start[-1], Hq, D), 74, dtype)
+    norms = value_norms(tables, pages.pool)
+    kept = norms.clone()
+    aR = np.abs(tables.rot.cpu().double().numpy())
+    for name, e in (("small", [-13]), ("large", [8]), ("mixed", [-9, 3, -15, -4, -9]), ("zeros", [-30, -10])):
+        e = torch.tensor(e, device=DEV).repeat(64)[:64]
+        norms.copy_(kept * 2.0 ** e)
+        kd, vd = (x.reshape(R, H, -1, D) for x in S.dense(tables, contiguous(pages), tokens))
+        f = S.parse(tables, contiguous(pages), tokens)
+        w = np.abs(tables.v_centroids.cpu().double().numpy())[f["v_idx"]] * f["v_norm"].astype(np.float64)[..., None]
+        want = S.attend(q, kd, vd, start, seq, D ** -0.5, True)
+        terms = S.attend(q, kd, w.reshape(R, H, -1, D), start, seq, D ** -0.5, True) @ aR
+        got = ops.attend_ragged(tables, pages, q, batch, engine=engine).double().cpu().numpy()
+        most = D ** -0.5 * np.linalg.norm(q.double().cpu().numpy(), axis=-1).max() * \
+            np.linalg.norm(kd, axis=-1).max()
+        tol = (2 * most * 2.0 ** -20 + 2.0 ** -18) * terms + S.half_ulp(dtype) * np.abs(want)
+        if dtype == F16:
+            tol = tol + 2.0 ** -25
+        assert (np.abs(got - want) <= tol).all(), (name, (np.abs(got - want) / tol).max())
+    assert ok_status() == 0
