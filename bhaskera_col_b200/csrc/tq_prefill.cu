@@ -26,6 +26,7 @@
 
 #include <limits.h>
 #include <math.h>
+#include <type_traits>
 
 namespace tq {
 namespace {
@@ -108,7 +109,9 @@ __device__ __forceinline__ void frag_b_kn(uint32_t (&r)[4], const __half* base, 
 // RG: a ragged batch (tq_attend_ragged).  A CTA takes one segment of the work
 // list: its request's rows and lengths, key tiles [kt0, kt1) of one block of
 // query positions; a tile cut into several segments leaves partial rows that
-// the tile's last CTA joins.
+// the tile's last CTA joins.  Value norms enter P' times a power of two that puts
+// the largest so far into [2^14, 2^15), and O keeps it through its last rotation:
+// fp16 ends at 2^-24, where a cache's norms need not.
 template <int D, int KB, int VB, bool RG, bool HP>
 __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p) {
   using G = Pf<D, KB, VB, HP>;
@@ -140,14 +143,21 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
   int qb = p.nqb - 1 - (int)blockIdx.x;                // long rows first
   int64_t group = blockIdx.y;                          // (b, kv head, chunk of its query heads)
   __shared__ int bad_key, last_flag;
+  __shared__ int v_exp;                                // RG: value norms are scaled by 2^v_exp
+  __shared__ float o_scale;                            // RG: what that changed by with this page
   if constexpr (RG) {
     if (!take_segment(p.rg, blockIdx.x, sw)) return;
     qb = sw.seg.tile;
     group = sw.seg.req * (p.Hkv * nchunk) + sw.group;
     p.Tq = sw.rq.q_len;
     p.n_tokens = sw.rq.seq;
-    if (threadIdx.x == 0) bad_key = INT_MAX;
+    if (threadIdx.x == 0) {
+      bad_key = INT_MAX;
+      v_exp = 38;
+    }
   }
+  // rows and keys of the request: 32 bits hold a ragged batch's
+  using Pos = typename std::conditional<RG, int, int64_t>::type;
   const int64_t stream = group / nchunk;               // b * Hkv + kv head
   const int chunk = (int)(group % nchunk);
   const int64_t b = stream / p.Hkv, kvh = stream % p.Hkv;
@@ -155,14 +165,14 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
   const int64_t qrow = RG ? sw.rq.q0 * p.qs[2] : b * p.qs[0];
   const int64_t orow = RG ? sw.rq.q0 * p.os[2] : b * p.os[0];
   const int64_t h = kvh * p.g + (int64_t)chunk * p.hc + warp / wph;   // this warp's head
-  const int64_t t_base = RG ? sw.rq.base : p.n_tokens - p.Tq;   // position of query 0
+  const Pos t_base = RG ? (Pos)sw.rq.base : p.n_tokens - p.Tq;     // position of query 0
   const int t0 = qb * P + (warp % wph) * 16;           // this warp's first query
-  const int64_t qpos_max = t_base + tmin<int64_t>((int64_t)(qb + 1) * P, p.Tq) - 1;
+  const Pos qpos_max = t_base + tmin<Pos>((Pos)(qb + 1) * P, p.Tq) - 1;
   // keys this CTA needs
-  const int64_t kend = p.causal ? tmin<int64_t>(qpos_max + 1, p.n_tokens) : p.n_tokens;
+  const Pos kend = !p.causal ? p.n_tokens : RG ? tmin<Pos>(qpos_max + 1, p.n_tokens) : qpos_max + 1;
   const int tile0 = RG ? sw.seg.kt0 : 0;
   const int ntiles = RG ? sw.seg.kt1 - tile0 : (int)((kend + 63) / 64);
-  int64_t kst = 0;                                     // first attended key (left padding)
+  Pos kst = 0;                                         // first attended key (left padding)
   if (p.kv_start) {
     const int v = __ldg(p.kv_start + b);
     kst = v < 0 ? 0 : v;
@@ -271,8 +281,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
 #pragma unroll
   for (int n = 0; n < NT; ++n) O[n][0] = O[n][1] = O[n][2] = O[n][3] = 0.f;
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-  const int64_t qp0 = t_base + t0 + gq, qp1 = qp0 + 8;           // query positions
-  const int64_t warp_kend = p.causal ? tmin<int64_t>(t_base + t0 + 16, p.n_tokens) : p.n_tokens;
+  const Pos qp0 = t_base + t0 + gq, qp1 = qp0 + 8;               // query positions
+  const Pos warp_kend = p.causal ? tmin<Pos>(t_base + t0 + 16, p.n_tokens) : p.n_tokens;
 
   int kt = 0;
   for (; kt < ntiles; ++kt) {
@@ -329,17 +339,45 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
           if constexpr (HP) Vl[tok * G::LD + oct + 8 * c] = lutvl[code];
         }
       }
-      if (tid < 64) {
+      if constexpr (RG) {
+        // warp 0: value norms, warp 1: key norms, two tokens a lane
+        if (warp < 2) {
+          const __half* src = reinterpret_cast<const __half*>(pg + (warp == 0 ? p.off_vn : p.off_kn));
+          float x[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int t = lane + 32 * i;
+            const Pos key = (Pos)(kt + tile0) * 64 + t;
+            x[i] = key < kend ? __half2float(src[t]) : 0.f;
+            // 0 x inf would reach rows that do not see the key: a norm that is not
+            // finite counts as 0 and the rows that see it become NaN at the end
+            if (!isfinite(x[i])) {
+              x[i] = 0.f;
+              atomicMin(&bad_key, (int)key);
+            }
+          }
+          if (warp == 0) {
+            // the page's largest norm, below 2^(e + 1): the scale keeps it below 2^15
+            const int e0 = v_exp;
+            const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(x[0], x[1])));
+            const int e = tmin(e0, 14 - ((int)(top >> 23) - 127));
+            const float scale = __uint_as_float((uint32_t)(127 + e) << 23);
+            x[0] *= scale;
+            x[1] *= scale;
+            if (lane == 0) {
+              o_scale = __uint_as_float((uint32_t)(127 + e - e0) << 23);
+              v_exp = e;
+            }
+          }
+          float* dst = warp == 0 ? vn : kn;
+          dst[lane] = x[0];
+          dst[lane + 32] = x[1];
+        }
+      } else if (tid < 64) {
         const int64_t key = (int64_t)(kt + tile0) * 64 + tid;
         const bool kok = key < kend;
         kn[tid] = kok ? __half2float(reinterpret_cast<const __half*>(pg + p.off_kn)[tid]) : 0.f;
         vn[tid] = kok ? __half2float(reinterpret_cast<const __half*>(pg + p.off_vn)[tid]) : 0.f;
-        // 0 x inf would reach rows that do not see the key: a token whose norm
-        // is not finite counts as 0 and the rows that see it become NaN at the end
-        if (RG && !(isfinite(kn[tid]) && isfinite(vn[tid]))) {
-          kn[tid] = vn[tid] = 0.f;
-          atomicMin(&bad_key, (int)key);
-        }
       }
     }
     __syncthreads();
@@ -350,7 +388,14 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
                &full[st]);
     }
 
-    const int64_t k0 = (int64_t)(kt + tile0) * 64;
+    const Pos k0 = (Pos)(kt + tile0) * 64;
+    if constexpr (RG) {
+      const float f = o_scale;                         // O follows the scale of the value norms
+      if (f != 1.f) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) { O[n][0] *= f; O[n][1] *= f; O[n][2] *= f; O[n][3] *= f; }
+      }
+    }
     if (active && k0 < warp_kend) {
       // ---- S = Q' K^T (16 x 64) -------------------------------------------
       float s[8][4];
@@ -380,7 +425,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const int kl = 8 * n + 2 * tq + c;
-          const int64_t key = k0 + kl;
+          const Pos key = k0 + kl;
           const float nk = kn[kl];
           float v0 = s[n][c] * nk, v1 = s[n][2 + c] * nk;
           const bool lim0 = key < p.n_tokens && key >= kst && (!p.causal || key <= qp0);
@@ -467,7 +512,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
     l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
     float i0 = l0 > 0.f ? 1.f / l0 : 0.f, i1 = l1 > 0.f ? 1.f / l1 : 0.f;
     if constexpr (RG) {
-      const int64_t last = p.n_tokens - 1;
+      const Pos last = p.n_tokens - 1;
       if (l0 != l0 || bad_key <= (p.causal ? tmin(qp0, last) : last)) l0 = i0 = NAN;
       if (l1 != l1 || bad_key <= (p.causal ? tmin(qp1, last) : last)) l1 = i1 = NAN;
     }
@@ -498,6 +543,11 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
           mma_f16_16816(acc[n + 1], a, bf[2], bf[3]);
         }
       }
+    }
+    if constexpr (RG) {
+      const float down = __uint_as_float((uint32_t)(127 - v_exp) << 23);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) { acc[n][0] *= down; acc[n][1] *= down; acc[n][2] *= down; acc[n][3] *= down; }
     }
     const int r0 = t0 + gq, r1 = r0 + 8;
     const int64_t obase = orow + h * p.os[1];

@@ -89,7 +89,7 @@ __device__ __forceinline__ bool take_job(TcPrefillParams& p, int pcta, Job& j) {
   j.orow = RG ? j.sw.rq.q0 * p.os[2] : j.b * p.os[0];
   j.t_base = RG ? j.sw.rq.base : p.n_tokens - p.Tq;
   j.qpos_max = j.t_base + tmin<int64_t>((int64_t)(j.qb + 1) * pcta, p.Tq) - 1;
-  j.kend = p.causal ? tmin<int64_t>(j.qpos_max + 1, p.n_tokens) : p.n_tokens;
+  j.kend = !p.causal ? p.n_tokens : RG ? tmin<int64_t>(j.qpos_max + 1, p.n_tokens) : j.qpos_max + 1;
   j.tile0 = RG ? j.sw.seg.kt0 : 0;
   j.ntiles = RG ? j.sw.seg.kt1 - j.tile0 : (int)((j.kend + kKeys - 1) / kKeys);
   return true;

@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
     const bool valid = id.pos < p.Tq;
     const int64_t qpos = valid ? t_base + id.pos : qpos_max;
     // keys <= lim are seen
-    const int64_t lim = p.causal ? tmin<int64_t>(qpos, p.n_tokens - 1) : p.n_tokens - 1;
+    const int64_t lim = !p.causal ? p.n_tokens - 1 : RG ? tmin<int64_t>(qpos, p.n_tokens - 1) : qpos;
     const int64_t kst = row_kstart(p.kv_start, b);           // keys >= kst are seen
     bool ok = __all_sync(0xffffffffu, wait_or_abort(&bars[B_ROT], 0u, abort_flag, p.status));
     if (ok) {

@@ -30,7 +30,9 @@ __device__ __forceinline__ Request request_at(const RaggedView& v, int64_t r) {
   q.q0 = tmin(tmax<int64_t>(a, 0), v.N);
   q.q_len = tmax<int64_t>(tmin(b, v.N) - q.q0, 0);
   q.seq = tmin(tmax<int64_t>(s, 0), v.cap);
-  q.base = tmax<int64_t>(s, 0) - q.q_len;   // of the length as it is: rows keep their places
+  // of the length as it is, so that rows keep their places (from 2^30 - 64 on, where no
+  // pages reach, all places are one: sums with rows stay within 32 bits)
+  q.base = tmin<int64_t>(tmax<int64_t>(s, 0) - q.q_len, (1 << 30) - 64);
   return q;
 }
 

@@ -953,11 +953,14 @@ def value_norms(tables, pool):
 SMALL = [(3, 700), (130, 300), (1, 1), (40, 1500), (2, 5000)]
 
 
-@pytest.mark.parametrize("engine,dtype", [(3, BF16), (3, F32), (0, F32)])
-@pytest.mark.parametrize("D,kb,vb,Hq,H", [(128, 4, 2, 8, 2), (128, 3, 3, 20, 1), (64, 2, 4, 3, 3)])
+@pytest.mark.parametrize("engine,dtype", [(3, BF16), (3, F32), (0, F32), (1, BF16), (1, F32)])
+@pytest.mark.parametrize("D,kb,vb,Hq,H", [(128, 4, 2, 8, 2), (128, 3, 3, 20, 1), (64, 2, 4, 3, 3),
+                                          (64, 6, 6, 4, 2)])
 def test_attend_ragged_scales_with_the_value_norms(D, kb, vb, Hq, H, engine, dtype):
     """Value norms times a power of two (all of them normal halves before and after) give the result
     times that power, to the bit: no product ends at fp16's smallest values."""
+    if engine == 3 and kb > 4 or engine == 1 and (kb, vb) == (2, 4):
+        pytest.skip("no such kernel")
     tables = make_tables(D, kb, vb, False)
     batch, start, _ = make_batch(SMALL)
     pages = make_paged(tables, len(SMALL) * H, 5000)
@@ -974,13 +977,16 @@ def test_attend_ragged_scales_with_the_value_norms(D, kb, vb, Hq, H, engine, dty
     assert ok_status() == 0
 
 
-@pytest.mark.parametrize("engine", [0, 3])
+@pytest.mark.parametrize("engine", [0, 1, 3])
 @pytest.mark.parametrize("dtype", [F16, F32])
-@pytest.mark.parametrize("D,kb,vb,Hq,H", [(128, 4, 2, 8, 2), (128, 3, 3, 20, 1), (64, 2, 4, 3, 3)])
+@pytest.mark.parametrize("D,kb,vb,Hq,H", [(128, 4, 2, 8, 2), (128, 3, 3, 20, 1), (64, 2, 4, 3, 3),
+                                          (128, 6, 6, 4, 2), (64, 5, 5, 4, 2)])
 def test_attend_ragged_results_of_small_and_mixed_value_norms(D, kb, vb, Hq, H, dtype, engine):
     """fp16 and fp32 results with the bounds of 22-bit operands (2 most 2^-20 + 2^-18, see above)
     taken of the very terms of each sum, W_i = sum_j |R_ji| sum_t p_t n_t |c_tj|, where the norms of
     all or some tokens are far below 1 or above it."""
+    if engine == 3 and kb > 4 or engine == 1 and (kb, vb) == (2, 4):
+        pytest.skip("no such kernel")
     tables = make_tables(D, kb, vb, False)
     batch, start, seq = make_batch(SMALL[:4])
     R = len(seq)
