@@ -18,6 +18,7 @@
 
 #include <limits.h>
 #include <math.h>
+#include <type_traits>
 
 namespace tq {
 namespace pftc {
@@ -59,18 +60,21 @@ struct TcPrefillParams {
 
 // What one CTA works on: a block of query positions of one head group, over
 // key tiles [tile0, tile0 + ntiles).
+template <bool RG>
 struct Job {
+  using Pos = typename std::conditional<RG, int, int64_t>::type;   // 32 bits hold a ragged batch's
   int qb, chunk, tile0, ntiles;
   int64_t stream, kvh, b;
   int64_t qrow, orow;           // element offsets of the batch row's first query row
-  int64_t t_base, qpos_max, kend;
+  Pos t_base, qpos_max, kend;
   SegWork sw;                   // RG: the segment
 };
 
 // The whole batch row of blockIdx.y, or (RG) one segment of the ragged work
 // list, whose lengths replace p's.  false: nothing for this CTA.
 template <bool RG>
-__device__ __forceinline__ bool take_job(TcPrefillParams& p, int pcta, Job& j) {
+__device__ __forceinline__ bool take_job(TcPrefillParams& p, int pcta, Job<RG>& j) {
+  using Pos = typename Job<RG>::Pos;
   const int nchunk = (int)(p.g / p.hc);
   int64_t group = blockIdx.y;
   j.qb = p.nqb - 1 - (int)blockIdx.x;                  // long rows first
@@ -78,8 +82,8 @@ __device__ __forceinline__ bool take_job(TcPrefillParams& p, int pcta, Job& j) {
     if (!take_segment(p.rg, blockIdx.x, j.sw)) return false;
     j.qb = j.sw.seg.tile;
     group = j.sw.seg.req * (p.Hkv * nchunk) + j.sw.group;
-    p.Tq = j.sw.rq.q_len;
-    p.n_tokens = j.sw.rq.seq;
+    p.Tq = (Pos)j.sw.rq.q_len;
+    p.n_tokens = (Pos)j.sw.rq.seq;
   }
   j.stream = group / nchunk;
   j.chunk = (int)(group % nchunk);
@@ -87,9 +91,9 @@ __device__ __forceinline__ bool take_job(TcPrefillParams& p, int pcta, Job& j) {
   j.kvh = j.stream % p.Hkv;
   j.qrow = RG ? j.sw.rq.q0 * p.qs[2] : j.b * p.qs[0];
   j.orow = RG ? j.sw.rq.q0 * p.os[2] : j.b * p.os[0];
-  j.t_base = RG ? j.sw.rq.base : p.n_tokens - p.Tq;
-  j.qpos_max = j.t_base + tmin<int64_t>((int64_t)(j.qb + 1) * pcta, p.Tq) - 1;
-  j.kend = !p.causal ? p.n_tokens : RG ? tmin<int64_t>(j.qpos_max + 1, p.n_tokens) : j.qpos_max + 1;
+  j.t_base = RG ? (Pos)j.sw.rq.base : p.n_tokens - p.Tq;
+  j.qpos_max = j.t_base + tmin<Pos>((Pos)(j.qb + 1) * pcta, p.Tq) - 1;
+  j.kend = !p.causal ? p.n_tokens : RG ? tmin<Pos>(j.qpos_max + 1, p.n_tokens) : j.qpos_max + 1;
   j.tile0 = RG ? j.sw.seg.kt0 : 0;
   j.ntiles = RG ? j.sw.seg.kt1 - j.tile0 : (int)((j.kend + kKeys - 1) / kKeys);
   return true;
@@ -358,10 +362,11 @@ struct HalfRegs {
 };
 
 // RG: a norm that is not finite counts as 0 (0 x inf would reach the rows of
-// the tile that do not see the key) and its key is noted.
+// the tile that do not see the key) and its key is noted; norms come times
+// `scale`, a power of two.
 template <int NB, int NR, bool RG = false>
 __device__ __forceinline__ void load_half(HalfRegs<NB, NR>& t, const TcParamsView& pv, int jj,
-                                          int off_codes, int off_norm) {
+                                          int off_codes, int off_norm, float scale = 1.f) {
   constexpr int RPP = NR / 2, STEP = 64 / RPP;
   const int j = RG ? jj + pv.tile0 : jj;
   const uint8_t* pgs[2];
@@ -387,6 +392,10 @@ __device__ __forceinline__ void load_half(HalfRegs<NB, NR>& t, const TcParamsVie
       if (RG && (t.n[r] & 0x7C00u) == 0x7C00u) {
         t.n[r] = 0u;
         atomicMin(pv.bad_key, (int)key);
+      }
+      if (RG) {
+        const float n = __half2float(__ushort_as_half((unsigned short)t.n[r])) * scale;
+        t.n[r] = __half_as_ushort(__float2half_rn(n));
       }
     } else {
 #pragma unroll

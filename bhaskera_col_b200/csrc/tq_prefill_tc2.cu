@@ -30,7 +30,10 @@
 // / q'_B, O^_A hi / lo the K stages and O^_B hi / lo the V stages.
 //
 // RG: a ragged batch (tq_attend_ragged); a CTA takes one segment of the work
-// list and leaves partial rows where the tile has several.
+// list and leaves partial rows where the tile has several.  V^ is fp16, which ends
+// at 2^-24 where a cache's norms need not: the CTA first looks through its keys'
+// value norms (2 of every 130 bytes at 4 bits) and takes them times the power of two
+// that puts the largest into [2^10, 2^11); results are divided by it.
 //
 // Every wait is bounded; on expiry the kernel sets TQ_DEV_WAIT_TIMEOUT in the
 // status word, the other roles see the abort flag, no MMA is left in flight
@@ -90,14 +93,17 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + OFF_BAR);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + B_COUNT);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + B_COUNT + 1);
-  int* flags = reinterpret_cast<int*>(bars + B_COUNT + 2);   // RG: last CTA, first bad key
+  // RG: last CTA, first bad key, then each warp's largest value norm
+  int* flags = reinterpret_cast<int*>(bars + B_COUNT + 2);
+  static_assert(8 * (B_COUNT + 2) + 4 * (2 + kWarps) <= 256, "room behind the barriers");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  Job jb;
+  using Pos = typename Job<RG>::Pos;
+  Job<RG> jb;
   if (!take_job<RG>(p, p.pcta, jb)) return;
   const int qb = jb.qb, chunk = jb.chunk, ntiles = jb.ntiles;
-  const int64_t stream = jb.stream, b = jb.b, kvh = jb.kvh, t_base = jb.t_base;
-  const int64_t qpos_max = jb.qpos_max, kend = jb.kend;
+  const int64_t stream = jb.stream, b = jb.b, kvh = jb.kvh;
+  const Pos t_base = jb.t_base, qpos_max = jb.qpos_max, kend = jb.kend;
   // output offset of the CTA's row (tile A's 128 rows, then tile B's), or -1
   auto row_out = [&](int row) -> int64_t {
     const RowId id = row_id(p, qb, row >> 7, row & 127);
@@ -132,6 +138,29 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
   if (warp == 0) {
     tc::tmem_alloc(tmem_slot, kTmemCols);
     tc::tmem_relinquish();
+  }
+
+  if constexpr (RG) {
+    // the warp's pages, kWarps apart: table entries first, 32 at once
+    const int end = (tmin<int>(kend, (jb.tile0 + ntiles) * kKeys) + 63) >> 6;
+    unsigned top = 0;
+    for (int p0 = 2 * jb.tile0 + warp; p0 < end; p0 += 32 * kWarps) {
+      int64_t slot = 0;
+      bool inside;                         // (the decoders flag pages outside the pool)
+      if (p0 + lane * kWarps < end) slot = page_slot(p.pm, stream, p0 + lane * kWarps, inside);
+#pragma unroll 8
+      for (int i = 0; i < 32; ++i) {
+        const int pg = p0 + i * kWarps;
+        if (pg >= end) break;
+        const uint8_t* page = p.pages + __shfl_sync(0xffffffffu, slot, i) * (int64_t)p.page_bytes;
+        const uint32_t h = __ldg(reinterpret_cast<const uint32_t*>(page + p.off_vn) + lane);
+        const unsigned a = h & 0x7FFFu, b = (h >> 16) & 0x7FFFu;
+        if (64 * pg + 2 * lane < kend && a < 0x7C00u) top = tmax(top, a);
+        if (64 * pg + 2 * lane + 1 < kend && b < 0x7C00u) top = tmax(top, b);
+      }
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) flags[2 + warp] = (int)top;
   }
 
   // ---- setup: Q rows (softmax groups), R_K and the pair tables (decoders) ----
@@ -202,6 +231,13 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+
+  // exponent of the largest norm (1 for fp16's subnormals): it lies below 2^(ve - 14)
+  int ve = 1;
+  if constexpr (RG) {
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) ve = tmax(ve, flags[2 + w] >> 10);
+  }
 
   constexpr uint32_t idesc_kk = tc::idesc_f16_f32(128, 128);                 // A, B K-major
   constexpr uint32_t idesc_kmn = tc::idesc_f16_f32(128, 128) | (1u << 16);    // B MN-major
@@ -303,10 +339,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
     const uint32_t ocol = tl + 256 + 128 * X;           // O_X
     const RowId id = row_id(p, qb, X, rr);
     const bool valid = id.pos < p.Tq;
-    const int64_t qpos = valid ? t_base + id.pos : qpos_max;
+    const Pos qpos = valid ? t_base + id.pos : qpos_max;
     // keys <= lim are seen
-    const int64_t lim = !p.causal ? p.n_tokens - 1 : RG ? tmin<int64_t>(qpos, p.n_tokens - 1) : qpos;
-    const int64_t kst = row_kstart(p.kv_start, b);           // keys >= kst are seen
+    const Pos lim = !p.causal ? p.n_tokens - 1 : RG ? tmin<Pos>(qpos, p.n_tokens - 1) : qpos;
+    const Pos kst = RG ? 0 : row_kstart(p.kv_start, b);      // keys >= kst are seen
     bool ok = __all_sync(0xffffffffu, wait_or_abort(&bars[B_ROT], 0u, abort_flag, p.status));
     if (ok) {
       // q'_X (fp32, K order) -> fp16 A operand over Q_X
@@ -337,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
                                                  abort_flag, p.status));
       if (!ok) break;
       tc::tc_fence_after();
-      const int64_t k0 = (int64_t)(j + jb.tile0) * kKeys;
+      const Pos k0 = (Pos)(j + jb.tile0) * kKeys;
       const bool need_mask = k0 + kKeys - 1 > lim || k0 < kst;
       // pass 1: row max (four independent 3-input chains)
       float mx;
@@ -465,6 +501,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
         tc::tmem_ld_x32(scol + 32 * c, x);
         tmem_ld_wait(x);
         if (!valid) continue;
+        if constexpr (RG) {
+          const float down = __uint_as_float((uint32_t)(127 + ve - 25) << 23);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * down);
+        }
         if (split) {
           uint4* dst = reinterpret_cast<uint4*>(p.rg.plan.part + pr * kD) + 8 * c;
 #pragma unroll
@@ -521,9 +562,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
     }
     pv.kend = kend;
     pv.W = RG ? 0 : p.W;
-    pv.kpacked = p.n_tokens - pv.W;
+    pv.kpacked = RG ? kend : p.n_tokens - pv.W;
     pv.tile0 = jb.tile0;
     pv.bad_key = flags + 1;
+    const float v_scale = __uint_as_float((uint32_t)(127 + 25 - ve) << 23);
     const unsigned char* lk = sm + OFF_LUT + 4 * (lane & (p.rk - 1));
     const unsigned char* lv = sm + OFF_LUT + 4 * nk * p.rk + 4 * (lane & (p.rv - 1));
     const int rk4 = 4 * p.rk, rv4 = 4 * p.rv;
@@ -538,10 +580,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
     __syncwarp();
     if (lane == 0) tc::mbar_arrive_cta(&bars[B_KFULL]);
     if (ntiles > 1) load_half<KB, 2, RG>(kc, pv, 1, 0, p.off_kn);
-    load_half<VB, 2, RG>(vc, pv, 0, p.off_v, p.off_vn);
+    load_half<VB, 2, RG>(vc, pv, 0, p.off_v, p.off_vn, v_scale);
     for (int j = 0; j < ntiles; ++j) {
       if (j + 2 < ntiles) load_half<KB, 2, RG>(kn, pv, j + 2, 0, p.off_kn);
-      if (j + 1 < ntiles) load_half<VB, 2, RG>(vn, pv, j + 1, p.off_v, p.off_vn);
+      if (j + 1 < ntiles) load_half<VB, 2, RG>(vn, pv, j + 1, p.off_v, p.off_vn, v_scale);
       if (j + 1 < ntiles) {
         // K^ of tile j + 1: both S MMAs of tile j - 1 have read this stage
         const int jk = j + 1, sk = jk & 1;

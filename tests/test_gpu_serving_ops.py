@@ -953,13 +953,14 @@ def value_norms(tables, pool):
 SMALL = [(3, 700), (130, 300), (1, 1), (40, 1500), (2, 5000)]
 
 
-@pytest.mark.parametrize("engine,dtype", [(3, BF16), (3, F32), (0, F32), (1, BF16), (1, F32)])
+@pytest.mark.parametrize("engine,dtype", [(3, BF16), (3, F32), (0, F32), (1, BF16), (1, F32), (2, BF16),
+                                          (2, F32), (0, BF16)])
 @pytest.mark.parametrize("D,kb,vb,Hq,H", [(128, 4, 2, 8, 2), (128, 3, 3, 20, 1), (64, 2, 4, 3, 3),
                                           (64, 6, 6, 4, 2)])
 def test_attend_ragged_scales_with_the_value_norms(D, kb, vb, Hq, H, engine, dtype):
     """Value norms times a power of two (all of them normal halves before and after) give the result
     times that power, to the bit: no product ends at fp16's smallest values."""
-    if engine == 3 and kb > 4 or engine == 1 and (kb, vb) == (2, 4):
+    if engine == 3 and kb > 4 or engine == 1 and (kb, vb) == (2, 4) or engine == 2 and D != 128:
         pytest.skip("no such kernel")
     tables = make_tables(D, kb, vb, False)
     batch, start, _ = make_batch(SMALL)
