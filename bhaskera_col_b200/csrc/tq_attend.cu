@@ -244,6 +244,7 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p0
   __shared__ unsigned place[kClasses + 1];                 // segments per class, then their next place
   __shared__ unsigned slots;
   const int tid = threadIdx.x, lane = tid & 31;
+  const OffsetCheck offsets(p.rv, tid);
   const Tiles own = listed_request(p, tid);
   for (int i = tid; i < p.max_slot * p.G; i += kPlanThreads) p.arrived[i] = 0;
   if (tid == 0) {
@@ -252,7 +253,10 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p0
     *p.next = 0;
   }
   if (tid <= kClasses) place[tid] = 0;
-  __syncthreads();
+  if (__syncthreads_or(offsets.fails(p.rv, tid, kPlanThreads, p.status))) {
+    if (tid == 0) *p.nseg = 0;
+    return;
+  }
   unsigned long long mine = 0;
   for_tiles(p, own, [&](int, int, int nkt) { mine += nkt + kOneTile; });
 #pragma unroll
@@ -273,8 +277,8 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p0
   });
   __syncthreads();
   if (tid < 32) {
-    // exclusive sums of the classes; the bounds of the list hold for ascending
-    // offsets, and a batch that breaks them is not run
+    // exclusive sums of the classes; the bounds of the list hold for offsets that
+    // ascend and stay as they were read
     const unsigned own = place[lane];
     unsigned x = own;
 #pragma unroll

@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kThreadsR) append_ragged_kernel(RaggedKV p) {
   for (int i = tid; i < nb; i += kThreadsR) bb[i] = p.bnd[which][i];
   if (which == 0) build_orders(ord, nullptr, nullptr, D, tid, kThreadsR);
   else build_orders(nullptr, ord, nullptr, D, tid, kThreadsR);
-  __syncthreads();
+  if (__syncthreads_or(OffsetCheck(p.rv, tid).fails(p.rv, tid, kThreadsR, p.status))) return;
   const int rowbytes = which == 0 ? g.krow : g.vrow;
   const int sec = which == 0 ? g.off_k : g.off_v, nsec = which == 0 ? g.off_kn : g.off_vn;
   const int64_t nvec = p.rv.N * p.H;
@@ -174,6 +174,7 @@ __global__ void __launch_bounds__(kThreadsR) read_ragged_kernel(RaggedKV p) {
   const int sec = which == 0 ? g.off_k : g.off_v, nsec = which == 0 ? g.off_kn : g.off_vn;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t nvec = p.rv.N * p.H;
+  if (__syncthreads_or(OffsetCheck(p.rv, tid).fails(p.rv, tid, kThreadsR, p.status))) return;
   for (int64_t v0 = (int64_t)blockIdx.x * kVecs; v0 < nvec; v0 += (int64_t)gridDim.x * kVecs) {
     const int nv = (int)tmin<int64_t>(kVecs, nvec - v0);
     for (int v = warp; v < nv; v += kThreadsR / 32) {

@@ -22,6 +22,29 @@ struct Request {
   int64_t base;               // position of the first row
 };
 
+// Do the offsets ascend within [0, N]?  Thread tid of n looks at every n-th request;
+// whoever sees one that does not sets TQ_DEV_BAD_BATCH, and the block agrees not to
+// run.  The first request's offsets are loaded when the check is made, so that other
+// loads hide their way (0.5 us of a launch of few tokens).
+struct OffsetCheck {
+  int a, b;
+  __device__ __forceinline__ OffsetCheck(const RaggedView& v, int tid) : a(0), b(0) {
+    if (tid < v.R) {
+      a = __ldg(v.q_start + tid);
+      b = __ldg(v.q_start + tid + 1);
+    }
+  }
+  __device__ __forceinline__ bool fails(const RaggedView& v, int tid, int n, uint32_t* status) const {
+    bool bad = a < 0 || a > b || b > v.N;
+    for (int64_t r = (int64_t)tid + n; r < v.R; r += n) {
+      const int c = __ldg(v.q_start + r), d = __ldg(v.q_start + r + 1);
+      bad = bad || c < 0 || c > d || d > v.N;
+    }
+    if (bad) atomicOr(status, TQ_DEV_BAD_BATCH);
+    return bad;
+  }
+};
+
 // Request r, with offsets outside the tensors cut to them: a wrong offset
 // never leads outside memory.
 __device__ __forceinline__ Request request_at(const RaggedView& v, int64_t r) {

@@ -501,6 +501,7 @@ append_ragged_tc_kernel(const __grid_constant__ RaggedTc p, int which) {
   // the V kernel may start beside the K kernel (they share no byte); it ends
   // after it, so that whatever follows sees both
   pdl_launch_dependents();
+  const OffsetCheck offsets(p.rv, tid);
   if (tid == 0) init_pipe(pp, kMakers, W::kEpi);
   if (warp == W::kIssuer) {
     tc::tmem_alloc(pp.tmem_slot, 2 * D);
@@ -517,7 +518,7 @@ append_ragged_tc_kernel(const __grid_constant__ RaggedTc p, int which) {
   stage_rotation<D, kThreads>(sm + SM::OFF_B, p.rot, which, tid);
   tc::fence_proxy_async_smem();
   tc::tc_fence_before();
-  __syncthreads();
+  const bool run = !__syncthreads_or(offsets.fails(p.rv, tid, kThreads, p.status));
   // the locators need no more; the others agree on the lookup table
   const bool locator = warp >= W::kLocators && warp < W::kEpi0;
   auto others_sync = [&] {
@@ -556,7 +557,7 @@ append_ragged_tc_kernel(const __grid_constant__ RaggedTc p, int which) {
     tc::tc_fence_after();
   }
   const uint32_t tmem = *pp.tmem_slot;
-  const int first = blockIdx.x, step = gridDim.x;
+  const int first = run ? blockIdx.x : p.ntiles, step = gridDim.x;
   const bool use_lo = p.use_lo[which] != 0;
 
   if (warp < kMakers) {
@@ -927,6 +928,7 @@ read_ragged_tc_kernel(RaggedTc p, int which) {
   // the V kernel may start beside the K kernel (they share no byte); it ends
   // after it, so that whatever follows sees both
   pdl_launch_dependents();
+  const OffsetCheck offsets(p.rv, tid);
   if (tid == 0) init_pipe(pp, kMakers, W::kEpi);
   if (warp == W::kIssuer) {
     tc::tmem_alloc(pp.tmem_slot, 2 * D);
@@ -952,10 +954,10 @@ read_ragged_tc_kernel(RaggedTc p, int which) {
   }
   tc::fence_proxy_async_smem();
   tc::tc_fence_before();
-  __syncthreads();
+  const bool run = !__syncthreads_or(offsets.fails(p.rv, tid, kThreads, p.status));
   tc::tc_fence_after();
   const uint32_t tmem = *pp.tmem_slot;
-  const int first = blockIdx.x, step = gridDim.x;
+  const int first = run ? blockIdx.x : p.ntiles, step = gridDim.x;
   const int row_bytes = D * BITS / 8;
   const int sec = which == 0 ? p.g.off_k : p.g.off_v, noff = which == 0 ? p.g.off_kn : p.g.off_vn;
 

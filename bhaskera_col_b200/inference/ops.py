@@ -533,7 +533,8 @@ class RaggedBatch(_Described):
     (q_start[r + 1] - q_start[r]) + i; seq_lens counts the new tokens.  Both
     stay on the device; ``max_q_len`` (>= the most new tokens of a request)
     shapes launches and never a result.  Rows outside [q_start[0],
-    q_start[-1]) belong to no request and are left alone."""
+    q_start[-1]) belong to no request and are left alone.  Offsets that do not
+    ascend within the rows run nothing and set _lib.DEV_BAD_BATCH."""
     q_start: torch.Tensor       # int32 (R + 1,), ascending
     seq_lens: torch.Tensor      # int32 (R,)
     max_q_len: int

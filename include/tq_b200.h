@@ -66,7 +66,7 @@ extern "C" {
 #define TQ_DEV_BAD_POSITION 4u  /* a position outside the rotation table or, in
                                    a ragged batch, outside the pages          */
 #define TQ_DEV_BAD_BATCH 8u     /* a ragged batch's row offsets do not ascend
-                                   within the tensor's rows                   */
+                                   within the tensor's rows: nothing was run  */
 
 typedef struct tq_geom {
   int32_t head_dim;    /* D: multiple of 32, 32..256                        */
@@ -391,7 +391,9 @@ int32_t tq_qk_rope(const tq_rope* rope, const tq_positions* pos, const tq_tensor
  * request r's new tokens, at position seq_lens[r] - (q_start[r+1] -
  * q_start[r]) + i of the request.  Rows outside [q_start[0],
  * q_start[requests]) belong to no request: they are neither read nor
- * written.  Request r's pages are those of streams r * Hkv + h. */
+ * written.  Request r's pages are those of streams r * Hkv + h.  The offsets
+ * ascend from 0 at least to N at most; a batch whose offsets do not is not run
+ * (nothing is stored or written) and sets TQ_DEV_BAD_BATCH. */
 typedef struct tq_ragged {
   int64_t requests;           /* R                                            */
   const int32_t* q_start;     /* device [R + 1], ascending                    */

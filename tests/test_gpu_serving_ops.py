@@ -1014,3 +1014,31 @@ def test_attend_ragged_results_of_small_and_mixed_value_norms(D, kb, vb, Hq, H, 
             tol = tol + 2.0 ** -25
         assert (np.abs(got - want) <= tol).all(), (name, (np.abs(got - want) / tol).max())
     assert ok_status() == 0
+
+
+@pytest.mark.parametrize("start", [
+    [0, 4, 2, 6], [0, 5, 5, 4], [-1, 2, 3, 6], [0, 2, 3, 9], [3, 2, 1, 0], [-5, 90, 1 << 30, -(1 << 31)],
+    [0, 1] * 300 + [6], [0, 4] * 750 + [6], list(range(0, 7)) + [6] * 1200 + [7]])
+@pytest.mark.parametrize("D,kb,vb", [(128, 4, 2), (96, 4, 4)])
+def test_offsets_that_do_not_ascend_run_nothing(D, kb, vb, start):
+    """Descending, negative and too large offsets, in batches of few and of many requests: flagged by
+    every operator, and nothing is stored or written."""
+    R, H, n = len(start) - 1, 1, 6
+    tables = make_tables(D, kb, vb, False)
+    batch = ops.RaggedBatch(int32(start), int32([64] * R), 4)
+    pages = make_paged(tables, R * H, 64)
+    fill(tables, pages, R, H, 64, 1)
+    kept = pages.pool.clone()
+    x = randn((n, H, D), 2)
+    ops.append_ragged(tables, pages, x, x, batch)
+    assert ok_status() == _lib.DEV_BAD_BATCH and torch.equal(pages.pool, kept)
+    out = [torch.full((n, H, D), 7.0, dtype=BF16, device=DEV) for _ in range(2)]
+    ops.dequantize_ragged(tables, pages, batch, *out)
+    assert ok_status() == _lib.DEV_BAD_BATCH and all((o == 7).all() for o in out)
+    if D != 96:
+        for engine in (0, 1, 2, 3):
+            ops.attend_ragged(tables, pages, x, batch, out=out[0], engine=engine)
+            assert ok_status() == _lib.DEV_BAD_BATCH and (out[0] == 7).all()
+    good = ops.RaggedBatch(int32([0] * R + [n]), int32([64] * R), n)
+    ops.append_ragged(tables, pages, x, x, good)
+    assert ok_status() == 0 and not torch.equal(pages.pool, kept)
