@@ -763,8 +763,9 @@ int32_t tq_attend_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c
   if ((rc = check_attend(g, c, a, fn)) || (rc = check_tables(g, t, fn))) return rc;
   if ((rc = check_written(a->out, "out", fn)) || (rc = check_alias(a->q, a->out, "out", fn)))
     return rc;
-  if (!t->rot_f16 || reinterpret_cast<uintptr_t>(t->rot_f16) % 16) {
-    set_error("%s: tables.rot_f16 (R as fp16, 16-byte aligned) is required", fn);
+  if (!t->rot_f16 ||
+      (reinterpret_cast<uintptr_t>(t->rot_f16) | reinterpret_cast<uintptr_t>(t->rot)) % 16) {
+    set_error("%s: tables.rot_f16 (R as fp16) is required, and it and tables.rot 16-byte aligned", fn);
     return TQ_ERR_INVALID;
   }
   if (!(a->scale > 0.f)) { set_error("%s: scale must be positive", fn); return TQ_ERR_INVALID; }

@@ -65,6 +65,8 @@ class LayerTables:
 
     def __post_init__(self):
         self.rot = self.rot.contiguous().float()
+        if self.rot.data_ptr() % 16:                     # a slice of something larger
+            self.rot = self.rot.clone()
         self.rot_t = self.rot.t().contiguous()
         self.rot_f16 = self.rot.half().contiguous()      # prefill attention
         if self.head_dim == 128:

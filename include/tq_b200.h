@@ -81,7 +81,8 @@ typedef struct tq_tables {
   const float* k_boundaries;  /* [2^kb - 1], ascending                       */
   const float* v_centroids;   /* [2^vb]                                      */
   const float* v_boundaries;  /* [2^vb - 1]                                  */
-  const float* rot;           /* R [D][D] row-major; y = x R^T               */
+  const float* rot;           /* R [D][D] row-major; y = x R^T (16-byte aligned
+                                 for tq_attend_ragged)                      */
   const float* qjl;           /* S [D][D] row-major (NULL when qjl == 0)     */
   const float* rot_t;         /* R^T [D][D] row-major                        */
   const float* qjl_t;         /* S^T [D][D] row-major (NULL when qjl == 0)   */
@@ -92,7 +93,8 @@ typedef struct tq_tables {
    * tq_append runs the rotation of bf16 inputs on the tensor cores; NULL
    * keeps every append on the CUDA-core kernel. */
   const uint16_t* rot_bf16x3;
-  /* R [D][D] fp16, row-major: required by tq_prefill_attn, unused elsewhere. */
+  /* R [D][D] fp16, row-major, 16-byte aligned: required by tq_prefill_attn and
+   * tq_attend_ragged, unused elsewhere. */
   const uint16_t* rot_f16;
   /* Optional, head_dim 128 with qjl only: S in bf16, [D][D], rows and columns
    * in K quad order ([p][c] = S[k_order[p]][k_order[c]]).  Set only when every

@@ -434,3 +434,18 @@ def test_attend_workspace_query_accepts_what_the_call_does(dtype, engine):
     rc, _, need = attend(g=geom(kb=5, vb=4), q=t4((1, 4, 10, 128), dtype=dtype),
                          out=far((1, 4, 10, 128), dtype=dtype), engine=engine, nbytes=0)
     assert (need > 0) == (engine < 3)
+
+
+def test_attend_needs_an_aligned_rotation():
+    """The rotation is read in pieces of up to 16 bytes; a table that LayerTables is given anywhere in
+    memory is moved to where that holds."""
+    for dtype in (_lib.TQ_BF16, _lib.TQ_F32):
+        t = _lib.Tables(*([4096] * 4), 4100, *([4096] * 6))
+        rc, err, need = attend(t=t, q=t4((1, 4, 10, 128), dtype=dtype), out=far((1, 4, 10, 128), dtype=dtype),
+                               nbytes=0)
+        assert rc == _lib.TQ_ERR_INVALID and "rot" in err and need > 0
+    z = lambda *n: torch.zeros(n)  # noqa: E731
+    R = torch.arange(128.0 * 128 + 3)[3:].view(128, 128)
+    assert R.data_ptr() % 16
+    t = ops.LayerTables(128, 4, 2, False, z(16), z(15), z(4), z(3), R)
+    assert t.rot.data_ptr() % 16 == 0 and torch.equal(t.rot, R) and torch.equal(t.rot_t, R.t())
