@@ -3,6 +3,7 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <initializer_list>
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -541,32 +542,69 @@ static int check_written(const tq_tensor4* x, const char* what, const char* fn) 
   return TQ_OK;
 }
 
-static void extent(const tq_tensor4* x, const char*& lo, const char*& hi) {
-  const int64_t es = x->dtype == TQ_F32 ? 4 : 2;
-  lo = hi = static_cast<const char*>(x->data);
-  for (int i = 0; i < 4; ++i) {
-    const int64_t d = (x->shape[i] - 1) * x->stride[i] * es;
-    if (d < 0) lo += d; else hi += d;
+// A view in bytes: base and (stride, count) of its dims, broadcast ones left out.
+struct Span {
+  int64_t base, size;                      // size: of an element
+  std::pair<int64_t, int64_t> dim[4];
+  int dims;
+
+  explicit Span(const tq_tensor4* x)
+      : base((int64_t)reinterpret_cast<intptr_t>(x->data)), size(x->dtype == TQ_F32 ? 4 : 2), dims(0) {
+    for (int i = 0; i < 4; ++i)
+      if (x->shape[i] > 1 && x->stride[i] != 0) dim[dims++] = {x->stride[i] * size, x->shape[i]};
   }
-  hi += es;
+  int64_t width() const {
+    int64_t w = size;
+    for (int i = 0; i < dims; ++i) w += (dim[i].second - 1) * dim[i].first;
+    return w;
+  }
+  // the view without its dim of that stride
+  Span inner(int64_t stride) const {
+    Span s = *this;
+    s.dims = 0;
+    for (int i = 0; i < dims; ++i)
+      if (dim[i].first != stride) s.dim[s.dims++] = dim[i];
+    return s;
+  }
+};
+
+// True only if no byte belongs to both.  Views that repeat with the same largest
+// stride (rows of one buffer) are apart if their parts of one period are: x's lie
+// in [0, S) of each, y's d further on.
+static bool apart(Span x, Span y) {
+  int64_t S = 0;
+  for (const Span* s : {&x, &y})
+    for (int i = 0; i < s->dims; ++i) {
+      if (s->dim[i].first < 0) return false;
+      S = s->dim[i].first > S ? s->dim[i].first : S;
+    }
+  if (x.base + x.width() <= y.base || y.base + y.width() <= x.base) return true;
+  if (S == 0) return false;
+  Span a = x.inner(S), b = y.inner(S);
+  if (a.width() > S || b.width() > S) return false;
+  for (int swap = 0; swap < 2; ++swap) {
+    const int64_t d = ((b.base - a.base) % S + S) % S;
+    if (d + b.width() <= S) {
+      a.base = 0;
+      b.base = d;
+      return apart(a, b);
+    }
+    std::swap(a, b);
+  }
+  return false;
 }
 
-// y may be x itself, else they must not overlap.
-static int check_alias(const tq_tensor4* x, const tq_tensor4* y, const char* what, const char* fn) {
-  bool same = x->data == y->data && x->dtype == y->dtype;
+// y must not overlap x; with `in_place` it may be x itself (same view).
+static int check_apart(const tq_tensor4* x, const tq_tensor4* y, bool in_place, const char* what,
+                       const char* with, const char* fn) {
+  bool same = in_place && x->data == y->data && x->dtype == y->dtype;
   for (int i = 0; i < 4; ++i) {
-    if (x->shape[i] == 0) return TQ_OK;
-    same = same && (x->shape[i] == 1 || x->stride[i] == y->stride[i]);
+    if (x->shape[i] == 0 || y->shape[i] == 0) return TQ_OK;
+    same = same && x->shape[i] == y->shape[i] && (x->shape[i] == 1 || x->stride[i] == y->stride[i]);
   }
-  if (same) return TQ_OK;
-  const char *a, *b, *c, *d;
-  extent(x, a, b);
-  extent(y, c, d);
-  if (a < d && c < b) {
-    set_error("%s: %s overlaps its input without being the same view", fn, what);
-    return TQ_ERR_INVALID;
-  }
-  return TQ_OK;
+  if (same || apart(Span(x), Span(y))) return TQ_OK;
+  set_error("%s: %s overlaps %s%s", fn, what, with, in_place ? " without being the same view" : "");
+  return TQ_ERR_INVALID;
 }
 
 int32_t tq_qk_rope(const tq_rope* rope, const tq_positions* pos, const tq_tensor4* q,
@@ -601,11 +639,17 @@ int32_t tq_qk_rope(const tq_rope* rope, const tq_positions* pos, const tq_tensor
         set_error("%s: shapes of q, k and their outputs disagree", fn);
         return TQ_ERR_INVALID;
       }
-    if ((rc = check_alias(x[w], y[w], outs[w], fn))) return rc;
     if (!rope && !norm[w]) {
       set_error("%s: %s has neither a rotation nor a norm", fn, names[w]);
       return TQ_ERR_INVALID;
     }
+  }
+  for (int w = 0; w < 2; ++w) {
+    if (!x[w]) continue;
+    if ((rc = check_apart(x[w], y[w], true, outs[w], names[w], fn)) ||
+        (x[1 - w] && (rc = check_apart(x[1 - w], y[w], false, outs[w], names[1 - w], fn))) ||
+        (w == 0 && k && (rc = check_apart(q_out, k_out, false, outs[1], outs[0], fn))))
+      return rc;
   }
   const int64_t D = one->shape[3];
   if (D < 1 || D > 256) {
@@ -702,6 +746,7 @@ int32_t tq_dequantize_ragged(const tq_geom* g, const tq_tables* t, const tq_cach
     set_error("%s: head_dim %d > 128 is not supported", fn, g->head_dim);
     return TQ_ERR_INVALID;
   }
+  if (k_out && v_out && (rc = check_apart(k_out, v_out, false, "v_out", "k_out", fn))) return rc;
   uint32_t* status = device_status_word();
   if (!status) { set_error("%s: device status word unavailable", fn); return TQ_ERR_CUDA; }
   return launch_dequant_ragged(g, t, c, batch, k_out, v_out, status, (cudaStream_t)stream);
@@ -761,7 +806,7 @@ int32_t tq_attend_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c
   const char* fn = "tq_attend_ragged";
   int rc;
   if ((rc = check_attend(g, c, a, fn)) || (rc = check_tables(g, t, fn))) return rc;
-  if ((rc = check_written(a->out, "out", fn)) || (rc = check_alias(a->q, a->out, "out", fn)))
+  if ((rc = check_written(a->out, "out", fn)) || (rc = check_apart(a->q, a->out, true, "out", "q", fn)))
     return rc;
   if (!t->rot_f16 ||
       (reinterpret_cast<uintptr_t>(t->rot_f16) | reinterpret_cast<uintptr_t>(t->rot)) % 16) {

@@ -449,3 +449,63 @@ def test_attend_needs_an_aligned_rotation():
     assert R.data_ptr() % 16
     t = ops.LayerTables(128, 4, 2, False, z(16), z(15), z(4), z(3), R)
     assert t.rot.data_ptr() % 16 == 0 and torch.equal(t.rot, R) and torch.equal(t.rot_t, R.t())
+
+
+def places(x):
+    """Byte addresses of a small view's elements."""
+    es = 4 if x.dtype == _lib.TQ_F32 else 2
+    at = {x.data}
+    for n, s in zip(x.shape, x.stride):
+        at = {a + i * s * es for a in at for i in range(n)}
+    return {a + b for a in at for b in range(es)}
+
+
+def test_outputs_beside_inputs_in_one_buffer():
+    """Slices of one buffer that share no element are taken, whatever their order; views that share one
+    are refused (but for an output that is its input)."""
+    rng = random.Random(1)
+    seen = [0, 0]
+    for _ in range(600):
+        B, T, D = rng.choice([1, 1, 2]), rng.choice([1, 2, 3]), 4
+        heads = [rng.choice([1, 2]) for _ in range(2)]
+        row = rng.choice([4, 6, 8]) * D
+        pad = rng.choice([0, 0, row])
+        b0 = 1 << 20
+        at = [b0 + 2 * rng.randrange(0, 2 * row, rng.choice([1, D])) for _ in range(2)]
+        tr = rng.random() < 0.5                            # token-major or head-major rows
+        view = lambda h, a: t4((B, h, T, D), stride=[T * row * 2 + pad, D if tr else T * row // 2,  # noqa: E731
+                                                     row if tr else D, 1], data=a)
+        x, y = view(heads[0], at[0]), view(heads[0], at[1])
+        rc, err = rope_call(rope=_lib.Rope(4096, 9, 4, 0), pos=POS, q=x, qo=y)
+        if "share memory" in err and rc == _lib.TQ_ERR_INVALID:
+            continue
+        shared = at[0] != at[1] and bool(places(x) & places(y))
+        assert rc == (_lib.TQ_ERR_INVALID if "overlaps" in err and rc == _lib.TQ_ERR_INVALID else _lib.TQ_ERR_CUDA)
+        if shared:
+            assert rc == _lib.TQ_ERR_INVALID
+        seen[shared] += 1
+    assert min(seen) > 50
+    n, D, hq, hkv = 7, 128, 4, 2
+    row = (hq + 2 * hkv) * D
+    fused = lambda h, first: t4((1, h, n, D), stride=[0, D, row, 1], data=(1 << 20) + 2 * first * D)  # noqa: E731
+    q, k, v = fused(hq, 0), fused(hkv, hq), fused(hkv, hq + hkv)
+    base = dict(rope=ROPE, pos=POS)
+    other = far((1, hkv, n, D))
+    for kw in (dict(q=q, qo=q, k=k, ko=k), dict(k=k, ko=v), dict(q=k, qo=v), dict(q=k, qo=v, k=q, ko=q)):
+        rc, err = rope_call(**base, **kw)
+        assert rc == _lib.TQ_ERR_CUDA, err                 # past the checks: there is no device here
+    for kw in (dict(q=k, qo=v, k=v, ko=v), dict(q=k, qo=k, k=v, ko=k), dict(q=k, qo=other, k=v, ko=other),
+               dict(q=k, qo=v, k=v, ko=other), dict(q=q, qo=fused(hq, 1))):
+        rc, err = rope_call(**base, **kw)
+        assert rc == _lib.TQ_ERR_INVALID and "overlaps" in err, err
+    # read-back: the two outputs
+    kv = lambda first: t4(KV, stride=[0, 128, 512, 1], data=(1 << 20) + 256 * first)  # noqa: E731
+    assert entry("read", k=kv(0), v=kv(2))[0] == _lib.TQ_ERR_CUDA
+    for v2 in (kv(0), kv(1)):
+        rc, err = entry("read", k=kv(0), v=v2)
+        assert rc == _lib.TQ_ERR_INVALID and "overlaps" in err
+    # attention: q a slice of the fused projection, out another or itself
+    a = lambda first: t4((1, 4, 10, 128), stride=[0, 128, 2048, 1], data=(1 << 20) + 256 * first)  # noqa: E731
+    for first, good in ((0, True), (4, True), (12, True), (3, False), (15, False)):
+        rc, err, _ = attend(q=a(0), out=a(first), nbytes=0)
+        assert (rc == _lib.TQ_ERR_WORKSPACE) == good and (good or "overlaps" in err), (first, err)
