@@ -15,6 +15,7 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 
@@ -564,10 +565,14 @@ class RaggedBatch(_Described):
 
 
 def _inference_only(name: str, device: torch.device, *ts) -> None:
-    """All tensors on ``device`` (CUDA) and none that a backward pass would need."""
+    """All tensors on ``device`` (CUDA) and none that a backward pass would need
+    or that carries a tangent of forward-mode differentiation."""
+    grad, forward = torch.is_grad_enabled(), forward_ad._current_level >= 0
+    for t in ts:
+        if forward and t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} has no derivative: a tangent would be dropped")
     if device.type != "cuda":
         raise RuntimeError("TurboQuant kernels need CUDA tensors (there is no CPU path)")
-    grad = torch.is_grad_enabled()
     for t in ts:
         if t is None:
             continue

@@ -509,3 +509,23 @@ def test_outputs_beside_inputs_in_one_buffer():
     for first, good in ((0, True), (4, True), (12, True), (3, False), (15, False)):
         rc, err, _ = attend(q=a(0), out=a(first), nbytes=0)
         assert (rc == _lib.TQ_ERR_WORKSPACE) == good and (good or "overlaps" in err), (first, err)
+
+
+def test_tangents_are_refused():
+    """Forward-mode differentiation: dropping the tangent would be a wrong derivative of 0."""
+    x = torch.zeros((3, 2, 128))
+    w = torch.ones(128)
+    table = ops.RopeTable(torch.zeros((5, 128)))
+    batch = ops.RaggedBatch(torch.tensor([0, 3], dtype=torch.int32), torch.tensor([3], dtype=torch.int32), 3)
+    ad = torch.autograd.forward_ad
+    with ad.dual_level():
+        d = ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: ops.qk_rope(d, None, table, torch.arange(3)),
+                     lambda: ops.qk_rope(x, None, None, q_norm=ops.HeadNorm(ad.make_dual(w, w))),
+                     lambda: ops.append_ragged(None, None, x, d, batch),
+                     lambda: ops.dequantize_ragged(None, None, batch, d, None),
+                     lambda: ops.attend_ragged(None, None, d, batch)):
+            with pytest.raises(RuntimeError, match="derivative"):
+                call()
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            ops.attend_ragged(None, None, x, batch)
