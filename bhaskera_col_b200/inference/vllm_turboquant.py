@@ -136,12 +136,18 @@ def layer_bits(layer_idx: int, num_layers: int, key_bits: int, value_bits: int,
 
 
 class TurboQuantPagedAttention:
-    """One attention layer's packed paged KV and its attention over vLLM batches."""
+    """One attention layer's packed paged KV and its attention over vLLM batches.
+
+    ``ragged_workspace``: scratch of ``forward(rope=...)`` (about 100 MB for
+    8,192 tokens of 64 requests), by default the layer's own.  Layers that run
+    one after the other on one stream can share one; graphs captured with it
+    keep it, and are replayed on that stream."""
 
     def __init__(self, layer_idx: int, num_layers: int, num_heads: int, num_kv_heads: int,
                  head_dim: int, num_blocks: int, block_size: int, key_bits: int = 4,
                  value_bits: int = 2, protected_layers: int = 2,
-                 scale: Optional[float] = None, device: torch.device = torch.device("cuda")):
+                 scale: Optional[float] = None, device: torch.device = torch.device("cuda"),
+                 ragged_workspace: Optional[ops.DecodeWorkspace] = None):
         if block_size % PAGE_TOKENS:
             raise ValueError(f"block_size {block_size} is not a multiple of {PAGE_TOKENS}")
         if num_heads % num_kv_heads:
@@ -164,7 +170,7 @@ class TurboQuantPagedAttention:
         self.pool = torch.zeros((num_blocks * self.pages_per_block * num_kv_heads,
                                  self.page_bytes), dtype=torch.uint8, device=self.device)
         self.workspace = ops.DecodeWorkspace()
-        self.ragged_workspace = ops.DecodeWorkspace()
+        self.ragged_workspace = ragged_workspace or ops.DecodeWorkspace()
         self.tokens_stored = 0
         self.decode_tokens = 0
 

@@ -1042,3 +1042,39 @@ def test_offsets_that_do_not_ascend_run_nothing(D, kb, vb, start):
     good = ops.RaggedBatch(int32([0] * R + [n]), int32([64] * R), n)
     ops.append_ragged(tables, pages, x, x, good)
     assert ok_status() == 0 and not torch.equal(pages.pool, kept)
+
+
+def test_layers_share_a_workspace():
+    """Layers of one stream with one workspace between them give what layers with their own do, eager
+    and in one captured graph of both."""
+    from bhaskera_col_b200.inference.vllm_turboquant import TurboQuantPagedAttention, VLLMBatch
+    D, Hq, H, R = 128, 8, 2, 3
+    rope = ops.RopeTable.build(D, 300, device=DEV)
+    table = torch.arange(4 * R, dtype=torch.int32, device=DEV).view(R, 4)
+    shared = ops.DecodeWorkspace()
+
+    def layers(**kw):
+        return [TurboQuantPagedAttention(i, 32, Hq, H, D, num_blocks=4 * R, block_size=64, key_bits=4,
+                                         value_bits=2, device=DEV, **kw) for i in (1, 7)]
+
+    steps = [([0, 70, 200, 201], [70, 130, 1]), ([0, 1, 2, 3], [71, 131, 2])]
+    results = []
+    for ls, graph in ((layers(), False), (layers(ragged_workspace=shared), False),
+                      (layers(ragged_workspace=shared), True)):
+        for j, (start, seq) in enumerate(steps):
+            n = start[-1]
+            batch = VLLMBatch(int32(start), int32(seq), table, n, max(b - a for a, b in zip(start, start[1:])))
+            q, k, v = (randn((n, h, D), 80 + 3 * j + i) for i, h in enumerate((Hq, H, H)))
+            outs = [torch.empty_like(q) for _ in ls]
+            step = lambda: [l.forward(x, k, v, batch, out=o, rope=rope)  # noqa: E731
+                            for l, x, o in zip(ls, (q, outs[0]), outs)]
+            step()
+            if graph:
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g):
+                    step()
+                g.replay()
+            results.append([o.clone() for o in outs] + [l.pool.clone() for l in ls])
+    for a, b, c in zip(results[:2], results[2:4], results[4:]):
+        assert all(torch.equal(x, y) and torch.equal(x, z) for x, y, z in zip(a, b, c))
+    assert shared.buf is not None and ok_status() == 0
