@@ -508,9 +508,10 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n) top = fmaxf(fmaxf(fmaxf(top, d[n][0]), fmaxf(d[n][1], d[n][2])), d[n][3]);
-    if (__any_sync(0xffffffffu, top > kRoom || fmaxf(vn[0], vn[1]) >= kNorm)) {
+    const float big = fmaxf(fabsf(vn[0]), fabsf(vn[1]));
+    if (__any_sync(0xffffffffu, top > kRoom || big >= kNorm)) {
       // the largest norm of the tile, below 2^(e + 1): down to below kNorm
-      const int e = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vn[0], vn[1]))) >> 23) - 127;
+      const int e = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(big)) >> 23) - 127;
       const float r = __uint_as_float((uint32_t)(127 - max(e - 7, 0)) << 23);
       vs *= r;
       vn[0] *= r;

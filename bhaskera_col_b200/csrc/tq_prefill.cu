@@ -359,7 +359,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
           if (warp == 0) {
             // the page's largest norm, below 2^(e + 1): the scale keeps it below 2^15
             const int e0 = v_exp;
-            const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(x[0], x[1])));
+            const unsigned top = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fabsf(x[0]), fabsf(x[1]))));
             const int e = tmin(e0, 14 - ((int)(top >> 23) - 127));
             const float scale = __uint_as_float((uint32_t)(127 + e) << 23);
             x[0] *= scale;

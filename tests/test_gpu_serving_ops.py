@@ -1078,3 +1078,26 @@ def test_layers_share_a_workspace():
     for a, b, c in zip(results[:2], results[2:4], results[4:]):
         assert all(torch.equal(x, y) and torch.equal(x, z) for x, y, z in zip(a, b, c))
     assert shared.buf is not None and ok_status() == 0
+
+
+@pytest.mark.parametrize("engine,dtype", [(0, BF16), (0, F32), (1, BF16), (1, F32), (2, BF16), (3, BF16), (3, F32)])
+def test_attend_ragged_norms_of_either_sign(engine, dtype):
+    """Norms are stored as they are given: a page written by hand may hold negative ones and -0."""
+    D, Hq, H = 128, 8, 2
+    tables = make_tables(D, 4, 4, False)
+    lens = [(3, 300), (70, 130), (1, 1)]
+    batch, start, seq = make_batch(lens)
+    pages = make_paged(tables, len(lens) * H, 320)
+    fill(tables, pages, len(lens), H, 320, 91)
+    q = randn((start[-1], Hq, D), 92, dtype)
+    for first in (0, 128):                                 # value norms, both
+        norms = pages.pool[:, pages.pool.shape[1] - 128 - first:].view(F16)
+        norms *= torch.tensor([-1, 1, -1, -0.0, -1], device=DEV).repeat(norms.shape[1])[: norms.shape[1]]
+        kd, vd = (x.reshape(len(lens), H, -1, D) for x in S.dense(tables, contiguous(pages), 320))
+        got = ops.attend_ragged(tables, pages, q, batch, engine=engine)
+        check_attend(got, S.attend(q, kd, vd, start, seq, S.default_scale(D), True), dtype)
+    pages.pool[:, pages.pool.shape[1] - 128:].view(F16).abs_().neg_()      # nothing but negative ones
+    kd, vd = (x.reshape(len(lens), H, -1, D) for x in S.dense(tables, contiguous(pages), 320))
+    got = ops.attend_ragged(tables, pages, q, batch, engine=engine)
+    check_attend(got, S.attend(q, kd, vd, start, seq, S.default_scale(D), True), dtype)
+    assert ok_status() == 0
