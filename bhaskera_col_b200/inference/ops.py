@@ -769,7 +769,8 @@ def attend_ragged(tables: LayerTables, pages, q: torch.Tensor, batch: RaggedBatc
     pages, each request's rows over its own tokens [0, seq_lens[r]): causal
     (prompt chunks, draft tokens, single tokens, mixed), or with ``causal``
     False every row over all of them (cross attention: the pages hold an
-    encoder's states, seq_lens their lengths).  A row that sees no key is
+    encoder's states, seq_lens their lengths).  Rows of no request stay as they
+    are in ``out``, and are not set in an ``out`` of the call's own.  A row that sees no key is
     zero; a request longer than its pages attends what they hold and sets
     _lib.DEV_BAD_POSITION.  Work is split along long contexts.  ``engine`` 0 picks the kernels
     by each request's rows and the type of ``out`` (fp16 and fp32 results are

@@ -269,10 +269,10 @@ class TurboQuantPagedAttention:
         """The stored keys and values of a batch's tokens as dense (N, Hkv, D)
         tensors (a batch whose query lengths are whole contexts reads those:
         for handing a prefix to another attention or cache).  Tokens without a
-        place in the pages read as 0."""
+        place in the pages and rows of no request (padding) read as 0."""
         st = stream_table if stream_table is not None else self.stream_table(batch.block_table)
         shape = (batch.num_actual_tokens, self.num_kv_heads, self.head_dim)
-        k, v = (torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
+        k, v = (torch.zeros(shape, dtype=dtype, device=self.device) for _ in range(2))
         ops.dequantize_ragged(self.tables, self.paged(st), batch.ragged(), k, v)
         return k, v
 

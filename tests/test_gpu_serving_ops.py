@@ -1101,3 +1101,20 @@ def test_attend_ragged_norms_of_either_sign(engine, dtype):
     got = ops.attend_ragged(tables, pages, q, batch, engine=engine)
     check_attend(got, S.attend(q, kd, vd, start, seq, S.default_scale(D), True), dtype)
     assert ok_status() == 0
+
+
+def test_paged_attention_read_of_a_padded_batch_is_zero_there():
+    """Rows of a padded batch that belong to no request come back as 0."""
+    from bhaskera_col_b200.inference.vllm_turboquant import TurboQuantPagedAttention, VLLMBatch
+    D, H = 128, 2
+    layer = TurboQuantPagedAttention(5, 32, 4, H, D, num_blocks=4, block_size=64, device=DEV)
+    table = torch.arange(4, dtype=torch.int32, device=DEV).view(2, 2)
+    batch = VLLMBatch(int32([1, 3, 4]), int32([2, 1]), table, 7, 2)
+    q, k, v = (randn((7, h, D), 5 + j) for j, h in enumerate((4, H, H)))
+    layer.forward(q, k, v, batch, rope=ops.RopeTable.build(D, 10, device=DEV))
+    junk = [torch.full((7, H, D), 9.0, dtype=BF16, device=DEV) for _ in range(8)]
+    del junk                                               # memory that an allocation may get
+    rk, rv = layer.read(batch)
+    for x in (rk, rv):
+        assert (x[[0, 4, 5, 6]] == 0).all() and (x[1:4].abs().sum((1, 2)) > 0).all()
+    assert ok_status() == 0
