@@ -224,11 +224,14 @@ def append_uses_tensor_cores(tables: LayerTables, k: torch.Tensor, v: torch.Tens
                                           ctypes.byref(vt)))
 
 
-def device_status(device: torch.device) -> int:
-    """Read and clear the library's device status word (0: no kernel timed out)."""
+def device_status(device: Optional[torch.device] = None) -> int:
+    """Read and clear the library's status word on ``device`` (by default the
+    current one), an OR of _lib.DEV_* (0: no kernel had anything to report)."""
     lib = _lib.load()
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
     st = ctypes.c_uint32(0)
-    rc = lib.tq_device_status(ctypes.byref(st), _stream(device))
+    with _on(device):                                    # each device has a word of its own
+        rc = lib.tq_device_status(ctypes.byref(st), _stream(device))
     if rc not in (_lib.TQ_OK, _lib.TQ_ERR_DEVICE):
         _lib.check("tq_device_status", rc)
     return int(st.value)

@@ -529,3 +529,34 @@ def test_tangents_are_refused():
                 call()
         with pytest.raises(RuntimeError, match="no CPU path"):
             ops.attend_ragged(None, None, x, batch)
+
+
+def test_device_status_reads_the_word_of_its_device(monkeypatch):
+    """The word is looked up on the current device: the one asked for is made current."""
+    current, seen = [0], []
+
+    class Device:                                          # torch.cuda.device without a driver
+        def __init__(self, device):
+            self.to = device.index
+
+        def __enter__(self):
+            self.back, current[0] = current[0], self.to
+
+        def __exit__(self, *a):
+            current[0] = self.back
+
+    class Lib:
+        @staticmethod
+        def tq_device_status(word, stream):
+            seen.append(current[0])
+            return _lib.TQ_OK
+
+    monkeypatch.setattr(ops._lib, "load", lambda: Lib)
+    monkeypatch.setattr(ops, "_stream", lambda device: 0)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    for d in (torch.device("cuda", 1), torch.device("cuda", 0), torch.device("cuda")):
+        assert ops.device_status(d) == 0
+    current[0] = 2
+    assert ops.device_status() == 0
+    assert seen == [1, 0, 0, 2] and current == [2]
