@@ -31,14 +31,17 @@
 //
 // Read-back: x = (c R) n with R's rows in packed order as the K dimension,
 // c and R as fp16 hi + lo (three products); for bf16 results c = hi alone: its
-// rounding, 2^-11 of each term, is an eighth of the result's own.
+// rounding, 2^-12 of each term on average, is an eighth of the result's own and
+// takes their error from 1.66e-3 to 1.68e-3, one bf16 step in 5 % of the values.  lo
+// too would leave room for one operand tile in flight instead of two (17,971 tokens
+// 58.5 us against 50); who wants it asks for fp32 results.
 //
 // Bounds: HBM (256 B in, 66 out per 4-bit vector of 128 bf16, or the reverse);
 // in fact a role's instructions per tile: append's makers (3 us a tile: norms,
 // rotation, split) and epilogue (2 us: 9 instructions a coordinate), read-back's
 // epilogue (3.2 us).  Measured, K and V: append of 11,272 tokens x 8 heads of 128,
-// 4-bit, with norm and rotation, and reading them back 107 us for 122 MB (half of
-// it each); read-back of 17,971 tokens 51 us for 93 MB, 1.8 TB/s; a launch of
+// 4-bit, with norm and rotation, and reading them back 103 us for 122 MB (half of
+// it each); read-back of 17,971 tokens 50 us for 93 MB, 1.9 TB/s; a launch of
 // few tiles 8-10 us, set-up (rotation, tables) and one tile's latency.
 //
 // Every wait is bounded; on expiry the kernel sets TQ_DEV_WAIT_TIMEOUT in the
@@ -370,7 +373,8 @@ struct Again {
 };
 // Noted per epilogue warp, in the warp's order; runs past that keep their first
 // values.  At one run in 1,600 the 8 warps' lists last for 100,000 vectors of 128
-// per SM and launch, 15 million in all.  (Redone at once in the epilogue, a run's
+// per SM and launch, 15 million in all; a vector beside a boundary that repeats fills
+// them after 32 times.  (Redone at once in the epilogue, a run's
 // cold code held up its warp: whole prompts 125 us against 107; by the locators
 // between their tiles, it held up the tiles: 138 us.)
 constexpr int kAgain = 32;

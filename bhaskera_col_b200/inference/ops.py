@@ -751,7 +751,10 @@ def dequantize_ragged(tables: LayerTables, pages, batch: RaggedBatch,
                       k_out: Optional[torch.Tensor], v_out: Optional[torch.Tensor]) -> None:
     """Write the stored keys and values of a flattened batch's tokens into the
     rows of (N, Hkv, D) tensors; either may be None.  A row whose position
-    lies outside the pages is zeroed and sets _lib.DEV_BAD_POSITION."""
+    lies outside the pages is zeroed and sets _lib.DEV_BAD_POSITION; rows of no
+    request stay as they are.  fp16 and fp32 results are those of fp32
+    arithmetic up to its last bits; bf16 ones (head dims 64 and 128) take the
+    centroids as fp16, which turns one value in twenty by a step."""
     one = k_out if k_out is not None else v_out
     if one is None:
         raise ValueError("neither k_out nor v_out is given")
@@ -772,14 +775,19 @@ def attend_ragged(tables: LayerTables, pages, q: torch.Tensor, batch: RaggedBatc
     pages, each request's rows over its own tokens [0, seq_lens[r]): causal
     (prompt chunks, draft tokens, single tokens, mixed), or with ``causal``
     False every row over all of them (cross attention: the pages hold an
-    encoder's states, seq_lens their lengths).  Rows of no request stay as they
-    are in ``out``, and are not set in an ``out`` of the call's own.  A row that sees no key is
-    zero; a request longer than its pages attends what they hold and sets
-    _lib.DEV_BAD_POSITION.  Work is split along long contexts.  ``engine`` 0 picks the kernels
-    by each request's rows and the type of ``out`` (fp16 and fp32 results are
-    exact to their rounding and to 2^-18); 1 is the mma.sync kernel, 2 the
-    tcgen05 kernel (error 7e-4 in any type), 3 the kernel of few query rows.  Pass a ``workspace`` to reuse one buffer
-    across calls on one stream."""
+    encoder's states, seq_lens their lengths).  A row that sees no key is zero;
+    a request longer than its pages attends what they hold and sets
+    _lib.DEV_BAD_POSITION.  Rows of no request stay as they are in ``out``, and
+    are not set in an ``out`` of the call's own.
+
+    Work is split along long contexts.  ``engine`` 0 picks the kernels by each
+    request's rows and by the type of ``out``, which may differ from q's: bf16
+    results come from fp16 operands (relative error 7e-4 beside the rounding's
+    1.7e-3), fp16 and fp32 ones from operands of 22 bits (2e-6), whatever the
+    size of the values; an fp32 ``out`` is the choice of who wants those bits
+    for bf16 queries.  1 is the mma.sync kernel, 2 the tcgen05 kernel (8e-4 in
+    any type), 3 the kernel of few query rows.  Pass a ``workspace`` to reuse
+    one buffer across calls on one stream."""
     _inference_only("attend_ragged", q.device, q, out, batch.q_start)
     if out is None:
         out = torch.empty_like(q)

@@ -384,7 +384,7 @@ typedef struct tq_positions {
  * (B, Hkv, T, D) to q_out and k_out of the same shapes and types, computed in
  * fp32 and rounded once.  Either pair may be NULL; so may a norm, and rope
  * (then positions are not read).  An output may be its input (same view), else
- * it must not overlap the inputs.  D: 1..256. */
+ * it must not overlap an input or the other output.  D: 1..256. */
 int32_t tq_qk_rope(const tq_rope* rope, const tq_positions* pos, const tq_tensor4* q,
                    const tq_tensor4* q_out, const tq_head_norm* q_norm, const tq_tensor4* k,
                    const tq_tensor4* k_out, const tq_head_norm* k_norm, void* stream);
@@ -414,10 +414,12 @@ typedef struct tq_ragged {
  * stored there would be a mix of both.  Codes as tq_append's of the
  * rotated vector, not rounded to k's type in between.  Head dims 64 and 128 on
  * 16-byte rows (and rot_dim a multiple of 16) run on the tensor cores, their
- * codes those of exact arithmetic (for some 10^7 vectors a call; behind them,
- * and in other shapes, which run on the CUDA cores, those of fp32: a code in
- * about a million is one off, beside its boundary).  head_dim <= 128,
- * no QJL sketch. */
+ * codes those of exact arithmetic.  Exact are the first 32 runs of 32 coordinates
+ * with one beside a boundary that each of a CTA's 8 warps meets: all of some 10^7
+ * different 4-bit vectors, but not of one such vector repeated.  Later ones, and
+ * other shapes, which run on the CUDA cores, have the codes of fp32: of these about
+ * one in a million is one off, beside its boundary.  head_dim <= 128, no QJL
+ * sketch. */
 int32_t tq_append_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                          const tq_tensor4* k, const tq_tensor4* v, const tq_ragged* batch,
                          const tq_rope* rope, const tq_head_norm* k_norm,
@@ -426,7 +428,9 @@ int32_t tq_append_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c
 /* tq_dequantize of a ragged batch: the stored keys and values of the batch's
  * tokens to their rows of k_out / v_out (1, Hkv, N, D); either may be NULL.  A
  * row whose position lies outside the pages is zeroed and sets
- * TQ_DEV_BAD_POSITION. */
+ * TQ_DEV_BAD_POSITION.  k_out and v_out must not overlap.  Head dims 64 and 128 run
+ * on the tensor cores: fp16 and fp32 results in 22 bits or more, bf16 ones with the
+ * centroids as fp16 (2^-12 of each term, an eighth of their rounding). */
 int32_t tq_dequantize_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                              const tq_ragged* batch, const tq_tensor4* k_out,
                              const tq_tensor4* v_out, void* stream);
@@ -448,12 +452,14 @@ typedef struct tq_attend_args {
   float scale;                /* softmax scale                                */
   int32_t causal;
   int32_t engine;             /* 0: the fastest kernels for the lengths whose
-                                 error stays below the result type's rounding;
-                                 1: the mma.sync kernel; 2: the tcgen05 kernel
-                                 (256 rows per CTA; fp16 operands, relative
-                                 error 7e-4 whatever the result's type); 3: the
-                                 kernel of 8 or 16 rows per CTA (codes of 2 to
-                                 4 bits)                                      */
+                                 error stays below the result type's rounding
+                                 (relative, 7e-4 for bf16 results, 2e-6 for fp32
+                                 ones, whatever the size of the values);
+                                 1: the mma.sync kernel (5e-6 for fp32); 2: the
+                                 tcgen05 kernel (256 rows per CTA; fp16
+                                 operands, 8e-4 whatever the result's type); 3:
+                                 the kernel of 8 or 16 rows per CTA (codes of 2
+                                 to 4 bits)                                   */
 } tq_attend_args;
 
 /* 0 on bad arguments.  The workspace must be 256-byte aligned and belongs to
