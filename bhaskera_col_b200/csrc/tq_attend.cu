@@ -344,17 +344,17 @@ struct AttendShape {
 
 // Query rows of a request and KV head up to which the few-row kernel is taken
 // where the tcgen05 kernel could be: 16 requests of 3,000-5,000 keys, D128, four
-// heads a group: 64 rows 132 us against 207, 128 rows 216 against 229, 256 rows 387
-// against 274.  Elsewhere it takes every request: the mma.sync kernel, which it
-// replaces there, is behind at any number of rows (D64: 16 rows 41 us against 234,
-// 1,024 rows 908 against 1,390; D128, fp16 results, 1,024 rows 3,397 against 4,009)
+// heads a group: 64 rows 128 us against 197, 128 rows 199 against 227, 256 rows 375
+// against 282.  Elsewhere it takes every request: the mma.sync kernel, which it
+// replaces there, is behind at any number of rows (D64: 16 rows 41 us against 233,
+// 1,024 rows 927 against 1,427; D128, fp16 results, 1,024 rows 3,281 against 3,925)
 // and runs the codes that the few-row kernel has no table for (above 4 bits).
 constexpr int kFewRows = 128;
 
 // The kernels that a call may use: few rows, and tcgen05 (else mma.sync) for the
 // others.  The tcgen05 kernel's operands are single fp16 values: for fp16 and fp32
 // results (error 7e-4, against 2.1e-4 of fp16's own rounding) only when asked for,
-// although it is six times as fast from 1,024 rows on (562 us against 3,397).
+// although it is six times as fast from 1,024 rows on (549 us against 3,281).
 struct Kernels {
   bool few, tc;
 };

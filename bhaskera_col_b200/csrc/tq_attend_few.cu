@@ -34,7 +34,7 @@
 // 1.25 us a page and CTA; HBM would allow a fifth.  K4/V2, 8 KV heads of 128, g 4:
 // 252 draft tokens over 256,960 156 us, 1.3 TB/s; K3/V3, g 5: 5 tokens over
 // 131,001 140 us.  HP reads eight bytes a lookup and multiplies three times:
-// 317 and 272 us.  168 registers are the most for three CTAs an SM; what the loop
+// 322 and 277 us.  168 registers are the most for three CTAs an SM; what the loop
 // needs rarely (each row's last key, the bad pages' flag) is kept out of them, since
 // a spilled one cost up to 25 us of the second.
 #include "tq_internal.h"
@@ -356,8 +356,19 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
       atomicOr(p.status, TQ_DEV_BAD_BLOCK);
       e = 0;
     }
-    const uint8_t* page = page_at(p.pages, e, p.page_bytes);
-    const uint8_t *k = page + at_k, *v = page + at_v, *n = page + at_n;
+    // heads of 128: one product, since three addresses across the loop cost spills; of
+    // 64, where there are registers, three products (encoder 35.0 us against 36.0)
+    const uint8_t *k, *v, *n;
+    if constexpr (D == 64) {
+      k = page_at(p.pages + at_k, e, p.page_bytes);
+      v = page_at(p.pages + at_v, e, p.page_bytes);
+      n = page_at(p.pages + at_n, e, p.page_bytes);
+    } else {
+      const uint8_t* page = page_at(p.pages, e, p.page_bytes);
+      k = page + at_k;
+      v = page + at_v;
+      n = page + at_n;
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       x.k[i].load(k + 8 * i * KROW);
