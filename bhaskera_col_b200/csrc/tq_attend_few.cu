@@ -35,8 +35,8 @@
 // 252 draft tokens over 256,960 156 us, 1.3 TB/s; K3/V3, g 5: 5 tokens over
 // 131,001 140 us.  HP reads eight bytes a lookup and multiplies three times:
 // 322 and 277 us.  168 registers are the most for three CTAs an SM; what the loop
-// needs rarely (each row's last key, the bad pages' flag) is kept out of them, since
-// a spilled one cost up to 25 us of the second.
+// needs rarely is kept out of them where it would spill, which cost up to 25 us of the
+// second.
 #include "tq_internal.h"
 #include "tq_ragged.cuh"
 
@@ -80,6 +80,12 @@ template <int D, int KB, int VB, int NT, bool HP>
 struct Few {
   static constexpr int NQ = 8 * NT;
   static constexpr bool KQ = KB == 2 && !HP, VQ = VB == 2 && !HP;   // two pairs per table entry
+  // Which rarely needed values the loop holds is settled by its time at 168 registers (64
+  // single tokens over 8,000 keys): with 8 rows each row's last key in registers (K3/V3
+  // 181 us against 199 from shared memory, K2/V2 152 against 174, heads of 64 117
+  // against 129); the first bad key noted at once for K4/V2 (162 us, kept to the end
+  // 175), at the end for the others (K3/V3 181, at once 197; heads of 64 117, 134).
+  static constexpr bool kLimits = NT == 1, kKeyNow = NT == 1 && D == 128 && KB == 4 && VB == 2;
   static constexpr int KT = 128 << (KQ ? 8 : 2 * KB), VT = 128 << (VQ ? 8 : 2 * VB);   // tables
   static constexpr int LDO = D + 4;                         // floats per row of an output (banks)
   static constexpr int LDA = D / 2 + 4;                     // words per row of a rotation operand
@@ -356,10 +362,10 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
       atomicOr(p.status, TQ_DEV_BAD_BLOCK);
       e = 0;
     }
-    // heads of 128: one product, since three addresses across the loop cost spills; of
-    // 64, where there are registers, three products (encoder 35.0 us against 36.0)
+    // 16 rows of 128: one product, since three addresses across the loop cost spills;
+    // elsewhere, where there are registers, three (encoder 35.0 us against 36.0)
     const uint8_t *k, *v, *n;
-    if constexpr (D == 64) {
+    if constexpr (D * NT <= 128) {
       k = page_at(p.pages + at_k, e, p.page_bytes);
       v = page_at(p.pages + at_v, e, p.page_bytes);
       n = page_at(p.pages + at_n, e, p.page_bytes);
@@ -423,13 +429,14 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
   // without keys needs no case of its own
   float m[NT][2], l[NT][2];
   float vs = 4194304.f;                                    // scale of the value norms, 2^22 at most
-  int lim_min = INT_MAX;
+  int lim_min = INT_MAX, lim[2] = {INT_MAX, INT_MAX};
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       m[n][c] = kNoMax;
       l[n][c] = 0.f;
+      if (F::kLimits) lim[c] = lims[2 * tq + c];
       lim_min = min(lim_min, lims[8 * n + 2 * tq + c]);
     }
   lim_min = min(lim_min, __shfl_xor_sync(0xffffffffu, lim_min, 1));
@@ -458,7 +465,10 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
       const bool in = key0 + 8 * i < kend;
       // exponent 31 in either half carries into its sign bit
       const bool fin = (((h & 0x7FFF7FFFu) + 0x04000400u) & 0x80008000u) == 0;
-      if (in && !fin) bad_key = min(bad_key, key0 + 8 * i);
+      if (in && !fin) {
+        if constexpr (F::kKeyNow) atomicMin(&flags[1], key0 + 8 * i);
+        else bad_key = min(bad_key, key0 + 8 * i);
+      }
       h = in && fin ? h : 0u;
       const __half2 h2 = *reinterpret_cast<const __half2*>(&h);
       kn[i] = __low2float(h2);
@@ -505,7 +515,7 @@ __device__ __forceinline__ void attend_segment(const FewParams& p, const SegWork
     float d[NT][4], top = -INFINITY;
     const bool edge = 64 * pg + s0 + 15 > lim_min;
     // key i of the tile hidden from column c of slice n
-    auto hidden = [&](int n, int i, int c) { return key0 + 8 * i > lims[8 * n + 2 * tq + c]; };
+    auto hidden = [&](int n, int i, int c) { return key0 + 8 * i > (F::kLimits ? lim[c] : lims[8 * n + 2 * tq + c]); };
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
