@@ -362,11 +362,10 @@ struct HalfRegs {
 };
 
 // RG: a norm that is not finite counts as 0 (0 x inf would reach the rows of
-// the tile that do not see the key) and its key is noted; norms come times
-// `scale`, a power of two.
+// the tile that do not see the key) and its key is noted.
 template <int NB, int NR, bool RG = false>
 __device__ __forceinline__ void load_half(HalfRegs<NB, NR>& t, const TcParamsView& pv, int jj,
-                                          int off_codes, int off_norm, float scale = 1.f) {
+                                          int off_codes, int off_norm) {
   constexpr int RPP = NR / 2, STEP = 64 / RPP;
   const int j = RG ? jj + pv.tile0 : jj;
   const uint8_t* pgs[2];
@@ -393,16 +392,21 @@ __device__ __forceinline__ void load_half(HalfRegs<NB, NR>& t, const TcParamsVie
         t.n[r] = 0u;
         atomicMin(pv.bad_key, (int)key);
       }
-      if (RG) {
-        const float n = __half2float(__ushort_as_half((unsigned short)t.n[r])) * scale;
-        t.n[r] = __half_as_ushort(__float2half_rn(n));
-      }
     } else {
 #pragma unroll
       for (int i = 0; i < NB; ++i) t.c[r].w[i] = 0u;
       t.n[r] = 0u;
     }
   }
+}
+
+// Norms times a power of two (which may be more than a half holds).
+template <int NB, int NR>
+__device__ __forceinline__ void scale_norms(HalfRegs<NB, NR>& t, float scale) {
+#pragma unroll
+  for (int r = 0; r < NR; ++r)
+    t.n[r] = __half_as_ushort(
+        __float2half_rn(__half2float(__ushort_as_half((unsigned short)t.n[r])) * scale));
 }
 
 // Decode the NR rows of one operand tile into the stage at `tile` (row

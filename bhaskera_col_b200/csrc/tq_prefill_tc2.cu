@@ -31,9 +31,11 @@
 //
 // RG: a ragged batch (tq_attend_ragged); a CTA takes one segment of the work
 // list and leaves partial rows where the tile has several.  V^ is fp16, which ends
-// at 2^-24 where a cache's norms need not: the CTA first looks through its keys'
-// value norms (2 of every 130 bytes at 4 bits) and takes them times the power of two
-// that puts the largest into [2^10, 2^11); results are divided by it.
+// at 2^-24 where a cache's norms need not: the decoders look through the segment's
+// value norms (2 of every 130 bytes at 4 bits), after the first K^ tile and before the
+// first V^ tile is due, and take them times the power of two that puts the largest
+// into [2^10, 2^11); results are divided by it.  (In front of the set-up a prompt of
+// 8,100 rows took 938 us, here 925.)
 //
 // Every wait is bounded; on expiry the kernel sets TQ_DEV_WAIT_TIMEOUT in the
 // status word, the other roles see the abort flag, no MMA is left in flight
@@ -93,9 +95,16 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + OFF_BAR);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + B_COUNT);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + B_COUNT + 1);
-  // RG: last CTA, first bad key, then each warp's largest value norm
+  // RG: last CTA, first bad key, then each decoder warp's largest value norm
   int* flags = reinterpret_cast<int*>(bars + B_COUNT + 2);
-  static_assert(8 * (B_COUNT + 2) + 4 * (2 + kWarps) <= 256, "room behind the barriers");
+  static_assert(8 * (B_COUNT + 2) + 4 * (2 + kDecWarps) <= 256, "room behind the barriers");
+  // exponent of the largest norm (1 for fp16's subnormals): it lies below 2^(e - 14)
+  auto norm_exponent = [&] {
+    int e = 1;
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) e = tmax(e, flags[2 + w] >> 10);
+    return e;
+  };
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   using Pos = typename Job<RG>::Pos;
@@ -138,29 +147,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
   if (warp == 0) {
     tc::tmem_alloc(tmem_slot, kTmemCols);
     tc::tmem_relinquish();
-  }
-
-  if constexpr (RG) {
-    // the warp's pages, kWarps apart: table entries first, 32 at once
-    const int end = (tmin<int>(kend, (jb.tile0 + ntiles) * kKeys) + 63) >> 6;
-    unsigned top = 0;
-    for (int p0 = 2 * jb.tile0 + warp; p0 < end; p0 += 32 * kWarps) {
-      int64_t slot = 0;
-      bool inside;                         // (the decoders flag pages outside the pool)
-      if (p0 + lane * kWarps < end) slot = page_slot(p.pm, stream, p0 + lane * kWarps, inside);
-#pragma unroll 8
-      for (int i = 0; i < 32; ++i) {
-        const int pg = p0 + i * kWarps;
-        if (pg >= end) break;
-        const uint8_t* page = p.pages + __shfl_sync(0xffffffffu, slot, i) * (int64_t)p.page_bytes;
-        const uint32_t h = __ldg(reinterpret_cast<const uint32_t*>(page + p.off_vn) + lane);
-        const unsigned a = h & 0x7FFFu, b = (h >> 16) & 0x7FFFu;
-        if (64 * pg + 2 * lane < kend && a < 0x7C00u) top = tmax(top, a);
-        if (64 * pg + 2 * lane + 1 < kend && b < 0x7C00u) top = tmax(top, b);
-      }
-    }
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0) flags[2 + warp] = (int)top;
   }
 
   // ---- setup: Q rows (softmax groups), R_K and the pair tables (decoders) ----
@@ -231,13 +217,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-
-  // exponent of the largest norm (1 for fp16's subnormals): it lies below 2^(ve - 14)
-  int ve = 1;
-  if constexpr (RG) {
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) ve = tmax(ve, flags[2 + w] >> 10);
-  }
 
   constexpr uint32_t idesc_kk = tc::idesc_f16_f32(128, 128);                 // A, B K-major
   constexpr uint32_t idesc_kmn = tc::idesc_f16_f32(128, 128) | (1u << 16);    // B MN-major
@@ -493,6 +472,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
       const int64_t h = kvh * p.g + (int64_t)chunk * p.hc + id.head;
       const int64_t base = jb.orow + h * p.os[1] + (int64_t)id.pos * p.os[2];
       const bool split = RG && jb.sw.seg.slot >= 0;
+      const float down = RG ? __uint_as_float((uint32_t)(127 - 25 + norm_exponent()) << 23) : 1.f;
       const int64_t pr = split ? part_row(p.rg.plan, jb.sw.seg.slot, jb.sw.group, 128 * X + rr) : 0;
       if (split && valid) p.rg.plan.ml[pr] = make_float2(m, l);
 #pragma unroll 1
@@ -502,7 +482,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
         tmem_ld_wait(x);
         if (!valid) continue;
         if constexpr (RG) {
-          const float down = __uint_as_float((uint32_t)(127 + ve - 25) << 23);
 #pragma unroll
           for (int e = 0; e < 32; ++e) x[e] = __float_as_uint(__uint_as_float(x[e]) * down);
         }
@@ -565,7 +544,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
     pv.kpacked = RG ? kend : p.n_tokens - pv.W;
     pv.tile0 = jb.tile0;
     pv.bad_key = flags + 1;
-    const float v_scale = __uint_as_float((uint32_t)(127 + 25 - ve) << 23);
     const unsigned char* lk = sm + OFF_LUT + 4 * (lane & (p.rk - 1));
     const unsigned char* lv = sm + OFF_LUT + 4 * nk * p.rk + 4 * (lane & (p.rv - 1));
     const int rk4 = 4 * p.rk, rv4 = 4 * p.rv;
@@ -580,10 +558,37 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
     __syncwarp();
     if (lane == 0) tc::mbar_arrive_cta(&bars[B_KFULL]);
     if (ntiles > 1) load_half<KB, 2, RG>(kc, pv, 1, 0, p.off_kn);
-    load_half<VB, 2, RG>(vc, pv, 0, p.off_v, p.off_vn, v_scale);
+    load_half<VB, 2, RG>(vc, pv, 0, p.off_v, p.off_vn);
+    float v_scale = 1.f;
+    if constexpr (RG) {
+      // the warp's pages, kDecWarps apart: table entries first, 32 at once
+      const int end = (tmin<int>(kend, (jb.tile0 + ntiles) * kKeys) + 63) >> 6;
+      unsigned top = 0;
+      for (int p0 = 2 * jb.tile0 + (dt >> 5); p0 < end; p0 += 32 * kDecWarps) {
+        int slot = 0;                      // (counted in 32 bits, like all pages)
+        bool inside;                       // (load_half flags pages outside the pool)
+        if (p0 + lane * kDecWarps < end)
+          slot = (int)page_slot(p.pm, stream, p0 + lane * kDecWarps, inside);
+#pragma unroll 8
+        for (int i = 0; i < 32; ++i) {
+          const int pg = p0 + i * kDecWarps;
+          if (pg >= end) break;
+          const uint8_t* page = p.pages + __shfl_sync(0xffffffffu, slot, i) * (int64_t)p.page_bytes;
+          const uint32_t h = __ldg(reinterpret_cast<const uint32_t*>(page + p.off_vn) + lane);
+          const unsigned x = h & 0x7FFFu, y = (h >> 16) & 0x7FFFu;
+          if (64 * pg + 2 * lane < kend && x < 0x7C00u) top = tmax(top, x);
+          if (64 * pg + 2 * lane + 1 < kend && y < 0x7C00u) top = tmax(top, y);
+        }
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) flags[2 + (dt >> 5)] = (int)top;
+      // the decoders only, none of whom has waited for anything yet
+      asm volatile("bar.sync 1, %0;" ::"n"(kDecThreads) : "memory");
+      v_scale = __uint_as_float((uint32_t)(127 + 25 - norm_exponent()) << 23);
+    }
     for (int j = 0; j < ntiles; ++j) {
       if (j + 2 < ntiles) load_half<KB, 2, RG>(kn, pv, j + 2, 0, p.off_kn);
-      if (j + 1 < ntiles) load_half<VB, 2, RG>(vn, pv, j + 1, p.off_v, p.off_vn, v_scale);
+      if (j + 1 < ntiles) load_half<VB, 2, RG>(vn, pv, j + 1, p.off_v, p.off_vn);
       if (j + 1 < ntiles) {
         // K^ of tile j + 1: both S MMAs of tile j - 1 have read this stage
         const int jk = j + 1, sk = jk & 1;
@@ -606,6 +611,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_tc2_kernel(TcPrefillParam
       else if (j == 0)
         ok = wait_or_abort(&bars[B_ROT], 0u, abort_flag, p.status);
       if (!__all_sync(0xffffffffu, ok)) break;
+      if (RG) scale_norms(vc, v_scale);
       decode_half<VB>(vc, lv, rv4, sm + OFF_V + s * kStage, co);
       if (!RG && tile_has_window(pv, j)) window_half<2>(pv, j, p.wv, sm + OFF_V + s * kStage, co);
       tc::fence_proxy_async_smem();
