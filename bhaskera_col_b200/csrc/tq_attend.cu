@@ -28,12 +28,12 @@ constexpr int kClasses = 32;               // length classes of segments
 // (three CTAs a SM): 131,001 keys 142 us with 5 a SM, 172 with 3, 157 with 8; 64
 // requests' drafts 163, 166, 168.  Shortest: one request of 2,000 keys 35 us with 512,
 // 33 with 256, 43 with 1,024; 64 of 1,000 keys 46, 57, 47.
-// Other batches, wide list with 1, 2, 3, 5 a SM: one prompt of 8,100 rows 944, 938,
-// 935, 1,051 us; four of 2,000 over 4,000 keys each 1,230, 1,241, 1,239, 1,238; forty of
-// 300 594, 592, 594, 653.  Few-row list with 3, 5, 8: one token over 32,771 keys 35, 45,
-// 47; 8 x 4 over 15,999 87, 77, 85; 32 over up to 9,000 58, 54, 60; 256 over up to
-// 2,000 60, 62, 62; 64 over 8,000 211, 180, 173; full attention of 100 x 20 rows, heads
-// of 64, 79, 78, 86.
+// Other batches, wide list with 1, 2, 3, 5 a SM: one prompt of 8,100 rows 934, 927,
+// 924, 1,039 us; four of 2,000 over 4,000 keys each 1,219, 1,228, 1,225, 1,225; forty of
+// 300 595, 595, 595, 650.  Few-row list with 3, 5, 8: one token over 32,771 keys 35, 45,
+// 46; 8 x 4 over 15,999 87, 77, 85; 32 over up to 9,000 58, 53, 60; 256 over up to
+// 2,000 60, 61, 61; 64 over 8,000 183, 163, 161; full attention of 100 x 20 rows, heads
+// of 64, 76, 76, 84.
 constexpr int kWaves = 2, kMinKeys = 512;
 constexpr int kFewWaves = 5, kFewMinKeys = 512;
 
