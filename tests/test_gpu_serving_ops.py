@@ -1118,3 +1118,23 @@ def test_paged_attention_read_of_a_padded_batch_is_zero_there():
     for x in (rk, rv):
         assert (x[[0, 4, 5, 6]] == 0).all() and (x[1:4].abs().sum((1, 2)) > 0).all()
     assert ok_status() == 0
+
+
+@pytest.mark.parametrize("engine", [1, 2])
+def test_attend_ragged_large_norms_far_into_long_segments(engine):
+    """Segments of more than 256 pages with a few pages of far larger value norms anywhere in them: as
+    the few-row kernel's 22-bit operands have it, within the bar of fp16 operands."""
+    D, Hq, H, T = 128, 8, 1, 1 << 17
+    tables = make_tables(D, 4, 2, False)
+    batch, start, _ = make_batch([(1500, T)])
+    pages = make_paged(tables, H, T)
+    fill(tables, pages, 1, H, T, 95)
+    norms = value_norms(tables, pages.pool)
+    norms *= 2.0 ** -9
+    far = torch.randperm(T // 64, generator=torch.Generator().manual_seed(4))[:12].to(DEV)
+    norms[pages.block_table[0, far].long()] *= 2.0 ** 12
+    q = 3 * randn((start[-1], Hq, D), 96, F32)
+    want = ops.attend_ragged(tables, pages, q, batch, engine=3).double().cpu().numpy()
+    got = ops.attend_ragged(tables, pages, q, batch, engine=engine)
+    check_attend(got, want, F32)
+    assert ok_status() == 0
