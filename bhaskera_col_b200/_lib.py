@@ -22,6 +22,7 @@ TQ_F32, TQ_F16, TQ_BF16 = 0, 1, 2
 DEV_WAIT_TIMEOUT, DEV_BAD_BLOCK, DEV_BAD_POSITION, DEV_BAD_BATCH = 1, 2, 4, 8
 PAGE_TOKENS = 64
 PHASE_QPREP, PHASE_DECODE, PHASE_MERGE = 1, 2, 4
+GATE_NONE, GATE_SIGMOID, GATE_TANH = 0, 1, 2
 
 # every symbol include/tq_b200.h declares
 EXPORTED = (
@@ -34,6 +35,7 @@ EXPORTED = (
     "tq_tables_bytes", "tq_init_tables",
     "tq_qk_rope", "tq_append_ragged", "tq_dequantize_ragged",
     "tq_attend_ragged_workspace_bytes", "tq_attend_ragged",
+    "tq_qk_rope_axes", "tq_append_ragged_axes", "tq_residual_norm",
 )
 MAX_PEERS = 8
 SHARED_HANDLE_BYTES = 64
@@ -111,6 +113,11 @@ class Positions(ctypes.Structure):
                 ("stride", ctypes.c_int64 * 2)]
 
 
+class RopeAxes(ctypes.Structure):
+    _fields_ = [("axes", ctypes.c_int32), ("stride", ctypes.c_int64),
+                ("axis", ctypes.c_uint8 * 128)]
+
+
 class Ragged(ctypes.Structure):
     _fields_ = [("requests", ctypes.c_int64), ("q_start", ctypes.c_void_p),
                 ("seq_lens", ctypes.c_void_p), ("max_q_len", ctypes.c_int64)]
@@ -120,6 +127,19 @@ class AttendArgs(ctypes.Structure):
     _fields_ = [("q", ctypes.POINTER(Tensor4)), ("out", ctypes.POINTER(Tensor4)),
                 ("batch", Ragged), ("scale", ctypes.c_float), ("causal", ctypes.c_int32),
                 ("engine", ctypes.c_int32)]
+
+
+class RowNorm(ctypes.Structure):
+    _fields_ = [("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("dtype", ctypes.c_int32),
+                ("eps", ctypes.c_float), ("offset", ctypes.c_float), ("centered", ctypes.c_int32)]
+
+
+class ResidualNormArgs(ctypes.Structure):
+    _fields_ = [("x", ctypes.POINTER(Tensor4)), ("residual", ctypes.POINTER(Tensor4)),
+                ("gate", ctypes.POINTER(Tensor4)), ("residual_out", ctypes.POINTER(Tensor4)),
+                ("out", ctypes.POINTER(Tensor4)), ("post", ctypes.POINTER(RowNorm)),
+                ("pre", ctypes.POINTER(RowNorm)), ("scale", ctypes.c_float),
+                ("gate_act", ctypes.c_int32)]
 
 
 _lock = threading.Lock()
@@ -167,7 +187,10 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
             "tq_init_tables": (I32, [P(Geom), VP, VP, VP, VP, VP, VP, VP, SZ, P(Tables), VP]),
             # descriptors of the serving operators are packed by ops.py: addresses
             "tq_qk_rope": (I32, [VP] * 9),
+            "tq_qk_rope_axes": (I32, [VP] * 10),
             "tq_append_ragged": (I32, [VP] * 10),
+            "tq_append_ragged_axes": (I32, [VP] * 11),
+            "tq_residual_norm": (I32, [VP] * 2),
             "tq_dequantize_ragged": (I32, [VP] * 7),
             "tq_attend_ragged_workspace_bytes": (SZ, [VP] * 3),
             "tq_attend_ragged": (I32, [VP] * 5 + [SZ, VP]),

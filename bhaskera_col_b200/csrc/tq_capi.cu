@@ -607,11 +607,23 @@ static int check_apart(const tq_tensor4* x, const tq_tensor4* y, bool in_place, 
   return TQ_ERR_INVALID;
 }
 
-int32_t tq_qk_rope(const tq_rope* rope, const tq_positions* pos, const tq_tensor4* q,
-                   const tq_tensor4* q_out, const tq_head_norm* q_norm, const tq_tensor4* k,
-                   const tq_tensor4* k_out, const tq_head_norm* k_norm, void* stream) {
-  NvtxRange range("tq_qk_rope");
-  const char* fn = "tq_qk_rope";
+static int check_axes(const tq_rope* rope, const tq_rope_axes* x, const char* fn) {
+  if (!x) return TQ_OK;
+  if (!rope) { set_error("%s: position axes come with a rotation", fn); return TQ_ERR_INVALID; }
+  bool ok = x->axes >= 1 && x->axes <= 4;
+  for (int i = 0; ok && i < rope->rot_dim / 2; ++i) ok = x->axis[i] < x->axes;
+  if (!ok) {
+    set_error("%s: 1 to 4 position axes, and each pair's axis one of them", fn);
+    return TQ_ERR_INVALID;
+  }
+  return TQ_OK;
+}
+
+static int qk_rope(const tq_rope* rope, const tq_rope_axes* axes, const tq_positions* pos,
+                   const tq_tensor4* q, const tq_tensor4* q_out, const tq_head_norm* q_norm,
+                   const tq_tensor4* k, const tq_tensor4* k_out, const tq_head_norm* k_norm,
+                   void* stream, const char* fn) {
+  NvtxRange range(fn);
   const tq_tensor4* x[2] = {q, k};
   const tq_tensor4* y[2] = {q_out, k_out};
   const tq_head_norm* norm[2] = {q_norm, k_norm};
@@ -656,13 +668,26 @@ int32_t tq_qk_rope(const tq_rope* rope, const tq_positions* pos, const tq_tensor
     set_error("%s: head_dim %lld is outside [1, 256]", fn, (long long)D);
     return TQ_ERR_INVALID;
   }
-  if ((rc = check_rope(rope, D, fn))) return rc;
+  if ((rc = check_rope(rope, D, fn)) || (rc = check_axes(rope, axes, fn))) return rc;
   if (rope && !pos) { set_error("%s: a rotation needs positions", fn); return TQ_ERR_INVALID; }
   if (one->shape[0] * one->shape[2] == 0) return TQ_OK;
   if ((rc = check_positions(pos, fn))) return rc;
   uint32_t* status = device_status_word();
   if (!status) { set_error("%s: device status word unavailable", fn); return TQ_ERR_CUDA; }
-  return launch_qk_rope(rope, pos, x, y, norm, status, (cudaStream_t)stream);
+  return launch_qk_rope(rope, axes, pos, x, y, norm, status, (cudaStream_t)stream);
+}
+
+int32_t tq_qk_rope(const tq_rope* rope, const tq_positions* pos, const tq_tensor4* q,
+                   const tq_tensor4* q_out, const tq_head_norm* q_norm, const tq_tensor4* k,
+                   const tq_tensor4* k_out, const tq_head_norm* k_norm, void* stream) {
+  return qk_rope(rope, nullptr, pos, q, q_out, q_norm, k, k_out, k_norm, stream, "tq_qk_rope");
+}
+
+int32_t tq_qk_rope_axes(const tq_rope* rope, const tq_rope_axes* axes, const tq_positions* pos,
+                        const tq_tensor4* q, const tq_tensor4* q_out, const tq_head_norm* q_norm,
+                        const tq_tensor4* k, const tq_tensor4* k_out, const tq_head_norm* k_norm,
+                        void* stream) {
+  return qk_rope(rope, axes, pos, q, q_out, q_norm, k, k_out, k_norm, stream, "tq_qk_rope_axes");
 }
 
 static int check_ragged(const tq_ragged* b, const tq_cache* c, const char* fn) {
@@ -691,19 +716,19 @@ static int check_flat(const tq_tensor4* x, const char* what, int64_t heads, cons
   return TQ_OK;
 }
 
-int32_t tq_append_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
+static int append_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                          const tq_tensor4* k, const tq_tensor4* v, const tq_ragged* batch,
-                         const tq_rope* rope, const tq_head_norm* k_norm,
-                         const tq_positions* pos, void* stream) {
-  NvtxRange range("tq_append_ragged");
-  const char* fn = "tq_append_ragged";
+                         const tq_rope* rope, const tq_rope_axes* axes, const tq_head_norm* k_norm,
+                         const tq_positions* pos, void* stream, const char* fn) {
+  NvtxRange range(fn);
   int rc;
   if ((rc = check_geom(g, fn)) || (rc = check_tables(g, t, fn)) || (rc = check_cache(c, fn)) ||
       (rc = check_ragged(batch, c, fn)))
     return rc;
   const int64_t heads = c->streams / batch->requests;
   if ((rc = check_flat(k, "k", heads, g, fn)) || (rc = check_flat(v, "v", heads, g, fn)) ||
-      (rc = check_rope(rope, g->head_dim, fn)) || (rc = check_norm(k_norm, fn)) ||
+      (rc = check_rope(rope, g->head_dim, fn)) || (rc = check_axes(rope, axes, fn)) ||
+      (rc = check_norm(k_norm, fn)) ||
       (k->shape[2] > 0 && (rc = check_positions(pos, fn))))
     return rc;
   if (g->head_dim > 128 || g->qjl) {
@@ -717,8 +742,23 @@ int32_t tq_append_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c
   }
   uint32_t* status = device_status_word();
   if (!status) { set_error("%s: device status word unavailable", fn); return TQ_ERR_CUDA; }
-  return launch_append_ragged(g, t, c, k, v, batch, rope, k_norm, pos, status,
+  return launch_append_ragged(g, t, c, k, v, batch, rope, axes, k_norm, pos, status,
                               (cudaStream_t)stream);
+}
+
+int32_t tq_append_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
+                         const tq_tensor4* k, const tq_tensor4* v, const tq_ragged* batch,
+                         const tq_rope* rope, const tq_head_norm* k_norm,
+                         const tq_positions* pos, void* stream) {
+  return append_ragged(g, t, c, k, v, batch, rope, nullptr, k_norm, pos, stream, "tq_append_ragged");
+}
+
+int32_t tq_append_ragged_axes(const tq_geom* g, const tq_tables* t, const tq_cache* c,
+                              const tq_tensor4* k, const tq_tensor4* v, const tq_ragged* batch,
+                              const tq_rope* rope, const tq_rope_axes* axes,
+                              const tq_head_norm* k_norm, const tq_positions* pos, void* stream) {
+  return append_ragged(g, t, c, k, v, batch, rope, axes, k_norm, pos, stream,
+                       "tq_append_ragged_axes");
 }
 
 int32_t tq_dequantize_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
@@ -750,6 +790,68 @@ int32_t tq_dequantize_ragged(const tq_geom* g, const tq_tables* t, const tq_cach
   uint32_t* status = device_status_word();
   if (!status) { set_error("%s: device status word unavailable", fn); return TQ_ERR_CUDA; }
   return launch_dequant_ragged(g, t, c, batch, k_out, v_out, status, (cudaStream_t)stream);
+}
+
+static int check_row_norm(const tq_row_norm* n, const char* what, const char* fn) {
+  if (!n) return TQ_OK;
+  if (!valid_dtype(n->dtype) || !(n->eps >= 0.f) ||
+      (reinterpret_cast<uintptr_t>(n->weight) | reinterpret_cast<uintptr_t>(n->bias)) %
+          (n->dtype == TQ_F32 ? 4 : 2)) {
+    set_error("%s: %s needs aligned parameters of a supported type and eps >= 0", fn, what);
+    return TQ_ERR_INVALID;
+  }
+  return TQ_OK;
+}
+
+int32_t tq_residual_norm(const tq_residual_norm_args* a, void* stream) {
+  NvtxRange range("tq_residual_norm");
+  const char* fn = "tq_residual_norm";
+  int rc;
+  if (!a || !a->x || !a->residual || !a->residual_out) {
+    set_error("%s: x, residual and residual_out are needed", fn);
+    return TQ_ERR_INVALID;
+  }
+  if ((a->out == nullptr) != (a->pre == nullptr)) {
+    set_error("%s: out comes with the norm behind the sum", fn);
+    return TQ_ERR_INVALID;
+  }
+  const tq_tensor4* all[5] = {a->x, a->residual, a->gate, a->residual_out, a->out};
+  const char* names[5] = {"x", "residual", "gate", "residual_out", "out"};
+  for (int i = 0; i < 5; ++i) {
+    if (!all[i]) continue;
+    if ((rc = check_maybe_empty(all[i], names[i], fn)) ||
+        (i >= 3 && (rc = check_written(all[i], names[i], fn))))
+      return rc;
+    for (int d = 0; d < 4; ++d)
+      if (all[i]->shape[d] != a->x->shape[d]) {
+        set_error("%s: shapes of x and %s disagree", fn, names[i]);
+        return TQ_ERR_INVALID;
+      }
+  }
+  if (a->residual_out->dtype != a->residual->dtype || (a->out && a->out->dtype != a->x->dtype)) {
+    set_error("%s: an output has the type of its input", fn);
+    return TQ_ERR_INVALID;
+  }
+  if ((rc = check_row_norm(a->post, "post", fn)) || (rc = check_row_norm(a->pre, "pre", fn))) return rc;
+  if (a->gate_act < TQ_GATE_NONE || a->gate_act > TQ_GATE_TANH) {
+    set_error("%s: gate_act must be 0 (none), 1 (sigmoid) or 2 (tanh), got %d", fn, a->gate_act);
+    return TQ_ERR_INVALID;
+  }
+  const int64_t* n = a->x->shape;
+  if (n[3] < 1 || n[3] > 32768) {
+    set_error("%s: rows of %lld values, 1 to 32768 are supported", fn, (long long)n[3]);
+    return TQ_ERR_INVALID;
+  }
+  if (n[0] && n[1] && n[2] && (n[0] > INT32_MAX / n[1] || n[0] * n[1] > INT32_MAX / n[2])) {
+    set_error("%s: 2^31 rows or more", fn);
+    return TQ_ERR_INVALID;
+  }
+  for (int o = 3; o < 5; ++o)
+    for (int i = 0; i < o; ++i) {
+      const bool own = (o == 3 && i == 1) || (o == 4 && i == 0);
+      if (all[o] && all[i] && (rc = check_apart(all[i], all[o], own, names[o], names[i], fn))) return rc;
+    }
+  return launch_residual_norm(a, (cudaStream_t)stream);
 }
 
 static int check_attend(const tq_geom* g, const tq_cache* c, const tq_attend_args* a,

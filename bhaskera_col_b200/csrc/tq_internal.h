@@ -62,15 +62,16 @@ int launch_decode(const tq_geom* g, const tq_tables* t, const tq_cache* c,
 struct HeadXform;
 struct RaggedView;
 struct RaggedAttend;
-HeadXform head_xform(const tq_rope* rope, const tq_head_norm* norm);
+HeadXform head_xform(const tq_rope* rope, const tq_rope_axes* axes, const tq_head_norm* norm);
 RaggedView ragged_view(const tq_ragged* b, int64_t N, const tq_cache* c);
-int launch_qk_rope(const tq_rope* rope, const tq_positions* pos, const tq_tensor4* const x[2],
+int launch_qk_rope(const tq_rope* rope, const tq_rope_axes* axes, const tq_positions* pos, const tq_tensor4* const x[2],
                    const tq_tensor4* const y[2], const tq_head_norm* const norm[2],
                    uint32_t* status, cudaStream_t st);
+int launch_residual_norm(const tq_residual_norm_args* a, cudaStream_t st);
 int launch_append_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                          const tq_tensor4* k, const tq_tensor4* v, const tq_ragged* batch,
-                         const tq_rope* rope, const tq_head_norm* norm, const tq_positions* pos,
-                         uint32_t* status, cudaStream_t st);
+                         const tq_rope* rope, const tq_rope_axes* axes, const tq_head_norm* norm,
+                         const tq_positions* pos, uint32_t* status, cudaStream_t st);
 int launch_dequant_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                           const tq_ragged* batch, const tq_tensor4* ko, const tq_tensor4* vo,
                           uint32_t* status, cudaStream_t st);
@@ -78,8 +79,8 @@ int launch_dequant_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* 
 // not apply (the caller runs the CUDA-core kernels), or an error.
 int launch_append_ragged_tc(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                             const tq_tensor4* k, const tq_tensor4* v, const tq_ragged* batch,
-                            const tq_rope* rope, const tq_head_norm* norm, const tq_positions* pos,
-                            uint32_t* status, cudaStream_t st);
+                            const tq_rope* rope, const tq_rope_axes* axes, const tq_head_norm* norm,
+                            const tq_positions* pos, uint32_t* status, cudaStream_t st);
 int launch_dequant_ragged_tc(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                              const tq_ragged* batch, const tq_tensor4* ko, const tq_tensor4* vo,
                              uint32_t* status, cudaStream_t st);

@@ -1,0 +1,348 @@
+// tq_norm.cu — a block's output onto the residual stream, and the next block's
+// norm of the sum (tq_residual_norm), a row at a time:
+//   z = post(x),  y = residual + scale act(gate) z,  h = pre(y)
+// with norms (x - mean) / sqrt(mean (x - mean)^2 + eps) (w + offset) + b, the
+// mean taken off only where the norm is centred (layer norm; else RMS norm).
+//
+// Bound by HBM: x, residual and a gate of its own per element are read once, y and h
+// written once.  T threads hold a row in registers, 8 VPT values each, so that the
+// sums of both norms need no second read; h is formed from y before its rounding.
+// Sums go by shuffles and one barrier each, always in the same order.
+#include "tq_common.cuh"
+#include "tq_internal.h"
+
+#include <type_traits>
+
+namespace tq {
+namespace {
+
+struct NormSide {
+  int on, centered, dtype;
+  const void* w;                // [C] or NULL: ones
+  const void* b;                // [C] or NULL: zeros
+  float eps, offset;
+};
+
+struct NormParams {
+  const void* x; const void* r; const void* g;
+  void* y; void* h;             // h: NULL without a norm behind the sum
+  int gd;                       // gate's type
+  int gmode;                    // 0: none, 1: a value per element, 2: one per row
+  int act;
+  float scale;
+  int64_t xs[4], rs[4], gs[4], ys[4], hs[4];
+  int64_t rows, n1, n2;         // rows: [rows / (n1 n2)][n1][n2], below 2^31
+  int C;
+  NormSide post, pre;
+};
+
+// V consecutive values of type DT, as they lie in memory.
+template <int DT, int V>
+struct Chunk {
+  static constexpr int ES = DT == TQ_F32 ? 4 : 2, B = ES * V;
+  using Word = typename std::conditional<B == 2, uint16_t, uint32_t>::type;
+  static constexpr int NW = B < 4 ? 1 : B / 4;
+  Word w[NW];
+  __device__ __forceinline__ void load(const void* base, int64_t i) {
+    // plain loads: an output may be its input
+    const char* at = static_cast<const char*>(base) + i * ES;
+    if constexpr (B >= 16) {
+#pragma unroll
+      for (int k = 0; k < NW; k += 4) {
+        const uint4 u = *reinterpret_cast<const uint4*>(at + 4 * k);
+        w[k] = u.x; w[k + 1] = u.y; w[k + 2] = u.z; w[k + 3] = u.w;
+      }
+    } else if constexpr (B == 8) {
+      const uint2 u = *reinterpret_cast<const uint2*>(at);
+      w[0] = u.x; w[1] = u.y;
+    } else {
+      w[0] = *reinterpret_cast<const Word*>(at);
+    }
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int k = 0; k < NW; ++k) w[k] = 0;
+  }
+  __device__ __forceinline__ float get(int e) const {
+    if constexpr (DT == TQ_F32) return __uint_as_float(w[e]);
+    else {
+      const uint32_t u = V == 1 ? (uint32_t)w[0] : (uint32_t)w[e / 2] >> (16 * (e & 1));
+      if constexpr (DT == TQ_BF16) return __uint_as_float(u << 16);
+      else return __half2float(__ushort_as_half((unsigned short)u));
+    }
+  }
+  static __device__ __forceinline__ void store(void* base, int64_t i, const float* v) {
+    char* at = static_cast<char*>(base) + i * ES;
+    uint32_t o[NW];
+    if constexpr (DT == TQ_F32) {
+#pragma unroll
+      for (int k = 0; k < NW; ++k) o[k] = __float_as_uint(v[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < NW; ++k) {
+        const float lo = v[2 * k], hi = V == 1 ? 0.f : v[2 * k + (V > 1)];
+        if constexpr (DT == TQ_BF16) {
+          const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+          o[k] = *reinterpret_cast<const uint32_t*>(&b);
+        } else {
+          o[k] = pack_half2(lo, hi);
+        }
+      }
+    }
+    if constexpr (B >= 16) {
+#pragma unroll
+      for (int k = 0; k < NW; k += 4)
+        *reinterpret_cast<uint4*>(at + 4 * k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+    } else if constexpr (B == 8) {
+      *reinterpret_cast<uint2*>(at) = make_uint2(o[0], o[1]);
+    } else {
+      *reinterpret_cast<Word*>(at) = (Word)o[0];
+    }
+  }
+};
+
+// V values of a parameter of any of the types (contiguous; V >= 2 aligned to V values).
+template <int V>
+__device__ __forceinline__ void load_param(float (&v)[V], const void* base, int dtype, int64_t i) {
+  if (dtype == TQ_F32) {
+    Chunk<TQ_F32, V> c;
+    c.load(base, i);
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = c.get(e);
+  } else {
+    Chunk<TQ_F16, V> c;
+    c.load(base, i);
+    if (dtype == TQ_F16) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = c.get(e);
+    } else {
+      Chunk<TQ_BF16, V> d;
+#pragma unroll
+      for (int k = 0; k < c.NW; ++k) d.w[k] = c.w[k];
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = d.get(e);
+    }
+  }
+}
+
+__device__ __forceinline__ float activate(float g, int act) {
+  return act == TQ_GATE_SIGMOID ? 1.f / (1.f + expf(-g)) : act == TQ_GATE_TANH ? tanhf(g) : g;
+}
+
+// Sum over the T threads of a row: a warp by itself, or a CTA through `part`, whose
+// two halves take turns, so that one barrier a sum is enough.
+__device__ __forceinline__ float row_sum(float x, int T, float (*part)[32], int& turn) {
+  x = warp_sum(x);
+  if (T == 32) return x;
+  const int warps = T / 32;
+  if ((threadIdx.x & 31) == 0) part[turn][threadIdx.x >> 5] = x;
+  __syncthreads();
+  float s = 0.f;
+  for (int i = 0; i < warps; ++i) s += part[turn][i];
+  turn ^= 1;
+  return s;
+}
+
+// T threads per row (a warp, or the CTA), 8 VPT values each in chunks of V
+// neighbours.  V = 1 takes any stride.
+template <int XT, int RT, int VPT, int V>
+__global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) residual_norm_kernel(NormParams p, int T) {
+  constexpr int NK = 8 * VPT / V;                          // chunks of a thread
+  __shared__ float part[2][32];
+  int turn = 0;
+  const int t = threadIdx.x % T;
+  const int64_t row = (int64_t)blockIdx.x * (blockDim.x / T) + threadIdx.x / T;
+  if (row >= p.rows) return;                               // whole warps where a row is one's
+  const uint32_t n1 = (uint32_t)p.n1, n2 = (uint32_t)p.n2, i01 = (uint32_t)row / n2;
+  const uint32_t i2 = (uint32_t)row - i01 * n2, i0 = i01 / n1, i1 = i01 - i0 * n1;
+  auto at = [&](const int64_t (&s)[4]) { return i0 * s[0] + i1 * s[1] + i2 * s[2]; };
+  const int64_t xb = at(p.xs), rb = at(p.rs);
+  // values of chunk k: from column c(k) on
+  auto col = [&](int k) { return (k * T + t) * V; };
+  auto inside = [&](int k) { return col(k) < p.C; };       // C is a multiple of V
+  auto place = [&](const int64_t (&s)[4], int k) { return V == 1 ? col(k) * s[3] : (int64_t)col(k); };
+  Chunk<XT, V> xr[NK];
+  Chunk<RT, V> rr[NK];
+#pragma unroll
+  for (int k = 0; k < NK; ++k) {
+    xr[k].clear();
+    rr[k].clear();
+    if (inside(k)) {
+      xr[k].load(p.x, xb + place(p.xs, k));
+      rr[k].load(p.r, rb + place(p.rs, k));
+    }
+  }
+  float v[NK][V];
+#pragma unroll
+  for (int k = 0; k < NK; ++k)
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[k][e] = xr[k].get(e);
+  const float inv_c = 1.f / (float)p.C;
+  auto norm = [&](const NormSide& s) {
+    if (s.centered) {
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < NK; ++k)
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum += v[k][e];
+      const float mean = row_sum(sum, T, part, turn) * inv_c;
+#pragma unroll
+      for (int k = 0; k < NK; ++k)
+        if (inside(k))
+#pragma unroll
+          for (int e = 0; e < V; ++e) v[k][e] -= mean;
+    }
+    float ss = 0.f;
+#pragma unroll
+    for (int k = 0; k < NK; ++k)
+#pragma unroll
+      for (int e = 0; e < V; ++e) ss = fmaf(v[k][e], v[k][e], ss);
+    const float r = 1.f / sqrtf(fmaf(row_sum(ss, T, part, turn), inv_c, s.eps));
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+      if (!inside(k)) continue;
+      float w[V], b[V];
+      if (s.w) load_param<V>(w, s.w, s.dtype, col(k));
+      if (s.b) load_param<V>(b, s.b, s.dtype, col(k));
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        v[k][e] = v[k][e] * r * (s.w ? w[e] + s.offset : 1.f);
+        if (s.b) v[k][e] += b[e];
+      }
+    }
+  };
+  if (p.post.on) norm(p.post);
+  const int64_t gb = p.gmode ? at(p.gs) : 0;
+  float one = p.scale;
+  if (p.gmode == 2) one *= activate(load_elem(p.g, p.gd, gb), p.act);
+  const int64_t yb = at(p.ys);
+#pragma unroll
+  for (int k = 0; k < NK; ++k) {
+    if (!inside(k)) continue;
+    float g[V];
+    if (p.gmode == 1) load_param<V>(g, p.g, p.gd, gb + place(p.gs, k));
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float f = p.gmode == 1 ? one * activate(g[e], p.act) : one;
+      v[k][e] = fmaf(f, v[k][e], rr[k].get(e));
+    }
+    Chunk<RT, V>::store(p.y, yb + place(p.ys, k), v[k]);
+  }
+  if (!p.h) return;
+  norm(p.pre);
+  const int64_t hb = at(p.hs);
+#pragma unroll
+  for (int k = 0; k < NK; ++k)
+    if (inside(k)) Chunk<XT, V>::store(p.h, hb + place(p.hs, k), v[k]);
+}
+
+using NormFn = void (*)(NormParams, int);
+
+template <int XT, int RT>
+NormFn norm_fn(int vpt, int v) {
+#define TQ_NORM(N, V) if (vpt == N && v == V) return residual_norm_kernel<XT, RT, N, V>;
+  TQ_NORM(1, 8) TQ_NORM(2, 8) TQ_NORM(4, 8) TQ_NORM(8, 8)
+  TQ_NORM(1, 2) TQ_NORM(2, 2) TQ_NORM(4, 2) TQ_NORM(8, 2)
+  TQ_NORM(1, 1) TQ_NORM(2, 1) TQ_NORM(4, 1) TQ_NORM(8, 1)
+#undef TQ_NORM
+  return nullptr;
+}
+
+template <int XT>
+NormFn norm_fn_x(int rd, int vpt, int v) {
+  return rd == TQ_F32 ? norm_fn<XT, TQ_F32>(vpt, v)
+         : rd == TQ_F16 ? norm_fn<XT, TQ_F16>(vpt, v) : norm_fn<XT, TQ_BF16>(vpt, v);
+}
+
+NormSide norm_side(const tq_row_norm* n) {
+  NormSide s = {};
+  if (!n) return s;
+  s.on = 1;
+  s.centered = n->centered;
+  s.dtype = n->dtype;
+  s.w = n->weight;
+  s.b = n->bias;
+  s.eps = n->eps;
+  s.offset = n->offset;
+  return s;
+}
+
+// Are rows of the view read and written v neighbours at a time?
+bool takes_chunks(const tq_tensor4* x, int v) {
+  const int bytes = tmin(16, v * (x->dtype == TQ_F32 ? 4 : 2));
+  const int es = x->dtype == TQ_F32 ? 4 : 2;
+  if (x->shape[3] % v || (x->shape[3] > 1 && x->stride[3] != 1) ||
+      reinterpret_cast<uintptr_t>(x->data) % bytes)
+    return false;
+  for (int i = 0; i < 3; ++i)
+    if (x->shape[i] > 1 && (x->stride[i] * es) % bytes) return false;
+  return true;
+}
+
+bool param_takes_chunks(const tq_row_norm* n, int v) {
+  if (!n) return true;
+  const int bytes = tmin(16, v * (n->dtype == TQ_F32 ? 4 : 2));
+  return (reinterpret_cast<uintptr_t>(n->weight) | reinterpret_cast<uintptr_t>(n->bias)) % bytes == 0;
+}
+
+}  // namespace
+
+int launch_residual_norm(const tq_residual_norm_args* a, cudaStream_t st) {
+  NormParams p = {};
+  const tq_tensor4 *x = a->x, *r = a->residual, *g = a->gate;
+  p.rows = x->shape[0] * x->shape[1] * x->shape[2];
+  if (p.rows == 0) return TQ_OK;
+  p.n1 = x->shape[1];
+  p.n2 = x->shape[2];
+  p.C = (int)x->shape[3];
+  p.x = x->data;
+  p.r = r->data;
+  p.y = a->residual_out->data;
+  p.h = a->pre ? a->out->data : nullptr;
+  for (int i = 0; i < 4; ++i) {
+    p.xs[i] = x->stride[i];
+    p.rs[i] = r->stride[i];
+    p.ys[i] = a->residual_out->stride[i];
+    if (p.h) p.hs[i] = a->out->stride[i];
+    if (g) p.gs[i] = g->stride[i];
+  }
+  if (g) {
+    p.g = g->data;
+    p.gd = g->dtype;
+    p.gmode = g->stride[3] == 0 ? 2 : 1;
+    p.act = a->gate_act;
+  }
+  p.scale = a->scale;
+  p.post = norm_side(a->post);
+  p.pre = norm_side(a->pre);
+  int v = 1;
+  for (int c : {8, 2}) {
+    if (takes_chunks(x, c) && takes_chunks(r, c) && takes_chunks(a->residual_out, c) &&
+        (!p.h || takes_chunks(a->out, c)) && (p.gmode != 1 || takes_chunks(g, c)) &&
+        param_takes_chunks(a->post, c) && param_takes_chunks(a->pre, c)) {
+      v = c;
+      break;
+    }
+  }
+  // Threads of a row and their values, 8 vpt each: 32 of them leave most rows in flight on
+  // an SM, 8 end a call of few rows sooner; 64 only where 512 threads need them.
+  const int units = (p.C + 7) / 8;
+  int vpt, T;
+  if (units <= 128) {
+    T = 32;
+    vpt = units <= 32 ? 1 : units <= 64 ? 2 : 4;
+  } else {
+    const bool few = p.rows <= 2 * device_sm_count();
+    vpt = few && units <= 1024 ? 1 : few && units <= 2048 ? 2 : units <= 2048 ? 4 : 8;
+    T = ((units + vpt - 1) / vpt + 31) & ~31;
+  }
+  const NormFn fn = x->dtype == TQ_F32   ? norm_fn_x<TQ_F32>(r->dtype, vpt, v)
+                    : x->dtype == TQ_F16 ? norm_fn_x<TQ_F16>(r->dtype, vpt, v)
+                                         : norm_fn_x<TQ_BF16>(r->dtype, vpt, v);
+  const int per = T == 32 ? 4 : 1;
+  const int64_t grid = (p.rows + per - 1) / per;
+  fn<<<(unsigned)grid, T * per, 0, st>>>(p, T);
+  return check_launch("tq_residual_norm");
+}
+
+}  // namespace tq

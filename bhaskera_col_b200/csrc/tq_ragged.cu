@@ -12,8 +12,14 @@
 
 namespace tq {
 
-HeadXform head_xform(const tq_rope* rope, const tq_head_norm* norm) {
+HeadXform head_xform(const tq_rope* rope, const tq_rope_axes* axes, const tq_head_norm* norm) {
   HeadXform f = {};
+  if (rope && axes) {
+    f.axes.n = axes->axes;
+    f.axes.stride = axes->stride;
+    for (int i = 0; i < rope->rot_dim / 2; ++i)
+      f.axes.of[i >> 4] |= (uint32_t)axes->axis[i] << (2 * (i & 15));
+  }
   if (rope) {
     f.cos_sin = rope->cos_sin;
     f.positions = rope->positions;
@@ -121,15 +127,14 @@ __global__ void __launch_bounds__(kThreadsR) append_ragged_kernel(RaggedKV p) {
         uv[c] = load_elem(p.x[which], p.dtype[which], base + c * p.stride[which][2]);
       __syncwarp();
       if (which == 0 && (p.f.weight || p.f.cos_sin)) {
-        int64_t row = 0;
-        if (p.f.cos_sin) {
-          int64_t at = pos;
-          if (p.pos)
-            at = p.pos64 ? reinterpret_cast<const long long*>(p.pos)[n * p.pos_stride]
-                         : (int64_t)reinterpret_cast<const int*>(p.pos)[n * p.pos_stride];
-          row = table_row(p.f, at, p.status);
+        if (p.f.axes.n) {
+          xform_axes(uv, D, p.f, p.pos, p.pos64, n * p.pos_stride, p.status, lane);
+        } else {
+          int64_t row = 0;
+          if (p.f.cos_sin)
+            row = table_row(p.f, p.pos ? load_pos(p.pos, p.pos64, n * p.pos_stride) : pos, p.status);
+          xform_row(uv, D, p.f, row, lane);
         }
-        xform_row(uv, D, p.f, row, lane);
       }
       float ss = 0.f;
       for (int c = lane; c < D; c += 32) ss = fmaf(uv[c], uv[c], ss);
@@ -235,18 +240,19 @@ RaggedKV ragged_kv(const tq_geom* G, const tq_tables* t, const tq_cache* c, cons
 
 int launch_append_ragged(const tq_geom* G, const tq_tables* t, const tq_cache* c,
                          const tq_tensor4* k, const tq_tensor4* v, const tq_ragged* batch,
-                         const tq_rope* rope, const tq_head_norm* norm, const tq_positions* pos,
-                         uint32_t* status, cudaStream_t st) {
+                         const tq_rope* rope, const tq_rope_axes* axes, const tq_head_norm* norm,
+                         const tq_positions* pos, uint32_t* status, cudaStream_t st) {
+  if (!pos) axes = nullptr;                                // every axis at the token's position
   RaggedKV p = ragged_kv(G, t, c, k, v, batch);
   p.R = t->rot_t;
   p.status = status;
-  p.f = head_xform(rope, norm);
+  p.f = head_xform(rope, axes, norm);
   p.pos = pos ? pos->data : nullptr;
   p.pos64 = pos && pos->bits == 64;
   p.pos_stride = pos ? pos->stride[1] : 0;
   const int64_t nvec = p.rv.N * p.H;
   if (nvec == 0) return TQ_OK;
-  if (const int rc = launch_append_ragged_tc(G, t, c, k, v, batch, rope, norm, pos, status, st); rc != 1)
+  if (const int rc = launch_append_ragged_tc(G, t, c, k, v, batch, rope, axes, norm, pos, status, st); rc != 1)
     return rc;
   const int D = G->head_dim;
   const size_t smem = D == 32 ? append_ragged_smem<32>() : D == 64 ? append_ragged_smem<64>()

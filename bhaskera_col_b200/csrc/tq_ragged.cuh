@@ -84,6 +84,15 @@ __device__ __forceinline__ bool locate_row(const RaggedView& v, int64_t n, int64
 // ---------------------------------------------------------------------------
 // x -> rotation(rms_norm(x)) of one head vector
 // ---------------------------------------------------------------------------
+// Position axes: pair i turns by the token's position on axis `of`[i], 2 bits a pair;
+// n = 0: one axis.
+struct AxisMap {
+  int n;
+  int64_t stride;             // of positions, from axis to axis
+  uint32_t of[8];
+  __device__ __forceinline__ int axis(int pair) const { return (of[pair >> 4] >> (2 * (pair & 15))) & 3; }
+};
+
 struct HeadXform {
   const float* cos_sin;       // [positions][rot]: cosines, then sines; NULL: no rotation
   int64_t positions;
@@ -91,7 +100,13 @@ struct HeadXform {
   const void* weight;         // [D] or NULL: no norm
   int w_dtype;
   float eps, w_offset;
+  AxisMap axes;
 };
+
+__device__ __forceinline__ int64_t load_pos(const void* pos, int pos64, int64_t i) {
+  return pos64 ? __ldg(reinterpret_cast<const long long*>(pos) + i)
+               : (int64_t)__ldg(reinterpret_cast<const int*>(pos) + i);
+}
 
 // Row index of a position in the rotation table; positions outside it take
 // row 0 and set TQ_DEV_BAD_POSITION.
@@ -103,8 +118,10 @@ __device__ __forceinline__ int64_t table_row(const HeadXform& f, int64_t pos, ui
 
 // One warp, the vector in shared memory (u[0..D), already visible to the
 // warp): norm and rotation in fp32, in place; visible to the warp on return.
-__device__ __forceinline__ void xform_row(float* u, int D, const HeadXform& f, int64_t row,
-                                          int lane) {
+// row_of(i) is the table's row for pair i.
+template <class RowOf>
+__device__ __forceinline__ void xform_row(float* u, int D, const HeadXform& f, int lane,
+                                          RowOf row_of) {
   if (f.weight) {
     float ss = 0.f;
     for (int c = lane; c < D; c += 32) ss = fmaf(u[c], u[c], ss);
@@ -115,14 +132,66 @@ __device__ __forceinline__ void xform_row(float* u, int D, const HeadXform& f, i
   }
   if (f.cos_sin) {
     const int half = f.rot / 2;
-    const float* cs = f.cos_sin + row * f.rot;
     for (int i = lane; i < half; i += 32) {
+      const float* cs = f.cos_sin + row_of(i) * f.rot;
       const int ia = f.interleaved ? 2 * i : i, ib = f.interleaved ? 2 * i + 1 : half + i;
       const float a = u[ia], b = u[ib], c = __ldg(cs + i), s = __ldg(cs + half + i);
       u[ia] = a * c - b * s;
       u[ib] = b * c + a * s;
     }
     __syncwarp();
+  }
+}
+
+// The same at one row for all pairs, or at the token's positions pos[at], a row an axis.
+__device__ __forceinline__ void xform_row(float* u, int D, const HeadXform& f, int64_t row,
+                                          int lane) {
+  xform_row(u, D, f, lane, [&](int) { return row; });
+}
+__device__ __forceinline__ void xform_axes(float* u, int D, const HeadXform& f, const void* pos,
+                                           int pos64, int64_t at, uint32_t* status, int lane) {
+  xform_row(u, D, f, lane, [&](int i) {
+    return table_row(f, load_pos(pos, pos64, at + f.axes.axis(i) * f.axes.stride), status);
+  });
+}
+
+// cos and sin of N neighbouring pairs from pair i0 on (a multiple of N), each from its
+// own axis' row of the table; row_of(a) is axis a's.  An axis that none of the pairs
+// follows is not read.  The table's row and its halves are N-aligned.
+template <int N, class RowOf>
+__device__ __forceinline__ void load_axes(float (&cs)[N], float (&sn)[N], const HeadXform& f, int i0,
+                                          RowOf row_of) {
+  const int half = f.rot / 2;
+  const uint32_t of = f.axes.of[i0 >> 4] >> (2 * (i0 & 15));
+#pragma unroll
+  for (int a = 0; a < 4; ++a) {
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < N; ++e) any = any || ((of >> (2 * e)) & 3u) == (uint32_t)a;
+    if (a >= f.axes.n || !any) continue;
+    const float* tab = f.cos_sin + row_of(a) * f.rot + i0;
+    float c[N], s[N];
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+      for (int e = 0; e < N; e += 4) {
+        const float4 x = __ldg(reinterpret_cast<const float4*>(tab + e));
+        const float4 y = __ldg(reinterpret_cast<const float4*>(tab + half + e));
+        c[e] = x.x; c[e + 1] = x.y; c[e + 2] = x.z; c[e + 3] = x.w;
+        s[e] = y.x; s[e + 1] = y.y; s[e + 2] = y.z; s[e + 3] = y.w;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        c[e] = __ldg(tab + e);
+        s[e] = __ldg(tab + half + e);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const bool mine = ((of >> (2 * e)) & 3u) == (uint32_t)a;
+      cs[e] = mine ? c[e] : cs[e];
+      sn[e] = mine ? s[e] : sn[e];
+    }
   }
 }
 

@@ -197,7 +197,7 @@ __device__ __forceinline__ void stage_rotation(unsigned char* b, const float* ro
 struct Vecs {
   uint8_t* page[kM];                       // NULL: no place
   int slot[kM];                            // token in its page
-  int row[kM];                             // row of the rotation table
+  int row[kM];                             // row of the rotation table; several axes: of the batch
   float n[kM];                             // norm
   float inv[kM];                           // append: factor of the accumulator
   uint8_t state[kM];                       // 0: row of no request, 1: no place, 2: stored
@@ -299,7 +299,9 @@ __device__ __forceinline__ void locate_tiles(const RaggedTc& p, const Pipe& pp, 
       if (state[k] && !in) atomicOr(p.status, TQ_DEV_BAD_POSITION);
       entry[k] = in ? page_entry(p.pm, (int64_t)lo * p.H + h, pos[k] / kPageTokens) : -1;
       to[k] = pos[k];
-      if (p.pos && in)
+      if (p.f.axes.n)
+        to[k] = n[k];
+      else if (p.pos && in)
         to[k] = p.pos64
                     ? (int64_t)__ldg(reinterpret_cast<const long long*>(p.pos) + n[k] * p.pos_stride)
                     : (int64_t)__ldg(reinterpret_cast<const int*>(p.pos) + n[k] * p.pos_stride);
@@ -315,7 +317,8 @@ __device__ __forceinline__ void locate_tiles(const RaggedTc& p, const Pipe& pp, 
       const bool in = state[k] == 2;
       ring[e].page[at] = in ? p.pages + entry[k] * (int64_t)p.g.page_bytes : nullptr;
       ring[e].slot[at] = (int)(pos[k] & (kPageTokens - 1));
-      ring[e].row[at] = in && p.f.cos_sin ? (int)table_row(p.f, to[k], p.status) : 0;
+      ring[e].row[at] = !in || !p.f.cos_sin ? 0
+                        : p.f.axes.n ? (int)to[k] : (int)table_row(p.f, to[k], p.status);
       ring[e].state[at] = (uint8_t)state[k];
     }
     __syncwarp();
@@ -429,7 +432,7 @@ __device__ __forceinline__ void exact_run(const RaggedTc& p, int which, const fl
   const int64_t* st = p.stride[which];
   const int n = p.by_h.div(e.i);
   const int64_t base = (int64_t)n * st[1] + (int64_t)(e.i - n * p.H) * st[0];
-  const float* cs = f.cos_sin + (int64_t)(e.row & 0x3FFFFFFFu) * rot;
+  const int64_t at_row = e.row & 0x3FFFFFFFu;
   auto value = [&](int d) {
     const double x = load_elem(p.x[which], p.dtype[which], base + d);
     return norm ? x * ((double)load_elem(f.weight, f.w_dtype, d) + f.w_offset) : x;
@@ -446,6 +449,11 @@ __device__ __forceinline__ void exact_run(const RaggedTc& p, int which, const fl
       const int a = f.interleaved ? d >> 1 : d < half ? d : d - half;    // angle
       const bool second = f.interleaved ? d & 1 : d >= half;
       const int with = f.interleaved ? d ^ 1 : second ? d - half : d + half;
+      const int64_t row =
+          f.axes.n ? table_row(f, load_pos(p.pos, p.pos64, at_row * p.pos_stride +
+                                                               f.axes.axis(a) * f.axes.stride), p.status)
+                   : at_row;
+      const float* cs = f.cos_sin + row * rot;
       x = x * cs[a] + value(with) * (second ? cs[half + a] : -cs[half + a]);
     }
     ss += x * x;
@@ -484,7 +492,8 @@ __device__ __forceinline__ void exact_run(const RaggedTc& p, int which, const fl
   }
 }
 
-template <int D, int BITS>
+// AXES: a rotation by several position axes (keys).
+template <int D, int BITS, bool AXES>
 __global__ void __launch_bounds__(AppendRoles<D>::kThreads, 1)
 append_ragged_tc_kernel(const __grid_constant__ RaggedTc p, int which) {
   using S = Shape<D>;
@@ -604,6 +613,9 @@ append_ragged_tc_kernel(const __grid_constant__ RaggedTc p, int which) {
       }
     };
     auto vec0 = [&](int tile) { return tile * kM + W::kVecs * warp; };
+    auto axis_row = [&](int64_t n, int a) {
+      return table_row(p.f, load_pos(p.pos, p.pos64, n * p.pos_stride + a * p.f.axes.stride), p.status);
+    };
     Raw cur, nxt;
     if (first < p.ntiles) load_raw(cur, vec0(first));
     int it = 0;
@@ -619,9 +631,12 @@ append_ragged_tc_kernel(const __grid_constant__ RaggedTc p, int which) {
         const int e = (it + 1) % kRing;
         ok = wait_for(&pp.loc_full[e], (uint32_t)(((it + 1) / kRing) & 1), pp.abort_flag, p.status);
         constexpr int LINES = 32 / W::kVecs;               // 128-byte lines per lane's vector
-        const float* at = f.cos_sin + (int64_t)ring[e].row[W::kVecs * warp + lane / LINES] * f.rot;
-        for (int c = 32 * (lane % LINES); c < f.rot; c += 32 * LINES)
-          asm volatile("prefetch.global.L1 [%0];" ::"l"(at + c));
+        const int64_t to = ring[e].row[W::kVecs * warp + lane / LINES];
+        for (int a = 0; a < (AXES ? p.f.axes.n : 1); ++a) {
+          const float* at = f.cos_sin + (AXES ? axis_row(to, a) : to) * f.rot;
+          for (int c = 32 * (lane % LINES); c < f.rot; c += 32 * LINES)
+            asm volatile("prefetch.global.L1 [%0];" ::"l"(at + c));
+        }
       }
       ok = ok && (it < 2 || wait_for(&pp.a_empty[st], (uint32_t)(((it / 2) - 1) & 1),
                                      pp.abort_flag, p.status));
@@ -664,13 +679,34 @@ append_ragged_tc_kernel(const __grid_constant__ RaggedTc p, int which) {
           }
         }
         if (f.cos_sin) {
-          const float* cs = f.cos_sin + (int64_t)vec.row[W::kVecs * warp + vi] * f.rot;
+          const int64_t to = vec.row[W::kVecs * warp + vi];
+          const float* cs = f.cos_sin + (AXES ? 0 : to * f.rot);
           auto rotate = [](float& a, float& b, float c, float s) {
             const float t = a * c - b * s;
             b = b * c + a * s;
             a = t;
           };
-          if (pairs) {
+          if constexpr (AXES) {
+            auto row_of = [&](int a) { return axis_row(to, a); };
+            float c[8], s[8];
+            if (pairs) {
+              if (turn_a) {
+                load_axes<8>(c, s, p.f, ga, row_of);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) rotate(v[e], v[8 + e], c[e], s[e]);
+              }
+            } else {
+#pragma unroll
+              for (int g = 0; g < 2; ++g) {
+                if (g ? turn_b : turn_a) {
+                  float c4[4], s4[4];
+                  load_axes<4>(c4, s4, p.f, (g ? gb : ga) / 2, row_of);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) rotate(v[8 * g + 2 * e], v[8 * g + 2 * e + 1], c4[e], s4[e]);
+                }
+              }
+            }
+          } else if (pairs) {
             if (turn_a) {
 #pragma unroll
               for (int e = 0; e < 8; e += 4) {
@@ -1180,17 +1216,17 @@ read_ragged_tc_kernel(RaggedTc p, int which) {
 // ---------------------------------------------------------------------------
 using RaggedFn = void (*)(RaggedTc, int);
 
-template <int D>
+template <int D, bool AXES>
 RaggedFn append_fn(int bits) {
   switch (bits) {
-    case 1: return append_ragged_tc_kernel<D, 1>;
-    case 2: return append_ragged_tc_kernel<D, 2>;
-    case 3: return append_ragged_tc_kernel<D, 3>;
-    case 4: return append_ragged_tc_kernel<D, 4>;
-    case 5: return append_ragged_tc_kernel<D, 5>;
-    case 6: return append_ragged_tc_kernel<D, 6>;
-    case 7: return append_ragged_tc_kernel<D, 7>;
-    default: return append_ragged_tc_kernel<D, 8>;
+    case 1: return append_ragged_tc_kernel<D, 1, AXES>;
+    case 2: return append_ragged_tc_kernel<D, 2, AXES>;
+    case 3: return append_ragged_tc_kernel<D, 3, AXES>;
+    case 4: return append_ragged_tc_kernel<D, 4, AXES>;
+    case 5: return append_ragged_tc_kernel<D, 5, AXES>;
+    case 6: return append_ragged_tc_kernel<D, 6, AXES>;
+    case 7: return append_ragged_tc_kernel<D, 7, AXES>;
+    default: return append_ragged_tc_kernel<D, 8, AXES>;
   }
 }
 
@@ -1248,17 +1284,18 @@ bool rows_aligned(const tq_tensor4* x) {
 // Both return TQ_OK when they ran, 1 when they do not apply, or an error.
 int launch_append_ragged_tc(const tq_geom* G, const tq_tables* t, const tq_cache* c,
                             const tq_tensor4* k, const tq_tensor4* v, const tq_ragged* batch,
-                            const tq_rope* rope, const tq_head_norm* norm, const tq_positions* pos,
-                            uint32_t* status, cudaStream_t st) {
+                            const tq_rope* rope, const tq_rope_axes* axes, const tq_head_norm* norm,
+                            const tq_positions* pos, uint32_t* status, cudaStream_t st) {
   const int D = G->head_dim;
   if (D != 64 && D != 128) return 1;
   if (k->shape[1] * k->shape[2] > INT32_MAX - kM || (rope && (rope->rot_dim % 16 || rope->positions >> 30))) return 1;
+  if (axes && k->shape[2] >> 30) return 1;                 // a noted run holds 30 bits of its row
   if (reinterpret_cast<uintptr_t>(t->rot) % 16) return 1;
   const tq_tensor4* x[2] = {k, v};
   for (int w = 0; w < 2; ++w)
     if (!rows_aligned(x[w])) return 1;
   RaggedTc p = tc_params(G, t, c, x, batch, status);
-  p.f = head_xform(rope, norm);
+  p.f = head_xform(rope, axes, norm);
   p.pos = pos ? pos->data : nullptr;
   p.pos64 = pos && pos->bits == 64;
   p.pos_stride = pos ? pos->stride[1] : 0;
@@ -1267,7 +1304,9 @@ int launch_append_ragged_tc(const tq_geom* G, const tq_tables* t, const tq_cache
   const unsigned grid = (unsigned)tmin(p.ntiles, device_sm_count());
   for (int w = 0; w < 2; ++w) {
     const int bits = w == 0 ? G->key_bits : G->value_bits;
-    RaggedFn fn = D == 128 ? append_fn<128>(bits) : append_fn<64>(bits);
+    const bool many = w == 0 && p.f.axes.n > 0;
+    RaggedFn fn = D == 128 ? (many ? append_fn<128, true>(bits) : append_fn<128, false>(bits))
+                           : (many ? append_fn<64, true>(bits) : append_fn<64, false>(bits));
     if (set_smem_attr((const void*)fn, kSmem) != TQ_OK) return TQ_ERR_CUDA;
     const int threads = D == 128 ? AppendRoles<128>::kThreads : AppendRoles<64>::kThreads;
     if (const int rc = launch_one(fn, grid, threads, kSmem, st, p, w, w == 1, "tq_append_ragged"))

@@ -42,11 +42,6 @@ struct RopeParams {
 
 constexpr int kRopeWarps = 8;
 
-__device__ __forceinline__ int64_t load_pos(const void* pos, int pos64, int64_t i) {
-  return pos64 ? __ldg(reinterpret_cast<const long long*>(pos) + i)
-               : (int64_t)__ldg(reinterpret_cast<const int*>(pos) + i);
-}
-
 // Any type, stride, head size and rotary part: one warp per head vector, the
 // vector staged in shared memory.
 __global__ void __launch_bounds__(32 * kRopeWarps) rope_any_kernel(RopeParams p) {
@@ -64,10 +59,14 @@ __global__ void __launch_bounds__(32 * kRopeWarps) rope_any_kernel(RopeParams p)
     const int64_t xb = b * s.xs[0] + h * s.xs[1] + t * s.xs[2];
     for (int c = lane; c < p.D; c += 32) u[c] = load_elem(s.x, s.dtype, xb + c * s.xs[3]);
     __syncwarp();
-    int64_t row = 0;
-    if (s.f.cos_sin)
-      row = table_row(s.f, load_pos(p.pos, p.pos64, b * p.ps[0] + t * p.ps[1]), p.status);
-    xform_row(u, p.D, s.f, row, lane);
+    const int64_t at = b * p.ps[0] + t * p.ps[1];
+    if (s.f.axes.n) {
+      xform_axes(u, p.D, s.f, p.pos, p.pos64, at, p.status, lane);
+    } else {
+      int64_t row = 0;
+      if (s.f.cos_sin) row = table_row(s.f, load_pos(p.pos, p.pos64, at), p.status);
+      xform_row(u, p.D, s.f, row, lane);
+    }
     const int64_t yb = b * s.ys[0] + h * s.ys[1] + t * s.ys[2];
     for (int c = lane; c < p.D; c += 32) store_elem(s.y, s.dtype, yb + c * s.ys[3], u[c]);
     __syncwarp();
@@ -171,7 +170,8 @@ __device__ __forceinline__ void load_weights(float (&w)[P], const HeadXform& f, 
 
 // D = 2 P LV values per vector.  Groups of LV lanes; a group's unit is (token,
 // run of kHeads heads of q or k).
-template <int DT, int LV, bool PAIRS>
+// AXES: several position axes.
+template <int DT, int LV, bool PAIRS, bool AXES>
 __global__ void __launch_bounds__(kRowThreads, 3) rope_rows_kernel(RopeParams p, int runs_q, int runs) {
   using X = Piece<DT>;
   constexpr int P = X::P, D = 2 * P * LV;
@@ -219,10 +219,16 @@ __global__ void __launch_bounds__(kRowThreads, 3) rope_rows_kernel(RopeParams p,
       load_weights<P>(wb, s.f, gb);
     }
     const float* tab = s.f.cos_sin;
-    if (tab)
-      tab += table_row(s.f, load_pos(p.pos, p.pos64, b * p.ps[0] + t * p.ps[1]), p.status) * s.f.rot;
+    const int64_t at = b * p.ps[0] + t * p.ps[1];
+    if (!AXES && tab) tab += table_row(s.f, load_pos(p.pos, p.pos64, at), p.status) * s.f.rot;
+    auto row_of = [&](int a) {
+      return table_row(s.f, load_pos(p.pos, p.pos64, at + a * s.f.axes.stride), p.status);
+    };
     if (PAIRS) {
-      if (turn_a) { load_f32<P>(cs, tab + ga); load_f32<P>(sn, tab + half + ga); }
+      if (turn_a) {
+        if constexpr (AXES) load_axes<P>(cs, sn, s.f, ga, row_of);
+        else { load_f32<P>(cs, tab + ga); load_f32<P>(sn, tab + half + ga); }
+      }
 #pragma unroll
       for (int e = 0; e < P; e += 2) {
         const float c0 = turn_a ? cs[e] : 1.f, c1 = turn_a ? cs[e + 1] : 1.f;
@@ -233,12 +239,17 @@ __global__ void __launch_bounds__(kRowThreads, 3) rope_rows_kernel(RopeParams p,
         E[e / 2] = tc::f2_make(wa[e] * s0, wa[e + 1] * s1);
       }
     } else {
+      float ac[P / 2], as[P / 2], bc[P / 2], bs[P / 2];
+      if constexpr (AXES) {
+        if (turn_a) load_axes<P / 2>(ac, as, s.f, ga / 2, row_of);
+        if (turn_b) load_axes<P / 2>(bc, bs, s.f, gb / 2, row_of);
+      }
 #pragma unroll
       for (int i = 0; i < P / 2; ++i) {
-        const float ca = turn_a ? __ldg(tab + ga / 2 + i) : 1.f;
-        const float sa = turn_a ? __ldg(tab + half + ga / 2 + i) : 0.f;
-        const float cb = turn_b ? __ldg(tab + gb / 2 + i) : 1.f;
-        const float sb = turn_b ? __ldg(tab + half + gb / 2 + i) : 0.f;
+        const float ca = !turn_a ? 1.f : AXES ? ac[i] : __ldg(tab + ga / 2 + i);
+        const float sa = !turn_a ? 0.f : AXES ? as[i] : __ldg(tab + half + ga / 2 + i);
+        const float cb = !turn_b ? 1.f : AXES ? bc[i] : __ldg(tab + gb / 2 + i);
+        const float sb = !turn_b ? 0.f : AXES ? bs[i] : __ldg(tab + half + gb / 2 + i);
         A[i] = tc::f2_make(wa[2 * i] * ca, wa[2 * i + 1] * ca);
         B[i] = tc::f2_make(-wa[2 * i + 1] * sa, wa[2 * i] * sa);
         C[i] = tc::f2_make(wb[2 * i] * cb, wb[2 * i + 1] * cb);
@@ -306,21 +317,27 @@ bool takes_pieces(const tq_tensor4* x) {
 
 using RopeFn = void (*)(RopeParams, int, int);
 
-template <int DT, bool PAIRS>
+template <int DT, bool PAIRS, bool AXES>
 RopeFn rows_fn(int lanes) {
   switch (lanes) {
-    case 2: return rope_rows_kernel<DT, 2, PAIRS>;
-    case 4: return rope_rows_kernel<DT, 4, PAIRS>;
-    case 8: return rope_rows_kernel<DT, 8, PAIRS>;
-    case 16: return rope_rows_kernel<DT, 16, PAIRS>;
-    case 32: return rope_rows_kernel<DT, 32, PAIRS>;
+    case 2: return rope_rows_kernel<DT, 2, PAIRS, AXES>;
+    case 4: return rope_rows_kernel<DT, 4, PAIRS, AXES>;
+    case 8: return rope_rows_kernel<DT, 8, PAIRS, AXES>;
+    case 16: return rope_rows_kernel<DT, 16, PAIRS, AXES>;
+    case 32: return rope_rows_kernel<DT, 32, PAIRS, AXES>;
     default: return nullptr;
   }
 }
 
+template <int DT>
+RopeFn rows_fn(int lanes, bool halves, bool axes) {
+  return halves ? (axes ? rows_fn<DT, true, true>(lanes) : rows_fn<DT, true, false>(lanes))
+                : (axes ? rows_fn<DT, false, true>(lanes) : rows_fn<DT, false, false>(lanes));
+}
+
 }  // namespace
 
-int launch_qk_rope(const tq_rope* rope, const tq_positions* pos, const tq_tensor4* const x[2],
+int launch_qk_rope(const tq_rope* rope, const tq_rope_axes* axes, const tq_positions* pos, const tq_tensor4* const x[2],
                    const tq_tensor4* const y[2], const tq_head_norm* const norm[2],
                    uint32_t* status, cudaStream_t st) {
   RopeParams p = {};
@@ -331,7 +348,7 @@ int launch_qk_rope(const tq_rope* rope, const tq_positions* pos, const tq_tensor
     s.x = x[w]->data; s.y = y[w]->data; s.dtype = x[w]->dtype;
     for (int i = 0; i < 4; ++i) { s.xs[i] = x[w]->stride[i]; s.ys[i] = y[w]->stride[i]; }
     s.H = x[w]->shape[1];
-    s.f = head_xform(rope, norm[w]);
+    s.f = head_xform(rope, axes, norm[w]);
     p.B = x[w]->shape[0];
     p.T = x[w]->shape[2];
     p.D = (int)x[w]->shape[3];
@@ -351,13 +368,13 @@ int launch_qk_rope(const tq_rope* rope, const tq_positions* pos, const tq_tensor
   for (int w = 0; w < 2; ++w)
     if (x[w])
       rows = rows && x[w]->dtype == one->dtype && takes_pieces(x[w]) && takes_pieces(y[w]);
-  const bool halves = rope && !rope->interleaved;
+  const bool halves = rope && !rope->interleaved, many = rope && axes;
   RopeFn fn = nullptr;
   if (rows) {
     const int lanes = p.D / (2 * P);
-    fn = one->dtype == TQ_F32   ? (halves ? rows_fn<TQ_F32, true>(lanes) : rows_fn<TQ_F32, false>(lanes))
-         : one->dtype == TQ_F16 ? (halves ? rows_fn<TQ_F16, true>(lanes) : rows_fn<TQ_F16, false>(lanes))
-                                : (halves ? rows_fn<TQ_BF16, true>(lanes) : rows_fn<TQ_BF16, false>(lanes));
+    fn = one->dtype == TQ_F32   ? rows_fn<TQ_F32>(lanes, halves, many)
+         : one->dtype == TQ_F16 ? rows_fn<TQ_F16>(lanes, halves, many)
+                                : rows_fn<TQ_BF16>(lanes, halves, many);
   }
   if (fn) {
     const int lanes = p.D / (2 * P), per = kRowThreads / lanes;

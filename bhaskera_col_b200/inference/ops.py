@@ -479,9 +479,14 @@ class RopeTable(_Described):
     """Rotary position embedding: row p of ``cos_sin`` (fp32 (positions,
     rot_dim)) holds the cosines, then the sines, of position p's rot_dim / 2
     angles.  Pair i is dims (i, rot_dim / 2 + i) of a head, or (2i, 2i + 1)
-    when ``interleaved``; dims from rot_dim on are not rotated."""
+    when ``interleaved``; dims from rot_dim on are not rotated.
+
+    ``axes`` (rot_dim / 2 numbers below 4): pair i follows the token's position
+    on axis axes[i] (time, height, width of images and video); positions then
+    come a row per axis (axis_of_pairs makes the usual orders)."""
     cos_sin: torch.Tensor
     interleaved: bool = False
+    axes: Optional[tuple] = None
 
     def _tensors(self):
         return (self.cos_sin,)
@@ -492,12 +497,38 @@ class RopeTable(_Described):
             raise ValueError("cos_sin must be a contiguous fp32 (positions, rot_dim) tensor")
         if c.shape[0] < 1 or c.shape[1] < 2 or c.shape[1] % 2:
             raise ValueError(f"cos_sin must hold a position and an even rot_dim, got {tuple(c.shape)}")
+        packed = None
+        if self.axes is not None:
+            pairs = tuple(int(a) for a in self.axes)
+            if len(pairs) != c.shape[1] // 2 or len(pairs) > 128 or \
+                    not all(0 <= a < 4 for a in pairs):
+                raise ValueError(f"axes must give each of the {c.shape[1] // 2} pairs an axis below "
+                                 f"4, got {self.axes}")
+            packed = (max(pairs) + 1, bytes(pairs))
+        object.__setattr__(self, "_axes", packed)
         return _lib.Rope(c.data_ptr(), c.shape[0], c.shape[1], 1 if self.interleaved else 0)
+
+    @property
+    def num_axes(self) -> int:
+        """Rows of positions that the table's pairs follow (1 without axes)."""
+        return 1 if self.axes is None else max(self.axes) + 1
+
+    @staticmethod
+    def axis_of_pairs(sections, mixed: bool = False) -> tuple:
+        """``axes`` for sections[a] pairs of every axis a: one run of pairs after
+        the other, or (``mixed``) one pair of each axis in turn for as long as
+        it has any left."""
+        left = [int(n) for n in sections]
+        if not 1 <= len(left) <= 4 or any(n < 0 for n in left) or not any(left):
+            raise ValueError(f"sections must be the pairs of 1 to 4 axes, got {sections}")
+        if not mixed:
+            return tuple(a for a, n in enumerate(left) for _ in range(n))
+        return tuple(a for i in range(max(left)) for a, n in enumerate(left) if i < n)
 
     @classmethod
     def build(cls, rot_dim: int, positions: int, base: float = 10000.0, interleaved: bool = False,
               inv_freq: Optional[torch.Tensor] = None, scale: float = 1.0,
-              device: torch.device = torch.device("cuda")) -> "RopeTable":
+              device: torch.device = torch.device("cuda"), axes: Optional[tuple] = None) -> "RopeTable":
         """Angles position * base^(-2i / rot_dim), or position * inv_freq[i],
         formed in 64 bits (an fp32 product is off by 0.03 rad at position
         10^6); ``scale`` multiplies the cosines and sines (YaRN's attention
@@ -509,7 +540,8 @@ class RopeTable(_Described):
         if f.shape != (rot_dim // 2,):
             raise ValueError(f"inv_freq must be ({rot_dim // 2},), got {tuple(f.shape)}")
         a = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * f
-        return cls((torch.cat([a.cos(), a.sin()], -1) * scale).float().contiguous(), interleaved)
+        return cls((torch.cat([a.cos(), a.sin()], -1) * scale).float().contiguous(), interleaved,
+                   axes)
 
 
 @dataclass(frozen=True, eq=False)
@@ -530,6 +562,36 @@ class HeadNorm(_Described):
         if not self.eps >= 0:
             raise ValueError(f"eps must be >= 0, got {self.eps}")
         return _lib.HeadNorm(w.data_ptr(), _DT[w.dtype], float(self.eps), float(self.offset))
+
+
+@dataclass(frozen=True, eq=False)
+class RowNorm(_Described):
+    """Norm of the rows of an activation: (x - mean) / sqrt(mean((x - mean)^2) +
+    eps) * (weight + offset) + bias.  mean is 0 (RMS norm) unless ``centered``
+    (layer norm); without a weight or a bias that part is left out."""
+    weight: Optional[torch.Tensor] = None
+    bias: Optional[torch.Tensor] = None
+    eps: float = 1e-6
+    offset: float = 0.0
+    centered: bool = False
+
+    def _tensors(self):
+        return tuple(x for x in (self.weight, self.bias) if x is not None)
+
+    def _describe(self):
+        for x in self._tensors():
+            if x.dim() != 1 or x.dtype not in _DT or not x.is_contiguous():
+                raise ValueError("weight and bias must be contiguous (C,) floating tensors")
+        w, b = self.weight, self.bias
+        if w is not None and b is not None and (w.shape != b.shape or w.dtype != b.dtype):
+            raise ValueError("weight and bias differ in shape or type")
+        if not self.eps >= 0:
+            raise ValueError(f"eps must be >= 0, got {self.eps}")
+        one = w if w is not None else b
+        return _lib.RowNorm(w.data_ptr() if w is not None else None,
+                            b.data_ptr() if b is not None else None,
+                            _DT[one.dtype] if one is not None else _lib.TQ_F32, float(self.eps),
+                            float(self.offset), 1 if self.centered else 0)
 
 
 @dataclass(frozen=True, eq=False)
@@ -598,18 +660,22 @@ class _Descriptors(threading.local):
     ctypes structure costs 2 us to fill, more than the kernels of a small step."""
 
     def __init__(self):
-        self.buf = ctypes.create_string_buffer(1024)
+        self.buf = ctypes.create_string_buffer(1408)
         self.base = ctypes.addressof(self.buf)
 
 
 _desc = _Descriptors()
 _T4, _POS, _CACHE = (struct.Struct(f) for f in ("@Pi8q", "@Pi2q", "@PqqPqq"))
 _ATTEND = struct.Struct("@PPqPPqfii")
+_AXES = struct.Struct("@iq128s")
+_NORM_ARGS = struct.Struct("@PPPPPPPfi")
 # where each descriptor of a call lies in the buffer
 _AT_Q, _AT_QO, _AT_K, _AT_KO, _AT_POS, _AT_CACHE, _AT_ARGS = 0, 128, 256, 384, 512, 576, 640
+_AT_GATE, _AT_AXES, _AT_DIFF = 896, 1024, 1216
 for _s, _c in ((_T4, _lib.Tensor4), (_POS, _lib.Positions), (_CACHE, _lib.Cache),
-               (_ATTEND, _lib.AttendArgs)):
+               (_ATTEND, _lib.AttendArgs), (_NORM_ARGS, _lib.ResidualNormArgs)):
     assert _s.size <= ctypes.sizeof(_c) <= 128
+assert _AXES.size <= ctypes.sizeof(_lib.RopeAxes) <= 192
 
 
 def _rows(at: int, x: Optional[torch.Tensor], name: str) -> Optional[int]:
@@ -637,21 +703,31 @@ def _heads(at: int, x: Optional[torch.Tensor], name: str) -> Optional[int]:
     return _desc.base + at
 
 
-def _positions(pos: Optional[torch.Tensor], b: int, t: int) -> Optional[int]:
+def _positions(pos: Optional[torch.Tensor], b: int, t: int, rope: Optional[RopeTable] = None,
+               flat: bool = False):
+    """Addresses of the positions' and the axes' descriptors (the latter None
+    where one position of a token serves all pairs)."""
     if pos is None:
-        return None
+        return None, None
     if pos.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"positions must be int32 or int64, got {pos.dtype}")
-    shape = tuple(pos.shape)
+    shape, axes = tuple(pos.shape), None
+    packed = rope._axes if rope is not None else None
     if shape == (t,):
         stride = (0, pos.stride(0))
+    elif packed is not None and shape == ((packed[0], t) if flat else (packed[0], b, t)):
+        stride = (0, pos.stride(1)) if flat else pos.stride()[1:]
+        _AXES.pack_into(_desc.buf, _AT_AXES, packed[0], pos.stride(0), packed[1])
+        axes = _desc.base + _AT_AXES
     elif shape == (b, t):
         stride = pos.stride()
     else:
-        raise ValueError(f"positions must be ({t},) or ({b}, {t}), got {shape}")
+        each = "" if packed is None else f", with an axis a row ({packed[0]}, " + \
+            (f"{t})" if flat else f"{b}, {t})")
+        raise ValueError(f"positions must be ({t},) or ({b}, {t}){each}, got {shape}")
     _POS.pack_into(_desc.buf, _AT_POS, pos.data_ptr(), 64 if pos.dtype == torch.int64 else 32,
                    *stride)
-    return _desc.base + _AT_POS
+    return _desc.base + _AT_POS, axes
 
 
 def _pages(tables: LayerTables, pages, device: torch.device) -> int:
@@ -697,7 +773,9 @@ def qk_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], rope: Optional
     """Norm (optional) and rotation (optional) of query and key heads in one
     pass, in fp32 with one rounding: q (N, Hq, D), k (N, Hkv, D) with
     positions (N,), or q (B, Hq, T, D), k (B, Hkv, T, D) with positions (T,)
-    or (B, T); any strides.  Either of q and k may be None.  ``q_out`` /
+    or (B, T); any strides.  A ``rope`` with axes takes positions (axes, N), or
+    (axes, B, T), a row for each axis; one position of a token then stands for all
+    its axes (text).  Either of q and k may be None.  ``q_out`` /
     ``k_out``: where the results go (may be q / k itself).  A position outside
     the table takes its row 0 and sets _lib.DEV_BAD_POSITION in the device
     status word.  Returns (q_out, k_out)."""
@@ -717,11 +795,17 @@ def qk_rope(q: Optional[torch.Tensor], k: Optional[torch.Tensor], rope: Optional
     if k is not None:
         _check_norm(k_norm, k.shape[-1])
         k_out = torch.empty_like(k) if k_out is None else k_out
+    table = rope and rope.c
+    pos, axes = _positions(positions, b, t, rope, one.dim() != 4)
     with _on(one.device):
-        _lib.check("tq_qk_rope", _lib.load().tq_qk_rope(
-            _ref(rope and rope.c), _positions(positions, b, t), _heads(_AT_Q, q, "q"),
-            _heads(_AT_QO, q_out, "q_out"), _ref(q_norm and q_norm.c), _heads(_AT_K, k, "k"),
-            _heads(_AT_KO, k_out, "k_out"), _ref(k_norm and k_norm.c), _raw_stream(one.device)))
+        rest = (_heads(_AT_Q, q, "q"), _heads(_AT_QO, q_out, "q_out"), _ref(q_norm and q_norm.c),
+                _heads(_AT_K, k, "k"), _heads(_AT_KO, k_out, "k_out"), _ref(k_norm and k_norm.c),
+                _raw_stream(one.device))
+        if axes is None:
+            _lib.check("tq_qk_rope", _lib.load().tq_qk_rope(_ref(table), pos, *rest))
+        else:
+            _lib.check("tq_qk_rope_axes",
+                       _lib.load().tq_qk_rope_axes(_ref(table), axes, pos, *rest))
     return q_out, k_out
 
 
@@ -732,19 +816,25 @@ def append_ragged(tables: LayerTables, pages, k: torch.Tensor, v: torch.Tensor,
     """Quantise and store a flattened batch's tokens, k and v (N, Hkv, D), at
     their requests' positions; ``pages`` holds stream r * Hkv + h of request
     r, head h.  k is normed and rotated on the way (both optional), by its
-    position in its request or by ``positions`` (N,).  A token whose position
+    position in its request or by ``positions`` (N,), or (axes, N) where ``rope``
+    has axes.  A token whose position
     lies outside the pages is dropped and sets _lib.DEV_BAD_POSITION."""
     _inference_only("append_ragged", k.device, k, v, batch.q_start, positions,
                     rope.cos_sin if rope is not None else None,
                     k_norm.weight if k_norm is not None else None)
     _check_norm(k_norm, k.shape[-1])
+    table = rope and rope.c
+    pos, axes = _positions(positions, 1, k.shape[0], rope, True)
     with _on(k.device):
-        _lib.check("tq_append_ragged", _lib.load().tq_append_ragged(
-            ctypes.byref(tables.geom()), ctypes.byref(tables.ctables()),
-            _pages(tables, pages, k.device),
-            _rows(_AT_K, k, "k"), _rows(_AT_KO, v, "v"), ctypes.byref(batch.c),
-            _ref(rope and rope.c), _ref(k_norm and k_norm.c),
-            _positions(positions, 1, k.shape[0]), _raw_stream(k.device)))
+        first = (ctypes.byref(tables.geom()), ctypes.byref(tables.ctables()),
+                 _pages(tables, pages, k.device),
+                 _rows(_AT_K, k, "k"), _rows(_AT_KO, v, "v"), ctypes.byref(batch.c), _ref(table))
+        rest = (_ref(k_norm and k_norm.c), pos, _raw_stream(k.device))
+        if axes is None:
+            _lib.check("tq_append_ragged", _lib.load().tq_append_ragged(*first, *rest))
+        else:
+            _lib.check("tq_append_ragged_axes",
+                       _lib.load().tq_append_ragged_axes(*first, axes, *rest))
 
 
 def dequantize_ragged(tables: LayerTables, pages, batch: RaggedBatch,
@@ -808,3 +898,68 @@ def attend_ragged(tables: LayerTables, pages, q: torch.Tensor, batch: RaggedBatc
             g, ctypes.byref(tables.ctables()), c, args, ws.data_ptr(), ws.numel(),
             _raw_stream(q.device)))
     return out
+
+
+_GATES = {"none": _lib.GATE_NONE, "sigmoid": _lib.GATE_SIGMOID, "tanh": _lib.GATE_TANH}
+
+
+def _row_tensor(at: int, x: torch.Tensor, name: str) -> int:
+    """A (..., C) tensor of up to four dims as the C ABI's (1, .., rows, C) view."""
+    dt = _DT.get(x.dtype)
+    if dt is None:
+        raise ValueError(f"unsupported dtype {x.dtype} of {name}")
+    lead = 4 - x.dim()
+    _T4.pack_into(_desc.buf, at, x.data_ptr(), dt, *(1,) * lead, *x.shape, *(0,) * lead, *x.stride())
+    return _desc.base + at
+
+
+def residual_norm(x: torch.Tensor, residual: torch.Tensor, post_norm: Optional[RowNorm] = None,
+                  gate: Optional[torch.Tensor] = None, gate_act: str = "none", scale: float = 1.0,
+                  pre_norm: Optional[RowNorm] = None, residual_out: Optional[torch.Tensor] = None,
+                  out: Optional[torch.Tensor] = None):
+    """A block's output x (..., C) onto the residual stream, and the next block's
+    norm of the sum, in one pass:
+
+        y = residual + scale * gate_act(gate) * post_norm(x),   h = pre_norm(y)
+
+    in fp32, y rounded to residual's type and h (formed from the unrounded y) to
+    x's.  Norms and gate are optional; ``gate`` broadcasts to x ((C,) a channel's,
+    (N, 1) a token's, (N, C)) and goes through ``gate_act``: "none", "sigmoid" or
+    "tanh".  x has one to four dims and any strides, C at most 32,768.
+    ``residual_out`` / ``out``: where the results go (may be residual / x
+    itself).  Returns (residual_out, out); out is None without ``pre_norm``."""
+    if x.dim() < 1 or x.dim() > 4 or residual.shape != x.shape:
+        raise ValueError(f"x and residual must have one shape of 1 to 4 dims, got "
+                         f"{tuple(x.shape)} and {tuple(residual.shape)}")
+    if gate_act not in _GATES:
+        raise ValueError(f"gate_act must be one of {sorted(_GATES)}, got {gate_act!r}")
+    if gate is None and gate_act != "none":
+        raise ValueError("gate_act comes with a gate")
+    norms = [n for n in (post_norm, pre_norm) if n is not None]
+    params = [p for n in norms for p in n._tensors()]
+    _inference_only("residual_norm", x.device, x, residual, gate, residual_out, out, *params)
+    for p in params:
+        if p.shape[0] != x.shape[-1]:
+            raise ValueError(f"a norm of {p.shape[0]} values for rows of {x.shape[-1]}")
+    if pre_norm is None and out is not None:
+        raise ValueError("out comes with pre_norm")
+    residual_out = torch.empty_like(residual) if residual_out is None else residual_out
+    if pre_norm is not None and out is None:
+        out = torch.empty_like(x)
+    for name, y in (("residual_out", residual_out), ("out", out)):
+        if y is not None and y.shape != x.shape:
+            raise ValueError(f"{name} must be {tuple(x.shape)}, got {tuple(y.shape)}")
+    if gate is not None:
+        gate = torch.broadcast_to(gate, x.shape)
+    at_x, at_r = _row_tensor(_AT_Q, x, "x"), _row_tensor(_AT_K, residual, "residual")
+    at_g = _row_tensor(_AT_GATE, gate, "gate") if gate is not None else 0
+    at_y = _row_tensor(_AT_KO, residual_out, "residual_out")
+    at_h = _row_tensor(_AT_QO, out, "out") if out is not None else 0
+    post, pre = (n.c if n is not None else None for n in (post_norm, pre_norm))
+    _NORM_ARGS.pack_into(_desc.buf, _AT_ARGS, at_x, at_r, at_g, at_y, at_h,
+                         ctypes.addressof(post) if post is not None else 0,
+                         ctypes.addressof(pre) if pre is not None else 0, scale, _GATES[gate_act])
+    with _on(x.device):
+        _lib.check("tq_residual_norm", _lib.load().tq_residual_norm(_desc.base + _AT_ARGS,
+                                                                    _raw_stream(x.device)))
+    return residual_out, out

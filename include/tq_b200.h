@@ -380,6 +380,17 @@ typedef struct tq_positions {
   int64_t stride[2];
 } tq_positions;
 
+/* Several position axes (time, height, width): pair i of the rotation turns by
+ * the angle of the token's position on axis axis[i].  Entry a of a token's
+ * positions lies a * stride elements after entry 0 (tq_positions.data).  Each
+ * axis' position outside the table takes the table's row 0 and sets
+ * TQ_DEV_BAD_POSITION. */
+typedef struct tq_rope_axes {
+  int32_t axes;               /* 1..4                                         */
+  int64_t stride;             /* of positions, from axis to axis, in elements */
+  uint8_t axis[128];          /* [rot_dim / 2], each below axes               */
+} tq_rope_axes;
+
 /* Norm and rotation of query and key heads in one pass: q (B, Hq, T, D) and k
  * (B, Hkv, T, D) to q_out and k_out of the same shapes and types, computed in
  * fp32 and rounded once.  Either pair may be NULL; so may a norm, and rope
@@ -388,6 +399,12 @@ typedef struct tq_positions {
 int32_t tq_qk_rope(const tq_rope* rope, const tq_positions* pos, const tq_tensor4* q,
                    const tq_tensor4* q_out, const tq_head_norm* q_norm, const tq_tensor4* k,
                    const tq_tensor4* k_out, const tq_head_norm* k_norm, void* stream);
+
+/* tq_qk_rope with several position axes (axes NULL: one). */
+int32_t tq_qk_rope_axes(const tq_rope* rope, const tq_rope_axes* axes, const tq_positions* pos,
+                        const tq_tensor4* q, const tq_tensor4* q_out, const tq_head_norm* q_norm,
+                        const tq_tensor4* k, const tq_tensor4* k_out, const tq_head_norm* k_norm,
+                        void* stream);
 
 /* A flattened batch: row q_start[r] + i of a tensor (1, H, N, D) is token i of
  * request r's new tokens, at position seq_lens[r] - (q_start[r+1] -
@@ -424,6 +441,13 @@ int32_t tq_append_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c
                          const tq_tensor4* k, const tq_tensor4* v, const tq_ragged* batch,
                          const tq_rope* rope, const tq_head_norm* k_norm,
                          const tq_positions* pos, void* stream);
+
+/* tq_append_ragged with several position axes (axes NULL: one; pos NULL: every
+ * axis at the token's position in its request). */
+int32_t tq_append_ragged_axes(const tq_geom* g, const tq_tables* t, const tq_cache* c,
+                              const tq_tensor4* k, const tq_tensor4* v, const tq_ragged* batch,
+                              const tq_rope* rope, const tq_rope_axes* axes,
+                              const tq_head_norm* k_norm, const tq_positions* pos, void* stream);
 
 /* tq_dequantize of a ragged batch: the stored keys and values of the batch's
  * tokens to their rows of k_out / v_out (1, Hkv, N, D); either may be NULL.  A
@@ -470,6 +494,42 @@ size_t tq_attend_ragged_workspace_bytes(const tq_geom* g, const tq_cache* c,
 int32_t tq_attend_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                          const tq_attend_args* a, void* workspace, size_t workspace_bytes,
                          void* stream);
+
+/* A norm over the rows of an activation, in fp32:
+ *   (x - mean) / sqrt(mean((x - mean)^2) + eps) * (weight + offset) + bias
+ * with mean = 0 unless centered (RMS norm; with centered, layer norm). */
+typedef struct tq_row_norm {
+  const void* weight;         /* [C] or NULL: ones                            */
+  const void* bias;           /* [C] or NULL: zeros                           */
+  int32_t dtype;              /* of both: TQ_F32 / TQ_F16 / TQ_BF16           */
+  float eps;
+  float offset;               /* 0, or 1 for weights stored as w - 1          */
+  int32_t centered;
+} tq_row_norm;
+
+#define TQ_GATE_NONE 0          /* the gate as it is                          */
+#define TQ_GATE_SIGMOID 1
+#define TQ_GATE_TANH 2
+
+/* A block's output onto the residual stream, and the next block's norm of the sum,
+ * in one pass over rows of C values, (.., .., .., C) each:
+ *   y = residual + scale act(gate) post(x)   (residual_out),   h = pre(y)   (out)
+ * in fp32, y and h each rounded once (h from the unrounded y).  post, gate and pre may
+ * be NULL; out comes with pre.  Strides of 0 broadcast the gate.  residual_out has the
+ * type of residual and may be it (same view), out that of x and may be it; else outputs
+ * overlap nothing.  C: 1..32768, rows below 2^31. */
+typedef struct tq_residual_norm_args {
+  const tq_tensor4* x;
+  const tq_tensor4* residual;
+  const tq_tensor4* gate;
+  const tq_tensor4* residual_out;
+  const tq_tensor4* out;
+  const tq_row_norm* post;
+  const tq_row_norm* pre;
+  float scale;
+  int32_t gate_act;           /* TQ_GATE_*                                    */
+} tq_residual_norm_args;
+int32_t tq_residual_norm(const tq_residual_norm_args* a, void* stream);
 
 /* Device memory shareable with the other processes of one node (CUDA IPC on
  * a plain allocation; no multicast object).  tq_shared_alloc returns a zeroed
