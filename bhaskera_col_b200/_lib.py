@@ -36,6 +36,7 @@ EXPORTED = (
     "tq_qk_rope", "tq_append_ragged", "tq_dequantize_ragged",
     "tq_attend_ragged_workspace_bytes", "tq_attend_ragged",
     "tq_qk_rope_axes", "tq_append_ragged_axes", "tq_residual_norm",
+    "tq_diff_attend_ragged_workspace_bytes", "tq_diff_attend_ragged",
 )
 MAX_PEERS = 8
 SHARED_HANDLE_BYTES = 64
@@ -129,6 +130,15 @@ class AttendArgs(ctypes.Structure):
                 ("engine", ctypes.c_int32)]
 
 
+class DiffArgs(ctypes.Structure):
+    _fields_ = [("q", ctypes.POINTER(Tensor4)), ("out", ctypes.POINTER(Tensor4)),
+                ("batch", Ragged), ("scale", ctypes.c_float), ("causal", ctypes.c_int32),
+                ("engine", ctypes.c_int32), ("shared_keys", ctypes.c_int32),
+                ("halves", ctypes.c_int32), ("lambda_", ctypes.c_void_p),
+                ("lambda_stride", ctypes.c_int64 * 2), ("norm", ctypes.POINTER(HeadNorm)),
+                ("out_scale", ctypes.c_float)]
+
+
 class RowNorm(ctypes.Structure):
     _fields_ = [("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("dtype", ctypes.c_int32),
                 ("eps", ctypes.c_float), ("offset", ctypes.c_float), ("centered", ctypes.c_int32)]
@@ -191,6 +201,8 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
             "tq_append_ragged": (I32, [VP] * 10),
             "tq_append_ragged_axes": (I32, [VP] * 11),
             "tq_residual_norm": (I32, [VP] * 2),
+            "tq_diff_attend_ragged_workspace_bytes": (SZ, [VP] * 3),
+            "tq_diff_attend_ragged": (I32, [VP] * 5 + [SZ, VP]),
             "tq_dequantize_ragged": (I32, [VP] * 7),
             "tq_attend_ragged_workspace_bytes": (SZ, [VP] * 3),
             "tq_attend_ragged": (I32, [VP] * 5 + [SZ, VP]),

@@ -48,6 +48,7 @@ struct PlanParams {
   int32_t* nseg;
   int32_t* next;
   int32_t* arrived;
+  int32_t* rows;                           // [2] first row and end of the batch (0, 0 where it is not run)
   uint32_t* status;
 };
 
@@ -259,7 +260,9 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p0
     *p.next = 0;
   }
   if (tid <= kClasses) place[tid] = 0;
-  if (__syncthreads_or(offsets.fails(p.rv, tid, kPlanThreads, p.status))) {
+  const bool bad = __syncthreads_or(offsets.fails(p.rv, tid, kPlanThreads, p.status));
+  if (tid < 2 && p.rows) p.rows[tid] = bad ? 0 : __ldg(p.rv.q_start + (tid ? p.rv.R : 0));
+  if (bad) {
     if (tid == 0) *p.nseg = 0;
     return;
   }
@@ -342,6 +345,25 @@ struct AttendShape {
   size_t bytes;
 };
 
+// What the kernels are asked for.  `a` gives types and strides; differential attention
+// comes with its own head view, the results' precision and 2 H heads.
+struct AttendCall {
+  const tq_attend_args* a;
+  int64_t Hkv;                             // KV heads as the head groups count them
+  bool precise;
+  HeadView hv;
+};
+
+AttendCall plain_call(const tq_cache* c, const tq_attend_args* a) {
+  AttendCall x = {};
+  x.a = a;
+  x.Hkv = c->streams / a->batch.requests;
+  x.precise = attend_precise(a);
+  x.hv.g = (int)(a->q->shape[1] / x.Hkv);
+  x.hv.streams = (int)x.Hkv;
+  return x;
+}
+
 // Query rows of a request and KV head up to which the few-row kernel is taken
 // where the tcgen05 kernel could be: 16 requests of 3,000-5,000 keys, D128, four
 // heads a group: 64 rows 128 us against 197, 128 rows 199 against 227, 256 rows 375
@@ -359,19 +381,20 @@ struct Kernels {
   bool few, tc;
 };
 
-Kernels attend_kernels(const tq_geom* G, const tq_attend_args* a) {
+Kernels attend_kernels(const tq_geom* G, int engine, bool precise, bool own) {
   Kernels k;
-  k.few = attend_few_applies(G) && (a->engine == 0 || a->engine == 3);
-  k.tc = prefill_tc_applies(G) && (a->engine == 2 || (a->engine == 0 && !attend_precise(a)));
+  k.few = attend_few_applies(G) && (engine == 0 || engine == 3) && !own;
+  k.tc = prefill_tc_applies(G) && (engine == 2 || (engine == 0 && !precise)) && !own;
   return k;
 }
 
-AttendShape attend_shape(const tq_geom* G, const tq_cache* c, const tq_attend_args* a) {
+AttendShape attend_shape(const tq_geom* G, const AttendCall& x) {
+  const tq_attend_args* a = x.a;
   AttendShape s = {};
   const int64_t R = a->batch.requests, N = a->q->shape[2], most = INT64_MAX;
-  s.Hkv = c->streams / R;
-  const int64_t g = a->q->shape[1] / s.Hkv;
-  const Kernels kernels = attend_kernels(G, a);
+  s.Hkv = x.Hkv;
+  const int64_t g = x.hv.g;
+  const Kernels kernels = attend_kernels(G, a->engine, x.precise, x.hv.own);
   s.tc = kernels.tc;
   const bool can = kernels.few;
   const int64_t few_q = s.tc ? tmax<int64_t>(kFewRows / g, 1) : most;
@@ -408,7 +431,7 @@ AttendShape attend_shape(const tq_geom* G, const tq_cache* c, const tq_attend_ar
     // q' rows of its tokens: beside a wide list at most few_q of each request
     s.qp_stride = wide ? few_q : 0;
     l.off_qp = take((size_t)(wide ? R * few_q : N) * a->q->shape[1] * G->head_dim *
-                    (attend_precise(a) ? 4 : 2));
+                    (x.precise ? 4 : 2));
   }
   if (wide) {
     ListShape& l = s.wide;
@@ -428,21 +451,11 @@ AttendShape attend_shape(const tq_geom* G, const tq_cache* c, const tq_attend_ar
   return s;
 }
 
-}  // namespace
-
-bool attend_applies(const tq_geom* G, const tq_attend_args* a) {
-  const Kernels k = attend_kernels(G, a);
-  return k.few || k.tc || (a->engine <= 1 && attend_mma_applies(G));
-}
-
-size_t attend_ragged_workspace(const tq_geom* G, const tq_cache* c, const tq_attend_args* a) {
-  return attend_shape(G, c, a).bytes;
-}
-
-int launch_attend_ragged(const tq_geom* G, const tq_tables* t, const tq_cache* c,
-                         const tq_attend_args* a, void* ws, uint32_t* status, cudaStream_t st) {
-  const AttendShape s = attend_shape(G, c, a);
-  if (a->q->shape[2] == 0) return TQ_OK;
+// `rows`: where the first list leaves the batch's rows, or NULL.
+int launch_attend(const tq_geom* G, const tq_tables* t, const tq_cache* c, const AttendCall& x,
+                  void* ws, int32_t* rows, uint32_t* status, cudaStream_t st) {
+  const tq_attend_args* a = x.a;
+  const AttendShape s = attend_shape(G, x);
   uint8_t* base = static_cast<uint8_t*>(ws);
   RaggedAttend rg[2];
   PlanParams plan[2];
@@ -467,7 +480,9 @@ int launch_attend_ragged(const tq_geom* G, const tq_tables* t, const tq_cache* c
     p.segs = reinterpret_cast<RaggedSeg*>(base + l->off_segs);
     p.arrived = reinterpret_cast<int32_t*>(base + l->off_arrived);
     p.status = status;
+    p.rows = lists == 0 ? rows : nullptr;
     RaggedAttend& r = rg[lists++];
+    r.hv = x.hv;
     r.rv = p.rv;
     r.plan.segs = p.segs;
     r.plan.nseg = p.nseg;
@@ -487,7 +502,7 @@ int launch_attend_ragged(const tq_geom* G, const tq_tables* t, const tq_cache* c
     qp.q_vec = qp.q_dtype != TQ_F32 && qp.qs[2] == 1 && reinterpret_cast<uintptr_t>(qp.q) % 16 == 0 &&
                qp.qs[0] % 8 == 0 && qp.qs[1] % 8 == 0;
     qp.rot_h = reinterpret_cast<const __half*>(t->rot_f16);
-    qp.rot = attend_precise(a) ? t->rot : nullptr;
+    qp.rot = x.precise ? t->rot : nullptr;
     qp.qp = reinterpret_cast<__half*>(base + s.few.off_qp);
     qp.qp_stride = s.qp_stride;
     qp.qscale = a->scale * 1.4426950408889634f;
@@ -500,7 +515,7 @@ int launch_attend_ragged(const tq_geom* G, const tq_tables* t, const tq_cache* c
   ragged_plan_kernel<<<lists + query_ctas, kPlanThreads, 0, st>>>(plan[0], plan[lists - 1], lists, qp);
   if (check_launch("tq_attend_ragged/plan") != TQ_OK) return TQ_ERR_CUDA;
   if (s.few.used) {
-    const int rc = launch_attend_few(G, t, c, a, rg[0], s.Hkv, s.few.hc, s.few.pcta, s.few.rows,
+    const int rc = launch_attend_few(G, t, c, a, x.precise, rg[0], s.Hkv, s.few.hc, s.few.pcta, s.few.rows,
                                      qp.qp, s.qp_stride, s.few.max_seg * s.few.G, status, st);
     if (rc != TQ_OK) return rc;
   }
@@ -508,9 +523,158 @@ int launch_attend_ragged(const tq_geom* G, const tq_tables* t, const tq_cache* c
     return launch_attend_tc(G, t, c, a, rg[lists - 1], s.Hkv, s.wide.max_seg * s.wide.G, status,
                             st);
   if (s.wide.used)
-    return launch_attend_mma(G, t, c, a, rg[lists - 1], s.Hkv, s.wide.hc,
+    return launch_attend_mma(G, t, c, a, x.precise, rg[lists - 1], s.Hkv, s.wide.hc,
                              s.wide.max_seg * s.wide.G, status, st);
   return TQ_OK;
+}
+
+// ---------------------------------------------------------------------------
+// Differential attention: both maps' results in fp32, [row][pair][map][W], and their join
+// ---------------------------------------------------------------------------
+struct DiffJoin {
+  const float* o;
+  const int32_t* rows;                     // [2] the batch's rows
+  int H;
+  int64_t N;
+  const float* lambda; int64_t ls[2];
+  const void* w; int w_dtype;              // norm's weight or NULL: no norm
+  float eps, offset, out_scale;
+  void* out; int o_dtype; int64_t os[3];   // head, row, dim
+};
+
+// A warp per row and pair: out = out_scale norm(o1 - lambda o2), W = 32 E values.
+template <int E>
+__global__ void __launch_bounds__(256) diff_join_kernel(DiffJoin p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t lo = p.rows[0], n = p.rows[1] - lo;
+  const int64_t step = (int64_t)gridDim.x * 8;
+  for (int64_t i = blockIdx.x * 8 + (threadIdx.x >> 5); i < n * p.H; i += step) {
+    const int64_t row = lo + i / p.H;
+    const int h = (int)(i % p.H);
+    const float* o = p.o + (row * p.H + h) * (2 * 32 * E);
+    const float lambda = __ldg(p.lambda + row * p.ls[0] + h * p.ls[1]);
+    float x[E], ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const float a = o[32 * e + lane], b = o[32 * (E + e) + lane];
+      x[e] = b == 0.f ? a : fmaf(-lambda, b, a);           // rows without keys are 0
+      ss = fmaf(x[e], x[e], ss);
+    }
+    if (p.w) {
+      ss = warp_sum(ss);
+      const float r = ss == 0.f ? 0.f : 1.f / sqrtf(ss * (1.f / (32 * E)) + p.eps);
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        x[e] = x[e] * r * (load_elem(p.w, p.w_dtype, 32 * e + lane) + p.offset);
+    }
+    const int64_t at = h * p.os[0] + row * p.os[1];
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      store_elem(p.out, p.o_dtype, at + (32 * e + lane) * p.os[2], x[e] * p.out_scale);
+  }
+}
+
+// The attention of both maps that differential attention is made of.
+struct DiffCall {
+  tq_attend_args a;
+  tq_tensor4 o;                            // fp32 results
+  int H, W;
+  AttendCall x;
+  size_t off_rows, off_o, bytes;           // in the workspace, behind the attention's
+};
+
+void diff_call(const tq_geom* G, const tq_cache* c, const tq_diff_args* d, DiffCall& k) {
+  const int64_t N = d->q->shape[2];
+  const int heads = (int)(c->streams / d->batch.requests);
+  k.H = (int)(d->q->shape[1] / 2);
+  k.W = d->shared_keys ? G->head_dim : 2 * G->head_dim;
+  k.a.q = d->q;
+  k.a.out = &k.o;
+  k.a.batch = d->batch;
+  k.a.scale = d->scale;
+  k.a.causal = d->causal;
+  k.a.engine = d->engine;
+  k.o.data = nullptr;
+  k.o.dtype = TQ_F32;
+  const int64_t shape[4] = {1, 2 * k.H, N, k.W}, stride[4] = {0, k.W, (int64_t)2 * k.H * k.W, 1};
+  for (int i = 0; i < 4; ++i) { k.o.shape[i] = shape[i]; k.o.stride[i] = stride[i]; }
+  AttendCall& x = k.x;
+  x.a = &k.a;
+  x.precise = d->out->dtype != TQ_BF16;
+  x.hv.own = !d->shared_keys;
+  x.hv.halves = d->halves != 0;
+  x.hv.H = k.H;
+  x.hv.P = d->shared_keys ? 0 : heads / 2;
+  x.hv.g = d->shared_keys ? 2 * k.H / heads : k.H / (heads / 2);
+  x.hv.streams = heads;
+  x.Hkv = d->shared_keys ? heads : 2 * heads;
+  const size_t at = attend_shape(G, x).bytes;
+  k.off_rows = at;
+  k.off_o = at + 256;
+  k.bytes = k.off_o + (size_t)N * 2 * k.H * k.W * 4;
+}
+
+}  // namespace
+
+bool attend_applies(const tq_geom* G, const tq_attend_args* a) {
+  const Kernels k = attend_kernels(G, a->engine, attend_precise(a), false);
+  return k.few || k.tc || (a->engine <= 1 && attend_mma_applies(G));
+}
+
+size_t attend_ragged_workspace(const tq_geom* G, const tq_cache* c, const tq_attend_args* a) {
+  return attend_shape(G, plain_call(c, a)).bytes;
+}
+
+int launch_attend_ragged(const tq_geom* G, const tq_tables* t, const tq_cache* c,
+                         const tq_attend_args* a, void* ws, uint32_t* status, cudaStream_t st) {
+  if (a->q->shape[2] == 0) return TQ_OK;
+  return launch_attend(G, t, c, plain_call(c, a), ws, nullptr, status, st);
+}
+
+bool diff_attend_applies(const tq_geom* G, const tq_diff_args* d) {
+  const Kernels k = attend_kernels(G, d->engine, d->out->dtype != TQ_BF16, !d->shared_keys);
+  return k.few || k.tc || (d->engine <= 1 && attend_mma_applies(G));
+}
+
+size_t diff_attend_workspace(const tq_geom* G, const tq_cache* c, const tq_diff_args* d) {
+  DiffCall k = {};
+  diff_call(G, c, d, k);
+  return k.bytes;
+}
+
+int launch_diff_attend(const tq_geom* G, const tq_tables* t, const tq_cache* c, const tq_diff_args* d,
+                       void* ws, uint32_t* status, cudaStream_t st) {
+  if (d->q->shape[2] == 0) return TQ_OK;
+  DiffCall k = {};
+  diff_call(G, c, d, k);
+  uint8_t* base = static_cast<uint8_t*>(ws);
+  k.o.data = base + k.off_o;
+  int32_t* rows = reinterpret_cast<int32_t*>(base + k.off_rows);
+  if (const int rc = launch_attend(G, t, c, k.x, ws, rows, status, st)) return rc;
+  DiffJoin p = {};
+  p.o = reinterpret_cast<const float*>(base + k.off_o);
+  p.rows = rows;
+  p.H = k.H;
+  p.N = d->q->shape[2];
+  p.lambda = d->lambda;
+  for (int i = 0; i < 2; ++i) p.ls[i] = d->lambda_stride[i];
+  if (d->norm) {
+    p.w = d->norm->weight;
+    p.w_dtype = d->norm->dtype;
+    p.eps = d->norm->eps;
+    p.offset = d->norm->offset;
+  }
+  p.out_scale = d->out_scale;
+  p.out = d->out->data;
+  p.o_dtype = d->out->dtype;
+  for (int i = 0; i < 3; ++i) p.os[i] = d->out->stride[i + 1];
+  const unsigned grid = (unsigned)tmin<int64_t>((p.N * p.H + 7) / 8, 8 * device_sm_count());
+  switch (k.W / 32) {
+    case 2: diff_join_kernel<2><<<grid, 256, 0, st>>>(p); break;
+    case 4: diff_join_kernel<4><<<grid, 256, 0, st>>>(p); break;
+    default: diff_join_kernel<8><<<grid, 256, 0, st>>>(p); break;
+  }
+  return check_launch("tq_diff_attend_ragged");
 }
 
 }  // namespace tq

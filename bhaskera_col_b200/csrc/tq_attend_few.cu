@@ -889,8 +889,8 @@ bool attend_few_applies(const tq_geom* G) {
 }
 
 int launch_attend_few(const tq_geom* G, const tq_tables* t, const tq_cache* c,
-                      const tq_attend_args* a, const RaggedAttend& rg, int64_t Hkv, int hc,
-                      int pcta, int rows, const __half* qp, int64_t qp_stride, int64_t grid,
+                      const tq_attend_args* a, bool precise, const RaggedAttend& rg, int64_t Hkv,
+                      int hc, int pcta, int rows, const __half* qp, int64_t qp_stride, int64_t grid,
                       uint32_t* status, cudaStream_t st) {
   FewParams p;
   const PageGeom g = make_geom(G->head_dim, G->key_bits, G->value_bits, G->qjl);
@@ -924,7 +924,7 @@ int launch_attend_few(const tq_geom* G, const tq_tables* t, const tq_cache* c,
   int bytes = 0;
   auto pick = [&](auto d, auto nt) {
     constexpr int D = decltype(d)::value, NT = decltype(nt)::value;
-    fn = attend_precise(a) ? few_fn<D, NT, true>(G->key_bits, G->value_bits, bytes)
+    fn = precise ? few_fn<D, NT, true>(G->key_bits, G->value_bits, bytes)
                            : few_fn<D, NT, false>(G->key_bits, G->value_bits, bytes);
   };
   using I1 = std::integral_constant<int, 1>;

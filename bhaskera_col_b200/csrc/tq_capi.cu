@@ -927,6 +927,94 @@ int32_t tq_attend_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c
   return launch_attend_ragged(g, t, c, a, workspace, status, (cudaStream_t)stream);
 }
 
+static int check_diff(const tq_geom* g, const tq_cache* c, const tq_diff_args* a, const char* fn) {
+  int rc;
+  if ((rc = check_geom(g, fn)) || (rc = check_cache(c, fn))) return rc;
+  if (!a) { set_error("%s: args are NULL", fn); return TQ_ERR_INVALID; }
+  if ((rc = check_ragged(&a->batch, c, fn)) || (rc = check_maybe_empty(a->q, "q", fn))) return rc;
+  const int64_t Hkv = c->streams / a->batch.requests, Hq = a->q->shape[1], H = Hq / 2;
+  if (a->shared_keys && a->halves) {
+    set_error("%s: pairs that share their keys lie next to each other", fn);
+    return TQ_ERR_INVALID;
+  }
+  if (Hq < 2 || Hq % 2) {
+    set_error("%s: query heads come in pairs, got %lld", fn, (long long)Hq);
+    return TQ_ERR_INVALID;
+  }
+  if (a->shared_keys ? H % Hkv != 0 : (Hkv % 2 != 0 || H % (Hkv / 2) != 0)) {
+    set_error(a->shared_keys ? "%s: %lld pairs of query heads are no multiple of %lld KV heads"
+                             : "%s: %lld pairs of query heads are no multiple of the pairs of %lld KV heads",
+              fn, (long long)H, (long long)Hkv);
+    return TQ_ERR_INVALID;
+  }
+  const tq_geom wide = {a->shared_keys ? g->head_dim : 2 * g->head_dim, 0, 0, 0};
+  if ((rc = check_flat(a->q, "q", Hq, g, fn)) || (rc = check_flat(a->out, "out", H, &wide, fn)))
+    return rc;
+  if (a->out->shape[2] != a->q->shape[2]) {
+    set_error("%s: q and out differ in rows", fn);
+    return TQ_ERR_INVALID;
+  }
+  if (a->engine < 0 || a->engine > 3) {
+    set_error("%s: engine must be 0 (fastest), 1 (mma.sync), 2 (tcgen05) or 3 (few rows), got %d",
+              fn, a->engine);
+    return TQ_ERR_INVALID;
+  }
+  if (!diff_attend_applies(g, a)) {
+    set_error("%s: no kernel for head_dim %d, key_bits %d, value_bits %d (engine %d)", fn,
+              g->head_dim, g->key_bits, g->value_bits, a->engine);
+    return TQ_ERR_INVALID;
+  }
+  if (a->q->shape[2] > (int64_t)1 << 30 || a->batch.requests > (int64_t)1 << 24 || Hq > 1024) {
+    set_error("%s: at most 2^30 rows, 2^24 requests and 1024 query heads", fn);
+    return TQ_ERR_INVALID;
+  }
+  if ((c->block_table ? c->num_blocks : c->streams * c->pages_per_stream) > INT32_MAX ||
+      c->pages_per_stream > INT32_MAX / TQ_PAGE_TOKENS / 2) {
+    set_error("%s: more pages than 32 bits count", fn);
+    return TQ_ERR_INVALID;
+  }
+  return TQ_OK;
+}
+
+size_t tq_diff_attend_ragged_workspace_bytes(const tq_geom* g, const tq_cache* c,
+                                             const tq_diff_args* a) {
+  if (check_diff(g, c, a, "tq_diff_attend_ragged_workspace_bytes")) return 0;
+  return diff_attend_workspace(g, c, a);
+}
+
+int32_t tq_diff_attend_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
+                              const tq_diff_args* a, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+  NvtxRange range("tq_diff_attend_ragged");
+  const char* fn = "tq_diff_attend_ragged";
+  int rc;
+  if ((rc = check_diff(g, c, a, fn)) || (rc = check_tables(g, t, fn))) return rc;
+  if ((rc = check_written(a->out, "out", fn)) || (rc = check_apart(a->q, a->out, false, "out", "q", fn)) ||
+      (rc = check_norm(a->norm, fn)))
+    return rc;
+  if (!t->rot_f16 ||
+      (reinterpret_cast<uintptr_t>(t->rot_f16) | reinterpret_cast<uintptr_t>(t->rot)) % 16) {
+    set_error("%s: tables.rot_f16 (R as fp16) is required, and it and tables.rot 16-byte aligned", fn);
+    return TQ_ERR_INVALID;
+  }
+  if (!(a->scale > 0.f)) { set_error("%s: scale must be positive", fn); return TQ_ERR_INVALID; }
+  const int64_t H = a->q->shape[1] / 2, N = a->q->shape[2];
+  tq_tensor4 lambda = {const_cast<float*>(a->lambda), TQ_F32, {1, H, N, 1},
+                       {0, a->lambda_stride[1], a->lambda_stride[0], 1}};
+  if ((rc = check_maybe_empty(&lambda, "lambda", fn)) ||
+      (rc = check_apart(&lambda, a->out, false, "out", "lambda", fn)))
+    return rc;
+  const size_t need = diff_attend_workspace(g, c, a);
+  if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256) {
+    set_error("%s: a 256-byte aligned workspace of %zu bytes is needed, %zu given", fn, need,
+              workspace_bytes);
+    return TQ_ERR_WORKSPACE;
+  }
+  uint32_t* status = device_status_word();
+  if (!status) { set_error("%s: device status word unavailable", fn); return TQ_ERR_CUDA; }
+  return launch_diff_attend(g, t, c, a, workspace, status, (cudaStream_t)stream);
+}
+
 int32_t tq_workspace_status(void* workspace, uint32_t* status, void* stream) {
   if (!workspace || !status) { set_error("tq_workspace_status: NULL argument"); return TQ_ERR_INVALID; }
   cudaStream_t st = (cudaStream_t)stream;

@@ -87,13 +87,18 @@ int launch_dequant_ragged_tc(const tq_geom* g, const tq_tables* t, const tq_cach
 size_t attend_ragged_workspace(const tq_geom* g, const tq_cache* c, const tq_attend_args* a);
 int launch_attend_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                          const tq_attend_args* a, void* ws, uint32_t* status, cudaStream_t st);
+// Differential attention: a workspace of 0 bytes where no kernel applies.
+bool diff_attend_applies(const tq_geom* g, const tq_diff_args* a);
+size_t diff_attend_workspace(const tq_geom* g, const tq_cache* c, const tq_diff_args* a);
+int launch_diff_attend(const tq_geom* g, const tq_tables* t, const tq_cache* c, const tq_diff_args* a,
+                       void* ws, uint32_t* status, cudaStream_t st);
 // Whether some kernel attends a batch of this geometry, result type and engine.
 bool attend_applies(const tq_geom* g, const tq_attend_args* a);
 bool attend_few_applies(const tq_geom* g);
 bool attend_mma_applies(const tq_geom* g);
 int launch_attend_few(const tq_geom* g, const tq_tables* t, const tq_cache* c,
-                      const tq_attend_args* a, const RaggedAttend& rg, int64_t Hkv, int hc,
-                      int pcta, int rows, const __half* qp, int64_t qp_stride, int64_t grid,
+                      const tq_attend_args* a, bool precise, const RaggedAttend& rg, int64_t Hkv,
+                      int hc, int pcta, int rows, const __half* qp, int64_t qp_stride, int64_t grid,
                       uint32_t* status, cudaStream_t st);
 int launch_attend_tc(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                      const tq_attend_args* a, const RaggedAttend& rg, int64_t Hkv, int64_t grid,
@@ -101,8 +106,8 @@ int launch_attend_tc(const tq_geom* g, const tq_tables* t, const tq_cache* c,
 // fp16 and fp32 results ask for more than the fp16 operands that a bf16 one hides.
 inline bool attend_precise(const tq_attend_args* a) { return a->out->dtype != TQ_BF16; }
 int launch_attend_mma(const tq_geom* g, const tq_tables* t, const tq_cache* c,
-                      const tq_attend_args* a, const RaggedAttend& rg, int64_t Hkv, int hc,
-                      int64_t grid, uint32_t* status, cudaStream_t st);
+                      const tq_attend_args* a, bool precise, const RaggedAttend& rg, int64_t Hkv,
+                      int hc, int64_t grid, uint32_t* status, cudaStream_t st);
 
 // cudaLaunchKernelEx with programmatic stream serialisation (see pdl_wait).
 template <typename... KArgs, typename... Args>

@@ -158,13 +158,20 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
   }
   // rows and keys of the request: 32 bits hold a ragged batch's
   using Pos = typename std::conditional<RG, int, int64_t>::type;
-  const int64_t stream = group / nchunk;               // b * Hkv + kv head
   const int chunk = (int)(group % nchunk);
-  const int64_t b = stream / p.Hkv, kvh = stream % p.Hkv;
+  const int64_t b = group / nchunk / p.Hkv, kvh = group / nchunk % p.Hkv;
+  // streams of the keys and of the values (RG: they may differ)
+  const int64_t stream = RG ? b * p.rg.hv.streams + p.rg.hv.key_head((int)kvh) : group / nchunk;
+  const int64_t vstream = RG ? b * p.rg.hv.streams + p.rg.hv.value_head((int)kvh) : stream;
   // the batch row's first query row: batch stride, or the request's first row
   const int64_t qrow = RG ? sw.rq.q0 * p.qs[2] : b * p.qs[0];
   const int64_t orow = RG ? sw.rq.q0 * p.os[2] : b * p.os[0];
-  const int64_t h = kvh * p.g + (int64_t)chunk * p.hc + warp / wph;   // this warp's head
+  const int64_t ocol = RG ? p.rg.hv.column((int)kvh, D) * p.os[3] : 0;
+  // head i of the CTA's, counted over all
+  auto head = [&](int i) -> int64_t {
+    return RG ? p.rg.hv.head((int)kvh, chunk * p.hc + i) : kvh * p.g + (int64_t)chunk * p.hc + i;
+  };
+  const int64_t h = head(warp / wph);                  // this warp's head
   const Pos t_base = RG ? (Pos)sw.rq.base : p.n_tokens - p.Tq;     // position of query 0
   const int t0 = qb * P + (warp % wph) * 16;           // this warp's first query
   const Pos qpos_max = t_base + tmin<Pos>((Pos)(qb + 1) * P, p.Tq) - 1;
@@ -209,19 +216,32 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
     }
   }
   __syncthreads();
-  // pool address of this stream's page pg (block table or contiguous)
-  auto page_src = [&](int64_t pg) -> const uint8_t* {
+  // pool address of a stream's page pg (block table or contiguous)
+  auto page_src = [&](int64_t of, int64_t pg) -> const uint8_t* {
     bool ok;
-    const int64_t ps = page_slot(p.pm, stream, pg + tile0, ok);
+    const int64_t ps = page_slot(p.pm, of, pg + tile0, ok);
     if (!ok) atomicOr(p.status, TQ_DEV_BAD_BLOCK);
     return p.pages + ps * (int64_t)PAGE;
   };
-  if (tid == 0) {
-    for (int i = 0; i < 2 && i < ntiles; ++i) {
+  // page pg into stage i: whole, or its key and value parts from the two streams' pages
+  auto fetch = [&](int i, int64_t pg) {
+    unsigned char* dst = smem + G::OFF_STG + i * p.page_pitch;
+    const uint8_t* src = page_src(stream, pg);
+    if (!RG || vstream == stream) {
       mbar_expect_tx(&full[i], PAGE);
-      bulk_g2s(smem + G::OFF_STG + i * p.page_pitch, page_src(i), PAGE, &full[i]);
+      bulk_g2s(dst, src, PAGE, &full[i]);
+      return;
     }
-  }
+    const uint8_t* vsrc = page_src(vstream, pg);
+    constexpr uint32_t KS = 64 * G::KROW, VS = 64 * G::VROW, NS = 128;
+    mbar_expect_tx(&full[i], KS + VS + 2 * NS);
+    bulk_g2s(dst, src, KS, &full[i]);
+    bulk_g2s(dst + p.off_kn, src + p.off_kn, NS, &full[i]);
+    bulk_g2s(dst + p.off_v, vsrc + p.off_v, VS, &full[i]);
+    bulk_g2s(dst + p.off_vn, vsrc + p.off_vn, NS, &full[i]);
+  };
+  if (tid == 0)
+    for (int i = 0; i < 2 && i < ntiles; ++i) fetch(i, i);
 
   // ---- queries: q' = (scale q) R^T as fp16 A fragments (log2e folded in) ----
   const bool active = t0 < p.Tq;
@@ -231,7 +251,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
     float acc[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-    const int64_t qbase = qrow + h * p.qs[1];
+    const int64_t qbase = qrow + (RG ? p.rg.hv.in_q((int)h) : h) * p.qs[1];
     const int r0 = t0 + gq, r1 = r0 + 8;
     auto ld2 = [&](int r, int c, uint32_t& lo) -> uint32_t {
       lo = 0u;
@@ -382,11 +402,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
     }
     __syncthreads();
     // the stage is decoded: refill it with page kt + 2
-    if (tid == 0 && kt + 2 < ntiles) {
-      mbar_expect_tx(&full[st], PAGE);
-      bulk_g2s(smem + G::OFF_STG + st * p.page_pitch, page_src(kt + 2), PAGE,
-               &full[st]);
-    }
+    if (tid == 0 && kt + 2 < ntiles) fetch(st, kt + 2);
 
     const Pos k0 = (Pos)(kt + tile0) * 64;
     if constexpr (RG) {
@@ -550,7 +566,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
       for (int n = 0; n < NT; ++n) { acc[n][0] *= down; acc[n][1] *= down; acc[n][2] *= down; acc[n][3] *= down; }
     }
     const int r0 = t0 + gq, r1 = r0 + 8;
-    const int64_t obase = orow + h * p.os[1];
+    const int64_t obase = orow + h * p.os[1] + ocol;
     const bool split = RG && sw.seg.slot >= 0;
     if (split) {
       const int64_t pr = part_row(p.rg.plan, sw.seg.slot, sw.group, 16 * warp + gq);
@@ -588,8 +604,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
                        [&](int row) -> int64_t {
                          const int wr = row >> 4, t = qb * P + (wr % wph) * 16 + (row & 15);
                          if (t >= p.Tq) return -1;
-                         const int64_t hh = kvh * p.g + (int64_t)chunk * p.hc + wr / wph;
-                         return orow + hh * p.os[1] + t * p.os[2];
+                         return orow + head(wr / wph) * p.os[1] + ocol + t * p.os[2];
                        });
   }
 }
@@ -625,8 +640,8 @@ bool attend_mma_applies(const tq_geom* G) {
 // take single fp16 operands (their rounding, 2^-12 of each, is a sixteenth of the
 // result's own); fp16 and fp32 ones hi + lo.
 int launch_attend_mma(const tq_geom* G, const tq_tables* t, const tq_cache* c,
-                      const tq_attend_args* a, const RaggedAttend& rg, int64_t Hkv, int hc,
-                      int64_t grid, uint32_t* status, cudaStream_t st) {
+                      const tq_attend_args* a, bool precise, const RaggedAttend& rg, int64_t Hkv,
+                      int hc, int64_t grid, uint32_t* status, cudaStream_t st) {
   PrefillParams p = {};
   const PageGeom g = make_geom(G->head_dim, G->key_bits, G->value_bits, G->qjl);
   p.pages = c->pages;
@@ -644,7 +659,7 @@ int launch_attend_mma(const tq_geom* G, const tq_tables* t, const tq_cache* c,
   for (int i = 0; i < 4; ++i) { p.qs[i] = a->q->stride[i]; p.os[i] = a->out->stride[i]; }
   p.Hq = a->q->shape[1];
   p.Hkv = Hkv;
-  p.g = p.Hq / Hkv;
+  p.g = rg.hv.g;
   p.hc = hc;
   p.scale = a->scale;
   p.causal = a->causal;
@@ -655,7 +670,7 @@ int launch_attend_mma(const tq_geom* G, const tq_tables* t, const tq_cache* c,
   const bool wide = G->head_dim == 128;
   PfFn fn;
   int smem;
-  if (attend_precise(a)) {
+  if (precise) {
     fn = wide ? pf_fn<128, true, true>(kb, vb) : pf_fn<64, true, true>(kb, vb);
     smem = wide ? Pf<128, 4, 4, true>::smem(p.page_pitch) : Pf<64, 4, 4, true>::smem(p.page_pitch);
   } else {

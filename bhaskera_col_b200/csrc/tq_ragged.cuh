@@ -219,9 +219,33 @@ struct RaggedPlan {
   int rows;                   // query rows of a CTA
 };
 
+// Which query heads, streams and columns a head group stands for.  Plain attention: KV
+// head kvh, its g query heads, columns of the head.  Differential attention works on
+// 2 H heads in pairs, head v = 2 h + m (map m of pair h), which lie in q as they are or
+// (halves) the first maps before the second ones.  own: maps with keys of their own,
+// kvh = (p, m, j): the heads of map m of KV pair p over the keys of its head m and the
+// values of its head j, columns D j of the result.
+struct HeadView {
+  int own, halves;
+  int H, P;                   // pairs of query heads; pairs of KV heads (own)
+  int g;                      // heads of a group's KV head, all chunks
+  int streams;                // KV heads of a request in the cache
+  __device__ __forceinline__ int kv_pair(int p, int m) const { return halves ? m * P + p : 2 * p + m; }
+  __device__ __forceinline__ int key_head(int kvh) const { return own ? kv_pair(kvh >> 2, (kvh >> 1) & 1) : kvh; }
+  __device__ __forceinline__ int value_head(int kvh) const { return own ? kv_pair(kvh >> 2, kvh & 1) : kvh; }
+  // head i of the group, and its place in q
+  __device__ __forceinline__ int head(int kvh, int i) const {
+    return own ? 2 * ((kvh >> 2) * g + i) + ((kvh >> 1) & 1) : kvh * g + i;
+  }
+  __device__ __forceinline__ int in_q(int v) const { return halves ? (v >> 1) + (v & 1) * H : v; }
+  // first column of the head's result
+  __device__ __forceinline__ int column(int kvh, int D) const { return own ? (kvh & 1) * D : 0; }
+};
+
 struct RaggedAttend {
   RaggedView rv;
   RaggedPlan plan;
+  HeadView hv;
 };
 
 // One CTA's share of the work list.

@@ -565,6 +565,51 @@ class HeadNorm(_Described):
 
 
 @dataclass(frozen=True, eq=False)
+class DiffHeads(_Described):
+    """The learned part of differential attention: a pair's result is
+    out_scale * norm(A1 V - lam A2 V), A1 and A2 the softmax maps of its two
+    query heads.
+
+    ``lam``: fp32 (H,), a pair's own; (N, H), of every row too; or (1,) for all.
+    ``keys``: "own", each map has a KV head of its own and V is the values of both
+    side by side (2D wide), or "shared", both query heads attend the same KV head.
+    ``pairs``: heads of a pair lie next to each other ("adjacent": 2h, 2h + 1) or,
+    with own keys, the first ones before the second ones ("halves": h, h + H),
+    query heads and KV heads alike.  ``norm``: RMS norm over a pair's result (as
+    many weights as it is wide), or None; ``out_scale`` multiplies what is left."""
+    lam: torch.Tensor
+    keys: str = "own"
+    pairs: str = "adjacent"
+    norm: Optional[HeadNorm] = None
+    out_scale: float = 1.0
+
+    def _tensors(self):
+        return (self.lam,)
+
+    def _describe(self):
+        x = self.lam
+        if x.dtype != torch.float32 or x.dim() not in (1, 2):
+            raise ValueError("lam must be an fp32 (H,), (N, H) or (1,) tensor")
+        if self.keys not in ("own", "shared"):
+            raise ValueError(f"keys must be 'own' or 'shared', got {self.keys!r}")
+        if self.pairs not in ("adjacent", "halves"):
+            raise ValueError(f"pairs must be 'adjacent' or 'halves', got {self.pairs!r}")
+        if self.keys == "shared" and self.pairs != "adjacent":
+            raise ValueError("pairs that share their keys lie next to each other ('adjacent')")
+        return (x.data_ptr(), 0 if x.dim() == 1 else x.stride(0),
+                0 if x.shape[-1] == 1 else x.stride(-1))
+
+    @staticmethod
+    def lam_of(q1: torch.Tensor, k1: torch.Tensor, q2: torch.Tensor, k2: torch.Tensor,
+               init: float) -> torch.Tensor:
+        """lam = exp(q1 . k1) - exp(q2 . k2) + init over the last dim of the learned
+        vectors, in 64 bits: (1,) for vectors, (H,) for (H, D).  Computed once, as
+        the vectors are fixed in serving."""
+        a, b = ((q.double() * k.double()).sum(-1).exp() for q, k in ((q1, k1), (q2, k2)))
+        return (a - b + init).float().reshape(-1).detach()
+
+
+@dataclass(frozen=True, eq=False)
 class RowNorm(_Described):
     """Norm of the rows of an activation: (x - mean) / sqrt(mean((x - mean)^2) +
     eps) * (weight + offset) + bias.  mean is 0 (RMS norm) unless ``centered``
@@ -669,12 +714,14 @@ _T4, _POS, _CACHE = (struct.Struct(f) for f in ("@Pi8q", "@Pi2q", "@PqqPqq"))
 _ATTEND = struct.Struct("@PPqPPqfii")
 _AXES = struct.Struct("@iq128s")
 _NORM_ARGS = struct.Struct("@PPPPPPPfi")
+_DIFF = struct.Struct("@PPqPPqfiiiiP2qPf")
 # where each descriptor of a call lies in the buffer
 _AT_Q, _AT_QO, _AT_K, _AT_KO, _AT_POS, _AT_CACHE, _AT_ARGS = 0, 128, 256, 384, 512, 576, 640
 _AT_GATE, _AT_AXES, _AT_DIFF = 896, 1024, 1216
 for _s, _c in ((_T4, _lib.Tensor4), (_POS, _lib.Positions), (_CACHE, _lib.Cache),
                (_ATTEND, _lib.AttendArgs), (_NORM_ARGS, _lib.ResidualNormArgs)):
     assert _s.size <= ctypes.sizeof(_c) <= 128
+assert _DIFF.size <= ctypes.sizeof(_lib.DiffArgs) <= 192
 assert _AXES.size <= ctypes.sizeof(_lib.RopeAxes) <= 192
 
 
@@ -895,6 +942,56 @@ def attend_ragged(tables: LayerTables, pages, q: torch.Tensor, batch: RaggedBatc
                                _lib.last_error())
         ws = (workspace or DecodeWorkspace()).get(nbytes, q.device)
         _lib.check("tq_attend_ragged", lib.tq_attend_ragged(
+            g, ctypes.byref(tables.ctables()), c, args, ws.data_ptr(), ws.numel(),
+            _raw_stream(q.device)))
+    return out
+
+
+def diff_attend_ragged(tables: LayerTables, pages, q: torch.Tensor, batch: RaggedBatch,
+                       pair: DiffHeads, scale: Optional[float] = None, causal: bool = True,
+                       out: Optional[torch.Tensor] = None,
+                       workspace: Optional[DecodeWorkspace] = None, engine: int = 0) -> torch.Tensor:
+    """Differential attention of a flattened batch straight off the packed pages:
+    the query heads q (N, 2H, D) come in pairs (``pair``), each the difference of
+    two softmax maps over the request's tokens.  Returns (N, H, 2D) with keys of
+    each map's own (the pages hold the KV heads of both maps, values in halves: a
+    layer's v of (N, Hkv / 2, 2D) is appended as (N, Hkv, D)), (N, H, D) with
+    shared ones.
+
+    Rows, masks, lengths, empty rows, ``scale``, ``causal``, ``engine`` and
+    ``workspace`` are those of attend_ragged; so are the errors of both maps'
+    results, of which the difference is taken in fp32: where the maps nearly
+    cancel, an fp32 ``out`` (operands of 22 bits) keeps what is left."""
+    norm = pair.norm
+    _inference_only("diff_attend_ragged", q.device, q, out, batch.q_start, pair.lam,
+                    norm.weight if norm is not None else None)
+    if q.dim() != 3:
+        raise ValueError(f"q must be (rows, heads, head_dim), got shape {tuple(q.shape)}")
+    own = pair.keys == "own"
+    n, h, d = q.shape[0], q.shape[1] // 2, q.shape[2]
+    width = 2 * d if own else d
+    lam = pair.lam
+    if lam.shape[-1] not in (1, h) or (lam.dim() == 2 and lam.shape[0] != n):
+        raise ValueError(f"lam must be ({h},), ({n}, {h}) or (1,), got {tuple(lam.shape)}")
+    _check_norm(norm, width)
+    if out is None:
+        out = torch.empty((n, h, width), dtype=q.dtype, device=q.device)
+    lib = _lib.load()
+    g, c, bc = ctypes.byref(tables.geom()), _pages(tables, pages, q.device), batch.c
+    weight = norm.c if norm is not None else None
+    _DIFF.pack_into(_desc.buf, _AT_DIFF, _rows(_AT_Q, q, "q"), _rows(_AT_QO, out, "out"),
+                    bc.requests, bc.q_start, bc.seq_lens, bc.max_q_len,
+                    scale if scale is not None else 1.0 / math.sqrt(d), 1 if causal else 0,
+                    int(engine), 0 if own else 1, 1 if pair.pairs == "halves" else 0, *pair.c,
+                    ctypes.addressof(weight) if weight is not None else 0, pair.out_scale)
+    args = _desc.base + _AT_DIFF
+    with _on(q.device):
+        nbytes = lib.tq_diff_attend_ragged_workspace_bytes(g, c, args)
+        if nbytes == 0:
+            raise _lib.TqError("tq_diff_attend_ragged_workspace_bytes", _lib.TQ_ERR_INVALID,
+                               _lib.last_error())
+        ws = (workspace or DecodeWorkspace()).get(nbytes, q.device)
+        _lib.check("tq_diff_attend_ragged", lib.tq_diff_attend_ragged(
             g, ctypes.byref(tables.ctables()), c, args, ws.data_ptr(), ws.numel(),
             _raw_stream(q.device)))
     return out

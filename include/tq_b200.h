@@ -495,6 +495,43 @@ int32_t tq_attend_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c
                          const tq_attend_args* a, void* workspace, size_t workspace_bytes,
                          void* stream);
 
+/* Differential attention of a ragged batch straight off the packed pages: head h of
+ * the result is
+ *   out_h = out_scale norm(A1 V - lambda_h A2 V),  Am = softmax(scale q_m K_m^T)
+ * with the masks, lengths, empty rows and errors of tq_attend_ragged; a row that sees
+ * no key is zero.  The query heads come in pairs, heads 2h and 2h + 1 of q, or (with
+ * own keys) h and h + H where `halves`.
+ *   shared_keys: both heads of a pair attend the same KV head, Hkv dividing H; out is
+ *     (1, H, N, D).
+ *   else each map has keys of its own: KV heads come in pairs like the query heads',
+ *     map m of the pair attends the keys of head m, V is the values of both side by
+ *     side; H is a multiple of Hkv / 2 and out is (1, H, N, 2D).
+ * The norm is an RMS norm of the head's vector (its weight as wide as out), NULL for
+ * none.  out must not overlap q or lambda. */
+typedef struct tq_diff_args {
+  const tq_tensor4* q;        /* (1, 2H, N, D)                                */
+  const tq_tensor4* out;      /* (1, H, N, D or 2D); type may differ from q's */
+  tq_ragged batch;
+  float scale;                /* softmax scale                                */
+  int32_t causal;
+  int32_t engine;             /* as in tq_attend_args                         */
+  int32_t shared_keys;
+  int32_t halves;
+  const float* lambda;        /* device; fp32, lambda of row n, head h at
+                                 n * lambda_stride[0] + h * lambda_stride[1]
+                                 (0: the same for all)                        */
+  int64_t lambda_stride[2];
+  const tq_head_norm* norm;
+  float out_scale;
+} tq_diff_args;
+
+/* As tq_attend_ragged_workspace_bytes and its workspace. */
+size_t tq_diff_attend_ragged_workspace_bytes(const tq_geom* g, const tq_cache* c,
+                                             const tq_diff_args* a);
+int32_t tq_diff_attend_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
+                              const tq_diff_args* a, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
 /* A norm over the rows of an activation, in fp32:
  *   (x - mean) / sqrt(mean((x - mean)^2) + eps) * (weight + offset) + bias
  * with mean = 0 unless centered (RMS norm; with centered, layer norm). */

@@ -75,23 +75,27 @@ def residual_norm(x, residual, post=None, gate=None, act="none", scale=1.0, pre=
 
 def diff_attend(q, k, v, lam, q_start, seq_lens, scale, causal, shared, halves, norm=None, eps=0.0,
                 offset=0.0, out_scale=1.0):
-    """q (N, 2H, D), k / v (R, Hkv, T, D): (out, o1, o2) of (N, H, W); rows outside the batch NaN, rows
-    without keys 0.  lam: (H,) or (N, H)."""
+    """q (N, 2H, D), k / v (R, Hkv, T, D) in 64 bits; lam (H,) or (N, H).  Returns (out, mag, gain) of
+    (N, H, W): rows outside the batch are NaN, rows without keys 0.  mag = sum_t (p1 + |lam| p2) |v_t|:
+    what errors of the weights and values are relative to, before the norm; gain: the bound of what the
+    norm and out_scale make of such an error (by itself, and through the sum of squares)."""
     n, hq, d = q.shape
     H, hkv = hq // 2, k.shape[1]
     qs = arr(q)
     qs = np.stack([qs[:, :H], qs[:, H:]] if halves else [qs[:, 0::2], qs[:, 1::2]])
+    lam = np.broadcast_to(arr(lam), (n, H))
     r, pos = S.positions(q_start, seq_lens, n)
     W = d if shared else 2 * d
-    o = np.full((2, n, H, W), np.nan)
+    out, mag = np.full((n, H, W), np.nan), np.zeros((n, H, W))
     for i in range(n):
         if r[i] < 0:
             continue
         m = seq_lens[r[i]]
         if causal:
             m = min(m, pos[i] + 1)
+        m = min(m, k.shape[2])
+        out[i] = 0
         if m <= 0:
-            o[:, i] = 0
             continue
         for h in range(H):
             if shared:
@@ -101,13 +105,17 @@ def diff_attend(q, k, v, lam, q_start, seq_lens, scale, causal, shared, halves, 
                 p, P = h // (H // (hkv // 2)), hkv // 2
                 ks = [p, P + p] if halves else [2 * p, 2 * p + 1]
                 val = np.concatenate([v[r[i], s, :m] for s in ks], -1)
-            for j in range(2):
+            for j, f in enumerate((1.0, -lam[i, h])):
                 s = k[r[i], ks[j], :m] @ qs[j, i, h] * scale
                 e = np.exp(s - s.max())
-                o[j, i, h] = e @ val / e.sum()
-    out = o[0] - np.broadcast_to(arr(lam), (n, H))[..., None] * o[1]
+                out[i, h] += f * (e @ val) / e.sum()
+                mag[i, h] += abs(f) * (e @ np.abs(val)) / e.sum()
+    gain = np.full((n, H, 1), abs(out_scale))
     if norm is not None:
+        w = np.abs(arr(norm) + offset) * abs(out_scale)
         with np.errstate(invalid="ignore", divide="ignore"):
-            y = out / np.sqrt((out * out).mean(-1, keepdims=True) + eps) * (arr(norm) + offset)
+            rms = np.sqrt((out * out).mean(-1, keepdims=True) + eps)
+            y = out / rms * (arr(norm) + offset)
+            gain = w * (1 + np.abs(out) / rms) / rms
         out = np.where(out == 0, 0, y)
-    return out * out_scale, o[0], o[1]
+    return out * out_scale, mag, gain

@@ -136,3 +136,63 @@ def test_residual_norm_wrapper_checks():
     meta = torch.zeros((3, 64), requires_grad=True)
     with pytest.raises(RuntimeError):
         ops.residual_norm(meta, x)
+
+
+def diff_call(g=None, c=_lib.Cache(1 << 20, 12, 4, 0, 0, 0), q=t4((1, 8, 10, 128)), out=None, batch=BATCH,
+              scale=0.1, engine=0, shared=0, halves=0, lam=1 << 40, ls=(0, 1), norm=None, t=TABLES,
+              ws=1 << 20, nbytes=None):
+    lib = _lib.load()
+    g = g or geom()
+    out = out or far((1, q.shape[1] // 2, q.shape[2], q.shape[3] * (1 if shared else 2)))
+    a = _lib.DiffArgs(ctypes.pointer(q), ctypes.pointer(out), batch, scale, 1, engine, shared, halves, lam,
+                      (ctypes.c_int64 * 2)(*ls), None if norm is None else ctypes.pointer(norm), 1.0)
+    need = lib.tq_diff_attend_ragged_workspace_bytes(r(g), r(c), r(a))
+    rc = lib.tq_diff_attend_ragged(r(g), r(t), r(c), r(a), ws, need if nbytes is None else nbytes, None)
+    return rc, _lib.last_error(), need
+
+
+@pytest.mark.parametrize("kw,what", [
+    (dict(engine=4), "engine"), (dict(engine=-1), "engine"), (dict(g=geom(D=96), q=t4((1, 8, 10, 96))), "no kernel"),
+    (dict(g=geom(kb=7)), "no kernel"), (dict(q=t4((1, 7, 10, 128)), out=far((1, 3, 10, 256))), "pairs"),
+    (dict(q=t4((1, 6, 10, 128))), "multiple"), (dict(c=_lib.Cache(1 << 20, 9, 4, 0, 0, 0), q=t4((1, 6, 10, 128))),
+                                                "multiple"),
+    (dict(shared=1, q=t4((1, 12, 10, 128))), "multiple"), (dict(shared=1, halves=1), "next to each other"),
+    (dict(out=far((1, 4, 10, 128))), "must be"), (dict(shared=1, out=far((1, 4, 10, 256))), "must be"),
+    (dict(out=far((1, 4, 9, 256))), "differ in rows"), (dict(q=t4((1, 2048, 1, 128))), "1024 query heads"),
+    (dict(batch=_lib.Ragged(5, 4096, 4096, 1)), "multiple"), (dict(c=_lib.Cache(1 << 20, 12, 1 << 27)), "32 bits"),
+])
+def test_diff_attend_refusals(kw, what):
+    rc, err, need = diff_call(**kw)
+    assert rc == _lib.TQ_ERR_INVALID and need == 0 and what in err, err
+
+
+def test_diff_attend_refusals_of_the_call_alone():
+    big = (1, 4, 10, 256)
+    for kw, what in ((dict(out=t4(big, data=(1 << 20) + 256)), "overlaps"), (dict(out=t4(big)), "overlaps"),
+                     (dict(out=far(big, stride=[0, 0, 1024, 1])), "share memory"), (dict(lam=None), "NULL"),
+                     (dict(lam=(1 << 40) + 2), "aligned"), (dict(lam=1 << 30, ls=(4, 1)), "lambda"),
+                     (dict(norm=_lib.HeadNorm(None, 0, 1e-6, 0)), "norm"),
+                     (dict(norm=_lib.HeadNorm(4096, 0, -1.0, 0)), "norm"),
+                     (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"),
+                     (dict(t=_lib.Tables(*([4096] * 9))), "rot_f16")):
+        rc, err, need = diff_call(**kw)
+        assert rc == _lib.TQ_ERR_INVALID and need > 0 and what in err, err
+    for kw in (dict(nbytes=100), dict(ws=(1 << 20) + 64), dict(ws=None)):
+        rc, err, need = diff_call(**kw)
+        assert rc == _lib.TQ_ERR_WORKSPACE and str(need) in err
+
+
+def test_diff_wrapper_checks():
+    x = torch.zeros((3, 4, 128))
+    batch = ops.RaggedBatch(torch.tensor([0, 3], dtype=torch.int32), torch.tensor([3], dtype=torch.int32), 3)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        ops.diff_attend_ragged(None, None, x, batch, ops.DiffHeads(torch.ones(2)))
+    for kw in (dict(lam=torch.ones(2).double()), dict(lam=torch.ones((1, 1, 2))), dict(lam=torch.ones(2), keys="both"),
+               dict(lam=torch.ones(2), pairs="odd"), dict(lam=torch.ones(2), keys="shared", pairs="halves")):
+        with pytest.raises(ValueError):
+            ops.DiffHeads(**kw)
+    lam = ops.DiffHeads.lam_of(*(torch.full((3, 4), f) for f in (0.1, 0.2, 0.3, 0.1)), 0.5)
+    want = torch.tensor(0.08, dtype=torch.float64).exp() - torch.tensor(0.12, dtype=torch.float64).exp() + 0.5
+    assert lam.shape == (3,) and (lam - want).abs().max() < 2e-8 + 2.0 ** -24
+    p = ops.DiffHeads(torch.ones((5, 4))[:, ::2])
+    assert p.c[1:] == (4, 2) and ops.DiffHeads(torch.ones((5, 1))).c[1:] == (1, 0)
