@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p0
 struct ListShape {
   bool used;
   int64_t q_lo, q_hi;
-  int hc, pcta, rows, keys, G;
+  int hc, pcta, rows, width, keys, G;      // width: of a partial row
   int64_t wanted, max_seg, max_slot;
   size_t off_nseg, off_segs, off_arrived, off_ml, off_part, off_qp;
 };
@@ -352,6 +352,7 @@ struct AttendCall {
   int64_t Hkv;                             // KV heads as the head groups count them
   bool precise;
   HeadView hv;
+  const tq_diff_args* diff;                // differential attention, or NULL
 };
 
 AttendCall plain_call(const tq_cache* c, const tq_attend_args* a) {
@@ -372,6 +373,8 @@ AttendCall plain_call(const tq_cache* c, const tq_attend_args* a) {
 // 1,024 rows 927 against 1,427; D128, fp16 results, 1,024 rows 3,281 against 3,925)
 // and runs the codes that the few-row kernel has no table for (above 4 bits).
 constexpr int kFewRows = 128;
+// The same of the kernel for pairs of maps (rows of one map) against the mma.sync kernel.
+constexpr int kPairRows = 64;
 
 // The kernels that a call may use: few rows, and tcgen05 (else mma.sync) for the
 // others.  The tcgen05 kernel's operands are single fp16 values: for fp16 and fp32
@@ -383,7 +386,7 @@ struct Kernels {
 
 Kernels attend_kernels(const tq_geom* G, int engine, bool precise, bool own) {
   Kernels k;
-  k.few = attend_few_applies(G) && (engine == 0 || engine == 3) && !own;
+  k.few = (own ? attend_pair_applies(G) : attend_few_applies(G)) && (engine == 0 || engine == 3);
   k.tc = prefill_tc_applies(G) && (engine == 2 || (engine == 0 && !precise)) && !own;
   return k;
 }
@@ -397,16 +400,19 @@ AttendShape attend_shape(const tq_geom* G, const AttendCall& x) {
   const Kernels kernels = attend_kernels(G, a->engine, x.precise, x.hv.own);
   s.tc = kernels.tc;
   const bool can = kernels.few;
-  const int64_t few_q = s.tc ? tmax<int64_t>(kFewRows / g, 1) : most;
+  const bool own = x.hv.own;
+  const int64_t few_q = s.tc ? tmax<int64_t>(kFewRows / g, 1)
+                        : own && a->engine == 0 && attend_mma_applies(G) ? tmax<int64_t>(kPairRows / g, 1)
+                                                                         : most;
   size_t off = 256;                        // the first 64 bytes: the decode's status word
   auto take = [&](size_t bytes) {
     const size_t at = off;
     off = (off + bytes + 255) & ~(size_t)255;
     return at;
   };
-  auto finish = [&](ListShape& l) {
+  auto finish = [&](ListShape& l, int64_t kv_heads) {
     l.used = true;
-    l.G = (int)(s.Hkv * ((g + l.hc - 1) / l.hc));
+    l.G = (int)(kv_heads * ((g + l.hc - 1) / l.hc));
     // tiles: one per started block of positions; L cuts off at most wanted / G
     // segments beyond them, and a cut tile has at most twice its extra ones
     const int64_t extra = l.wanted / l.G + 1;
@@ -415,19 +421,21 @@ AttendShape attend_shape(const tq_geom* G, const AttendCall& x) {
     l.off_segs = take(l.max_seg * sizeof(RaggedSeg));
     l.off_arrived = take(l.max_slot * l.G * 4);
     l.off_ml = take((size_t)l.max_slot * l.G * l.rows * 8);
-    l.off_part = take((size_t)l.max_slot * l.G * l.rows * G->head_dim * 4);
+    l.off_part = take((size_t)l.max_slot * l.G * l.rows * l.width * 4);
   };
   const bool wide = !can || a->batch.max_q_len > few_q;
   if (can) {
     ListShape& l = s.few;
     l.q_hi = wide ? few_q : most;
-    l.rows = g * a->batch.max_q_len <= 8 ? 8 : 16;
-    l.hc = (int)tmin<int64_t>(g, l.rows);
-    l.pcta = l.rows / l.hc;
+    l.rows = own || g * a->batch.max_q_len > 8 ? 16 : 8;   // own: 8 of either map
+    const int rows = own ? 8 : l.rows;
+    l.hc = (int)tmin<int64_t>(g, rows);
+    l.pcta = rows / l.hc;
+    l.width = own ? 2 * G->head_dim : G->head_dim;
     l.keys = kPageTokens;
     l.wanted = (int64_t)kFewWaves * device_sm_count();
     l.off_nseg = 64;
-    finish(l);
+    finish(l, own ? x.hv.P : s.Hkv);
     // q' rows of its tokens: beside a wide list at most few_q of each request
     s.qp_stride = wide ? few_q : 0;
     l.off_qp = take((size_t)(wide ? R * few_q : N) * a->q->shape[1] * G->head_dim *
@@ -442,10 +450,11 @@ AttendShape attend_shape(const tq_geom* G, const AttendCall& x) {
     l.hc = g % 8 == 0 ? 8 : g % 4 == 0 ? 4 : g % 2 == 0 ? 2 : 1;
     l.rows = s.tc ? 256 : 128;
     l.pcta = l.rows / l.hc;
+    l.width = G->head_dim;
     l.keys = s.tc ? 2 * kPageTokens : kPageTokens;
     l.wanted = (int64_t)kWaves * device_sm_count();
     l.off_nseg = 72;
-    finish(l);
+    finish(l, s.Hkv);
   }
   s.bytes = off;
   return s;
@@ -515,8 +524,11 @@ int launch_attend(const tq_geom* G, const tq_tables* t, const tq_cache* c, const
   ragged_plan_kernel<<<lists + query_ctas, kPlanThreads, 0, st>>>(plan[0], plan[lists - 1], lists, qp);
   if (check_launch("tq_attend_ragged/plan") != TQ_OK) return TQ_ERR_CUDA;
   if (s.few.used) {
-    const int rc = launch_attend_few(G, t, c, a, x.precise, rg[0], s.Hkv, s.few.hc, s.few.pcta, s.few.rows,
-                                     qp.qp, s.qp_stride, s.few.max_seg * s.few.G, status, st);
+    const int64_t most = s.few.max_seg * s.few.G;
+    const int rc = x.hv.own ? launch_attend_pair(G, t, c, x.diff, x.precise, rg[0], s.few.hc, s.few.pcta,
+                                                 qp.qp, s.qp_stride, most, status, st)
+                            : launch_attend_few(G, t, c, a, x.precise, rg[0], s.Hkv, s.few.hc, s.few.pcta,
+                                                s.few.rows, qp.qp, s.qp_stride, most, status, st);
     if (rc != TQ_OK) return rc;
   }
   if (s.wide.used && s.tc)
@@ -534,6 +546,8 @@ int launch_attend(const tq_geom* G, const tq_tables* t, const tq_cache* c, const
 struct DiffJoin {
   const float* o;
   const int32_t* rows;                     // [2] the batch's rows
+  RaggedView rv;
+  int64_t q_lo;                            // requests of up to so many rows are done already
   int H;
   int64_t N;
   const float* lambda; int64_t ls[2];
@@ -551,6 +565,7 @@ __global__ void __launch_bounds__(256) diff_join_kernel(DiffJoin p) {
   for (int64_t i = blockIdx.x * 8 + (threadIdx.x >> 5); i < n * p.H; i += step) {
     const int64_t row = lo + i / p.H;
     const int h = (int)(i % p.H);
+    if (p.q_lo && request_at(p.rv, request_of(p.rv, row)).q_len <= p.q_lo) continue;
     const float* o = p.o + (row * p.H + h) * (2 * 32 * E);
     const float lambda = __ldg(p.lambda + row * p.ls[0] + h * p.ls[1]);
     float x[E], ss = 0.f;
@@ -580,6 +595,7 @@ struct DiffCall {
   tq_tensor4 o;                            // fp32 results
   int H, W;
   AttendCall x;
+  int64_t join_lo;                         // rows that the join leaves to the kernel of pairs; -1: all
   size_t off_rows, off_o, bytes;           // in the workspace, behind the attention's
 };
 
@@ -608,10 +624,12 @@ void diff_call(const tq_geom* G, const tq_cache* c, const tq_diff_args* d, DiffC
   x.hv.g = d->shared_keys ? 2 * k.H / heads : k.H / (heads / 2);
   x.hv.streams = heads;
   x.Hkv = d->shared_keys ? heads : 2 * heads;
-  const size_t at = attend_shape(G, x).bytes;
-  k.off_rows = at;
-  k.off_o = at + 256;
-  k.bytes = k.off_o + (size_t)N * 2 * k.H * k.W * 4;
+  x.diff = d;
+  const AttendShape s = attend_shape(G, x);
+  k.join_lo = !x.hv.own || !s.few.used ? 0 : s.wide.used ? s.few.q_hi : -1;
+  k.off_rows = s.bytes;
+  k.off_o = s.bytes + 256;
+  k.bytes = k.off_o + (k.join_lo < 0 ? 0 : (size_t)N * 2 * k.H * k.W * 4);
 }
 
 }  // namespace
@@ -651,7 +669,10 @@ int launch_diff_attend(const tq_geom* G, const tq_tables* t, const tq_cache* c, 
   k.o.data = base + k.off_o;
   int32_t* rows = reinterpret_cast<int32_t*>(base + k.off_rows);
   if (const int rc = launch_attend(G, t, c, k.x, ws, rows, status, st)) return rc;
+  if (k.join_lo < 0) return TQ_OK;
   DiffJoin p = {};
+  p.rv = ragged_view(&d->batch, d->q->shape[2], c);
+  p.q_lo = k.join_lo;
   p.o = reinterpret_cast<const float*>(base + k.off_o);
   p.rows = rows;
   p.H = k.H;

@@ -88,6 +88,10 @@ size_t attend_ragged_workspace(const tq_geom* g, const tq_cache* c, const tq_att
 int launch_attend_ragged(const tq_geom* g, const tq_tables* t, const tq_cache* c,
                          const tq_attend_args* a, void* ws, uint32_t* status, cudaStream_t st);
 // Differential attention: a workspace of 0 bytes where no kernel applies.
+bool attend_pair_applies(const tq_geom* g);
+int launch_attend_pair(const tq_geom* g, const tq_tables* t, const tq_cache* c, const tq_diff_args* a,
+                       bool precise, const RaggedAttend& rg, int hc, int pcta, const __half* qp,
+                       int64_t qp_stride, int64_t grid, uint32_t* status, cudaStream_t st);
 bool diff_attend_applies(const tq_geom* g, const tq_diff_args* a);
 size_t diff_attend_workspace(const tq_geom* g, const tq_cache* c, const tq_diff_args* a);
 int launch_diff_attend(const tq_geom* g, const tq_tables* t, const tq_cache* c, const tq_diff_args* a,

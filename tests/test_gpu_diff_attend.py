@@ -118,7 +118,7 @@ def skip_without_kernel(keys, engine):
         pytest.skip("no such kernel")
 
 
-NO_OWN = (2, 3)
+NO_OWN = (2,)
 
 
 def setup_case(lens, D=128, kb=4, vb=4, H=4, Hkv=4, keys="own", pairs="adjacent", seed=3, norm=True, lead=0):
