@@ -10,6 +10,7 @@
 // Sums go by shuffles and one barrier each, always in the same order.
 #include "tq_common.cuh"
 #include "tq_internal.h"
+#include "tq_tc.cuh"
 
 #include <type_traits>
 
@@ -31,7 +32,7 @@ struct NormParams {
   int act;
   float scale;
   int64_t xs[4], rs[4], gs[4], ys[4], hs[4];
-  int64_t rows, n1, n2;         // rows: [rows / (n1 n2)][n1][n2], below 2^31
+  int64_t rows, n1, n2;         // rows: [rows / (n1 n2)][n1][n2], below 2^31; n2 = 0: one dim, stride [2]
   int C;
   NormSide post, pre;
 };
@@ -125,8 +126,17 @@ __device__ __forceinline__ void load_param(float (&v)[V], const void* base, int 
   }
 }
 
+// 1 / (1 + e^-g): e^-g = 2^t (1 + d ln 2) with t + d = -g log2 e in two parts, as t alone is
+// off by |g| 2^-24 (2^-22 in all; the library's exponential and quotient took half of the
+// instructions of a gated row).
 __device__ __forceinline__ float activate(float g, int act) {
-  return act == TQ_GATE_SIGMOID ? 1.f / (1.f + expf(-g)) : act == TQ_GATE_TANH ? tanhf(g) : g;
+  if (act == TQ_GATE_SIGMOID) {
+    const float x = fminf(fmaxf(-g, -126.f), 126.f);       // (a NaN gate is let through below)
+    const float t = x * 1.44269504f, d = fmaf(x, 1.44269504f, -t) + x * 1.92596299e-8f;
+    const float e = fast_exp2(t) * fmaf(d, 0.693147181f, 1.f);
+    return g != g ? g : __fdividef(1.f, 1.f + e);
+  }
+  return act == TQ_GATE_TANH ? tanhf(g) : g;
 }
 
 // Sum over the T threads of a row: a warp by itself, or a CTA through `part`, whose
@@ -143,19 +153,231 @@ __device__ __forceinline__ float row_sum(float x, int T, float (*part)[32], int&
   return s;
 }
 
-// T threads per row (a warp, or the CTA), 8 VPT values each in chunks of V
+// Offset of a row.
+__device__ __forceinline__ int64_t row_at(const NormParams& p, const int64_t (&s)[4], uint32_t r) {
+  if (p.n2 == 0) return r * s[2];
+  const uint32_t n1 = (uint32_t)p.n1, n2 = (uint32_t)p.n2, i01 = r / n2, i0 = i01 / n1;
+  return i0 * s[0] + (i01 - i0 * n1) * s[1] + (r - i01 * n2) * s[2];
+}
+
+using tc::f2;
+
+// The common case: rows of up to 8,192 values in chunks of V = 8 or 2 neighbours.  T threads
+// (a warp, or the CTA) take row after row, 8 values each, with what a column needs in
+// registers in 32 bits, gate and scale folded in:
+//   y = residual + (x r) A + B,   h = (y r') C + D
+// and the next two rows' values on their way.  GE: a gate per element, BIAS: B and D.  The
+// arithmetic, on fp32 pairs, is 6 instructions a value without a gate per element.
+template <int XT, int RT, int V, bool GE, bool BIAS, int MAXT>
+__global__ void __launch_bounds__(MAXT) residual_norm_rows_kernel(NormParams p, int T) {
+  constexpr int NK = 8 / V, NP = 4;                        // chunks and pairs of a thread
+  __shared__ float part[2][32];
+  int turn = 0;
+  const int t = threadIdx.x % T;
+  const uint32_t per = blockDim.x / T, step = gridDim.x * per, rows = (uint32_t)p.rows;
+  uint32_t row = blockIdx.x * per + threadIdx.x / T;
+  if (row >= rows) return;                                 // whole warps where a row is one's
+  auto col = [&](int k) { return (k * T + t) * V; };
+  auto inside = [&](int k) { return col(k) < p.C; };       // C is a multiple of V
+  struct Raw {
+    Chunk<XT, V> x[NK];
+    Chunk<RT, V> r[NK];
+    uint32_t g[GE ? NK : 1][V / 2];                        // a gate of 16 bits
+  };
+  auto fetch = [&](Raw& w, uint32_t r) {
+    const int64_t xb = row_at(p, p.xs, r), rb = row_at(p, p.rs, r), gb = GE ? row_at(p, p.gs, r) : 0;
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+      w.x[k].clear();
+      w.r[k].clear();
+      if (!inside(k)) continue;
+      w.x[k].load(p.x, xb + col(k));
+      w.r[k].load(p.r, rb + col(k));
+      if constexpr (GE) {
+        Chunk<TQ_F16, V> g;
+        g.load(p.g, gb + col(k));
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) w.g[k][i] = g.w[i];
+      }
+    }
+  };
+  Raw cur, nxt;
+  fetch(cur, row);
+  if (rows - row > step) fetch(nxt, row + step);
+  // a column's factors
+  f2 A[NP], B[BIAS ? NP : 1], C[NP], D[BIAS ? NP : 1];
+#pragma unroll
+  for (int k = 0; k < NK; ++k) {
+    float a[V], b[V], c[V], d[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) { a[e] = c[e] = 1.f; b[e] = d[e] = 0.f; }
+    if (inside(k)) {
+      auto param = [&](float (&v)[V], const void* base, int dtype, float add) {
+        if (!base) return;
+        load_param<V>(v, base, dtype, col(k));
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] += add;
+      };
+      param(a, p.post.w, p.post.dtype, p.post.offset);
+      param(c, p.pre.w, p.pre.dtype, p.pre.offset);
+      if (BIAS) {
+        param(b, p.post.b, p.post.dtype, 0.f);
+        param(d, p.pre.b, p.pre.dtype, 0.f);
+      }
+      float g[V];
+      const bool channel = !GE && p.gmode == 1;            // one for all rows
+      if (channel) load_param<V>(g, p.g, p.gd, col(k));
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float f = p.scale * (channel ? activate(g[e], p.act) : 1.f);
+        a[e] *= f;
+        b[e] *= f;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      const int i = (k * V + e) / 2;
+      A[i] = tc::f2_make(a[e], a[e + 1]);
+      C[i] = tc::f2_make(c[e], c[e + 1]);
+      if constexpr (BIAS) {
+        B[i] = tc::f2_make(b[e], b[e + 1]);
+        D[i] = tc::f2_make(d[e], d[e + 1]);
+      }
+    }
+  }
+  const float inv_c = 1.f / (float)p.C;
+  const f2 zero = tc::f2_make(0.f, 0.f);
+  auto pair_sum = [](f2 x) {
+    float lo, hi;
+    tc::f2_split(x, lo, hi);
+    return lo + hi;
+  };
+  for (;;) {
+    Raw far;
+    if (rows - row > 2 * (uint64_t)step) fetch(far, row + 2 * step);
+    f2 v[NP];
+#pragma unroll
+    for (int k = 0; k < NK; ++k)
+#pragma unroll
+      for (int e = 0; e < V; e += 2) v[(k * V + e) / 2] = tc::f2_make(cur.x[k].get(e), cur.x[k].get(e + 1));
+    // takes the mean off (where the norm does) and returns the factor
+    auto norm = [&](const NormSide& n) {
+      if (n.centered) {
+        f2 sum = v[0];
+        const f2 one = tc::f2_make(1.f, 1.f);
+#pragma unroll
+        for (int i = 1; i < NP; ++i) sum = tc::f2_fma(v[i], one, sum);
+        const float mean = row_sum(pair_sum(sum), T, part, turn) * inv_c;
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+          const f2 m = inside(k) ? tc::f2_make(-mean, -mean) : zero;
+#pragma unroll
+          for (int i = k * V / 2; i < (k + 1) * V / 2; ++i) v[i] = tc::f2_fma(m, one, v[i]);
+        }
+      }
+      f2 ss = tc::f2_mul(v[0], v[0]);
+#pragma unroll
+      for (int i = 1; i < NP; ++i) ss = tc::f2_fma(v[i], v[i], ss);
+      return 1.f / sqrtf(fmaf(row_sum(pair_sum(ss), T, part, turn), inv_c, n.eps));
+    };
+    const float r1 = p.post.on ? norm(p.post) : 1.f;
+    const f2 rr = tc::f2_make(r1, r1);
+    float one = 1.f;
+    if (!GE && p.gmode == 2) one = activate(load_elem(p.g, p.gd, row_at(p, p.gs, row)), p.act);
+    const int64_t yb = row_at(p, p.ys, row);
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+      float o[V];
+#pragma unroll
+      for (int e = 0; e < V; e += 2) {
+        const int i = (k * V + e) / 2;
+        const f2 res = tc::f2_make(cur.r[k].get(e), cur.r[k].get(e + 1));
+        f2 z = tc::f2_mul(v[i], rr);
+        if (GE || p.gmode == 2) {
+          f2 f = tc::f2_make(one, one);
+          if constexpr (GE) {
+            const uint32_t u = cur.g[k][e / 2];
+            float lo, hi;
+            if (p.gd == TQ_F16) {
+              const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&u));
+              lo = h.x; hi = h.y;
+            } else {
+              lo = __uint_as_float(u << 16);
+              hi = __uint_as_float(u & 0xFFFF0000u);
+            }
+            f = tc::f2_make(activate(lo, p.act), activate(hi, p.act));
+          }
+          z = BIAS ? tc::f2_fma(z, A[i], B[i]) : tc::f2_mul(z, A[i]);
+          v[i] = tc::f2_fma(z, f, res);
+        } else if constexpr (BIAS) {
+          const f2 zb = tc::f2_fma(z, A[i], B[i]);
+          v[i] = tc::f2_fma(zb, tc::f2_make(1.f, 1.f), res);
+        } else {
+          v[i] = tc::f2_fma(z, A[i], res);
+        }
+        if (!inside(k)) v[i] = zero;
+        tc::f2_split(v[i], o[e], o[e + 1]);
+      }
+      if (inside(k)) Chunk<RT, V>::store(p.y, yb + col(k), o);
+    }
+    if (p.h) {
+      const float r2 = norm(p.pre);
+      const f2 r2r = tc::f2_make(r2, r2);
+      const int64_t hb = row_at(p, p.hs, row);
+#pragma unroll
+      for (int k = 0; k < NK; ++k) {
+        float o[V];
+#pragma unroll
+        for (int e = 0; e < V; e += 2) {
+          const int i = (k * V + e) / 2;
+          f2 z = tc::f2_mul(v[i], r2r);
+          z = BIAS ? tc::f2_fma(z, C[i], D[i]) : tc::f2_mul(z, C[i]);
+          tc::f2_split(z, o[e], o[e + 1]);
+        }
+        if (inside(k)) Chunk<XT, V>::store(p.h, hb + col(k), o);
+      }
+    }
+    if (rows - row <= step) return;
+    row += step;
+    cur = nxt;
+    nxt = far;
+  }
+}
+
+using NormFn = void (*)(NormParams, int);
+
+// Where the plain form's registers would halve the CTAs of an SM, 64; else what up to 384
+// threads may have: gates and biases then go without spills.
+template <int XT, int RT, int V>
+NormFn rows_fn(bool ge, bool bias, bool wide) {
+#define TQ_ROWS(GE, BIAS) \
+  if (ge == GE && bias == BIAS) \
+    return wide ? residual_norm_rows_kernel<XT, RT, V, GE, BIAS, 1024> : residual_norm_rows_kernel<XT, RT, V, GE, BIAS, 384>;
+  TQ_ROWS(false, false) TQ_ROWS(false, true) TQ_ROWS(true, false) TQ_ROWS(true, true)
+#undef TQ_ROWS
+  return nullptr;
+}
+
+template <int XT>
+NormFn rows_fn_x(int rd, int v, bool ge, bool bias, bool wide) {
+#define TQ_ROWS(RT) \
+  if (rd == RT) return v == 8 ? rows_fn<XT, RT, 8>(ge, bias, wide) : rows_fn<XT, RT, 2>(ge, bias, wide);
+  TQ_ROWS(TQ_F32) TQ_ROWS(TQ_F16) TQ_ROWS(TQ_BF16)
+#undef TQ_ROWS
+  return nullptr;
+}
+
+// Everything else: T threads per row (a warp, or the CTA), 8 VPT values each in chunks of V
 // neighbours.  V = 1 takes any stride.
 template <int XT, int RT, int VPT, int V>
-__global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) residual_norm_kernel(NormParams p, int T) {
+__global__ void __launch_bounds__(VPT == 1 ? 1024 : 512) residual_norm_kernel(NormParams p, int T) {
   constexpr int NK = 8 * VPT / V;                          // chunks of a thread
   __shared__ float part[2][32];
   int turn = 0;
   const int t = threadIdx.x % T;
   const int64_t row = (int64_t)blockIdx.x * (blockDim.x / T) + threadIdx.x / T;
   if (row >= p.rows) return;                               // whole warps where a row is one's
-  const uint32_t n1 = (uint32_t)p.n1, n2 = (uint32_t)p.n2, i01 = (uint32_t)row / n2;
-  const uint32_t i2 = (uint32_t)row - i01 * n2, i0 = i01 / n1, i1 = i01 - i0 * n1;
-  auto at = [&](const int64_t (&s)[4]) { return i0 * s[0] + i1 * s[1] + i2 * s[2]; };
+  auto at = [&](const int64_t (&s)[4]) { return row_at(p, s, (uint32_t)row); };
   const int64_t xb = at(p.xs), rb = at(p.rs);
   // values of chunk k: from column c(k) on
   auto col = [&](int k) { return (k * T + t) * V; };
@@ -236,8 +458,6 @@ __global__ void __launch_bounds__(VPT <= 2 ? 1024 : 512) residual_norm_kernel(No
     if (inside(k)) Chunk<XT, V>::store(p.h, hb + place(p.hs, k), v[k]);
 }
 
-using NormFn = void (*)(NormParams, int);
-
 template <int XT, int RT>
 NormFn norm_fn(int vpt, int v) {
 #define TQ_NORM(N, V) if (vpt == N && v == V) return residual_norm_kernel<XT, RT, N, V>;
@@ -312,6 +532,12 @@ int launch_residual_norm(const tq_residual_norm_args* a, cudaStream_t st) {
     p.gmode = g->stride[3] == 0 ? 2 : 1;
     p.act = a->gate_act;
   }
+  // leading dims that are one run of rows in every tensor
+  bool flat = true;
+  for (const tq_tensor4* z : {x, r, g, a->residual_out, p.h ? a->out : nullptr})
+    for (int i = 0; z && i < 2; ++i)
+      flat = flat && (z->shape[i] == 1 || z->stride[i] == z->stride[2] * (i ? z->shape[2] : z->shape[1] * z->shape[2]));
+  if (flat) p.n2 = 0;
   p.scale = a->scale;
   p.post = norm_side(a->post);
   p.pre = norm_side(a->pre);
@@ -324,16 +550,33 @@ int launch_residual_norm(const tq_residual_norm_args* a, cudaStream_t st) {
       break;
     }
   }
+  const int units = (p.C + 7) / 8;
+  // a gate that differs from row to row
+  bool per_row = false;
+  for (int i = 0; g && i < 3; ++i) per_row = per_row || (g->shape[i] > 1 && g->stride[i] != 0);
+  const bool ge = p.gmode == 1 && per_row;
+  if (v > 1 && units <= 1024 && !(ge && p.gd == TQ_F32)) {
+    const bool bias = p.post.b || p.pre.b;
+    const int T = (units + 31) & ~31, per = T == 32 ? 4 : 1;
+    const bool wide = T > 384;
+    const NormFn fn = x->dtype == TQ_F32   ? rows_fn_x<TQ_F32>(r->dtype, v, ge, bias, wide)
+                      : x->dtype == TQ_F16 ? rows_fn_x<TQ_F16>(r->dtype, v, ge, bias, wide)
+                                           : rows_fn_x<TQ_BF16>(r->dtype, v, ge, bias, wide);
+    int64_t grid = (p.rows + per - 1) / per;
+    if (grid > device_sm_count())
+      grid = tmin(grid, (int64_t)device_sm_count() * occupancy((const void*)fn, T * per, 0));
+    fn<<<(unsigned)grid, T * per, 0, st>>>(p, T);
+    return check_launch("tq_residual_norm");
+  }
   // Threads of a row and their values, 8 vpt each: 32 of them leave most rows in flight on
   // an SM, 8 end a call of few rows sooner; 64 only where 512 threads need them.
-  const int units = (p.C + 7) / 8;
   int vpt, T;
   if (units <= 128) {
     T = 32;
     vpt = units <= 32 ? 1 : units <= 64 ? 2 : 4;
   } else {
     const bool few = p.rows <= 2 * device_sm_count();
-    vpt = few && units <= 1024 ? 1 : few && units <= 2048 ? 2 : units <= 2048 ? 4 : 8;
+    vpt = units <= 1024 && few ? 1 : units <= 1024 ? 2 : units <= 2048 ? 4 : 8;
     T = ((units + vpt - 1) / vpt + 31) & ~31;
   }
   const NormFn fn = x->dtype == TQ_F32   ? norm_fn_x<TQ_F32>(r->dtype, vpt, v)
