@@ -36,13 +36,18 @@ constexpr int kClasses = 32;               // length classes of segments
 // of 64, 76, 76, 84.
 constexpr int kWaves = 2, kMinKeys = 512;
 constexpr int kFewWaves = 5, kFewMinKeys = 512;
+// The list of both maps' rows (two CTAs a SM for heads of 128): 3 a SM, or 2, all at once, where
+// there are fewer tiles than a quarter of the segments: a decode step of 64 requests, 124
+// us with 5, 123 with 3, 126 with 2; 16 x 4 rows over 16,000 keys 224, 211, 258; 64 single
+// rows over 1,000 76, 49, 49; one over 65,000 114, 106, 82.
+constexpr int kPairWaves = 3, kPairOnce = 2;
 
 struct PlanParams {
   RaggedView rv;
   int64_t q_lo, q_hi;                      // the list's requests: q_lo < q_len <= q_hi
   int pcta, keys, key_shift;               // query positions per tile, keys per key tile (2^shift)
   int causal, G;
-  int64_t wanted;                          // segments wanted, all head groups together
+  int64_t wanted, once;                    // segments wanted, all head groups together; with few tiles
   int min_tiles, max_seg, max_slot;
   RaggedSeg* segs;
   int32_t* nseg;
@@ -276,7 +281,8 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(PlanParams p0
   // tiles that fill half of the wanted CTAs by themselves need no short segments
   // (16 batches of encoder states, 304 rows: 36.7 us, with them 41.2)
   const int least = (all / kOneTile) * (unsigned)p.G * 2 >= p.wanted ? 2 * p.min_tiles : p.min_tiles;
-  const int L = (int)tmax<unsigned long long>(least, (total + p.wanted - 1) / p.wanted);
+  const int64_t wanted = (all / kOneTile) * (unsigned)p.G * 4 < (unsigned long long)p.wanted ? p.once : p.wanted;
+  const int L = (int)tmax<unsigned long long>(least, (total + wanted - 1) / wanted);
   // class of a segment of n key tiles: 0 the longest (L), 31 the shortest
   auto class_of = [&](int n) { return kClasses - 1 - (int)((unsigned)(n * kClasses - 1) / (unsigned)L); };
   for_tiles(p, own, [&](int, int, int nkt) {
@@ -334,7 +340,7 @@ struct ListShape {
   bool used;
   int64_t q_lo, q_hi;
   int hc, pcta, rows, width, keys, G;      // width: of a partial row
-  int64_t wanted, max_seg, max_slot;
+  int64_t wanted, once, max_seg, max_slot;
   size_t off_nseg, off_segs, off_arrived, off_ml, off_part, off_qp;
 };
 
@@ -373,8 +379,6 @@ AttendCall plain_call(const tq_cache* c, const tq_attend_args* a) {
 // 1,024 rows 927 against 1,427; D128, fp16 results, 1,024 rows 3,281 against 3,925)
 // and runs the codes that the few-row kernel has no table for (above 4 bits).
 constexpr int kFewRows = 128;
-// The same of the kernel for pairs of maps (rows of one map) against the mma.sync kernel.
-constexpr int kPairRows = 64;
 
 // The kernels that a call may use: few rows, and tcgen05 (else mma.sync) for the
 // others.  The tcgen05 kernel's operands are single fp16 values: for fp16 and fp32
@@ -401,9 +405,7 @@ AttendShape attend_shape(const tq_geom* G, const AttendCall& x) {
   s.tc = kernels.tc;
   const bool can = kernels.few;
   const bool own = x.hv.own;
-  const int64_t few_q = s.tc ? tmax<int64_t>(kFewRows / g, 1)
-                        : own && a->engine == 0 && attend_mma_applies(G) ? tmax<int64_t>(kPairRows / g, 1)
-                                                                         : most;
+  const int64_t few_q = s.tc ? tmax<int64_t>(kFewRows / g, 1) : most;
   size_t off = 256;                        // the first 64 bytes: the decode's status word
   auto take = [&](size_t bytes) {
     const size_t at = off;
@@ -433,7 +435,8 @@ AttendShape attend_shape(const tq_geom* G, const AttendCall& x) {
     l.pcta = rows / l.hc;
     l.width = own ? 2 * G->head_dim : G->head_dim;
     l.keys = kPageTokens;
-    l.wanted = (int64_t)kFewWaves * device_sm_count();
+    l.wanted = (int64_t)(own ? kPairWaves : kFewWaves) * device_sm_count();
+    l.once = own ? (int64_t)kPairOnce * device_sm_count() : l.wanted;
     l.off_nseg = 64;
     finish(l, own ? x.hv.P : s.Hkv);
     // q' rows of its tokens: beside a wide list at most few_q of each request
@@ -452,7 +455,7 @@ AttendShape attend_shape(const tq_geom* G, const AttendCall& x) {
     l.pcta = l.rows / l.hc;
     l.width = G->head_dim;
     l.keys = s.tc ? 2 * kPageTokens : kPageTokens;
-    l.wanted = (int64_t)kWaves * device_sm_count();
+    l.wanted = l.once = (int64_t)kWaves * device_sm_count();
     l.off_nseg = 72;
     finish(l, s.Hkv);
   }
@@ -481,6 +484,7 @@ int launch_attend(const tq_geom* G, const tq_tables* t, const tq_cache* c, const
     p.G = l->G;
     p.wanted = l->wanted;
     p.min_tiles = (l == &s.few ? kFewMinKeys : kMinKeys) / l->keys;
+    p.once = l->once;
     p.max_seg = (int)l->max_seg;
     p.max_slot = (int)l->max_slot;
     p.nseg = reinterpret_cast<int32_t*>(base + l->off_nseg);
@@ -546,8 +550,6 @@ int launch_attend(const tq_geom* G, const tq_tables* t, const tq_cache* c, const
 struct DiffJoin {
   const float* o;
   const int32_t* rows;                     // [2] the batch's rows
-  RaggedView rv;
-  int64_t q_lo;                            // requests of up to so many rows are done already
   int H;
   int64_t N;
   const float* lambda; int64_t ls[2];
@@ -565,7 +567,6 @@ __global__ void __launch_bounds__(256) diff_join_kernel(DiffJoin p) {
   for (int64_t i = blockIdx.x * 8 + (threadIdx.x >> 5); i < n * p.H; i += step) {
     const int64_t row = lo + i / p.H;
     const int h = (int)(i % p.H);
-    if (p.q_lo && request_at(p.rv, request_of(p.rv, row)).q_len <= p.q_lo) continue;
     const float* o = p.o + (row * p.H + h) * (2 * 32 * E);
     const float lambda = __ldg(p.lambda + row * p.ls[0] + h * p.ls[1]);
     float x[E], ss = 0.f;
@@ -595,7 +596,7 @@ struct DiffCall {
   tq_tensor4 o;                            // fp32 results
   int H, W;
   AttendCall x;
-  int64_t join_lo;                         // rows that the join leaves to the kernel of pairs; -1: all
+  bool join;                               // false: the kernel of both maps joins them itself
   size_t off_rows, off_o, bytes;           // in the workspace, behind the attention's
 };
 
@@ -626,10 +627,10 @@ void diff_call(const tq_geom* G, const tq_cache* c, const tq_diff_args* d, DiffC
   x.Hkv = d->shared_keys ? heads : 2 * heads;
   x.diff = d;
   const AttendShape s = attend_shape(G, x);
-  k.join_lo = !x.hv.own || !s.few.used ? 0 : s.wide.used ? s.few.q_hi : -1;
+  k.join = !(x.hv.own && s.few.used);
   k.off_rows = s.bytes;
   k.off_o = s.bytes + 256;
-  k.bytes = k.off_o + (k.join_lo < 0 ? 0 : (size_t)N * 2 * k.H * k.W * 4);
+  k.bytes = k.off_o + (k.join ? (size_t)N * 2 * k.H * k.W * 4 : 0);
 }
 
 }  // namespace
@@ -669,10 +670,8 @@ int launch_diff_attend(const tq_geom* G, const tq_tables* t, const tq_cache* c, 
   k.o.data = base + k.off_o;
   int32_t* rows = reinterpret_cast<int32_t*>(base + k.off_rows);
   if (const int rc = launch_attend(G, t, c, k.x, ws, rows, status, st)) return rc;
-  if (k.join_lo < 0) return TQ_OK;
+  if (!k.join) return TQ_OK;
   DiffJoin p = {};
-  p.rv = ragged_view(&d->batch, d->q->shape[2], c);
-  p.q_lo = k.join_lo;
   p.o = reinterpret_cast<const float*>(base + k.off_o);
   p.rows = rows;
   p.H = k.H;

@@ -642,6 +642,9 @@ append_ragged_tc_kernel(const __grid_constant__ RaggedTc p, int which) {
                                      pp.abort_flag, p.status));
       if (!__all_sync(0xffffffffu, ok)) break;
       Vecs& vec = ring[it % kRing];
+      // AXES: the angles of a token serve its heads, which lie next to each other
+      int64_t turned = -1;
+      float ac[8], as[8];
       unsigned char* hi = sm + SM::OFF_A + st * 2 * S::kTerm;
 #pragma unroll
       for (int k = 0; k < NIT; ++k) {
@@ -688,23 +691,32 @@ append_ragged_tc_kernel(const __grid_constant__ RaggedTc p, int which) {
           };
           if constexpr (AXES) {
             auto row_of = [&](int a) { return axis_row(to, a); };
-            float c[8], s[8];
-            if (pairs) {
-              if (turn_a) {
-                load_axes<8>(c, s, p.f, ga, row_of);
+            if (to != turned) {
+              turned = to;
+              if (pairs) {
+                if (turn_a) load_axes<8>(ac, as, p.f, ga, row_of);
+              } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) rotate(v[e], v[8 + e], c[e], s[e]);
-              }
-            } else {
-#pragma unroll
-              for (int g = 0; g < 2; ++g) {
-                if (g ? turn_b : turn_a) {
+                for (int g = 0; g < 2; ++g) {
+                  if (!(g ? turn_b : turn_a)) continue;
                   float c4[4], s4[4];
                   load_axes<4>(c4, s4, p.f, (g ? gb : ga) / 2, row_of);
 #pragma unroll
-                  for (int e = 0; e < 4; ++e) rotate(v[8 * g + 2 * e], v[8 * g + 2 * e + 1], c4[e], s4[e]);
+                  for (int e = 0; e < 4; ++e) { ac[4 * g + e] = c4[e]; as[4 * g + e] = s4[e]; }
                 }
               }
+            }
+            if (pairs) {
+              if (turn_a)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) rotate(v[e], v[8 + e], ac[e], as[e]);
+            } else {
+#pragma unroll
+              for (int g = 0; g < 2; ++g)
+                if (g ? turn_b : turn_a)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)
+                    rotate(v[8 * g + 2 * e], v[8 * g + 2 * e + 1], ac[4 * g + e], as[4 * g + e]);
             }
           } else if (pairs) {
             if (turn_a) {

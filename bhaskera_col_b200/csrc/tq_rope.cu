@@ -170,7 +170,10 @@ __device__ __forceinline__ void load_weights(float (&w)[P], const HeadXform& f, 
 
 // D = 2 P LV values per vector.  Groups of LV lanes; a group's unit is (token,
 // run of kHeads heads of q or k).
-// AXES: several position axes.
+// AXES: several position axes.  The CTA's tokens are few: their angles' cosines and sines
+// are picked pair by pair into shared memory once, while the heads are on their way
+// (16,381 tokens of 48 heads, normed, axes' pairs in turn: 102 us; with each group reading
+// the table's rows by itself 112, at two CTAs an SM 123).
 template <int DT, int LV, bool PAIRS, bool AXES>
 __global__ void __launch_bounds__(kRowThreads, 3) rope_rows_kernel(RopeParams p, int runs_q, int runs) {
   using X = Piece<DT>;
@@ -178,11 +181,12 @@ __global__ void __launch_bounds__(kRowThreads, 3) rope_rows_kernel(RopeParams p,
   const int l = threadIdx.x % LV;
   const uint32_t unit = blockIdx.x * (uint32_t)(kRowThreads / LV) + threadIdx.x / LV;
   const uint32_t tok = unit / (uint32_t)runs;
-  if (tok >= (uint32_t)(p.B * p.T)) return;                // whole groups leave together
+  const bool live = tok < (uint32_t)(p.B * p.T);           // for whole groups
+  if (!AXES && !live) return;
   const int run = (int)(unit - tok * (uint32_t)runs), w = run >= runs_q;
   const RopeSide& s = p.side[w];
   const int h0 = (w ? run - runs_q : run) * kHeads;
-  const int nh = tmin(kHeads, (int)s.H - h0);
+  const int nh = live ? tmin(kHeads, (int)s.H - h0) : 0;
   const uint32_t b = tok / (uint32_t)p.T, t = tok - b * (uint32_t)p.T;
   // the two pieces: rotation partners, or halves of the vector
   const int half = s.f.rot / 2;
@@ -221,13 +225,41 @@ __global__ void __launch_bounds__(kRowThreads, 3) rope_rows_kernel(RopeParams p,
     const float* tab = s.f.cos_sin;
     const int64_t at = b * p.ps[0] + t * p.ps[1];
     if (!AXES && tab) tab += table_row(s.f, load_pos(p.pos, p.pos64, at), p.status) * s.f.rot;
-    auto row_of = [&](int a) {
-      return table_row(s.f, load_pos(p.pos, p.pos64, at + a * s.f.axes.stride), p.status);
-    };
+    // units of a CTA are those of at most that many tokens
+    constexpr int kTokens = kRowThreads / LV + 1;
+    __shared__ float4 own[AXES ? kTokens * D / 4 : 1];
+    if constexpr (AXES) {
+      const HeadXform& f = p.side[runs_q ? 0 : 1].f;       // the rotation is both sides'
+      float* row = reinterpret_cast<float*>(own);
+      const uint32_t tok0 = blockIdx.x * (uint32_t)(kRowThreads / LV) / (uint32_t)runs;
+      const uint32_t last = (blockIdx.x + 1) * (uint32_t)(kRowThreads / LV) - 1;
+      const uint32_t end = tmin(last / (uint32_t)runs + 1, (uint32_t)(p.B * p.T));
+      for (uint32_t i = threadIdx.x; i < (end - tok0) * (uint32_t)half; i += kRowThreads) {
+        const uint32_t n = i / (uint32_t)half, pair = i - n * (uint32_t)half, tk = tok0 + n;
+        const uint32_t tb = tk / (uint32_t)p.T;
+        const int64_t where = tb * p.ps[0] + (tk - tb * (uint32_t)p.T) * p.ps[1] + f.axes.axis(pair) * f.axes.stride;
+        const float* src = f.cos_sin + table_row(f, load_pos(p.pos, p.pos64, where), p.status) * f.rot + pair;
+        row[n * f.rot + pair] = __ldg(src);
+        row[n * f.rot + half + pair] = __ldg(src + half);
+      }
+      __syncthreads();
+      if (!live) return;
+      tab = row + (tok - tok0) * f.rot;
+    }
     if (PAIRS) {
       if (turn_a) {
-        if constexpr (AXES) load_axes<P>(cs, sn, s.f, ga, row_of);
-        else { load_f32<P>(cs, tab + ga); load_f32<P>(sn, tab + half + ga); }
+        if constexpr (AXES) {
+#pragma unroll
+          for (int e = 0; e < P; e += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(tab + ga + e);
+            const float4 y = *reinterpret_cast<const float4*>(tab + half + ga + e);
+            cs[e] = x.x; cs[e + 1] = x.y; cs[e + 2] = x.z; cs[e + 3] = x.w;
+            sn[e] = y.x; sn[e + 1] = y.y; sn[e + 2] = y.z; sn[e + 3] = y.w;
+          }
+        } else {
+          load_f32<P>(cs, tab + ga);
+          load_f32<P>(sn, tab + half + ga);
+        }
       }
 #pragma unroll
       for (int e = 0; e < P; e += 2) {
@@ -239,17 +271,13 @@ __global__ void __launch_bounds__(kRowThreads, 3) rope_rows_kernel(RopeParams p,
         E[e / 2] = tc::f2_make(wa[e] * s0, wa[e + 1] * s1);
       }
     } else {
-      float ac[P / 2], as[P / 2], bc[P / 2], bs[P / 2];
-      if constexpr (AXES) {
-        if (turn_a) load_axes<P / 2>(ac, as, s.f, ga / 2, row_of);
-        if (turn_b) load_axes<P / 2>(bc, bs, s.f, gb / 2, row_of);
-      }
+      auto angle = [](const float* x) { return AXES ? *x : __ldg(x); };
 #pragma unroll
       for (int i = 0; i < P / 2; ++i) {
-        const float ca = !turn_a ? 1.f : AXES ? ac[i] : __ldg(tab + ga / 2 + i);
-        const float sa = !turn_a ? 0.f : AXES ? as[i] : __ldg(tab + half + ga / 2 + i);
-        const float cb = !turn_b ? 1.f : AXES ? bc[i] : __ldg(tab + gb / 2 + i);
-        const float sb = !turn_b ? 0.f : AXES ? bs[i] : __ldg(tab + half + gb / 2 + i);
+        const float ca = turn_a ? angle(tab + ga / 2 + i) : 1.f;
+        const float sa = turn_a ? angle(tab + half + ga / 2 + i) : 0.f;
+        const float cb = turn_b ? angle(tab + gb / 2 + i) : 1.f;
+        const float sb = turn_b ? angle(tab + half + gb / 2 + i) : 0.f;
         A[i] = tc::f2_make(wa[2 * i] * ca, wa[2 * i + 1] * ca);
         B[i] = tc::f2_make(-wa[2 * i + 1] * sa, wa[2 * i] * sa);
         C[i] = tc::f2_make(wb[2 * i] * cb, wb[2 * i + 1] * cb);

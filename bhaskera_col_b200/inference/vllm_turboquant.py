@@ -16,10 +16,11 @@ computes the attention from those pages with the fused kernels:
 * prefill and chunked-prefill requests append their new tokens at position
   seq_len - query_len and run the prefill attention over the packed context;
 * a model that hands over its heads before their norms and rotation
-  (``forward(..., rope=...)``) runs every batch, whatever its mix, as three
+  (``forward(..., rope=...)``) or attends differentially (``forward(...,
+  pair=...)``) runs every batch, whatever its mix, as three
   calls without host synchronisation: ops.qk_rope on the queries,
   ops.append_ragged (keys normed and rotated on the way into their pages) and
-  ops.attend_ragged.
+  ops.attend_ragged or ops.diff_attend_ragged.
 
 The compressor is the reference's vLLM one (vllm_turboquant.py:170-230): the
 MSE codebooks without the QJL sketch, rotation seed 42 + 13 * layer
@@ -37,7 +38,7 @@ from __future__ import annotations
 
 import logging
 import re
-from dataclasses import dataclass
+from dataclasses import dataclass, replace
 from typing import Dict, List, Optional
 
 import torch
@@ -194,20 +195,31 @@ class TurboQuantPagedAttention:
                 stream_table: Optional[torch.Tensor] = None,
                 rope: Optional[ops.RopeTable] = None, q_norm: Optional[ops.HeadNorm] = None,
                 k_norm: Optional[ops.HeadNorm] = None,
-                positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+                positions: Optional[torch.Tensor] = None,
+                pair: Optional[ops.DiffHeads] = None) -> torch.Tensor:
         """query (N, Hq, D), key / value (N, Hkv, D) in vLLM's flattened token
         order; stores the tokens, returns the (N, Hq, D) attention output.
 
         With ``rope`` (and / or the head norms) query and key come as they
         leave their projections: they are normed and rotated here, by each
-        token's position in its request or by ``positions`` (N,), and the
-        whole batch runs as three calls."""
-        if out is None:
+        token's position in its request or by ``positions`` (N,) ((axes, N) for
+        a rope with axes), and the whole batch runs as three calls.
+
+        With ``pair`` the query heads are attended in pairs, as the difference
+        of two softmax maps (ops.diff_attend_ragged), and the output is (N, Hq /
+        2, 2D), or (N, Hq / 2, D) with shared keys."""
+        if out is None and pair is not None:
+            n, h, d = query.shape
+            out = torch.empty((n, h // 2, 2 * d if pair.keys == "own" else d), dtype=query.dtype,
+                              device=query.device)
+        elif out is None:
             out = torch.empty_like(query)
         st = stream_table if stream_table is not None else self.stream_table(batch.block_table)
-        if rope is not None or q_norm is not None or k_norm is not None:
+        if rope is not None or q_norm is not None or k_norm is not None or pair is not None:
+            if rope is None and positions is not None:
+                raise ValueError("positions come with rope")
             return self._forward_ragged(query, key, value, batch, out, st, rope, q_norm, k_norm,
-                                        positions)
+                                        positions, pair)
         if positions is not None:
             raise ValueError("positions come with rope")
         H = self.num_kv_heads
@@ -247,7 +259,8 @@ class TurboQuantPagedAttention:
                                   out=out[qs:qe].permute(1, 0, 2).unsqueeze(0))
         return out
 
-    def _forward_ragged(self, query, key, value, batch, out, st, rope, q_norm, k_norm, positions):
+    def _forward_ragged(self, query, key, value, batch, out, st, rope, q_norm, k_norm, positions,
+                        pair):
         n = batch.num_actual_tokens
         rb, pages = batch.ragged(), self.paged(st)
         self.tokens_stored += n
@@ -255,11 +268,17 @@ class TurboQuantPagedAttention:
             self.decode_tokens += n
         q = query[:n]
         if rope is not None or q_norm is not None:
-            at = positions[:n] if positions is not None else \
+            at = positions[..., :n] if positions is not None else \
                 (batch.positions() if rope is not None else None)
             q, _ = ops.qk_rope(q, None, rope, at, q_norm=q_norm)
         ops.append_ragged(self.tables, pages, key[:n], value[:n], rb, rope=rope, k_norm=k_norm,
-                          positions=positions[:n] if positions is not None else None)
+                          positions=positions[..., :n] if positions is not None else None)
+        if pair is not None:
+            if pair.lam.dim() == 2 and pair.lam.shape[0] != n:
+                pair = replace(pair, lam=pair.lam[:n])
+            ops.diff_attend_ragged(self.tables, pages, q, rb, pair, scale=self.scale, out=out[:n],
+                                   workspace=self.ragged_workspace)
+            return out
         ops.attend_ragged(self.tables, pages, q, rb, scale=self.scale, out=out[:n],
                           workspace=self.ragged_workspace)
         return out

@@ -367,3 +367,79 @@ def test_layer_runs_together():
     ye, de, he, dhe = L.residual_norm(o.flatten(1) @ back, mid, post,
                                       torch.full((C,), 0.3, dtype=BF16), "sigmoid", 1.0, pre)
     assert (np.abs(L.arr(h2) - he) <= dhe * (1 + 2.0 ** -8) + S.half_ulp(BF16) * np.abs(he)).all()
+
+
+@pytest.mark.parametrize("keys", ["own", "shared"])
+def test_paged_attention_layer_with_axes_and_pairs(keys):
+    """TurboQuantPagedAttention.forward with positions of three axes and differential heads over a served
+    schedule, rows behind the batch: what the operators give for the same pages."""
+    from bhaskera_col_b200.inference.vllm_turboquant import TurboQuantPagedAttention, VLLMBatch
+    D, Hq, H = 128, 8, 2
+    layer = TurboQuantPagedAttention(3, 32, Hq, H, D, num_blocks=12, block_size=64, device=DEV)
+    axes = ops.RopeTable.axis_of_pairs((24, 20, 20), True)
+    rope = ops.RopeTable.build(D, 500, device=DEV, axes=axes)
+    qn, kn = (ops.HeadNorm(1 + 0.1 * randn((D,), i, F32)) for i in range(2))
+    bt = torch.randperm(12, generator=torch.Generator().manual_seed(2))[:8].view(2, 4).to(torch.int32).to(DEV)
+    length = [0, 0]
+    for i, new in enumerate(([130, 5], [1, 1], [3, 100])):
+        length = [a + b for a, b in zip(length, new)]
+        start, N = [0, new[0], sum(new)], sum(new)
+        batch = VLLMBatch(torch.tensor(start, dtype=torch.int32, device=DEV),
+                          torch.tensor(length, dtype=torch.int32, device=DEV), bt, N, max(new))
+        q, k, v = (randn((N + 2, h, D), 10 * i + j) for j, h in enumerate((Hq, H, H)))
+        pos = torch.randint(0, 500, (3, N + 2), generator=torch.Generator().manual_seed(i)).to(DEV)
+        pair = make_pair(N + 2, Hq // 2, 2 * D if keys == "own" else D, i, keys, "adjacent", rows=True)
+        out = layer.forward(q, k, v, batch, rope=rope, q_norm=qn, k_norm=kn, positions=pos, pair=pair)
+        pages = layer.paged(layer.stream_table(bt))
+        req, at = S.positions(start, length, N)
+        kx = L.rope_axes(k[:N], rope.cos_sin, pos[:, :N].cpu().numpy(), axes, False, kn.weight, 1e-6)
+        from test_gpu_serving_ops import check_stored
+        check_stored(layer.tables, pages, k[:N], v[:N], start, length, 2, H, kx)
+        qr, _ = ops.qk_rope(q[:N], None, rope, pos[:, :N], q_norm=qn)
+        short = ops.DiffHeads(pair.lam[:N], keys, "adjacent", pair.norm, pair.out_scale)
+        want = ops.diff_attend_ragged(layer.tables, pages, qr, batch.ragged(), short, scale=layer.scale)
+        assert torch.equal(out[:N], want) and ok_status() == 0
+        check_diff(want, want_diff(layer.tables, pages, qr, short, start, length, True, H, layer.scale), False)
+    with pytest.raises(ValueError, match="rope"):
+        layer.forward(q, k, v, batch, positions=pos, pair=pair)
+
+
+def test_cache_with_axes_matches_rotated_heads():
+    """TurboQuantKVCache.prefill / decode with a rope of several axes: positions (axes, B, T)."""
+    from bhaskera_col_b200.inference import TurboQuantKVCache
+    B, Hq, H, D = 2, 4, 2, 128
+    rope = ops.RopeTable.build(D, 500, device=DEV, axes=ops.RopeTable.axis_of_pairs((16, 24, 24)))
+    a, b = (TurboQuantKVCache(1, B, H, D, residual_window=0, protected_layers=0, device=DEV, max_seq_len=128)
+            for _ in range(2))
+    for i, n in enumerate((37, 1)):
+        q, k, v = (randn((B, h, n, D), 5 * i + j) for j, h in enumerate((Hq, H, H)))
+        pos = torch.randint(0, 500, (3, B, n), generator=torch.Generator().manual_seed(i)).to(DEV)
+        call = (a.prefill, b.prefill) if n > 1 else (a.decode, b.decode)
+        qr, kr = ops.qk_rope(q, k, rope, pos)
+        assert torch.equal(call[0](q, k, v, 0, rope=rope, positions=pos), call[1](qr, kr, v, 0))
+    assert torch.equal(a._stores[0]._pages, b._stores[0]._pages) and ok_status() == 0
+
+
+def test_inputs_of_a_backward_pass_and_mixed_devices_are_refused():
+    tables, batch, start, seq, pages, pair = setup_case([(3, 3)])
+    q = randn((3, 8, 128), 1)
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        ops.diff_attend_ragged(tables, pages, q.float().requires_grad_(), batch, pair)
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        ops.diff_attend_ragged(tables, pages, q, batch, ops.DiffHeads(pair.lam.clone().requires_grad_()))
+    with pytest.raises(ValueError, match="tensors on"):
+        ops.diff_attend_ragged(tables, pages, q, batch, ops.DiffHeads(pair.lam.cpu()))
+    with pytest.raises(ValueError, match="lam must be"):
+        ops.diff_attend_ragged(tables, pages, q, batch, ops.DiffHeads(torch.ones(3, device=DEV)))
+    with pytest.raises(ValueError, match="weights"):
+        ops.diff_attend_ragged(tables, pages, q, batch,
+                               ops.DiffHeads(pair.lam, norm=ops.HeadNorm(torch.ones(128, device=DEV))))
+    x = randn((3, 64), 2, F32)
+    for kw in (dict(residual=x.clone().requires_grad_()), dict(gate=x.clone().requires_grad_()),
+               dict(pre_norm=ops.RowNorm(torch.ones(64, device=DEV, requires_grad=True)))):
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            ops.residual_norm(x, **{"residual": x.clone(), **kw})
+    with pytest.raises(ValueError, match="tensors on"):
+        ops.residual_norm(x, x.clone(), gate=torch.ones(64))
+    with pytest.raises(ValueError, match="values for rows"):
+        ops.residual_norm(x, x.clone(), post_norm=ops.RowNorm(torch.ones(32, device=DEV)))
