@@ -5,9 +5,11 @@
 // mean taken off only where the norm is centred (layer norm; else RMS norm).
 //
 // Bound by HBM: x, residual and a gate of its own per element are read once, y and h
-// written once.  T threads hold a row in registers, 8 VPT values each, so that the
-// sums of both norms need no second read; h is formed from y before its rounding.
-// Sums go by shuffles and one barrier each, always in the same order.
+// written once; in fact by instructions beside it (issue slots 72 % busy).  16,381 rows
+// of 4,096 (bf16, channel gate) 117 us for 537 MB, 4.6 TB/s; 16 rows of 5,120 3.8 us on
+// the GPU; 2,051 rows of 2,050 (4-byte chunks, gate per element, layer norms) 33 us.  Sums go by
+// shuffles and one barrier each, always in the same order; h is formed from y before its
+// rounding.
 #include "tq_common.cuh"
 #include "tq_internal.h"
 #include "tq_tc.cuh"
@@ -70,6 +72,17 @@ struct Chunk {
       const uint32_t u = V == 1 ? (uint32_t)w[0] : (uint32_t)w[e / 2] >> (16 * (e & 1));
       if constexpr (DT == TQ_BF16) return __uint_as_float(u << 16);
       else return __half2float(__ushort_as_half((unsigned short)u));
+    }
+  }
+  // values e, e + 1 (e even)
+  __device__ __forceinline__ tc::f2 pair(int e) const {
+    if constexpr (DT == TQ_F32) return tc::f2_make(__uint_as_float(w[e]), __uint_as_float(w[e + 1]));
+    else if constexpr (DT == TQ_BF16)
+      return tc::f2_make(__uint_as_float((uint32_t)w[e / 2] << 16), __uint_as_float(w[e / 2] & 0xFFFF0000u));
+    else {
+      const uint32_t u = w[e / 2];
+      const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&u));
+      return tc::f2_make(h.x, h.y);
     }
   }
   static __device__ __forceinline__ void store(void* base, int64_t i, const float* v) {
@@ -144,13 +157,14 @@ __device__ __forceinline__ float activate(float g, int act) {
 __device__ __forceinline__ float row_sum(float x, int T, float (*part)[32], int& turn) {
   x = warp_sum(x);
   if (T == 32) return x;
-  const int warps = T / 32;
-  if ((threadIdx.x & 31) == 0) part[turn][threadIdx.x >> 5] = x;
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) part[turn][threadIdx.x >> 5] = x;
   __syncthreads();
-  float s = 0.f;
-  for (int i = 0; i < warps; ++i) s += part[turn][i];
+  // a partial sum a lane: read one after the other by every thread, 16 of them were half of a
+  // row's instructions
+  x = warp_sum(lane < T / 32 ? part[turn][lane] : 0.f);
   turn ^= 1;
-  return s;
+  return x;
 }
 
 // Offset of a row.
@@ -166,11 +180,14 @@ using tc::f2;
 // (a warp, or the CTA) take row after row, 8 values each, with what a column needs in
 // registers in 32 bits, gate and scale folded in:
 //   y = residual + (x r) A + B,   h = (y r') C + D
-// and the next two rows' values on their way.  GE: a gate per element, BIAS: B and D.  The
+// and the next rows' values on their way: two with chunks of 8 (16,381 rows of 4,096: one
+// 144 us, two 117), one with chunks of 2, whose registers leave less room (2,051 rows of
+// 2,050: 33 us, 41).  GE: a gate per element, BIAS: B and D.  The
 // arithmetic, on fp32 pairs, is 6 instructions a value without a gate per element.
 template <int XT, int RT, int V, bool GE, bool BIAS, int MAXT>
 __global__ void __launch_bounds__(MAXT) residual_norm_rows_kernel(NormParams p, int T) {
   constexpr int NK = 8 / V, NP = 4;                        // chunks and pairs of a thread
+  constexpr bool TWO = V == 8;                             // rows on their way
   __shared__ float part[2][32];
   int turn = 0;
   const int t = threadIdx.x % T;
@@ -203,7 +220,7 @@ __global__ void __launch_bounds__(MAXT) residual_norm_rows_kernel(NormParams p, 
   };
   Raw cur, nxt;
   fetch(cur, row);
-  if (rows - row > step) fetch(nxt, row + step);
+  if (TWO && rows - row > step) fetch(nxt, row + step);
   // a column's factors
   f2 A[NP], B[BIAS ? NP : 1], C[NP], D[BIAS ? NP : 1];
 #pragma unroll
@@ -254,12 +271,16 @@ __global__ void __launch_bounds__(MAXT) residual_norm_rows_kernel(NormParams p, 
   };
   for (;;) {
     Raw far;
-    if (rows - row > 2 * (uint64_t)step) fetch(far, row + 2 * step);
+    if (TWO) {
+      if (rows - row > 2 * (uint64_t)step) fetch(far, row + 2 * step);
+    } else if (rows - row > step) {
+      fetch(nxt, row + step);
+    }
     f2 v[NP];
 #pragma unroll
     for (int k = 0; k < NK; ++k)
 #pragma unroll
-      for (int e = 0; e < V; e += 2) v[(k * V + e) / 2] = tc::f2_make(cur.x[k].get(e), cur.x[k].get(e + 1));
+      for (int e = 0; e < V; e += 2) v[(k * V + e) / 2] = cur.x[k].pair(e);
     // takes the mean off (where the norm does) and returns the factor
     auto norm = [&](const NormSide& n) {
       if (n.centered) {
@@ -291,7 +312,7 @@ __global__ void __launch_bounds__(MAXT) residual_norm_rows_kernel(NormParams p, 
 #pragma unroll
       for (int e = 0; e < V; e += 2) {
         const int i = (k * V + e) / 2;
-        const f2 res = tc::f2_make(cur.r[k].get(e), cur.r[k].get(e + 1));
+        const f2 res = cur.r[k].pair(e);
         f2 z = tc::f2_mul(v[i], rr);
         if (GE || p.gmode == 2) {
           f2 f = tc::f2_make(one, one);
@@ -340,14 +361,14 @@ __global__ void __launch_bounds__(MAXT) residual_norm_rows_kernel(NormParams p, 
     if (rows - row <= step) return;
     row += step;
     cur = nxt;
-    nxt = far;
+    if (TWO) nxt = far;
   }
 }
 
 using NormFn = void (*)(NormParams, int);
 
-// Where the plain form's registers would halve the CTAs of an SM, 64; else what up to 384
-// threads may have: gates and biases then go without spills.
+// Up to 384 threads have registers for gates and biases without spills above,
+// 64 each.
 template <int XT, int RT, int V>
 NormFn rows_fn(bool ge, bool bias, bool wide) {
 #define TQ_ROWS(GE, BIAS) \
@@ -568,15 +589,14 @@ int launch_residual_norm(const tq_residual_norm_args* a, cudaStream_t st) {
     fn<<<(unsigned)grid, T * per, 0, st>>>(p, T);
     return check_launch("tq_residual_norm");
   }
-  // Threads of a row and their values, 8 vpt each: 32 of them leave most rows in flight on
-  // an SM, 8 end a call of few rows sooner; 64 only where 512 threads need them.
+  // Threads of a row and their values, 8 vpt each, by the width alone: a row's sums do not
+  // depend on how many rows come with it.
   int vpt, T;
   if (units <= 128) {
     T = 32;
     vpt = units <= 32 ? 1 : units <= 64 ? 2 : 4;
   } else {
-    const bool few = p.rows <= 2 * device_sm_count();
-    vpt = units <= 1024 && few ? 1 : units <= 1024 ? 2 : units <= 2048 ? 4 : 8;
+    vpt = units <= 1024 ? 1 : units <= 2048 ? 4 : 8;
     T = ((units + vpt - 1) / vpt + 31) & ~31;
   }
   const NormFn fn = x->dtype == TQ_F32   ? norm_fn_x<TQ_F32>(r->dtype, vpt, v)

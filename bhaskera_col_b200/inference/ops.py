@@ -958,8 +958,8 @@ def diff_attend_ragged(tables: LayerTables, pages, q: torch.Tensor, batch: Ragge
     layer's v of (N, Hkv / 2, 2D) is appended as (N, Hkv, D)), (N, H, D) with
     shared ones.
 
-    Rows, masks, lengths, empty rows, ``scale``, ``causal``, ``engine`` and
-    ``workspace`` are those of attend_ragged; so are the errors of both maps'
+    Rows, masks, lengths, empty rows, ``scale``, ``causal``, ``engine`` (own keys
+    have no tcgen05 kernel: not 2) and ``workspace`` are those of attend_ragged; so are the errors of both maps'
     results, of which the difference is taken in fp32: where the maps nearly
     cancel, an fp32 ``out`` (operands of 22 bits) keeps what is left."""
     norm = pair.norm

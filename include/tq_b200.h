@@ -514,7 +514,8 @@ typedef struct tq_diff_args {
   tq_ragged batch;
   float scale;                /* softmax scale                                */
   int32_t causal;
-  int32_t engine;             /* as in tq_attend_args                         */
+  int32_t engine;             /* as in tq_attend_args; own keys have no tcgen05
+                                 kernel (2), 3 holds both maps' rows          */
   int32_t shared_keys;
   int32_t halves;
   const float* lambda;        /* device; fp32, lambda of row n, head h at
