@@ -316,3 +316,19 @@ def test_residual_norm_captured_and_on_another_stream():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("n,C", [(20011, 64), (2003, 1026), (1201, 4096), (601, 8192)])
+@pytest.mark.parametrize("gate", [None, "full"])
+def test_residual_norm_in_place_over_many_rows(n, C, gate):
+    """Rows that are on their way while earlier ones are written over: the same bits as into
+    other memory, and the first and last rows those of a call of their own."""
+    post, pre = row_norm(C, 1, BF16, "rms"), row_norm(C, 2, BF16, "layer")
+    x, res = randn((n, C), 3), randn((n, C), 4, F32)
+    g = randn((n, C), 5) if gate else None
+    y, h = ops.residual_norm(x, res, post, g, "none", 1.0, pre)
+    for at in (slice(0, 3), slice(n - 3, n)):
+        a, b = run_norm(x[at], res[at], post, g if g is None else g[at], "none", 1.0, pre)
+        assert torch.equal(a, y[at]) and torch.equal(b, h[at])
+    ops.residual_norm(x, res, post, g, "none", 1.0, pre, residual_out=res, out=x)
+    assert torch.equal(res, y) and torch.equal(x, h)
