@@ -145,9 +145,8 @@ __device__ __forceinline__ void load_param(float (&v)[V], const void* base, int 
 __device__ __forceinline__ float activate(float g, int act) {
   if (act == TQ_GATE_SIGMOID) {
     const float x = fminf(fmaxf(-g, -126.f), 126.f);       // (a NaN gate is let through below)
-    const float t = x * 1.44269504f, d = fmaf(x, 1.44269504f, -t) + x * 1.92596299e-8f;
-    const float e = fast_exp2(t) * fmaf(d, 0.693147181f, 1.f);
-    return g != g ? g : __fdividef(1.f, 1.f + e);
+    const float t = __fmul_rn(x, 1.44269504f), d = fmaf(x, 1.92596299e-8f, fmaf(x, 1.44269504f, -t));
+    return g != g ? g : __fdividef(1.f, fmaf(fast_exp2(t), fmaf(d, 0.693147181f, 1.f), 1.f));
   }
   return act == TQ_GATE_TANH ? tanhf(g) : g;
 }
@@ -180,10 +179,13 @@ using tc::f2;
 // (a warp, or the CTA) take row after row, 8 values each, with what a column needs in
 // registers in 32 bits, gate and scale folded in:
 //   y = residual + (x r) A + B,   h = (y r') C + D
-// and the next rows' values on their way: two with chunks of 8 (16,381 rows of 4,096: one
+// (A = (w + offset) F, B = b F, F = scale act(gate); with a gate per element the products
+// with F are made where it is used, to the same bits: a row alone, whose gate is either, is the
+// row of a batch) and the next rows' values on their way: two with chunks of 8 (16,381 rows of 4,096: one
 // 144 us, two 117), one with chunks of 2, whose registers leave less room (2,051 rows of
 // 2,050: 33 us, 41).  GE: a gate per element, BIAS: B and D.  The
 // arithmetic, on fp32 pairs, is 6 instructions a value without a gate per element.
+// residual_norm_kernel below goes through the same roundings.
 template <int XT, int RT, int V, bool GE, bool BIAS, int MAXT>
 __global__ void __launch_bounds__(MAXT) residual_norm_rows_kernel(NormParams p, int T) {
   constexpr int NK = 8 / V, NP = 4;                        // chunks and pairs of a thread
@@ -246,7 +248,7 @@ __global__ void __launch_bounds__(MAXT) residual_norm_rows_kernel(NormParams p, 
       if (channel) load_param<V>(g, p.g, p.gd, col(k));
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float f = p.scale * (channel ? activate(g[e], p.act) : 1.f);
+        const float f = GE ? 1.f : p.scale * (channel ? activate(g[e], p.act) : 1.f);
         a[e] *= f;
         b[e] *= f;
       }
@@ -314,22 +316,27 @@ __global__ void __launch_bounds__(MAXT) residual_norm_rows_kernel(NormParams p, 
         const int i = (k * V + e) / 2;
         const f2 res = cur.r[k].pair(e);
         f2 z = tc::f2_mul(v[i], rr);
-        if (GE || p.gmode == 2) {
-          f2 f = tc::f2_make(one, one);
-          if constexpr (GE) {
-            const uint32_t u = cur.g[k][e / 2];
-            float lo, hi;
-            if (p.gd == TQ_F16) {
-              const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&u));
-              lo = h.x; hi = h.y;
-            } else {
-              lo = __uint_as_float(u << 16);
-              hi = __uint_as_float(u & 0xFFFF0000u);
-            }
-            f = tc::f2_make(activate(lo, p.act), activate(hi, p.act));
+        if constexpr (GE) {
+          const uint32_t u = cur.g[k][e / 2];
+          float lo, hi;
+          if (p.gd == TQ_F16) {
+            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&u));
+            lo = h.x; hi = h.y;
+          } else {
+            lo = __uint_as_float(u << 16);
+            hi = __uint_as_float(u & 0xFFFF0000u);
           }
+          const f2 f = tc::f2_mul(tc::f2_make(p.scale, p.scale),
+                                  tc::f2_make(activate(lo, p.act), activate(hi, p.act)));
+          if constexpr (BIAS) {
+            z = tc::f2_fma(z, tc::f2_mul(A[i], f), tc::f2_mul(B[i], f));
+            v[i] = tc::f2_fma(z, tc::f2_make(1.f, 1.f), res);
+          } else {
+            v[i] = tc::f2_fma(z, tc::f2_mul(A[i], f), res);
+          }
+        } else if (p.gmode == 2) {
           z = BIAS ? tc::f2_fma(z, A[i], B[i]) : tc::f2_mul(z, A[i]);
-          v[i] = tc::f2_fma(z, f, res);
+          v[i] = tc::f2_fma(z, tc::f2_make(one, one), res);
         } else if constexpr (BIAS) {
           const f2 zb = tc::f2_fma(z, A[i], B[i]);
           v[i] = tc::f2_fma(zb, tc::f2_make(1.f, 1.f), res);
@@ -389,7 +396,10 @@ NormFn rows_fn_x(int rd, int v, bool ge, bool bias, bool wide) {
 }
 
 // Everything else: T threads per row (a warp, or the CTA), 8 VPT values each in chunks of V
-// neighbours.  V = 1 takes any stride.
+// neighbours.  V = 1 takes any stride.  Sums and products go in the order of the kernel above,
+// even and odd values by themselves, and no product joins a sum but by fmaf: a gate of 32 bits
+// per element (whose rows on their way the registers above have no room for) gives the bits
+// that a gate of the channels gives there.
 template <int XT, int RT, int VPT, int V>
 __global__ void __launch_bounds__(VPT == 1 ? 1024 : 512) residual_norm_kernel(NormParams p, int T) {
   constexpr int NK = 8 * VPT / V;                          // chunks of a thread
@@ -415,75 +425,97 @@ __global__ void __launch_bounds__(VPT == 1 ? 1024 : 512) residual_norm_kernel(No
       rr[k].load(p.r, rb + place(p.rs, k));
     }
   }
+  // a gate per element, on its way beside them where there are registers
+  constexpr bool EARLY = VPT == 1;
+  const int64_t gb = p.gmode ? at(p.gs) : 0;
+  float early[EARLY ? NK : 1][V];
+  if (EARLY && p.gmode == 1)
+#pragma unroll
+    for (int k = 0; k < NK; ++k)
+      if (inside(k)) load_param<V>(early[k], p.g, p.gd, gb + place(p.gs, k));
   float v[NK][V];
 #pragma unroll
   for (int k = 0; k < NK; ++k)
 #pragma unroll
     for (int e = 0; e < V; ++e) v[k][e] = xr[k].get(e);
   const float inv_c = 1.f / (float)p.C;
+  auto val = [&](int i) -> float& { return v[i / V][i % V]; };
+  // takes the mean off (where the norm does) and returns the factor
   auto norm = [&](const NormSide& s) {
     if (s.centered) {
-      float sum = 0.f;
+      float lo = val(0), hi = val(1);
 #pragma unroll
-      for (int k = 0; k < NK; ++k)
-#pragma unroll
-        for (int e = 0; e < V; ++e) sum += v[k][e];
-      const float mean = row_sum(sum, T, part, turn) * inv_c;
+      for (int i = 2; i < 8 * VPT; i += 2) {
+        lo = __fadd_rn(lo, val(i));
+        hi = __fadd_rn(hi, val(i + 1));
+      }
+      const float mean = __fmul_rn(row_sum(__fadd_rn(lo, hi), T, part, turn), inv_c);
 #pragma unroll
       for (int k = 0; k < NK; ++k)
         if (inside(k))
 #pragma unroll
-          for (int e = 0; e < V; ++e) v[k][e] -= mean;
+          for (int e = 0; e < V; ++e) v[k][e] = __fsub_rn(v[k][e], mean);
     }
-    float ss = 0.f;
+    float lo = __fmul_rn(val(0), val(0)), hi = __fmul_rn(val(1), val(1));
 #pragma unroll
-    for (int k = 0; k < NK; ++k)
-#pragma unroll
-      for (int e = 0; e < V; ++e) ss = fmaf(v[k][e], v[k][e], ss);
-    const float r = 1.f / sqrtf(fmaf(row_sum(ss, T, part, turn), inv_c, s.eps));
-#pragma unroll
-    for (int k = 0; k < NK; ++k) {
-      if (!inside(k)) continue;
-      float w[V], b[V];
-      if (s.w) load_param<V>(w, s.w, s.dtype, col(k));
-      if (s.b) load_param<V>(b, s.b, s.dtype, col(k));
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        v[k][e] = v[k][e] * r * (s.w ? w[e] + s.offset : 1.f);
-        if (s.b) v[k][e] += b[e];
-      }
+    for (int i = 2; i < 8 * VPT; i += 2) {
+      lo = fmaf(val(i), val(i), lo);
+      hi = fmaf(val(i + 1), val(i + 1), hi);
     }
+    return 1.f / sqrtf(fmaf(row_sum(__fadd_rn(lo, hi), T, part, turn), inv_c, s.eps));
   };
-  if (p.post.on) norm(p.post);
-  const int64_t gb = p.gmode ? at(p.gs) : 0;
-  float one = p.scale;
-  if (p.gmode == 2) one *= activate(load_elem(p.g, p.gd, gb), p.act);
+  // weights and biases of chunk k
+  auto params = [&](const NormSide& s, int k, float (&w)[V], float (&b)[V]) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) { w[e] = 1.f; b[e] = 0.f; }
+    if (s.w) {
+      load_param<V>(w, s.w, s.dtype, col(k));
+#pragma unroll
+      for (int e = 0; e < V; ++e) w[e] += s.offset;
+    }
+    if (s.b) load_param<V>(b, s.b, s.dtype, col(k));
+  };
+  const bool bias = p.post.b || p.pre.b;
+  const float r1 = p.post.on ? norm(p.post) : 1.f;
+  const float one = p.gmode == 2 ? p.scale * activate(load_elem(p.g, p.gd, gb), p.act) : p.scale;
   const int64_t yb = at(p.ys);
 #pragma unroll
   for (int k = 0; k < NK; ++k) {
     if (!inside(k)) continue;
-    float g[V];
-    if (p.gmode == 1) load_param<V>(g, p.g, p.gd, gb + place(p.gs, k));
+    float g[V], w[V], b[V];
+    params(p.post, k, w, b);
+    if (!EARLY && p.gmode == 1) load_param<V>(g, p.g, p.gd, gb + place(p.gs, k));
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const float f = p.gmode == 1 ? one * activate(g[e], p.act) : one;
-      v[k][e] = fmaf(f, v[k][e], rr[k].get(e));
+      const float x = EARLY ? early[EARLY ? k : 0][e] : g[e];
+      const float f = p.gmode == 1 ? __fmul_rn(p.scale, activate(x, p.act)) : one;
+      const float z = __fmul_rn(v[k][e], r1), a = __fmul_rn(w[e], f), res = rr[k].get(e);
+      v[k][e] = bias ? __fadd_rn(fmaf(z, a, __fmul_rn(b[e], f)), res) : fmaf(z, a, res);
     }
     Chunk<RT, V>::store(p.y, yb + place(p.ys, k), v[k]);
   }
   if (!p.h) return;
-  norm(p.pre);
+  const float r2 = norm(p.pre);
   const int64_t hb = at(p.hs);
 #pragma unroll
-  for (int k = 0; k < NK; ++k)
-    if (inside(k)) Chunk<XT, V>::store(p.h, hb + place(p.hs, k), v[k]);
+  for (int k = 0; k < NK; ++k) {
+    if (!inside(k)) continue;
+    float w[V], b[V];
+    params(p.pre, k, w, b);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float z = __fmul_rn(v[k][e], r2);
+      v[k][e] = bias ? fmaf(z, w[e], b[e]) : __fmul_rn(z, w[e]);
+    }
+    Chunk<XT, V>::store(p.h, hb + place(p.hs, k), v[k]);
+  }
 }
 
 template <int XT, int RT>
 NormFn norm_fn(int vpt, int v) {
 #define TQ_NORM(N, V) if (vpt == N && v == V) return residual_norm_kernel<XT, RT, N, V>;
-  TQ_NORM(1, 8) TQ_NORM(2, 8) TQ_NORM(4, 8) TQ_NORM(8, 8)
-  TQ_NORM(1, 2) TQ_NORM(2, 2) TQ_NORM(4, 2) TQ_NORM(8, 2)
+  TQ_NORM(1, 8) TQ_NORM(4, 8) TQ_NORM(8, 8)
+  TQ_NORM(1, 2) TQ_NORM(4, 2) TQ_NORM(8, 2)
   TQ_NORM(1, 1) TQ_NORM(2, 1) TQ_NORM(4, 1) TQ_NORM(8, 1)
 #undef TQ_NORM
   return nullptr;
@@ -508,7 +540,8 @@ NormSide norm_side(const tq_row_norm* n) {
   return s;
 }
 
-// Are rows of the view read and written v neighbours at a time?
+// Are rows of the view read and written v neighbours at a time?  By the strides as they are
+// given, those of single entries too: a row taken out of a batch by slicing goes like the batch.
 bool takes_chunks(const tq_tensor4* x, int v) {
   const int bytes = tmin(16, v * (x->dtype == TQ_F32 ? 4 : 2));
   const int es = x->dtype == TQ_F32 ? 4 : 2;
@@ -516,7 +549,7 @@ bool takes_chunks(const tq_tensor4* x, int v) {
       reinterpret_cast<uintptr_t>(x->data) % bytes)
     return false;
   for (int i = 0; i < 3; ++i)
-    if (x->shape[i] > 1 && (x->stride[i] * es) % bytes) return false;
+    if ((x->stride[i] * es) % bytes) return false;
   return true;
 }
 
@@ -572,7 +605,7 @@ int launch_residual_norm(const tq_residual_norm_args* a, cudaStream_t st) {
     }
   }
   const int units = (p.C + 7) / 8;
-  // a gate that differs from row to row
+  // a gate that differs from row to row (what a single row's gate is, its bits do not say)
   bool per_row = false;
   for (int i = 0; g && i < 3; ++i) per_row = per_row || (g->shape[i] > 1 && g->stride[i] != 0);
   const bool ge = p.gmode == 1 && per_row;
@@ -589,10 +622,13 @@ int launch_residual_norm(const tq_residual_norm_args* a, cudaStream_t st) {
     fn<<<(unsigned)grid, T * per, 0, st>>>(p, T);
     return check_launch("tq_residual_norm");
   }
-  // Threads of a row and their values, 8 vpt each, by the width alone: a row's sums do not
-  // depend on how many rows come with it.
+  // Threads of a row and their values, 8 vpt each, by the width (and chunks, those of the kernel
+  // above) alone: a row's sums do not depend on how many rows come with it.
   int vpt, T;
-  if (units <= 128) {
+  if (v > 1 && units <= 1024) {
+    vpt = 1;
+    T = (units + 31) & ~31;
+  } else if (units <= 128) {
     T = 32;
     vpt = units <= 32 ? 1 : units <= 64 ? 2 : 4;
   } else {

@@ -332,3 +332,37 @@ def test_residual_norm_in_place_over_many_rows(n, C, gate):
         assert torch.equal(a, y[at]) and torch.equal(b, h[at])
     ops.residual_norm(x, res, post, g, "none", 1.0, pre, residual_out=res, out=x)
     assert torch.equal(res, y) and torch.equal(x, h)
+
+
+@pytest.mark.parametrize("kind", ["rms", "layer", "bare"])
+@pytest.mark.parametrize("gdtype", [BF16, F16, F32, None])
+@pytest.mark.parametrize("n,C,extra", [(5, 64, 0), (7, 1024, 0), (3, 1000, 1), (4, 2050, 0), (3, 4096, 0), (3, 4096, 1),
+                                       (3, 4096, 2), (3, 5128, 0), (2, 8192, 0), (3, 8200, 0), (3, 4097, 0), (2, 20000, 0)])
+def test_residual_norm_of_one_row_is_the_row_of_a_batch(n, C, extra, gdtype, kind):
+    """Rows called one by one give the bits that the batch gives, whatever the gate is a row of (a gate of
+    its own per element, the channels', one number) and its type, and for slices of wider buffers."""
+    dtype = F16 if gdtype == F16 else BF16
+    post, pre = row_norm(C, 1, dtype, kind), row_norm(C, 2, F32, kind)
+    x, res = (randn((n, C + extra), i, d)[:, :C] for i, d in ((3, dtype), (4, F32)))
+    gates = [None] if gdtype is None else [2 * randn(s, 5, gdtype) for s in ((n, C), (C,), (1, C), (n, 1), (1,))]
+    for gate in gates:
+        y, h = ops.residual_norm(x, res, post, gate, "sigmoid" if gate is not None else "none", 0.7, pre)
+        for i in range(n):
+            at = slice(i, i + 1)
+            g = gate[at] if gate is not None and gate.shape[0] == n and gate.dim() == 2 else gate
+            a, b = ops.residual_norm(x[at], res[at], post, g, "sigmoid" if g is not None else "none", 0.7, pre)
+            assert torch.equal(a, y[at]) and torch.equal(b, h[at]), (gate is not None and gate.shape, i)
+
+
+def test_residual_norm_of_one_sequence_is_that_of_a_batch():
+    """(B, T, C) with gates (B, 1, C): a sequence by itself, and a token of it."""
+    B, T, C = 3, 4, 1032
+    post, pre = row_norm(C, 1, BF16, "layer"), row_norm(C, 2, F32, "rms")
+    x, res = randn((B, T, C), 3), randn((B, T, C), 4, F32)
+    for gdtype in (BF16, F32):
+        gate = randn((B, 1, C), 5, gdtype)
+        y, h = ops.residual_norm(x, res, post, gate, "tanh", 0.7, pre)
+        for b in range(B):
+            for t in (slice(0, T), slice(2, 3)):
+                one = ops.residual_norm(x[b: b + 1, t], res[b: b + 1, t], post, gate[b: b + 1], "tanh", 0.7, pre)
+                assert torch.equal(one[0], y[b: b + 1, t]) and torch.equal(one[1], h[b: b + 1, t])
