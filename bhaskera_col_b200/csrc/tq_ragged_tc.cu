@@ -197,7 +197,7 @@ __device__ __forceinline__ void stage_rotation(unsigned char* b, const float* ro
 struct Vecs {
   uint8_t* page[kM];                       // NULL: no place
   int slot[kM];                            // token in its page
-  int row[kM];                             // row of the rotation table; several axes: of the batch
+  int row[kM];                             // row of the rotation table; several axes: of the batch, -1: no place
   float n[kM];                             // norm
   float inv[kM];                           // append: factor of the accumulator
   uint8_t state[kM];                       // 0: row of no request, 1: no place, 2: stored
@@ -269,7 +269,9 @@ __device__ __forceinline__ void init_pipe(const Pipe& p, int makers, int epi_war
 
 // Two warps, half a tile each: two vectors per lane.  A vector's place is a
 // chain of dependent loads (offsets, length, block table); found by warps of
-// their own and up to kRing tiles ahead, the chain delays nobody.
+// their own and up to kRing tiles ahead, the chain delays nobody.  AXES: a stored
+// vector's row is that of its positions, which nobody looks up for any other.
+template <bool AXES>
 __device__ __forceinline__ void locate_tiles(const RaggedTc& p, const Pipe& pp, Vecs* ring,
                                              const Requests& rq, int half, int first, int step) {
   constexpr int NV = kM / 64;
@@ -299,9 +301,7 @@ __device__ __forceinline__ void locate_tiles(const RaggedTc& p, const Pipe& pp, 
       if (state[k] && !in) atomicOr(p.status, TQ_DEV_BAD_POSITION);
       entry[k] = in ? page_entry(p.pm, (int64_t)lo * p.H + h, pos[k] / kPageTokens) : -1;
       to[k] = pos[k];
-      if (p.f.axes.n)
-        to[k] = n[k];
-      else if (p.pos && in)
+      if (!AXES && p.pos && in)
         to[k] = p.pos64
                     ? (int64_t)__ldg(reinterpret_cast<const long long*>(p.pos) + n[k] * p.pos_stride)
                     : (int64_t)__ldg(reinterpret_cast<const int*>(p.pos) + n[k] * p.pos_stride);
@@ -317,8 +317,7 @@ __device__ __forceinline__ void locate_tiles(const RaggedTc& p, const Pipe& pp, 
       const bool in = state[k] == 2;
       ring[e].page[at] = in ? p.pages + entry[k] * (int64_t)p.g.page_bytes : nullptr;
       ring[e].slot[at] = (int)(pos[k] & (kPageTokens - 1));
-      ring[e].row[at] = !in || !p.f.cos_sin ? 0
-                        : p.f.axes.n ? (int)to[k] : (int)table_row(p.f, to[k], p.status);
+      ring[e].row[at] = AXES ? (in ? n[k] : -1) : in && p.f.cos_sin ? (int)table_row(p.f, to[k], p.status) : 0;
       ring[e].state[at] = (uint8_t)state[k];
     }
     __syncwarp();
@@ -421,7 +420,7 @@ __device__ __forceinline__ float sum_lanes(float x) {
 }
 
 // The run's codes in 64 bits, a coordinate per lane; xs: D doubles of the warp's.
-template <int D, int BITS>
+template <int D, int BITS, bool AXES>
 __device__ __forceinline__ void exact_run(const RaggedTc& p, int which, const float* bnd,
                                           const Again& e, double* xs) {
   constexpr int nb = (1 << BITS) - 1;
@@ -450,9 +449,9 @@ __device__ __forceinline__ void exact_run(const RaggedTc& p, int which, const fl
       const bool second = f.interleaved ? d & 1 : d >= half;
       const int with = f.interleaved ? d ^ 1 : second ? d - half : d + half;
       const int64_t row =
-          f.axes.n ? table_row(f, load_pos(p.pos, p.pos64, at_row * p.pos_stride +
-                                                               f.axes.axis(a) * f.axes.stride), p.status)
-                   : at_row;
+          AXES ? table_row(f, load_pos(p.pos, p.pos64, at_row * p.pos_stride +
+                                                           f.axes.axis(a) * f.axes.stride), p.status)
+               : at_row;
       const float* cs = f.cos_sin + row * rot;
       x = x * cs[a] + value(with) * (second ? cs[half + a] : -cs[half + a]);
     }
@@ -633,7 +632,13 @@ append_ragged_tc_kernel(const __grid_constant__ RaggedTc p, int which) {
         constexpr int LINES = 32 / W::kVecs;               // 128-byte lines per lane's vector
         const int64_t to = ring[e].row[W::kVecs * warp + lane / LINES];
         for (int a = 0; a < (AXES ? p.f.axes.n : 1); ++a) {
-          const float* at = f.cos_sin + (AXES ? axis_row(to, a) : to) * f.rot;
+          int64_t row = to;
+          if constexpr (AXES) {                            // a row that the table has not is flagged where it turns
+            if (to < 0) break;
+            row = load_pos(p.pos, p.pos64, to * p.pos_stride + a * p.f.axes.stride);
+            if ((uint64_t)row >= (uint64_t)f.positions) continue;
+          }
+          const float* at = f.cos_sin + row * f.rot;
           for (int c = 32 * (lane % LINES); c < f.rot; c += 32 * LINES)
             asm volatile("prefetch.global.L1 [%0];" ::"l"(at + c));
         }
@@ -691,7 +696,7 @@ append_ragged_tc_kernel(const __grid_constant__ RaggedTc p, int which) {
           };
           if constexpr (AXES) {
             auto row_of = [&](int a) { return axis_row(to, a); };
-            if (to != turned) {
+            if (to >= 0 && to != turned) {                 // without a place: as it is, nobody reads it
               turned = to;
               if (pairs) {
                 if (turn_a) load_axes<8>(ac, as, p.f, ga, row_of);
@@ -707,13 +712,13 @@ append_ragged_tc_kernel(const __grid_constant__ RaggedTc p, int which) {
               }
             }
             if (pairs) {
-              if (turn_a)
+              if (turn_a && to >= 0)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) rotate(v[e], v[8 + e], ac[e], as[e]);
             } else {
 #pragma unroll
               for (int g = 0; g < 2; ++g)
-                if (g ? turn_b : turn_a)
+                if ((g ? turn_b : turn_a) && to >= 0)
 #pragma unroll
                   for (int e = 0; e < 4; ++e)
                     rotate(v[8 * g + 2 * e], v[8 * g + 2 * e + 1], ac[4 * g + e], as[4 * g + e]);
@@ -791,7 +796,7 @@ append_ragged_tc_kernel(const __grid_constant__ RaggedTc p, int which) {
     }
     __syncwarp();
   } else if (warp < W::kEpi0) {
-    locate_tiles(p, pp, ring, requests, warp - W::kLocators, first, step);
+    locate_tiles<AXES>(p, pp, ring, requests, warp - W::kLocators, first, step);
   } else {
     // ------------------------------------------------------------ epilogue
     constexpr int NCH = D / W::kSplit / 32;                // runs of 32 columns per thread
@@ -914,7 +919,7 @@ append_ragged_tc_kernel(const __grid_constant__ RaggedTc p, int which) {
   double* xs = reinterpret_cast<double*>(sm + SM::OFF_A) + D * warp;
   for (int w = 0, k = warp; w < W::kEpi; ++w) {
     for (; k < nagain[w]; k += kThreads / 32)
-      exact_run<D, BITS>(p, which, bnd, again[kAgain * w + k], xs);
+      exact_run<D, BITS, AXES>(p, which, bnd, again[kAgain * w + k], xs);
     k -= nagain[w];
   }
   pdl_wait();
@@ -1100,7 +1105,7 @@ read_ragged_tc_kernel(RaggedTc p, int which) {
     }
     __syncwarp();
   } else if (warp < W::kEpi0) {
-    locate_tiles(p, pp, ring, requests, warp - W::kLocators, first, step);
+    locate_tiles<false>(p, pp, ring, requests, warp - W::kLocators, first, step);
   } else {
     // ------------------------------------------------------------ epilogue
     // The kSplit warps of a lane quarter hold 32 rows x 32 columns each; they
@@ -1321,6 +1326,7 @@ int launch_append_ragged_tc(const tq_geom* G, const tq_tables* t, const tq_cache
                            : (many ? append_fn<64, true>(bits) : append_fn<64, false>(bits));
     if (set_smem_attr((const void*)fn, kSmem) != TQ_OK) return TQ_ERR_CUDA;
     const int threads = D == 128 ? AppendRoles<128>::kThreads : AppendRoles<64>::kThreads;
+    if (w == 1 && axes) p.f = HeadXform{}, p.pos = nullptr;    // values are not turned: no positions looked up
     if (const int rc = launch_one(fn, grid, threads, kSmem, st, p, w, w == 1, "tq_append_ragged"))
       return rc;
   }

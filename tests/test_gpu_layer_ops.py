@@ -193,6 +193,36 @@ def test_append_with_axes_bad_positions_and_places():
         assert torch.equal(bad, pages.pool) and ok_status() == _lib.DEV_BAD_POSITION   # 64, 65: no place
 
 
+@pytest.mark.parametrize("D", [128, 64, 96])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_with_axes_looks_at_the_positions_of_stored_tokens_alone(D, interleaved):
+    """Rows of no request, in front of the batch and behind it, and tokens without a place have positions
+    outside the table, and so does everybody on an axis that no pair follows: nothing is flagged for them,
+    whichever kernel runs and however many tiles a CTA takes."""
+    H = 8
+    tables = make_tables(D, 4, 4, False)
+    rope = ops.RopeTable.build(32, 50, interleaved=interleaved, device=DEV,
+                               axes=ops.RopeTable.axis_of_pairs((8, 0, 8)))
+    for lens in ([(3, 60), (2, 2)], [(2500, 2500), (1, 70)]):
+        batch, start, seq = make_batch(lens, lead=5)
+        n = start[-1] + 4
+        pages = make_paged(tables, 2 * H, max(seq))
+        k = randn((n, H, D), 1)
+        good = torch.randint(0, 50, (3, n), generator=torch.Generator().manual_seed(n)).to(DEV)
+        good[1] = 0
+        ops.append_ragged(tables, pages, k, k, batch, rope=rope, positions=good)
+        assert ok_status() == 0
+        want = pages.pool.clone()
+        pos = good.clone()
+        pos[:, :start[0]], pos[:, start[-1]:], pos[1] = -1, 1 << 40, 77
+        pages.pool.zero_()
+        ops.append_ragged(tables, pages, k, k, batch, rope=rope, positions=pos)
+        assert ok_status() == 0 and torch.equal(pages.pool, want)
+        pos[2, start[0] + 1] = 50                          # a stored token's own
+        ops.append_ragged(tables, pages, k, k, batch, rope=rope, positions=pos)
+        assert ok_status() == _lib.DEV_BAD_POSITION
+
+
 # ------------------------------------------------------------------------------- residual_norm
 def check_norm(got, want, err, dtype):
     tol = S.half_ulp(dtype) * np.abs(want) + err * (1 + S.half_ulp(dtype))
