@@ -558,7 +558,9 @@ struct DiffJoin {
   void* out; int o_dtype; int64_t os[3];   // head, row, dim
 };
 
-// A warp per row and pair: out = out_scale norm(o1 - lambda o2), W = 32 E values.
+// A warp per row and pair: out = out_scale norm(o1 - lambda o2), W = 32 E values.  With own
+// keys a head group saw one half of the values: a norm that is not finite in that half made NaN
+// there alone, and the row that sees it is NaN whole, as in the kernel of both maps.
 template <int E>
 __global__ void __launch_bounds__(256) diff_join_kernel(DiffJoin p) {
   const int lane = threadIdx.x & 31;
@@ -570,10 +572,17 @@ __global__ void __launch_bounds__(256) diff_join_kernel(DiffJoin p) {
     const float* o = p.o + (row * p.H + h) * (2 * 32 * E);
     const float lambda = __ldg(p.lambda + row * p.ls[0] + h * p.ls[1]);
     float x[E], ss = 0.f;
+    bool nan = false;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const float a = o[32 * e + lane], b = o[32 * (E + e) + lane];
       x[e] = b == 0.f ? a : fmaf(-lambda, b, a);           // rows without keys are 0
+      nan = nan || a != a || b != b;
+    }
+    nan = __any_sync(0xffffffffu, nan);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (nan) x[e] = NAN;
       ss = fmaf(x[e], x[e], ss);
     }
     if (p.w) {

@@ -211,6 +211,37 @@ def test_diff_attend_infinite_and_nan_norms(keys, engine):
     assert ok_status() == 0
 
 
+@pytest.mark.parametrize("kb,vb,engine", [(4, 4, 0), (4, 4, 1), (4, 4, 3), (6, 6, 0), (8, 8, 0), (6, 4, 1)])
+@pytest.mark.parametrize("keys,pairs", [("own", "adjacent"), ("own", "halves"), ("shared", "adjacent")])
+def test_diff_attend_rows_that_see_a_norm_that_is_not_finite_are_nan_whole(keys, pairs, kb, vb, engine):
+    """Without a norm behind the difference, which would carry NaN over the row: every column of the rows
+    that see the token, and nothing else, on every kernel."""
+    lens = [(150, 150), (3, 200)]
+    tables, batch, start, seq, pages, pair = setup_case(lens, kb=kb, vb=vb, keys=keys, pairs=pairs, norm=False)
+    if keys == "shared" and engine == 3 and kb > 4:
+        pytest.skip("no such kernel")
+    n, H, D, Hkv = start[-1], 4, 128, 4
+    off = pages.pool.shape[1] - 256
+    for dtype in (BF16, F32):
+        q = randn((n, 2 * H, D), 6, dtype)
+        want = ops.diff_attend_ragged(tables, pages, q, batch, pair, engine=engine)
+        for head in (0, 1, 3):
+            for at in (0, 128):                            # key norms, value norms
+                for bad in (float("inf"), float("-inf"), float("nan")):
+                    page = int(pages.block_table[head, 70 // 64])
+                    place = pages.pool[page, off + at: off + at + 128].view(F16)
+                    keep = place[70 % 64].clone()
+                    place[70 % 64] = bad
+                    got = ops.diff_attend_ragged(tables, pages, q, batch, pair, engine=engine)
+                    hit = [h for h in range(H) if (h == head if keys == "shared" else
+                                                   h // 2 == (head // 2 if pairs == "adjacent" else head % 2))]
+                    seen = torch.zeros((n, H), dtype=torch.bool, device=DEV)
+                    seen[70:150, hit] = True
+                    assert got[seen].isnan().all() and torch.equal(got[~seen], want[~seen]), (head, at, bad)
+                    place[70 % 64] = keep
+    assert ok_status() == 0
+
+
 @pytest.mark.parametrize("engine,dtype", [(0, BF16), (1, BF16), (2, BF16), (3, BF16), (0, F32)])
 @pytest.mark.parametrize("keys", ["own", "shared"])
 def test_diff_attend_small_value_norms_and_long_requests(keys, engine, dtype):
