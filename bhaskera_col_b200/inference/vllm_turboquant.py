@@ -203,7 +203,8 @@ class TurboQuantPagedAttention:
         With ``rope`` (and / or the head norms) query and key come as they
         leave their projections: they are normed and rotated here, by each
         token's position in its request or by ``positions`` (N,) ((axes, N) for
-        a rope with axes), and the whole batch runs as three calls.
+        a rope with axes), and the whole batch runs as three calls.  A layer
+        with norms and no rope may be given positions: it turns nothing.
 
         With ``pair`` the query heads are attended in pairs, as the difference
         of two softmax maps (ops.diff_attend_ragged), and the output is (N, Hq /
@@ -216,7 +217,7 @@ class TurboQuantPagedAttention:
             out = torch.empty_like(query)
         st = stream_table if stream_table is not None else self.stream_table(batch.block_table)
         if rope is not None or q_norm is not None or k_norm is not None or pair is not None:
-            if rope is None and positions is not None:
+            if rope is None and q_norm is None and k_norm is None and positions is not None:
                 raise ValueError("positions come with rope")
             return self._forward_ragged(query, key, value, batch, out, st, rope, q_norm, k_norm,
                                         positions, pair)
@@ -267,12 +268,12 @@ class TurboQuantPagedAttention:
         if batch.max_query_len <= 1:
             self.decode_tokens += n
         q = query[:n]
+        given = positions[..., :n] if rope is not None and positions is not None else None
         if rope is not None or q_norm is not None:
-            at = positions[..., :n] if positions is not None else \
-                (batch.positions() if rope is not None else None)
+            at = batch.positions() if rope is not None and given is None else given
             q, _ = ops.qk_rope(q, None, rope, at, q_norm=q_norm)
         ops.append_ragged(self.tables, pages, key[:n], value[:n], rb, rope=rope, k_norm=k_norm,
-                          positions=positions[..., :n] if positions is not None else None)
+                          positions=given)
         if pair is not None:
             if pair.lam.dim() == 2 and pair.lam.shape[0] != n:
                 pair = replace(pair, lam=pair.lam[:n])

@@ -396,3 +396,26 @@ def test_residual_norm_of_one_sequence_is_that_of_a_batch():
             for t in (slice(0, T), slice(2, 3)):
                 one = ops.residual_norm(x[b: b + 1, t], res[b: b + 1, t], post, gate[b: b + 1], "tanh", 0.7, pre)
                 assert torch.equal(one[0], y[b: b + 1, t]) and torch.equal(one[1], h[b: b + 1, t])
+
+
+def test_paged_attention_with_norms_and_no_rotation_takes_positions():
+    """A model whose layers partly have no rotation passes positions always: a layer with head norms alone
+    does not look at them."""
+    from bhaskera_col_b200.inference.vllm_turboquant import TurboQuantPagedAttention, VLLMBatch
+    D, Hq, H, n = 128, 4, 2, 135
+    norms = [ops.HeadNorm(1 + 0.1 * randn((D,), i, F32)) for i in range(2)]
+    bt = torch.arange(8, dtype=torch.int32, device=DEV).view(2, 4)
+    batch = VLLMBatch(torch.tensor([0, 130, n], dtype=torch.int32, device=DEV),
+                      torch.tensor([130, 5], dtype=torch.int32, device=DEV), bt, n, 130)
+    q, k, v = (randn((n + 2, h, D), 10 + h) for h in (Hq, H, H + 2))
+    v = v[:, :H]
+    outs = []
+    for pos in (None, torch.arange(n + 2, device=DEV), torch.full((3, n + 2), -1, device=DEV)):
+        for kw in (dict(q_norm=norms[0], k_norm=norms[1]), dict(q_norm=norms[0]), dict(k_norm=norms[1])):
+            layer = TurboQuantPagedAttention(3, 32, Hq, H, D, num_blocks=8, block_size=64, device=DEV)
+            layer.pool.zero_()
+            outs.append((layer.forward(q, k, v, batch, positions=pos, **kw)[:n],
+                         layer.paged(layer.stream_table(bt)).pool))
+    for i in range(3, 9):
+        assert all(torch.equal(a, b) for a, b in zip(outs[i], outs[i % 3]))
+    assert ok_status() == 0
