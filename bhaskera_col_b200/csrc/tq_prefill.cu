@@ -160,13 +160,11 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
   using Pos = typename std::conditional<RG, int, int64_t>::type;
   const int chunk = (int)(group % nchunk);
   const int64_t b = group / nchunk / p.Hkv, kvh = group / nchunk % p.Hkv;
-  // streams of the keys and of the values (RG: they may differ)
+  // stream of the keys (RG: the values' may differ, see fetch)
   const int64_t stream = RG ? b * p.rg.hv.streams + p.rg.hv.key_head((int)kvh) : group / nchunk;
-  const int64_t vstream = RG ? b * p.rg.hv.streams + p.rg.hv.value_head((int)kvh) : stream;
   // the batch row's first query row: batch stride, or the request's first row
   const int64_t qrow = RG ? sw.rq.q0 * p.qs[2] : b * p.qs[0];
   const int64_t orow = RG ? sw.rq.q0 * p.os[2] : b * p.os[0];
-  const int64_t ocol = RG ? p.rg.hv.column((int)kvh, D) * p.os[3] : 0;
   // head i of the CTA's, counted over all
   auto head = [&](int i) -> int64_t {
     return RG ? p.rg.hv.head((int)kvh, chunk * p.hc + i) : kvh * p.g + (int64_t)chunk * p.hc + i;
@@ -227,7 +225,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
   auto fetch = [&](int i, int64_t pg) {
     unsigned char* dst = smem + G::OFF_STG + i * p.page_pitch;
     const uint8_t* src = page_src(stream, pg);
-    if (!RG || vstream == stream) {
+    const int64_t vstream = RG && p.rg.hv.own ? b * p.rg.hv.streams + p.rg.hv.value_head((int)kvh) : stream;
+    if (vstream == stream) {
       mbar_expect_tx(&full[i], PAGE);
       bulk_g2s(dst, src, PAGE, &full[i]);
       return;
@@ -566,6 +565,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
       for (int n = 0; n < NT; ++n) { acc[n][0] *= down; acc[n][1] *= down; acc[n][2] *= down; acc[n][3] *= down; }
     }
     const int r0 = t0 + gq, r1 = r0 + 8;
+    const int64_t ocol = RG ? p.rg.hv.column((int)kvh, D) * p.os[3] : 0;
     const int64_t obase = orow + h * p.os[1] + ocol;
     const bool split = RG && sw.seg.slot >= 0;
     if (split) {
@@ -604,7 +604,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) prefill_kernel(PrefillParams p)
                        [&](int row) -> int64_t {
                          const int wr = row >> 4, t = qb * P + (wr % wph) * 16 + (row & 15);
                          if (t >= p.Tq) return -1;
-                         return orow + head(wr / wph) * p.os[1] + ocol + t * p.os[2];
+                         return orow + head(wr / wph) * p.os[1] + p.rg.hv.column((int)kvh, D) * p.os[3] +
+                                t * p.os[2];
                        });
   }
 }
