@@ -112,6 +112,40 @@ def test_diff_attend_matches_plain_form(D, kb, vb, H, Hkv, keys, pairs, case):
     assert ws.status() == 0
 
 
+@pytest.mark.parametrize("case", ["tokens", "chunks", "cross", "split"])
+@pytest.mark.parametrize("D,kb,vb,H,Hkv,keys,pairs", GEOM)
+def test_diff_attend_bf16_results_row_by_row(D, kb, vb, H, Hkv, keys, pairs, case):
+    """bf16 results where the maps do not cancel (no norm, lam below 0.3), every row and pair by itself: the
+    root of the mean square of the error beside that of the row.  The result's rounding is 2^-8 at worst and
+    0.43 x 2^-8 over mantissas alike likely (their step over sqrt(12), root of the mean of 1 / m^2 0.735).
+    Operands: a score's 2^-12 roundings of q', key and norm are independent over the dims, at most
+    sqrt(3 / D) `most` 2^-11 of them, seldom more than 2^-10; P and V 2^-11 each: together below 2^-9.
+    So 2^-8 + 2^-9 for the worst row and sqrt(0.43^2 + 0.5^2) 2^-8 = 2.6e-3 over all."""
+    lens, causal = DIFF[case]
+    tables = make_tables(D, kb, vb, False)
+    R = len(lens)
+    batch, start, seq = make_batch(lens)
+    n = start[-1]
+    pages = make_paged(tables, R * Hkv, max(max(seq), 1))
+    fill(tables, pages, R, Hkv, pages.shape[1] * 64, 3)
+    q = randn((n, 2 * H, D), 4, BF16)
+    lam = (0.3 * torch.rand((H,), generator=torch.Generator().manual_seed(5))).to(DEV)
+    pair = ops.DiffHeads(lam, keys, pairs)
+    want = want_diff(tables, pages, q, pair, start, seq, causal, Hkv)[0]
+    for engine in (0, 1, 2, 3):
+        try:
+            out = L.arr(ops.diff_attend_ragged(tables, pages, q, batch, pair, causal=causal, engine=engine))
+        except _lib.TqError as e:
+            assert engine > 1 and "no kernel" in str(e)
+            continue
+        keys_seen = ~(want == 0).all(-1)
+        err, size = ((x * x).mean(-1)[keys_seen] ** 0.5 for x in (out - want, want))
+        assert (err <= (2.0 ** -8 + 2.0 ** -9) * size).all(), (engine, (err / size).max())
+        assert (((err / size) ** 2).mean() ** 0.5) <= 2.6e-3, engine
+        assert (out[~keys_seen] == 0).all()
+    assert ok_status() == 0
+
+
 def skip_without_kernel(keys, engine):
     """Own keys have no kernel of 256 rows (engine 2)."""
     if keys == "own" and engine in NO_OWN:
@@ -398,6 +432,25 @@ def test_layer_runs_together():
     ye, de, he, dhe = L.residual_norm(o.flatten(1) @ back, mid, post,
                                       torch.full((C,), 0.3, dtype=BF16), "sigmoid", 1.0, pre)
     assert (np.abs(L.arr(h2) - he) <= dhe * (1 + 2.0 ** -8) + S.half_ulp(BF16) * np.abs(he)).all()
+
+
+def test_sum_and_norm_behind_differential_attention():
+    """Both results of residual_norm on what differential attention and its projection leave, fp16 and bf16
+    blocks on an fp32 stream: the sum that the next layer starts from, and its norm."""
+    tables, batch, start, seq, pages, pair = setup_case([(70, 170), (1, 200), (5, 5)])
+    n, H, D, C = start[-1], 4, 128, 512
+    post, pre = ops.RowNorm(1 + 0.1 * randn((C,), 5, F32)), ops.RowNorm(1 + 0.1 * randn((C,), 6, F32), centered=True)
+    stream = randn((n, C), 13, F32)
+    for dtype in (BF16, F16):
+        back = randn((H * 2 * D, C), 12, dtype) / (2 * H * D) ** 0.5
+        o = ops.diff_attend_ragged(tables, pages, randn((n, 2 * H, D), 3, dtype), batch, pair).flatten(1) @ back
+        for gate in (torch.full((C,), 0.3, device=DEV, dtype=dtype), randn((n, C), 4, F32), None):
+            act = "none" if gate is None else "sigmoid"
+            end, h = ops.residual_norm(o, stream, post, gate, act, 1.0, pre)
+            ye, de, he, dh = L.residual_norm(o, stream, post, gate, act, 1.0, pre)
+            assert (np.abs(L.arr(end) - ye) <= de + S.half_ulp(F32) * np.abs(ye)).all()
+            assert (np.abs(L.arr(h) - he) <= dh * (1 + 2.0 ** -8) + S.half_ulp(dtype) * np.abs(he) + 2.0 ** -25).all()
+    assert ok_status() == 0
 
 
 @pytest.mark.parametrize("keys", ["own", "shared"])

@@ -419,3 +419,47 @@ def test_paged_attention_with_norms_and_no_rotation_takes_positions():
     for i in range(3, 9):
         assert all(torch.equal(a, b) for a, b in zip(outs[i], outs[i % 3]))
     assert ok_status() == 0
+
+
+def gates_over_the_range(dtype, n=4096):
+    """Gates over the type's whole range, both signs, beside the places where the function's parts end."""
+    top = float(torch.finfo(dtype).max)
+    x = torch.cat([torch.linspace(-20, 20, n // 2, dtype=torch.float64),
+                   torch.logspace(-30, np.log10(top) - 1e-6, n // 4, dtype=torch.float64)])
+    x = torch.cat([x, -x[n // 2:]]).clamp(-top, top)
+    edges = [0.0, -0.0, top, -top, float("inf"), -float("inf"), 1e-8, -1e-8]
+    edges += [s * (c + d) for c in (87.0, 87.33655, 87.5, 88.72284, 89.0, 126.0, 127.0) for d in (-1e-5, 0.0, 1e-5)
+              for s in (-1.0, 1.0) if c < top]
+    x[: len(edges)] = torch.tensor(edges, dtype=torch.float64).clamp(-top, top) * 1.0
+    x[4], x[5] = float("inf"), -float("inf")
+    return x.to(dtype).to(DEV)
+
+
+@pytest.mark.parametrize("act", ["sigmoid", "tanh"])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("kind", ["channel", "element", "row"])
+def test_gate_functions_over_their_range(kind, dtype, act):
+    """y = act(gate) alone (x = 1, residual 0, fp32).  sigmoid = 1 / (1 + e^-g): e^-g is off, relatively,
+    by the exponential's 2^-22 and three roundings of 2^-24 at most, the sum by one more, the quotient by
+    2 ulp (2^-22): 2^-21 + 2^-22 in all; below 2^-126 results may be flushed.  tanh: 2 ulp (2^-22) and a
+    rounding.  Infinite gates give the limits, NaN gives NaN in its own place."""
+    g = gates_over_the_range(dtype)
+    C = g.numel()
+    want = g.double()
+    want = torch.tanh(want) if act == "tanh" else torch.where(want >= 0, 1 / (1 + (-want).exp()),
+                                                               want.exp() / (1 + want.exp()))
+    one, zero = torch.ones((3, C), device=DEV), torch.zeros((3, C), device=DEV)
+    gate = {"channel": g, "element": torch.stack([g.roll(i) for i in range(3)]), "row": g[:, None]}[kind]
+    if kind == "row":
+        one, zero, want = torch.ones((C, 8), device=DEV), torch.zeros((C, 8), device=DEV), want[:, None].expand(C, 8)
+    elif kind == "element":
+        want = torch.stack([want.roll(i) for i in range(3)])
+    y, _ = ops.residual_norm(one, zero, gate=gate, gate_act=act)
+    err = (y.double() - want).abs()
+    assert (err <= (2.0 ** -21 + 2.0 ** -22) * want.abs() + 2.0 ** -126).all(), (err / want.abs()).nan_to_num().max()
+    assert (y.abs() <= 1).all()
+    bad = gate.clone()
+    bad.view(-1)[7] = float("nan")
+    y2, _ = ops.residual_norm(one, zero, gate=bad, gate_act=act)
+    hit = bad.isnan().expand(y2.shape)
+    assert hit.any() and y2[hit].isnan().all() and torch.equal(y2[~hit], y[~hit])
