@@ -6,10 +6,11 @@
 //
 // Bound by HBM: x, residual and a gate of its own per element are read once, y and h
 // written once; in fact by instructions beside it (issue slots 72 % busy).  16,381 rows
-// of 4,096 (bf16, channel gate) 117 us for 537 MB, 4.6 TB/s; 16 rows of 5,120 3.8 us on
-// the GPU; 2,051 rows of 2,050 (4-byte chunks, gate per element, layer norms) 33 us.  Sums go by
-// shuffles and one barrier each, always in the same order; h is formed from y before its
-// rounding.
+// of 4,096 (bf16, channel gate) 110 us for 537 MB, 4.9 TB/s; 16 rows of 5,120 4.6 us on
+// the GPU; 2,051 rows of 2,050 (4-byte chunks, gate per element, layer norms) 35 us.  Sums go by
+// shuffles and one barrier each, in an order that the width and the accesses that the views
+// allow settle, so that a row called by itself is the row of a batch to the bit; h is formed
+// from y before its rounding.
 #include "tq_common.cuh"
 #include "tq_internal.h"
 #include "tq_tc.cuh"
@@ -140,8 +141,9 @@ __device__ __forceinline__ void load_param(float (&v)[V], const void* base, int 
 }
 
 // 1 / (1 + e^-g): e^-g = 2^t (1 + d ln 2) with t + d = -g log2 e in two parts, as t alone is
-// off by |g| 2^-24 (2^-22 in all; the library's exponential and quotient took half of the
-// instructions of a gated row).
+// off by |g| 2^-24 (the library's exponential and quotient took half of the instructions of a
+// gated row).  Off by 2^-21 + 2^-22 at most: the exponential's 2^-22, four roundings, the
+// quotient's 2 ulp (the worst of 4 million gates from -87 to 87: 5.0 x 2^-24); below 2^-126 it is 0.
 __device__ __forceinline__ float activate(float g, int act) {
   if (act == TQ_GATE_SIGMOID) {
     const float x = fminf(fmaxf(-g, -126.f), 126.f);       // (a NaN gate is let through below)
@@ -181,7 +183,7 @@ using tc::f2;
 //   y = residual + (x r) A + B,   h = (y r') C + D
 // (A = (w + offset) F, B = b F, F = scale act(gate); with a gate per element the products
 // with F are made where it is used, to the same bits: a row alone, whose gate is either, is the
-// row of a batch) and the next rows' values on their way: two with chunks of 8 (16,381 rows of 4,096: one
+// row of a batch), and the next rows' values on their way: two with chunks of 8 (16,381 rows of 4,096: one
 // 144 us, two 117), one with chunks of 2, whose registers leave less room (2,051 rows of
 // 2,050: 33 us, 41).  GE: a gate per element, BIAS: B and D.  The
 // arithmetic, on fp32 pairs, is 6 instructions a value without a gate per element.
@@ -374,8 +376,12 @@ __global__ void __launch_bounds__(MAXT) residual_norm_rows_kernel(NormParams p, 
 
 using NormFn = void (*)(NormParams, int);
 
-// Up to 384 threads have registers for gates and biases without spills above,
-// 64 each.
+// Up to 384 threads no instance spills, at 64 to 118 registers.  Above,
+// two CTAs of 512 threads an SM leave 64: rows of 16 bits without biases and gates per element fit,
+// layer norms spill 80 bytes a thread, with a gate of their own 164, with an fp32 residual 28
+// to 272, fp32 throughout 68 to 348.  8,192 rows of 4,096: bf16 layer norms 98 us for 268 MB
+// (2.7 TB/s), an fp32 residual 84 for 403 MB (4.8), a gate per element 87 for 336 MB (3.8), that
+// with layer norms 139.
 template <int XT, int RT, int V>
 NormFn rows_fn(bool ge, bool bias, bool wide) {
 #define TQ_ROWS(GE, BIAS) \
@@ -395,8 +401,11 @@ NormFn rows_fn_x(int rd, int v, bool ge, bool bias, bool wide) {
   return nullptr;
 }
 
-// Everything else: T threads per row (a warp, or the CTA), 8 VPT values each in chunks of V
-// neighbours.  V = 1 takes any stride.  Sums and products go in the order of the kernel above,
+// Everything else: rows above 8,192 values (more than 1,024 threads' 8), views whose rows start on
+// odd elements, and fp32 gates per element, eight registers a row on its way more than the
+// instances above have.  T threads per row (a warp, or the CTA), 8 VPT values each in chunks of V
+// neighbours; V = 1 takes any stride.  8,192 fp32 rows of 4,096 with fp32 gates 152 us for 671
+// MB (4.4 TB/s), 2,048 bf16 rows of 16,384 with gates 142 (2.4), 2,048 of 4,097 111.  Sums and products go in the order of the kernel above,
 // even and odd values by themselves, and no product joins a sum but by fmaf: a gate of 32 bits
 // per element (whose rows on their way the registers above have no room for) gives the bits
 // that a gate of the channels gives there.

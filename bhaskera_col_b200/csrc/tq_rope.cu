@@ -14,8 +14,8 @@
 // a warp per vector.
 // 16,381 tokens x 48 heads of 128, bf16, normed: 89.5 us for 411 MB, 4.6 TB/s (a
 // plain copy of the bytes takes 64); 16 tokens 4.1 us, the launch.  The 16-bit
-// instances spill 40-48 bytes a thread at the 80 registers of three CTAs an SM; two
-// CTAs of 126 registers without a spill took 97 us.
+// instances spill 40-48 bytes a thread (with several position axes 80) at the 80 registers
+// of three CTAs an SM; two CTAs of 126 registers without a spill took 97 us.
 #include "tq_internal.h"
 #include "tq_ragged.cuh"
 #include "tq_tc.cuh"

@@ -959,9 +959,11 @@ def diff_attend_ragged(tables: LayerTables, pages, q: torch.Tensor, batch: Ragge
     shared ones.
 
     Rows, masks, lengths, empty rows, ``scale``, ``causal``, ``engine`` (own keys
-    have no tcgen05 kernel: not 2) and ``workspace`` are those of attend_ragged; so are the errors of both maps'
-    results, of which the difference is taken in fp32: where the maps nearly
-    cancel, an fp32 ``out`` (operands of 22 bits) keeps what is left."""
+    have no tcgen05 kernel: not 2) and ``workspace`` are those of attend_ragged.
+    Shared keys, and own keys with codes above 4 bits, leave both maps' results in
+    the workspace, 8 bytes an element of the result.  The errors of both maps are
+    those of attend_ragged too, and the difference is taken in fp32: where the maps
+    nearly cancel, an fp32 ``out`` (operands of 22 bits) keeps what is left."""
     norm = pair.norm
     _inference_only("diff_attend_ragged", q.device, q, out, batch.q_start, pair.lam,
                     norm.weight if norm is not None else None)
@@ -1024,7 +1026,8 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, post_norm: Optional[R
     (N, 1) a token's, (N, C)) and goes through ``gate_act``: "none", "sigmoid" or
     "tanh".  x has one to four dims and any strides, C at most 32,768.
     ``residual_out`` / ``out``: where the results go (may be residual / x
-    itself).  Returns (residual_out, out); out is None without ``pre_norm``."""
+    itself).  A row sliced out of a batch gives the bits that the batch gives.
+    Returns (residual_out, out); out is None without ``pre_norm``."""
     if x.dim() < 1 or x.dim() > 4 or residual.shape != x.shape:
         raise ValueError(f"x and residual must have one shape of 1 to 4 dims, got "
                          f"{tuple(x.shape)} and {tuple(residual.shape)}")
